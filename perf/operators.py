@@ -75,7 +75,7 @@ def draw(rng):
         case.update(channels=channels, activation=rng.choice(["none", "relu", "silu", "gelu"]), affine=rng.random() < 0.85)
         rows = min(_log(rng, 64, 2_000_000), 120_000_000 / getattr(torch, case["type"]).itemsize / channels)
         case["batch"] = max(1, round(_log(rng, 1, rows))) if rng.random() < 0.5 else rng.randint(1, 4)
-        case["length"] = max(1, round(rows / case["batch"]))
+        case["length"] = max(1, int(rows // case["batch"]))
         return case
     shared = rng.choice([1, 1, 3, 4, 16, 64, 128])
     if kind == "step":
