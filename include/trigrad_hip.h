@@ -495,6 +495,106 @@ int tg_clip_emit(const tg_real *clip, int32_t n_vertices, const int32_t *indices
 /* (x, y, z, w) -> (x/w, y/w, z/w, 1/w) (viewer.py:276-278). */
 int tg_clip_to_render(const tg_real *clip, int64_t n_vertices, tg_real *out, void *stream);
 
+/* ---- gated linear recurrence, group norm ----------------------------------------- */
+
+/* Element types.  The float library takes the first three, the double library the last. */
+#define TG_TYPE_F32 0
+#define TG_TYPE_F16 1
+#define TG_TYPE_BF16 2
+#define TG_TYPE_F64 3
+
+/* h_t = a_t h_{t-1} + u_t for every sequence and channel, the recurrence that compositing front to back or back to front is.
+ *   a = f(gate): TG_GATE_VALUE the gate itself, TG_GATE_LOG exp(gate), TG_GATE_LOGIT 1 / (1 + exp(-gate));
+ *   u = x (TG_INPUT_PLAIN) or (1 - a) x (TG_INPUT_COMPLEMENT).
+ * Without offsets inputs is (sequences, length, channels); with them (length, channels), sequence s being the rows
+ * offsets[s] to offsets[s + 1], which do not decrease, the first of them >= 0, the last <= length: rows of no sequence get
+ * zeros, in the states and in the gradients.  gates has `gates` columns where inputs has `channels`: gate g is that of the channels
+ * g * channels / gates up to the next gate's.  reverse: each sequence from its last row to its first.  Products of successive gates
+ * of a sequence are formed, of up to 4096 of them: they have to be representable, which those of decays (|a| <= 1) are.
+ * initial, final and their gradients are (sequences, channels) tg_real; initial, grad_states, grad_final, and every output
+ * but `final` may be null.  The final state of an empty sequence is its initial one.
+ * tg_linear_recurrence_sizes writes the bytes of `kept` (what the forward call leaves for the backward call; null where none
+ * follows) and of the forward and the backward call's workspaces. */
+#define TG_GATE_VALUE 0
+#define TG_GATE_LOG 1
+#define TG_GATE_LOGIT 2
+#define TG_INPUT_PLAIN 0
+#define TG_INPUT_COMPLEMENT 1
+
+typedef struct tg_recurrence {
+    const void *inputs;       /* type */
+    const void *gates;        /* gate_type: that of inputs, or tg_real */
+    const tg_real *initial;
+    const int32_t *offsets;   /* (sequences + 1) or null */
+    void *states;             /* type, as inputs */
+    tg_real *final;
+    void *kept;
+    void *workspace;
+    void *stream;
+    const void *grad_states;  /* type */
+    const tg_real *grad_final;
+    void *grad_inputs;        /* type */
+    void *grad_gates;         /* gate_type */
+    tg_real *grad_initial;
+    int64_t sequences;
+    int64_t length;
+    int64_t channels;
+    int64_t gate_count;
+    int64_t type;
+    int64_t gate_type;
+    int64_t gate_form;
+    int64_t input_form;
+    int64_t reverse;
+    int64_t kept_bytes;
+    int64_t workspace_bytes;
+} tg_recurrence;
+
+int tg_linear_recurrence_sizes(const tg_recurrence *r, int64_t out[3]);
+int tg_linear_recurrence_forward(const tg_recurrence *r);
+int tg_linear_recurrence_backward(const tg_recurrence *r);
+/* One step: inputs (sequences, channels), state and new_state (sequences, channels) tg_real, which may be the same; states, as
+ * inputs, is the new state in the inputs' type. */
+int tg_linear_recurrence_step(const void *inputs, const void *gates, const tg_real *state, void *states, tg_real *new_state,
+                              int64_t sequences, int64_t channels, int64_t gate_count, int type, int gate_type, int gate_form,
+                              int input_form, void *stream);
+
+/* Group norm of x (samples, positions, channels), channels last as in an image, and an activation behind it:
+ * y = act((x - mean) rstd weight + bias), mean and rstd = 1 / sqrt(variance + eps) of a sample's positions x (channels / groups).
+ * weight and bias ((channels), weight_type: x's or tg_real) may be null, both or either.  statistics: (samples, groups, 2) tg_real,
+ * mean and rstd, which the backward call reads; grad_weight and grad_bias may be null, grad_x too. */
+#define TG_ACTIVATION_NONE 0
+#define TG_ACTIVATION_RELU 1
+#define TG_ACTIVATION_SILU 2
+#define TG_ACTIVATION_GELU 3 /* z Phi(z), by the error function */
+
+typedef struct tg_norm {
+    const void *x;
+    const void *weight;
+    const void *bias;
+    void *y;
+    tg_real *statistics;
+    void *workspace;
+    void *stream;
+    const void *grad_y;
+    void *grad_x;
+    void *grad_weight;
+    void *grad_bias;
+    int64_t samples;
+    int64_t positions;
+    int64_t channels;
+    int64_t groups;
+    int64_t type;
+    int64_t weight_type;
+    int64_t activation;
+    int64_t workspace_bytes;
+    double eps;
+} tg_norm;
+
+/* out: bytes of the forward and of the backward call's workspace. */
+int tg_group_norm_sizes(const tg_norm *n, int64_t out[2]);
+int tg_group_norm_forward(const tg_norm *n);
+int tg_group_norm_backward(const tg_norm *n);
+
 /* ---- host-side component hooks ---------------------------------------------- */
 
 /* HOST pointers, run on the CPU.  The reference exports the same six functions

@@ -1251,3 +1251,113 @@ def set_precision(dtype):
         raise TypeError(f"precision must be torch.float32 or torch.float64, got {dtype}")
     _lib.load(64 if dtype == torch.float64 else 32)
     precision = dtype
+
+
+# ---- gated linear recurrence, group norm ------------------------------------------------
+
+TYPE_CODES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2, torch.float64: 3}  # TG_TYPE_*
+
+
+def real_type(dtype):
+    """What tensors of `dtype` are summed in: tg_real of the library that serves them."""
+    return torch.float64 if dtype == torch.float64 else torch.float32
+
+
+def _address(t):
+    return 0 if t is None else t.data_ptr()
+
+
+def _bytes(n, dev):
+    return torch.empty((n,), dtype=torch.uint8, device=dev) if n else None
+
+
+def _recurrence(inputs, gates, offsets, sequences, length, gate_form, input_form, reverse):
+    r = _lib.Recurrence(inputs=_address(inputs), gates=_address(gates), offsets=_address(offsets), stream=_raw_stream(inputs.device),
+                        sequences=sequences, length=length, channels=inputs.shape[-1], gate_count=gates.shape[-1],
+                        type=TYPE_CODES[inputs.dtype], gate_type=TYPE_CODES[gates.dtype], gate_form=gate_form, input_form=input_form,
+                        reverse=reverse)
+    lib, sizes = _lib.load(_bits(inputs)), (C.c_int64 * 3)()
+    _lib.check(lib.tg_linear_recurrence_sizes(C.byref(r), sizes), "tg_linear_recurrence_sizes", _bits(inputs))
+    return lib, r, sizes
+
+
+def linear_recurrence_forward(inputs, gates, initial, offsets, sequences, length, gate_form, input_form, reverse, return_states, for_backward):
+    """-> (states or None, final, kept or None); contiguous arguments, checked by trigrad_amd.linear_recurrence."""
+    dev = inputs.device
+    with _on_device(dev):
+        lib, r, sizes = _recurrence(inputs, gates, offsets, sequences, length, gate_form, input_form, reverse)
+        states = torch.empty_like(inputs) if return_states else None
+        final = torch.empty((sequences, inputs.shape[-1]), dtype=real_type(inputs.dtype), device=dev)
+        kept = torch.empty((sizes[0],), dtype=torch.uint8, device=dev) if for_backward else None
+        workspace = _bytes(sizes[1], dev)
+        r.initial, r.states, r.final, r.kept, r.kept_bytes = _address(initial), _address(states), _address(final), _address(kept), sizes[0]
+        r.workspace, r.workspace_bytes = _address(workspace), sizes[1]
+        _lib.check(lib.tg_linear_recurrence_forward(C.byref(r)), "tg_linear_recurrence_forward", _bits(inputs))
+    return states, final, kept
+
+
+def linear_recurrence_backward(inputs, gates, offsets, kept, grad_states, grad_final, sequences, length, gate_form, input_form, reverse,
+                               need_inputs, need_gates, need_initial):
+    """-> gradients of inputs, gates and the initial states, None where not needed."""
+    dev = inputs.device
+    with _on_device(dev):
+        lib, r, sizes = _recurrence(inputs, gates, offsets, sequences, length, gate_form, input_form, reverse)
+        grad_states, grad_final = (None if t is None else t.contiguous() for t in (grad_states, grad_final))
+        grad_inputs = torch.empty_like(inputs) if need_inputs else None
+        grad_gates = torch.empty_like(gates) if need_gates else None
+        grad_initial = torch.empty((sequences, inputs.shape[-1]), dtype=real_type(inputs.dtype), device=dev) if need_initial else None
+        workspace = _bytes(sizes[2], dev)
+        r.kept, r.kept_bytes, r.workspace, r.workspace_bytes = _address(kept), sizes[0], _address(workspace), sizes[2]
+        r.grad_states, r.grad_final = _address(grad_states), _address(grad_final)
+        r.grad_inputs, r.grad_gates, r.grad_initial = _address(grad_inputs), _address(grad_gates), _address(grad_initial)
+        _lib.check(lib.tg_linear_recurrence_backward(C.byref(r)), "tg_linear_recurrence_backward", _bits(inputs))
+    return grad_inputs, grad_gates, grad_initial
+
+
+def linear_recurrence_step(inputs, gates, state, new_state, gate_form, input_form):
+    """-> the new state in the inputs' type; new_state receives it in float32."""
+    states = torch.empty_like(inputs)
+    with _on_device(inputs.device):
+        code = _lib.load(_bits(inputs)).tg_linear_recurrence_step(
+            inputs.data_ptr(), gates.data_ptr(), state.data_ptr(), states.data_ptr(), new_state.data_ptr(), inputs.shape[0], inputs.shape[1],
+            gates.shape[1], TYPE_CODES[inputs.dtype], TYPE_CODES[gates.dtype], gate_form, input_form, _raw_stream(inputs.device))
+        _lib.check(code, "tg_linear_recurrence_step", _bits(inputs))
+    return states
+
+
+def _norm(x, groups, weight, bias, statistics, eps, activation):
+    samples, channels = x.shape[0], x.shape[-1]
+    second = weight if weight is not None else bias if bias is not None else x
+    n = _lib.Norm(x=_address(x), weight=_address(weight), bias=_address(bias), statistics=_address(statistics), stream=_raw_stream(x.device),
+                  samples=samples, positions=x.shape[1:-1].numel(), channels=channels, groups=groups, type=TYPE_CODES[x.dtype],
+                  weight_type=TYPE_CODES[second.dtype], activation=activation, eps=eps)
+    lib, sizes = _lib.load(_bits(x)), (C.c_int64 * 2)()
+    _lib.check(lib.tg_group_norm_sizes(C.byref(n), sizes), "tg_group_norm_sizes", _bits(x))
+    return lib, n, sizes
+
+
+def group_norm_forward(x, groups, weight, bias, eps, activation):
+    """-> (y, statistics); contiguous arguments, checked by trigrad_amd.group_norm."""
+    with _on_device(x.device):
+        y = torch.empty_like(x)
+        statistics = torch.empty((x.shape[0], groups, 2), dtype=real_type(x.dtype), device=x.device)
+        lib, n, sizes = _norm(x, groups, weight, bias, statistics, eps, activation)
+        workspace = _bytes(sizes[0], x.device)
+        n.y, n.workspace, n.workspace_bytes = _address(y), _address(workspace), sizes[0]
+        _lib.check(lib.tg_group_norm_forward(C.byref(n)), "tg_group_norm_forward", _bits(x))
+    return y, statistics
+
+
+def group_norm_backward(grad_y, x, groups, weight, bias, statistics, eps, activation, need_x, need_weight, need_bias):
+    """-> gradients of x, weight and bias, None where not needed."""
+    with _on_device(x.device):
+        grad_y = grad_y.contiguous()
+        lib, n, sizes = _norm(x, groups, weight, bias, statistics, eps, activation)
+        grad_x = torch.empty_like(x) if need_x else None
+        grad_weight = torch.empty_like(weight) if need_weight else None
+        grad_bias = torch.empty_like(bias) if need_bias else None
+        workspace = _bytes(sizes[1], x.device)
+        n.grad_y, n.workspace, n.workspace_bytes = _address(grad_y), _address(workspace), sizes[1]
+        n.grad_x, n.grad_weight, n.grad_bias = _address(grad_x), _address(grad_weight), _address(grad_bias)
+        _lib.check(lib.tg_group_norm_backward(C.byref(n)), "tg_group_norm_backward", _bits(x))
+    return grad_x, grad_weight, grad_bias

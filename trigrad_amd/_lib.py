@@ -75,6 +75,13 @@ SIGNATURES = {
     "tg_clip_count": (_i, [_p, _i32, _p, _i64, _p, _p, _p]),
     "tg_clip_emit": (_i, [_p, _i32, _p, _i64, _p, _i32, _p, _i32, _p, _i64, _p, _p, _p, _p, _p]),
     "tg_clip_to_render": (_i, [_p, _i64, _p, _p]),
+    "tg_linear_recurrence_sizes": (_i, [_p, _p]),
+    "tg_linear_recurrence_forward": (_i, [_p]),
+    "tg_linear_recurrence_backward": (_i, [_p]),
+    "tg_linear_recurrence_step": (_i, [_p] * 5 + [_i64] * 3 + [_i] * 4 + [_p]),
+    "tg_group_norm_sizes": (_i, [_p, _p]),
+    "tg_group_norm_forward": (_i, [_p]),
+    "tg_group_norm_backward": (_i, [_p]),
     "tg_barycentric": (None, [_p] * 5),
     "tg_barycentric_backward": (None, [_p] * 6),
     "tg_interpolate3_scalar": (_f, [_p, _f, _f, _f, _p]),
@@ -82,6 +89,24 @@ SIGNATURES = {
     "tg_interpolate3_vector": (None, [_p] * 6),
     "tg_interpolate3_vector_backward": (None, [_p] * 11),
 }
+
+
+def _fields(pointers, sizes, *more):
+    return [(name, _p) for name in pointers.split()] + [(name, _i64) for name in sizes.split()] + list(more)
+
+
+class Recurrence(C.Structure):
+    """tg_recurrence"""
+    _fields_ = _fields("inputs gates initial offsets states final kept workspace stream grad_states grad_final grad_inputs grad_gates "
+                       "grad_initial", "sequences length channels gate_count type gate_type gate_form input_form reverse kept_bytes "
+                       "workspace_bytes")
+
+
+class Norm(C.Structure):
+    """tg_norm"""
+    _fields_ = _fields("x weight bias y statistics workspace stream grad_y grad_x grad_weight grad_bias",
+                       "samples positions channels groups type weight_type activation workspace_bytes", ("eps", C.c_double))
+
 
 _libs = {}
 
