@@ -512,7 +512,7 @@ int tg_clip_to_render(const tg_real *clip, int64_t n_vertices, tg_real *out, voi
  * g * channels / gates up to the next gate's.  reverse: each sequence from its last row to its first.  Products of successive gates
  * of a sequence are formed, of up to 4096 of them: they have to be representable, which those of decays (|a| <= 1) are.
  * initial, final and their gradients are (sequences, channels) tg_real; initial, grad_states, grad_final, and every output
- * but `final` may be null.  The final state of an empty sequence is its initial one.
+ * but `final` may be null.  The backward call reads inputs, gates, initial and offsets as the forward call did.  The final state of an empty sequence is its initial one.
  * tg_linear_recurrence_sizes writes the bytes of `kept` (what the forward call leaves for the backward call; null where none
  * follows) and of the forward and the backward call's workspaces. */
 #define TG_GATE_VALUE 0

@@ -392,6 +392,27 @@ def test_other_streams_and_graphs(cuda):
 
 
 @pytest.mark.gpu
+def test_more_elements_than_31_bits_count(cuda):
+    """2^31 elements and some: the last rows against the definition, started far enough before them that what is in front is forgotten."""
+    import trigrad_amd
+    rows, channels, tail = 2 ** 20 + 77, 2048, 400
+    x = torch.empty((1, rows, channels), dtype=torch.bfloat16, device=cuda)
+    g = torch.full((1, rows, 1), 0.5, dtype=torch.bfloat16, device=cuda)
+    for p in range(0, rows, 1 << 18):
+        x[:, p:p + (1 << 18)].normal_()
+    states, final = trigrad_amd.linear_recurrence(x, g)
+    want = reference(x[:, -tail:], g[:, -tail:], None, None, "value", "plain", False)
+    assert_near("states", states[:, -200:], tuple(t[:, -200:] for t in want["states"]))
+    assert_near("final", final, want["final"])
+    del states
+    leaf = x.requires_grad_()
+    states, _ = trigrad_amd.linear_recurrence(leaf, g)
+    (got,) = torch.autograd.grad(states, leaf, x.detach())
+    want = reference(x[:, -tail:], g[:, -tail:], None, None, "value", "plain", False, x.detach()[:, -tail:])
+    assert_near("grad_inputs", got[:, -tail:], want["grad_inputs"])
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("types", sorted(TYPES))
 @pytest.mark.parametrize("sequences,channels,gates", [(1, 1, 1), (1, 1024, 1024), (3, 30, 10), (7, 129, 129), (33, 256, 2), (2, 260, 1)])
 def test_step(sequences, channels, gates, types, cuda):
@@ -505,7 +526,7 @@ def test_native_refusals(bits):
         assert call(name) == -1 and name.encode() in lib.tg_last_error()  # null pointers
         assert call(name, channels=0, gate_count=0) == 0 and call(name, sequences=0) == 0  # nothing to do
         assert getattr(lib, name)(None) == -1
-    assert call("tg_linear_recurrence_backward", inputs=64, gates=64, kept=64, kept_bytes=1 << 30) == -2
+    assert call("tg_linear_recurrence_backward", length=5000, inputs=64, gates=64, kept=64, kept_bytes=1 << 30) == -2
     assert lib.tg_linear_recurrence_step(None, None, None, None, None, 2, 8, 4, kind, kind, 0, 0, None) == -1
     assert lib.tg_linear_recurrence_step(None, None, None, None, None, 2, 8, 3, kind, kind, 0, 0, None) == -1
     assert lib.tg_linear_recurrence_step(None, None, None, None, None, 0, 8, 4, kind, kind, 0, 0, None) == 0

@@ -1296,7 +1296,7 @@ def linear_recurrence_forward(inputs, gates, initial, offsets, sequences, length
     return states, final, kept
 
 
-def linear_recurrence_backward(inputs, gates, offsets, kept, grad_states, grad_final, sequences, length, gate_form, input_form, reverse,
+def linear_recurrence_backward(inputs, gates, initial, offsets, kept, grad_states, grad_final, sequences, length, gate_form, input_form, reverse,
                                need_inputs, need_gates, need_initial):
     """-> gradients of inputs, gates and the initial states, None where not needed."""
     dev = inputs.device
@@ -1307,7 +1307,7 @@ def linear_recurrence_backward(inputs, gates, offsets, kept, grad_states, grad_f
         grad_gates = torch.empty_like(gates) if need_gates else None
         grad_initial = torch.empty((sequences, inputs.shape[-1]), dtype=real_type(inputs.dtype), device=dev) if need_initial else None
         workspace = _bytes(sizes[2], dev)
-        r.kept, r.kept_bytes, r.workspace, r.workspace_bytes = _address(kept), sizes[0], _address(workspace), sizes[2]
+        r.initial, r.kept, r.kept_bytes, r.workspace, r.workspace_bytes = _address(initial), _address(kept), sizes[0], _address(workspace), sizes[2]
         r.grad_states, r.grad_final = _address(grad_states), _address(grad_final)
         r.grad_inputs, r.grad_gates, r.grad_initial = _address(grad_inputs), _address(grad_gates), _address(grad_initial)
         _lib.check(lib.tg_linear_recurrence_backward(C.byref(r)), "tg_linear_recurrence_backward", _bits(inputs))

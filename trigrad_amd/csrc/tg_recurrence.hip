@@ -1,54 +1,18 @@
-// tg_recurrence.hip -- the gated linear recurrence h_t = a_t h_{t-1} + u_t: whole sequences forward and backward, and a single step.
+// tg_recurrence.hip -- the gated linear recurrence h_t = a_t h_{t-1} + u_t: sizes, the calls, a single step (and, in the double library, a
+// plain walk through the rows; the float library's kernels are in tg_recurrence_forward.hip and tg_recurrence_backward.hip).
 //
 // With a = f(gate) and u = x or (1 - a) x, and l_t the gradient of h_t with all that follows from it,
 //     l_t = dh_t + a_{t+1} l_{t+1},   dx_t = l_t or (1 - a_t) l_t,   da_t = l_t h_{t-1} or l_t (h_{t-1} - x_t),   dgate = f'(gate) sum da
 // over the channels that share the gate.
-#include "tg_elements.hpp"
+#ifdef TG_DOUBLE_PRECISION
+#include "tg_recurrence.hpp"
+#else
+#include "tg_recurrence_scan.hpp"
+#endif
 
 namespace tg {
 
-// 1 - exp(g) for g <= 0 without the loss of its leading digits: near 0 by its series (the first term left out is below 2^-25 of it).
-__device__ __forceinline__ real one_minus_exp(real g, real e) {
 #ifdef TG_DOUBLE_PRECISION
-    return -expm1(g);
-#else
-    const float s = g * (1.0f + g * (1.0f / 2) * (1.0f + g * (1.0f / 3) * (1.0f + g * (1.0f / 4) * (1.0f + g * (1.0f / 5) *
-                    (1.0f + g * (1.0f / 6) * (1.0f + g * (1.0f / 7)))))));
-    return fabsf(g) < 0.35f ? -s : 1.0f - e;
-#endif
-}
-
-struct Gate {
-    real a, rest, slope;  // a, 1 - a, da / dgate
-};
-
-__device__ __forceinline__ Gate gate_of(int form, real g) {
-    Gate r;
-    if (form == TG_GATE_VALUE) {
-        r.a = g;
-        r.rest = (real)1 - g;
-        r.slope = (real)1;
-    } else if (form == TG_GATE_LOG) {
-        r.a = exp(g);
-        r.rest = one_minus_exp(g, r.a);
-        r.slope = r.a;
-    } else {
-        const real e = exp(-fabs(g)), big = (real)1 / ((real)1 + e), small = e * big;
-        r.a = g >= 0 ? big : small;
-        r.rest = g >= 0 ? small : big;
-        r.slope = big * small;
-    }
-    return r;
-}
-
-struct Shape {
-    int64_t sequences, length, channels, gates, shared;  // shared: channels of a gate
-    int gate_form;
-    bool complement, reverse;
-};
-
-__device__ __forceinline__ real fma_real(real a, real b, real c) { return fma(a, b, c); }
-
 // ---- one thread a sequence and channel ------------------------------------------------
 
 struct Rows {
@@ -91,7 +55,7 @@ __global__ void recurrence_forward_kernel(Shape m, const T *__restrict__ inputs,
         const Gate gate = gate_of(m.gate_form, (real)gates[r * m.gates + g]);
         const real x = (real)inputs[r * m.channels + d];
         if (kept) kept[r * m.channels + d] = h;
-        h = fma_real(gate.a, h, m.complement ? gate.rest * x : x);
+        h = fma(gate.a, h, m.complement ? gate.rest * x : x);
         if (states) states[r * m.channels + d] = (T)h;
     }
     final[id] = h;
@@ -116,7 +80,7 @@ __global__ void recurrence_backward_kernel(Shape m, const T *__restrict__ inputs
         for (int64_t d = g * m.shared; d < (g + 1) * m.shared; d++) {
             const int64_t at = r * m.channels + d;
             const real l = e[d] + (grad_states ? (real)grad_states[at] : (real)0);
-            sum = fma_real(l, m.complement ? kept[at] - (real)inputs[at] : kept[at], sum);
+            sum = fma(l, m.complement ? kept[at] - (real)inputs[at] : kept[at], sum);
             if (grad_inputs) grad_inputs[at] = (T)(m.complement ? gate.rest * l : l);
             e[d] = gate.a * l;
         }
@@ -128,6 +92,7 @@ __global__ void recurrence_backward_kernel(Shape m, const T *__restrict__ inputs
     }
     clear_outside(m, offsets, s, grad_gates, g, m.gates);
 }
+#endif  // TG_DOUBLE_PRECISION
 
 // ---- a single step ----------------------------------------------------------------------
 
@@ -141,14 +106,14 @@ __global__ __launch_bounds__(kStepThreads) void recurrence_step_kernel(Shape m, 
     const int64_t s = id / m.channels, g = id % m.channels / m.shared;
     const Gate gate = gate_of(m.gate_form, (real)gates[s * m.gates + g]);
     const real x = (real)inputs[id];
-    const real h = fma_real(gate.a, state[id], m.complement ? gate.rest * x : x);
+    const real h = fma(gate.a, state[id], m.complement ? gate.rest * x : x);
     new_state[id] = h;
     states[id] = (T)h;
 }
 
 // ---- host ---------------------------------------------------------------------------------
 
-static int check_shape(const char *fn, const tg_recurrence &r, Shape &m) {
+int recurrence_shape(const char *fn, const tg_recurrence &r, Shape &m) {
     if (r.sequences < 0 || r.length < 0 || r.channels < 0 || r.gate_count < 0 || (r.gate_count == 0) != (r.channels == 0) ||
         (r.gate_count > 0 && r.channels % r.gate_count != 0)) {
         set_error("%s: sizes", fn);
@@ -180,21 +145,189 @@ static int check_shape(const char *fn, const tg_recurrence &r, Shape &m) {
     return 0;
 }
 
+#ifdef TG_DOUBLE_PRECISION
+
+static int sizes_of(const char *, const tg_recurrence &r, const Shape &m, int64_t out[3]) {
+    out[0] = (r.offsets ? m.length : m.sequences * m.length) * m.channels * (int64_t)sizeof(real);
+    out[1] = 0;
+    out[2] = m.sequences * m.channels * (int64_t)sizeof(real);
+    return 0;
+}
+
+static int forward(const char *fn, const tg_recurrence &r, const Shape &m) {
+    TG_LAUNCH_AS("recurrence_forward", (recurrence_forward_kernel<real, real>), dim3((unsigned)ceil_div64(m.sequences * m.channels, 256)), dim3(256), 0,
+                 (hipStream_t)r.stream, m, (const real *)r.inputs, (const real *)r.gates, r.initial, r.offsets, (real *)r.states, r.final,
+                 (real *)r.kept);
+    return check_launch(fn);
+}
+
+static int backward(const char *fn, const tg_recurrence &r, const Shape &m) {
+    TG_LAUNCH_AS("recurrence_backward", (recurrence_backward_kernel<real, real>), dim3((unsigned)ceil_div64(m.sequences * m.gates, 256)), dim3(256), 0,
+                 (hipStream_t)r.stream, m, (const real *)r.inputs, (const real *)r.gates, r.offsets, (const real *)r.kept,
+                 (const real *)r.grad_states, r.grad_final, (real *)r.grad_inputs, (real *)r.grad_gates, r.grad_initial, (real *)r.workspace);
+    return check_launch(fn);
+}
+
+#else
+
+static int log2_above(int64_t n) {  // of the power of two that is n or more
+    int k = 0;
+    while (((int64_t)1 << k) < n) k++;
+    return k;
+}
+
+// Channels of a lane: two neighbours where they are aligned (or all three of a gate that has three), else one.
+static int vector_of(int64_t shared, int64_t channels, bool aligned) {
+    const int64_t run = shared > 1 ? shared : channels;
+    return run % 2 == 0 ? (aligned ? 2 : 1) : shared % 3 == 0 ? 3 : 1;
+}
+
+static bool aligned_for(int64_t bytes, std::initializer_list<const void *> pointers) {
+    for (const void *p : pointers)
+        if ((uintptr_t)p % (uintptr_t)bytes != 0) return false;
+    return true;
+}
+
+// Rows and columns of a call in one direction.  What the two directions have to agree on (whether the rows are chained, the rows
+// between kept states) does not depend on alignment.
+static Split split_of(const Shape &s, bool packed, int64_t wide_gates, int vector, bool backward) {
+    Split m = {};
+    m.packed = packed;
+    m.rows = packed ? s.length : s.sequences * s.length;
+    m.channels = s.channels;
+    m.gates = s.gates;
+    m.shared = s.shared;
+    m.length = s.length;
+    m.sequences = s.sequences;
+    m.gate_form = s.gate_form;
+    m.wide_gates = (int)wide_gates;
+    m.complement = s.complement;
+    m.reverse = s.reverse;
+    const int best = vector_of(s.shared, s.channels, true);
+    const auto columns = [&](int v, int most_lanes_log2) {
+        m.parts = 1;
+        m.gate_lanes_log2 = 0;
+        if (s.shared == 1) return ceil_div64(s.channels, v);
+        m.gate_lanes_log2 = std::min(log2_above(ceil_div64(s.shared, v)), most_lanes_log2);
+        m.parts = (int)ceil_div64(ceil_div64(s.shared, v), (int64_t)1 << m.gate_lanes_log2);
+        return s.gates * m.parts << m.gate_lanes_log2;
+    };
+    const int64_t wanted = columns(best, 6), axis = packed ? m.rows : s.length;
+    const int narrow = std::min(6, log2_above(wanted));  // lanes of a row where there are many rows
+    m.block_rows = (int64_t)(kBackwardThreads >> narrow) * kBackwardRows;
+    m.chained = axis > m.block_rows;
+    const int threads = backward ? kBackwardThreads : kForwardThreads, rows = backward ? kBackwardRows : kForwardRows;
+    const int threads_log2 = log2_above(threads);
+    m.lanes_log2 = narrow;
+    if (!m.chained) m.lanes_log2 = std::min(log2_above(wanted), std::max(narrow, threads_log2 - log2_above(ceil_div64(axis, rows))));
+    m.columns = columns(vector, std::min(6, m.lanes_log2));
+    m.tiles = ceil_div64(m.columns, (int64_t)1 << m.lanes_log2);
+    m.chunk_rows = (int64_t)(threads >> m.lanes_log2) * rows;
+    if (!m.chained) m.chunk_rows = packed ? std::max<int64_t>(m.rows, 1) : m.chunk_rows / s.length * s.length;
+    m.chunks = ceil_div64(m.rows, m.chunk_rows);
+    return m;
+}
+
+struct Room {
+    int64_t maps, states, words, sequences, partial, bytes;  // elements, and bytes of it all
+};
+static Room room_of(const Split &m, int vector, bool backward) {
+    Room r = {};
+    const int64_t row = m.tiles * vector << m.lanes_log2;
+    if (m.chained) {
+        r.maps = m.chunks * row;
+        r.states = ceil_div64(m.chunks, kChain) * row;
+    }
+    r.words = r.maps + ceil_div64(r.states, 2);
+    r.sequences = m.packed ? 2 * m.chunks : 0;
+    r.partial = backward && m.parts > 1 ? m.parts * m.rows * m.gates : 0;
+    r.bytes = m.chained || m.packed || r.partial ? r.words * 8 + 8 + r.sequences * 4 + r.partial * 4 : 0;
+    return r;
+}
+
+static int sizes_of(const char *fn, const tg_recurrence &r, const Shape &m, int64_t out[3]) {
+    out[0] = out[1] = out[2] = 0;
+    if (m.length == 0 || m.sequences == 0 || m.channels == 0) return 0;
+    const bool packed = r.offsets != nullptr;
+    for (int aligned = 0; aligned < 2; aligned++)
+        for (int backward = 0; backward < 2; backward++) {
+            const int vector = vector_of(m.shared, m.channels, aligned);
+            const Split s = split_of(m, packed, 0, vector, backward);
+            if (s.chunks * s.tiles >= (1 << 24)) {
+                set_error("%s: %lld rows of %lld channels are too many", fn, (long long)s.rows, (long long)s.channels);
+                return TG_E_ARG;
+            }
+            out[1 + backward] = std::max(out[1 + backward], room_of(s, vector, backward).bytes);
+            if (s.chained) out[0] = ceil_div64(s.rows, s.block_rows) * s.channels * 4;
+        }
+    return 0;
+}
+
+// The workspace's parts, and the kernel in front.
+static int prepare(const tg_recurrence &r, const Split &m, const Room &room, Chain &c, float *&partial, const float *from, float *to) {
+    char *at = (char *)r.workspace;
+    c.maps = (uint64_t *)at;
+    c.states = (uint32_t *)(at + room.maps * 8);
+    at += room.words * 8;
+    c.ticket = (uint32_t *)at;
+    at += 8;
+    c.first_sequence = (int32_t *)at;
+    at += room.sequences * 4;
+    partial = (float *)at;
+    if (!m.chained && !m.packed) return 0;
+    return launch_prepare(m, c, (uint64_t *)r.workspace, room.words, r.offsets, from, m.packed ? to : nullptr, (hipStream_t)r.stream);
+}
+
+static int forward(const char *fn, const tg_recurrence &r, const Shape &s) {
+    if (s.length == 0) {
+        const Split none = {0, s.channels, s.gates, s.shared, 0, s.sequences};
+        return launch_prepare(none, Chain(), nullptr, 0, nullptr, r.initial, r.final, (hipStream_t)r.stream);
+    }
+    const int64_t bytes = type_bytes(r.type), gate_bytes = type_bytes(r.gate_type);
+    const bool aligned = aligned_for(2 * bytes, {r.inputs, r.states}) && (s.shared > 1 || aligned_for(2 * gate_bytes, {r.gates}));
+    const int vector = vector_of(s.shared, s.channels, aligned);
+    const Split m = split_of(s, r.offsets != nullptr, r.gate_type == TG_TYPE_F32, vector, false);
+    Chain c = {};
+    float *partial;
+    if (const int code = prepare(r, m, room_of(m, vector, false), c, partial, r.initial, r.final)) return code;
+    tg_recurrence call = r;
+    if (!m.chained) call.kept = nullptr;  // every chunk begins with a sequence
+    (void)fn;
+    return launch_forward(call, m, c, vector, (unsigned)(m.chunks * m.tiles), (hipStream_t)r.stream);
+}
+
+static int backward(const char *fn, const tg_recurrence &r, const Shape &s) {
+    if (s.length == 0) {
+        if (!r.grad_initial) return 0;
+        const Split none = {0, s.channels, s.gates, s.shared, 0, s.sequences};
+        return launch_prepare(none, Chain(), nullptr, 0, nullptr, r.grad_final, r.grad_initial, (hipStream_t)r.stream);
+    }
+    const int64_t bytes = type_bytes(r.type), gate_bytes = type_bytes(r.gate_type);
+    const bool aligned = aligned_for(2 * bytes, {r.inputs, r.grad_states, r.grad_inputs}) &&
+                         (s.shared > 1 || aligned_for(2 * gate_bytes, {r.gates, r.grad_gates}));
+    const int vector = vector_of(s.shared, s.channels, aligned);
+    const Split m = split_of(s, r.offsets != nullptr, r.gate_type == TG_TYPE_F32, vector, true);
+    Chain c = {};
+    float *partial;
+    if (const int code = prepare(r, m, room_of(m, vector, true), c, partial, r.grad_final, r.grad_initial)) return code;
+    (void)fn;
+    return launch_backward(r, m, c, partial, vector, (unsigned)(m.chunks * m.tiles), (hipStream_t)r.stream);
+}
+
+#endif  // TG_DOUBLE_PRECISION
+
 }  // namespace tg
 
 extern "C" int tg_linear_recurrence_sizes(const tg_recurrence *r, int64_t out[3]) {
     using namespace tg;
+    const char *fn = "tg_linear_recurrence_sizes";
     if (!r || !out) {
-        set_error("tg_linear_recurrence_sizes: null pointer");
+        set_error("%s: null pointer", fn);
         return TG_E_ARG;
     }
     Shape m;
-    if (const int code = check_shape("tg_linear_recurrence_sizes", *r, m)) return code;
-    const int64_t rows = r->offsets ? m.length : m.sequences * m.length;
-    out[0] = rows * m.channels * (int64_t)sizeof(real);
-    out[1] = 0;
-    out[2] = m.sequences * m.channels * (int64_t)sizeof(real);
-    return 0;
+    if (const int code = recurrence_shape(fn, *r, m)) return code;
+    return sizes_of(fn, *r, m, out);
 }
 
 extern "C" int tg_linear_recurrence_forward(const tg_recurrence *r) {
@@ -206,22 +339,18 @@ extern "C" int tg_linear_recurrence_forward(const tg_recurrence *r) {
         set_error("%s: null pointer", fn);
         return TG_E_ARG;
     }
-    if (const int code = check_shape(fn, *r, m)) return code;
+    if (const int code = recurrence_shape(fn, *r, m)) return code;
     if (m.sequences == 0 || m.channels == 0) return 0;
-    tg_linear_recurrence_sizes(r, sizes);
+    if (const int code = sizes_of(fn, *r, m, sizes)) return code;
     if ((m.length > 0 && (!r->inputs || !r->gates)) || !r->final || (r->kept && r->kept_bytes < sizes[0])) {
         set_error("%s: null pointer, or kept too small", fn);
         return TG_E_ARG;
     }
-    hipStream_t stream = (hipStream_t)r->stream;
-    return by_types(r->type, r->gate_type, [&](auto t, auto s) {
-        using T = decltype(t);
-        using S = decltype(s);
-        const int64_t n = m.sequences * m.channels;
-        TG_LAUNCH_AS("recurrence_forward", (recurrence_forward_kernel<T, S>), dim3((unsigned)ceil_div64(n, 256)), dim3(256), 0, stream, m,
-                     (const T *)r->inputs, (const S *)r->gates, r->initial, r->offsets, (T *)r->states, r->final, (real *)r->kept);
-        return check_launch(fn);
-    });
+    if (sizes[1] > 0 && (!r->workspace || r->workspace_bytes < sizes[1])) {
+        set_error("%s: workspace of %lld bytes, %lld needed", fn, (long long)r->workspace_bytes, (long long)sizes[1]);
+        return TG_E_WORKSPACE;
+    }
+    return forward(fn, *r, m);
 }
 
 extern "C" int tg_linear_recurrence_backward(const tg_recurrence *r) {
@@ -233,27 +362,18 @@ extern "C" int tg_linear_recurrence_backward(const tg_recurrence *r) {
         set_error("%s: null pointer", fn);
         return TG_E_ARG;
     }
-    if (const int code = check_shape(fn, *r, m)) return code;
+    if (const int code = recurrence_shape(fn, *r, m)) return code;
     if (m.sequences == 0 || m.channels == 0) return 0;
-    tg_linear_recurrence_sizes(r, sizes);
-    if (m.length > 0 && (!r->inputs || !r->gates || !r->kept || r->kept_bytes < sizes[0])) {
+    if (const int code = sizes_of(fn, *r, m, sizes)) return code;
+    if (m.length > 0 && (!r->inputs || !r->gates || (sizes[0] > 0 && (!r->kept || r->kept_bytes < sizes[0])))) {
         set_error("%s: null pointer, or kept too small", fn);
         return TG_E_ARG;
     }
-    if (!r->workspace || r->workspace_bytes < sizes[2]) {
+    if (sizes[2] > 0 && (!r->workspace || r->workspace_bytes < sizes[2])) {
         set_error("%s: workspace of %lld bytes, %lld needed", fn, (long long)r->workspace_bytes, (long long)sizes[2]);
         return TG_E_WORKSPACE;
     }
-    hipStream_t stream = (hipStream_t)r->stream;
-    return by_types(r->type, r->gate_type, [&](auto t, auto s) {
-        using T = decltype(t);
-        using S = decltype(s);
-        const int64_t n = m.sequences * m.gates;
-        TG_LAUNCH_AS("recurrence_backward", (recurrence_backward_kernel<T, S>), dim3((unsigned)ceil_div64(n, 256)), dim3(256), 0, stream, m,
-                     (const T *)r->inputs, (const S *)r->gates, r->offsets, (const real *)r->kept, (const T *)r->grad_states, r->grad_final,
-                     (T *)r->grad_inputs, (S *)r->grad_gates, r->grad_initial, (real *)r->workspace);
-        return check_launch(fn);
-    });
+    return backward(fn, *r, m);
 }
 
 extern "C" int tg_linear_recurrence_step(const void *inputs, const void *gates, const tg_real *state, void *states, tg_real *new_state,
@@ -271,7 +391,7 @@ extern "C" int tg_linear_recurrence_step(const void *inputs, const void *gates, 
     r.gate_form = gate_form;
     r.input_form = input_form;
     Shape m;
-    if (const int code = check_shape(fn, r, m)) return code;
+    if (const int code = recurrence_shape(fn, r, m)) return code;
     if (m.sequences == 0 || m.channels == 0) return 0;
     if (!inputs || !gates || !state || !states || !new_state) {
         set_error("%s: null pointer", fn);

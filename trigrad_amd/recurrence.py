@@ -77,8 +77,8 @@ class LinearRecurrence(Function):
     @once_differentiable
     def backward(ctx, grad_states, grad_final):
         inputs, gates, kept, *more = ctx.saved_tensors
-        offsets = more[-1] if ctx.has[1] else None
-        grads = _C.linear_recurrence_backward(inputs, gates, offsets, kept, grad_states, grad_final, *ctx.form, *ctx.needs_input_grad[:3])
+        initial, offsets = more[0] if ctx.has[0] else None, more[-1] if ctx.has[1] else None
+        grads = _C.linear_recurrence_backward(inputs, gates, initial, offsets, kept, grad_states, grad_final, *ctx.form, *ctx.needs_input_grad[:3])
         return (*grads, None, None, None, None, None)
 
 
