@@ -229,16 +229,17 @@ static Split split_of(const Shape &s, bool packed, int64_t wide_gates, int vecto
 }
 
 struct Room {
-    int64_t maps, states, words, sequences, partial, bytes;  // elements, and bytes of it all
+    int64_t maps, groups, states, words, sequences, partial, bytes;  // elements, and bytes of it all
 };
 static Room room_of(const Split &m, int vector, bool backward) {
     Room r = {};
     const int64_t row = m.tiles * vector << m.lanes_log2;
     if (m.chained) {
         r.maps = m.chunks * row;
-        r.states = ceil_div64(m.chunks, kChain) * row;
+        r.groups = ceil_div64(m.chunks, kChain) * row;
+        r.states = ceil_div64(m.chunks, kChain * kChain) * row;
     }
-    r.words = r.maps + ceil_div64(r.states, 2);
+    r.words = r.maps + r.groups + ceil_div64(r.states, 2);
     r.sequences = m.packed ? 2 * m.chunks : 0;
     r.partial = backward && m.parts > 1 ? m.parts * m.rows * m.gates : 0;
     r.bytes = m.chained || m.packed || r.partial ? r.words * 8 + 8 + r.sequences * 4 + r.partial * 4 : 0;
@@ -267,7 +268,8 @@ static int sizes_of(const char *fn, const tg_recurrence &r, const Shape &m, int6
 static int prepare(const tg_recurrence &r, const Split &m, const Room &room, Chain &c, float *&partial, const float *from, float *to) {
     char *at = (char *)r.workspace;
     c.maps = (uint64_t *)at;
-    c.states = (uint32_t *)(at + room.maps * 8);
+    c.groups = (uint64_t *)(at + room.maps * 8);
+    c.states = (uint32_t *)(at + (room.maps + room.groups) * 8);
     at += room.words * 8;
     c.ticket = (uint32_t *)at;
     at += 8;

@@ -10,7 +10,7 @@ struct Marks {
 };
 
 template <class T, int V, bool Shared, int K, int Threads>
-__global__ __launch_bounds__(Threads) void recurrence_forward_kernel(Split m, Chain c, const T *__restrict__ inputs, const void *__restrict__ gates,
+__global__ __launch_bounds__(Threads, 4) void recurrence_forward_kernel(Split m, Chain c, const T *__restrict__ inputs, const void *__restrict__ gates,
                                                                      const float *__restrict__ initial, const int32_t *__restrict__ offsets,
                                                                      T *__restrict__ states, float *__restrict__ final, float *__restrict__ kept) {
     constexpr int GV = Shared ? 1 : V;

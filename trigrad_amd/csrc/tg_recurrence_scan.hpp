@@ -6,9 +6,10 @@
 // rows of V channels in registers, so the inputs are read once.  Its map is composed
 //   1. over the threads of a wave that hold other rows of the same channels (there are some where there are few channels),
 //   2. over the workgroup's waves, through LDS,
-//   3. over the workgroups: a chunk of rows publishes its map, the last chunk of every kChain publishes the state behind it, and a
-//      chunk starts from that state and the maps of the chunks between: a fixed order of operations, so results do not depend on
-//      timing, and one wait for kChain chunks in the chain from the first to the last.
+//   3. over the workgroups: a chunk of rows publishes its map; the last of every kChain chunks that of their group; the last of every
+//      kChain groups the state behind it.  A chunk starts from the last such state and goes over the groups and then the chunks
+//      between: a fixed order of operations, so results do not depend on timing, and one wait for kChain^2 chunks in the chain from the
+//      first chunk to the last.  Nothing in front of a closed map is waited for.
 // Chunks are numbered by a ticket, taken when a workgroup starts, so every chunk that is waited for is running or done and waits
 // only on lower ones itself.  Waits are bounded all the same: one that expires makes its chunk's states NaN.
 // A published word holds its own "not there yet" (all ones, a NaN that no result has), so no fence orders a flag with its data: 8 bytes
@@ -43,7 +44,8 @@ struct Split {
 // Workspace of a chained or packed call; where[] says at what byte.
 struct Chain {
     uint64_t *maps;       // [chunks][tiles * lanes * V]
-    uint32_t *states;     // [groups of kChain chunks][tiles * lanes * V]
+    uint64_t *groups;     // [chunks / kChain][tiles * lanes * V]
+    uint32_t *states;     // [chunks / kChain^2][tiles * lanes * V]
     uint32_t *ticket;
     int32_t *first_sequence;  // [chunks][2] (packed): the sequences that the chunk's first and last row are searched between
 };
@@ -69,14 +71,35 @@ template <int V> __device__ __forceinline__ void compose(Map<V> &later, const Ma
 
 __device__ __forceinline__ uint32_t word_of(float f) { return f != f ? 0x7fc00000u : __float_as_uint(f); }
 
-template <class W> __device__ __forceinline__ W wait_for(const W *word, W absent, bool &expired) {
-    W w = __hip_atomic_load(word, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    for (uint32_t spins = 0; w == absent && spins < kWaitLimit; spins++) {
+template <class W> __device__ __forceinline__ W look(const W *word) {
+    return __hip_atomic_load(word, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+
+// The word, once it is there; `seen` is what a look at it found.
+template <class W> __device__ __forceinline__ W wait_for(const W *word, W absent, W seen, bool &expired) {
+    for (uint32_t spins = 0; seen == absent && spins < kWaitLimit; spins++) {
         __builtin_amdgcn_s_sleep(1);
-        w = __hip_atomic_load(word, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        seen = look(word);
     }
-    if (w == absent) expired = true;
-    return w;
+    if (seen == absent) expired = true;
+    return seen;
+}
+
+template <int V> __device__ __forceinline__ void publish(uint64_t *words, const Map<V> &map) {
+#pragma unroll
+    for (int v = 0; v < V; v++) {
+        const uint32_t a = map.closed ? kClosedMap : word_of(map.a[v]);
+        __hip_atomic_store(&words[v], (uint64_t)a << 32 | word_of(map.u[v]), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    }
+}
+template <int V> __device__ __forceinline__ void publish(uint32_t *words, const float (&h)[V]) {
+#pragma unroll
+    for (int v = 0; v < V; v++) __hip_atomic_store(&words[v], word_of(h[v]), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+
+template <int V> __device__ __forceinline__ void step_over(float (&h)[V], const Map<V> &map) {
+#pragma unroll
+    for (int v = 0; v < V; v++) h[v] = map.closed ? map.u[v] : apply(map.a[v], h[v], map.u[v]);
 }
 
 // What each place of the chunk is, and whose: by one thread a place.  seq[i] is in [0, sequences) wherever flags say it is used.
@@ -168,14 +191,40 @@ __device__ __forceinline__ void load_gates(const Split &m, const void *gates, in
     }
 }
 
-// The maps of the workgroup's threads in the order of the recurrence (or, Backward, against it), composed: on return `map` is the map
-// of all rows of the workgroup before the thread's own (within its wave) and entry[] those of the waves or threads before; an entry's
-// maps are [lane of the row][V].
+// Maps that other workgroups published, in LDS: [which][lane][V].
+template <int V> struct Published {
+    float a[kChain * kWave * V], u[kChain * kWave * V];
+    bool closed[kChain];
+    template <int W> __device__ __forceinline__ Map<W> at(int i, int lanes, int lane) const {
+        Map<W> r;
+#pragma unroll
+        for (int v = 0; v < V; v++) {
+            r.a[v] = a[(i * lanes + lane) * V + v];
+            r.u[v] = u[(i * lanes + lane) * V + v];
+        }
+        r.closed = closed[i];
+        return r;
+    }
+};
+
+template <int V>
+__device__ __forceinline__ void settle(Published<V> &to, int i, int lanes, int lane, const uint64_t (&seen)[V], const uint64_t *words, bool &expired) {
+#pragma unroll
+    for (int v = 0; v < V; v++) {
+        const uint64_t w = wait_for(&words[v], ~(uint64_t)0, seen[v], expired);
+        const uint32_t a = (uint32_t)(w >> 32);
+        to.a[(i * lanes + lane) * V + v] = __uint_as_float(a);
+        to.u[(i * lanes + lane) * V + v] = __uint_as_float((uint32_t)w);
+        if (lane == 0 && v == 0) to.closed[i] = a == kClosedMap;
+    }
+}
+
+// The maps of the workgroup's threads, or waves, [entry][lane][V].
 template <int V, int Threads> struct Joint {
     float a[Threads * V], u[Threads * V];
-    float chain_a[kChain * kWave * V], chain_u[kChain * kWave * V];
+    Published<V> maps, groups;
     float state[Threads * V];
-    uint8_t closed[Threads], chain_closed[kChain];
+    bool closed[Threads];
 };
 
 template <int V> __device__ __forceinline__ Map<V> shifted(const Map<V> &m, int lanes, bool backward) {
@@ -257,8 +306,9 @@ __device__ __forceinline__ void join(const Split &m, const Chain &c, Joint<V, Th
     __syncthreads();
     const int64_t words = m.tiles * lanes * V, at = (tile * lanes + p.lane) * V;
     if (chained) {
+        const bool ends_group = order % kChain == kChain - 1, ends_super = order % (kChain * kChain) == kChain * kChain - 1;
+        const int64_t group = order / kChain, super = group / kChain;
         Map<V> total = unit_map<V>();
-        const bool last_of_group = (order + 1) % kChain == 0 || order + 1 == m.chunks;
         if (p.leads) {
             for (int i = 0; i < p.entries; i++) {
                 const int e = Backward ? p.entries - 1 - i : i;
@@ -272,61 +322,78 @@ __device__ __forceinline__ void join(const Split &m, const Chain &c, Joint<V, Th
                 compose(next, total);
                 total = next;
             }
-            if (!last_of_group) {
+            if (!ends_group) publish(c.maps + order * words + at, total);
+            else if (total.closed && !ends_super) publish(c.groups + group * words + at, total);
+            if (ends_super && total.closed) publish(c.states + super * words + at, total.u);
+        }
+        const int maps = (int)(order % kChain), groups = (int)(group % kChain);
+        if (!chunk_closed) {
+            // one look at all that may be needed, then waits for what was not there
+            constexpr int Turns = Threads / kWave, Rounds = kChain / Turns + (kChain % Turns ? 1 : 0);
+            const int turns = Threads >> m.lanes_log2;
+            bool expired = false;
+            uint64_t seen_map[Rounds][V], seen_group[Rounds][V];
+            uint32_t seen_state[V];
+#pragma unroll
+            for (int r = 0; r < Rounds; r++) {
+                const int i = p.turn + r * turns;
 #pragma unroll
                 for (int v = 0; v < V; v++) {
-                    const uint32_t a = total.closed ? kClosedMap : word_of(total.a[v]);
-                    __hip_atomic_store(&c.maps[order * words + at + v], (uint64_t)a << 32 | word_of(total.u[v]), __ATOMIC_RELAXED,
-                                       __HIP_MEMORY_SCOPE_AGENT);
+                    seen_map[r][v] = i < maps ? look(&c.maps[(group * kChain + i) * words + at + v]) : 0;
+                    seen_group[r][v] = i < groups ? look(&c.groups[(super * kChain + i) * words + at + v]) : 0;
                 }
             }
-        }
-        const int64_t group = order / kChain;
-        const int in_front = (int)(order - group * kChain);
-        if (!chunk_closed) {
-            bool expired = false;
-            const int turns = Threads >> m.lanes_log2;
-            for (int i = p.turn; i < in_front; i += turns) {
 #pragma unroll
-                for (int v = 0; v < V; v++) {
-                    const uint64_t w = wait_for(&c.maps[(group * kChain + i) * words + at + v], ~(uint64_t)0, expired);
-                    const uint32_t a = (uint32_t)(w >> 32);
-                    j.chain_a[(i * lanes + p.lane) * V + v] = a == kClosedMap ? 0.0f : __uint_as_float(a);
-                    j.chain_u[(i * lanes + p.lane) * V + v] = __uint_as_float((uint32_t)w);
-                    if (p.lane == 0 && v == 0) j.chain_closed[i] = a == kClosedMap;
+            for (int v = 0; v < V; v++) seen_state[v] = p.leads && super > 0 ? look(&c.states[(super - 1) * words + at + v]) : 0;
+#pragma unroll
+            for (int r = 0; r < Rounds; r++) {
+                const int i = p.turn + r * turns;
+                if (i < maps) settle<V>(j.maps, i, lanes, p.lane, seen_map[r], c.maps + (group * kChain + i) * words + at, expired);
+            }
+            bool failed = __syncthreads_or(expired) != 0, shut = false;
+            for (int i = 0; i < maps; i++) shut = shut || j.maps.closed[i];
+            if (ends_group && !ends_super && !total.closed && p.leads) {
+                Map<V> all = total;
+                for (int i = maps - 1; i >= 0; i--) compose(all, j.maps.template at<V>(i, lanes, p.lane));
+                if (failed)
+#pragma unroll
+                    for (int v = 0; v < V; v++) all.u[v] = __uint_as_float(0x7fc00000u);
+                publish(c.groups + group * words + at, all);
+            }
+            if (!shut) {
+#pragma unroll
+                for (int r = 0; r < Rounds; r++) {
+                    const int i = p.turn + r * turns;
+                    if (i < groups) settle<V>(j.groups, i, lanes, p.lane, seen_group[r], c.groups + (super * kChain + i) * words + at, expired);
                 }
+                failed = __syncthreads_or(expired) != 0;
             }
             if (p.leads) {
+                bool open = !shut;
+                if (open)
+                    for (int i = 0; i < groups; i++) open = open && !j.groups.closed[i];
+                expired = false;
 #pragma unroll
                 for (int v = 0; v < V; v++)
-                    h[v] = group == 0 ? 0.0f : __uint_as_float(wait_for(&c.states[(group - 1) * words + at + v], kAbsent, expired));
-            }
-            const bool any = __syncthreads_or(expired);
-            if (p.leads) {
-                for (int i = 0; i < in_front; i++) {
-                    const bool closed = j.chain_closed[i];
-#pragma unroll
-                    for (int v = 0; v < V; v++) {
-                        const float u = j.chain_u[(i * lanes + p.lane) * V + v];
-                        h[v] = closed ? u : apply(j.chain_a[(i * lanes + p.lane) * V + v], h[v], u);
-                    }
-                }
-                if (any) {
+                    h[v] = open && super > 0 ? __uint_as_float(wait_for(&c.states[(super - 1) * words + at + v], kAbsent, seen_state[v], expired)) : 0.0f;
+                if (!shut)
+                    for (int i = 0; i < groups; i++) step_over(h, j.groups.template at<V>(i, lanes, p.lane));
+                for (int i = 0; i < maps; i++) step_over(h, j.maps.template at<V>(i, lanes, p.lane));
+                if (failed || expired)
 #pragma unroll
                     for (int v = 0; v < V; v++) h[v] = __uint_as_float(0x7fc00000u);
-                }
             }
         } else if (p.leads) {
 #pragma unroll
             for (int v = 0; v < V; v++) h[v] = 0.0f;
         }
         if (p.leads) {
-            if (last_of_group && order + 1 != m.chunks) {
+            if (ends_super && !total.closed) {
+                float end[V];
 #pragma unroll
-                for (int v = 0; v < V; v++) {
-                    const float end = total.closed ? total.u[v] : apply(total.a[v], h[v], total.u[v]);
-                    __hip_atomic_store(&c.states[group * words + at + v], word_of(end), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-                }
+                for (int v = 0; v < V; v++) end[v] = h[v];
+                step_over(end, total);
+                publish(c.states + super * words + at, end);
             }
 #pragma unroll
             for (int v = 0; v < V; v++) j.state[p.lane * V + v] = h[v];
@@ -342,15 +409,16 @@ __device__ __forceinline__ void join(const Split &m, const Chain &c, Joint<V, Th
     const int mine = Backward ? p.entries - 1 - p.entry : p.entry;
     for (int i = 0; i < mine; i++) {
         const int e = Backward ? p.entries - 1 - i : i;
-        const bool closed = j.closed[e];
+        Map<V> next;
 #pragma unroll
         for (int v = 0; v < V; v++) {
-            const float u = j.u[(e * lanes + p.lane) * V + v];
-            h[v] = closed ? u : apply(j.a[(e * lanes + p.lane) * V + v], h[v], u);
+            next.a[v] = j.a[(e * lanes + p.lane) * V + v];
+            next.u[v] = j.u[(e * lanes + p.lane) * V + v];
         }
+        next.closed = j.closed[e];
+        step_over(h, next);
     }
-#pragma unroll
-    for (int v = 0; v < V; v++) h[v] = before.closed ? before.u[v] : apply(before.a[v], h[v], before.u[v]);
+    step_over(h, before);
 }
 
 // The workgroup's chunk in the order of the chain, and its tile of columns.  Chained: by ticket.
