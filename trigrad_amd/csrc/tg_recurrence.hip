@@ -129,9 +129,9 @@ int recurrence_shape(const char *fn, const tg_recurrence &r, Shape &m) {
     }
     const int64_t limit = (int64_t)1 << 40;
     const int64_t rows = r.offsets ? r.length : r.length == 0 ? 0 : r.sequences > limit / r.length ? limit : r.sequences * r.length;
-    if (rows >= limit || (r.offsets && r.length > 0x7fffffff) || r.channels >= ((int64_t)1 << 31) || r.sequences >= ((int64_t)1 << 31) ||
+    if (rows >= limit || (r.offsets && r.length > 0x7fffffff) || r.channels >= ((int64_t)1 << 31) || r.sequences >= ((int64_t)1 << 29) ||
         (r.channels > 0 && (rows > limit / r.channels || r.sequences > limit / r.channels))) {
-        set_error("%s: more than 2^40 elements, or a size of 2^31", fn);
+        set_error("%s: more than 2^40 elements, 2^29 sequences or 2^31 channels", fn);
         return TG_E_ARG;
     }
     m.sequences = r.sequences;
@@ -188,8 +188,8 @@ static bool aligned_for(int64_t bytes, std::initializer_list<const void *> point
     return true;
 }
 
-// Rows and columns of a call in one direction.  What the two directions have to agree on (whether the rows are chained, the rows
-// between kept states) does not depend on alignment.
+// Rows and columns of a call in one direction.  What the two directions have to agree on (whether the rows are chained, and into which
+// chunks) does not depend on alignment.
 static Split split_of(const Shape &s, bool packed, int64_t wide_gates, int vector, bool backward) {
     Split m = {};
     m.packed = packed;
@@ -214,8 +214,7 @@ static Split split_of(const Shape &s, bool packed, int64_t wide_gates, int vecto
     };
     const int64_t wanted = columns(best, 6), axis = packed ? m.rows : s.length;
     const int narrow = std::min(6, log2_above(wanted));  // lanes of a row where there are many rows
-    m.block_rows = (int64_t)(kBackwardThreads >> narrow) * kBackwardRows;
-    m.chained = axis > m.block_rows;
+    m.chained = axis > kChunk >> narrow;
     const int threads = backward ? kBackwardThreads : kForwardThreads, rows = backward ? kBackwardRows : kForwardRows;
     const int threads_log2 = log2_above(threads);
     m.lanes_log2 = narrow;
@@ -228,21 +227,17 @@ static Split split_of(const Shape &s, bool packed, int64_t wide_gates, int vecto
     return m;
 }
 
+// The workspace: sequences to search between (packed), what chunks start from, their maps, sums of gates' gradients by waves.  Bytes.
 struct Room {
-    int64_t maps, groups, states, words, sequences, partial, bytes;  // elements, and bytes of it all
+    int64_t sequences, starts, maps, partial, all;
 };
-static Room room_of(const Split &m, int vector, bool backward) {
+static Room room_of(const Split &m, bool backward) {
     Room r = {};
-    const int64_t row = m.tiles * vector << m.lanes_log2;
-    if (m.chained) {
-        r.maps = m.chunks * row;
-        r.groups = ceil_div64(m.chunks, kChain) * row;
-        r.states = ceil_div64(m.chunks, kChain * kChain) * row;
-    }
-    r.words = r.maps + r.groups + ceil_div64(r.states, 2);
-    r.sequences = m.packed ? 2 * m.chunks : 0;
-    r.partial = backward && m.parts > 1 ? m.parts * m.rows * m.gates : 0;
-    r.bytes = m.chained || m.packed || r.partial ? r.words * 8 + 8 + r.sequences * 4 + r.partial * 4 : 0;
+    r.maps = m.chained ? m.chunks * m.channels * (int64_t)sizeof(MapWords) : 0;
+    r.starts = m.chained ? (m.chunks * m.channels + 1) / 2 * 8 : 0;
+    r.sequences = m.packed ? m.chunks * 8 : 0;
+    r.partial = backward && m.parts > 1 ? m.parts * m.rows * m.gates * 4 : 0;
+    r.all = r.sequences + r.starts + r.maps + r.partial;
     return r;
 }
 
@@ -252,69 +247,49 @@ static int sizes_of(const char *fn, const tg_recurrence &r, const Shape &m, int6
     const bool packed = r.offsets != nullptr;
     for (int aligned = 0; aligned < 2; aligned++)
         for (int backward = 0; backward < 2; backward++) {
-            const int vector = vector_of(m.shared, m.channels, aligned);
-            const Split s = split_of(m, packed, 0, vector, backward);
-            if (s.chunks * s.tiles >= (1 << 24)) {
+            const Split s = split_of(m, packed, 0, vector_of(m.shared, m.channels, aligned), backward);
+            if (s.chunks * s.tiles >= (1 << 22)) {
                 set_error("%s: %lld rows of %lld channels are too many", fn, (long long)s.rows, (long long)s.channels);
                 return TG_E_ARG;
             }
-            out[1 + backward] = std::max(out[1 + backward], room_of(s, vector, backward).bytes);
-            if (s.chained) out[0] = ceil_div64(s.rows, s.block_rows) * s.channels * 4;
+            const Room room = room_of(s, backward);
+            out[1 + backward] = std::max(out[1 + backward], room.all);
+            out[0] = room.starts;
         }
     return 0;
 }
 
-// The workspace's parts, and the kernel in front.
-static int prepare(const tg_recurrence &r, const Split &m, const Room &room, Chain &c, float *&partial, const float *from, float *to) {
+static int run(const tg_recurrence &r, const Shape &s, bool backward) {
+    hipStream_t stream = (hipStream_t)r.stream;
+    const float *from = backward ? r.grad_final : r.initial;
+    float *to = backward ? r.grad_initial : r.final;
+    if (s.length == 0) {
+        const Split none = {0, s.channels, s.gates, s.shared, 0, s.sequences};
+        return to ? launch_prepare(none, nullptr, nullptr, from, to, stream) : 0;
+    }
+    const int64_t bytes = type_bytes(r.type), gate_bytes = type_bytes(r.gate_type);
+    bool aligned = aligned_for(2 * bytes, {r.inputs, r.states, r.grad_states, r.grad_inputs});
+    if (s.shared == 1) aligned = aligned && aligned_for(2 * gate_bytes, {r.gates, r.grad_gates});
+    const int vector = vector_of(s.shared, s.channels, aligned);
+    const Split m = split_of(s, r.offsets != nullptr, r.gate_type == TG_TYPE_F32, vector, backward);
+    const Room room = room_of(m, backward);
     char *at = (char *)r.workspace;
-    c.maps = (uint64_t *)at;
-    c.groups = (uint64_t *)(at + room.maps * 8);
-    c.states = (uint32_t *)(at + (room.maps + room.groups) * 8);
-    at += room.words * 8;
-    c.ticket = (uint32_t *)at;
-    at += 8;
-    c.first_sequence = (int32_t *)at;
-    at += room.sequences * 4;
-    partial = (float *)at;
-    if (!m.chained && !m.packed) return 0;
-    return launch_prepare(m, c, (uint64_t *)r.workspace, room.words, r.offsets, from, m.packed ? to : nullptr, (hipStream_t)r.stream);
+    int32_t *first_sequence = (int32_t *)at;
+    float *starts = (float *)(at + room.sequences);
+    MapWords *maps = (MapWords *)(at + room.sequences + room.starts);
+    float *partial = (float *)(at + room.sequences + room.starts + room.maps);
+    if (!backward && r.kept) starts = (float *)r.kept;
+    if (m.packed)
+        if (const int code = launch_prepare(m, first_sequence, r.offsets, from, to, stream)) return code;
+    if (m.chained)
+        if (const int code = launch_starts(r, m, first_sequence, maps, starts, vector, backward, stream)) return code;
+    const unsigned blocks = (unsigned)(m.chunks * m.tiles);
+    return backward ? launch_backward(r, m, first_sequence, starts, partial, vector, blocks, stream)
+                    : launch_forward(r, m, first_sequence, starts, vector, blocks, stream);
 }
 
-static int forward(const char *fn, const tg_recurrence &r, const Shape &s) {
-    if (s.length == 0) {
-        const Split none = {0, s.channels, s.gates, s.shared, 0, s.sequences};
-        return launch_prepare(none, Chain(), nullptr, 0, nullptr, r.initial, r.final, (hipStream_t)r.stream);
-    }
-    const int64_t bytes = type_bytes(r.type), gate_bytes = type_bytes(r.gate_type);
-    const bool aligned = aligned_for(2 * bytes, {r.inputs, r.states}) && (s.shared > 1 || aligned_for(2 * gate_bytes, {r.gates}));
-    const int vector = vector_of(s.shared, s.channels, aligned);
-    const Split m = split_of(s, r.offsets != nullptr, r.gate_type == TG_TYPE_F32, vector, false);
-    Chain c = {};
-    float *partial;
-    if (const int code = prepare(r, m, room_of(m, vector, false), c, partial, r.initial, r.final)) return code;
-    tg_recurrence call = r;
-    if (!m.chained) call.kept = nullptr;  // every chunk begins with a sequence
-    (void)fn;
-    return launch_forward(call, m, c, vector, (unsigned)(m.chunks * m.tiles), (hipStream_t)r.stream);
-}
-
-static int backward(const char *fn, const tg_recurrence &r, const Shape &s) {
-    if (s.length == 0) {
-        if (!r.grad_initial) return 0;
-        const Split none = {0, s.channels, s.gates, s.shared, 0, s.sequences};
-        return launch_prepare(none, Chain(), nullptr, 0, nullptr, r.grad_final, r.grad_initial, (hipStream_t)r.stream);
-    }
-    const int64_t bytes = type_bytes(r.type), gate_bytes = type_bytes(r.gate_type);
-    const bool aligned = aligned_for(2 * bytes, {r.inputs, r.grad_states, r.grad_inputs}) &&
-                         (s.shared > 1 || aligned_for(2 * gate_bytes, {r.gates, r.grad_gates}));
-    const int vector = vector_of(s.shared, s.channels, aligned);
-    const Split m = split_of(s, r.offsets != nullptr, r.gate_type == TG_TYPE_F32, vector, true);
-    Chain c = {};
-    float *partial;
-    if (const int code = prepare(r, m, room_of(m, vector, true), c, partial, r.grad_final, r.grad_initial)) return code;
-    (void)fn;
-    return launch_backward(r, m, c, partial, vector, (unsigned)(m.chunks * m.tiles), (hipStream_t)r.stream);
-}
+static int forward(const char *, const tg_recurrence &r, const Shape &s) { return run(r, s, false); }
+static int backward(const char *, const tg_recurrence &r, const Shape &s) { return run(r, s, true); }
 
 #endif  // TG_DOUBLE_PRECISION
 

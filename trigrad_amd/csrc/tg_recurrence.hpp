@@ -13,43 +13,43 @@ __device__ __forceinline__ real exp_real(real g) { return exp(g); }
 __device__ __forceinline__ real one_minus_exp(real g, real) { return -expm1(g); }
 __device__ __forceinline__ real reciprocal(real v) { return 1.0 / v; }
 #else
-// exp(g) to about one unit: 2^(g log2 e) with the product's rounding error, and the constant's, put back to first order.  Where that
-// would meet an infinity (beyond e^87) the plain power is left as it is: 0, infinity, NaN, or off by 2^-18 of a value that small or large.
-__device__ __forceinline__ float exp_real(float g) {
-    const float t = g * 1.44269504f, low = fmaf(g, 1.44269504f, -t), r = __builtin_amdgcn_exp2f(t);
-    const float fine = fmaf(r, fmaf(g, 1.925963033e-8f, low) * 0.693147181f, r);
-    return fabsf(g) < 87.0f ? fine : r;
-}
+// exp(g) as a power of two: off by |g| / 2 + 1 units of 2^-24 of itself, so by more than a few units only where it is below e^-8.  (Putting the
+// product's rounding error back took four more instructions of the about twenty that an element has.)
+__device__ __forceinline__ float exp_real(float g) { return __builtin_amdgcn_exp2f(g * 1.44269504f); }
 // 1 - exp(g) without the loss of its leading digits: near 0 by its series (the first term left out is below 2^-25 of it).
 __device__ __forceinline__ float one_minus_exp(float g, float e) {
-    const float s = g * (1.0f + g * (1.0f / 2) * (1.0f + g * (1.0f / 3) * (1.0f + g * (1.0f / 4) * (1.0f + g * (1.0f / 5) *
-                    (1.0f + g * (1.0f / 6) * (1.0f + g * (1.0f / 7)))))));
-    return fabsf(g) < 0.35f ? -s : 1.0f - e;
+    float s = fmaf(g, 1.0f / 5040, 1.0f / 720);
+    s = fmaf(g, s, 1.0f / 120);
+    s = fmaf(g, s, 1.0f / 24);
+    s = fmaf(g, s, 1.0f / 6);
+    s = fmaf(g, s, 0.5f);
+    s = -fmaf(g * g, s, g);
+    return fabsf(g) < 0.35f ? s : 1.0f - e;
 }
-// 1 / v for v in [1, 2]: the hardware's approximation and one step of Newton's.
-__device__ __forceinline__ float reciprocal(float v) {
-    const float r = __builtin_amdgcn_rcpf(v);
-    return fmaf(r, fmaf(-v, r, 1.0f), r);
-}
+__device__ __forceinline__ float reciprocal(float v) { return __builtin_amdgcn_rcpf(v); }  // to one unit
 #endif
 
-__device__ __forceinline__ Gate gate_of(int form, real g) {
+template <int Form> __device__ __forceinline__ Gate gate_of(real g) {
     Gate r;
-    if (form == TG_GATE_VALUE) {
+    if (Form == TG_GATE_VALUE) {
         r.a = g;
         r.rest = (real)1 - g;
         r.slope = (real)1;
-    } else if (form == TG_GATE_LOG) {
+    } else if (Form == TG_GATE_LOG) {
         r.a = exp_real(g);
         r.rest = one_minus_exp(g, r.a);
         r.slope = r.a;
     } else {
+        // from exp(-|g|), so that neither 1 - a near a = 1 nor a near 0 loses digits, and infinite logits are 0 and 1
         const real e = exp_real(-fabs(g)), big = reciprocal((real)1 + e), small = e * big;
         r.a = g >= 0 ? big : small;
         r.rest = g >= 0 ? small : big;
         r.slope = big * small;
     }
     return r;
+}
+__device__ __forceinline__ Gate gate_of(int form, real g) {
+    return form == TG_GATE_VALUE ? gate_of<TG_GATE_VALUE>(g) : form == TG_GATE_LOG ? gate_of<TG_GATE_LOG>(g) : gate_of<TG_GATE_LOGIT>(g);
 }
 
 struct Shape {

@@ -2,7 +2,7 @@
 //
 // e_t = a_{t+1} l_{t+1} is what reaches h_t from behind: l_t = dh_t + e_t, e_{t-1} = a_t l_t, a chain of maps like the forward one, against
 // the order.  The states h_{t-1} that the gates' gradients need are not read but computed again, from the float32 states that the
-// forward call kept every chunk_rows rows: x has to be read where the input is (1 - a) x or not, in the place of h, and h comes
+// forward call kept for every chunk: x has to be read where the input is (1 - a) x or not, in the place of h, and h comes
 // without having been rounded.
 #include "tg_recurrence_scan.hpp"
 
@@ -10,77 +10,58 @@
 namespace tg {
 
 template <class T, int V, bool Shared, int K, int Threads>
-__global__ __launch_bounds__(Threads) void recurrence_backward_kernel(Split m, Chain c, const T *__restrict__ inputs, const void *__restrict__ gates,
+__global__ __launch_bounds__(Threads) void recurrence_backward_kernel(Split m, const int32_t *__restrict__ first_sequence,
+                                                                      const float *__restrict__ starts, const T *__restrict__ inputs, const void *__restrict__ gates,
                                                                       const float *__restrict__ initial, const int32_t *__restrict__ offsets,
                                                                       const float *__restrict__ kept, const T *__restrict__ grad_states,
                                                                       const float *__restrict__ grad_final, T *__restrict__ grad_inputs,
                                                                       void *__restrict__ grad_gates, float *__restrict__ grad_initial,
                                                                       float *__restrict__ partial) {
     constexpr int GV = Shared ? 1 : V;
-    extern __shared__ int32_t table[];
+    extern __shared__ uint32_t table[];
     __shared__ Joint<V, Threads> joint;
-    __shared__ uint32_t ticket;
-    int64_t order, tile, channel, gate;
+    int64_t channel, gate;
     int part;
-    numbered(m, c, &ticket, order, tile);
-    const int64_t chunk = m.chunks - 1 - order;
+    const int64_t chunk = blockIdx.x / (uint32_t)m.tiles, tile = blockIdx.x % (uint32_t)m.tiles;
     const Place p = place_of<Threads>(m);
     const int places = (Threads >> m.lanes_log2) * K, at = p.turn * K;
     const int64_t start = chunk * m.chunk_rows;
     const int there = (int)min(m.chunk_rows, m.rows - start);
-    const int n = max(0, min(there - at, K)), last = max(n - 1, 0);
+    const int n = max(0, min(there - at, K));
     const bool valid = column_of<V, Shared>(m, (tile << m.lanes_log2) + p.lane, channel, gate, part);
-    if (!valid) channel = gate = 0;
-    const int64_t place = start + (n > 0 ? at : 0), row = m.reverse ? m.rows - 1 - place : place, step = m.reverse ? -1 : 1;
-    const int64_t pitch = m.channels * step;
+    const Walk w = walk_of<K, Threads>(m, start, p.turn, n);
+    const Column cx = column(m.channels, channel), cg = column(m.gates, gate);
 
     Pack<T, V> x[K], dh[K];
     float a[K][GV], rest[K][GV];
-    {
-        const T *from = inputs + row * m.channels + channel;
-#pragma unroll
-        for (int k = 0; k < K; k++) x[k] = load_pack<V>(from + pitch * min(k, last));
-    }
-    load_gates<T, K, GV>(m, gates, row, step, gate, last, a);
+    each_row<K>(w, cx, inputs, [&](int k, const T *from) { x[k] = load_pack<V>(from); });
+    read_gates<T, K, GV>(m, gates, w, cg, a);
     if (grad_states) {
-        const T *from = grad_states + row * m.channels + channel;
-#pragma unroll
-        for (int k = 0; k < K; k++) dh[k] = load_pack<V>(from + pitch * min(k, last));
+        each_row<K>(w, cx, grad_states, [&](int k, const T *from) { dh[k] = load_pack<V>(from); });
     } else {
 #pragma unroll
         for (int k = 0; k < K; k++)
 #pragma unroll
             for (int v = 0; v < V; v++) dh[k].v[v] = (T)0.0f;
     }
-    float known[V];
+    float h[V], e[V];  // the state in front of the chunk, what comes from behind it
 #pragma unroll
-    for (int v = 0; v < V; v++) known[v] = m.chained ? kept[chunk * m.channels + channel + v] : 0.0f;
+    for (int v = 0; v < V; v++) {
+        h[v] = m.chained ? kept[chunk * m.channels + channel + v] : 0.0f;
+        e[v] = m.chained ? starts[chunk * m.channels + channel + v] : 0.0f;
+    }
 
     uint32_t firsts = 0, lasts = 0, outside = 0;
-    bool chunk_closed = false;
-    int32_t *seq = table;
-    if (!inside_one_sequence(m, c, offsets, chunk)) {
-        uint8_t *flags = (uint8_t *)(table + places);
-        chunk_table<Threads>(m, c, offsets, chunk, places, seq, flags);
+    if (!inside_one_sequence(m, first_sequence, offsets, chunk)) {
+        chunk_table<Threads>(m, first_sequence, offsets, chunk, places, table);
         __syncthreads();
-        for (int k = 0; k < n; k++) {
-            const uint32_t f = flags[at + k];
-            firsts |= (f & kFirst ? 1u : 0u) << k;
-            lasts |= (f & kLast ? 1u : 0u) << k;
-            outside |= (f & kOutside ? 1u : 0u) << k;
-        }
-        chunk_closed = (flags[there - 1] & kLast) != 0;
+        const Marks marks = marks_of(table + at, n);
+        firsts = marks.firsts;
+        lasts = marks.lasts;
+        outside = marks.outside;
     }
 
-#pragma unroll
-    for (int k = 0; k < K; k++) {
-#pragma unroll
-        for (int v = 0; v < GV; v++) {
-            const Gate g = gate_of(m.gate_form, a[k][v]);
-            a[k][v] = g.a;
-            rest[k][v] = g.rest;
-        }
-    }
+    compute_gates<K, GV>(m, a, rest);
     if (n < K || outside) {
 #pragma unroll
         for (int k = 0; k < K; k++) {
@@ -97,96 +78,155 @@ __global__ __launch_bounds__(Threads) void recurrence_backward_kernel(Split m, C
         }
     }
     const auto begin = [&](int k, int v) {
-        return initial && !(outside >> k & 1) && valid ? initial[seq[at + k] * m.channels + channel + v] : 0.0f;
+        return initial && !(outside >> k & 1) && valid ? initial[sequence_of(table[at + k]) * m.channels + channel + v] : 0.0f;
     };
     const auto end = [&](int k, int v) {
-        return grad_final && !(outside >> k & 1) && valid ? grad_final[seq[at + k] * m.channels + channel + v] : 0.0f;
+        return grad_final && !(outside >> k & 1) && valid ? grad_final[sequence_of(table[at + k]) * m.channels + channel + v] : 0.0f;
     };
     const auto input = [&](int k, int v) { return m.complement ? rest[k][Shared ? 0 : v] * x[k][v] : x[k][v]; };
+
+    const bool marked = __any((firsts | lasts) != 0);
 
     // the states again
     Map<V> map = unit_map<V>();
     map.closed = firsts != 0;
+    const auto map_of_states = [&](auto with_marks) {
 #pragma unroll
-    for (int k = 0; k < K; k++)
+        for (int k = 0; k < K; k++)
 #pragma unroll
-        for (int v = 0; v < V; v++) {
-            if (firsts >> k & 1) map.u[v] = begin(k, v);
-            map.u[v] = fmaf(a[k][Shared ? 0 : v], map.u[v], input(k, v));
-            map.a[v] *= a[k][Shared ? 0 : v];
-        }
-    float h[V], before[K][V];
-    join<V, Threads, false>(m, c, joint, p, tile, chunk, map, false, false, known, h);
+            for (int v = 0; v < V; v++) {
+                if (with_marks.value && (firsts >> k & 1)) map.u[v] = begin(k, v);
+                map.u[v] = fmaf(a[k][Shared ? 0 : v], map.u[v], input(k, v));
+                map.a[v] *= a[k][Shared ? 0 : v];
+            }
+    };
+    if (marked) map_of_states(std::true_type());
+    else map_of_states(std::false_type());
+    float before[K][V];
+    join<V, Threads, false>(m, joint, p, map, h);
+    const auto walk_states = [&](auto with_marks) {
 #pragma unroll
-    for (int k = 0; k < K; k++)
+        for (int k = 0; k < K; k++)
 #pragma unroll
-        for (int v = 0; v < V; v++) {
-            if (firsts >> k & 1) h[v] = begin(k, v);
-            before[k][v] = h[v];
-            h[v] = fmaf(a[k][Shared ? 0 : v], h[v], input(k, v));
-        }
+            for (int v = 0; v < V; v++) {
+                if (with_marks.value && (firsts >> k & 1)) h[v] = begin(k, v);
+                before[k][v] = h[v];
+                h[v] = fmaf(a[k][Shared ? 0 : v], h[v], input(k, v));
+            }
+    };
+    if (marked) walk_states(std::true_type());
+    else walk_states(std::false_type());
 
     // what reaches the last of the thread's rows from behind
     map = unit_map<V>();
     map.closed = lasts != 0;
+    const auto map_of_gradients = [&](auto with_marks) {
 #pragma unroll
-    for (int k = K - 1; k >= 0; k--)
+        for (int k = K - 1; k >= 0; k--)
 #pragma unroll
-        for (int v = 0; v < V; v++) {
-            if (lasts >> k & 1) map.u[v] = end(k, v);
-            map.u[v] = a[k][Shared ? 0 : v] * (map.u[v] + dh[k][v]);
-            map.a[v] *= a[k][Shared ? 0 : v];
-        }
+            for (int v = 0; v < V; v++) {
+                if (with_marks.value && (lasts >> k & 1)) map.u[v] = end(k, v);
+                map.u[v] = a[k][Shared ? 0 : v] * (map.u[v] + dh[k][v]);
+                map.a[v] *= a[k][Shared ? 0 : v];
+            }
+    };
+    if (marked) map_of_gradients(std::true_type());
+    else map_of_gradients(std::false_type());
     __syncthreads();
-    float e[V];
-    join<V, Threads, true>(m, c, joint, p, tile, order, map, chunk_closed, m.chained, nullptr, e);
+    join<V, Threads, true>(m, joint, p, map, e);
 
-    float q[K];
-    const int64_t gate_pitch = m.gates * step;
-#pragma unroll
-    for (int k = K - 1; k >= 0; k--) {
-        float dx[V], dg[V];
-        q[k] = 0.0f;
+    float q[K];  // of a shared gate: the sum over the lane's channels
+    // dx of row k, and da in its place in before[]
+    const auto gradients = [&](auto with_marks, int k, float (&dx)[V]) {
 #pragma unroll
         for (int v = 0; v < V; v++) {
-            const float ak = a[k][Shared ? 0 : v], rk = rest[k][Shared ? 0 : v];
-            if (lasts >> k & 1) e[v] = end(k, v);
+            if (with_marks.value && (lasts >> k & 1)) e[v] = end(k, v);
             const float l = e[v] + dh[k][v];
-            dx[v] = m.complement ? rk * l : l;
-            const float da = l * (m.complement ? before[k][v] - x[k][v] : before[k][v]);
-            e[v] = ak * l;
-            if (Shared) q[k] += da;
-            else dg[v] = m.gate_form == TG_GATE_VALUE ? da : m.gate_form == TG_GATE_LOG ? da * ak : da * (ak * rk);
+            dx[v] = m.complement ? rest[k][Shared ? 0 : v] * l : l;
+            before[k][v] = l * (m.complement ? before[k][v] - x[k][v] : before[k][v]);
+            e[v] = a[k][Shared ? 0 : v] * l;
         }
-        if (valid && k < n) {
-            if (grad_inputs) store_pack<V>(grad_inputs + row * m.channels + channel + pitch * k, dx);
+        if (Shared) {
+            q[k] = before[k][0];
+#pragma unroll
+            for (int v = 1; v < V; v++) q[k] += before[k][v];
+        }
+    };
+    const auto slope = [&](int k, int v) {
+        return m.gate_form == TG_GATE_VALUE ? 1.0f : m.gate_form == TG_GATE_LOG ? a[k][v] : a[k][v] * rest[k][v];
+    };
+    const auto gate_gradients = [&](int k, float (&dg)[V]) {
+#pragma unroll
+        for (int v = 0; v < V; v++) dg[v] = before[k][v] * slope(k, Shared ? 0 : v);
+    };
+    const bool wide = sizeof(T) == 4 || m.wide_gates;
+    if (w.whole && !marked) {
+        const Walk back = against<K>(w);
+        each_row<K>(back, cx, grad_inputs ? grad_inputs : const_cast<T *>(inputs), [&](int i, T *to) {
+            float dx[V];
+            gradients(std::false_type(), K - 1 - i, dx);
+            if (grad_inputs && valid) store_pack<V>(to, dx);
+        });
+        if (!Shared && grad_gates && valid) {
+            if (wide)
+                each_row<K>(w, cg, (float *)grad_gates, [&](int k, float *to) {
+                    float dg[V];
+                    gate_gradients(k, dg);
+                    store_pack<V>(to, dg);
+                });
+            else
+                each_row<K>(w, cg, (T *)grad_gates, [&](int k, T *to) {
+                    float dg[V];
+                    gate_gradients(k, dg);
+                    store_pack<V>(to, dg);
+                });
+        }
+    } else {
+#pragma unroll
+        for (int k = K - 1; k >= 0; k--) {
+            float dx[V], dg[V];
+            gradients(std::true_type(), k, dx);
+            if (!valid || k >= n) continue;
+            const int64_t row = w.row + k * w.step;
+            if (grad_inputs) store_pack<V>(grad_inputs + row * m.channels + channel, dx);
             if (!Shared && grad_gates) {
-                const int64_t to = row * m.gates + gate + gate_pitch * k;
-                if (sizeof(T) == 4 || m.wide_gates) store_pack<V>((float *)grad_gates + to, dg);
-                else store_pack<V>((T *)grad_gates + to, dg);
+                gate_gradients(k, dg);
+                if (wide) store_pack<V>((float *)grad_gates + row * m.gates + gate, dg);
+                else store_pack<V>((T *)grad_gates + row * m.gates + gate, dg);
             }
             if (grad_initial && ((firsts & ~outside) >> k & 1)) {
 #pragma unroll
-                for (int v = 0; v < V; v++) grad_initial[seq[at + k] * m.channels + channel + v] = e[v];
+                for (int v = 0; v < V; v++) grad_initial[sequence_of(table[at + k]) * m.channels + channel + v] = e[v];
             }
         }
     }
     if (!Shared || !grad_gates) return;
-    const int gate_lanes = 1 << m.gate_lanes_log2, lane = threadIdx.x & (gate_lanes - 1);
+    const auto store_gate = [&](int k, float sum, float s) {
+        const int64_t to = (w.row + k * w.step) * m.gates + gate;
+        if (m.parts > 1) partial[part * m.rows * m.gates + to] = sum;
+        else if (wide) ((float *)grad_gates)[to] = sum * s;
+        else ((T *)grad_gates)[to] = (T)(sum * s);
+    };
+    if (!valid) {
 #pragma unroll
-    for (int k = 0; k < K; k++) {
-        float sum = valid && !(outside >> k & 1) ? q[k] : 0.0f;
-        for (int d = gate_lanes >> 1; d > 0; d >>= 1) sum += __shfl_xor(sum, d);
-        if (lane == 0 && valid && k < n) {
-            const int64_t to = row * m.gates + gate + gate_pitch * k;
-            if (m.parts > 1) {
-                partial[part * m.rows * m.gates + to] = sum;
-                continue;
-            }
-            const float ak = a[k][0];
-            sum = m.gate_form == TG_GATE_VALUE ? sum : m.gate_form == TG_GATE_LOG ? sum * ak : sum * (ak * rest[k][0]);
-            if (sizeof(T) == 4 || m.wide_gates) ((float *)grad_gates)[to] = sum;
-            else ((T *)grad_gates)[to] = (T)sum;
+        for (int k = 0; k < K; k++) q[k] = 0.0f;
+    }
+    const bool any_valid = __builtin_amdgcn_readfirstlane(valid ? 1 : 0) != 0;
+    if (m.gate_lanes_log2 == 6) {
+        // the rows' sums over the wave: halves of the rows go to halves of the lanes, so the first steps sum several rows at once
+        const float sum = sum_rows<K>(q);
+        const int k = row_of_sum<K>(threadIdx.x & (kWave - 1));
+        float s = 1.0f;
+#pragma unroll
+        for (int i = 0; i < K; i++) s = i == k ? slope(i, 0) : s;
+        if (sum_is_here<K>(threadIdx.x & (kWave - 1)) && k < n && any_valid) store_gate(k, sum, s);
+    } else {
+        const int gate_lanes = 1 << m.gate_lanes_log2, lane = threadIdx.x & (gate_lanes - 1);
+#pragma unroll
+        for (int k = 0; k < K; k++) {
+            float sum = q[k];
+            for (int d = gate_lanes >> 1; d > 0; d >>= 1) sum += __shfl_xor(sum, d);
+            if (lane == 0 && valid && k < n) store_gate(k, sum, slope(k, 0));
         }
     }
 }
@@ -207,23 +247,21 @@ __global__ __launch_bounds__(256) void recurrence_gate_sums_kernel(Split m, cons
     }
 }
 
-template <class T, int V, bool Shared>
-int launch_backward(const tg_recurrence &r, const Split &m, const Chain &c, float *partial, unsigned blocks, hipStream_t stream) {
-    constexpr int K = kBackwardRows, Threads = kBackwardThreads;
-    const size_t lds = (size_t)(Threads >> m.lanes_log2) * K * 5;
-    TG_LAUNCH_AS("recurrence_backward", (recurrence_backward_kernel<T, V, Shared, K, Threads>), dim3(blocks), dim3(Threads), lds, stream, m, c,
-                 (const T *)r.inputs, r.gates, r.initial, r.offsets, (const float *)r.kept, (const T *)r.grad_states, r.grad_final,
-                 (T *)r.grad_inputs, r.grad_gates, r.grad_initial, partial);
-    if (Shared && r.grad_gates && m.parts > 1) {
-        const unsigned sum_blocks = (unsigned)std::min<int64_t>(ceil_div64(m.rows * m.gates, 256), 4096);
-        TG_LAUNCH_AS("recurrence_gate_sums", (recurrence_gate_sums_kernel<T>), dim3(sum_blocks), dim3(256), 0, stream, m, r.gates, partial, r.grad_gates);
-    }
-    return check_launch("tg_linear_recurrence_backward");
-}
-
-int launch_backward(const tg_recurrence &r, const Split &m, const Chain &c, float *partial, int vector, unsigned blocks, hipStream_t stream) {
+int launch_backward(const tg_recurrence &r, const Split &m, const int32_t *first_sequence, const float *starts, float *partial, int vector,
+                    unsigned blocks, hipStream_t stream) {
     return by_layout(r.type, vector, m.shared, [&](auto t, auto v, auto shared) {
-        return launch_backward<decltype(t), decltype(v)::value, decltype(shared)::value>(r, m, c, partial, blocks, stream);
+        using T = decltype(t);
+        constexpr int K = kBackwardRows, Threads = kBackwardThreads;
+        constexpr bool Shared = decltype(shared)::value;
+        TG_LAUNCH_AS("recurrence_backward", (recurrence_backward_kernel<T, decltype(v)::value, Shared, K, Threads>), dim3(blocks), dim3(Threads),
+                     table_bytes(m, Threads * K), stream, m, first_sequence, starts, (const T *)r.inputs, r.gates, r.initial, r.offsets,
+                     (const float *)r.kept, (const T *)r.grad_states, r.grad_final, (T *)r.grad_inputs, r.grad_gates, r.grad_initial, partial);
+        if (Shared && r.grad_gates && m.parts > 1) {
+            const unsigned sum_blocks = (unsigned)std::min<int64_t>(ceil_div64(m.rows * m.gates, 256), 4096);
+            TG_LAUNCH_AS("recurrence_gate_sums", (recurrence_gate_sums_kernel<T>), dim3(sum_blocks), dim3(256), 0, stream, m, r.gates, partial,
+                         r.grad_gates);
+        }
+        return check_launch("tg_linear_recurrence_backward");
     });
 }
 

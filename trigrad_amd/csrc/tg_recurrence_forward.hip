@@ -4,67 +4,54 @@
 #ifndef TG_DOUBLE_PRECISION
 namespace tg {
 
-// What a thread's rows are: places [at, at + n) of the chunk, by the table's flags.
-struct Marks {
-    uint32_t firsts, lasts, outside;
-};
-
 template <class T, int V, bool Shared, int K, int Threads>
-__global__ __launch_bounds__(Threads, 4) void recurrence_forward_kernel(Split m, Chain c, const T *__restrict__ inputs, const void *__restrict__ gates,
+__global__ __launch_bounds__(Threads, 4) void recurrence_forward_kernel(Split m, const int32_t *__restrict__ first_sequence,
+                                                                     const float *__restrict__ starts, const T *__restrict__ inputs, const void *__restrict__ gates,
                                                                      const float *__restrict__ initial, const int32_t *__restrict__ offsets,
-                                                                     T *__restrict__ states, float *__restrict__ final, float *__restrict__ kept) {
+                                                                     T *__restrict__ states, float *__restrict__ final) {
     constexpr int GV = Shared ? 1 : V;
-    extern __shared__ int32_t table[];
+    extern __shared__ uint32_t table[];
     __shared__ Joint<V, Threads> joint;
-    __shared__ uint32_t ticket;
-    int64_t chunk, tile, channel, gate;
+    int64_t channel, gate;
     int part;
-    numbered(m, c, &ticket, chunk, tile);
+    const int64_t chunk = blockIdx.x / (uint32_t)m.tiles, tile = blockIdx.x % (uint32_t)m.tiles;
     const Place p = place_of<Threads>(m);
     const int places = (Threads >> m.lanes_log2) * K, at = p.turn * K;
     const int64_t start = chunk * m.chunk_rows;
-    const int n = (int)max((int64_t)0, min(min(m.chunk_rows, m.rows - start) - at, (int64_t)K)), last = max(n - 1, 0);
+    const int n = (int)max((int64_t)0, min(min(m.chunk_rows, m.rows - start) - at, (int64_t)K));
     const bool valid = column_of<V, Shared>(m, (tile << m.lanes_log2) + p.lane, channel, gate, part);
-    if (!valid) channel = gate = 0;
-    const int64_t place = start + (n > 0 ? at : 0), row = m.reverse ? m.rows - 1 - place : place, step = m.reverse ? -1 : 1;
+    const Walk w = walk_of<K, Threads>(m, start, p.turn, n);
+    const Column cx = column(m.channels, channel), cg = column(m.gates, gate);
 
     Pack<T, V> x[K];
-    {
-        const T *from = inputs + row * m.channels + channel;
-        const int64_t pitch = m.channels * step;
-#pragma unroll
-        for (int k = 0; k < K; k++) x[k] = load_pack<V>(from + pitch * min(k, last));
-    }
+    each_row<K>(w, cx, inputs, [&](int k, const T *from) { x[k] = load_pack<V>(from); });
     float a[K][GV], u[K][V];
-    load_gates<T, K, GV>(m, gates, row, step, gate, last, a);
+    read_gates<T, K, GV>(m, gates, w, cg, a);
 
     uint32_t firsts = 0, lasts = 0, outside = 0;
-    bool chunk_closed = false;
-    int32_t *seq = table;
-    if (!inside_one_sequence(m, c, offsets, chunk)) {
-        uint8_t *flags = (uint8_t *)(table + places);
-        chunk_table<Threads>(m, c, offsets, chunk, places, seq, flags);
+    if (!inside_one_sequence(m, first_sequence, offsets, chunk)) {
+        chunk_table<Threads>(m, first_sequence, offsets, chunk, places, table);
         __syncthreads();
-        for (int k = 0; k < n; k++) {
-            const uint32_t f = flags[at + k];
-            firsts |= (f & kFirst ? 1u : 0u) << k;
-            lasts |= (f & kLast ? 1u : 0u) << k;
-            outside |= (f & kOutside ? 1u : 0u) << k;
-        }
-        chunk_closed = (flags[0] & kFirst) != 0;
+        const Marks marks = marks_of(table + at, n);
+        firsts = marks.firsts;
+        lasts = marks.lasts;
+        outside = marks.outside;
     }
 
+    {
+        float rest[K][GV];
+        compute_gates<K, GV>(m, a, rest);
+        if (m.complement) {
 #pragma unroll
-    for (int k = 0; k < K; k++) {
-        float rest[GV];
+            for (int k = 0; k < K; k++)
 #pragma unroll
-        for (int v = 0; v < GV; v++) {
-            const Gate g = gate_of(m.gate_form, a[k][v]);
-            a[k][v] = g.a;
-            rest[v] = g.rest;
+                for (int v = 0; v < V; v++) u[k][v] = rest[k][Shared ? 0 : v] * x[k][v];
+        } else {
+#pragma unroll
+            for (int k = 0; k < K; k++)
+#pragma unroll
+                for (int v = 0; v < V; v++) u[k][v] = x[k][v];
         }
-#pragma unroll
-        for (int v = 0; v < V; v++) u[k][v] = m.complement ? rest[Shared ? 0 : v] * x[k][v] : x[k][v];
     }
     if (n < K || outside) {
 #pragma unroll
@@ -77,7 +64,7 @@ __global__ __launch_bounds__(Threads, 4) void recurrence_forward_kernel(Split m,
         }
     }
     const auto begin = [&](int k, int v) {
-        return initial && !(outside >> k & 1) && valid ? initial[seq[at + k] * m.channels + channel + v] : 0.0f;
+        return initial && !(outside >> k & 1) && valid ? initial[sequence_of(table[at + k]) * m.channels + channel + v] : 0.0f;
     };
 
     Map<V> map = unit_map<V>();
@@ -100,22 +87,17 @@ __global__ __launch_bounds__(Threads, 4) void recurrence_forward_kernel(Split m,
             }
     }
     float h[V];
-    join<V, Threads, false>(m, c, joint, p, tile, chunk, map, chunk_closed, m.chained, nullptr, h);
+#pragma unroll
+    for (int v = 0; v < V; v++) h[v] = m.chained ? starts[chunk * m.channels + channel + v] : 0.0f;
+    join<V, Threads, false>(m, joint, p, map, h);
     if (!valid || n == 0) return;
-    if (kept && at % m.block_rows == 0) {
-#pragma unroll
-        for (int v = 0; v < V; v++) kept[(start + at) / m.block_rows * m.channels + channel + v] = h[v];
-    }
-    T *to = states ? states + row * m.channels + channel : nullptr;
-    const int64_t pitch = m.channels * step;
-    if (n == K && !(firsts | lasts)) {
-        if (!to) return;
-#pragma unroll
-        for (int k = 0; k < K; k++) {
+    if (w.whole && !(firsts | lasts)) {
+        if (!states) return;
+        each_row<K>(w, cx, states, [&](int k, T *to) {
 #pragma unroll
             for (int v = 0; v < V; v++) h[v] = fmaf(a[k][Shared ? 0 : v], h[v], u[k][v]);
-            store_pack<V>(to + pitch * k, h);
-        }
+            store_pack<V>(to, h);
+        });
     } else {
 #pragma unroll
         for (int k = 0; k < K; k++) {
@@ -124,22 +106,157 @@ __global__ __launch_bounds__(Threads, 4) void recurrence_forward_kernel(Split m,
                 if (firsts >> k & 1) h[v] = begin(k, v);
                 h[v] = fmaf(a[k][Shared ? 0 : v], h[v], u[k][v]);
             }
-            if (to && k < n) store_pack<V>(to + pitch * k, h);
+            if (states && k < n) store_pack<V>(states + (w.row + k * w.step) * m.channels + channel, h);
             if ((lasts & ~outside) >> k & 1) {
 #pragma unroll
-                for (int v = 0; v < V; v++) final[seq[at + k] * m.channels + channel + v] = h[v];
+                for (int v = 0; v < V; v++) final[sequence_of(table[at + k]) * m.channels + channel + v] = h[v];
             }
         }
     }
 }
 
-// In front of a chained or packed call: words that say "not there yet", the ticket, the sequences that each chunk's rows are searched
-// between, and the final states (or, backward, the initial states' gradients) of sequences without rows.
-__global__ __launch_bounds__(256) void recurrence_prepare_kernel(Split m, Chain c, uint64_t *words, int64_t n_words, const int32_t *__restrict__ offsets,
+// The map of each chunk, by a first look at what it needs: inputs and gates, or, Backward, gradients of the states and gates.
+template <class T, int V, bool Shared, bool Backward>
+__global__ __launch_bounds__(kMapThreads) void recurrence_maps_kernel(Split m, const int32_t *__restrict__ first_sequence, const T *__restrict__ inputs,
+                                                                      const void *__restrict__ gates, const float *__restrict__ ends,
+                                                                      const int32_t *__restrict__ offsets, MapWords *__restrict__ maps) {
+    constexpr int GV = Shared ? 1 : V, K = kMapRows, Threads = kMapThreads, Batches = kChunk / (Threads * K);
+    extern __shared__ uint32_t table[];
+    __shared__ Joint<V, Threads> joint;
+    int64_t channel, gate;
+    int part;
+    const int64_t chunk = blockIdx.x / (uint32_t)m.tiles, tile = blockIdx.x % (uint32_t)m.tiles;
+    const Place p = place_of<Threads>(m);
+    const int places = (Threads >> m.lanes_log2) * K * Batches;
+    const int64_t start = chunk * m.chunk_rows;
+    const bool valid = column_of<V, Shared>(m, (tile << m.lanes_log2) + p.lane, channel, gate, part);
+    const Column cx = column(m.channels, channel), cg = column(m.gates, gate);
+    const bool marked = !inside_one_sequence(m, first_sequence, offsets, chunk);
+    if (marked) {
+        chunk_table<Threads>(m, first_sequence, offsets, chunk, places, table);
+        __syncthreads();
+    }
+    Map<V> map = unit_map<V>();
+    for (int batch = 0; batch < Batches; batch++) {
+        const int turn = p.turn * Batches + (Backward ? Batches - 1 - batch : batch), at = turn * K;
+        const int n = (int)max((int64_t)0, min(min(m.chunk_rows, m.rows - start) - at, (int64_t)K));
+        const Walk w = walk_of<K, Threads>(m, start, turn, n, Batches);
+        Pack<T, V> x[K];
+        float a[K][GV], rest[K][GV];
+        if (inputs) {
+            each_row<K>(w, cx, inputs, [&](int k, const T *from) { x[k] = load_pack<V>(from); });
+        } else {
+#pragma unroll
+            for (int k = 0; k < K; k++)
+#pragma unroll
+                for (int v = 0; v < V; v++) x[k].v[v] = (T)0.0f;
+        }
+        read_gates<T, K, GV>(m, gates, w, cg, a);
+        compute_gates<K, GV>(m, a, rest);
+        uint32_t marks = 0, outside = 0;
+        if (marked) {
+            const Marks found = marks_of(table + at, n);
+            marks = Backward ? found.lasts : found.firsts;
+            outside = found.outside;
+        }
+        const auto step = [&](int k, int v) {
+            if (Backward) {
+                map.u[v] = a[k][Shared ? 0 : v] * (map.u[v] + x[k][v]);
+            } else {
+                const float u = m.complement ? rest[k][Shared ? 0 : v] * x[k][v] : x[k][v];
+                map.u[v] = fmaf(a[k][Shared ? 0 : v], map.u[v], u);
+            }
+            map.a[v] *= a[k][Shared ? 0 : v];
+        };
+        if (w.whole && !__any(marks != 0)) {
+#pragma unroll
+            for (int i = 0; i < K; i++)
+#pragma unroll
+                for (int v = 0; v < V; v++) step(Backward ? K - 1 - i : i, v);
+        } else {
+#pragma unroll
+            for (int i = 0; i < K; i++) {
+                const int k = Backward ? K - 1 - i : i;
+                const bool mark = (marks >> k & 1) != 0, out = (outside >> k & 1) != 0;
+                if (k >= n) continue;
+#pragma unroll
+                for (int v = 0; v < V; v++) {
+                    if (mark) map.u[v] = ends && !out && valid ? ends[sequence_of(table[at + k]) * m.channels + channel + v] : 0.0f;
+                    if (out) map.a[v] = map.u[v] = 0.0f;
+                    else step(k, v);
+                }
+                map.closed = map.closed || mark;
+            }
+        }
+    }
+    gather<V, Threads, Backward>(m, joint, p, map);
+    if (!p.leads || !valid) return;
+    Map<V> total = unit_map<V>();
+    for (int i = 0; i < p.entries; i++) {
+        Map<V> next = joint.at(Backward ? p.entries - 1 - i : i, 1 << m.lanes_log2, p.lane);
+        compose(next, total);
+        total = next;
+    }
+#pragma unroll
+    for (int v = 0; v < V; v++) {
+        MapWords words;
+        words.a = total.closed ? __uint_as_float(kClosedMap) : total.a[v] != total.a[v] ? __uint_as_float(0x7fc00000u) : total.a[v];
+        words.u = total.u[v];
+        maps[chunk * m.channels + channel + v] = words;
+    }
+}
+
+// The states that the chunks start from.  A wave goes over a run of chunks for 64 channels, twice: for the run's map, and, once the runs before
+// are known, from their state.
+constexpr int kStartWaves = 16, kStartAhead = 8;
+__global__ __launch_bounds__(kStartWaves * kWave) void recurrence_starts_kernel(int64_t chunks, int64_t channels, bool backward,
+                                                                                const MapWords *__restrict__ maps, float *__restrict__ starts) {
+    __shared__ Joint<1, kStartWaves * kWave> joint;
+    const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x >> 6;
+    const int64_t channel = (int64_t)blockIdx.x * kWave + lane, run = (chunks + kStartWaves - 1) / kStartWaves;
+    const int64_t begin = min(wave * run, chunks), end = min(begin + run, chunks);
+    const bool valid = channel < channels;
+    const auto over = [&](auto &&call) {
+        for (int64_t i = begin; i < end; i += kStartAhead) {
+            MapWords next[kStartAhead];
+#pragma unroll
+            for (int k = 0; k < kStartAhead; k++) {
+                const int64_t c = min(i + k, end - 1);
+                next[k] = maps[(backward ? chunks - 1 - c : c) * channels + (valid ? channel : 0)];
+            }
+#pragma unroll
+            for (int k = 0; k < kStartAhead; k++) {
+                Map<1> map;
+                map.a[0] = next[k].a;
+                map.u[0] = next[k].u;
+                map.closed = __float_as_uint(next[k].a) == kClosedMap;
+                if (map.closed) map.a[0] = 0.0f;
+                if (i + k < end) call(i + k, map);
+            }
+        }
+    };
+    Map<1> total = unit_map<1>();
+    over([&](int64_t, Map<1> map) {
+        compose(map, total);
+        total = map;
+    });
+    joint.a[threadIdx.x] = total.a[0];
+    joint.u[threadIdx.x] = total.u[0];
+    if (lane == 0) joint.closed[wave] = total.closed;
+    __syncthreads();
+    float h[1] = {0.0f};
+    for (int i = 0; i < wave; i++) step_over(h, joint.at(i, kWave, lane));
+    over([&](int64_t c, const Map<1> &map) {
+        if (valid) starts[(backward ? chunks - 1 - c : c) * channels + channel] = h[0];
+        step_over(h, map);
+    });
+}
+
+// In front of a call on packed sequences: those that each chunk's rows are searched between, and the final states (or, backward, the initial
+// states' gradients) of sequences without rows; the latter alone where no sequence has any.
+__global__ __launch_bounds__(256) void recurrence_prepare_kernel(Split m, int32_t *__restrict__ first_sequence, const int32_t *__restrict__ offsets,
                                                                  const float *__restrict__ from, float *__restrict__ to) {
     const int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x, all = (int64_t)gridDim.x * 256;
-    for (int64_t i = id; i < n_words; i += all) words[i] = ~(uint64_t)0;
-    if (id == 0 && m.chained) *c.ticket = 0;
     if (m.packed) {
         for (int64_t i = id; i < 2 * m.chunks; i += all) {
             const int64_t start = (i >> 1) * m.chunk_rows, place = (i & 1) ? min(start + m.chunk_rows, m.rows) - 1 : start;
@@ -149,7 +266,7 @@ __global__ __launch_bounds__(256) void recurrence_prepare_kernel(Split m, Chain 
                 const int32_t mid = lo + (hi - lo + 1) / 2;
                 if (offsets[mid] <= row) lo = mid; else hi = mid - 1;
             }
-            c.first_sequence[m.reverse ? i ^ 1 : i] = lo;
+            first_sequence[m.reverse ? i ^ 1 : i] = lo;
         }
     }
     if (to) {
@@ -160,26 +277,43 @@ __global__ __launch_bounds__(256) void recurrence_prepare_kernel(Split m, Chain 
     }
 }
 
-template <class T, int V, bool Shared>
-int launch_forward(const tg_recurrence &r, const Split &m, const Chain &c, unsigned blocks, hipStream_t stream) {
-    constexpr int K = kForwardRows, Threads = kForwardThreads;
-    const size_t lds = (size_t)(Threads >> m.lanes_log2) * K * 5;
-    TG_LAUNCH_AS("recurrence_forward", (recurrence_forward_kernel<T, V, Shared, K, Threads>), dim3(blocks), dim3(Threads), lds, stream, m, c,
-                 (const T *)r.inputs, r.gates, r.initial, r.offsets, (T *)r.states, r.final, (float *)r.kept);
-    return check_launch("tg_linear_recurrence_forward");
-}
-
-int launch_forward(const tg_recurrence &r, const Split &m, const Chain &c, int vector, unsigned blocks, hipStream_t stream) {
+int launch_forward(const tg_recurrence &r, const Split &m, const int32_t *first_sequence, const float *starts, int vector, unsigned blocks,
+                   hipStream_t stream) {
     return by_layout(r.type, vector, m.shared, [&](auto t, auto v, auto shared) {
-        return launch_forward<decltype(t), decltype(v)::value, decltype(shared)::value>(r, m, c, blocks, stream);
+        using T = decltype(t);
+        constexpr int K = kForwardRows, Threads = kForwardThreads;
+        TG_LAUNCH_AS("recurrence_forward", (recurrence_forward_kernel<T, decltype(v)::value, decltype(shared)::value, K, Threads>), dim3(blocks),
+                     dim3(Threads), table_bytes(m, Threads * K), stream, m, first_sequence, starts, (const T *)r.inputs, r.gates, r.initial, r.offsets,
+                     (T *)r.states, r.final);
+        return check_launch("tg_linear_recurrence_forward");
     });
 }
 
-int launch_prepare(const Split &m, const Chain &c, uint64_t *words, int64_t n_words, const int32_t *offsets, const float *from, float *to,
-                   hipStream_t stream) {
-    const int64_t most = std::max(std::max(n_words, 2 * m.chunks), to ? m.sequences * m.channels : 0);
+int launch_starts(const tg_recurrence &r, const Split &m, const int32_t *first_sequence, MapWords *maps, float *starts, int vector, bool backward,
+                  hipStream_t stream) {
+    const unsigned blocks = (unsigned)(m.chunks * m.tiles);
+    const int code = by_layout(r.type, vector, m.shared, [&](auto t, auto v, auto shared) {
+        using T = decltype(t);
+        constexpr int V = decltype(v)::value;
+        constexpr bool Shared = decltype(shared)::value;
+        if (backward)
+            TG_LAUNCH_AS("recurrence_maps_backward", (recurrence_maps_kernel<T, V, Shared, true>), dim3(blocks), dim3(kMapThreads), table_bytes(m, kChunk),
+                         stream, m, first_sequence, (const T *)r.grad_states, r.gates, r.grad_final, r.offsets, maps);
+        else
+            TG_LAUNCH_AS("recurrence_maps", (recurrence_maps_kernel<T, V, Shared, false>), dim3(blocks), dim3(kMapThreads), table_bytes(m, kChunk), stream,
+                         m, first_sequence, (const T *)r.inputs, r.gates, r.initial, r.offsets, maps);
+        return check_launch("tg_linear_recurrence");
+    });
+    if (code) return code;
+    TG_LAUNCH_AS("recurrence_starts", recurrence_starts_kernel, dim3((unsigned)ceil_div64(m.channels, kWave)), dim3(kStartWaves * kWave), 0, stream,
+                 m.chunks, m.channels, backward, maps, starts);
+    return check_launch("tg_linear_recurrence");
+}
+
+int launch_prepare(const Split &m, int32_t *first_sequence, const int32_t *offsets, const float *from, float *to, hipStream_t stream) {
+    const int64_t most = std::max(2 * m.chunks, to ? m.sequences * m.channels : 0);
     const unsigned blocks = (unsigned)std::min<int64_t>(std::max<int64_t>(ceil_div64(most, 1024), 1), 2048);
-    TG_LAUNCH_AS("recurrence_prepare", recurrence_prepare_kernel, dim3(blocks), dim3(256), 0, stream, m, c, words, n_words, offsets, from, to);
+    TG_LAUNCH_AS("recurrence_prepare", recurrence_prepare_kernel, dim3(blocks), dim3(256), 0, stream, m, first_sequence, offsets, from, to);
     return check_launch("tg_linear_recurrence");
 }
 

@@ -6,14 +6,15 @@
 // rows of V channels in registers, so the inputs are read once.  Its map is composed
 //   1. over the threads of a wave that hold other rows of the same channels (there are some where there are few channels),
 //   2. over the workgroup's waves, through LDS,
-//   3. over the workgroups: a chunk of rows publishes its map; the last of every kChain chunks that of their group; the last of every
-//      kChain groups the state behind it.  A chunk starts from the last such state and goes over the groups and then the chunks
-//      between: a fixed order of operations, so results do not depend on timing, and one wait for kChain^2 chunks in the chain from the
-//      first chunk to the last.  Nothing in front of a closed map is waited for.
-// Chunks are numbered by a ticket, taken when a workgroup starts, so every chunk that is waited for is running or done and waits
-// only on lower ones itself.  Waits are bounded all the same: one that expires makes its chunk's states NaN.
-// A published word holds its own "not there yet" (all ones, a NaN that no result has), so no fence orders a flag with its data: 8 bytes
-// (map) and 4 bytes (state) are written and read whole.
+//   3. over the chunks of rows that workgroups have, in three launches: the chunks' maps, from a first look at the inputs; the states that
+//      the chunks start from, by going over the maps; and the chunks themselves, each from its state.  Calls whose sequences fit a chunk
+//      are the third launch alone.
+// The order of operations is fixed: results do not depend on timing.
+//
+// The first look costs reading inputs twice (backward: gates and dh, not x).  A single launch in which chunks waited for the maps of those
+// before them read them once, and was slower: a chunk held its registers for three round trips through memory more, and the ticket
+// that orders such workgroups, the words to wait on and their clearing came on top (4 x 4096 x 2048, 16 gates: backward 148 us, with
+// every wait left out 66).
 #pragma once
 #include <algorithm>
 #include <type_traits>
@@ -22,12 +23,18 @@
 
 namespace tg {
 
-constexpr int kForwardThreads = 256, kForwardRows = 16;    // rows of a thread; at most 32, a bit each
-constexpr int kBackwardThreads = 256, kBackwardRows = 16;
-constexpr int kChain = 8;
-constexpr uint32_t kAbsent = 0xffffffffu;    // not published yet
+#ifndef TG_RF_THREADS
+#define TG_RF_THREADS 512
+#define TG_RF_ROWS 16
+#define TG_RB_THREADS 1024
+#define TG_RB_ROWS 8
+#endif
+constexpr int kChunk = 8192;  // rows of a chunk x lanes of a row, where there are several chunks to a sequence
+constexpr int kForwardThreads = TG_RF_THREADS, kForwardRows = TG_RF_ROWS;    // rows of a thread; at most 32, a bit each
+constexpr int kBackwardThreads = TG_RB_THREADS, kBackwardRows = TG_RB_ROWS;
+constexpr int kMapThreads = 256, kMapRows = 8;
+static_assert(kForwardThreads * kForwardRows == kChunk && kBackwardThreads * kBackwardRows == kChunk && kChunk % (kMapThreads * kMapRows) == 0, "");
 constexpr uint32_t kClosedMap = 0xfffffffeu;  // in the place of a map's factor: closed
-constexpr uint32_t kWaitLimit = 1u << 20;
 
 // Rows in the order of the recurrence ("places"): row = reverse ? rows - 1 - place : place.  Columns are lanes: a lane has V successive
 // channels; the lanes of a shared gate are padded to a power of two (gate_lanes), above 64 of them it has `parts` such runs.
@@ -35,22 +42,27 @@ struct Split {
     int64_t rows, channels, gates, shared, length, sequences;
     int64_t chunks, columns, tiles;  // columns: lanes of a row, padding included
     int64_t chunk_rows;
-    int64_t block_rows;              // rows between two states that are kept for the backward call
     int lanes_log2, gate_lanes_log2, parts;
     int gate_form, wide_gates;       // gates are float whatever T is
-    bool complement, reverse, chained, packed;
+    bool complement, reverse, chained, packed;  // chained: chunks do not all begin with a sequence
 };
 
-// Workspace of a chained or packed call; where[] says at what byte.
-struct Chain {
-    uint64_t *maps;       // [chunks][tiles * lanes * V]
-    uint64_t *groups;     // [chunks / kChain][tiles * lanes * V]
-    uint32_t *states;     // [chunks / kChain^2][tiles * lanes * V]
-    uint32_t *ticket;
-    int32_t *first_sequence;  // [chunks][2] (packed): the sequences that the chunk's first and last row are searched between
+// A word of the table of a chunk's places: its sequence, and what the place is in it.
+constexpr uint32_t kSequences = 1u << 29, kFirst = 1u << 29, kLast = 1u << 30, kOutside = 1u << 31;
+struct Marks {
+    uint32_t firsts, lasts, outside;  // a bit for each of a thread's rows
 };
-
-constexpr uint8_t kFirst = 1, kLast = 2, kOutside = 4;
+__device__ __forceinline__ Marks marks_of(const uint32_t *table, int n) {
+    Marks r = {0, 0, 0};
+    for (int k = 0; k < n; k++) {
+        const uint32_t w = table[k];
+        r.firsts |= (w & kFirst ? 1u : 0u) << k;
+        r.lasts |= (w & kLast ? 1u : 0u) << k;
+        r.outside |= (w & kOutside ? 1u : 0u) << k;
+    }
+    return r;
+}
+__device__ __forceinline__ int64_t sequence_of(uint32_t word) { return word % kSequences; }
 
 template <int V> struct Map {
     float a[V], u[V];
@@ -71,41 +83,14 @@ template <int V> __device__ __forceinline__ void compose(Map<V> &later, const Ma
 
 __device__ __forceinline__ uint32_t word_of(float f) { return f != f ? 0x7fc00000u : __float_as_uint(f); }
 
-template <class W> __device__ __forceinline__ W look(const W *word) {
-    return __hip_atomic_load(word, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-}
-
-// The word, once it is there; `seen` is what a look at it found.
-template <class W> __device__ __forceinline__ W wait_for(const W *word, W absent, W seen, bool &expired) {
-    for (uint32_t spins = 0; seen == absent && spins < kWaitLimit; spins++) {
-        __builtin_amdgcn_s_sleep(1);
-        seen = look(word);
-    }
-    if (seen == absent) expired = true;
-    return seen;
-}
-
-template <int V> __device__ __forceinline__ void publish(uint64_t *words, const Map<V> &map) {
-#pragma unroll
-    for (int v = 0; v < V; v++) {
-        const uint32_t a = map.closed ? kClosedMap : word_of(map.a[v]);
-        __hip_atomic_store(&words[v], (uint64_t)a << 32 | word_of(map.u[v]), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    }
-}
-template <int V> __device__ __forceinline__ void publish(uint32_t *words, const float (&h)[V]) {
-#pragma unroll
-    for (int v = 0; v < V; v++) __hip_atomic_store(&words[v], word_of(h[v]), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-}
-
 template <int V> __device__ __forceinline__ void step_over(float (&h)[V], const Map<V> &map) {
 #pragma unroll
     for (int v = 0; v < V; v++) h[v] = map.closed ? map.u[v] : apply(map.a[v], h[v], map.u[v]);
 }
 
-// What each place of the chunk is, and whose: by one thread a place.  seq[i] is in [0, sequences) wherever flags say it is used.
+// What each place of the chunk is, and whose (its sequence, in [0, sequences) for places that have one): by one thread a place.
 template <int Threads>
-__device__ __forceinline__ void chunk_table(const Split &m, const Chain &c, const int32_t *offsets, int64_t chunk, int places, int32_t *seq,
-                                            uint8_t *flags) {
+__device__ __forceinline__ void chunk_table(const Split &m, const int32_t *first_sequence, const int32_t *offsets, int64_t chunk, int places, uint32_t *table) {
     const int64_t start = chunk * m.chunk_rows;
     if (!m.packed) {
         const int64_t s0 = start / m.length;
@@ -117,11 +102,11 @@ __device__ __forceinline__ void chunk_table(const Split &m, const Chain &c, cons
                 s += over;
                 q -= (int64_t)over * m.length;
             }
-            seq[i] = (int32_t)(m.reverse ? m.sequences - 1 - s : s);
-            flags[i] = start + i >= m.rows ? 0 : (q == 0 ? kFirst : 0) | (q == m.length - 1 ? kLast : 0);
+            const uint32_t flags = start + i >= m.rows ? 0 : (q == 0 ? kFirst : 0) | (q == m.length - 1 ? kLast : 0);
+            table[i] = (uint32_t)(m.reverse ? m.sequences - 1 - s : s) % kSequences | flags;
         }
     } else {
-        const int32_t low = c.first_sequence[2 * chunk], high = c.first_sequence[2 * chunk + 1];
+        const int32_t low = first_sequence[2 * chunk], high = first_sequence[2 * chunk + 1];
         for (int i = threadIdx.x; i < places; i += Threads) {
             const int64_t place = start + i, row = m.reverse ? m.rows - 1 - place : place;
             int32_t lo = low, hi = high;  // the last sequence that begins at or in front of the row
@@ -130,60 +115,126 @@ __device__ __forceinline__ void chunk_table(const Split &m, const Chain &c, cons
                 if (offsets[mid] <= row) lo = mid; else hi = mid - 1;
             }
             const int64_t begin = offsets[lo], end = offsets[lo + 1];
-            seq[i] = lo;
-            if (place >= m.rows) flags[i] = 0;
-            else if (row < begin || row >= end) flags[i] = kFirst | kLast | kOutside;
-            else flags[i] = (row == (m.reverse ? end - 1 : begin) ? kFirst : 0) | (row == (m.reverse ? begin : end - 1) ? kLast : 0);
+            uint32_t flags = 0;
+            if (place < m.rows) {
+                if (row < begin || row >= end) flags = kFirst | kLast | kOutside;
+                else flags = (row == (m.reverse ? end - 1 : begin) ? kFirst : 0) | (row == (m.reverse ? begin : end - 1) ? kLast : 0);
+            }
+            table[i] = (uint32_t)lo | flags;
         }
     }
 }
 
 // Whether all rows of the chunk are of one sequence that neither begins nor ends among them: no table is needed then.
-__device__ __forceinline__ bool inside_one_sequence(const Split &m, const Chain &c, const int32_t *offsets, int64_t chunk) {
+__device__ __forceinline__ bool inside_one_sequence(const Split &m, const int32_t *first_sequence, const int32_t *offsets, int64_t chunk) {
     const int64_t start = chunk * m.chunk_rows, end = min(start + m.chunk_rows, m.rows);
     if (!m.packed) {
         const int64_t q = start % m.length;
         return q > 0 && q + (end - start) < m.length;
     }
-    const int32_t s = c.first_sequence[2 * chunk];
+    const int32_t s = first_sequence[2 * chunk];
     const int64_t low = m.reverse ? m.rows - end : start, high = m.reverse ? m.rows - start : end;
-    return s == c.first_sequence[2 * chunk + 1] && offsets[s] < low && high < offsets[s + 1];
+    return s == first_sequence[2 * chunk + 1] && offsets[s] < low && high < offsets[s + 1];
 }
 
-// The channel and the gate of a lane's column; false: padding.
+__device__ __forceinline__ int64_t uniform(int64_t v) {  // of a wave whose lanes all have the same, or whose first lane's it is
+    const uint32_t low = __builtin_amdgcn_readfirstlane((uint32_t)v), high = __builtin_amdgcn_readfirstlane((uint32_t)(v >> 32));
+    return (int64_t)((uint64_t)high << 32 | low);
+}
+
+// The channel and the gate of a lane's column; false: padding (which no wave's first lane is unless all of its lanes are).
 template <int V, bool Shared> __device__ __forceinline__ bool column_of(const Split &m, int64_t column, int64_t &channel, int64_t &gate, int &part) {
     part = 0;
+    bool valid;
     if (!Shared) {
         channel = gate = column * V;
-        return channel < m.channels;
+        valid = channel < m.channels;
+    } else {
+        const uint32_t run = (uint32_t)(column >> m.gate_lanes_log2);
+        const uint32_t g = run / (uint32_t)m.parts;
+        part = (int)(run - g * (uint32_t)m.parts);
+        const int64_t within = (((int64_t)part << m.gate_lanes_log2) + (column & ((1 << m.gate_lanes_log2) - 1))) * V;
+        gate = g;
+        channel = gate * m.shared + within;
+        valid = g < m.gates && within < m.shared;
     }
-    const uint32_t run = (uint32_t)(column >> m.gate_lanes_log2);
-    const uint32_t g = run / (uint32_t)m.parts;
-    part = (int)(run - g * (uint32_t)m.parts);
-    const int64_t within = (((int64_t)part << m.gate_lanes_log2) + (column & ((1 << m.gate_lanes_log2) - 1))) * V;
-    gate = g;
-    channel = gate * m.shared + within;
-    return g < m.gates && within < m.shared;
+    // padding reads what the wave's first lane reads
+    const bool any = __builtin_amdgcn_readfirstlane(valid ? 1 : 0) != 0;
+    const int64_t first_channel = uniform(channel), first_gate = uniform(gate);
+    if (!valid) {
+        channel = any ? first_channel : 0;
+        gate = any ? first_gate : 0;
+    }
+    return valid;
 }
 
-// K successive gates of a lane from place `first` on, GV of them a row.  Nothing behind `last` is read.
-template <class T, int K, int GV>
-__device__ __forceinline__ void load_gates(const Split &m, const void *gates, int64_t row, int64_t step, int64_t at, int last, float (&g)[K][GV]) {
-    const int64_t pitch = m.gates * step;
-    if (sizeof(T) == 4 || m.wide_gates) {
-        const float *p = (const float *)gates + row * m.gates + at;
-        Pack<float, GV> raw[K];
+// Where a thread's K rows are.  Rows of a wave that has all of them are addressed from a scalar base with 32-bit offsets of the lanes: a
+// row costs no vector instruction but its load.  (Lanes of a wave with several rows' threads have few channels: offsets stay small.)
+struct Walk {
+    int64_t row, step;       // the thread's first row; 1, or -1 where the order is reversed
+    int64_t wave_row;        // the lowest of the wave's threads' first rows
+    uint32_t above;          // the thread's first row, from there
+    int last;                // the thread's last row, by number
+    bool whole;              // all of the wave's threads have K rows
+};
+
+template <int K, int Threads> __device__ __forceinline__ Walk walk_of(const Split &m, int64_t start, int turn, int n, int batches = 1) {
+    Walk w;
+    const int at = turn * K, subs = m.lanes_log2 < 6 ? kWave >> m.lanes_log2 : 1;
+    const int64_t place = start + (n > 0 ? at : 0);
+    w.row = m.reverse ? m.rows - 1 - place : place;
+    w.step = m.reverse ? -1 : 1;
+    w.last = max(n - 1, 0);
+    w.whole = __all(n == K);
+    const int first_turn = __builtin_amdgcn_readfirstlane(turn), sub = turn - first_turn;
+    const int reach = (subs - 1) * batches;  // a thread's rows are those of every batches-th turn
+    w.wave_row = m.reverse ? m.rows - 1 - (start + (int64_t)(first_turn + reach) * K) : start + (int64_t)first_turn * K;
+    w.above = (uint32_t)((m.reverse ? reach - sub : sub) * K);
+    return w;
+}
+
+// A column of an array of `width` a row: the wave's first one, and the lane's from there.
+struct Column {
+    int64_t width, wave, lane;
+    uint32_t offset;
+};
+__device__ __forceinline__ Column column(int64_t width, int64_t at) {
+    Column c;
+    c.width = width;
+    c.lane = at;
+    c.wave = uniform(at);
+    c.offset = (uint32_t)(at - c.wave);
+    return c;
+}
+
+// call(k, pointer to the thread's row k): rows behind the last are the last again.
+template <int K, class T, class Call> __device__ __forceinline__ void each_row(const Walk &w, const Column &c, T *array, Call &&call) {
+    const int64_t pitch = c.width * w.step;
+    if (w.whole) {
+        T *from = array + (w.wave_row * c.width + c.wave);
+        const uint32_t offset = w.above * (uint32_t)c.width + c.offset;
 #pragma unroll
-        for (int k = 0; k < K; k++) raw[k] = load_pack<GV>(p + pitch * min(k, last));
+        for (int k = 0; k < K; k++) call(k, from + pitch * k + offset);
+    } else {
+        T *from = array + (w.row * c.width + c.lane);
+#pragma unroll
+        for (int k = 0; k < K; k++) call(k, from + pitch * min(k, w.last));
+    }
+}
+
+// K successive gates of a lane, GV of them a row.
+template <class T, int K, int GV>
+__device__ __forceinline__ void load_gates(const Split &m, const void *gates, const Walk &w, const Column &c, float (&g)[K][GV]) {
+    if (sizeof(T) == 4 || m.wide_gates) {
+        Pack<float, GV> raw[K];
+        each_row<K>(w, c, (const float *)gates, [&](int k, const float *p) { raw[k] = load_pack<GV>(p); });
 #pragma unroll
         for (int k = 0; k < K; k++)
 #pragma unroll
             for (int v = 0; v < GV; v++) g[k][v] = raw[k].v[v];
     } else {
-        const T *p = (const T *)gates + row * m.gates + at;
         Pack<T, GV> raw[K];
-#pragma unroll
-        for (int k = 0; k < K; k++) raw[k] = load_pack<GV>(p + pitch * min(k, last));
+        each_row<K>(w, c, (const T *)gates, [&](int k, const T *p) { raw[k] = load_pack<GV>(p); });
 #pragma unroll
         for (int k = 0; k < K; k++)
 #pragma unroll
@@ -191,40 +242,112 @@ __device__ __forceinline__ void load_gates(const Split &m, const void *gates, in
     }
 }
 
-// Maps that other workgroups published, in LDS: [which][lane][V].
-template <int V> struct Published {
-    float a[kChain * kWave * V], u[kChain * kWave * V];
-    bool closed[kChain];
-    template <int W> __device__ __forceinline__ Map<W> at(int i, int lanes, int lane) const {
-        Map<W> r;
-#pragma unroll
-        for (int v = 0; v < V; v++) {
-            r.a[v] = a[(i * lanes + lane) * V + v];
-            r.u[v] = u[(i * lanes + lane) * V + v];
-        }
-        r.closed = closed[i];
-        return r;
-    }
-};
+// The same rows from the last to the first (of a wave that has all of them).
+template <int K> __device__ __forceinline__ Walk against(const Walk &w) {
+    Walk b = w;
+    b.row = w.row + (K - 1) * w.step;
+    b.wave_row = w.wave_row + (K - 1) * w.step;
+    b.step = -w.step;
+    return b;
+}
 
-template <int V>
-__device__ __forceinline__ void settle(Published<V> &to, int i, int lanes, int lane, const uint64_t (&seen)[V], const uint64_t *words, bool &expired) {
-#pragma unroll
-    for (int v = 0; v < V; v++) {
-        const uint64_t w = wait_for(&words[v], ~(uint64_t)0, seen[v], expired);
-        const uint32_t a = (uint32_t)(w >> 32);
-        to.a[(i * lanes + lane) * V + v] = __uint_as_float(a);
-        to.u[(i * lanes + lane) * V + v] = __uint_as_float((uint32_t)w);
-        if (lane == 0 && v == 0) to.closed[i] = a == kClosedMap;
+// The gates of a thread's rows in two steps, reading and computing.  Where all lanes of a wave share a gate, lane k reads and computes that
+// of row k, for all.
+template <class T, int K, int GV>
+__device__ __forceinline__ void read_gates(const Split &m, const void *gates, const Walk &w, const Column &c, float (&g)[K][GV]) {
+    if (GV == 1 && m.shared > 1 && m.gate_lanes_log2 == 6) {
+        const int64_t at = (w.row + min((int)(threadIdx.x & (kWave - 1)), w.last) * w.step) * c.width + c.lane;
+        g[0][0] = sizeof(T) == 4 || m.wide_gates ? ((const float *)gates)[at] : (float)((const T *)gates)[at];
+    } else {
+        load_gates<T, K, GV>(m, gates, w, c, g);
     }
 }
+template <int K, int GV> __device__ __forceinline__ void compute_gates(const Split &m, float (&a)[K][GV], float (&rest)[K][GV]) {
+    if (GV == 1 && m.shared > 1 && m.gate_lanes_log2 == 6) {
+        const Gate own = gate_of(m.gate_form, a[0][0]);
+#pragma unroll
+        for (int k = 0; k < K; k++) {
+            a[k][0] = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(own.a), k));
+            rest[k][0] = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(own.rest), k));
+        }
+    } else {
+        const auto all = [&](auto form) {
+#pragma unroll
+            for (int k = 0; k < K; k++)
+#pragma unroll
+                for (int v = 0; v < GV; v++) {
+                    const Gate g = gate_of<decltype(form)::value>(a[k][v]);
+                    a[k][v] = g.a;
+                    rest[k][v] = g.rest;
+                }
+        };
+        if (m.gate_form == TG_GATE_VALUE) all(std::integral_constant<int, TG_GATE_VALUE>());
+        else if (m.gate_form == TG_GATE_LOGIT) all(std::integral_constant<int, TG_GATE_LOGIT>());
+        else if (m.complement) all(std::integral_constant<int, TG_GATE_LOG>());
+        else {
+#pragma unroll
+            for (int k = 0; k < K; k++)
+#pragma unroll
+                for (int v = 0; v < GV; v++) a[k][v] = rest[k][v] = exp_real(a[k][v]);  // 1 - a is not asked for
+        }
+    }
+}
+
+template <int Control> __device__ __forceinline__ float from_lane(float v) {  // of the sixteen: by the data-parallel move's control
+    return __uint_as_float((uint32_t)__builtin_amdgcn_update_dpp(0, (int)__float_as_uint(v), Control, 0xf, 0xf, true));
+}
+constexpr int kRotate8 = 0x128, kMirrorOf8 = 0x141, kSwapOnes = 0xb1, kSwapTwos = 0x4e;
+
+// Sums of K rows' values over the wave.  Each step hands half of the rows to half of the lanes, so K + K / 2 + ... additions do what six a
+// row would; a lane ends with the sum of row_of_sum, and the lanes that sum_is_here names have each of them once.
+template <int K> __device__ __forceinline__ float sum_rows(float (&q)[K]) {
+    static_assert(K == 8 || K == 16, "");
+    const int lane = threadIdx.x & (kWave - 1);
+#pragma unroll
+    for (int i = 0; i < K / 2; i++) {
+        const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(q[i]), __float_as_uint(q[i + K / 2]), false, false);
+        q[i] = __uint_as_float(r[0]) + __uint_as_float(r[1]);
+    }
+#pragma unroll
+    for (int i = 0; i < K / 4; i++) {
+        const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(q[i]), __float_as_uint(q[i + K / 4]), false, false);
+        q[i] = __uint_as_float(r[0]) + __uint_as_float(r[1]);
+    }
+#pragma unroll
+    for (int i = 0; i < K / 8; i++) {
+        const float keep = lane & 8 ? q[i + K / 8] : q[i], give = lane & 8 ? q[i] : q[i + K / 8];
+        q[i] = keep + from_lane<kRotate8>(give);
+    }
+    if (K == 16) {
+        const float keep = lane & 4 ? q[1] : q[0], give = lane & 4 ? q[0] : q[1];
+        q[0] = keep + from_lane<kMirrorOf8>(give);
+    } else {
+        q[0] += from_lane<kMirrorOf8>(q[0]);
+    }
+    q[0] += from_lane<kSwapOnes>(q[0]);
+    q[0] += from_lane<kSwapTwos>(q[0]);
+    return q[0];
+}
+template <int K> __device__ __forceinline__ int row_of_sum(int lane) {
+    const int eighth = (lane >> 5) * 4 + (lane >> 4 & 1) * 2 + (lane >> 3 & 1);
+    return K == 16 ? eighth * 2 + (lane >> 2 & 1) : eighth;
+}
+template <int K> __device__ __forceinline__ bool sum_is_here(int lane) { return (lane & (K == 16 ? 3 : 7)) == 0; }
 
 // The maps of the workgroup's threads, or waves, [entry][lane][V].
 template <int V, int Threads> struct Joint {
     float a[Threads * V], u[Threads * V];
-    Published<V> maps, groups;
-    float state[Threads * V];
     bool closed[Threads];
+    __device__ __forceinline__ Map<V> at(int entry, int lanes, int lane) const {
+        Map<V> r;
+#pragma unroll
+        for (int v = 0; v < V; v++) {
+            r.a[v] = a[(entry * lanes + lane) * V + v];
+            r.u[v] = u[(entry * lanes + lane) * V + v];
+        }
+        r.closed = closed[entry];
+        return r;
+    }
 };
 
 template <int V> __device__ __forceinline__ Map<V> shifted(const Map<V> &m, int lanes, bool backward) {
@@ -272,13 +395,13 @@ template <int Threads> __device__ __forceinline__ Place place_of(const Split &m)
     return p;
 }
 
-// Composes `map` over the workgroup and the chunks before: returns the state (or, backward, what reaches the last row from behind) that the
-// thread's own rows start from.  known: what the chunk starts from, for a call that knows (h of the leading threads).
+// Puts the threads' maps into the Joint, composed over the threads of a wave where several hold rows of the same channels, and returns the
+// map of those in front of the thread in its wave.  Backward: the order is that against the rows.
 template <int V, int Threads, bool Backward>
-__device__ __forceinline__ void join(const Split &m, const Chain &c, Joint<V, Threads> &j, const Place &p, int64_t tile, int64_t order, Map<V> map,
-                                     bool chunk_closed, bool chained, const float *known, float (&h)[V]) {
+__device__ __forceinline__ Map<V> gather(const Split &m, Joint<V, Threads> &j, const Place &p, Map<V> map) {
     const int lanes = 1 << m.lanes_log2;
     Map<V> before = unit_map<V>();
+    bool stores = true;
     if (m.lanes_log2 < 6) {
         const int sub = (threadIdx.x & (kWave - 1)) >> m.lanes_log2, subs = kWave >> m.lanes_log2;
         for (int d = 1; d < subs; d <<= 1) {
@@ -287,150 +410,27 @@ __device__ __forceinline__ void join(const Split &m, const Chain &c, Joint<V, Th
         }
         const Map<V> other = shifted(map, lanes, Backward);
         if (Backward ? sub + 1 < subs : sub >= 1) before = other;
-        if (sub == (Backward ? 0 : subs - 1)) {
-#pragma unroll
-            for (int v = 0; v < V; v++) {
-                j.a[(p.entry * lanes + p.lane) * V + v] = map.a[v];
-                j.u[(p.entry * lanes + p.lane) * V + v] = map.u[v];
-            }
-            if (p.lane == 0) j.closed[p.entry] = map.closed;
-        }
-    } else {
+        stores = sub == (Backward ? 0 : subs - 1);
+    }
+    if (stores) {
 #pragma unroll
         for (int v = 0; v < V; v++) {
-            j.a[threadIdx.x * V + v] = map.a[v];
-            j.u[threadIdx.x * V + v] = map.u[v];
+            j.a[(p.entry * lanes + p.lane) * V + v] = map.a[v];
+            j.u[(p.entry * lanes + p.lane) * V + v] = map.u[v];
         }
         if (p.lane == 0) j.closed[p.entry] = map.closed;
     }
     __syncthreads();
-    const int64_t words = m.tiles * lanes * V, at = (tile * lanes + p.lane) * V;
-    if (chained) {
-        const bool ends_group = order % kChain == kChain - 1, ends_super = order % (kChain * kChain) == kChain * kChain - 1;
-        const int64_t group = order / kChain, super = group / kChain;
-        Map<V> total = unit_map<V>();
-        if (p.leads) {
-            for (int i = 0; i < p.entries; i++) {
-                const int e = Backward ? p.entries - 1 - i : i;
-                Map<V> next;
-#pragma unroll
-                for (int v = 0; v < V; v++) {
-                    next.a[v] = j.a[(e * lanes + p.lane) * V + v];
-                    next.u[v] = j.u[(e * lanes + p.lane) * V + v];
-                }
-                next.closed = j.closed[e];
-                compose(next, total);
-                total = next;
-            }
-            if (!ends_group) publish(c.maps + order * words + at, total);
-            else if (total.closed && !ends_super) publish(c.groups + group * words + at, total);
-            if (ends_super && total.closed) publish(c.states + super * words + at, total.u);
-        }
-        const int maps = (int)(order % kChain), groups = (int)(group % kChain);
-        if (!chunk_closed) {
-            // one look at all that may be needed, then waits for what was not there
-            constexpr int Turns = Threads / kWave, Rounds = kChain / Turns + (kChain % Turns ? 1 : 0);
-            const int turns = Threads >> m.lanes_log2;
-            bool expired = false;
-            uint64_t seen_map[Rounds][V], seen_group[Rounds][V];
-            uint32_t seen_state[V];
-#pragma unroll
-            for (int r = 0; r < Rounds; r++) {
-                const int i = p.turn + r * turns;
-#pragma unroll
-                for (int v = 0; v < V; v++) {
-                    seen_map[r][v] = i < maps ? look(&c.maps[(group * kChain + i) * words + at + v]) : 0;
-                    seen_group[r][v] = i < groups ? look(&c.groups[(super * kChain + i) * words + at + v]) : 0;
-                }
-            }
-#pragma unroll
-            for (int v = 0; v < V; v++) seen_state[v] = p.leads && super > 0 ? look(&c.states[(super - 1) * words + at + v]) : 0;
-#pragma unroll
-            for (int r = 0; r < Rounds; r++) {
-                const int i = p.turn + r * turns;
-                if (i < maps) settle<V>(j.maps, i, lanes, p.lane, seen_map[r], c.maps + (group * kChain + i) * words + at, expired);
-            }
-            bool failed = __syncthreads_or(expired) != 0, shut = false;
-            for (int i = 0; i < maps; i++) shut = shut || j.maps.closed[i];
-            if (ends_group && !ends_super && !total.closed && p.leads) {
-                Map<V> all = total;
-                for (int i = maps - 1; i >= 0; i--) compose(all, j.maps.template at<V>(i, lanes, p.lane));
-                if (failed)
-#pragma unroll
-                    for (int v = 0; v < V; v++) all.u[v] = __uint_as_float(0x7fc00000u);
-                publish(c.groups + group * words + at, all);
-            }
-            if (!shut) {
-#pragma unroll
-                for (int r = 0; r < Rounds; r++) {
-                    const int i = p.turn + r * turns;
-                    if (i < groups) settle<V>(j.groups, i, lanes, p.lane, seen_group[r], c.groups + (super * kChain + i) * words + at, expired);
-                }
-                failed = __syncthreads_or(expired) != 0;
-            }
-            if (p.leads) {
-                bool open = !shut;
-                if (open)
-                    for (int i = 0; i < groups; i++) open = open && !j.groups.closed[i];
-                expired = false;
-#pragma unroll
-                for (int v = 0; v < V; v++)
-                    h[v] = open && super > 0 ? __uint_as_float(wait_for(&c.states[(super - 1) * words + at + v], kAbsent, seen_state[v], expired)) : 0.0f;
-                if (!shut)
-                    for (int i = 0; i < groups; i++) step_over(h, j.groups.template at<V>(i, lanes, p.lane));
-                for (int i = 0; i < maps; i++) step_over(h, j.maps.template at<V>(i, lanes, p.lane));
-                if (failed || expired)
-#pragma unroll
-                    for (int v = 0; v < V; v++) h[v] = __uint_as_float(0x7fc00000u);
-            }
-        } else if (p.leads) {
-#pragma unroll
-            for (int v = 0; v < V; v++) h[v] = 0.0f;
-        }
-        if (p.leads) {
-            if (ends_super && !total.closed) {
-                float end[V];
-#pragma unroll
-                for (int v = 0; v < V; v++) end[v] = h[v];
-                step_over(end, total);
-                publish(c.states + super * words + at, end);
-            }
-#pragma unroll
-            for (int v = 0; v < V; v++) j.state[p.lane * V + v] = h[v];
-        }
-        __syncthreads();
-#pragma unroll
-        for (int v = 0; v < V; v++) h[v] = j.state[p.lane * V + v];
-    } else {
-#pragma unroll
-        for (int v = 0; v < V; v++) h[v] = known ? known[v] : 0.0f;
-    }
-    // through the entries before the thread's own, then through the threads before it in its wave
-    const int mine = Backward ? p.entries - 1 - p.entry : p.entry;
-    for (int i = 0; i < mine; i++) {
-        const int e = Backward ? p.entries - 1 - i : i;
-        Map<V> next;
-#pragma unroll
-        for (int v = 0; v < V; v++) {
-            next.a[v] = j.a[(e * lanes + p.lane) * V + v];
-            next.u[v] = j.u[(e * lanes + p.lane) * V + v];
-        }
-        next.closed = j.closed[e];
-        step_over(h, next);
-    }
-    step_over(h, before);
+    return before;
 }
 
-// The workgroup's chunk in the order of the chain, and its tile of columns.  Chained: by ticket.
-__device__ __forceinline__ void numbered(const Split &m, const Chain &c, uint32_t *shared, int64_t &order, int64_t &tile) {
-    uint32_t id = blockIdx.x;
-    if (m.chained) {
-        if (threadIdx.x == 0) *shared = __hip_atomic_fetch_add(c.ticket, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        __syncthreads();
-        id = *shared;
-    }
-    order = id / (uint32_t)m.tiles;
-    tile = id - (uint32_t)order * (uint32_t)m.tiles;
+// What the thread's own rows start from; h on entry is what the chunk starts from.
+template <int V, int Threads, bool Backward>
+__device__ __forceinline__ void join(const Split &m, Joint<V, Threads> &j, const Place &p, const Map<V> &map, float (&h)[V]) {
+    const Map<V> before = gather<V, Threads, Backward>(m, j, p, map);
+    const int mine = Backward ? p.entries - 1 - p.entry : p.entry;
+    for (int i = 0; i < mine; i++) step_over(h, j.at(Backward ? p.entries - 1 - i : i, 1 << m.lanes_log2, p.lane));
+    step_over(h, before);
 }
 
 // call(T(), integral_constant V, bool_constant Shared) for a layout that split_of makes.
@@ -446,9 +446,20 @@ template <class Call> int by_layout(int64_t type, int vector, int64_t shared, Ca
     return type == TG_TYPE_F32 ? by_vector(float()) : type == TG_TYPE_F16 ? by_vector(half_t()) : by_vector(bf16_t());
 }
 
-int launch_forward(const tg_recurrence &r, const Split &m, const Chain &c, int vector, unsigned blocks, hipStream_t stream);
-int launch_backward(const tg_recurrence &r, const Split &m, const Chain &c, float *partial, int vector, unsigned blocks, hipStream_t stream);
-int launch_prepare(const Split &m, const Chain &c, uint64_t *words, int64_t n_words, const int32_t *offsets, const float *from, float *to,
+// LDS for the table of a chunk's places.
+inline size_t table_bytes(const Split &m, int chunk) { return (size_t)(chunk >> m.lanes_log2) * 4; }
+
+struct MapWords {
+    float a, u;  // a: kClosedMap's bits where the map is closed
+};
+
+int launch_forward(const tg_recurrence &r, const Split &m, const int32_t *first_sequence, const float *starts, int vector, unsigned blocks,
                    hipStream_t stream);
+int launch_backward(const tg_recurrence &r, const Split &m, const int32_t *first_sequence, const float *starts, float *partial, int vector,
+                    unsigned blocks, hipStream_t stream);
+int launch_prepare(const Split &m, int32_t *first_sequence, const int32_t *offsets, const float *from, float *to, hipStream_t stream);
+// The states (backward: what comes from behind) that the chunks of `m` start from.
+int launch_starts(const tg_recurrence &r, const Split &m, const int32_t *first_sequence, MapWords *maps, float *starts, int vector, bool backward,
+                  hipStream_t stream);
 
 }  // namespace tg
