@@ -115,34 +115,31 @@ __global__ __launch_bounds__(Threads, 4) void recurrence_forward_kernel(Split m,
     }
 }
 
-// The map of each chunk, by a first look at what it needs: inputs and gates, or, Backward, gradients of the states and gates.
+// The map of each chunk, by a first look at what it needs: inputs and gates, or, Backward, gradients of the states and gates.  A thread
+// goes over its rows as they were read, eight at a time, so little else is held.
 template <class T, int V, bool Shared, bool Backward>
 __global__ __launch_bounds__(kMapThreads) void recurrence_maps_kernel(Split m, const int32_t *__restrict__ first_sequence, const T *__restrict__ inputs,
                                                                       const void *__restrict__ gates, const float *__restrict__ ends,
                                                                       const int32_t *__restrict__ offsets, MapWords *__restrict__ maps) {
-    constexpr int GV = Shared ? 1 : V, K = kMapRows, Threads = kMapThreads, Batches = kChunk / (Threads * K);
+    constexpr int GV = Shared ? 1 : V, Threads = kMapThreads, Rows = kChunk / Threads;
     extern __shared__ uint32_t table[];
     __shared__ Joint<V, Threads> joint;
     int64_t channel, gate;
     int part;
     const int64_t chunk = blockIdx.x / (uint32_t)m.tiles, tile = blockIdx.x % (uint32_t)m.tiles;
     const Place p = place_of<Threads>(m);
-    const int places = (Threads >> m.lanes_log2) * K * Batches;
     const int64_t start = chunk * m.chunk_rows;
     const bool valid = column_of<V, Shared>(m, (tile << m.lanes_log2) + p.lane, channel, gate, part);
     const Column cx = column(m.channels, channel), cg = column(m.gates, gate);
-    const bool marked = !inside_one_sequence(m, first_sequence, offsets, chunk);
-    if (marked) {
-        chunk_table<Threads>(m, first_sequence, offsets, chunk, places, table);
-        __syncthreads();
-    }
+    const bool wide = sizeof(T) == 4 || m.wide_gates;
     Map<V> map = unit_map<V>();
-    for (int batch = 0; batch < Batches; batch++) {
-        const int turn = p.turn * Batches + (Backward ? Batches - 1 - batch : batch), at = turn * K;
-        const int n = (int)max((int64_t)0, min(min(m.chunk_rows, m.rows - start) - at, (int64_t)K));
-        const Walk w = walk_of<K, Threads>(m, start, turn, n, Batches);
-        Pack<T, V> x[K];
-        float a[K][GV], rest[K][GV];
+    const auto step = [&](int v, const Gate &g, float x) {
+        if (Backward) map.u[v] = g.a * (map.u[v] + x);
+        else map.u[v] = fmaf(g.a, map.u[v], m.complement ? g.rest * x : x);
+        map.a[v] *= g.a;
+    };
+    const auto read = [&](auto &x, const Walk &w) {
+        constexpr int K = sizeof(x) / sizeof(x[0]);
         if (inputs) {
             each_row<K>(w, cx, inputs, [&](int k, const T *from) { x[k] = load_pack<V>(from); });
         } else {
@@ -151,41 +148,71 @@ __global__ __launch_bounds__(kMapThreads) void recurrence_maps_kernel(Split m, c
 #pragma unroll
                 for (int v = 0; v < V; v++) x[k].v[v] = (T)0.0f;
         }
-        read_gates<T, K, GV>(m, gates, w, cg, a);
-        compute_gates<K, GV>(m, a, rest);
-        uint32_t marks = 0, outside = 0;
-        if (marked) {
-            const Marks found = marks_of(table + at, n);
-            marks = Backward ? found.lasts : found.firsts;
-            outside = found.outside;
-        }
-        const auto step = [&](int k, int v) {
-            if (Backward) {
-                map.u[v] = a[k][Shared ? 0 : v] * (map.u[v] + x[k][v]);
-            } else {
-                const float u = m.complement ? rest[k][Shared ? 0 : v] * x[k][v] : x[k][v];
-                map.u[v] = fmaf(a[k][Shared ? 0 : v], map.u[v], u);
+    };
+    if (start + m.chunk_rows <= m.rows && inside_one_sequence(m, first_sequence, offsets, chunk)) {
+        constexpr int K = 8, Batches = Rows / K;
+        for (int batch = 0; batch < Batches; batch++) {
+            const Walk w = walk_of<K, Threads>(m, start, p.turn * Batches + (Backward ? Batches - 1 - batch : batch), K, Batches);
+            Pack<T, V> x[K];
+            read(x, w);
+            const auto all = [&](auto &&gate_at) {
+#pragma unroll
+                for (int i = 0; i < K; i++) {
+                    const int k = Backward ? K - 1 - i : i;
+#pragma unroll
+                    for (int v = 0; v < V; v++) step(v, gate_at(k, Shared ? 0 : v), x[k][v]);
+                }
+            };
+            if (Shared && m.gate_lanes_log2 == 6) {
+                // all lanes share a gate: lane k computes that of row k
+                const int64_t at = (w.row + min((int)(threadIdx.x & (kWave - 1)), K - 1) * w.step) * m.gates + gate;
+                const Gate own = gate_of(m.gate_form, wide ? ((const float *)gates)[at] : (float)((const T *)gates)[at]);
+                all([&](int k, int) {
+                    Gate g;
+                    g.a = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(own.a), k));
+                    g.rest = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(own.rest), k));
+                    return g;
+                });
+                continue;
             }
-            map.a[v] *= a[k][Shared ? 0 : v];
-        };
-        if (w.whole && !__any(marks != 0)) {
-#pragma unroll
-            for (int i = 0; i < K; i++)
-#pragma unroll
-                for (int v = 0; v < V; v++) step(Backward ? K - 1 - i : i, v);
-        } else {
+            const auto by_type = [&](auto like) {
+                Pack<decltype(like), GV> g[K];
+                each_row<K>(w, cg, (const decltype(like) *)gates, [&](int k, const decltype(like) *from) { g[k] = load_pack<GV>(from); });
+                if (m.gate_form == TG_GATE_VALUE) all([&](int k, int v) { return gate_of<TG_GATE_VALUE>(g[k][v]); });
+                else if (m.gate_form == TG_GATE_LOG) all([&](int k, int v) { return gate_of<TG_GATE_LOG>(g[k][v]); });
+                else all([&](int k, int v) { return gate_of<TG_GATE_LOGIT>(g[k][v]); });
+            };
+            if (wide) by_type(float());
+            else by_type(T());
+        }
+    } else {
+        constexpr int K = 8, Batches = Rows / K;
+        const int places = (Threads >> m.lanes_log2) * Rows;
+        chunk_table<Threads>(m, first_sequence, offsets, chunk, places, table);
+        __syncthreads();
+        for (int batch = 0; batch < Batches; batch++) {
+            const int turn = p.turn * Batches + (Backward ? Batches - 1 - batch : batch), at = turn * K;
+            const int n = (int)max((int64_t)0, min(min(m.chunk_rows, m.rows - start) - at, (int64_t)K));
+            const Walk w = walk_of<K, Threads>(m, start, turn, n, Batches);
+            Pack<T, V> x[K];
+            float g[K][GV];
+            read(x, w);
+            load_gates<T, K, GV>(m, gates, w, cg, g);
+            const Marks marks = marks_of(table + at, n);
 #pragma unroll
             for (int i = 0; i < K; i++) {
                 const int k = Backward ? K - 1 - i : i;
-                const bool mark = (marks >> k & 1) != 0, out = (outside >> k & 1) != 0;
+                const bool out = (marks.outside >> k & 1) != 0;
                 if (k >= n) continue;
+                if ((Backward ? marks.lasts : marks.firsts) >> k & 1) {
 #pragma unroll
-                for (int v = 0; v < V; v++) {
-                    if (mark) map.u[v] = ends && !out && valid ? ends[sequence_of(table[at + k]) * m.channels + channel + v] : 0.0f;
-                    if (out) map.a[v] = map.u[v] = 0.0f;
-                    else step(k, v);
+                    for (int v = 0; v < V; v++)
+                        map.u[v] = ends && !out && valid ? ends[sequence_of(table[at + k]) * m.channels + channel + v] : 0.0f;
+                    map.closed = true;
                 }
-                map.closed = map.closed || mark;
+                if (out) continue;
+#pragma unroll
+                for (int v = 0; v < V; v++) step(v, gate_of(m.gate_form, g[k][Shared ? 0 : v]), x[k][v]);
             }
         }
     }
@@ -208,7 +235,7 @@ __global__ __launch_bounds__(kMapThreads) void recurrence_maps_kernel(Split m, c
 
 // The states that the chunks start from.  A wave goes over a run of chunks for 64 channels, twice: for the run's map, and, once the runs before
 // are known, from their state.
-constexpr int kStartWaves = 16, kStartAhead = 8;
+constexpr int kStartWaves = 16, kStartAhead = 16;
 __global__ __launch_bounds__(kStartWaves * kWave) void recurrence_starts_kernel(int64_t chunks, int64_t channels, bool backward,
                                                                                 const MapWords *__restrict__ maps, float *__restrict__ starts) {
     __shared__ Joint<1, kStartWaves * kWave> joint;
@@ -216,40 +243,45 @@ __global__ __launch_bounds__(kStartWaves * kWave) void recurrence_starts_kernel(
     const int64_t channel = (int64_t)blockIdx.x * kWave + lane, run = (chunks + kStartWaves - 1) / kStartWaves;
     const int64_t begin = min(wave * run, chunks), end = min(begin + run, chunks);
     const bool valid = channel < channels;
-    const auto over = [&](auto &&call) {
-        for (int64_t i = begin; i < end; i += kStartAhead) {
-            MapWords next[kStartAhead];
+    MapWords next[kStartAhead];
+    const auto read = [&](int64_t i) {
 #pragma unroll
-            for (int k = 0; k < kStartAhead; k++) {
-                const int64_t c = min(i + k, end - 1);
-                next[k] = maps[(backward ? chunks - 1 - c : c) * channels + (valid ? channel : 0)];
-            }
+        for (int k = 0; k < kStartAhead; k++) {
+            const int64_t c = min(i + k, end - 1);
+            next[k] = maps[(backward ? chunks - 1 - c : c) * channels + (valid ? channel : 0)];
+        }
+    };
+    const auto over = [&](int64_t i, auto &&call) {
 #pragma unroll
-            for (int k = 0; k < kStartAhead; k++) {
-                Map<1> map;
-                map.a[0] = next[k].a;
-                map.u[0] = next[k].u;
-                map.closed = __float_as_uint(next[k].a) == kClosedMap;
-                if (map.closed) map.a[0] = 0.0f;
-                if (i + k < end) call(i + k, map);
-            }
+        for (int k = 0; k < kStartAhead; k++) {
+            Map<1> map;
+            map.closed = __float_as_uint(next[k].a) == kClosedMap;
+            map.a[0] = map.closed ? 0.0f : next[k].a;
+            map.u[0] = next[k].u;
+            if (i + k < end) call(i + k, map);
         }
     };
     Map<1> total = unit_map<1>();
-    over([&](int64_t, Map<1> map) {
-        compose(map, total);
-        total = map;
-    });
+    for (int64_t i = begin; i < end; i += kStartAhead) {
+        read(i);
+        over(i, [&](int64_t, Map<1> map) {
+            compose(map, total);
+            total = map;
+        });
+    }
     joint.a[threadIdx.x] = total.a[0];
     joint.u[threadIdx.x] = total.u[0];
     if (lane == 0) joint.closed[wave] = total.closed;
     __syncthreads();
     float h[1] = {0.0f};
     for (int i = 0; i < wave; i++) step_over(h, joint.at(i, kWave, lane));
-    over([&](int64_t c, const Map<1> &map) {
-        if (valid) starts[(backward ? chunks - 1 - c : c) * channels + channel] = h[0];
-        step_over(h, map);
-    });
+    for (int64_t i = begin; i < end; i += kStartAhead) {
+        if (run > kStartAhead) read(i);
+        over(i, [&](int64_t c, const Map<1> &map) {
+            if (valid) starts[(backward ? chunks - 1 - c : c) * channels + channel] = h[0];
+            step_over(h, map);
+        });
+    }
 }
 
 // In front of a call on packed sequences: those that each chunk's rows are searched between, and the final states (or, backward, the initial

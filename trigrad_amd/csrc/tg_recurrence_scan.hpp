@@ -23,17 +23,11 @@
 
 namespace tg {
 
-#ifndef TG_RF_THREADS
-#define TG_RF_THREADS 512
-#define TG_RF_ROWS 16
-#define TG_RB_THREADS 1024
-#define TG_RB_ROWS 8
-#endif
 constexpr int kChunk = 8192;  // rows of a chunk x lanes of a row, where there are several chunks to a sequence
-constexpr int kForwardThreads = TG_RF_THREADS, kForwardRows = TG_RF_ROWS;    // rows of a thread; at most 32, a bit each
-constexpr int kBackwardThreads = TG_RB_THREADS, kBackwardRows = TG_RB_ROWS;
-constexpr int kMapThreads = 256, kMapRows = 8;
-static_assert(kForwardThreads * kForwardRows == kChunk && kBackwardThreads * kBackwardRows == kChunk && kChunk % (kMapThreads * kMapRows) == 0, "");
+constexpr int kForwardThreads = 512, kForwardRows = 16;    // rows of a thread; at most 32, a bit each
+constexpr int kBackwardThreads = 1024, kBackwardRows = 8;
+constexpr int kMapThreads = 512;
+static_assert(kForwardThreads * kForwardRows == kChunk && kBackwardThreads * kBackwardRows == kChunk, "");
 constexpr uint32_t kClosedMap = 0xfffffffeu;  // in the place of a map's factor: closed
 
 // Rows in the order of the recurrence ("places"): row = reverse ? rows - 1 - place : place.  Columns are lanes: a lane has V successive
