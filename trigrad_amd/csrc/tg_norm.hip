@@ -2,134 +2,615 @@
 //
 //     xh = (x - mean) rstd,  z = weight xh + bias,  y = act(z),  mean and rstd of a sample's positions x (channels / groups)
 //     dz = dy act'(z),  dweight = sum dz xh,  dbias = sum dz,  dxh = weight dz,  dx = rstd (dxh - avg dxh - xh avg(dxh xh))
+//
+// Bound by memory traffic: x in and y out, x and dy in and dx out.  Two ways:
+//   held      a sample's groups fit the registers of a workgroup: read once, summed, written.  A workgroup has `teams` samples at a
+//             time and goes over many, so that the weights' gradients are summed in registers and come to few partial sums.
+//   streamed  a sample's rows are split over workgroups: one launch sums them, a small one joins the sums, one reads the rows again
+//             (from the last to the first, so that what the first launch read last is still near) and writes.
+// Sums are float32 (of at most a few hundred successive additions), joined in float64; all in a fixed order.
+#include <algorithm>
+#include <type_traits>
+
 #include "tg_elements.hpp"
 
 namespace tg {
 
 struct NormShape {
     int64_t samples, positions, channels, groups, width;  // width: channels of a group
-    int activation;
+    int activation, wide_weights;                          // wide_weights: weight and bias are tg_real whatever x is
     real eps;
 };
 
-// act(z) and act'(z)
-__device__ __forceinline__ void activate(int kind, real z, real &y, real &slope) {
-    if (kind == TG_ACTIVATION_RELU) {
-        y = z < 0 ? (real)0 : z;  // NaN stays
-        slope = z > 0 ? (real)1 : (real)0;
-    } else if (kind == TG_ACTIVATION_SILU) {
-        const real s = (real)1 / ((real)1 + exp(-z));
-        y = z * s;
-        slope = s * ((real)1 + z * ((real)1 - s));
-    } else if (kind == TG_ACTIVATION_GELU) {
+#ifdef TG_DOUBLE_PRECISION
+__device__ __forceinline__ real exp_norm(real z) { return exp(z); }
+__device__ __forceinline__ real inverse(real v) { return 1.0 / v; }
+#else
+__device__ __forceinline__ real exp_norm(real z) { return __builtin_amdgcn_exp2f(z * 1.44269504f); }
+__device__ __forceinline__ real inverse(real v) { return __builtin_amdgcn_rcpf(v); }
+#endif
+
+// act(z); Slope: act'(z)
+template <int Kind, bool Slope> __device__ __forceinline__ real activate(real z) {
+    if (Kind == TG_ACTIVATION_RELU) {
+        if (Slope) return z > 0 ? (real)1 : (real)0;
+        return z < 0 ? (real)0 : z;  // NaN stays
+    }
+    if (Kind == TG_ACTIVATION_SILU) {
+        const real s = inverse((real)1 + exp_norm(-z));
+        return Slope ? s * fma(z, (real)1 - s, (real)1) : z * s;
+    }
+    if (Kind == TG_ACTIVATION_GELU) {
         const real phi = (real)0.5 * erfc(z * (real)-0.70710678118654752440);
-        y = z * phi;
-        slope = phi + z * exp((real)-0.5 * z * z) * (real)0.39894228040143267794;
-    } else {
-        y = z;
-        slope = (real)1;
+        return Slope ? fma(z * exp_norm((real)-0.5 * z * z), (real)0.39894228040143267794, phi) : z * phi;
     }
+    return Slope ? (real)1 : z;
 }
 
-constexpr int kNormThreads = 256;
+template <class Call> __device__ __forceinline__ void by_activation(int kind, Call &&call) {
+    if (kind == TG_ACTIVATION_NONE) call(std::integral_constant<int, TG_ACTIVATION_NONE>());
+    else if (kind == TG_ACTIVATION_RELU) call(std::integral_constant<int, TG_ACTIVATION_RELU>());
+    else if (kind == TG_ACTIVATION_SILU) call(std::integral_constant<int, TG_ACTIVATION_SILU>());
+    else call(std::integral_constant<int, TG_ACTIVATION_GELU>());
+}
 
-__device__ __forceinline__ real block_sum(real v, real *shared) {
+template <class T, int V> __device__ __forceinline__ void load_weights(const NormShape &m, const void *from, int64_t at, real missing, real (&w)[V]) {
+#pragma unroll
+    for (int v = 0; v < V; v++)
+        w[v] = !from ? missing : sizeof(T) == sizeof(real) || m.wide_weights ? ((const real *)from)[at + v] : (real)((const T *)from)[at + v];
+}
+template <class T> __device__ __forceinline__ void store_weight(const NormShape &m, void *to, int64_t at, real w) {
+    if (sizeof(T) == sizeof(real) || m.wide_weights) ((real *)to)[at] = w;
+    else ((T *)to)[at] = (T)w;
+}
+
+// ---- held -------------------------------------------------------------------------------------
+
+// Threads of a workgroup: team (a sample each), row (of the sample's positions), unit (V successive channels) -- the unit fastest.  A slab is a run
+// of whole groups.
+struct Held {
+    int threads, units, rows, teams;
+    int unit_groups;   // units of a group
+    int slab_groups;   // groups of a slab
+    int64_t turns;     // sets of `teams` samples
+    int workgroups;    // that go over them
+    bool in_wave;      // a group's threads are neighbours in a wave, a power of two of them
+};
+
+// Sums of two values over the threads of each group: by neighbours, or through LDS, halving the members of all groups together.
+__device__ __forceinline__ void sum_groups(const Held &p, int segment, int member, int members, bool active, real &a, real &b, real *shared) {
+    if (p.in_wave) {
+        for (int d = members >> 1; d > 0; d >>= 1) {
+            a += __shfl_xor(a, d);
+            b += __shfl_xor(b, d);
+        }
+        return;
+    }
+    real *at = shared + 2 * (segment * members + member);
     __syncthreads();
-    shared[threadIdx.x] = v;
-    for (int n = kNormThreads / 2; n > 0; n >>= 1) {
+    if (active) {
+        at[0] = a;
+        at[1] = b;
+    }
+    for (int left = members; left > 1;) {
+        const int half = (left + 1) / 2;
         __syncthreads();
-        if ((int)threadIdx.x < n) shared[threadIdx.x] += shared[threadIdx.x + n];
+        if (active && member + half < left) {
+            at[0] += at[2 * half];
+            at[1] += at[2 * half + 1];
+        }
+        left = half;
     }
     __syncthreads();
-    return shared[0];
-}
-
-// A workgroup for a sample's group.
-template <class T, class S>
-__global__ __launch_bounds__(kNormThreads) void norm_forward_kernel(NormShape m, const T *__restrict__ x, const S *__restrict__ weight,
-                                                                    const S *__restrict__ bias, T *__restrict__ y,
-                                                                    real *__restrict__ statistics) {
-    __shared__ real shared[kNormThreads];
-    const int64_t n = blockIdx.x / m.groups, g = blockIdx.x % m.groups, count = m.positions * m.width;
-    const int64_t base = n * m.positions * m.channels + g * m.width;
-    const real pivot = (real)x[base];  // sums of differences from it: a mean far from zero takes no digits of the variance
-    real sum = 0;
-    for (int64_t i = threadIdx.x; i < count; i += kNormThreads) sum += (real)x[base + i / m.width * m.channels + i % m.width] - pivot;
-    const real mean = pivot + block_sum(sum, shared) / (real)count;
-    sum = 0;
-    for (int64_t i = threadIdx.x; i < count; i += kNormThreads) {
-        const real d = (real)x[base + i / m.width * m.channels + i % m.width] - mean;
-        sum += d * d;
-    }
-    const real rstd = (real)1 / sqrt(block_sum(sum, shared) / (real)count + m.eps);
-    if (threadIdx.x == 0) {
-        statistics[2 * (int64_t)blockIdx.x] = mean;
-        statistics[2 * (int64_t)blockIdx.x + 1] = rstd;
-    }
-    for (int64_t i = threadIdx.x; i < count; i += kNormThreads) {
-        const int64_t c = i % m.width, at = base + i / m.width * m.channels + c;
-        real z = ((real)x[at] - mean) * rstd, out, slope;
-        if (weight) z = z * (real)weight[g * m.width + c];
-        if (bias) z = z + (real)bias[g * m.width + c];
-        activate(m.activation, z, out, slope);
-        y[at] = (T)out;
+    if (active) {
+        a = shared[2 * segment * members];
+        b = shared[2 * segment * members + 1];
     }
 }
 
-template <class T, class S>
-__global__ __launch_bounds__(kNormThreads) void norm_backward_kernel(NormShape m, const T *__restrict__ x, const S *__restrict__ weight,
-                                                                     const S *__restrict__ bias, const real *__restrict__ statistics,
-                                                                     const T *__restrict__ grad_y, T *__restrict__ grad_x) {
-    __shared__ real shared[kNormThreads];
-    const int64_t n = blockIdx.x / m.groups, g = blockIdx.x % m.groups, count = m.positions * m.width;
-    const int64_t base = n * m.positions * m.channels + g * m.width;
-    const real mean = statistics[2 * (int64_t)blockIdx.x], rstd = statistics[2 * (int64_t)blockIdx.x + 1];
-    real sum = 0, product = 0;
-    for (int pass = 0; pass < 2; pass++) {
-        for (int64_t i = threadIdx.x; i < count; i += kNormThreads) {
-            const int64_t c = i % m.width, at = base + i / m.width * m.channels + c;
-            const real hat = ((real)x[at] - mean) * rstd, w = weight ? (real)weight[g * m.width + c] : (real)1;
-            real out, slope;
-            activate(m.activation, hat * w + (bias ? (real)bias[g * m.width + c] : (real)0), out, slope);
-            const real d = (real)grad_y[at] * slope * w;
-            if (pass == 0) {
-                sum += d;
-                product += d * hat;
-            } else {
-                grad_x[at] = (T)(rstd * (d - sum - hat * product));
+struct HeldPlace {
+    int unit, row, team, group, segment, member, members;
+    int64_t channel;
+    bool active;
+};
+template <int V> __device__ __forceinline__ HeldPlace held_place(const NormShape &m, const Held &p, int slab) {
+    HeldPlace t;
+    const int id = threadIdx.x, line = id / p.units;
+    t.unit = id - line * p.units;
+    t.team = line / p.rows;
+    t.row = line - t.team * p.rows;
+    t.active = t.team < p.teams;
+    t.group = t.unit / p.unit_groups;
+    t.segment = t.team * p.slab_groups + t.group;
+    t.member = t.row * p.unit_groups + t.unit - t.group * p.unit_groups;
+    t.members = p.rows * p.unit_groups;
+    t.channel = (int64_t)slab * p.slab_groups * m.width + (int64_t)t.unit * V;
+    // the last slab may have fewer groups
+    t.active = t.active && t.channel < m.channels;
+    t.group += slab * p.slab_groups;
+    return t;
+}
+
+template <class T, int V, int K>
+__global__ __launch_bounds__(1024) void norm_held_forward_kernel(NormShape m, Held p, const T *__restrict__ x, const void *__restrict__ weight,
+                                                                 const void *__restrict__ bias, T *__restrict__ y, real *__restrict__ statistics) {
+    extern __shared__ real shared[];
+    const int slab = (int)(blockIdx.x / (unsigned)p.workgroups), first_turn = (int)(blockIdx.x % (unsigned)p.workgroups);
+    const HeldPlace t = held_place<V>(m, p, slab);
+    const real per_value = (real)1 / (real)(m.positions * m.width);
+    real w[V], b[V];
+    load_weights<T, V>(m, weight, t.active ? t.channel : 0, (real)1, w);
+    load_weights<T, V>(m, bias, t.active ? t.channel : 0, (real)0, b);
+    for (int64_t turn = first_turn; turn < p.turns; turn += p.workgroups) {
+        const int64_t n = turn * p.teams + t.team;
+        const bool active = t.active && n < m.samples;
+        const int64_t base = active ? (n * m.positions + t.row) * m.channels + t.channel : 0, pitch = (int64_t)p.rows * m.channels;
+        const int rows = active ? (int)((m.positions - t.row + p.rows - 1) / p.rows) : 0;  // of the thread: at most K
+        Pack<T, V> in[K];
+#pragma unroll
+        for (int k = 0; k < K; k++) in[k] = load_pack<V>(x + (k < rows ? base + pitch * k : 0));
+        real sum = 0, none = 0;
+#pragma unroll
+        for (int k = 0; k < K; k++)
+#pragma unroll
+            for (int v = 0; v < V; v++) sum += k < rows ? in[k][v] : (real)0;
+        sum_groups(p, t.segment, t.member, t.members, active, sum, none, shared);
+        // about the mean of the first sum, again: what its rounding left, and the variance
+        const real about = sum * per_value;
+        real first = 0, second = 0;
+#pragma unroll
+        for (int k = 0; k < K; k++)
+#pragma unroll
+            for (int v = 0; v < V; v++) {
+                const real d = k < rows ? in[k][v] - about : (real)0;
+                first += d;
+                second = fma(d, d, second);
+            }
+        sum_groups(p, t.segment, t.member, t.members, active, first, second, shared);
+        const real rest = first * per_value, mean = about + rest, variance = fma(-rest, rest, second * per_value);
+        const real rstd = (real)1 / sqrt((variance < 0 ? (real)0 : variance) + m.eps);
+        if (!active) continue;
+        if (t.member == 0) {
+            statistics[2 * (n * m.groups + t.group)] = mean;
+            statistics[2 * (n * m.groups + t.group) + 1] = rstd;
+        }
+        by_activation(m.activation, [&](auto kind) {
+#pragma unroll
+            for (int k = 0; k < K; k++) {
+                if (k >= rows) break;
+                real out[V];
+#pragma unroll
+                for (int v = 0; v < V; v++) out[v] = activate<decltype(kind)::value, false>(fma((in[k][v] - mean) * rstd, w[v], b[v]));
+                store_pack<V>(y + base + pitch * k, out);
+            }
+        });
+    }
+}
+
+template <class T, int V, int K>
+__global__ __launch_bounds__(1024) void norm_held_backward_kernel(NormShape m, Held p, const T *__restrict__ x, const void *__restrict__ weight,
+                                                                  const void *__restrict__ bias, const real *__restrict__ statistics,
+                                                                  const T *__restrict__ grad_y, T *__restrict__ grad_x, real *__restrict__ partial) {
+    extern __shared__ real shared[];
+    const int slab = (int)(blockIdx.x / (unsigned)p.workgroups), first_turn = (int)(blockIdx.x % (unsigned)p.workgroups);
+    const HeldPlace t = held_place<V>(m, p, slab);
+    const real per_value = (real)1 / (real)(m.positions * m.width);
+    real w[V], b[V], dw[V], db[V];
+    load_weights<T, V>(m, weight, t.active ? t.channel : 0, (real)1, w);
+    load_weights<T, V>(m, bias, t.active ? t.channel : 0, (real)0, b);
+#pragma unroll
+    for (int v = 0; v < V; v++) dw[v] = db[v] = 0;
+    for (int64_t turn = first_turn; turn < p.turns; turn += p.workgroups) {
+        const int64_t n = turn * p.teams + t.team;
+        const bool active = t.active && n < m.samples;
+        const int64_t base = active ? (n * m.positions + t.row) * m.channels + t.channel : 0, pitch = (int64_t)p.rows * m.channels;
+        const int rows = active ? (int)((m.positions - t.row + p.rows - 1) / p.rows) : 0;
+        const int64_t of = active ? 2 * (n * m.groups + t.group) : 0;
+        Pack<T, V> in[K], dy[K];
+#pragma unroll
+        for (int k = 0; k < K; k++) in[k] = load_pack<V>(x + (k < rows ? base + pitch * k : 0));
+#pragma unroll
+        for (int k = 0; k < K; k++) dy[k] = load_pack<V>(grad_y + (k < rows ? base + pitch * k : 0));
+        const real mean = statistics[of], rstd = statistics[of + 1];
+        real sum = 0, product = 0;
+        // dz is computed again where it is used: its 32 bits are not held
+        by_activation(m.activation, [&](auto kind) {
+#pragma unroll
+            for (int k = 0; k < K; k++)
+#pragma unroll
+                for (int v = 0; v < V; v++) {
+                    const real hat = (in[k][v] - mean) * rstd;
+                    const real dz = k < rows ? dy[k][v] * activate<decltype(kind)::value, true>(fma(hat, w[v], b[v])) : (real)0;
+                    db[v] += dz;
+                    if (k < rows) dw[v] = fma(dz, hat, dw[v]);
+                    const real dh = dz * w[v];
+                    sum += dh;
+                    if (k < rows) product = fma(dh, hat, product);
+                }
+        });
+        if (!grad_x) continue;
+        sum_groups(p, t.segment, t.member, t.members, active, sum, product, shared);
+        sum *= per_value;
+        product *= per_value;
+        if (!active) continue;
+        by_activation(m.activation, [&](auto kind) {
+#pragma unroll
+            for (int k = 0; k < K; k++) {
+                if (k >= rows) break;
+                real out[V];
+#pragma unroll
+                for (int v = 0; v < V; v++) {
+                    const real hat = (in[k][v] - mean) * rstd;
+                    const real dh = dy[k][v] * activate<decltype(kind)::value, true>(fma(hat, w[v], b[v])) * w[v];
+                    out[v] = rstd * (dh - sum - hat * product);
+                }
+                store_pack<V>(grad_x + base + pitch * k, out);
+            }
+        });
+    }
+    if (!partial) return;
+    // sums over the threads that have the same channels
+    const int lines = p.teams * p.rows, columns = p.units * V;
+    real *at = shared;
+#pragma unroll
+    for (int which = 0; which < 2; which++) {
+        __syncthreads();
+#pragma unroll
+        for (int v = 0; v < V; v++)
+            if (t.active) at[(threadIdx.x / p.units) * columns + t.unit * V + v] = which ? db[v] : dw[v];
+        __syncthreads();
+        for (int c = threadIdx.x; c < columns; c += p.threads) {
+            const int64_t channel = (int64_t)slab * p.slab_groups * m.width + c;
+            if (channel >= m.channels) continue;
+            real sum = 0;
+            for (int i = 0; i < lines; i++) sum += at[i * columns + c];
+            partial[((int64_t)which * p.workgroups + first_turn) * m.channels + channel] = sum;
+        }
+    }
+}
+
+// ---- streamed -----------------------------------------------------------------------------------
+
+struct Streamed {
+    int units, rows, tiles;  // units of a row that a workgroup has, its rows at a time, workgroups side by side on a row
+    int splits;              // workgroups one after another on a sample
+    int64_t split_rows;
+};
+constexpr int kNormThreads = 256, kNormAhead = 8;
+
+struct StreamedPlace {
+    int unit, row;
+    int64_t channel, begin, end;
+    bool active;
+};
+template <int V> __device__ __forceinline__ StreamedPlace streamed_place(const NormShape &m, const Streamed &p, int split, int tile) {
+    StreamedPlace t;
+    t.row = threadIdx.x / p.units;
+    t.unit = threadIdx.x - t.row * p.units;
+    t.channel = ((int64_t)tile * p.units + t.unit) * V;
+    t.active = t.row < p.rows && t.channel < m.channels;
+    t.begin = min(split * p.split_rows, m.positions);
+    t.end = min(t.begin + p.split_rows, m.positions);
+    return t;
+}
+
+// The rows of a workgroup's split, kNormAhead of a thread at a time: call(in[], how many).
+template <class T, int V, class Call>
+__device__ __forceinline__ void over_rows(const NormShape &m, const Streamed &p, const StreamedPlace &t, const T *x, Call &&call) {
+    for (int64_t r = t.begin + t.row; r < t.end; r += (int64_t)kNormAhead * p.rows) {
+        const int there = (int)min((int64_t)kNormAhead, (t.end - r + p.rows - 1) / p.rows);
+        call(x + r * m.channels + t.channel, there, r);
+    }
+}
+
+// A tile's sums of two values by channel, summed by group: a wave each.  A group that goes on in the next tile has a sum there too.
+// [sample][split][tile][group][2]
+__device__ __forceinline__ void group_sums(const NormShape &m, const Streamed &p, int64_t n, int split, int tile, int columns, const real *first,
+                                           const real *second, real *partial) {
+    const int lane = threadIdx.x & (kWave - 1);
+    const int64_t low = (int64_t)tile * columns, high = min(low + columns, m.channels), g0 = low / m.width, g1 = (high - 1) / m.width;
+    for (int64_t i = threadIdx.x / kWave; i < 2 * (g1 - g0 + 1); i += kNormThreads / kWave) {
+        const int64_t g = g0 + (i >> 1);
+        const real *from = i & 1 ? second : first;
+        real sum = 0;
+        for (int64_t c = max(low, g * m.width) + lane; c < min(high, (g + 1) * m.width); c += kWave) sum += from[c - low];
+        for (int d = kWave / 2; d > 0; d >>= 1) sum += __shfl_xor(sum, d);
+        if (lane == 0) partial[((((n * p.splits + split) * p.tiles + tile) * m.groups + g) << 1) + (i & 1)] = sum;
+    }
+}
+
+// The sum over the splits and tiles of those of a group, by a wave, in every lane.
+template <int V> __device__ __forceinline__ void sum_splits(const NormShape &m, const Streamed &p, int64_t n, int64_t g, const real *partial, double &first,
+                                                            double &second) {
+    const int64_t columns = (int64_t)p.units * V;
+    const int t0 = (int)(g * m.width / columns), t1 = (int)(((g + 1) * m.width - 1) / columns);
+    first = second = 0;
+    for (int s = threadIdx.x & (kWave - 1); s < p.splits; s += kWave)
+        for (int t = t0; t <= t1; t++) {
+            const real *at = partial + (((((n * p.splits + s) * p.tiles + t) * m.groups) + g) << 1);
+            first += at[0];
+            second += at[1];
+        }
+    for (int d = kWave / 2; d > 0; d >>= 1) {
+        first += __shfl_xor(first, d);
+        second += __shfl_xor(second, d);
+    }
+}
+
+// Sums of x - p and its square by sample, split and group, around the group's first value p.  [sample][split][group][2]
+template <class T, int V>
+__global__ __launch_bounds__(kNormThreads) void norm_sums_kernel(NormShape m, Streamed p, const T *__restrict__ x, real *__restrict__ partial) {
+    __shared__ real shared[2][kNormThreads * V];
+    const int split = (int)(blockIdx.x % (unsigned)p.splits), tile = (int)(blockIdx.x / (unsigned)p.splits % (unsigned)p.tiles);
+    const int64_t n = blockIdx.x / (unsigned)p.splits / (unsigned)p.tiles;
+    const StreamedPlace t = streamed_place<V>(m, p, split, tile);
+    x += n * m.positions * m.channels;
+    real pivot[V], first[V], second[V];
+#pragma unroll
+    for (int v = 0; v < V; v++) {
+        pivot[v] = t.active ? (real)x[(t.channel + v) / m.width * m.width] : (real)0;
+        first[v] = second[v] = 0;
+    }
+    const int64_t pitch = (int64_t)p.rows * m.channels;
+    if (t.active)
+        over_rows<T, V>(m, p, t, x, [&](const T *from, int there, int64_t) {
+            Pack<T, V> in[kNormAhead];
+#pragma unroll
+            for (int k = 0; k < kNormAhead; k++) in[k] = load_pack<V>(from + (k < there ? pitch * k : 0));
+#pragma unroll
+            for (int k = 0; k < kNormAhead; k++)
+#pragma unroll
+                for (int v = 0; v < V; v++) {
+                    const real d = k < there ? in[k][v] - pivot[v] : (real)0;
+                    first[v] += d;
+                    second[v] = fma(d, d, second[v]);
+                }
+        });
+#pragma unroll
+    for (int v = 0; v < V; v++) {
+        shared[0][threadIdx.x * V + v] = first[v];
+        shared[1][threadIdx.x * V + v] = second[v];
+    }
+    __syncthreads();
+    const int columns = p.units * V;
+    for (int c = threadIdx.x; c < 2 * columns; c += kNormThreads) {
+        real *at = shared[c >= columns] + (c >= columns ? c - columns : c);
+        real sum = at[0];
+        for (int i = 1; i < p.rows; i++) sum += at[i * columns];
+        at[0] = sum;
+    }
+    __syncthreads();
+    group_sums(m, p, n, split, tile, columns, shared[0], shared[1], partial);
+}
+
+// mean and rstd of each group: a wave each
+template <class T, int V>
+__global__ __launch_bounds__(kNormThreads) void norm_statistics_kernel(NormShape m, Streamed p, const T *__restrict__ x, const real *__restrict__ partial,
+                                                                       real *__restrict__ statistics) {
+    const int lane = threadIdx.x & (kWave - 1);
+    const int64_t id = (int64_t)blockIdx.x * (kNormThreads / kWave) + threadIdx.x / kWave;
+    if (id >= m.samples * m.groups) return;
+    const int64_t n = id / m.groups, g = id % m.groups;
+    double first, second;
+    sum_splits<V>(m, p, n, g, partial, first, second);
+    if (lane != 0) return;
+    const double count = (double)m.positions * (double)m.width, rest = first / count, variance = second / count - rest * rest;
+    statistics[2 * id] = (real)((double)(real)x[n * m.positions * m.channels + g * m.width] + rest);
+    statistics[2 * id + 1] = (real)(1.0 / sqrt((variance < 0 ? 0.0 : variance) + (double)m.eps));
+}
+
+template <class T, int V>
+__global__ __launch_bounds__(kNormThreads) void norm_apply_kernel(NormShape m, Streamed p, const T *__restrict__ x, const void *__restrict__ weight,
+                                                                  const void *__restrict__ bias, const real *__restrict__ statistics,
+                                                                  T *__restrict__ y) {
+    const unsigned turned = gridDim.x - 1 - blockIdx.x;
+    const int64_t n = turned / (unsigned)p.splits / (unsigned)p.tiles;
+    const StreamedPlace t = streamed_place<V>(m, p, (int)(turned % (unsigned)p.splits), (int)(turned / (unsigned)p.splits % (unsigned)p.tiles));
+    if (!t.active) return;
+    x += n * m.positions * m.channels;
+    y += n * m.positions * m.channels;
+    real w[V], b[V], mean[V], rstd[V];
+    load_weights<T, V>(m, weight, t.channel, (real)1, w);
+    load_weights<T, V>(m, bias, t.channel, (real)0, b);
+#pragma unroll
+    for (int v = 0; v < V; v++) {
+        const int64_t of = 2 * (n * m.groups + (t.channel + v) / m.width);
+        mean[v] = statistics[of];
+        rstd[v] = statistics[of + 1];
+    }
+    const int64_t pitch = (int64_t)p.rows * m.channels;
+    by_activation(m.activation, [&](auto kind) {
+        over_rows<T, V>(m, p, t, x, [&](const T *from, int there, int64_t r) {
+            Pack<T, V> in[kNormAhead];
+#pragma unroll
+            for (int k = 0; k < kNormAhead; k++) in[k] = load_pack<V>(from + (k < there ? pitch * k : 0));
+            T *to = y + r * m.channels + t.channel;
+#pragma unroll
+            for (int k = 0; k < kNormAhead; k++) {
+                if (k >= there) break;
+                real out[V];
+#pragma unroll
+                for (int v = 0; v < V; v++) out[v] = activate<decltype(kind)::value, false>(fma((in[k][v] - mean[v]) * rstd[v], w[v], b[v]));
+                store_pack<V>(to + pitch * k, out);
+            }
+        });
+    });
+}
+
+// Sums of dz and dz xh by sample, split and channel, [sample][split][2][channel], and of these times the weight by group.
+constexpr int kNormPairs = 4;  // rows of a thread at a time where there are two arrays to read
+template <class T, int V>
+__global__ __launch_bounds__(kNormThreads) void norm_gradient_sums_kernel(NormShape m, Streamed p, const T *__restrict__ x, const void *__restrict__ weight,
+                                                                          const void *__restrict__ bias, const real *__restrict__ statistics,
+                                                                          const T *__restrict__ grad_y, real *__restrict__ partial, real *__restrict__ group_partial) {
+    __shared__ real shared[2][kNormThreads * V];
+    const int split = (int)(blockIdx.x % (unsigned)p.splits), tile = (int)(blockIdx.x / (unsigned)p.splits % (unsigned)p.tiles);
+    const int64_t n = blockIdx.x / (unsigned)p.splits / (unsigned)p.tiles;
+    const StreamedPlace t = streamed_place<V>(m, p, split, tile);
+    real sum[V], product[V];
+#pragma unroll
+    for (int v = 0; v < V; v++) sum[v] = product[v] = 0;
+    if (t.active) {
+        real w[V], b[V], mean[V], rstd[V];
+        load_weights<T, V>(m, weight, t.channel, (real)1, w);
+        load_weights<T, V>(m, bias, t.channel, (real)0, b);
+#pragma unroll
+        for (int v = 0; v < V; v++) {
+            const int64_t of = 2 * (n * m.groups + (t.channel + v) / m.width);
+            mean[v] = statistics[of];
+            rstd[v] = statistics[of + 1];
+        }
+        const int64_t pitch = (int64_t)p.rows * m.channels;
+        by_activation(m.activation, [&](auto kind) {
+            for (int64_t r = t.begin + t.row; r < t.end; r += (int64_t)kNormPairs * p.rows) {
+                const int there = (int)min((int64_t)kNormPairs, (t.end - r + p.rows - 1) / p.rows);
+                const int64_t at = (n * m.positions + r) * m.channels + t.channel;
+                Pack<T, V> in[kNormPairs], dy[kNormPairs];
+#pragma unroll
+                for (int k = 0; k < kNormPairs; k++) {
+                    in[k] = load_pack<V>(x + at + (k < there ? pitch * k : 0));
+                    dy[k] = load_pack<V>(grad_y + at + (k < there ? pitch * k : 0));
+                }
+#pragma unroll
+                for (int k = 0; k < kNormPairs; k++)
+#pragma unroll
+                    for (int v = 0; v < V; v++) {
+                        const real hat = (in[k][v] - mean[v]) * rstd[v];
+                        const real dz = dy[k][v] * activate<decltype(kind)::value, true>(fma(hat, w[v], b[v]));
+                        sum[v] += k < there ? dz : (real)0;
+                        if (k < there) product[v] = fma(dz, hat, product[v]);
+                    }
+            }
+        });
+    }
+#pragma unroll
+    for (int v = 0; v < V; v++) {
+        shared[0][threadIdx.x * V + v] = sum[v];
+        shared[1][threadIdx.x * V + v] = product[v];
+    }
+    __syncthreads();
+    const int columns = p.units * V;
+    for (int c = threadIdx.x; c < 2 * columns; c += kNormThreads) {
+        const int which = c >= columns, column = which ? c - columns : c;
+        const int64_t channel = (int64_t)tile * columns + column;
+        if (channel >= m.channels) continue;
+        real *at = shared[which] + column;
+        real total = at[0];
+        for (int i = 1; i < p.rows; i++) total += at[i * columns];
+        if (partial) partial[((n * p.splits + split) * 2 + which) * m.channels + channel] = total;
+        real w[1];
+        load_weights<T, 1>(m, weight, channel, (real)1, w);
+        at[0] = total * w[0];
+    }
+    __syncthreads();
+    group_sums(m, p, n, split, tile, columns, shared[0], shared[1], group_partial);
+}
+
+// Sums of the weights' gradients over the parts, at the given strides: 64 threads a channel.
+constexpr int kJoinThreads = 1024, kJoinColumns = 16, kJoinLines = kJoinThreads / kJoinColumns;
+template <class T>
+__device__ __forceinline__ void join_channel(const NormShape &m, int64_t parts, int64_t stride, int64_t which_stride, int64_t block, const real *partial,
+                                             int weight_at, void *grad_weight, void *grad_bias, double (*shared)[kJoinThreads]) {
+    const int column = threadIdx.x % kJoinColumns, line = threadIdx.x / kJoinColumns;
+    const int64_t channel = block * kJoinColumns + column;
+    double sum[2] = {0, 0};
+    if (channel < m.channels)
+        for (int64_t i = line; i < parts; i += kJoinLines) {
+            sum[0] += partial[i * stride + channel];
+            sum[1] += partial[i * stride + which_stride + channel];
+        }
+    shared[0][threadIdx.x] = sum[0];
+    shared[1][threadIdx.x] = sum[1];
+    for (int left = kJoinLines / 2; left > 0; left >>= 1) {
+        __syncthreads();
+        if (line < left) {
+            shared[0][threadIdx.x] += shared[0][threadIdx.x + left * kJoinColumns];
+            shared[1][threadIdx.x] += shared[1][threadIdx.x + left * kJoinColumns];
+        }
+    }
+    __syncthreads();
+    if (line < 2 && channel < m.channels) {
+        void *to = line == weight_at ? grad_weight : grad_bias;
+        if (to) store_weight<T>(m, to, channel, (real)shared[line][column]);
+    }
+}
+
+// By group avg dxh and avg(dxh xh), a wave each; then the weights' gradients.
+template <class T, int V>
+__global__ __launch_bounds__(kJoinThreads) void norm_join_kernel(NormShape m, Streamed p, const real *__restrict__ partial,
+                                                                 const real *__restrict__ group_partial, real *__restrict__ averages,
+                                                                 int64_t group_blocks, void *__restrict__ grad_weight, void *__restrict__ grad_bias) {
+    __shared__ double shared[2][kJoinThreads];
+    if (blockIdx.x < group_blocks) {
+        const int64_t id = (int64_t)blockIdx.x * (kJoinThreads / kWave) + threadIdx.x / kWave;
+        if (id >= m.samples * m.groups) return;
+        double sum, product;
+        sum_splits<V>(m, p, id / m.groups, id % m.groups, group_partial, sum, product);
+        const double count = (double)m.positions * (double)m.width;
+        if ((threadIdx.x & (kWave - 1)) == 0) {
+            averages[2 * id] = (real)(sum / count);
+            averages[2 * id + 1] = (real)(product / count);
+        }
+    } else {
+        join_channel<T>(m, m.samples * p.splits, 2 * m.channels, m.channels, (int64_t)blockIdx.x - group_blocks, partial, 1, grad_weight, grad_bias, shared);
+    }
+}
+
+template <class T>
+__global__ __launch_bounds__(kJoinThreads) void norm_join_held_kernel(NormShape m, int64_t parts, const real *__restrict__ partial,
+                                                                      void *__restrict__ grad_weight, void *__restrict__ grad_bias) {
+    __shared__ double shared[2][kJoinThreads];
+    join_channel<T>(m, parts, m.channels, parts * m.channels, blockIdx.x, partial, 0, grad_weight, grad_bias, shared);
+}
+
+template <class T, int V>
+__global__ __launch_bounds__(kNormThreads) void norm_gradient_kernel(NormShape m, Streamed p, const T *__restrict__ x, const void *__restrict__ weight,
+                                                                     const void *__restrict__ bias, const real *__restrict__ statistics,
+                                                                     const real *__restrict__ averages, const T *__restrict__ grad_y,
+                                                                     T *__restrict__ grad_x) {
+    const unsigned turned = gridDim.x - 1 - blockIdx.x;
+    const int64_t n = turned / (unsigned)p.splits / (unsigned)p.tiles;
+    const StreamedPlace t = streamed_place<V>(m, p, (int)(turned % (unsigned)p.splits), (int)(turned / (unsigned)p.splits % (unsigned)p.tiles));
+    if (!t.active) return;
+    real w[V], b[V], mean[V], rstd[V], sum[V], product[V];
+    load_weights<T, V>(m, weight, t.channel, (real)1, w);
+    load_weights<T, V>(m, bias, t.channel, (real)0, b);
+#pragma unroll
+    for (int v = 0; v < V; v++) {
+        const int64_t of = 2 * (n * m.groups + (t.channel + v) / m.width);
+        mean[v] = statistics[of];
+        rstd[v] = statistics[of + 1];
+        sum[v] = averages[of];
+        product[v] = averages[of + 1];
+    }
+    const int64_t pitch = (int64_t)p.rows * m.channels;
+    by_activation(m.activation, [&](auto kind) {
+        for (int64_t r = t.begin + t.row; r < t.end; r += (int64_t)kNormPairs * p.rows) {
+            const int there = (int)min((int64_t)kNormPairs, (t.end - r + p.rows - 1) / p.rows);
+            const int64_t at = (n * m.positions + r) * m.channels + t.channel;
+            Pack<T, V> in[kNormPairs], dy[kNormPairs];
+#pragma unroll
+            for (int k = 0; k < kNormPairs; k++) {
+                in[k] = load_pack<V>(x + at + (k < there ? pitch * k : 0));
+                dy[k] = load_pack<V>(grad_y + at + (k < there ? pitch * k : 0));
+            }
+#pragma unroll
+            for (int k = 0; k < kNormPairs; k++) {
+                if (k >= there) break;
+                real out[V];
+#pragma unroll
+                for (int v = 0; v < V; v++) {
+                    const real hat = (in[k][v] - mean[v]) * rstd[v];
+                    const real dh = dy[k][v] * activate<decltype(kind)::value, true>(fma(hat, w[v], b[v])) * w[v];
+                    out[v] = rstd[v] * (dh - sum[v] - hat * product[v]);
+                }
+                store_pack<V>(grad_x + at + pitch * k, out);
             }
         }
-        if (pass == 0) {
-            sum = block_sum(sum, shared) / (real)count;
-            product = block_sum(product, shared) / (real)count;
-        }
-    }
+    });
 }
 
-// A workgroup for a channel.
-template <class T, class S>
-__global__ __launch_bounds__(kNormThreads) void norm_weights_kernel(NormShape m, const T *__restrict__ x, const S *__restrict__ weight,
-                                                                    const S *__restrict__ bias, const real *__restrict__ statistics,
-                                                                    const T *__restrict__ grad_y, S *__restrict__ grad_weight,
-                                                                    S *__restrict__ grad_bias) {
-    __shared__ real shared[kNormThreads];
-    const int64_t c = blockIdx.x, g = c / m.width;
-    real sum = 0, product = 0;
-    for (int64_t i = threadIdx.x; i < m.samples * m.positions; i += kNormThreads) {
-        const int64_t n = i / m.positions, at = i * m.channels + c;
-        const real hat = ((real)x[at] - statistics[2 * (n * m.groups + g)]) * statistics[2 * (n * m.groups + g) + 1];
-        real out, slope;
-        activate(m.activation, hat * (weight ? (real)weight[c] : (real)1) + (bias ? (real)bias[c] : (real)0), out, slope);
-        sum += (real)grad_y[at] * slope;
-        product += (real)grad_y[at] * slope * hat;
-    }
-    sum = block_sum(sum, shared);
-    product = block_sum(product, shared);
-    if (threadIdx.x == 0) {
-        if (grad_weight) grad_weight[c] = (S)product;
-        if (grad_bias) grad_bias[c] = (S)sum;
-    }
-}
+// ---- host -----------------------------------------------------------------------------------------
 
 static int check_norm(const char *fn, const tg_norm *n, NormShape &m) {
     if (!n) {
@@ -156,8 +637,127 @@ static int check_norm(const char *fn, const tg_norm *n, NormShape &m) {
     m.groups = n->groups;
     m.width = n->channels / n->groups;
     m.activation = (int)n->activation;
+    m.wide_weights = n->weight_type == kRealType;
     m.eps = (real)n->eps;
     return 0;
+}
+
+// Elements of an access: all 16 bytes, two, or one: what divides `run` and is aligned.
+static int vector_of(int64_t run, int64_t bytes, std::initializer_list<const void *> pointers) {
+    for (int v : {(int)(16 / bytes), 2}) {
+        bool fits = run % v == 0 && (v == 2 ? bytes == 2 : true);
+        for (const void *p : pointers) fits = fits && (uintptr_t)p % (uintptr_t)(v * bytes) == 0;
+        if (fits) return v;
+    }
+    return 1;
+}
+
+template <class Call> static int by_vector(int64_t type, int vector, Call &&call) {
+    const auto with = [&](auto t) {
+        using widest = std::integral_constant<int, 16 / (int)sizeof(t)>;
+        using two = std::integral_constant<int, 2>;
+        using one = std::integral_constant<int, 1>;
+        if (vector == widest::value) return call(t, widest());
+        if (sizeof(t) == 2 && vector == 2) return call(t, std::conditional_t<sizeof(t) == 2, two, one>());
+        return call(t, one());
+    };
+#ifdef TG_DOUBLE_PRECISION
+    (void)type;
+    return with(double());
+#else
+    return type == TG_TYPE_F32 ? with(float()) : type == TG_TYPE_F16 ? with(half_t()) : with(bf16_t());
+#endif
+}
+
+constexpr int kHeldRows = 8;        // accesses of a thread that are held
+constexpr int kHeldWorkgroups = 512;  // at most, where they sum the weights' gradients
+
+// A slab of groups whose rows are 64 bytes or more, if a workgroup can hold it; threads == 0: it cannot.
+static Held held_of(const NormShape &m, int vector, int64_t bytes) {
+    Held p = {};
+    const int64_t row = m.width * bytes;
+    p.slab_groups = (int)std::min<int64_t>(m.groups, std::max<int64_t>(1, 64 / row));
+    // all of a row where that is little: its neighbours are read by the same workgroup
+    while (p.slab_groups < m.groups && (int64_t)p.slab_groups * m.width * m.positions <= 1024 * vector / 2) p.slab_groups = (int)std::min<int64_t>(m.groups, p.slab_groups * 2);
+    p.unit_groups = (int)(m.width / vector);
+    if (m.width / vector > 1024) return p;
+    const int64_t units = (int64_t)p.slab_groups * p.unit_groups;
+    if (units > 1024) return p;
+    p.units = (int)units;
+    const int64_t most = 1024 / units;  // rows at a time of the largest workgroup
+    if (m.positions > most * kHeldRows) return p;
+    // few accesses a thread where there are few positions, more where it takes them
+    p.rows = (int)std::min<int64_t>(m.positions, m.positions <= most ? m.positions : most);
+    const int line = p.rows * p.units;
+    p.teams = (int)std::max<int64_t>(1, std::min<int64_t>(m.samples, (line < 256 ? 256 : 1024) / line));
+    p.threads = (p.teams * line + kWave - 1) / kWave * kWave;
+    p.turns = ceil_div64(m.samples, p.teams);
+    p.in_wave = p.rows == 1 && (p.unit_groups & (p.unit_groups - 1)) == 0 && p.unit_groups <= kWave;
+    return p;
+}
+static size_t held_lds(const Held &p, int vector, bool backward) {
+    return sizeof(real) * std::max<size_t>(p.in_wave ? 0 : 2 * (size_t)p.threads, backward ? (size_t)p.threads * vector : 0);
+}
+
+static Streamed streamed_of(const NormShape &m, int vector) {
+    Streamed p = {};
+    const int64_t units = m.channels / vector;
+    p.units = (int)std::min<int64_t>(units, kNormThreads);
+    p.tiles = (int)ceil_div64(units, p.units);
+    p.rows = kNormThreads / p.units;
+    // about eight workgroups a CU, of no fewer rows than a thread reads ahead
+    const int64_t most = std::max<int64_t>(1, ceil_div64(m.positions, (int64_t)p.rows * kNormAhead));
+    p.splits = (int)std::min<int64_t>(most, std::max<int64_t>(1, ceil_div64(2048, m.samples * p.tiles)));
+    p.split_rows = ceil_div64(ceil_div64(m.positions, p.splits), p.rows) * p.rows;
+    p.splits = (int)ceil_div64(m.positions, p.split_rows);
+    return p;
+}
+
+struct NormPlan {
+    bool held;
+    int vector;
+    Held h;
+    Streamed s;
+    int64_t parts, partial, by_group, averages;  // partial sums by channel and by group, averages: elements
+    int64_t blocks;
+};
+static NormPlan plan_of(const NormShape &m, int64_t type, bool backward, bool aligned_only, std::initializer_list<const void *> pointers) {
+    NormPlan p = {};
+    const int64_t bytes = type_bytes(type);
+    p.vector = aligned_only ? vector_of(m.width, bytes, {}) : vector_of(m.width, bytes, pointers);
+    p.h = held_of(m, p.vector, bytes);
+    const int64_t slabs = p.h.slab_groups ? ceil_div64(m.groups, p.h.slab_groups) : 0;
+    // few workgroups leave most of the chip idle: a sample is then better split
+    p.held = p.h.threads > 0 && (p.h.turns * slabs >= 128 || m.samples * m.positions * m.channels * bytes <= (1 << 18));
+    if (p.held) {
+        p.h.workgroups = (int)std::min<int64_t>(p.h.turns, std::max<int64_t>(1, (backward ? kHeldWorkgroups : 8192) / slabs));
+        p.parts = backward ? p.h.workgroups : 0;
+        p.partial = 2 * p.parts * m.channels;
+        p.blocks = p.h.workgroups * slabs;
+        return p;
+    }
+    p.vector = aligned_only ? vector_of(m.channels, bytes, {}) : vector_of(m.channels, bytes, pointers);
+    p.s = streamed_of(m, p.vector);
+    p.parts = m.samples * p.s.splits;
+    p.partial = backward ? p.parts * 2 * m.channels : 0;
+    p.by_group = p.parts * p.s.tiles * m.groups * 2;
+    p.blocks = p.parts * p.s.tiles;
+    p.averages = backward ? m.samples * m.groups * 2 : 0;
+    return p;
+}
+static int64_t norm_bytes(const NormPlan &p) { return (p.partial + p.by_group + p.averages) * (int64_t)sizeof(real); }
+
+static int too_many(const char *fn) {
+    set_error("%s: too many samples", fn);
+    return TG_E_ARG;
+}
+
+// Of the workspace, whatever the alignment of the tensors turns out to be.
+static int64_t norm_room(const NormShape &m, int64_t type, bool backward) {
+    if (m.samples == 0 || m.positions == 0) return 0;
+    int64_t most = norm_bytes(plan_of(m, type, backward, true, {}));
+    for (int by : {1, 2, 4, 8}) most = std::max(most, norm_bytes(plan_of(m, type, backward, false, {(const void *)(uintptr_t)(16 + by)})));
+    return most;
 }
 
 }  // namespace tg
@@ -170,7 +770,8 @@ extern "C" int tg_group_norm_sizes(const tg_norm *n, int64_t out[2]) {
         set_error("tg_group_norm_sizes: null pointer");
         return TG_E_ARG;
     }
-    out[0] = out[1] = 0;
+    out[0] = norm_room(m, n->type, false);
+    out[1] = norm_room(m, n->type, true);
     return 0;
 }
 
@@ -184,37 +785,100 @@ extern "C" int tg_group_norm_forward(const tg_norm *n) {
         set_error("%s: null pointer", fn);
         return TG_E_ARG;
     }
-    return by_types(n->type, n->weight_type, [&](auto t, auto s) {
+    const NormPlan p = plan_of(m, n->type, false, false, {n->x, n->y});
+    if (p.blocks >= (1 << 22)) return too_many(fn);
+    if (norm_bytes(p) > 0 && (!n->workspace || n->workspace_bytes < norm_bytes(p))) {
+        set_error("%s: workspace of %lld bytes, %lld needed", fn, (long long)n->workspace_bytes, (long long)norm_bytes(p));
+        return TG_E_WORKSPACE;
+    }
+    hipStream_t stream = (hipStream_t)n->stream;
+    return by_vector(n->type, p.vector, [&](auto t, auto v) {
         using T = decltype(t);
-        using S = decltype(s);
-        TG_LAUNCH_AS("norm_forward", (norm_forward_kernel<T, S>), dim3((unsigned)(m.samples * m.groups)), dim3(kNormThreads), 0,
-                     (hipStream_t)n->stream, m, (const T *)n->x, (const S *)n->weight, (const S *)n->bias, (T *)n->y, n->statistics);
+        constexpr int V = decltype(v)::value;
+        const T *x = (const T *)n->x;
+        if (p.held) {
+            const dim3 grid((unsigned)p.blocks), block((unsigned)p.h.threads);
+            const size_t lds = held_lds(p.h, V, false);
+            if (m.positions <= p.h.rows)
+                TG_LAUNCH_AS("norm_forward", (norm_held_forward_kernel<T, V, 1>), grid, block, lds, stream, m, p.h, x, n->weight, n->bias, (T *)n->y,
+                             n->statistics);
+            else
+                TG_LAUNCH_AS("norm_forward", (norm_held_forward_kernel<T, V, kHeldRows>), grid, block, lds, stream, m, p.h, x, n->weight, n->bias,
+                             (T *)n->y, n->statistics);
+            return check_launch(fn);
+        }
+        const dim3 grid((unsigned)p.blocks), block(kNormThreads);
+        real *partial = (real *)n->workspace;
+        TG_LAUNCH_AS("norm_sums", (norm_sums_kernel<T, V>), grid, block, 0, stream, m, p.s, x, partial);
+        TG_LAUNCH_AS("norm_statistics", (norm_statistics_kernel<T, V>), dim3((unsigned)ceil_div64(m.samples * m.groups, kNormThreads / kWave)), block, 0,
+                     stream, m, p.s, x, partial, n->statistics);
+        TG_LAUNCH_AS("norm_apply", (norm_apply_kernel<T, V>), grid, block, 0, stream, m, p.s, x, n->weight, n->bias, n->statistics, (T *)n->y);
         return check_launch(fn);
     });
 }
+
+namespace tg {
+template <class T> __global__ __launch_bounds__(kNormThreads) void norm_no_gradient_kernel(NormShape m, void *grad_weight, void *grad_bias) {
+    for (int64_t c = threadIdx.x; c < m.channels; c += kNormThreads) {
+        if (grad_weight) store_weight<T>(m, grad_weight, c, (real)0);
+        if (grad_bias) store_weight<T>(m, grad_bias, c, (real)0);
+    }
+}
+}  // namespace tg
 
 extern "C" int tg_group_norm_backward(const tg_norm *n) {
     using namespace tg;
     const char *fn = "tg_group_norm_backward";
     NormShape m;
     if (const int code = check_norm(fn, n, m)) return code;
-    const bool empty = m.samples == 0 || m.positions == 0;
-    if ((empty || !n->grad_x) && !n->grad_weight && !n->grad_bias) return 0;
-    if (!empty && (!n->x || !n->grad_y || !n->statistics)) {
+    const bool empty = m.samples == 0 || m.positions == 0, weights = n->grad_weight || n->grad_bias;
+    if ((empty || !n->grad_x) && !weights) return 0;
+    hipStream_t stream = (hipStream_t)n->stream;
+    if (empty)
+        return by_vector(n->type, 1, [&](auto t, auto) {
+            TG_LAUNCH_AS("norm_no_gradient", (norm_no_gradient_kernel<decltype(t)>), dim3(1), dim3(kNormThreads), 0, stream, m, n->grad_weight, n->grad_bias);
+            return check_launch(fn);
+        });
+    if (!n->x || !n->grad_y || !n->statistics) {
         set_error("%s: null pointer", fn);
         return TG_E_ARG;
     }
-    return by_types(n->type, n->weight_type, [&](auto t, auto s) {
+    const NormPlan p = plan_of(m, n->type, true, false, {n->x, n->grad_y, n->grad_x});
+    if (p.blocks >= (1 << 22)) return too_many(fn);
+    if (!n->workspace || n->workspace_bytes < norm_bytes(p)) {
+        set_error("%s: workspace of %lld bytes, %lld needed", fn, (long long)n->workspace_bytes, (long long)norm_bytes(p));
+        return TG_E_WORKSPACE;
+    }
+    return by_vector(n->type, p.vector, [&](auto t, auto v) {
         using T = decltype(t);
-        using S = decltype(s);
-        hipStream_t stream = (hipStream_t)n->stream;
-        if (n->grad_x && !empty)
-            TG_LAUNCH_AS("norm_backward", (norm_backward_kernel<T, S>), dim3((unsigned)(m.samples * m.groups)), dim3(kNormThreads), 0, stream, m,
-                         (const T *)n->x, (const S *)n->weight, (const S *)n->bias, n->statistics, (const T *)n->grad_y, (T *)n->grad_x);
-        if (n->grad_weight || n->grad_bias)
-            TG_LAUNCH_AS("norm_weights", (norm_weights_kernel<T, S>), dim3((unsigned)m.channels), dim3(kNormThreads), 0, stream, m,
-                         (const T *)n->x, (const S *)n->weight, (const S *)n->bias, n->statistics, (const T *)n->grad_y,
-                         (S *)n->grad_weight, (S *)n->grad_bias);
+        constexpr int V = decltype(v)::value;
+        const T *x = (const T *)n->x, *dy = (const T *)n->grad_y;
+        real *partial = (real *)n->workspace;
+        const unsigned channel_blocks = (unsigned)ceil_div64(m.channels, kJoinColumns);
+        if (p.held) {
+            const dim3 grid((unsigned)p.blocks), block((unsigned)p.h.threads);
+            const size_t lds = held_lds(p.h, V, true);
+            if (m.positions <= p.h.rows)
+                TG_LAUNCH_AS("norm_backward", (norm_held_backward_kernel<T, V, 1>), grid, block, lds, stream, m, p.h, x, n->weight, n->bias, n->statistics,
+                             dy, (T *)n->grad_x, weights ? partial : nullptr);
+            else
+                TG_LAUNCH_AS("norm_backward", (norm_held_backward_kernel<T, V, kHeldRows>), grid, block, lds, stream, m, p.h, x, n->weight, n->bias,
+                             n->statistics, dy, (T *)n->grad_x, weights ? partial : nullptr);
+            if (weights)
+                TG_LAUNCH_AS("norm_join", (norm_join_held_kernel<T>), dim3(channel_blocks), dim3(kJoinThreads), 0, stream, m, p.parts, partial,
+                             n->grad_weight, n->grad_bias);
+            return check_launch(fn);
+        }
+        const dim3 grid((unsigned)p.blocks), block(kNormThreads);
+        real *by_group = partial + p.partial, *averages = by_group + p.by_group;
+        TG_LAUNCH_AS("norm_gradient_sums", (norm_gradient_sums_kernel<T, V>), grid, block, 0, stream, m, p.s, x, n->weight, n->bias, n->statistics, dy,
+                     weights ? partial : nullptr, by_group);
+        const int64_t group_blocks = n->grad_x ? ceil_div64(m.samples * m.groups, kJoinThreads / kWave) : 0;
+        TG_LAUNCH_AS("norm_join", (norm_join_kernel<T, V>), dim3((unsigned)group_blocks + (weights ? channel_blocks : 0)), dim3(kJoinThreads), 0, stream, m,
+                     p.s, partial, by_group, averages, group_blocks, n->grad_weight, n->grad_bias);
+        if (n->grad_x)
+            TG_LAUNCH_AS("norm_gradient", (norm_gradient_kernel<T, V>), grid, block, 0, stream, m, p.s, x, n->weight, n->bias, n->statistics, averages, dy,
+                         (T *)n->grad_x);
         return check_launch(fn);
     });
 }
