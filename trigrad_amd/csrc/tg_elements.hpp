@@ -23,6 +23,29 @@ template <int V, class T> __device__ __forceinline__ void store_pack(T *p, const
     *reinterpret_cast<Pack<T, V> *>(p) = out;
 }
 
+// The value of another lane of the sixteen, by the data-parallel move's control.
+template <int Control> __device__ __forceinline__ float from_lane(float v) {
+    return __uint_as_float((uint32_t)__builtin_amdgcn_update_dpp(0, (int)__float_as_uint(v), Control, 0xf, 0xf, true));
+}
+template <int Control> __device__ __forceinline__ double from_lane(double v) {
+    const uint64_t bits = (uint64_t)__double_as_longlong(v);
+    const uint32_t low = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)bits, Control, 0xf, 0xf, true);
+    const uint32_t high = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)(bits >> 32), Control, 0xf, 0xf, true);
+    return __longlong_as_double((long long)((uint64_t)high << 32 | low));
+}
+constexpr int kRotate8 = 0x128, kMirrorOf8 = 0x141, kSwapOnes = 0xb1, kSwapTwos = 0x4e;
+
+// The sum over `lanes` neighbouring lanes (a power of two, aligned), in each of them.
+template <class R> __device__ __forceinline__ R sum_lanes(R v, int lanes) {
+    if (lanes >= 2) v += from_lane<kSwapOnes>(v);
+    if (lanes >= 4) v += from_lane<kSwapTwos>(v);
+    if (lanes >= 8) v += from_lane<kMirrorOf8>(v);
+    if (lanes >= 16) v += from_lane<kRotate8>(v);
+    if (lanes >= 32) v += __shfl_xor(v, 16);
+    if (lanes >= 64) v += __shfl_xor(v, 32);
+    return v;
+}
+
 inline int64_t type_bytes(int64_t type) { return type == TG_TYPE_F64 ? 8 : type == TG_TYPE_F32 ? 4 : 2; }
 #ifdef TG_DOUBLE_PRECISION
 constexpr int64_t kRealType = TG_TYPE_F64;

@@ -25,7 +25,10 @@ struct NormShape {
 #ifdef TG_DOUBLE_PRECISION
 __device__ __forceinline__ real exp_norm(real z) { return exp(z); }
 __device__ __forceinline__ real inverse(real v) { return 1.0 / v; }
+__device__ __forceinline__ real inverse_root(real v) { return 1.0 / sqrt(v); }
 #else
+// 1 / sqrt(v) to one unit; the hardware's takes numbers below the normal ones for 0
+__device__ __forceinline__ real inverse_root(real v) { return v < 2.0f * FLT_MIN ? 1.0f / sqrtf(v) : __builtin_amdgcn_rsqf(v); }
 __device__ __forceinline__ real exp_norm(real z) { return __builtin_amdgcn_exp2f(z * 1.44269504f); }
 __device__ __forceinline__ real inverse(real v) { return __builtin_amdgcn_rcpf(v); }
 #endif
@@ -80,10 +83,8 @@ struct Held {
 // Sums of two values over the threads of each group: by neighbours, or through LDS, halving the members of all groups together.
 __device__ __forceinline__ void sum_groups(const Held &p, int segment, int member, int members, bool active, real &a, real &b, real *shared) {
     if (p.in_wave) {
-        for (int d = members >> 1; d > 0; d >>= 1) {
-            a += __shfl_xor(a, d);
-            b += __shfl_xor(b, d);
-        }
+        a = sum_lanes(a, members);
+        b = sum_lanes(b, members);
         return;
     }
     real *at = shared + 2 * (segment * members + member);
@@ -131,6 +132,36 @@ template <int V> __device__ __forceinline__ HeldPlace held_place(const NormShape
     return t;
 }
 
+// A thread's rows of a turn, from which it goes on by `workgroups` turns.
+struct HeldRows {
+    int64_t n, base, pitch, n_step, base_step;
+    int all;      // rows of the thread where it has a sample: at most K
+    int rows;     // 0: none
+    bool active;
+};
+__device__ __forceinline__ HeldRows held_rows(const NormShape &m, const Held &p, const HeldPlace &t, int64_t turn) {
+    HeldRows r;
+    r.n = turn * p.teams + t.team;
+    r.n_step = (int64_t)p.workgroups * p.teams;
+    r.base = (r.n * m.positions + t.row) * m.channels + t.channel;
+    r.base_step = r.n_step * m.positions * m.channels;
+    r.pitch = (int64_t)p.rows * m.channels;
+    r.all = t.active ? ((int)m.positions - t.row + p.rows - 1) / p.rows : 0;
+    r.active = t.active && r.n < m.samples;
+    r.rows = r.active ? r.all : 0;
+    return r;
+}
+__device__ __forceinline__ void next_turn(const NormShape &m, HeldRows &r) {
+    r.n += r.n_step;
+    r.base += r.base_step;
+    r.active = r.active && r.n < m.samples;
+    r.rows = r.active ? r.all : 0;
+}
+template <class T, int V, int K> __device__ __forceinline__ void load_held(const HeldRows &r, const T *x, Pack<T, V> (&in)[K]) {
+#pragma unroll
+    for (int k = 0; k < K; k++) in[k] = load_pack<V>(x + (k < r.rows ? r.base + r.pitch * k : 0));
+}
+
 template <class T, int V, int K>
 __global__ __launch_bounds__(1024) void norm_held_forward_kernel(NormShape m, Held p, const T *__restrict__ x, const void *__restrict__ weight,
                                                                  const void *__restrict__ bias, T *__restrict__ y, real *__restrict__ statistics) {
@@ -141,14 +172,13 @@ __global__ __launch_bounds__(1024) void norm_held_forward_kernel(NormShape m, He
     real w[V], b[V];
     load_weights<T, V>(m, weight, t.active ? t.channel : 0, (real)1, w);
     load_weights<T, V>(m, bias, t.active ? t.channel : 0, (real)0, b);
-    for (int64_t turn = first_turn; turn < p.turns; turn += p.workgroups) {
-        const int64_t n = turn * p.teams + t.team;
-        const bool active = t.active && n < m.samples;
-        const int64_t base = active ? (n * m.positions + t.row) * m.channels + t.channel : 0, pitch = (int64_t)p.rows * m.channels;
-        const int rows = active ? (int)((m.positions - t.row + p.rows - 1) / p.rows) : 0;  // of the thread: at most K
+    HeldRows r = held_rows(m, p, t, first_turn);
+    for (int64_t turn = first_turn; turn < p.turns; turn += p.workgroups, next_turn(m, r)) {
+        const int64_t n = r.n, base = r.base, pitch = r.pitch;
+        const int rows = r.rows;
+        const bool active = r.active;
         Pack<T, V> in[K];
-#pragma unroll
-        for (int k = 0; k < K; k++) in[k] = load_pack<V>(x + (k < rows ? base + pitch * k : 0));
+        load_held(r, x, in);
         real sum = 0, none = 0;
 #pragma unroll
         for (int k = 0; k < K; k++)
@@ -168,9 +198,8 @@ __global__ __launch_bounds__(1024) void norm_held_forward_kernel(NormShape m, He
             }
         sum_groups(p, t.segment, t.member, t.members, active, first, second, shared);
         const real rest = first * per_value, mean = about + rest, variance = fma(-rest, rest, second * per_value);
-        const real rstd = (real)1 / sqrt((variance < 0 ? (real)0 : variance) + m.eps);
-        if (!active) continue;
-        if (t.member == 0) {
+        const real rstd = inverse_root((variance < 0 ? (real)0 : variance) + m.eps);
+        if (active && t.member == 0) {
             statistics[2 * (n * m.groups + t.group)] = mean;
             statistics[2 * (n * m.groups + t.group) + 1] = rstd;
         }
@@ -180,7 +209,7 @@ __global__ __launch_bounds__(1024) void norm_held_forward_kernel(NormShape m, He
                 if (k >= rows) break;
                 real out[V];
 #pragma unroll
-                for (int v = 0; v < V; v++) out[v] = activate<decltype(kind)::value, false>(fma((in[k][v] - mean) * rstd, w[v], b[v]));
+                for (int v = 0; v < V; v++) out[v] = activate<decltype(kind)::value, false>(fma(in[k][v] - mean, rstd * w[v], b[v]));
                 store_pack<V>(y + base + pitch * k, out);
             }
         });
@@ -200,18 +229,15 @@ __global__ __launch_bounds__(1024) void norm_held_backward_kernel(NormShape m, H
     load_weights<T, V>(m, bias, t.active ? t.channel : 0, (real)0, b);
 #pragma unroll
     for (int v = 0; v < V; v++) dw[v] = db[v] = 0;
-    for (int64_t turn = first_turn; turn < p.turns; turn += p.workgroups) {
-        const int64_t n = turn * p.teams + t.team;
-        const bool active = t.active && n < m.samples;
-        const int64_t base = active ? (n * m.positions + t.row) * m.channels + t.channel : 0, pitch = (int64_t)p.rows * m.channels;
-        const int rows = active ? (int)((m.positions - t.row + p.rows - 1) / p.rows) : 0;
-        const int64_t of = active ? 2 * (n * m.groups + t.group) : 0;
+    HeldRows r = held_rows(m, p, t, first_turn);
+    for (int64_t turn = first_turn; turn < p.turns; turn += p.workgroups, next_turn(m, r)) {
+        const int64_t base = r.base, pitch = r.pitch;
+        const int rows = r.rows;
         Pack<T, V> in[K], dy[K];
-#pragma unroll
-        for (int k = 0; k < K; k++) in[k] = load_pack<V>(x + (k < rows ? base + pitch * k : 0));
-#pragma unroll
-        for (int k = 0; k < K; k++) dy[k] = load_pack<V>(grad_y + (k < rows ? base + pitch * k : 0));
-        const real mean = statistics[of], rstd = statistics[of + 1];
+        load_held(r, x, in);
+        load_held(r, grad_y, dy);
+        const Pack<real, 2> of = load_pack<2>(statistics + (r.active ? 2 * (r.n * m.groups + t.group) : 0));
+        const real mean = of[0], rstd = of[1];
         real sum = 0, product = 0;
         // dz is computed again where it is used: its 32 bits are not held
         by_activation(m.activation, [&](auto kind) {
@@ -220,33 +246,33 @@ __global__ __launch_bounds__(1024) void norm_held_backward_kernel(NormShape m, H
 #pragma unroll
                 for (int v = 0; v < V; v++) {
                     const real hat = (in[k][v] - mean) * rstd;
-                    const real dz = k < rows ? dy[k][v] * activate<decltype(kind)::value, true>(fma(hat, w[v], b[v])) : (real)0;
-                    db[v] += dz;
-                    if (k < rows) dw[v] = fma(dz, hat, dw[v]);
-                    const real dh = dz * w[v];
-                    sum += dh;
-                    if (k < rows) product = fma(dh, hat, product);
+                    const real dz = dy[k][v] * activate<decltype(kind)::value, true>(fma(hat, w[v], b[v]));
+                    if (k < rows) {
+                        db[v] += dz;
+                        dw[v] = fma(dz, hat, dw[v]);
+                        sum = fma(dz, w[v], sum);
+                        product = fma(dz * w[v], hat, product);
+                    }
                 }
         });
-        if (!grad_x) continue;
-        sum_groups(p, t.segment, t.member, t.members, active, sum, product, shared);
-        sum *= per_value;
-        product *= per_value;
-        if (!active) continue;
-        by_activation(m.activation, [&](auto kind) {
+        if (grad_x) {
+            sum_groups(p, t.segment, t.member, t.members, r.active, sum, product, shared);
+            const real c0 = sum * per_value * rstd, c1 = product * per_value * rstd * rstd;
+            by_activation(m.activation, [&](auto kind) {
 #pragma unroll
-            for (int k = 0; k < K; k++) {
-                if (k >= rows) break;
-                real out[V];
+                for (int k = 0; k < K; k++) {
+                    if (k >= rows) break;
+                    real out[V];
 #pragma unroll
-                for (int v = 0; v < V; v++) {
-                    const real hat = (in[k][v] - mean) * rstd;
-                    const real dh = dy[k][v] * activate<decltype(kind)::value, true>(fma(hat, w[v], b[v])) * w[v];
-                    out[v] = rstd * (dh - sum - hat * product);
+                    for (int v = 0; v < V; v++) {
+                        const real d = in[k][v] - mean, wr = rstd * w[v];
+                        const real dz = dy[k][v] * activate<decltype(kind)::value, true>(fma(d, wr, b[v]));
+                        out[v] = fma(dz, wr, fma(d, -c1, -c0));
+                    }
+                    store_pack<V>(grad_x + base + pitch * k, out);
                 }
-                store_pack<V>(grad_x + base + pitch * k, out);
-            }
-        });
+            });
+        }
     }
     if (!partial) return;
     // sums over the threads that have the same channels
@@ -319,13 +345,14 @@ __device__ __forceinline__ void group_sums(const NormShape &m, const Streamed &p
     }
 }
 
-// The sum over the splits and tiles of those of a group, by a wave, in every lane.
-template <int V> __device__ __forceinline__ void sum_splits(const NormShape &m, const Streamed &p, int64_t n, int64_t g, const real *partial, double &first,
-                                                            double &second) {
+// The sum over the splits and tiles of those of a group, by a workgroup; in its first thread.
+template <int V, int Threads>
+__device__ __forceinline__ void sum_splits(const NormShape &m, const Streamed &p, int64_t n, int64_t g, const real *partial, double &first, double &second) {
+    __shared__ double shared[2][Threads / kWave];
     const int64_t columns = (int64_t)p.units * V;
     const int t0 = (int)(g * m.width / columns), t1 = (int)(((g + 1) * m.width - 1) / columns);
     first = second = 0;
-    for (int s = threadIdx.x & (kWave - 1); s < p.splits; s += kWave)
+    for (int s = threadIdx.x; s < p.splits; s += Threads)
         for (int t = t0; t <= t1; t++) {
             const real *at = partial + (((((n * p.splits + s) * p.tiles + t) * m.groups) + g) << 1);
             first += at[0];
@@ -334,6 +361,15 @@ template <int V> __device__ __forceinline__ void sum_splits(const NormShape &m, 
     for (int d = kWave / 2; d > 0; d >>= 1) {
         first += __shfl_xor(first, d);
         second += __shfl_xor(second, d);
+    }
+    if ((threadIdx.x & (kWave - 1)) == 0) {
+        shared[0][threadIdx.x / kWave] = first;
+        shared[1][threadIdx.x / kWave] = second;
+    }
+    __syncthreads();
+    for (int i = 1; threadIdx.x == 0 && i < Threads / kWave; i++) {
+        first += shared[0][i];
+        second += shared[1][i];
     }
 }
 
@@ -358,13 +394,15 @@ __global__ __launch_bounds__(kNormThreads) void norm_sums_kernel(NormShape m, St
 #pragma unroll
             for (int k = 0; k < kNormAhead; k++) in[k] = load_pack<V>(from + (k < there ? pitch * k : 0));
 #pragma unroll
-            for (int k = 0; k < kNormAhead; k++)
+            for (int k = 0; k < kNormAhead; k++) {
+                if (k >= there) break;
 #pragma unroll
                 for (int v = 0; v < V; v++) {
-                    const real d = k < there ? in[k][v] - pivot[v] : (real)0;
+                    const real d = in[k][v] - pivot[v];
                     first[v] += d;
                     second[v] = fma(d, d, second[v]);
                 }
+            }
         });
 #pragma unroll
     for (int v = 0; v < V; v++) {
@@ -383,17 +421,14 @@ __global__ __launch_bounds__(kNormThreads) void norm_sums_kernel(NormShape m, St
     group_sums(m, p, n, split, tile, columns, shared[0], shared[1], partial);
 }
 
-// mean and rstd of each group: a wave each
+// mean and rstd of each group: a workgroup each
 template <class T, int V>
 __global__ __launch_bounds__(kNormThreads) void norm_statistics_kernel(NormShape m, Streamed p, const T *__restrict__ x, const real *__restrict__ partial,
                                                                        real *__restrict__ statistics) {
-    const int lane = threadIdx.x & (kWave - 1);
-    const int64_t id = (int64_t)blockIdx.x * (kNormThreads / kWave) + threadIdx.x / kWave;
-    if (id >= m.samples * m.groups) return;
-    const int64_t n = id / m.groups, g = id % m.groups;
+    const int64_t id = blockIdx.x, n = id / m.groups, g = id % m.groups;
     double first, second;
-    sum_splits<V>(m, p, n, g, partial, first, second);
-    if (lane != 0) return;
+    sum_splits<V, kNormThreads>(m, p, n, g, partial, first, second);
+    if (threadIdx.x != 0) return;
     const double count = (double)m.positions * (double)m.width, rest = first / count, variance = second / count - rest * rest;
     statistics[2 * id] = (real)((double)(real)x[n * m.positions * m.channels + g * m.width] + rest);
     statistics[2 * id + 1] = (real)(1.0 / sqrt((variance < 0 ? 0.0 : variance) + (double)m.eps));
@@ -409,14 +444,14 @@ __global__ __launch_bounds__(kNormThreads) void norm_apply_kernel(NormShape m, S
     if (!t.active) return;
     x += n * m.positions * m.channels;
     y += n * m.positions * m.channels;
-    real w[V], b[V], mean[V], rstd[V];
+    real w[V], b[V], mean[V];
     load_weights<T, V>(m, weight, t.channel, (real)1, w);
     load_weights<T, V>(m, bias, t.channel, (real)0, b);
 #pragma unroll
     for (int v = 0; v < V; v++) {
         const int64_t of = 2 * (n * m.groups + (t.channel + v) / m.width);
         mean[v] = statistics[of];
-        rstd[v] = statistics[of + 1];
+        w[v] *= statistics[of + 1];
     }
     const int64_t pitch = (int64_t)p.rows * m.channels;
     by_activation(m.activation, [&](auto kind) {
@@ -430,7 +465,7 @@ __global__ __launch_bounds__(kNormThreads) void norm_apply_kernel(NormShape m, S
                 if (k >= there) break;
                 real out[V];
 #pragma unroll
-                for (int v = 0; v < V; v++) out[v] = activate<decltype(kind)::value, false>(fma((in[k][v] - mean[v]) * rstd[v], w[v], b[v]));
+                for (int v = 0; v < V; v++) out[v] = activate<decltype(kind)::value, false>(fma(in[k][v] - mean[v], w[v], b[v]));
                 store_pack<V>(to + pitch * k, out);
             }
         });
@@ -459,6 +494,7 @@ __global__ __launch_bounds__(kNormThreads) void norm_gradient_sums_kernel(NormSh
             const int64_t of = 2 * (n * m.groups + (t.channel + v) / m.width);
             mean[v] = statistics[of];
             rstd[v] = statistics[of + 1];
+            w[v] *= rstd[v];
         }
         const int64_t pitch = (int64_t)p.rows * m.channels;
         by_activation(m.activation, [&](auto kind) {
@@ -472,16 +508,19 @@ __global__ __launch_bounds__(kNormThreads) void norm_gradient_sums_kernel(NormSh
                     dy[k] = load_pack<V>(grad_y + at + (k < there ? pitch * k : 0));
                 }
 #pragma unroll
-                for (int k = 0; k < kNormPairs; k++)
+                for (int k = 0; k < kNormPairs; k++) {
+                    if (k >= there) break;
 #pragma unroll
                     for (int v = 0; v < V; v++) {
-                        const real hat = (in[k][v] - mean[v]) * rstd[v];
-                        const real dz = dy[k][v] * activate<decltype(kind)::value, true>(fma(hat, w[v], b[v]));
-                        sum[v] += k < there ? dz : (real)0;
-                        if (k < there) product[v] = fma(dz, hat, product[v]);
+                        const real d = in[k][v] - mean[v], dz = dy[k][v] * activate<decltype(kind)::value, true>(fma(d, w[v], b[v]));
+                        sum[v] += dz;
+                        product[v] = fma(dz, d, product[v]);
                     }
+                }
             }
         });
+#pragma unroll
+        for (int v = 0; v < V; v++) product[v] *= rstd[v];
     }
 #pragma unroll
     for (int v = 0; v < V; v++) {
@@ -535,19 +574,18 @@ __device__ __forceinline__ void join_channel(const NormShape &m, int64_t parts, 
     }
 }
 
-// By group avg dxh and avg(dxh xh), a wave each; then the weights' gradients.
+// By group avg dxh and avg(dxh xh), a workgroup each; then the weights' gradients.
 template <class T, int V>
 __global__ __launch_bounds__(kJoinThreads) void norm_join_kernel(NormShape m, Streamed p, const real *__restrict__ partial,
                                                                  const real *__restrict__ group_partial, real *__restrict__ averages,
                                                                  int64_t group_blocks, void *__restrict__ grad_weight, void *__restrict__ grad_bias) {
     __shared__ double shared[2][kJoinThreads];
     if (blockIdx.x < group_blocks) {
-        const int64_t id = (int64_t)blockIdx.x * (kJoinThreads / kWave) + threadIdx.x / kWave;
-        if (id >= m.samples * m.groups) return;
+        const int64_t id = blockIdx.x;
         double sum, product;
-        sum_splits<V>(m, p, id / m.groups, id % m.groups, group_partial, sum, product);
+        sum_splits<V, kJoinThreads>(m, p, id / m.groups, id % m.groups, group_partial, sum, product);
         const double count = (double)m.positions * (double)m.width;
-        if ((threadIdx.x & (kWave - 1)) == 0) {
+        if (threadIdx.x == 0) {
             averages[2 * id] = (real)(sum / count);
             averages[2 * id + 1] = (real)(product / count);
         }
@@ -572,16 +610,17 @@ __global__ __launch_bounds__(kNormThreads) void norm_gradient_kernel(NormShape m
     const int64_t n = turned / (unsigned)p.splits / (unsigned)p.tiles;
     const StreamedPlace t = streamed_place<V>(m, p, (int)(turned % (unsigned)p.splits), (int)(turned / (unsigned)p.splits % (unsigned)p.tiles));
     if (!t.active) return;
-    real w[V], b[V], mean[V], rstd[V], sum[V], product[V];
+    real w[V], b[V], mean[V], sum[V], product[V];  // from here on times rstd, rstd and its square
     load_weights<T, V>(m, weight, t.channel, (real)1, w);
     load_weights<T, V>(m, bias, t.channel, (real)0, b);
 #pragma unroll
     for (int v = 0; v < V; v++) {
         const int64_t of = 2 * (n * m.groups + (t.channel + v) / m.width);
+        const real rstd = statistics[of + 1];
         mean[v] = statistics[of];
-        rstd[v] = statistics[of + 1];
-        sum[v] = averages[of];
-        product[v] = averages[of + 1];
+        w[v] *= rstd;
+        sum[v] = averages[of] * rstd;
+        product[v] = averages[of + 1] * rstd * rstd;
     }
     const int64_t pitch = (int64_t)p.rows * m.channels;
     by_activation(m.activation, [&](auto kind) {
@@ -600,9 +639,8 @@ __global__ __launch_bounds__(kNormThreads) void norm_gradient_kernel(NormShape m
                 real out[V];
 #pragma unroll
                 for (int v = 0; v < V; v++) {
-                    const real hat = (in[k][v] - mean[v]) * rstd[v];
-                    const real dh = dy[k][v] * activate<decltype(kind)::value, true>(fma(hat, w[v], b[v])) * w[v];
-                    out[v] = rstd[v] * (dh - sum[v] - hat * product[v]);
+                    const real d = in[k][v] - mean[v], dz = dy[k][v] * activate<decltype(kind)::value, true>(fma(d, w[v], b[v]));
+                    out[v] = fma(dz, w[v], fma(d, -product[v], -sum[v]));
                 }
                 store_pack<V>(grad_x + at + pitch * k, out);
             }
@@ -670,7 +708,7 @@ template <class Call> static int by_vector(int64_t type, int vector, Call &&call
 }
 
 constexpr int kHeldRows = 8;        // accesses of a thread that are held
-constexpr int kHeldWorkgroups = 512;  // at most, where they sum the weights' gradients
+constexpr int kHeldThreads = 1 << 19;  // of all workgroups together, which go over the samples: the chip's places
 
 // A slab of groups whose rows are 64 bytes or more, if a workgroup can hold it; threads == 0: it cannot.
 static Held held_of(const NormShape &m, int vector, int64_t bytes) {
@@ -730,7 +768,7 @@ static NormPlan plan_of(const NormShape &m, int64_t type, bool backward, bool al
     // few workgroups leave most of the chip idle: a sample is then better split
     p.held = p.h.threads > 0 && (p.h.turns * slabs >= 128 || m.samples * m.positions * m.channels * bytes <= (1 << 18));
     if (p.held) {
-        p.h.workgroups = (int)std::min<int64_t>(p.h.turns, std::max<int64_t>(1, (backward ? kHeldWorkgroups : 8192) / slabs));
+        p.h.workgroups = (int)std::min<int64_t>(p.h.turns, std::max<int64_t>(1, kHeldThreads / p.h.threads / slabs));
         p.parts = backward ? p.h.workgroups : 0;
         p.partial = 2 * p.parts * m.channels;
         p.blocks = p.h.workgroups * slabs;
@@ -786,7 +824,7 @@ extern "C" int tg_group_norm_forward(const tg_norm *n) {
         return TG_E_ARG;
     }
     const NormPlan p = plan_of(m, n->type, false, false, {n->x, n->y});
-    if (p.blocks >= (1 << 22)) return too_many(fn);
+    if (p.blocks >= (1 << 22) || (!p.held && m.samples * m.groups >= (1 << 21))) return too_many(fn);
     if (norm_bytes(p) > 0 && (!n->workspace || n->workspace_bytes < norm_bytes(p))) {
         set_error("%s: workspace of %lld bytes, %lld needed", fn, (long long)n->workspace_bytes, (long long)norm_bytes(p));
         return TG_E_WORKSPACE;
@@ -810,7 +848,7 @@ extern "C" int tg_group_norm_forward(const tg_norm *n) {
         const dim3 grid((unsigned)p.blocks), block(kNormThreads);
         real *partial = (real *)n->workspace;
         TG_LAUNCH_AS("norm_sums", (norm_sums_kernel<T, V>), grid, block, 0, stream, m, p.s, x, partial);
-        TG_LAUNCH_AS("norm_statistics", (norm_statistics_kernel<T, V>), dim3((unsigned)ceil_div64(m.samples * m.groups, kNormThreads / kWave)), block, 0,
+        TG_LAUNCH_AS("norm_statistics", (norm_statistics_kernel<T, V>), dim3((unsigned)(m.samples * m.groups)), block, 0,
                      stream, m, p.s, x, partial, n->statistics);
         TG_LAUNCH_AS("norm_apply", (norm_apply_kernel<T, V>), grid, block, 0, stream, m, p.s, x, n->weight, n->bias, n->statistics, (T *)n->y);
         return check_launch(fn);
@@ -844,7 +882,7 @@ extern "C" int tg_group_norm_backward(const tg_norm *n) {
         return TG_E_ARG;
     }
     const NormPlan p = plan_of(m, n->type, true, false, {n->x, n->grad_y, n->grad_x});
-    if (p.blocks >= (1 << 22)) return too_many(fn);
+    if (p.blocks >= (1 << 22) || (!p.held && m.samples * m.groups >= (1 << 21))) return too_many(fn);
     if (!n->workspace || n->workspace_bytes < norm_bytes(p)) {
         set_error("%s: workspace of %lld bytes, %lld needed", fn, (long long)n->workspace_bytes, (long long)norm_bytes(p));
         return TG_E_WORKSPACE;
@@ -873,7 +911,7 @@ extern "C" int tg_group_norm_backward(const tg_norm *n) {
         real *by_group = partial + p.partial, *averages = by_group + p.by_group;
         TG_LAUNCH_AS("norm_gradient_sums", (norm_gradient_sums_kernel<T, V>), grid, block, 0, stream, m, p.s, x, n->weight, n->bias, n->statistics, dy,
                      weights ? partial : nullptr, by_group);
-        const int64_t group_blocks = n->grad_x ? ceil_div64(m.samples * m.groups, kJoinThreads / kWave) : 0;
+        const int64_t group_blocks = n->grad_x ? m.samples * m.groups : 0;
         TG_LAUNCH_AS("norm_join", (norm_join_kernel<T, V>), dim3((unsigned)group_blocks + (weights ? channel_blocks : 0)), dim3(kJoinThreads), 0, stream, m,
                      p.s, partial, by_group, averages, group_blocks, n->grad_weight, n->grad_bias);
         if (n->grad_x)

@@ -224,8 +224,7 @@ __global__ __launch_bounds__(Threads) void recurrence_backward_kernel(Split m, c
         const int gate_lanes = 1 << m.gate_lanes_log2, lane = threadIdx.x & (gate_lanes - 1);
 #pragma unroll
         for (int k = 0; k < K; k++) {
-            float sum = q[k];
-            for (int d = gate_lanes >> 1; d > 0; d >>= 1) sum += __shfl_xor(sum, d);
+            const float sum = sum_lanes(q[k], gate_lanes);
             if (lane == 0 && valid && k < n) store_gate(k, sum, slope(k, 0));
         }
     }

@@ -287,11 +287,6 @@ template <int K, int GV> __device__ __forceinline__ void compute_gates(const Spl
     }
 }
 
-template <int Control> __device__ __forceinline__ float from_lane(float v) {  // of the sixteen: by the data-parallel move's control
-    return __uint_as_float((uint32_t)__builtin_amdgcn_update_dpp(0, (int)__float_as_uint(v), Control, 0xf, 0xf, true));
-}
-constexpr int kRotate8 = 0x128, kMirrorOf8 = 0x141, kSwapOnes = 0xb1, kSwapTwos = 0x4e;
-
 // Sums of K rows' values over the wave.  Each step hands half of the rows to half of the lanes, so K + K / 2 + ... additions do what six a
 // row would; a lane ends with the sum of row_of_sum, and the lanes that sum_is_here names have each of them once.
 template <int K> __device__ __forceinline__ float sum_rows(float (&q)[K]) {
