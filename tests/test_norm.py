@@ -107,10 +107,17 @@ TYPES = {"f32": (torch.float32, None), "bf16": (torch.bfloat16, None), "f16": (t
          "bf16_f32": (torch.bfloat16, torch.float32), "f16_f32": (torch.float16, torch.float32), "f64": (torch.float64, None)}
 
 
+@pytest.fixture(params=["module", "python"])
+def route(request, monkeypatch):
+    """Calls by the torch module, which takes the ordinary ones, and all of them by the Python functions."""
+    from trigrad_amd import _C
+    monkeypatch.setattr(_C, "ONE_CALL_OPERATORS", request.param == "module")
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("activation", ["none", "relu", "silu", "gelu"])
 @pytest.mark.parametrize("types", sorted(TYPES))
-def test_types_and_activations(types, activation, cuda):
+def test_types_and_activations(types, activation, cuda, route):
     for seed, (shape, groups) in enumerate([((2, 9, 11, 24), 4), ((50, 64), 8), ((1, 700, 40), 5)]):
         x, w, b, dy = make(cuda, seed, shape, *TYPES[types])
         run_and_check(x, groups, w, b, dy, activation)
@@ -145,7 +152,7 @@ def test_large(shape, groups, cuda):
 
 
 @pytest.mark.gpu
-def test_only_weight_only_bias_and_partial_gradients(cuda):
+def test_only_weight_only_bias_and_partial_gradients(cuda, route):
     import trigrad_amd
     x, w, b, dy = make(cuda, 2, (2, 50, 48))
     full = run_and_check(x, 6, w, b, dy, "silu")
@@ -180,7 +187,7 @@ def test_gradient_against_differences(cuda):
 
 
 @pytest.mark.gpu
-def test_strides_and_alignment(cuda):
+def test_strides_and_alignment(cuda, route):
     import trigrad_amd
     for dtype in (torch.float32, torch.bfloat16):
         x, w, b, dy = make(cuda, 6, (2, 31, 24), dtype)
@@ -222,7 +229,7 @@ def test_saturated_activations(cuda):
 
 
 @pytest.mark.gpu
-def test_empty_inputs(cuda):
+def test_empty_inputs(cuda, route):
     import trigrad_amd
     for shape in ((0, 5, 8), (3, 0, 8), (0, 8)):
         x = torch.zeros(shape, device=cuda, requires_grad=True)
@@ -248,7 +255,7 @@ def test_same_bits_every_time(cuda):
 
 
 @pytest.mark.gpu
-def test_other_streams_and_graphs(cuda):
+def test_other_streams_and_graphs(cuda, route):
     """Two captured graphs on two streams, replayed together with eager calls between, every replay checked."""
     import trigrad_amd
     graphs = []
@@ -348,7 +355,7 @@ def test_refusals_without_gpu():
 
 
 @pytest.mark.gpu
-def test_refusals(cuda):
+def test_refusals(cuda, route):
     import trigrad_amd
     f = trigrad_amd.group_norm
     x, w, b, _ = make(cuda, 1, (2, 3, 8))

@@ -126,12 +126,19 @@ TYPES = {"f32": (torch.float32, None), "bf16": (torch.bfloat16, None), "f16": (t
          "bf16_f32": (torch.bfloat16, torch.float32), "f16_f32": (torch.float16, torch.float32), "f64": (torch.float64, None)}
 
 
+@pytest.fixture(params=["module", "python"])
+def route(request, monkeypatch):
+    """Calls by the torch module, which takes the ordinary ones, and all of them by the Python functions."""
+    from trigrad_amd import _C
+    monkeypatch.setattr(_C, "ONE_CALL_OPERATORS", request.param == "module")
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("reverse", [False, True])
 @pytest.mark.parametrize("input_form", ["plain", "complement"])
 @pytest.mark.parametrize("gate_form", ["value", "log", "logit"])
 @pytest.mark.parametrize("types", sorted(TYPES))
-def test_forms_and_types(types, gate_form, input_form, reverse, cuda):
+def test_forms_and_types(types, gate_form, input_form, reverse, cuda, route):
     dtype, gate_dtype = TYPES[types]
     for seed, (rows, channels, gates) in enumerate([((3, 37), 24, 24), ((2, 70), 40, 10), ((1, 300), 6, 2)]):
         x, g, h0, rng = make(cuda, seed, rows, channels, gates, dtype, gate_dtype, gate_form, initial=seed != 1)
@@ -199,7 +206,7 @@ def test_sequence_ends_on_every_row_of_a_piece(cuda):
 
 
 @pytest.mark.gpu
-def test_only_the_final_state(cuda):
+def test_only_the_final_state(cuda, route):
     """The compositing call: no states out, no gradient of them in; a short axis and very many channels, three to a gate."""
     for rows, channels, gates in (((1, 8), 3 * 5000, 5000), ((4, 3), 600, 200), ((1, 700), 12, 12)):
         x, g, h0, rng = make(cuda, 3, rows, channels, gates)
@@ -207,7 +214,7 @@ def test_only_the_final_state(cuda):
 
 
 @pytest.mark.gpu
-def test_gradients_that_are_asked_for(cuda):
+def test_gradients_that_are_asked_for(cuda, route):
     import trigrad_amd
     x, g, h0, rng = make(cuda, 5, (2, 90), 24, 6)
     _, _, full = run_and_check(x, g, h0, use_final=False, rng=torch.Generator().manual_seed(9))
@@ -237,7 +244,7 @@ def test_gradient_against_differences(cuda):
 
 
 @pytest.mark.gpu
-def test_strides_and_alignment(cuda):
+def test_strides_and_alignment(cuda, route):
     """Views: channels taken out of wider rows, rows transposed, storage that begins off a vector's alignment."""
     import trigrad_amd
     for dtype in (torch.float32, torch.bfloat16):
@@ -320,7 +327,7 @@ def test_gates_of_zero_one_and_more(cuda):
 
 
 @pytest.mark.gpu
-def test_empty_inputs(cuda):
+def test_empty_inputs(cuda, route):
     import trigrad_amd
     for shape, gates in (((0, 5, 8), 8), ((3, 0, 8), 2), ((2, 4, 0), 0)):
         x = torch.zeros(shape, device=cuda, requires_grad=True)
@@ -357,7 +364,7 @@ def test_same_bits_every_time(cuda):
 
 
 @pytest.mark.gpu
-def test_other_streams_and_graphs(cuda):
+def test_other_streams_and_graphs(cuda, route):
     """Two captured graphs on two streams, replayed in turn with eager calls between, every replay checked."""
     import trigrad_amd
     graphs = []
@@ -415,7 +422,7 @@ def test_more_elements_than_31_bits_count(cuda):
 @pytest.mark.gpu
 @pytest.mark.parametrize("types", sorted(TYPES))
 @pytest.mark.parametrize("sequences,channels,gates", [(1, 1, 1), (1, 1024, 1024), (3, 30, 10), (7, 129, 129), (33, 256, 2), (2, 260, 1)])
-def test_step(sequences, channels, gates, types, cuda):
+def test_step(sequences, channels, gates, types, cuda, route):
     """One step is a sequence of one row, in place or beside the state."""
     import trigrad_amd
     dtype, gate_dtype = TYPES[types]
@@ -433,7 +440,7 @@ def test_step(sequences, channels, gates, types, cuda):
 
 
 @pytest.mark.gpu
-def test_step_after_step_is_the_sequence(cuda):
+def test_step_after_step_is_the_sequence(cuda, route):
     import trigrad_amd
     x, g, h0, _ = make(cuda, 1, (4, 30), 96, 12, torch.bfloat16, torch.float32, "logit")
     want = reference(x, g, h0, None, "logit", "complement", False)
@@ -471,7 +478,7 @@ def test_refusals_without_gpu():
 
 
 @pytest.mark.gpu
-def test_refusals(cuda):
+def test_refusals(cuda, route):
     import trigrad_amd
     f, step = trigrad_amd.linear_recurrence, trigrad_amd.linear_recurrence_step
     x, g, h0, _ = make(cuda, 1, (2, 3), 8, 4)

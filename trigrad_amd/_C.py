@@ -1263,6 +1263,18 @@ def real_type(dtype):
     return torch.float64 if dtype == torch.float64 else torch.float32
 
 
+# The operators' ordinary calls on float32, float16 and bfloat16 go through the torch module (csrc/tg_torch_operators.hpp), which returns
+# None for what the Python functions have a check, an error or another library for.  False: the Python functions make all calls.
+ONE_CALL_OPERATORS = True
+
+
+def operators_by_torch_module(tensor):
+    """The torch module where it may have a call on `tensor`, else None."""
+    if not ONE_CALL_OPERATORS or not isinstance(tensor, torch.Tensor) or not tensor.is_cuda or tensor.dtype is torch.float64:
+        return None
+    return _lib._torch_module or _module()
+
+
 def _address(t):
     return 0 if t is None else t.data_ptr()
 

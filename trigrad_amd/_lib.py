@@ -157,5 +157,8 @@ def torch_module(key_counts):
         lib = load(32)
         module.bind(*[C.cast(getattr(lib, name), C.c_void_p).value for name in (
             "tg_frame_forward", "tg_frame_backward", "tg_frame_wait", "tg_force_tickets", "tg_last_error")], key_counts)
+        module.bind_operators(*[C.cast(getattr(lib, name), C.c_void_p).value for name in (
+            "tg_linear_recurrence_sizes", "tg_linear_recurrence_forward", "tg_linear_recurrence_backward", "tg_linear_recurrence_step",
+            "tg_group_norm_sizes", "tg_group_norm_forward", "tg_group_norm_backward")])
         _torch_module = module
     return _torch_module

@@ -439,7 +439,18 @@ PyObject *py_verify(PyObject *, PyObject *wait) {
     END_HANDLE_TH_ERRORS
 }
 
+}  // namespace
+
+#include "tg_torch_operators.hpp"
+
+namespace {
+
 PyMethodDef methods[] = {{"render", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_render)), METH_FASTCALL, nullptr},
+                         {"linear_recurrence", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_linear_recurrence)), METH_FASTCALL, nullptr},
+                         {"linear_recurrence_step", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_linear_recurrence_step)), METH_FASTCALL,
+                          nullptr},
+                         {"group_norm", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_group_norm)), METH_FASTCALL, nullptr},
+                         {"bind_operators", py_bind_operators, METH_VARARGS, nullptr},
                          {"bind", py_bind, METH_VARARGS, nullptr},
                          {"remember", py_remember, METH_VARARGS, nullptr},
                          {"add_state", py_add_state, METH_VARARGS, nullptr},

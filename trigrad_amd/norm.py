@@ -73,4 +73,9 @@ def group_norm(
 
     Sums and statistics are float32 whatever the types.  Returns y as x.
     """
+    module = _C.operators_by_torch_module(x)
+    if module is not None:
+        y = module.group_norm(x, num_groups, weight, bias, eps, ACTIVATIONS.get(activation))
+        if y is not None:
+            return y
     return GroupNorm.apply(x, num_groups, weight, bias, eps, activation)

@@ -112,6 +112,11 @@ def linear_recurrence(
         states : as inputs, or None
         final : (S, D) float32, the state behind the last step of each sequence
     """
+    module = _C.operators_by_torch_module(inputs)
+    if module is not None:
+        out = module.linear_recurrence(inputs, gates, initial, offsets, GATE_FORMS.get(gate_form), INPUT_FORMS.get(input_form), reverse, return_states)
+        if out is not None:
+            return out
     return LinearRecurrence.apply(inputs, gates, initial, offsets, gate_form, input_form, reverse, return_states)
 
 
@@ -133,6 +138,11 @@ def linear_recurrence_step(
         states : (S, D) in the inputs' type
         state : the new state in float32 (`state` itself, or `out`)
     """
+    module = _C.operators_by_torch_module(inputs)
+    if module is not None:
+        result = module.linear_recurrence_step(inputs, gates, state, GATE_FORMS.get(gate_form), INPUT_FORMS.get(input_form), out)
+        if result is not None:
+            return result
     if inputs.dim() != 2:
         raise ValueError(f"inputs must have 2 dimensions, but got {inputs.dim()}")
     _check(inputs[:, None], gates[:, None], state, None, gate_form, input_form, "state")
@@ -146,4 +156,6 @@ def linear_recurrence_step(
     if torch.is_grad_enabled() and any(t.requires_grad for t in (inputs, gates, state, new_state)):
         raise RuntimeError("linear_recurrence_step has no gradient: use linear_recurrence, or torch.no_grad()")
     states = _C.linear_recurrence_step(inputs.contiguous(), gates.contiguous(), state, new_state, GATE_FORMS[gate_form], INPUT_FORMS[input_form])
+    if not new_state.is_inference():
+        torch.autograd.graph.increment_version(new_state)
     return states, new_state
