@@ -80,32 +80,51 @@ struct Held {
     bool in_wave;      // a group's threads are neighbours in a wave, a power of two of them
 };
 
-// Sums of two values over the threads of each group: by neighbours, or through LDS, halving the members of all groups together.
+// Sums of two values over the threads of each group: by neighbours, or through LDS.
 __device__ __forceinline__ void sum_groups(const Held &p, int segment, int member, int members, bool active, real &a, real &b, real *shared) {
     if (p.in_wave) {
         a = sum_lanes(a, members);
         b = sum_lanes(b, members);
         return;
     }
-    real *at = shared + 2 * (segment * members + member);
+    // all of a group's values to LDS, and their sum by every thread of the group (few of them) or by a wave
+    real *sums = shared + 2 * p.threads;
     __syncthreads();
     if (active) {
-        at[0] = a;
-        at[1] = b;
+        shared[2 * (segment * members + member)] = a;
+        shared[2 * (segment * members + member) + 1] = b;
     }
-    for (int left = members; left > 1;) {
-        const int half = (left + 1) / 2;
-        __syncthreads();
-        if (active && member + half < left) {
-            at[0] += at[2 * half];
-            at[1] += at[2 * half + 1];
+    __syncthreads();
+    if (members <= 8) {
+        if (active) {
+            const real *from = shared + 2 * segment * members;
+            a = from[0];
+            b = from[1];
+            for (int i = 1; i < members; i++) {
+                a += from[2 * i];
+                b += from[2 * i + 1];
+            }
         }
-        left = half;
+        return;
+    }
+    const int segments = p.teams * p.slab_groups, lane = threadIdx.x & (kWave - 1);
+    for (int s = threadIdx.x / kWave; s < segments; s += p.threads / kWave) {
+        real first = 0, second = 0;
+        for (int i = lane; i < members; i += kWave) {
+            first += shared[2 * (s * members + i)];
+            second += shared[2 * (s * members + i) + 1];
+        }
+        first = sum_lanes(first, kWave);
+        second = sum_lanes(second, kWave);
+        if (lane == 0) {
+            sums[2 * s] = first;
+            sums[2 * s + 1] = second;
+        }
     }
     __syncthreads();
     if (active) {
-        a = shared[2 * segment * members];
-        b = shared[2 * segment * members + 1];
+        a = sums[2 * segment];
+        b = sums[2 * segment + 1];
     }
 }
 
@@ -725,7 +744,8 @@ static Held held_of(const NormShape &m, int vector, int64_t bytes) {
     const int64_t most = 1024 / units;  // rows at a time of the largest workgroup
     if (m.positions > most * kHeldRows) return p;
     // few accesses a thread where there are few positions, more where it takes them
-    p.rows = (int)std::min<int64_t>(m.positions, m.positions <= most ? m.positions : most);
+    p.rows = (int)std::min<int64_t>(m.positions, std::max<int64_t>(ceil_div64(m.positions, kHeldRows), std::max<int64_t>(1, 256 / units)));
+    if (p.rows > most) p.rows = (int)most;
     const int line = p.rows * p.units;
     p.teams = (int)std::max<int64_t>(1, std::min<int64_t>(m.samples, (line < 256 ? 256 : 1024) / line));
     p.threads = (p.teams * line + kWave - 1) / kWave * kWave;
@@ -734,7 +754,7 @@ static Held held_of(const NormShape &m, int vector, int64_t bytes) {
     return p;
 }
 static size_t held_lds(const Held &p, int vector, bool backward) {
-    return sizeof(real) * std::max<size_t>(p.in_wave ? 0 : 2 * (size_t)p.threads, backward ? (size_t)p.threads * vector : 0);
+    return sizeof(real) * std::max<size_t>(p.in_wave ? 0 : 2 * ((size_t)p.threads + (size_t)p.teams * p.slab_groups), backward ? (size_t)p.threads * vector : 0);
 }
 
 static Streamed streamed_of(const NormShape &m, int vector) {

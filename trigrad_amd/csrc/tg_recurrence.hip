@@ -214,8 +214,10 @@ static Split split_of(const Shape &s, bool packed, int64_t wide_gates, int vecto
     };
     const int64_t wanted = columns(best, 6), axis = packed ? m.rows : s.length;
     const int narrow = std::min(6, log2_above(wanted));  // lanes of a row where there are many rows
-    m.chained = axis > kChunk >> narrow;
-    const int threads = backward ? kBackwardThreads : kForwardThreads, rows = backward ? kBackwardRows : kForwardRows;
+    m.kept_rows = kBackwardChunk >> narrow;
+    m.chained = axis > m.kept_rows;
+    const int threads = backward ? kBackwardThreads : kForwardThreads;
+    const int rows = backward ? kBackwardRows : kForwardRows;
     const int threads_log2 = log2_above(threads);
     m.lanes_log2 = narrow;
     if (!m.chained) m.lanes_log2 = std::min(log2_above(wanted), std::max(narrow, threads_log2 - log2_above(ceil_div64(axis, rows))));
@@ -248,13 +250,13 @@ static int sizes_of(const char *fn, const tg_recurrence &r, const Shape &m, int6
     for (int aligned = 0; aligned < 2; aligned++)
         for (int backward = 0; backward < 2; backward++) {
             const Split s = split_of(m, packed, 0, vector_of(m.shared, m.channels, aligned), backward);
-            if (s.chunks * s.tiles >= (1 << 22)) {
+            if (s.chunks * s.tiles >= (1 << 24) || (!packed && m.length <= kShortRows && m.sequences * s.columns >= ((int64_t)1 << 32))) {
                 set_error("%s: %lld rows of %lld channels are too many", fn, (long long)s.rows, (long long)s.channels);
                 return TG_E_ARG;
             }
             const Room room = room_of(s, backward);
             out[1 + backward] = std::max(out[1 + backward], room.all);
-            out[0] = room.starts;
+            out[0] = s.chained ? ceil_div64(s.rows, s.kept_rows) * s.channels * 4 : 0;
         }
     return 0;
 }
@@ -278,11 +280,11 @@ static int run(const tg_recurrence &r, const Shape &s, bool backward) {
     float *starts = (float *)(at + room.sequences);
     MapWords *maps = (MapWords *)(at + room.sequences + room.starts);
     float *partial = (float *)(at + room.sequences + room.starts + room.maps);
-    if (!backward && r.kept) starts = (float *)r.kept;
     if (m.packed)
         if (const int code = launch_prepare(m, first_sequence, r.offsets, from, to, stream)) return code;
     if (m.chained)
         if (const int code = launch_starts(r, m, first_sequence, maps, starts, vector, backward, stream)) return code;
+    if (!m.packed && m.length <= kShortRows) return launch_short(r, m, partial, vector, backward, stream);
     const unsigned blocks = (unsigned)(m.chunks * m.tiles);
     return backward ? launch_backward(r, m, first_sequence, starts, partial, vector, blocks, stream)
                     : launch_forward(r, m, first_sequence, starts, vector, blocks, stream);

@@ -10,7 +10,7 @@
 namespace tg {
 
 template <class T, int V, bool Shared, int K, int Threads>
-__global__ __launch_bounds__(Threads) void recurrence_backward_kernel(Split m, const int32_t *__restrict__ first_sequence,
+__global__ __launch_bounds__(Threads, Shared ? 4 : 3) void recurrence_backward_kernel(Split m, const int32_t *__restrict__ first_sequence,
                                                                       const float *__restrict__ starts, const T *__restrict__ inputs, const void *__restrict__ gates,
                                                                       const float *__restrict__ initial, const int32_t *__restrict__ offsets,
                                                                       const float *__restrict__ kept, const T *__restrict__ grad_states,
@@ -52,7 +52,8 @@ __global__ __launch_bounds__(Threads) void recurrence_backward_kernel(Split m, c
     }
 
     uint32_t firsts = 0, lasts = 0, outside = 0;
-    if (!inside_one_sequence(m, first_sequence, offsets, chunk)) {
+    const bool open = inside_one_sequence(m, first_sequence, offsets, chunk);
+    if (!open) {
         chunk_table<Threads>(m, first_sequence, offsets, chunk, places, table);
         __syncthreads();
         const Marks marks = marks_of(table + at, n);
@@ -83,39 +84,46 @@ __global__ __launch_bounds__(Threads) void recurrence_backward_kernel(Split m, c
     const auto end = [&](int k, int v) {
         return grad_final && !(outside >> k & 1) && valid ? grad_final[sequence_of(table[at + k]) * m.channels + channel + v] : 0.0f;
     };
-    const auto input = [&](int k, int v) { return m.complement ? rest[k][Shared ? 0 : v] * x[k][v] : x[k][v]; };
-
+    // Where none of the wave's rows begins or ends a sequence the loops know it, and the form of the input too.
     const bool marked = __any((firsts | lasts) != 0);
+    const auto by_rows = [&](auto &&call) {
+        if (marked) call(std::true_type(), std::integral_constant<int, 2>());
+        else if (!Shared) call(std::false_type(), std::integral_constant<int, 2>());
+        else if (m.complement) call(std::false_type(), std::integral_constant<int, 1>());
+        else call(std::false_type(), std::integral_constant<int, 0>());
+    };
+    const auto input = [&](auto form, int k, int v) {
+        const bool complement = decltype(form)::value == 2 ? m.complement : decltype(form)::value == 1;
+        return complement ? rest[k][Shared ? 0 : v] * x[k][v] : x[k][v];
+    };
+
 
     // the states again
+    const bool alone = Threads >> m.lanes_log2 == 1;  // a thread has all rows of its chunk: nothing comes from another
     Map<V> map = unit_map<V>();
     map.closed = firsts != 0;
-    const auto map_of_states = [&](auto with_marks) {
+    if (!alone) by_rows([&](auto with_marks, auto form) {
 #pragma unroll
         for (int k = 0; k < K; k++)
 #pragma unroll
             for (int v = 0; v < V; v++) {
                 if (with_marks.value && (firsts >> k & 1)) map.u[v] = begin(k, v);
-                map.u[v] = fmaf(a[k][Shared ? 0 : v], map.u[v], input(k, v));
+                map.u[v] = fmaf(a[k][Shared ? 0 : v], map.u[v], input(form, k, v));
                 map.a[v] *= a[k][Shared ? 0 : v];
             }
-    };
-    if (marked) map_of_states(std::true_type());
-    else map_of_states(std::false_type());
+    });
     float before[K][V];
-    join<V, Threads, false>(m, joint, p, map, h);
-    const auto walk_states = [&](auto with_marks) {
+    if (!alone) join<V, Threads, false>(m, joint, p, map, open, h);
+    by_rows([&](auto with_marks, auto form) {
 #pragma unroll
         for (int k = 0; k < K; k++)
 #pragma unroll
             for (int v = 0; v < V; v++) {
                 if (with_marks.value && (firsts >> k & 1)) h[v] = begin(k, v);
                 before[k][v] = h[v];
-                h[v] = fmaf(a[k][Shared ? 0 : v], h[v], input(k, v));
+                h[v] = fmaf(a[k][Shared ? 0 : v], h[v], input(form, k, v));
             }
-    };
-    if (marked) walk_states(std::true_type());
-    else walk_states(std::false_type());
+    });
 
     // what reaches the last of the thread's rows from behind
     map = unit_map<V>();
@@ -130,20 +138,23 @@ __global__ __launch_bounds__(Threads) void recurrence_backward_kernel(Split m, c
                 map.a[v] *= a[k][Shared ? 0 : v];
             }
     };
-    if (marked) map_of_gradients(std::true_type());
-    else map_of_gradients(std::false_type());
-    __syncthreads();
-    join<V, Threads, true>(m, joint, p, map, e);
+    if (!alone) {
+        if (marked) map_of_gradients(std::true_type());
+        else map_of_gradients(std::false_type());
+        __syncthreads();
+        join<V, Threads, true>(m, joint, p, map, open, e);
+    }
 
     float q[K];  // of a shared gate: the sum over the lane's channels
     // dx of row k, and da in its place in before[]
-    const auto gradients = [&](auto with_marks, int k, float (&dx)[V]) {
+    const auto gradients = [&](auto with_marks, auto form, int k, float (&dx)[V]) {
+        const bool complement = decltype(form)::value == 2 ? m.complement : decltype(form)::value == 1;
 #pragma unroll
         for (int v = 0; v < V; v++) {
             if (with_marks.value && (lasts >> k & 1)) e[v] = end(k, v);
             const float l = e[v] + dh[k][v];
-            dx[v] = m.complement ? rest[k][Shared ? 0 : v] * l : l;
-            before[k][v] = l * (m.complement ? before[k][v] - x[k][v] : before[k][v]);
+            dx[v] = complement ? rest[k][Shared ? 0 : v] * l : l;
+            before[k][v] = l * (complement ? before[k][v] - x[k][v] : before[k][v]);
             e[v] = a[k][Shared ? 0 : v] * l;
         }
         if (Shared) {
@@ -162,10 +173,13 @@ __global__ __launch_bounds__(Threads) void recurrence_backward_kernel(Split m, c
     const bool wide = sizeof(T) == 4 || m.wide_gates;
     if (w.whole && !marked) {
         const Walk back = against<K>(w);
-        each_row<K>(back, cx, grad_inputs ? grad_inputs : const_cast<T *>(inputs), [&](int i, T *to) {
-            float dx[V];
-            gradients(std::false_type(), K - 1 - i, dx);
-            if (grad_inputs && valid) store_pack<V>(to, dx);
+        by_rows([&](auto with_marks, auto form) {
+            if (with_marks.value) return;
+            each_row<K>(back, cx, grad_inputs ? grad_inputs : const_cast<T *>(inputs), [&](int i, T *to) {
+                float dx[V];
+                gradients(with_marks, form, K - 1 - i, dx);
+                if (grad_inputs && valid) store_pack<V>(to, dx);
+            });
         });
         if (!Shared && grad_gates && valid) {
             if (wide)
@@ -185,7 +199,7 @@ __global__ __launch_bounds__(Threads) void recurrence_backward_kernel(Split m, c
 #pragma unroll
         for (int k = K - 1; k >= 0; k--) {
             float dx[V], dg[V];
-            gradients(std::true_type(), k, dx);
+            gradients(std::true_type(), std::integral_constant<int, 2>(), k, dx);
             if (!valid || k >= n) continue;
             const int64_t row = w.row + k * w.step;
             if (grad_inputs) store_pack<V>(grad_inputs + row * m.channels + channel, dx);
@@ -255,13 +269,20 @@ int launch_backward(const tg_recurrence &r, const Split &m, const int32_t *first
         TG_LAUNCH_AS("recurrence_backward", (recurrence_backward_kernel<T, decltype(v)::value, Shared, K, Threads>), dim3(blocks), dim3(Threads),
                      table_bytes(m, Threads * K), stream, m, first_sequence, starts, (const T *)r.inputs, r.gates, r.initial, r.offsets,
                      (const float *)r.kept, (const T *)r.grad_states, r.grad_final, (T *)r.grad_inputs, r.grad_gates, r.grad_initial, partial);
-        if (Shared && r.grad_gates && m.parts > 1) {
-            const unsigned sum_blocks = (unsigned)std::min<int64_t>(ceil_div64(m.rows * m.gates, 256), 4096);
-            TG_LAUNCH_AS("recurrence_gate_sums", (recurrence_gate_sums_kernel<T>), dim3(sum_blocks), dim3(256), 0, stream, m, r.gates, partial,
-                         r.grad_gates);
-        }
-        return check_launch("tg_linear_recurrence_backward");
+        const int code = check_launch("tg_linear_recurrence_backward");
+        return code ? code : launch_gate_sums(r, m, partial, stream);
     });
+}
+
+int launch_gate_sums(const tg_recurrence &r, const Split &m, const float *partial, hipStream_t stream) {
+    if (m.shared == 1 || !r.grad_gates || m.parts == 1) return 0;
+    const unsigned blocks = (unsigned)std::min<int64_t>(ceil_div64(m.rows * m.gates, 256), 4096);
+    const auto with = [&](auto t) {
+        TG_LAUNCH_AS("recurrence_gate_sums", (recurrence_gate_sums_kernel<decltype(t)>), dim3(blocks), dim3(256), 0, stream, m, r.gates, partial,
+                     r.grad_gates);
+        return check_launch("tg_linear_recurrence_backward");
+    };
+    return r.type == TG_TYPE_F32 ? with(float()) : r.type == TG_TYPE_F16 ? with(half_t()) : with(bf16_t());
 }
 
 }  // namespace tg

@@ -8,7 +8,7 @@ template <class T, int V, bool Shared, int K, int Threads>
 __global__ __launch_bounds__(Threads, 4) void recurrence_forward_kernel(Split m, const int32_t *__restrict__ first_sequence,
                                                                      const float *__restrict__ starts, const T *__restrict__ inputs, const void *__restrict__ gates,
                                                                      const float *__restrict__ initial, const int32_t *__restrict__ offsets,
-                                                                     T *__restrict__ states, float *__restrict__ final) {
+                                                                     T *__restrict__ states, float *__restrict__ final, float *__restrict__ kept) {
     constexpr int GV = Shared ? 1 : V;
     extern __shared__ uint32_t table[];
     __shared__ Joint<V, Threads> joint;
@@ -29,7 +29,8 @@ __global__ __launch_bounds__(Threads, 4) void recurrence_forward_kernel(Split m,
     read_gates<T, K, GV>(m, gates, w, cg, a);
 
     uint32_t firsts = 0, lasts = 0, outside = 0;
-    if (!inside_one_sequence(m, first_sequence, offsets, chunk)) {
+    const bool open = inside_one_sequence(m, first_sequence, offsets, chunk);
+    if (!open) {
         chunk_table<Threads>(m, first_sequence, offsets, chunk, places, table);
         __syncthreads();
         const Marks marks = marks_of(table + at, n);
@@ -67,8 +68,10 @@ __global__ __launch_bounds__(Threads, 4) void recurrence_forward_kernel(Split m,
         return initial && !(outside >> k & 1) && valid ? initial[sequence_of(table[at + k]) * m.channels + channel + v] : 0.0f;
     };
 
+    const bool alone = Threads >> m.lanes_log2 == 1;  // a thread has all rows of its chunk: nothing comes from another
     Map<V> map = unit_map<V>();
-    if (!firsts) {
+    if (alone) {
+    } else if (!firsts) {
 #pragma unroll
         for (int k = 0; k < K; k++)
 #pragma unroll
@@ -89,8 +92,12 @@ __global__ __launch_bounds__(Threads, 4) void recurrence_forward_kernel(Split m,
     float h[V];
 #pragma unroll
     for (int v = 0; v < V; v++) h[v] = m.chained ? starts[chunk * m.channels + channel + v] : 0.0f;
-    join<V, Threads, false>(m, joint, p, map, h);
+    if (!alone) join<V, Threads, false>(m, joint, p, map, open, h);
     if (!valid || n == 0) return;
+    if (kept && at % (int)m.kept_rows == 0) {
+#pragma unroll
+        for (int v = 0; v < V; v++) kept[(start + at) / m.kept_rows * m.channels + channel + v] = h[v];
+    }
     if (w.whole && !(firsts | lasts)) {
         if (!states) return;
         each_row<K>(w, cx, states, [&](int k, T *to) {
@@ -121,7 +128,7 @@ template <class T, int V, bool Shared, bool Backward>
 __global__ __launch_bounds__(kMapThreads) void recurrence_maps_kernel(Split m, const int32_t *__restrict__ first_sequence, const T *__restrict__ inputs,
                                                                       const void *__restrict__ gates, const float *__restrict__ ends,
                                                                       const int32_t *__restrict__ offsets, MapWords *__restrict__ maps) {
-    constexpr int GV = Shared ? 1 : V, Threads = kMapThreads, Rows = kChunk / Threads;
+    constexpr int GV = Shared ? 1 : V, Threads = kMapThreads, Rows = (Backward ? kBackwardChunk : kForwardChunk) / Threads;
     extern __shared__ uint32_t table[];
     __shared__ Joint<V, Threads> joint;
     int64_t channel, gate;
@@ -233,21 +240,22 @@ __global__ __launch_bounds__(kMapThreads) void recurrence_maps_kernel(Split m, c
     }
 }
 
-// The states that the chunks start from.  A wave goes over a run of chunks for 64 channels, twice: for the run's map, and, once the runs before
-// are known, from their state.
-constexpr int kStartWaves = 16, kStartAhead = 16;
-__global__ __launch_bounds__(kStartWaves * kWave) void recurrence_starts_kernel(int64_t chunks, int64_t channels, bool backward,
-                                                                                const MapWords *__restrict__ maps, float *__restrict__ starts) {
-    __shared__ Joint<1, kStartWaves * kWave> joint;
-    const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x >> 6;
-    const int64_t channel = (int64_t)blockIdx.x * kWave + lane, run = (chunks + kStartWaves - 1) / kStartWaves;
-    const int64_t begin = min(wave * run, chunks), end = min(begin + run, chunks);
+// The states that the chunks start from: the chunks' maps composed as a thread's rows are, 16 channels and 64 runs of chunks a workgroup.
+constexpr int kStartThreads = 1024, kStartLanesLog2 = 4, kStartAhead = 8;
+__global__ __launch_bounds__(kStartThreads) void recurrence_starts_kernel(int64_t chunks, int64_t channels, bool backward,
+                                                                          const MapWords *__restrict__ maps, float *__restrict__ starts) {
+    __shared__ Joint<1, kStartThreads> joint;
+    Split m = {};
+    m.lanes_log2 = kStartLanesLog2;
+    const Place p = place_of<kStartThreads>(m);
+    const int64_t channel = ((int64_t)blockIdx.x << kStartLanesLog2) + p.lane, turns = kStartThreads >> kStartLanesLog2, run = (chunks + turns - 1) / turns;
+    const int64_t begin = min(p.turn * run, chunks), end = min(begin + run, chunks);
     const bool valid = channel < channels;
     MapWords next[kStartAhead];
     const auto read = [&](int64_t i) {
 #pragma unroll
         for (int k = 0; k < kStartAhead; k++) {
-            const int64_t c = min(i + k, end - 1);
+            const int64_t c = min(i + k, max(end - 1, (int64_t)0));
             next[k] = maps[(backward ? chunks - 1 - c : c) * channels + (valid ? channel : 0)];
         }
     };
@@ -269,12 +277,8 @@ __global__ __launch_bounds__(kStartWaves * kWave) void recurrence_starts_kernel(
             total = map;
         });
     }
-    joint.a[threadIdx.x] = total.a[0];
-    joint.u[threadIdx.x] = total.u[0];
-    if (lane == 0) joint.closed[wave] = total.closed;
-    __syncthreads();
     float h[1] = {0.0f};
-    for (int i = 0; i < wave; i++) step_over(h, joint.at(i, kWave, lane));
+    join<1, kStartThreads, false>(m, joint, p, total, false, h);
     for (int64_t i = begin; i < end; i += kStartAhead) {
         if (run > kStartAhead) read(i);
         over(i, [&](int64_t c, const Map<1> &map) {
@@ -316,7 +320,7 @@ int launch_forward(const tg_recurrence &r, const Split &m, const int32_t *first_
         constexpr int K = kForwardRows, Threads = kForwardThreads;
         TG_LAUNCH_AS("recurrence_forward", (recurrence_forward_kernel<T, decltype(v)::value, decltype(shared)::value, K, Threads>), dim3(blocks),
                      dim3(Threads), table_bytes(m, Threads * K), stream, m, first_sequence, starts, (const T *)r.inputs, r.gates, r.initial, r.offsets,
-                     (T *)r.states, r.final);
+                     (T *)r.states, r.final, m.chained ? (float *)r.kept : nullptr);
         return check_launch("tg_linear_recurrence_forward");
     });
 }
@@ -329,15 +333,16 @@ int launch_starts(const tg_recurrence &r, const Split &m, const int32_t *first_s
         constexpr int V = decltype(v)::value;
         constexpr bool Shared = decltype(shared)::value;
         if (backward)
-            TG_LAUNCH_AS("recurrence_maps_backward", (recurrence_maps_kernel<T, V, Shared, true>), dim3(blocks), dim3(kMapThreads), table_bytes(m, kChunk),
+            TG_LAUNCH_AS("recurrence_maps_backward", (recurrence_maps_kernel<T, V, Shared, true>), dim3(blocks), dim3(kMapThreads), table_bytes(m, kBackwardChunk),
                          stream, m, first_sequence, (const T *)r.grad_states, r.gates, r.grad_final, r.offsets, maps);
         else
-            TG_LAUNCH_AS("recurrence_maps", (recurrence_maps_kernel<T, V, Shared, false>), dim3(blocks), dim3(kMapThreads), table_bytes(m, kChunk), stream,
+            TG_LAUNCH_AS("recurrence_maps", (recurrence_maps_kernel<T, V, Shared, false>), dim3(blocks), dim3(kMapThreads), table_bytes(m, kForwardChunk), stream,
                          m, first_sequence, (const T *)r.inputs, r.gates, r.initial, r.offsets, maps);
         return check_launch("tg_linear_recurrence");
     });
     if (code) return code;
-    TG_LAUNCH_AS("recurrence_starts", recurrence_starts_kernel, dim3((unsigned)ceil_div64(m.channels, kWave)), dim3(kStartWaves * kWave), 0, stream,
+    TG_LAUNCH_AS("recurrence_starts", recurrence_starts_kernel, dim3((unsigned)ceil_div64(m.channels, 1 << kStartLanesLog2)), dim3(kStartThreads), 0,
+                 stream,
                  m.chunks, m.channels, backward, maps, starts);
     return check_launch("tg_linear_recurrence");
 }

@@ -16,6 +16,7 @@
 // that orders such workgroups, the words to wait on and their clearing came on top (4 x 4096 x 2048, 16 gates: backward 148 us, with
 // every wait left out 66).
 #pragma once
+#include <cfloat>
 #include <algorithm>
 #include <type_traits>
 
@@ -23,11 +24,13 @@
 
 namespace tg {
 
-constexpr int kChunk = 8192;  // rows of a chunk x lanes of a row, where there are several chunks to a sequence
-constexpr int kForwardThreads = 512, kForwardRows = 16;    // rows of a thread; at most 32, a bit each
-constexpr int kBackwardThreads = 1024, kBackwardRows = 8;
-constexpr int kMapThreads = 512;
-static_assert(kForwardThreads * kForwardRows == kChunk && kBackwardThreads * kBackwardRows == kChunk, "");
+// Rows of a thread (at most 32, a bit each) and threads; their product is a chunk's rows x lanes of a row, where there are several chunks to
+// a sequence.  A forward chunk is a whole number of backward ones: the states in front of those are what the forward call keeps.
+constexpr int kForwardThreads = 256, kForwardRows = 16, kForwardChunk = kForwardThreads * kForwardRows;
+constexpr int kShortRows = 8;  // sequences of no more have kernels of their own
+constexpr int kBackwardThreads = 256, kBackwardRows = 8, kBackwardChunk = kBackwardThreads * kBackwardRows;
+constexpr int kMapThreads = 256;
+static_assert(kForwardChunk % kBackwardChunk == 0 && kForwardChunk % (8 * kMapThreads) == 0 && kBackwardChunk % (8 * kMapThreads) == 0, "");
 constexpr uint32_t kClosedMap = 0xfffffffeu;  // in the place of a map's factor: closed
 
 // Rows in the order of the recurrence ("places"): row = reverse ? rows - 1 - place : place.  Columns are lanes: a lane has V successive
@@ -36,6 +39,7 @@ struct Split {
     int64_t rows, channels, gates, shared, length, sequences;
     int64_t chunks, columns, tiles;  // columns: lanes of a row, padding included
     int64_t chunk_rows;
+    int64_t kept_rows;               // rows between two states that the forward call keeps
     int lanes_log2, gate_lanes_log2, parts;
     int gate_form, wide_gates;       // gates are float whatever T is
     bool complement, reverse, chained, packed;  // chained: chunks do not all begin with a sequence
@@ -65,6 +69,9 @@ template <int V> struct Map {
 
 // A factor may have left the range of float32 while the state it is applied to is 0: that stays 0.
 __device__ __forceinline__ float apply(float a, float h, float u) { return h == 0.0f ? u : fmaf(a, h, u); }
+
+// A factor that left the range as the largest number: times 0 that is 0.  (NaN becomes a number too: then the map's u is NaN.)
+__device__ __forceinline__ float bounded(float a) { return __builtin_amdgcn_fmed3f(a, -FLT_MAX, FLT_MAX); }
 
 template <int V> __device__ __forceinline__ void compose(Map<V> &later, const Map<V> &earlier) {
 #pragma unroll
@@ -404,7 +411,7 @@ __device__ __forceinline__ Map<V> gather(const Split &m, Joint<V, Threads> &j, c
     if (stores) {
 #pragma unroll
         for (int v = 0; v < V; v++) {
-            j.a[(p.entry * lanes + p.lane) * V + v] = map.a[v];
+            j.a[(p.entry * lanes + p.lane) * V + v] = bounded(map.a[v]);
             j.u[(p.entry * lanes + p.lane) * V + v] = map.u[v];
         }
         if (p.lane == 0) j.closed[p.entry] = map.closed;
@@ -413,12 +420,22 @@ __device__ __forceinline__ Map<V> gather(const Split &m, Joint<V, Threads> &j, c
     return before;
 }
 
-// What the thread's own rows start from; h on entry is what the chunk starts from.
+// What the thread's own rows start from; h on entry is what the chunk starts from.  open: no map of the chunk is closed.
 template <int V, int Threads, bool Backward>
-__device__ __forceinline__ void join(const Split &m, Joint<V, Threads> &j, const Place &p, const Map<V> &map, float (&h)[V]) {
+__device__ __forceinline__ void join(const Split &m, Joint<V, Threads> &j, const Place &p, const Map<V> &map, bool open, float (&h)[V]) {
     const Map<V> before = gather<V, Threads, Backward>(m, j, p, map);
-    const int mine = Backward ? p.entries - 1 - p.entry : p.entry;
-    for (int i = 0; i < mine; i++) step_over(h, j.at(Backward ? p.entries - 1 - i : i, 1 << m.lanes_log2, p.lane));
+    const int mine = Backward ? p.entries - 1 - p.entry : p.entry, lanes = 1 << m.lanes_log2;
+    if (open) {
+        const int step = Backward ? -lanes * V : lanes * V;
+        int at = ((Backward ? p.entries - 1 : 0) * lanes + p.lane) * V;
+#pragma unroll 4
+        for (int i = 0; i < mine; i++, at += step)
+#pragma unroll
+            for (int v = 0; v < V; v++) h[v] = fmaf(j.a[at + v], h[v], j.u[at + v]);
+        if (m.lanes_log2 < 6) step_over(h, before);
+        return;
+    }
+    for (int i = 0; i < mine; i++) step_over(h, j.at(Backward ? p.entries - 1 - i : i, lanes, p.lane));
     step_over(h, before);
 }
 
@@ -446,6 +463,10 @@ int launch_forward(const tg_recurrence &r, const Split &m, const int32_t *first_
                    hipStream_t stream);
 int launch_backward(const tg_recurrence &r, const Split &m, const int32_t *first_sequence, const float *starts, float *partial, int vector,
                     unsigned blocks, hipStream_t stream);
+// The sum of the waves' sums, where a gate has more channels than a wave.
+int launch_gate_sums(const tg_recurrence &r, const Split &m, const float *partial, hipStream_t stream);
+// Sequences of at most kShortRows rows, none of them of another length.
+int launch_short(const tg_recurrence &r, const Split &m, float *partial, int vector, bool backward, hipStream_t stream);
 int launch_prepare(const Split &m, int32_t *first_sequence, const int32_t *offsets, const float *from, float *to, hipStream_t stream);
 // The states (backward: what comes from behind) that the chunks of `m` start from.
 int launch_starts(const tg_recurrence &r, const Split &m, const int32_t *first_sequence, MapWords *maps, float *starts, int vector, bool backward,
