@@ -240,8 +240,8 @@ __global__ __launch_bounds__(kMapThreads) void recurrence_maps_kernel(Split m, c
     }
 }
 
-// The states that the chunks start from: the chunks' maps composed as a thread's rows are, 16 channels and 64 runs of chunks a workgroup.
-constexpr int kStartThreads = 1024, kStartLanesLog2 = 4, kStartAhead = 8;
+// The states that the chunks start from: the chunks' maps composed as a thread's rows are, 8 channels and 128 runs of chunks a workgroup.
+constexpr int kStartThreads = 1024, kStartLanesLog2 = 3, kStartAhead = 8;
 __global__ __launch_bounds__(kStartThreads) void recurrence_starts_kernel(int64_t chunks, int64_t channels, bool backward,
                                                                           const MapWords *__restrict__ maps, float *__restrict__ starts) {
     __shared__ Joint<1, kStartThreads> joint;
