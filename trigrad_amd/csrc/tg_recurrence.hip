@@ -215,9 +215,10 @@ static Split split_of(const Shape &s, bool packed, int64_t wide_gates, int vecto
     const int64_t wanted = columns(best, 6), axis = packed ? m.rows : s.length;
     const int narrow = std::min(6, log2_above(wanted));  // lanes of a row where there are many rows
     m.kept_rows = kBackwardChunk >> narrow;
-    m.chained = axis > m.kept_rows;
-    const int threads = backward ? kBackwardThreads : kForwardThreads;
-    const int rows = backward ? kBackwardRows : kForwardRows;
+    m.chained = axis > kWideChunk >> narrow;
+    m.wide = !m.chained && axis > m.kept_rows;
+    const int threads = m.wide ? kWideThreads : backward ? kBackwardThreads : kForwardThreads;
+    const int rows = m.wide ? kWideRows : backward ? kBackwardRows : kForwardRows;
     const int threads_log2 = log2_above(threads);
     m.lanes_log2 = narrow;
     if (!m.chained) m.lanes_log2 = std::min(log2_above(wanted), std::max(narrow, threads_log2 - log2_above(ceil_div64(axis, rows))));
@@ -250,7 +251,7 @@ static int sizes_of(const char *fn, const tg_recurrence &r, const Shape &m, int6
     for (int aligned = 0; aligned < 2; aligned++)
         for (int backward = 0; backward < 2; backward++) {
             const Split s = split_of(m, packed, 0, vector_of(m.shared, m.channels, aligned), backward);
-            if (s.chunks * s.tiles >= (1 << 24) || (!packed && m.length <= kShortRows && m.sequences * s.columns >= ((int64_t)1 << 32))) {
+            if (s.chunks * s.tiles >= (s.wide ? 1 << 22 : 1 << 24) || (!packed && m.length <= kShortRows && m.sequences * s.columns >= ((int64_t)1 << 32))) {
                 set_error("%s: %lld rows of %lld channels are too many", fn, (long long)s.rows, (long long)s.channels);
                 return TG_E_ARG;
             }

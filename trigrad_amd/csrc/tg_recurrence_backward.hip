@@ -10,7 +10,7 @@
 namespace tg {
 
 template <class T, int V, bool Shared, int K, int Threads>
-__global__ __launch_bounds__(Threads, Shared ? 4 : 3) void recurrence_backward_kernel(Split m, const int32_t *__restrict__ first_sequence,
+__global__ __launch_bounds__(Threads, Shared || Threads == kWideThreads ? 4 : 3) void recurrence_backward_kernel(Split m, const int32_t *__restrict__ first_sequence,
                                                                       const float *__restrict__ starts, const T *__restrict__ inputs, const void *__restrict__ gates,
                                                                       const float *__restrict__ initial, const int32_t *__restrict__ offsets,
                                                                       const float *__restrict__ kept, const T *__restrict__ grad_states,
@@ -264,12 +264,16 @@ int launch_backward(const tg_recurrence &r, const Split &m, const int32_t *first
                     unsigned blocks, hipStream_t stream) {
     return by_layout(r.type, vector, m.shared, [&](auto t, auto v, auto shared) {
         using T = decltype(t);
-        constexpr int K = kBackwardRows, Threads = kBackwardThreads;
-        constexpr bool Shared = decltype(shared)::value;
-        TG_LAUNCH_AS("recurrence_backward", (recurrence_backward_kernel<T, decltype(v)::value, Shared, K, Threads>), dim3(blocks), dim3(Threads),
-                     table_bytes(m, Threads * K), stream, m, first_sequence, starts, (const T *)r.inputs, r.gates, r.initial, r.offsets,
-                     (const float *)r.kept, (const T *)r.grad_states, r.grad_final, (T *)r.grad_inputs, r.grad_gates, r.grad_initial, partial);
-        const int code = check_launch("tg_linear_recurrence_backward");
+        const auto with = [&](auto rows, auto threads) {
+            constexpr int K = decltype(rows)::value, Threads = decltype(threads)::value;
+            TG_LAUNCH_AS("recurrence_backward", (recurrence_backward_kernel<T, decltype(v)::value, decltype(shared)::value, K, Threads>), dim3(blocks),
+                         dim3(Threads), table_bytes(m, Threads * K), stream, m, first_sequence, starts, (const T *)r.inputs, r.gates, r.initial,
+                         r.offsets, (const float *)r.kept, (const T *)r.grad_states, r.grad_final, (T *)r.grad_inputs, r.grad_gates,
+                         r.grad_initial, partial);
+            return check_launch("tg_linear_recurrence_backward");
+        };
+        const int code = m.wide ? with(std::integral_constant<int, kWideRows>(), std::integral_constant<int, kWideThreads>())
+                                : with(std::integral_constant<int, kBackwardRows>(), std::integral_constant<int, kBackwardThreads>());
         return code ? code : launch_gate_sums(r, m, partial, stream);
     });
 }

@@ -317,11 +317,15 @@ int launch_forward(const tg_recurrence &r, const Split &m, const int32_t *first_
                    hipStream_t stream) {
     return by_layout(r.type, vector, m.shared, [&](auto t, auto v, auto shared) {
         using T = decltype(t);
-        constexpr int K = kForwardRows, Threads = kForwardThreads;
-        TG_LAUNCH_AS("recurrence_forward", (recurrence_forward_kernel<T, decltype(v)::value, decltype(shared)::value, K, Threads>), dim3(blocks),
-                     dim3(Threads), table_bytes(m, Threads * K), stream, m, first_sequence, starts, (const T *)r.inputs, r.gates, r.initial, r.offsets,
-                     (T *)r.states, r.final, m.chained ? (float *)r.kept : nullptr);
-        return check_launch("tg_linear_recurrence_forward");
+        const auto with = [&](auto rows, auto threads) {
+            constexpr int K = decltype(rows)::value, Threads = decltype(threads)::value;
+            TG_LAUNCH_AS("recurrence_forward", (recurrence_forward_kernel<T, decltype(v)::value, decltype(shared)::value, K, Threads>), dim3(blocks),
+                         dim3(Threads), table_bytes(m, Threads * K), stream, m, first_sequence, starts, (const T *)r.inputs, r.gates, r.initial,
+                         r.offsets, (T *)r.states, r.final, m.chained ? (float *)r.kept : nullptr);
+            return check_launch("tg_linear_recurrence_forward");
+        };
+        return m.wide ? with(std::integral_constant<int, kWideRows>(), std::integral_constant<int, kWideThreads>())
+                      : with(std::integral_constant<int, kForwardRows>(), std::integral_constant<int, kForwardThreads>());
     });
 }
 

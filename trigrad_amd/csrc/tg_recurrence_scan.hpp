@@ -30,6 +30,8 @@ constexpr int kForwardThreads = 256, kForwardRows = 16, kForwardChunk = kForward
 constexpr int kShortRows = 8;  // sequences of no more have kernels of their own
 constexpr int kBackwardThreads = 256, kBackwardRows = 8, kBackwardChunk = kBackwardThreads * kBackwardRows;
 constexpr int kMapThreads = 256;
+// Sequences of one chunk to about four have a large workgroup each instead: no first look, no starting states, one launch.
+constexpr int kWideThreads = 1024, kWideRows = 8, kWideChunk = kWideThreads * kWideRows;
 static_assert(kForwardChunk % kBackwardChunk == 0 && kForwardChunk % (8 * kMapThreads) == 0 && kBackwardChunk % (8 * kMapThreads) == 0, "");
 constexpr uint32_t kClosedMap = 0xfffffffeu;  // in the place of a map's factor: closed
 
@@ -42,6 +44,7 @@ struct Split {
     int64_t kept_rows;               // rows between two states that the forward call keeps
     int lanes_log2, gate_lanes_log2, parts;
     int gate_form, wide_gates;       // gates are float whatever T is
+    bool wide;                       // workgroups of kWideThreads
     bool complement, reverse, chained, packed;  // chained: chunks do not all begin with a sequence
 };
 
