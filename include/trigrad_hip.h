@@ -507,10 +507,10 @@ int tg_clip_to_render(const tg_real *clip, int64_t n_vertices, tg_real *out, voi
  *   a = f(gate): TG_GATE_VALUE the gate itself, TG_GATE_LOG exp(gate), TG_GATE_LOGIT 1 / (1 + exp(-gate));
  *   u = x (TG_INPUT_PLAIN) or (1 - a) x (TG_INPUT_COMPLEMENT).
  * Without offsets inputs is (sequences, length, channels); with them (length, channels), sequence s being the rows
- * offsets[s] to offsets[s + 1], which do not decrease, the first of them >= 0, the last <= length: rows of no sequence get
- * zeros, in the states and in the gradients.  gates has `gates` columns where inputs has `channels`: gate g is that of the channels
+ * offsets[s] to offsets[s + 1], which do not decrease (what lies outside of 0 and length counts as these): rows of
+ * no sequence get zeros, in the states and in the gradients.  gates has `gates` columns where inputs has `channels`: gate g is that of the channels
  * g * channels / gates up to the next gate's.  reverse: each sequence from its last row to its first.  Products of successive gates
- * of a sequence are formed, of up to 4096 of them: they have to be representable, which those of decays (|a| <= 1) are.
+ * of a sequence are formed: they have to be representable, which those of decays (|a| <= 1) are.
  * initial, final and their gradients are (sequences, channels) tg_real; initial, grad_states, grad_final, and every output
  * but `final` may be null.  The backward call reads inputs, gates, initial and offsets as the forward call did.  The final state of an empty sequence is its initial one.
  * tg_linear_recurrence_sizes writes the bytes of `kept` (what the forward call leaves for the backward call; null where none

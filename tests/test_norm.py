@@ -289,6 +289,47 @@ def test_other_streams_and_graphs(cuda, route):
 
 
 @pytest.mark.gpu
+def test_capture_beside_an_eager_graph_of_the_same_leaves(cuda, route):
+    import trigrad_amd
+    x, w, b, dy = make(cuda, 1, (2, 50, 32))
+    leaf = w.requires_grad_()
+    eager = trigrad_amd.group_norm(x, 4, leaf, b, activation="silu")
+    want = torch.autograd.grad(eager, leaf, dy, retain_graph=True)[0]
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+
+    def capture():
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=stream):
+            out = torch.autograd.grad(trigrad_amd.group_norm(x, 4, leaf, b, activation="silu"), leaf, dy)[0]
+        return graph, out
+    with pytest.raises(RuntimeError, match="made on another stream"):
+        capture()
+    del eager
+    graph, out = capture()
+    for _ in range(3):
+        out.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want)
+
+
+@pytest.mark.gpu
+def test_backward_twice_and_after_a_change(cuda, route):
+    import trigrad_amd
+    x, w, b, dy = make(cuda, 1, (2, 300, 16))
+    leaves = [t.requires_grad_() for t in (x, w, b)]
+    y = trigrad_amd.group_norm(*leaves[:1], 4, *leaves[1:], activation="silu")
+    first, second = (torch.autograd.grad(y, leaves, dy, retain_graph=True) for _ in range(2))
+    assert all(torch.equal(p, q) for p, q in zip(first, second))
+    with torch.no_grad():
+        w.add_(0.1)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        torch.autograd.grad(y, leaves, dy)
+    assert torch.equal(trigrad_amd.group_norm(x, np.int64(4)), trigrad_amd.group_norm(x, 4))
+
+
+@pytest.mark.gpu
 def test_more_elements_than_31_bits_count(cuda):
     """2^31 elements and some in samples of 2^20: the last sample against the definition."""
     import trigrad_amd

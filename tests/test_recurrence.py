@@ -399,6 +399,65 @@ def test_other_streams_and_graphs(cuda, route):
 
 
 @pytest.mark.gpu
+def test_capture_beside_an_eager_graph_of_the_same_leaves(cuda, route):
+    """The engine would join the eager graph's stream into the capture: refused, and taken once that graph is gone."""
+    import trigrad_amd
+    x, g, _, _ = make(cuda, 1, (2, 50), 32, 32)
+    leaf = x.requires_grad_()
+    eager = trigrad_amd.linear_recurrence(leaf, g)[0]
+    want = torch.autograd.grad(eager, leaf, torch.ones_like(eager), retain_graph=True)[0]
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+
+    def capture():
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=stream):
+            states, _ = trigrad_amd.linear_recurrence(leaf, g)
+            out = torch.autograd.grad(states, leaf, torch.ones_like(states))[0]
+        return graph, out
+    with pytest.raises(RuntimeError, match="made on another stream"):
+        capture()
+    del eager
+    graph, out = capture()
+    for _ in range(3):
+        out.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want)
+
+
+@pytest.mark.gpu
+def test_backward_twice_and_after_a_change(cuda, route):
+    import trigrad_amd
+    x, g, h0, _ = make(cuda, 1, (2, 300), 16, 16)
+    leaves = [t.requires_grad_() for t in (x, g, h0)]
+    states, final = trigrad_amd.linear_recurrence(*leaves)
+    first = torch.autograd.grad([states, final], leaves, [torch.ones_like(states), torch.ones_like(final)], retain_graph=True)
+    second = torch.autograd.grad([states, final], leaves, [torch.ones_like(states), torch.ones_like(final)], retain_graph=True)
+    assert all(torch.equal(a, b) for a, b in zip(first, second))
+    with torch.no_grad():
+        g.add_(0.1)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        torch.autograd.grad(states, leaves, torch.ones_like(states))
+    # a state that a step writes over is a change too
+    _, final = trigrad_amd.linear_recurrence(*leaves)
+    kept = final.square()
+    with torch.no_grad():
+        trigrad_amd.linear_recurrence_step(x[:, 0], g[:, 0], final.detach())
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        kept.sum().backward()
+
+
+@pytest.mark.gpu
+def test_offsets_beyond_the_rows_end_at_them(cuda):
+    import trigrad_amd
+    x, g, h0, _ = make(cuda, 1, (100,), 8, 8, sequences=4)
+    for given, meant in (([0, 40, 130, 150, 150], [0, 40, 100, 100, 100]), ([-7, 3, 3, 90, 1000], [0, 3, 3, 90, 100])):
+        a, b = (trigrad_amd.linear_recurrence(x, g, h0, torch.tensor(c, dtype=torch.int32, device=cuda)) for c in (given, meant))
+        assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+
+
+@pytest.mark.gpu
 def test_more_elements_than_31_bits_count(cuda):
     """2^31 elements and some: the last rows against the definition, started far enough before them that what is in front is forgotten."""
     import trigrad_amd
@@ -499,6 +558,9 @@ def test_refusals(cuda, route):
             (lambda: step(x[:, 0], g[:, 0], h0.half()), TypeError, "state must be of type torch.float32"),
             (lambda: step(x[:, 0], g[:, 0], torch.zeros((8, 2), device=cuda).t()), ValueError, "state must be contiguous"),
             (lambda: step(x[:, 0], g[:, 0], h0, out=h0[:1]), ValueError, "out must be of shape"),
+            (lambda: step(x[:, 0], g[:, 0], h0, out=x.view(-1)[:16].view(2, 8)), ValueError, "inputs must not overlap"),
+            (lambda: step(x[:, 0], g[:, 0], h0, out=g.view(-1)[:16].view(2, 8)), ValueError, "gates must not overlap"),
+            (lambda: step(x[:1, 0], g[:1, 0], h0.view(-1)[:8].view(1, 8), out=h0.view(-1)[4:12].view(1, 8)), ValueError, "out must be state itself"),
             (lambda: step(x[:, 0].requires_grad_(), g[:, 0], h0), RuntimeError, "linear_recurrence_step has no gradient")):
         with pytest.raises(error, match=match):
             bad()

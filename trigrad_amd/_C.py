@@ -1275,6 +1275,21 @@ def operators_by_torch_module(tensor):
     return _lib._torch_module or _module()
 
 
+def refuse_stale_leaves(*tensors):
+    """While the current stream is captured, raises RuntimeError for a leaf of a graph that was made on another stream and still lives."""
+    if torch.cuda.is_current_stream_capturing():
+        _module().refuse_stale_leaves(*tensors)
+
+
+def overlap(a, b):
+    """Whether the bytes between a tensor's first and last element meet another's."""
+    def extent(t):
+        last = sum((size - 1) * stride for size, stride in zip(t.shape, t.stride()))
+        return t.data_ptr(), t.data_ptr() + ((last + 1) * t.element_size() if t.numel() else 0)
+    (a0, a1), (b0, b1) = extent(a), extent(b)
+    return a0 < b1 and b0 < a1
+
+
 def _address(t):
     return 0 if t is None else t.data_ptr()
 

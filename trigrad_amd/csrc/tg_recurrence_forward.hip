@@ -308,7 +308,7 @@ __global__ __launch_bounds__(256) void recurrence_prepare_kernel(Split m, int32_
     if (to) {
         for (int64_t i = id; i < m.sequences * m.channels; i += all) {
             const int64_t s = i / m.channels;
-            if (!m.packed || offsets[s + 1] <= offsets[s]) to[i] = from ? from[i] : 0.0f;
+            if (!m.packed || min((int64_t)offsets[s + 1], m.rows) <= max((int64_t)offsets[s], (int64_t)0)) to[i] = from ? from[i] : 0.0f;
         }
     }
 }

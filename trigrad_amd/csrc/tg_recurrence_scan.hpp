@@ -118,7 +118,7 @@ __device__ __forceinline__ void chunk_table(const Split &m, const int32_t *first
                 const int32_t mid = lo + (hi - lo + 1) / 2;
                 if (offsets[mid] <= row) lo = mid; else hi = mid - 1;
             }
-            const int64_t begin = offsets[lo], end = offsets[lo + 1];
+            const int64_t begin = max(offsets[lo], 0), end = min((int64_t)offsets[lo + 1], m.rows);
             uint32_t flags = 0;
             if (place < m.rows) {
                 if (row < begin || row >= end) flags = kFirst | kLast | kOutside;
@@ -138,7 +138,7 @@ __device__ __forceinline__ bool inside_one_sequence(const Split &m, const int32_
     }
     const int32_t s = first_sequence[2 * chunk];
     const int64_t low = m.reverse ? m.rows - end : start, high = m.reverse ? m.rows - start : end;
-    return s == first_sequence[2 * chunk + 1] && offsets[s] < low && high < offsets[s + 1];
+    return s == first_sequence[2 * chunk + 1] && max(offsets[s], 0) < low && high < min((int64_t)offsets[s + 1], m.rows);
 }
 
 __device__ __forceinline__ int64_t uniform(int64_t v) {  // of a wave whose lanes all have the same, or whose first lane's it is

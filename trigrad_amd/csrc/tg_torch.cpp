@@ -450,6 +450,7 @@ PyMethodDef methods[] = {{"render", reinterpret_cast<PyCFunction>(reinterpret_ca
                          {"linear_recurrence_step", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_linear_recurrence_step)), METH_FASTCALL,
                           nullptr},
                          {"group_norm", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_group_norm)), METH_FASTCALL, nullptr},
+                         {"refuse_stale_leaves", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_refuse_stale_leaves)), METH_FASTCALL, nullptr},
                          {"bind_operators", py_bind_operators, METH_VARARGS, nullptr},
                          {"bind", py_bind, METH_VARARGS, nullptr},
                          {"remember", py_remember, METH_VARARGS, nullptr},

@@ -48,11 +48,41 @@ bool goes_with(const at::Tensor &t, const at::Tensor &with, bool wide) {
 bool state_of(const at::Tensor &t, const at::Tensor &with, int64_t sequences, int64_t channels) {
     return t.device() == with.device() && t.scalar_type() == at::kFloat && t.dim() == 2 && t.size(0) == sequences && t.size(1) == channels;
 }
+// Whether the bytes between a tensor's first and last element meet another's.
+bool overlap(const at::Tensor &a, const at::Tensor &b) {
+    const auto extent = [](const at::Tensor &t) {
+        int64_t last = 0;
+        for (int64_t d = 0; d < t.dim(); d++) last += (t.size(d) - 1) * t.stride(d);
+        const char *first = static_cast<const char *>(t.data_ptr());
+        return std::make_pair(first, first + (t.numel() ? (last + 1) * (int64_t)t.element_size() : 0));
+    };
+    const auto x = extent(a), y = extent(b);
+    return x.first < y.second && y.first < x.second;
+}
 bool plain_call() { return !c10::impl::tls_is_dispatch_key_included(c10::DispatchKey::Tracer); }
 const void *address(const at::Tensor &t) { return t.defined() ? t.data_ptr() : nullptr; }
 void *target(const at::Tensor &t) { return t.defined() ? t.data_ptr() : nullptr; }
 void *stream_of(const at::Tensor &t) { return c10::hip::getCurrentHIPStream(t.device().index()).stream(); }
 at::Tensor room(const at::Tensor &like, int64_t bytes) { return bytes ? at::empty({bytes}, on(like, at::kByte)) : at::Tensor(); }
+
+// While `stream` is captured: a leaf whose gradient accumulates on another stream, because an eager graph of it made there still lives.  The
+// engine would join that stream into the capture, which invalidates it or ends the process.
+void refuse_stale_leaves(void *stream, std::initializer_list<const at::Tensor *> inputs) {
+    hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+    if (hipStreamIsCapturing(static_cast<hipStream_t>(stream), &status) != hipSuccess) {
+        (void)hipGetLastError();
+        return;
+    }
+    if (status != hipStreamCaptureStatusActive) return;
+    for (const at::Tensor *t : inputs) {
+        if (!t->defined() || !t->requires_grad() || !t->is_leaf()) continue;
+        const auto accumulator = torch::autograd::impl::try_get_grad_accumulator(*t);
+        const auto made_on = accumulator ? accumulator->stream() : std::nullopt;
+        if (made_on && c10::hip::HIPStream(c10::hip::HIPStream::UNCHECKED, *made_on).stream() != stream)
+            throw std::runtime_error("a call under capture has a leaf of a graph that was made on another stream and still lives: release that graph "
+                                     "(its outputs, and what was computed from them) before the capture");
+    }
+}
 
 // Gradients of gradients are refused where they are asked for, as torch's once_differentiable does.
 variable_list once(const variable_list &grads, variable_list out) {
@@ -193,6 +223,7 @@ PyObject *py_linear_recurrence(PyObject *, PyObject *const *args, Py_ssize_t n) 
             check(operators.recurrence_forward(&r), "tg_linear_recurrence_forward");
         }
         if (for_backward) {
+            refuse_stale_leaves(r.stream, {&inputs, &gates, &initial});
             out = LinearRecurrence::apply(inputs, gates, initial.defined() ? std::optional<at::Tensor>(initial) : std::nullopt, s);
         } else {
             if (return_states) out.push_back(s->states);
@@ -227,6 +258,8 @@ PyObject *py_linear_recurrence_step(PyObject *, PyObject *const *args, Py_ssize_
     for (const at::Tensor *t : {&state, &out})
         if (!state_of(*t, inputs, inputs.size(0), inputs.size(1)) || !t->is_contiguous()) Py_RETURN_NONE;
     if (at::GradMode::is_enabled() && (inputs.requires_grad() || gates.requires_grad() || state.requires_grad() || out.requires_grad())) Py_RETURN_NONE;
+    // what is written may be the state itself and nothing else that is read
+    if (overlap(out, inputs) || overlap(out, gates) || (out.data_ptr() != state.data_ptr() && overlap(out, state))) Py_RETURN_NONE;
     {
         const Unlocked unlocked;
         const c10::DeviceGuard guard(inputs.device());
@@ -348,13 +381,27 @@ PyObject *py_group_norm(PyObject *, PyObject *const *args, Py_ssize_t n) {
             c.stream = stream_of(in);
             check(operators.norm_forward(&c), "tg_group_norm_forward");
         }
-        if (for_backward)
+        if (for_backward) {
+            refuse_stale_leaves(c.stream, {&x, &weight, &bias});
             y = GroupNorm::apply(x, weight.defined() ? std::optional<at::Tensor>(weight) : std::nullopt,
                                  bias.defined() ? std::optional<at::Tensor>(bias) : std::nullopt, s)[0];
-        else
+        } else {
             y = s->y;
+        }
     }
     return THPVariable_Wrap(std::move(y));
+    END_HANDLE_TH_ERRORS
+}
+
+// refuse_stale_leaves(tensors or None ...): for calls that the Python functions make themselves
+PyObject *py_refuse_stale_leaves(PyObject *, PyObject *const *args, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    for (Py_ssize_t k = 0; k < n; k++) {
+        if (!THPVariable_Check(args[k])) continue;
+        const at::Tensor &t = THPVariable_Unpack(args[k]);
+        if (t.is_cuda()) refuse_stale_leaves(stream_of(t), {&t});
+    }
+    Py_RETURN_NONE;
     END_HANDLE_TH_ERRORS
 }
 

@@ -1,4 +1,5 @@
 """Group norm with an activation for tensors whose channels lie last, as an image that `render` returns has them."""
+import operator
 from typing import Optional
 
 import torch
@@ -24,6 +25,7 @@ class GroupNorm(Function):
         if x.dim() < 2:
             raise ValueError(f"x must have at least 2 dimensions, but got {x.dim()}")
         channels = x.shape[-1]
+        num_groups = operator.index(num_groups)
         if num_groups < 1 or channels < 1 or channels % num_groups != 0:
             raise ValueError(f"the number of channels must be a multiple of the number of groups, but got {channels} and {num_groups}")
         if not eps >= 0.0:
@@ -36,6 +38,8 @@ class GroupNorm(Function):
                     raise TypeError(f"{name} must be on {x.device}, but got {t.device}")
         if weight is not None and bias is not None and weight.dtype != bias.dtype:
             raise TypeError(f"bias must be of type {weight.dtype}, but got {bias.dtype}")
+        if any(ctx.needs_input_grad):
+            _C.refuse_stale_leaves(x, weight, bias)
         x, weight, bias = (None if t is None else t.contiguous() for t in (x, weight, bias))
         y, statistics = _C.group_norm_forward(x, num_groups, weight, bias, eps, ACTIVATIONS[activation])
         ctx.form = (num_groups, eps, ACTIVATIONS[activation])
@@ -71,7 +75,8 @@ def group_norm(
         weight, bias : (C,) of x's type or float32
         activation : "none", "relu", "silu" or "gelu" (by the error function)
 
-    Sums and statistics are float32 whatever the types.  Returns y as x.
+    Sums and statistics are float32 whatever the types.  The call can be captured into a graph, with its backward pass; under capture a
+    leaf of a graph that was made on another stream and still lives is refused.  Returns y as x.
     """
     module = _C.operators_by_torch_module(x)
     if module is not None:

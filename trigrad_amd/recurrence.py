@@ -66,6 +66,8 @@ class LinearRecurrence(Function):
         ctx.set_materialize_grads(False)  # an output the loss does not use arrives as None instead of a zero tensor
         ctx.form = (sequences, length, GATE_FORMS[gate_form], INPUT_FORMS[input_form], bool(reverse))
         ctx.has = (initial is not None, offsets is not None)
+        if any(ctx.needs_input_grad):
+            _C.refuse_stale_leaves(inputs, gates, initial)
         inputs, gates, initial, offsets = (None if t is None else t.contiguous() for t in (inputs, gates, initial, offsets))
         states, final, kept = _C.linear_recurrence_forward(inputs, gates, initial, offsets, *ctx.form, return_states,
                                                            any(ctx.needs_input_grad))
@@ -105,8 +107,9 @@ def linear_recurrence(
         reverse : every sequence from its last row to its first
         return_states : False: only the final state is of interest, no others are written
 
-    Gates are decays, |a| <= 1.  Larger ones are computed as long as no product of successive gates (of up to 4096 rows)
-    leaves the range of float32.  States are summed in float32 whatever the types.
+    Gates are decays, |a| <= 1.  Larger ones are computed as long as no product of successive gates of a sequence leaves the range of
+    float32, which is formed for all but the shortest.  States are summed in float32 whatever the types.  The call can be captured into
+    a graph, with its backward pass; under capture a leaf of a graph that was made on another stream and still lives is refused.
 
     Returns:
         states : as inputs, or None
@@ -153,6 +156,11 @@ def linear_recurrence_step(
             raise ValueError(f"{name} must be contiguous")
     if new_state.device != inputs.device:
         raise TypeError(f"out must be on {inputs.device}, but got {new_state.device}")
+    for name, t in (("inputs", inputs), ("gates", gates)):
+        if _C.overlap(new_state, t):
+            raise ValueError(f"{name} must not overlap the state that is written")
+    if new_state.data_ptr() != state.data_ptr() and _C.overlap(new_state, state):
+        raise ValueError("out must be state itself or not overlap it")
     if torch.is_grad_enabled() and any(t.requires_grad for t in (inputs, gates, state, new_state)):
         raise RuntimeError("linear_recurrence_step has no gradient: use linear_recurrence, or torch.no_grad()")
     states = _C.linear_recurrence_step(inputs.contiguous(), gates.contiguous(), state, new_state, GATE_FORMS[gate_form], INPUT_FORMS[input_form])
