@@ -18,7 +18,7 @@ namespace tg {
 
 struct NormShape {
     int64_t samples, positions, channels, groups, width;  // width: channels of a group
-    int activation, wide_weights;                          // wide_weights: weight and bias are tg_real whatever x is
+    int activation, wide_weights, aligned_weights;         // wide_weights: weight and bias are tg_real whatever x is
     real eps;
 };
 
@@ -76,10 +76,48 @@ template <class Call> __device__ __forceinline__ void by_activation(int kind, Ca
     else call(std::integral_constant<int, TG_ACTIVATION_GELU>());
 }
 
-template <class T, int V> __device__ __forceinline__ void load_weights(const NormShape &m, const void *from, int64_t at, real missing, real (&w)[V]) {
+// V successive weights: one access where they are aligned.
+template <class S, int V> __device__ __forceinline__ void load_weights_of(const NormShape &m, const S *from, real (&w)[V]) {
+    if (m.aligned_weights) {
+        const Pack<S, V> in = load_pack<V>(from);
 #pragma unroll
-    for (int v = 0; v < V; v++)
-        w[v] = !from ? missing : sizeof(T) == sizeof(real) || m.wide_weights ? ((const real *)from)[at + v] : (real)((const T *)from)[at + v];
+        for (int v = 0; v < V; v++) w[v] = in[v];
+    } else {
+#pragma unroll
+        for (int v = 0; v < V; v++) w[v] = (real)from[v];
+    }
+}
+template <class T, int V> __device__ __forceinline__ void load_weights(const NormShape &m, const void *from, int64_t at, real missing, real (&w)[V]) {
+    if (!from) {
+#pragma unroll
+        for (int v = 0; v < V; v++) w[v] = missing;
+    } else if (sizeof(T) == sizeof(real) || m.wide_weights) {
+        load_weights_of(m, (const real *)from + at, w);
+    } else {
+        load_weights_of(m, (const T *)from + at, w);
+    }
+}
+// The groups of V successive channels: one division, then steps.
+template <int V> __device__ __forceinline__ void groups_of(const NormShape &m, int64_t channel, int (&g)[V]) {
+    const uint32_t width = (uint32_t)m.width;
+    g[0] = (int)((uint32_t)channel / width);
+    uint32_t within = (uint32_t)channel - (uint32_t)g[0] * width;
+#pragma unroll
+    for (int v = 1; v < V; v++) {
+        within++;
+        const bool next = within == width;
+        g[v] = g[v - 1] + (next ? 1 : 0);
+        if (next) within = 0;
+    }
+}
+// mean and rstd (or two averages) of each channel's group
+template <int V> __device__ __forceinline__ void load_pairs(const NormShape &m, int64_t n, const int (&g)[V], const real *pairs, real (&a)[V], real (&b)[V]) {
+#pragma unroll
+    for (int v = 0; v < V; v++) {
+        const Pack<real, 2> pair = load_pack<2>(pairs + 2 * (n * m.groups + g[v]));
+        a[v] = pair[0];
+        b[v] = pair[1];
+    }
 }
 template <class T> __device__ __forceinline__ void store_weight(const NormShape &m, void *to, int64_t at, real w) {
     if (sizeof(T) == sizeof(real) || m.wide_weights) ((real *)to)[at] = w;
@@ -420,9 +458,11 @@ __global__ __launch_bounds__(kNormThreads) void norm_sums_kernel(NormShape m, St
     const StreamedPlace t = streamed_place<V>(m, p, split, tile);
     x += n * m.positions * m.channels;
     real pivot[V], first[V], second[V];
+    int g[V];
+    groups_of(m, t.active ? t.channel : 0, g);
 #pragma unroll
     for (int v = 0; v < V; v++) {
-        pivot[v] = t.active ? (real)x[(t.channel + v) / m.width * m.width] : (real)0;
+        pivot[v] = (real)x[(int64_t)g[v] * m.width];
         first[v] = second[v] = 0;
     }
     const int64_t pitch = (int64_t)p.rows * m.channels;
@@ -482,15 +522,14 @@ __global__ __launch_bounds__(kNormThreads) void norm_apply_kernel(NormShape m, S
     if (!t.active) return;
     x += n * m.positions * m.channels;
     y += n * m.positions * m.channels;
-    real w[V], b[V], mean[V];
+    real w[V], b[V], mean[V], rstd[V];
+    int g[V];
+    groups_of(m, t.channel, g);
     load_weights<T, V>(m, weight, t.channel, (real)1, w);
     load_weights<T, V>(m, bias, t.channel, (real)0, b);
+    load_pairs(m, n, g, statistics, mean, rstd);
 #pragma unroll
-    for (int v = 0; v < V; v++) {
-        const int64_t of = 2 * (n * m.groups + (t.channel + v) / m.width);
-        mean[v] = statistics[of];
-        w[v] *= statistics[of + 1];
-    }
+    for (int v = 0; v < V; v++) w[v] *= rstd[v];
     const int64_t pitch = (int64_t)p.rows * m.channels;
     by_activation(m.activation, [&](auto kind) {
         over_rows<T, V>(m, p, t, x, [&](const T *from, int there, int64_t r) {
@@ -525,15 +564,13 @@ __global__ __launch_bounds__(kNormThreads) void norm_gradient_sums_kernel(NormSh
     for (int v = 0; v < V; v++) sum[v] = product[v] = 0;
     if (t.active) {
         real w[V], b[V], mean[V], rstd[V];
+        int g[V];
+        groups_of(m, t.channel, g);
         load_weights<T, V>(m, weight, t.channel, (real)1, w);
         load_weights<T, V>(m, bias, t.channel, (real)0, b);
+        load_pairs(m, n, g, statistics, mean, rstd);
 #pragma unroll
-        for (int v = 0; v < V; v++) {
-            const int64_t of = 2 * (n * m.groups + (t.channel + v) / m.width);
-            mean[v] = statistics[of];
-            rstd[v] = statistics[of + 1];
-            w[v] *= rstd[v];
-        }
+        for (int v = 0; v < V; v++) w[v] *= rstd[v];
         const int64_t pitch = (int64_t)p.rows * m.channels;
         by_activation(m.activation, [&](auto kind) {
             for (int64_t r = t.begin + t.row; r < t.end; r += (int64_t)kNormPairs * p.rows) {
@@ -592,6 +629,7 @@ __device__ __forceinline__ void join_channel(const NormShape &m, int64_t parts, 
     const int64_t channel = block * kJoinColumns + column;
     double sum[2] = {0, 0};
     if (channel < m.channels)
+#pragma unroll 8
         for (int64_t i = line; i < parts; i += kJoinLines) {
             sum[0] += partial[i * stride + channel];
             sum[1] += partial[i * stride + which_stride + channel];
@@ -648,17 +686,18 @@ __global__ __launch_bounds__(kNormThreads) void norm_gradient_kernel(NormShape m
     const int64_t n = turned / (unsigned)p.splits / (unsigned)p.tiles;
     const StreamedPlace t = streamed_place<V>(m, p, (int)(turned % (unsigned)p.splits), (int)(turned / (unsigned)p.splits % (unsigned)p.tiles));
     if (!t.active) return;
-    real w[V], b[V], mean[V], sum[V], product[V];  // from here on times rstd, rstd and its square
+    real w[V], b[V], mean[V], rstd[V], sum[V], product[V];
+    int g[V];
+    groups_of(m, t.channel, g);
     load_weights<T, V>(m, weight, t.channel, (real)1, w);
     load_weights<T, V>(m, bias, t.channel, (real)0, b);
+    load_pairs(m, n, g, statistics, mean, rstd);
+    load_pairs(m, n, g, averages, sum, product);
 #pragma unroll
     for (int v = 0; v < V; v++) {
-        const int64_t of = 2 * (n * m.groups + (t.channel + v) / m.width);
-        const real rstd = statistics[of + 1];
-        mean[v] = statistics[of];
-        w[v] *= rstd;
-        sum[v] = averages[of] * rstd;
-        product[v] = averages[of + 1] * rstd * rstd;
+        w[v] *= rstd[v];
+        sum[v] *= rstd[v];
+        product[v] *= rstd[v] * rstd[v];
     }
     const int64_t pitch = (int64_t)p.rows * m.channels;
     by_activation(m.activation, [&](auto kind) {
@@ -714,6 +753,8 @@ static int check_norm(const char *fn, const tg_norm *n, NormShape &m) {
     m.width = n->channels / n->groups;
     m.activation = (int)n->activation;
     m.wide_weights = n->weight_type == kRealType;
+    const uintptr_t at = (uintptr_t)n->weight | (uintptr_t)n->bias;  // the widest access: eight elements of 32 bits
+    m.aligned_weights = at % std::min<uintptr_t>(32, (uintptr_t)(16 / type_bytes(n->type) * type_bytes(n->weight_type))) == 0;
     m.eps = (real)n->eps;
     return 0;
 }
