@@ -2,19 +2,25 @@
 // pieces are joined again (float library).
 //
 // A step is the map h -> a h + u; maps compose, (a2, u2) after (a1, u1) = (a2 a1, a2 u1 + u2), and a map whose sequence began within it
-// does not look at what came before ("closed").  All sequences laid end to end are one axis of rows; every thread holds kRows successive
-// rows of V channels in registers, so the inputs are read once.  Its map is composed
+// does not look at what came before ("closed").  All sequences laid end to end are one axis of rows; every thread holds a few
+// successive rows of V channels in registers.  Its map is composed
 //   1. over the threads of a wave that hold other rows of the same channels (there are some where there are few channels),
 //   2. over the workgroup's waves, through LDS,
 //   3. over the chunks of rows that workgroups have, in three launches: the chunks' maps, from a first look at the inputs; the states that
 //      the chunks start from, by going over the maps; and the chunks themselves, each from its state.  Calls whose sequences fit a chunk
 //      are the third launch alone.
-// The order of operations is fixed: results do not depend on timing.
+// The order of operations is fixed: results do not depend on timing, and no workgroup waits for another.
 //
-// The first look costs reading inputs twice (backward: gates and dh, not x).  A single launch in which chunks waited for the maps of those
-// before them read them once, and was slower: a chunk held its registers for three round trips through memory more, and the ticket
-// that orders such workgroups, the words to wait on and their clearing came on top (4 x 4096 x 2048, 16 gates: backward 148 us, with
-// every wait left out 66).
+// Bound by memory traffic, and by vector instructions beside it (about 20 an element with a logistic function, 10 without).  The first look
+// costs reading inputs twice (backward: gates and dh, not x), the second time mostly from the last-level cache: what is read for
+// the first time comes at 3.9 TB/s on this chip, a copy goes at 4.9 TB/s in and out together.  For 32768 x 2048 in bfloat16 with a gate for every channel
+// the first look takes 69 us (268 MB), the starting states 6, the chunks 91 (402 MB, 4.4 TB/s).  A single launch in which chunks waited for the
+// maps of those before them read everything once and was no faster forward (165 us and the clearing of its words) and slower backward
+// (4 x 4096 x 2048, 16 gates: 148 us against 57 + 6 + 21): a chunk held its registers for three round trips through memory more.
+//
+// Chunks are small, four or eight waves a SIMD's worth of workgroups beside each other, because a workgroup reads, computes and writes one after
+// another: with 1024 threads, one workgroup a CU, the same backward pass took 80 us.  Chunks of half the rows again would double what the maps and
+// starting states cost (24 bytes a chunk and channel).
 #pragma once
 #include <cfloat>
 #include <algorithm>
@@ -27,7 +33,7 @@ namespace tg {
 // Rows of a thread (at most 32, a bit each) and threads; their product is a chunk's rows x lanes of a row, where there are several chunks to
 // a sequence.  A forward chunk is a whole number of backward ones: the states in front of those are what the forward call keeps.
 constexpr int kForwardThreads = 256, kForwardRows = 16, kForwardChunk = kForwardThreads * kForwardRows;
-constexpr int kShortRows = 8;  // sequences of no more have kernels of their own
+constexpr int kShortRows = 8, kShortThreads = 256;  // sequences of no more rows have kernels of their own
 constexpr int kBackwardThreads = 256, kBackwardRows = 8, kBackwardChunk = kBackwardThreads * kBackwardRows;
 constexpr int kMapThreads = 256;
 // Sequences of one chunk to about four have a large workgroup each instead: no first look, no starting states, one launch.
@@ -84,8 +90,6 @@ template <int V> __device__ __forceinline__ void compose(Map<V> &later, const Ma
     }
     later.closed = later.closed || earlier.closed;
 }
-
-__device__ __forceinline__ uint32_t word_of(float f) { return f != f ? 0x7fc00000u : __float_as_uint(f); }
 
 template <int V> __device__ __forceinline__ void step_over(float (&h)[V], const Map<V> &map) {
 #pragma unroll
@@ -297,41 +301,23 @@ template <int K, int GV> __device__ __forceinline__ void compute_gates(const Spl
     }
 }
 
-// Sums of K rows' values over the wave.  Each step hands half of the rows to half of the lanes, so K + K / 2 + ... additions do what six a
-// row would; a lane ends with the sum of row_of_sum, and the lanes that sum_is_here names have each of them once.
-template <int K> __device__ __forceinline__ float sum_rows(float (&q)[K]) {
-    static_assert(K == 8 || K == 16, "");
-    const int lane = threadIdx.x & (kWave - 1);
+// Sums of eight rows' values over the wave.  Each step hands half of the rows to half of the lanes, so 4 + 2 + 1 + 3 additions do what six
+// for each row would; lane i ends with the sum of row i / 8.
+__device__ __forceinline__ float sum_rows(float (&q)[8]) {
 #pragma unroll
-    for (int i = 0; i < K / 2; i++) {
-        const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(q[i]), __float_as_uint(q[i + K / 2]), false, false);
+    for (int i = 0; i < 4; i++) {
+        const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(q[i]), __float_as_uint(q[i + 4]), false, false);
         q[i] = __uint_as_float(r[0]) + __uint_as_float(r[1]);
     }
 #pragma unroll
-    for (int i = 0; i < K / 4; i++) {
-        const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(q[i]), __float_as_uint(q[i + K / 4]), false, false);
+    for (int i = 0; i < 2; i++) {
+        const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(q[i]), __float_as_uint(q[i + 2]), false, false);
         q[i] = __uint_as_float(r[0]) + __uint_as_float(r[1]);
     }
-#pragma unroll
-    for (int i = 0; i < K / 8; i++) {
-        const float keep = lane & 8 ? q[i + K / 8] : q[i], give = lane & 8 ? q[i] : q[i + K / 8];
-        q[i] = keep + from_lane<kRotate8>(give);
-    }
-    if (K == 16) {
-        const float keep = lane & 4 ? q[1] : q[0], give = lane & 4 ? q[0] : q[1];
-        q[0] = keep + from_lane<kMirrorOf8>(give);
-    } else {
-        q[0] += from_lane<kMirrorOf8>(q[0]);
-    }
-    q[0] += from_lane<kSwapOnes>(q[0]);
-    q[0] += from_lane<kSwapTwos>(q[0]);
-    return q[0];
+    const bool upper = (threadIdx.x & 8) != 0;
+    const float keep = upper ? q[1] : q[0], give = upper ? q[0] : q[1];
+    return sum_lanes(keep + from_lane<kRotate8>(give), 8);
 }
-template <int K> __device__ __forceinline__ int row_of_sum(int lane) {
-    const int eighth = (lane >> 5) * 4 + (lane >> 4 & 1) * 2 + (lane >> 3 & 1);
-    return K == 16 ? eighth * 2 + (lane >> 2 & 1) : eighth;
-}
-template <int K> __device__ __forceinline__ bool sum_is_here(int lane) { return (lane & (K == 16 ? 3 : 7)) == 0; }
 
 // The maps of the workgroup's threads, or waves, [entry][lane][V].
 template <int V, int Threads> struct Joint {
