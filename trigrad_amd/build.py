@@ -12,6 +12,8 @@ The flags are part of the arithmetic contract of the kernels:
 import os
 import subprocess
 import sys
+import tempfile
+from concurrent.futures import ThreadPoolExecutor
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
@@ -25,7 +27,7 @@ SOURCES = ["tg_api.hip", "tg_binning.hip", "tg_scan.hip", "tg_sort.hip", "tg_for
            "tg_recurrence.hip", "tg_recurrence_forward.hip", "tg_recurrence_backward.hip", "tg_recurrence_short.hip", "tg_norm.hip"]
 
 FLAGS = [
-    "--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-shared",
+    "--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC",
     "-ffp-contract=off", "-fno-fast-math",
     "-munsafe-fp-atomics",  # float atomic adds use the hardware instruction (coarse-grained memory)
     "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
@@ -33,11 +35,13 @@ FLAGS = [
 ]
 
 
-def _compile(out, flags, verbose):
-    hipcc = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
-    cmd = [hipcc, *FLAGS, *flags, *[os.path.join(CSRC, s) for s in SOURCES], "-o", out]
+COMPILERS_AT_ONCE = 8  # processes; one takes up to a GiB of host memory
+
+
+def _hipcc(arguments, verbose):
+    cmd = [os.environ.get("HIPCC", "/opt/rocm/bin/hipcc"), *FLAGS, *arguments]
     if verbose:
-        print(" ".join(cmd))
+        print(" ".join(cmd), flush=True)
     res = subprocess.run(cmd, capture_output=True, text=True)
     noise = "is not a recognized feature for this target"
     err = "\n".join(l for l in res.stderr.splitlines() if noise not in l)
@@ -45,7 +49,18 @@ def _compile(out, flags, verbose):
         raise RuntimeError(f"hipcc failed ({res.returncode}):\n{err}")
     if verbose and err.strip():
         print(err, file=sys.stderr)
-    return out
+
+
+def _compile(libraries, verbose):
+    """Builds the (path, flags) of `libraries`: every source of each to an object of its own, some at once, then links them."""
+    with tempfile.TemporaryDirectory() as objects, ThreadPoolExecutor(min(COMPILERS_AT_ONCE, os.cpu_count() or 1)) as pool:
+        parts = [[(os.path.join(CSRC, s), os.path.join(objects, f"{n}_{s}.o")) for s in SOURCES] for n in range(len(libraries))]
+        done = [pool.submit(_hipcc, [*flags, "-c", source, "-o", part], verbose)
+                for (_, flags), sources in zip(libraries, parts) for source, part in sources]
+        for d in done:
+            d.result()
+        for (out, flags), sources in zip(libraries, parts):
+            _hipcc([*flags, "-shared", *[part for _, part in sources], "-o", out], verbose)
 
 
 def _compile_torch_module(verbose):
@@ -70,9 +85,10 @@ def build(verbose=False, extra_flags=(), double_too=True):
     """Builds the float library, (double_too) the double one and the torch module; returns the float library's path."""
     os.makedirs(LIB_DIR, exist_ok=True)
     _compile_torch_module(verbose)
-    _compile(LIB_PATH, list(extra_flags), verbose)
+    libraries = [(LIB_PATH, list(extra_flags))]
     if double_too:
-        _compile(LIB_PATH_F64, [*extra_flags, "-DTG_DOUBLE_PRECISION"], verbose)
+        libraries.append((LIB_PATH_F64, [*extra_flags, "-DTG_DOUBLE_PRECISION"]))
+    _compile(libraries, verbose)
     return LIB_PATH
 
 
