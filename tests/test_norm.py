@@ -346,6 +346,23 @@ def test_more_elements_than_31_bits_count(cuda):
 
 
 @pytest.mark.gpu
+def test_more_workgroups_than_22_bits_count(cuda):
+    """Rows of an odd number of channels that no workgroup holds, in 18 workgroups each: the first and last rows against the definition."""
+    import trigrad_amd
+    samples, channels = 2 ** 18, 4353
+    x = torch.empty((samples, channels), dtype=torch.bfloat16, device=cuda)
+    for p in range(0, samples, 1 << 14):
+        x[p:p + (1 << 14)].normal_()
+    leaf = x.requires_grad_()
+    y = trigrad_amd.group_norm(leaf, 3)
+    (got,) = torch.autograd.grad(y, leaf, x.detach())
+    for part in (slice(0, 3), slice(samples // 2, samples // 2 + 2), slice(samples - 3, samples)):
+        want = reference(x[part], 3, None, None, 1e-5, "none", x.detach()[part])
+        assert_near("y", y[part], want["y"])
+        assert_near("grad_x", got[part], want["grad_x"])
+
+
+@pytest.mark.gpu
 def test_run_of_operators(cuda, oracle):
     """Slabs of a scene rendered apart, composited, a recurrence over their features, its states normalised by head and by frame: the image is
     that of the slabs one by one, and the gradient reaches the scene's colours."""

@@ -872,6 +872,12 @@ static NormPlan plan_of(const NormShape &m, int64_t type, bool backward, bool al
 }
 static int64_t norm_bytes(const NormPlan &p) { return (p.partial + p.by_group + p.averages) * (int64_t)sizeof(real); }
 
+// A grid has fewer than 2^32 threads (of the held kernels it has kHeldThreads, or a workgroup a slab).
+static bool beyond_a_grid(const NormShape &m, const NormPlan &p) {
+    const int64_t joins = m.samples * m.groups + ceil_div64(m.channels, kJoinColumns);
+    return !p.held && (p.blocks >= ((int64_t)1 << 32) / kNormThreads || joins >= ((int64_t)1 << 32) / kJoinThreads);
+}
+
 static int too_many(const char *fn) {
     set_error("%s: too many samples", fn);
     return TG_E_ARG;
@@ -911,7 +917,7 @@ extern "C" int tg_group_norm_forward(const tg_norm *n) {
         return TG_E_ARG;
     }
     const NormPlan p = plan_of(m, n->type, false, false, {n->x, n->y});
-    if (p.blocks >= (1 << 22) || (!p.held && m.samples * m.groups >= (1 << 21))) return too_many(fn);
+    if (beyond_a_grid(m, p)) return too_many(fn);
     if (norm_bytes(p) > 0 && (!n->workspace || n->workspace_bytes < norm_bytes(p))) {
         set_error("%s: workspace of %lld bytes, %lld needed", fn, (long long)n->workspace_bytes, (long long)norm_bytes(p));
         return TG_E_WORKSPACE;
@@ -969,7 +975,7 @@ extern "C" int tg_group_norm_backward(const tg_norm *n) {
         return TG_E_ARG;
     }
     const NormPlan p = plan_of(m, n->type, true, false, {n->x, n->grad_y, n->grad_x});
-    if (p.blocks >= (1 << 22) || (!p.held && m.samples * m.groups >= (1 << 21))) return too_many(fn);
+    if (beyond_a_grid(m, p)) return too_many(fn);
     if (!n->workspace || n->workspace_bytes < norm_bytes(p)) {
         set_error("%s: workspace of %lld bytes, %lld needed", fn, (long long)n->workspace_bytes, (long long)norm_bytes(p));
         return TG_E_WORKSPACE;
