@@ -363,6 +363,19 @@ def test_more_workgroups_than_22_bits_count(cuda):
 
 
 @pytest.mark.gpu
+def test_a_negation_still_to_be_done(cuda, route):
+    """Tensors whose values are the negatives of what is in memory, as a conjugate's imaginary part."""
+    import trigrad_amd
+    x, w, b, dy = make(cuda, 7, (2, 9, 8))
+    y = run_and_check(x, 2, w, b, dy, "silu")
+    leaves = [torch._neg_view(-t).requires_grad_() for t in (x, w, b)]
+    again = trigrad_amd.group_norm(leaves[0], 2, *leaves[1:], activation="silu")
+    assert torch.equal(y[0], again)
+    for want, got in zip(y[1:], torch.autograd.grad(again, leaves, torch._neg_view(-dy))):
+        assert torch.equal(want, got)
+
+
+@pytest.mark.gpu
 def test_run_of_operators(cuda, oracle):
     """Slabs of a scene rendered apart, composited, a recurrence over their features, its states normalised by head and by frame: the image is
     that of the slabs one by one, and the gradient reaches the scene's colours."""

@@ -265,6 +265,27 @@ def test_strides_and_alignment(cuda, route):
 
 
 @pytest.mark.gpu
+def test_a_negation_still_to_be_done(cuda, route):
+    """Tensors whose values are the negatives of what is in memory, as a conjugate's imaginary part."""
+    import trigrad_amd
+    x, g, h0, rng = make(cuda, 5, (2, 40), 6, 3)
+    ends = [torch.randn(s, generator=rng).to(cuda) for s in ((2, 40, 6), (2, 6))]
+    plain = [t.clone().requires_grad_() for t in (x, g, h0)]
+    negated = [torch._neg_view(-t).requires_grad_() for t in (x, g, h0)]
+    results = []
+    for leaves, given in ((plain, ends), (negated, [torch._neg_view(-t) for t in ends])):
+        out = trigrad_amd.linear_recurrence(*leaves)
+        results.append([*out, *torch.autograd.grad(out, leaves, given)])
+    assert all(torch.equal(want, got) for want, got in zip(*results))
+    with torch.no_grad():
+        want = trigrad_amd.linear_recurrence_step(x[:, 0], g[:, 0], h0.clone())
+        got = trigrad_amd.linear_recurrence_step(negated[0][:, 0], negated[1][:, 0], h0.clone())
+        assert all(torch.equal(*pair) for pair in zip(want, got))
+        with pytest.raises(ValueError, match="no negation"):
+            trigrad_amd.linear_recurrence_step(x[:, 0], g[:, 0], torch._neg_view(h0))
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("reverse", [False, True])
 def test_nothing_leaks_across_sequences(reverse, cuda):
     """NaN and infinities in one sequence, and in rows that belong to none, leave the others' states and gradients as they are."""

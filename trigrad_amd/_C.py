@@ -1281,6 +1281,11 @@ def refuse_stale_leaves(*tensors):
         _module().refuse_stale_leaves(*tensors)
 
 
+def dense(t):
+    """`t` in memory as its elements are: contiguous, and without a negation that is still to be done (as of a conjugate's imaginary part)."""
+    return t.resolve_neg().contiguous()
+
+
 def overlap(a, b):
     """Whether the bytes between a tensor's first and last element meet another's."""
     def extent(t):
@@ -1329,7 +1334,7 @@ def linear_recurrence_backward(inputs, gates, initial, offsets, kept, grad_state
     dev = inputs.device
     with _on_device(dev):
         lib, r, sizes = _recurrence(inputs, gates, offsets, sequences, length, gate_form, input_form, reverse)
-        grad_states, grad_final = (None if t is None else t.contiguous() for t in (grad_states, grad_final))
+        grad_states, grad_final = (None if t is None else dense(t) for t in (grad_states, grad_final))
         grad_inputs = torch.empty_like(inputs) if need_inputs else None
         grad_gates = torch.empty_like(gates) if need_gates else None
         grad_initial = torch.empty((sequences, inputs.shape[-1]), dtype=real_type(inputs.dtype), device=dev) if need_initial else None
@@ -1378,7 +1383,7 @@ def group_norm_forward(x, groups, weight, bias, eps, activation):
 def group_norm_backward(grad_y, x, groups, weight, bias, statistics, eps, activation, need_x, need_weight, need_bias):
     """-> gradients of x, weight and bias, None where not needed."""
     with _on_device(x.device):
-        grad_y = grad_y.contiguous()
+        grad_y = dense(grad_y)
         lib, n, sizes = _norm(x, groups, weight, bias, statistics, eps, activation)
         grad_x = torch.empty_like(x) if need_x else None
         grad_weight = torch.empty_like(weight) if need_weight else None

@@ -63,6 +63,7 @@ bool plain_call() { return !c10::impl::tls_is_dispatch_key_included(c10::Dispatc
 const void *address(const at::Tensor &t) { return t.defined() ? t.data_ptr() : nullptr; }
 void *target(const at::Tensor &t) { return t.defined() ? t.data_ptr() : nullptr; }
 void *stream_of(const at::Tensor &t) { return c10::hip::getCurrentHIPStream(t.device().index()).stream(); }
+at::Tensor dense(const at::Tensor &t) { return (t.is_neg() ? t.resolve_neg() : t).contiguous(); }
 at::Tensor room(const at::Tensor &like, int64_t bytes) { return bytes ? at::empty({bytes}, on(like, at::kByte)) : at::Tensor(); }
 
 // While `stream` is captured: a leaf whose gradient accumulates on another stream, because an eager graph of it made there still lives.  The
@@ -130,10 +131,10 @@ struct LinearRecurrence : torch::autograd::Function<LinearRecurrence> {
         tg_recurrence r = static_cast<const Sequences *>(capsule.get())->call;
         const bool has_initial = ctx->saved_data["initial"].toBool(), has_states = ctx->saved_data["states"].toBool();
         const c10::DeviceGuard guard(saved[0].device());
-        const at::Tensor inputs = saved[0].contiguous(), gates = saved[1].contiguous(),
-                         initial = has_initial ? saved[2].contiguous() : at::Tensor();
-        const at::Tensor grad_states = has_states && grads[0].defined() ? grads[0].contiguous() : at::Tensor(),
-                         grad_final = grads.back().defined() ? grads.back().contiguous() : at::Tensor();
+        const at::Tensor inputs = dense(saved[0]), gates = dense(saved[1]),
+                         initial = has_initial ? dense(saved[2]) : at::Tensor();
+        const at::Tensor grad_states = has_states && grads[0].defined() ? dense(grads[0]) : at::Tensor(),
+                         grad_final = grads.back().defined() ? dense(grads.back()) : at::Tensor();
         at::Tensor grad_inputs, grad_gates, grad_initial;
         {
             const at::NoGradGuard no_grad;
@@ -200,8 +201,8 @@ PyObject *py_linear_recurrence(PyObject *, PyObject *const *args, Py_ssize_t n) 
         const c10::DeviceGuard guard(inputs.device());
         {
             const at::NoGradGuard no_grad;
-            const at::Tensor x = inputs.contiguous(), g = gates.contiguous(), h = initial.defined() ? initial.contiguous() : initial;
-            if (s->offsets.defined()) s->offsets = s->offsets.contiguous();
+            const at::Tensor x = dense(inputs), g = dense(gates), h = initial.defined() ? dense(initial) : initial;
+            if (s->offsets.defined()) s->offsets = dense(s->offsets);
             r.inputs = address(x);
             r.gates = address(g);
             r.initial = static_cast<const float *>(address(h));
@@ -256,7 +257,7 @@ PyObject *py_linear_recurrence_step(PyObject *, PyObject *const *args, Py_ssize_
         gates.size(1) < 1 || inputs.size(1) % gates.size(1) != 0)
         Py_RETURN_NONE;
     for (const at::Tensor *t : {&state, &out})
-        if (!state_of(*t, inputs, inputs.size(0), inputs.size(1)) || !t->is_contiguous()) Py_RETURN_NONE;
+        if (!state_of(*t, inputs, inputs.size(0), inputs.size(1)) || !t->is_contiguous() || t->is_neg()) Py_RETURN_NONE;
     if (at::GradMode::is_enabled() && (inputs.requires_grad() || gates.requires_grad() || state.requires_grad() || out.requires_grad())) Py_RETURN_NONE;
     // what is written may be the state itself and nothing else that is read
     if (overlap(out, inputs) || overlap(out, gates) || (out.data_ptr() != state.data_ptr() && overlap(out, state))) Py_RETURN_NONE;
@@ -264,7 +265,7 @@ PyObject *py_linear_recurrence_step(PyObject *, PyObject *const *args, Py_ssize_
         const Unlocked unlocked;
         const c10::DeviceGuard guard(inputs.device());
         const at::NoGradGuard no_grad;
-        const at::Tensor x = inputs.contiguous(), g = gates.contiguous();
+        const at::Tensor x = dense(inputs), g = dense(gates);
         states = at::empty(x.sizes(), x.options());
         check(operators.recurrence_step(address(x), address(g), static_cast<const float *>(address(state)), target(states), static_cast<float *>(target(out)),
                                         x.size(0), x.size(1), g.size(1), type_code(x.scalar_type()), type_code(g.scalar_type()), (int)gate_form,
@@ -308,8 +309,8 @@ struct GroupNorm : torch::autograd::Function<GroupNorm> {
         tg_norm c = static_cast<const Normed *>(capsule.get())->call;
         const bool has_weight = ctx->saved_data["weight"].toBool(), has_bias = ctx->saved_data["bias"].toBool();
         const c10::DeviceGuard guard(saved[0].device());
-        const at::Tensor x = saved[0].contiguous(), weight = has_weight ? saved[1].contiguous() : at::Tensor(),
-                         bias = has_bias ? saved[2].contiguous() : at::Tensor(), grad_y = grads[0].contiguous();
+        const at::Tensor x = dense(saved[0]), weight = has_weight ? dense(saved[1]) : at::Tensor(),
+                         bias = has_bias ? dense(saved[2]) : at::Tensor(), grad_y = dense(grads[0]);
         at::Tensor grad_x, grad_weight, grad_bias;
         {
             const at::NoGradGuard no_grad;
@@ -364,7 +365,7 @@ PyObject *py_group_norm(PyObject *, PyObject *const *args, Py_ssize_t n) {
         const c10::DeviceGuard guard(x.device());
         {
             const at::NoGradGuard no_grad;
-            const at::Tensor in = x.contiguous(), w = weight.defined() ? weight.contiguous() : weight, b = bias.defined() ? bias.contiguous() : bias;
+            const at::Tensor in = dense(x), w = weight.defined() ? dense(weight) : weight, b = bias.defined() ? dense(bias) : bias;
             int64_t sizes[2];
             check(operators.norm_sizes(&c, sizes), "tg_group_norm_sizes");
             s->y = at::empty(in.sizes(), in.options());

@@ -40,7 +40,7 @@ class GroupNorm(Function):
             raise TypeError(f"bias must be of type {weight.dtype}, but got {bias.dtype}")
         if any(ctx.needs_input_grad):
             _C.refuse_stale_leaves(x, weight, bias)
-        x, weight, bias = (None if t is None else t.contiguous() for t in (x, weight, bias))
+        x, weight, bias = (None if t is None else _C.dense(t) for t in (x, weight, bias))
         y, statistics = _C.group_norm_forward(x, num_groups, weight, bias, eps, ACTIVATIONS[activation])
         ctx.form = (num_groups, eps, ACTIVATIONS[activation])
         ctx.has = (weight is not None, bias is not None)

@@ -68,7 +68,7 @@ class LinearRecurrence(Function):
         ctx.has = (initial is not None, offsets is not None)
         if any(ctx.needs_input_grad):
             _C.refuse_stale_leaves(inputs, gates, initial)
-        inputs, gates, initial, offsets = (None if t is None else t.contiguous() for t in (inputs, gates, initial, offsets))
+        inputs, gates, initial, offsets = (None if t is None else _C.dense(t) for t in (inputs, gates, initial, offsets))
         states, final, kept = _C.linear_recurrence_forward(inputs, gates, initial, offsets, *ctx.form, return_states,
                                                            any(ctx.needs_input_grad))
         if kept is not None:
@@ -152,8 +152,8 @@ def linear_recurrence_step(
     new_state = state if out is None else out
     check_tensor(new_state, "out", tuple(state.shape), state.dtype)
     for name, t in (("state", state), ("out", new_state)):
-        if not t.is_contiguous():
-            raise ValueError(f"{name} must be contiguous")
+        if not t.is_contiguous() or t.is_neg():
+            raise ValueError(f"{name} must be contiguous, with no negation still to be done")
     if new_state.device != inputs.device:
         raise TypeError(f"out must be on {inputs.device}, but got {new_state.device}")
     for name, t in (("inputs", inputs), ("gates", gates)):
@@ -163,7 +163,7 @@ def linear_recurrence_step(
         raise ValueError("out must be state itself or not overlap it")
     if torch.is_grad_enabled() and any(t.requires_grad for t in (inputs, gates, state, new_state)):
         raise RuntimeError("linear_recurrence_step has no gradient: use linear_recurrence, or torch.no_grad()")
-    states = _C.linear_recurrence_step(inputs.contiguous(), gates.contiguous(), state, new_state, GATE_FORMS[gate_form], INPUT_FORMS[input_form])
+    states = _C.linear_recurrence_step(_C.dense(inputs), _C.dense(gates), state, new_state, GATE_FORMS[gate_form], INPUT_FORMS[input_form])
     if not new_state.is_inference():
         torch.autograd.graph.increment_version(new_state)
     return states, new_state
