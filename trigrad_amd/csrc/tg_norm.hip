@@ -3,7 +3,8 @@
 //     xh = (x - mean) rstd,  z = weight xh + bias,  y = act(z),  mean and rstd of a sample's positions x (channels / groups)
 //     dz = dy act'(z),  dweight = sum dz xh,  dbias = sum dz,  dxh = weight dz,  dx = rstd (dxh - avg dxh - xh avg(dxh xh))
 //
-// Bound by memory traffic: x in and y out, x and dy in and dx out.  Two ways:
+// Bound by memory traffic: x in and y out, x and dy in and dx out.  Three ways:
+//   token     a sample is one position and its groups are wider than a wave: a workgroup has a group in registers.
 //   held      a sample's groups fit the registers of a workgroup: read once, summed, written.  A workgroup has `teams` samples at a
 //             time and goes over many, so that the weights' gradients are summed in registers and come to few partial sums.
 //   streamed  a sample's rows are split over workgroups: one launch sums them, a small one joins the sums, one reads the rows again
@@ -87,15 +88,19 @@ template <class S, int V> __device__ __forceinline__ void load_weights_of(const 
         for (int v = 0; v < V; v++) w[v] = (real)from[v];
     }
 }
-template <class T, int V> __device__ __forceinline__ void load_weights(const NormShape &m, const void *from, int64_t at, real missing, real (&w)[V]) {
+template <class T, int V>
+__device__ __forceinline__ void load_weights(const NormShape &m, const void *from, int64_t base, uint32_t at, real missing, real (&w)[V]) {
     if (!from) {
 #pragma unroll
         for (int v = 0; v < V; v++) w[v] = missing;
     } else if (sizeof(T) == sizeof(real) || m.wide_weights) {
-        load_weights_of(m, (const real *)from + at, w);
+        load_weights_of(m, (const real *)from + base + at, w);
     } else {
-        load_weights_of(m, (const T *)from + at, w);
+        load_weights_of(m, (const T *)from + base + at, w);
     }
+}
+template <class T, int V> __device__ __forceinline__ void load_weights(const NormShape &m, const void *from, int64_t at, real missing, real (&w)[V]) {
+    load_weights<T, V>(m, from, at, 0, missing, w);
 }
 // The groups of V successive channels: one division, then steps.
 template <int V> __device__ __forceinline__ void groups_of(const NormShape &m, int64_t channel, int (&g)[V]) {
@@ -368,6 +373,175 @@ __global__ __launch_bounds__(1024) void norm_held_backward_kernel(NormShape m, H
             for (int i = 0; i < lines; i++) sum += at[i * columns + c];
             partial[((int64_t)which * p.workgroups + first_turn) * m.channels + channel] = sum;
         }
+    }
+}
+
+// ---- tokens -------------------------------------------------------------------------------------
+
+// A sample of one position whose groups are wider than a wave: a workgroup has a group of it in registers and goes over many
+// samples.  8192 x 8192 in bfloat16: 53 us forward (5.1 TB/s) and 112 backward with its joining (3.6); the held kernels took 103 and 125.  A thread
+// has several accesses (forward 53 us, backward 120) or, backward where a workgroup can, one (112): its sums of the weights' gradients take registers.
+struct Token {
+    int threads, units;  // units: accesses of a group
+    bool single;         // one of them a thread
+    int workgroups;      // that go over the samples, for each group
+};
+// Accesses of a thread where it has several: sixteen elements, or four accesses (more of narrow ones spill registers).
+constexpr int token_accesses(int vector) { return std::min((sizeof(real) == 4 ? 16 : 8) / vector, 4); }
+
+// Sums of two values over the workgroup.  The two buffers take turns, so that one barrier is enough.
+struct TokenSums {
+    real at[2][1024 / kWave][2];
+};
+__device__ __forceinline__ void sum_token(TokenSums &s, int &buffer, real &a, real &b) {
+    a = sum_lanes(a, kWave);
+    b = sum_lanes(b, kWave);
+    const int waves = blockDim.x / kWave, wave = threadIdx.x / kWave;
+    if (waves == 1) return;
+    if ((threadIdx.x & (kWave - 1)) == 0) {
+        s.at[buffer][wave][0] = a;
+        s.at[buffer][wave][1] = b;
+    }
+    __syncthreads();
+    a = b = 0;
+    for (int i = 0; i < waves; i++) {
+        a += s.at[buffer][i][0];
+        b += s.at[buffer][i][1];
+    }
+    buffer ^= 1;
+}
+
+// Of a thread's access k from the group's first channel; that of its first channels where it has no such access.
+template <int V> __device__ __forceinline__ uint32_t token_offset(const Token &p, int k, int left) {
+    return k * p.threads < left ? (threadIdx.x + k * p.threads) * V : 0;
+}
+
+template <class T, int V, int K>
+__global__ __launch_bounds__(1024) void norm_token_forward_kernel(NormShape m, Token p, const T *__restrict__ x, const void *__restrict__ weight,
+                                                                  const void *__restrict__ bias, T *__restrict__ y, real *__restrict__ statistics) {
+    __shared__ TokenSums shared;
+    const int64_t group = blockIdx.x / (unsigned)p.workgroups, low = group * m.width;
+    const real per_value = (real)1 / (real)m.width;
+    const int left = p.units - (int)threadIdx.x;  // accesses k with k * threads < left are the thread's
+    int buffer = 0;
+    for (int64_t n = blockIdx.x % (unsigned)p.workgroups; n < m.samples; n += p.workgroups) {
+        const int64_t base = n * m.channels + low;
+        Pack<T, V> in[K];
+#pragma unroll
+        for (int k = 0; k < K; k++) in[k] = load_pack<V>(x + base + token_offset<V>(p, k, left));
+        real sum = 0, none = 0;
+#pragma unroll
+        for (int k = 0; k < K; k++)
+#pragma unroll
+            for (int v = 0; v < V; v++) sum += k * p.threads < left ? in[k][v] : (real)0;
+        sum_token(shared, buffer, sum, none);
+        const real about = sum * per_value;  // as in the held kernels
+        real first = 0, second = 0;
+#pragma unroll
+        for (int k = 0; k < K; k++)
+#pragma unroll
+            for (int v = 0; v < V; v++) {
+                const real d = k * p.threads < left ? in[k][v] - about : (real)0;
+                first += d;
+                second = fma(d, d, second);
+            }
+        sum_token(shared, buffer, first, second);
+        const real rest = first * per_value, mean = about + rest, variance = fma(-rest, rest, second * per_value);
+        const real rstd = inverse_root((variance < 0 ? (real)0 : variance) + m.eps);
+        if (threadIdx.x == 0) {
+            statistics[2 * (n * m.groups + group)] = mean;
+            statistics[2 * (n * m.groups + group) + 1] = rstd;
+        }
+        by_activation(m.activation, [&](auto kind) {
+#pragma unroll
+            for (int k = 0; k < K; k++) {
+                if (k * p.threads >= left) break;
+                const uint32_t at = token_offset<V>(p, k, left);
+                real w[V], b[V], out[V];
+                load_weights<T, V>(m, weight, low, at, (real)1, w);
+                load_weights<T, V>(m, bias, low, at, (real)0, b);
+#pragma unroll
+                for (int v = 0; v < V; v++) out[v] = activate<decltype(kind)::value, false>(fma(in[k][v] - mean, rstd * w[v], b[v]));
+                store_pack<V>(y + base + at, out);
+            }
+        });
+    }
+}
+
+template <class T, int V, int K>
+__global__ __launch_bounds__(1024) void norm_token_backward_kernel(NormShape m, Token p, const T *__restrict__ x, const void *__restrict__ weight,
+                                                                   const void *__restrict__ bias, const real *__restrict__ statistics,
+                                                                   const T *__restrict__ grad_y, T *__restrict__ grad_x, real *__restrict__ partial) {
+    __shared__ TokenSums shared;
+    const int64_t group = blockIdx.x / (unsigned)p.workgroups, first_sample = blockIdx.x % (unsigned)p.workgroups, low = group * m.width;
+    const real per_value = (real)1 / (real)m.width;
+    const int left = p.units - (int)threadIdx.x;
+    int buffer = 0;
+    real dw[K][V], db[K][V];
+#pragma unroll
+    for (int k = 0; k < K; k++)
+#pragma unroll
+        for (int v = 0; v < V; v++) dw[k][v] = db[k][v] = 0;
+    for (int64_t n = first_sample; n < m.samples; n += p.workgroups) {
+        const int64_t base = n * m.channels + low;
+        Pack<T, V> in[K], dy[K];
+#pragma unroll
+        for (int k = 0; k < K; k++) {
+            const uint32_t at = token_offset<V>(p, k, left);
+            in[k] = load_pack<V>(x + base + at);
+            dy[k] = load_pack<V>(grad_y + base + at);
+        }
+        const Pack<real, 2> of = load_pack<2>(statistics + 2 * (n * m.groups + group));
+        const real mean = of[0], rstd = of[1];
+        real sum = 0, product = 0;
+        // dz is computed again where it is used, as in the held kernels
+        by_activation(m.activation, [&](auto kind) {
+#pragma unroll
+            for (int k = 0; k < K; k++) {
+                if (k * p.threads >= left) break;
+                const uint32_t at = token_offset<V>(p, k, left);
+                real w[V], b[V];
+                load_weights<T, V>(m, weight, low, at, (real)1, w);
+                load_weights<T, V>(m, bias, low, at, (real)0, b);
+#pragma unroll
+                for (int v = 0; v < V; v++) {
+                    const real hat = (in[k][v] - mean) * rstd;
+                    const real dz = dy[k][v] * activate<decltype(kind)::value, true>(fma(hat, w[v], b[v]));
+                    db[k][v] += dz;
+                    dw[k][v] = fma(dz, hat, dw[k][v]);
+                    sum = fma(dz, w[v], sum);
+                    product = fma(dz * w[v], hat, product);
+                }
+            }
+        });
+        if (!grad_x) continue;
+        sum_token(shared, buffer, sum, product);
+        const real c0 = sum * per_value * rstd, c1 = product * per_value * rstd * rstd;
+        by_activation(m.activation, [&](auto kind) {
+#pragma unroll
+            for (int k = 0; k < K; k++) {
+                if (k * p.threads >= left) break;
+                const uint32_t at = token_offset<V>(p, k, left);
+                real w[V], b[V], out[V];
+                load_weights<T, V>(m, weight, low, at, (real)1, w);
+                load_weights<T, V>(m, bias, low, at, (real)0, b);
+#pragma unroll
+                for (int v = 0; v < V; v++) {
+                    const real d = in[k][v] - mean, wr = rstd * w[v];
+                    const real dz = dy[k][v] * activate<decltype(kind)::value, true>(fma(d, wr, b[v]));
+                    out[v] = fma(dz, wr, fma(d, -c1, -c0));
+                }
+                store_pack<V>(grad_x + base + at, out);
+            }
+        });
+    }
+    if (!partial) return;
+#pragma unroll
+    for (int k = 0; k < K; k++) {
+        if (k * p.threads >= left) break;
+        const uint32_t at = token_offset<V>(p, k, left);
+        store_pack<V>(partial + first_sample * m.channels + low + at, dw[k]);
+        store_pack<V>(partial + (p.workgroups + first_sample) * m.channels + low + at, db[k]);
     }
 }
 
@@ -792,6 +966,8 @@ constexpr int kHeldRows = 8;        // accesses of a thread that are held
 constexpr int64_t kLittle = 1 << 20, kLittleBackward = 1 << 18;
 constexpr int kHeldThreads = 1 << 19;  // of all workgroups together, which go over the samples: the chip's places
 
+constexpr int kTokenThreadsBackward = 1 << 18;  // half as many: each has sums of the weights' gradients to write
+
 // A slab of groups whose rows are 64 bytes or more, if a workgroup can hold it; threads == 0: it cannot.
 static Held held_of(const NormShape &m, int vector, int64_t bytes, bool backward) {
     Held p = {};
@@ -821,6 +997,19 @@ static size_t held_lds(const Held &p, int vector, bool backward) {
     return sizeof(real) * std::max<size_t>(p.in_wave ? 0 : 2 * ((size_t)p.threads + (size_t)p.teams * p.slab_groups), backward ? (size_t)p.threads * vector : 0);
 }
 
+// threads == 0: the samples have more positions, their groups fit a wave or no workgroup holds one.
+static Token token_of(const NormShape &m, int vector, bool backward) {
+    Token p = {};
+    const int64_t units = m.width / vector, all = token_accesses(vector);
+    if (m.positions != 1 || units <= kWave || units > 1024 * all) return p;
+    p.units = (int)units;
+    p.single = backward && units <= 1024;
+    const int64_t most = p.single ? 1 : all;
+    p.threads = (int)(ceil_div64(ceil_div64(units, most), kWave) * kWave);
+    p.workgroups = (int)std::min<int64_t>(m.samples, std::max<int64_t>(1, (backward ? kTokenThreadsBackward : kHeldThreads) / p.threads / m.groups));
+    return p;
+}
+
 static Streamed streamed_of(const NormShape &m, int vector) {
     Streamed p = {};
     const int64_t units = m.channels / vector;
@@ -839,9 +1028,10 @@ static Streamed streamed_of(const NormShape &m, int vector) {
 }
 
 struct NormPlan {
-    bool held;
+    bool held, token;
     int vector;
     Held h;
+    Token t;
     Streamed s;
     int64_t parts, partial, by_group, averages;  // partial sums by channel and by group, averages: elements
     int64_t blocks;
@@ -850,6 +1040,14 @@ static NormPlan plan_of(const NormShape &m, int64_t type, bool backward, bool al
     NormPlan p = {};
     const int64_t bytes = type_bytes(type);
     p.vector = aligned_only ? vector_of(m.width, bytes, {}) : vector_of(m.width, bytes, pointers);
+    p.t = token_of(m, p.vector, backward);
+    p.token = p.t.threads > 0;
+    if (p.token) {
+        p.parts = backward ? p.t.workgroups : 0;
+        p.partial = 2 * p.parts * m.channels;
+        p.blocks = p.t.workgroups * m.groups;
+        return p;
+    }
     p.h = held_of(m, p.vector, bytes, backward);
     const int64_t slabs = p.h.slab_groups ? ceil_div64(m.groups, p.h.slab_groups) : 0;
     // few workgroups leave most of the chip idle: a sample is then better split
@@ -875,7 +1073,7 @@ static int64_t norm_bytes(const NormPlan &p) { return (p.partial + p.by_group + 
 // A grid has fewer than 2^32 threads (of the held kernels it has kHeldThreads, or a workgroup a slab).
 static bool beyond_a_grid(const NormShape &m, const NormPlan &p) {
     const int64_t joins = m.samples * m.groups + ceil_div64(m.channels, kJoinColumns);
-    return !p.held && (p.blocks >= ((int64_t)1 << 32) / kNormThreads || joins >= ((int64_t)1 << 32) / kJoinThreads);
+    return !p.held && !p.token && (p.blocks >= ((int64_t)1 << 32) / kNormThreads || joins >= ((int64_t)1 << 32) / kJoinThreads);
 }
 
 static int too_many(const char *fn) {
@@ -927,6 +1125,11 @@ extern "C" int tg_group_norm_forward(const tg_norm *n) {
         using T = decltype(t);
         constexpr int V = decltype(v)::value;
         const T *x = (const T *)n->x;
+        if (p.token) {
+            TG_LAUNCH_AS("norm_token_forward", (norm_token_forward_kernel<T, V, token_accesses(V)>), dim3((unsigned)p.blocks), dim3((unsigned)p.t.threads), 0, stream, m, p.t, x,
+                         n->weight, n->bias, (T *)n->y, n->statistics);
+            return check_launch(fn);
+        }
         if (p.held) {
             const dim3 grid((unsigned)p.blocks), block((unsigned)p.h.threads);
             const size_t lds = held_lds(p.h, V, false);
@@ -986,10 +1189,16 @@ extern "C" int tg_group_norm_backward(const tg_norm *n) {
         const T *x = (const T *)n->x, *dy = (const T *)n->grad_y;
         real *partial = (real *)n->workspace;
         const unsigned channel_blocks = (unsigned)ceil_div64(m.channels, kJoinColumns);
-        if (p.held) {
-            const dim3 grid((unsigned)p.blocks), block((unsigned)p.h.threads);
-            const size_t lds = held_lds(p.h, V, true);
-            if (m.positions <= p.h.rows)
+        if (p.token || p.held) {
+            const dim3 grid((unsigned)p.blocks), block((unsigned)(p.token ? p.t.threads : p.h.threads));
+            const size_t lds = p.token ? 0 : held_lds(p.h, V, true);
+            if (p.token && p.t.single)
+                TG_LAUNCH_AS("norm_token_backward", (norm_token_backward_kernel<T, V, 1>), grid, block, lds, stream, m, p.t, x, n->weight, n->bias,
+                             n->statistics, dy, (T *)n->grad_x, weights ? partial : nullptr);
+            else if (p.token)
+                TG_LAUNCH_AS("norm_token_backward", (norm_token_backward_kernel<T, V, token_accesses(V)>), grid, block, lds, stream, m, p.t, x, n->weight,
+                             n->bias, n->statistics, dy, (T *)n->grad_x, weights ? partial : nullptr);
+            else if (m.positions <= p.h.rows)
                 TG_LAUNCH_AS("norm_backward", (norm_held_backward_kernel<T, V, 1>), grid, block, lds, stream, m, p.h, x, n->weight, n->bias, n->statistics,
                              dy, (T *)n->grad_x, weights ? partial : nullptr);
             else
