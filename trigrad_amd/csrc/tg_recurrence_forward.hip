@@ -244,28 +244,31 @@ __global__ __launch_bounds__(kMapThreads) void recurrence_maps_kernel(Split m, c
     }
 }
 
-// The states that the chunks start from: the chunks' maps composed as a thread's rows are, 8 channels and 128 runs of chunks a workgroup.
-constexpr int kStartThreads = 1024, kStartLanesLog2 = 3, kStartAhead = 8;
+// The states that the chunks start from: the chunks' maps composed as a thread's rows are, 8 channels and 128 runs of chunks a workgroup.  A run
+// of up to Ahead chunks is read at once and kept; longer ones are read again.  1094 and 2188 chunks of 384 channels, runs of 9 and 18: 24 us
+// together with 24 ahead, 31 with 8; 512 chunks of 2048: 8.5 with 8, 11 with 24.
+constexpr int kStartThreads = 1024, kStartLanesLog2 = 3, kStartRuns = kStartThreads >> kStartLanesLog2, kStartAhead = 8, kStartFurther = 24;
+template <int Ahead>
 __global__ __launch_bounds__(kStartThreads) void recurrence_starts_kernel(int64_t chunks, int64_t channels, bool backward,
                                                                           const MapWords *__restrict__ maps, float *__restrict__ starts) {
     __shared__ Joint<1, kStartThreads> joint;
     Split m = {};
     m.lanes_log2 = kStartLanesLog2;
     const Place p = place_of<kStartThreads>(m);
-    const int64_t channel = ((int64_t)blockIdx.x << kStartLanesLog2) + p.lane, turns = kStartThreads >> kStartLanesLog2, run = (chunks + turns - 1) / turns;
+    const int64_t channel = ((int64_t)blockIdx.x << kStartLanesLog2) + p.lane, run = (chunks + kStartRuns - 1) / kStartRuns;
     const int64_t begin = min(p.turn * run, chunks), end = min(begin + run, chunks);
     const bool valid = channel < channels;
-    MapWords next[kStartAhead];
+    MapWords next[Ahead];
     const auto read = [&](int64_t i) {
 #pragma unroll
-        for (int k = 0; k < kStartAhead; k++) {
+        for (int k = 0; k < Ahead; k++) {
             const int64_t c = min(i + k, max(end - 1, (int64_t)0));
             next[k] = maps[(backward ? chunks - 1 - c : c) * channels + (valid ? channel : 0)];
         }
     };
     const auto over = [&](int64_t i, auto &&call) {
 #pragma unroll
-        for (int k = 0; k < kStartAhead; k++) {
+        for (int k = 0; k < Ahead; k++) {
             Map<1> map;
             map.closed = __float_as_uint(next[k].a) == kClosedMap;
             map.a[0] = map.closed ? 0.0f : next[k].a;
@@ -274,7 +277,7 @@ __global__ __launch_bounds__(kStartThreads) void recurrence_starts_kernel(int64_
         }
     };
     Map<1> total = unit_map<1>();
-    for (int64_t i = begin; i < end; i += kStartAhead) {
+    for (int64_t i = begin; i < end; i += Ahead) {
         read(i);
         over(i, [&](int64_t, Map<1> map) {
             compose(map, total);
@@ -283,8 +286,8 @@ __global__ __launch_bounds__(kStartThreads) void recurrence_starts_kernel(int64_
     }
     float h[1] = {0.0f};
     join<1, kStartThreads, false>(m, joint, p, total, false, h);
-    for (int64_t i = begin; i < end; i += kStartAhead) {
-        if (run > kStartAhead) read(i);
+    for (int64_t i = begin; i < end; i += Ahead) {
+        if (run > Ahead) read(i);
         over(i, [&](int64_t c, const Map<1> &map) {
             if (valid) starts[(backward ? chunks - 1 - c : c) * channels + channel] = h[0];
             step_over(h, map);
@@ -349,9 +352,11 @@ int launch_starts(const tg_recurrence &r, const Split &m, const int32_t *first_s
         return check_launch("tg_linear_recurrence");
     });
     if (code) return code;
-    TG_LAUNCH_AS("recurrence_starts", recurrence_starts_kernel, dim3((unsigned)ceil_div64(m.channels, 1 << kStartLanesLog2)), dim3(kStartThreads), 0,
-                 stream,
-                 m.chunks, m.channels, backward, maps, starts);
+    const dim3 grid((unsigned)ceil_div64(m.channels, 1 << kStartLanesLog2)), block(kStartThreads);
+    if (m.chunks <= kStartRuns * kStartAhead)
+        TG_LAUNCH_AS("recurrence_starts", recurrence_starts_kernel<kStartAhead>, grid, block, 0, stream, m.chunks, m.channels, backward, maps, starts);
+    else
+        TG_LAUNCH_AS("recurrence_starts", recurrence_starts_kernel<kStartFurther>, grid, block, 0, stream, m.chunks, m.channels, backward, maps, starts);
     return check_launch("tg_linear_recurrence");
 }
 
