@@ -11,6 +11,8 @@ an outlier in it.  These go through the formulas to first order; beside that an 
 import pytest
 import torch
 
+import test_norm
+
 U = 2.0 ** -24
 
 
@@ -65,3 +67,12 @@ def test_channels_with_means_of_their_own(cuda):
     rng = torch.Generator(cuda).manual_seed(1)
     x = torch.randn((1, 30000, 64), generator=rng, device=cuda) + 3000.0 + 20.0 * torch.randn((64,), generator=rng, device=cuda)
     assert_near("y", trigrad_amd.group_norm(x, 2), *bounds(x, 2))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("channels,groups,dtype", [(3000, 3000, torch.float32), (3000, 1500, torch.float32), (5000, 1000, torch.bfloat16), (4104, 27, torch.bfloat16),
+                                                   (2999, 2999, torch.float16), (1025, 5, torch.float32)])
+def test_groups_of_several_tiles(channels, groups, dtype, cuda):
+    """Rows of several workgroups, each with some of the groups, the ends of which lie anywhere."""
+    x, w, b, dy = test_norm.make(cuda, groups, (1, 1100, channels), dtype, torch.float32)
+    test_norm.run_and_check(x, groups, w, b, dy, "silu")

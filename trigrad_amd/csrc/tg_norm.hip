@@ -550,6 +550,7 @@ __global__ __launch_bounds__(1024) void norm_token_backward_kernel(NormShape m, 
 struct Streamed {
     int units, rows, tiles;  // units of a row that a workgroup has, its rows at a time, workgroups side by side on a row
     int splits;              // workgroups one after another on a sample
+    int slots;               // groups that a tile can meet
     int64_t split_rows;
 };
 constexpr int kNormThreads = 256, kNormAhead = 8;
@@ -580,7 +581,7 @@ __device__ __forceinline__ void over_rows(const NormShape &m, const Streamed &p,
 }
 
 // A tile's sums of two values by channel, summed by group: a wave each.  A group that goes on in the next tile has a sum there too.
-// [sample][split][tile][group][2]
+// [sample][split][tile][group from the tile's first][2]
 template <class R>
 __device__ __forceinline__ void group_sums(const NormShape &m, const Streamed &p, int64_t n, int split, int tile, int columns, const R *first,
                                            const R *second, R *partial) {
@@ -592,7 +593,7 @@ __device__ __forceinline__ void group_sums(const NormShape &m, const Streamed &p
         R sum = 0;
         for (int64_t c = max(low, g * m.width) + lane; c < min(high, (g + 1) * m.width); c += kWave) sum += from[c - low];
         for (int d = kWave / 2; d > 0; d >>= 1) sum += __shfl_xor(sum, d);
-        if (lane == 0) partial[((((n * p.splits + split) * p.tiles + tile) * m.groups + g) << 1) + (i & 1)] = sum;
+        if (lane == 0) partial[((((n * p.splits + split) * p.tiles + tile) * p.slots + g - g0) << 1) + (i & 1)] = sum;
     }
 }
 
@@ -602,10 +603,11 @@ __device__ __forceinline__ void sum_splits(const NormShape &m, const Streamed &p
     __shared__ double shared[2][Threads / kWave];
     const int64_t columns = (int64_t)p.units * V;
     const int t0 = (int)(g * m.width / columns), t1 = (int)(((g + 1) * m.width - 1) / columns);
+    const int64_t slot = g - t0 * columns / m.width;  // in the group's first tile; the others begin within it
     first = second = 0;
     for (int s = threadIdx.x; s < p.splits; s += Threads)
         for (int t = t0; t <= t1; t++) {
-            const R *at = partial + (((((n * p.splits + s) * p.tiles + t) * m.groups) + g) << 1);
+            const R *at = partial + (((((n * p.splits + s) * p.tiles + t) * p.slots) + (t == t0 ? slot : 0)) << 1);
             first += at[0];
             second += at[1];
         }
@@ -652,7 +654,7 @@ template <class T, int V> __device__ __forceinline__ void merge(Seen<T, V> &s, c
 }
 
 // Sums of x - p and its square by sample, split and group, around the group's first value p: in float32 by thread about means of its own,
-// moved to p and joined in float64, where it does not matter which value of the group p is.  [sample][split][tile][group][2]
+// moved to p and joined in float64, where it does not matter which value of the group p is.
 // 1920 x 1080 x 32 in bfloat16: 45 us (2.9 TB/s) with 126 registers; the pivot read in front of the rows takes six more and 53 us, sums about p
 // in float32 took 43 and lost the variance's digits where p is far from the mean.
 template <class T, int V>
@@ -1055,6 +1057,7 @@ static Streamed streamed_of(const NormShape &m, int vector) {
     p.splits = (int)std::max(splits(kNormAhead, 2048), splits(2, 512));
     p.split_rows = ceil_div64(ceil_div64(m.positions, p.splits), p.rows) * p.rows;
     p.splits = (int)ceil_div64(m.positions, p.split_rows);
+    p.slots = (int)std::min<int64_t>(m.groups, ((int64_t)p.units * vector - 2 + m.width) / m.width + 1);
     return p;
 }
 
@@ -1095,7 +1098,7 @@ static NormPlan plan_of(const NormShape &m, int64_t type, bool backward, bool al
     p.s = streamed_of(m, p.vector);
     p.parts = m.samples * p.s.splits;
     p.partial = backward ? p.parts * 2 * m.channels : 0;
-    p.by_group = p.parts * p.s.tiles * m.groups * 2 * (backward ? 1 : (int64_t)(sizeof(double) / sizeof(real)));  // forward: float64
+    p.by_group = p.parts * p.s.tiles * p.s.slots * 2 * (backward ? 1 : (int64_t)(sizeof(double) / sizeof(real)));  // forward: float64
     p.blocks = p.parts * p.s.tiles;
     p.averages = backward ? m.samples * m.groups * 2 : 0;
     return p;
