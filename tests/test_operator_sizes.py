@@ -22,3 +22,25 @@ def test_group_norm_workspace_is_a_fraction_of_its_input(bits, positions, channe
     there are."""
     code, sizes = norm_sizes(bits, samples=1, positions=positions, channels=channels, groups=groups)
     assert code == 0 and max(sizes) <= positions * channels * TYPES[bits][1] // 4
+
+
+def recurrence_sizes(bits, **kw):
+    from trigrad_amd import _lib
+    kind = TYPES[bits][0]
+    out = (C.c_int64 * 3)()
+    r = _lib.Recurrence(**{**dict(type=kind, gate_type=kind), **kw})
+    return _lib.load(bits).tg_linear_recurrence_sizes(C.byref(r), out), list(out)
+
+
+def test_linear_recurrence_beyond_a_grid():
+    """A grid has fewer than 2^32 threads: of calls that one of the launches is too large for none is made."""
+    most = (1 << 25) - 8  # channels of the starting states' launch, 1024 threads for eight
+    assert recurrence_sizes(32, sequences=1, length=129, channels=most, gate_count=most)[0] == 0
+    assert recurrence_sizes(32, sequences=1, length=129, channels=most + 1, gate_count=most + 1)[0] == -1
+    assert recurrence_sizes(32, sequences=1, length=129, channels=1 << 25, gate_count=1, type=2)[0] == -1
+    assert recurrence_sizes(32, sequences=1, length=128, channels=1 << 25, gate_count=1 << 25)[0] == 0  # a chunk: no such launch
+    # a thread a sequence and channel
+    most = (1 << 32) // 256 - 1
+    assert recurrence_sizes(64, sequences=256, length=1, channels=most, gate_count=1)[0] == 0
+    assert recurrence_sizes(64, sequences=256, length=1, channels=most + 1, gate_count=1)[0] == -1
+    assert recurrence_sizes(64, sequences=1 << 20, length=3, channels=1 << 12, gate_count=1)[0] == -1

@@ -12,6 +12,10 @@
 
 namespace tg {
 
+#ifndef TG_DOUBLE_PRECISION
+static_assert(kForwardThreads == kBackwardThreads && kForwardThreads == kMapThreads, "one bound for the grids of all three");
+#endif
+
 #ifdef TG_DOUBLE_PRECISION
 // ---- one thread a sequence and channel ------------------------------------------------
 
@@ -124,6 +128,13 @@ __global__ __launch_bounds__(kStepThreads) void recurrence_step_kernel(Shape m, 
 
 // ---- host ---------------------------------------------------------------------------------
 
+constexpr int64_t kGridThreads = (int64_t)1 << 32;  // a grid has fewer
+
+static int too_many(const char *fn, int64_t rows, int64_t channels) {
+    set_error("%s: %lld rows of %lld channels are too many", fn, (long long)rows, (long long)channels);
+    return TG_E_ARG;
+}
+
 int recurrence_shape(const char *fn, const tg_recurrence &r, Shape &m) {
     if (r.sequences < 0 || r.length < 0 || r.channels < 0 || r.gate_count < 0 || (r.gate_count == 0) != (r.channels == 0) ||
         (r.gate_count > 0 && r.channels % r.gate_count != 0)) {
@@ -158,7 +169,8 @@ int recurrence_shape(const char *fn, const tg_recurrence &r, Shape &m) {
 
 #ifdef TG_DOUBLE_PRECISION
 
-static int sizes_of(const char *, const tg_recurrence &r, const Shape &m, int64_t out[3]) {
+static int sizes_of(const char *fn, const tg_recurrence &r, const Shape &m, int64_t out[3]) {
+    if (m.sequences * m.channels > kGridThreads - 256) return too_many(fn, m.sequences, m.channels);
     out[0] = (r.offsets ? m.length : m.sequences * m.length) * m.channels * (int64_t)sizeof(real);
     out[1] = 0;
     out[2] = m.sequences * m.channels * (int64_t)sizeof(real);
@@ -262,10 +274,10 @@ static int sizes_of(const char *fn, const tg_recurrence &r, const Shape &m, int6
     for (int aligned = 0; aligned < 2; aligned++)
         for (int backward = 0; backward < 2; backward++) {
             const Split s = split_of(m, packed, 0, vector_of(m.shared, m.channels, aligned), backward);
-            if (s.chunks * s.tiles >= (s.wide ? 1 << 22 : 1 << 24) || (!packed && m.length <= kShortRows && m.sequences * s.columns >= ((int64_t)1 << 32) - kShortThreads)) {
-                set_error("%s: %lld rows of %lld channels are too many", fn, (long long)s.rows, (long long)s.channels);
-                return TG_E_ARG;
-            }
+            if (s.chunks * s.tiles >= kGridThreads / (s.wide ? kWideThreads : kForwardThreads) ||
+                (s.chained && ceil_div64(s.channels, 1 << kStartLanesLog2) >= kGridThreads / kStartThreads) ||
+                (!packed && m.length <= kShortRows && m.sequences * s.columns >= kGridThreads - kShortThreads))
+                return too_many(fn, s.rows, s.channels);
             const Room room = room_of(s, backward);
             out[1 + backward] = std::max(out[1 + backward], room.all);
             out[0] = s.chained ? ceil_div64(s.rows, s.kept_rows) * s.channels * 4 : 0;
@@ -388,7 +400,7 @@ extern "C" int tg_linear_recurrence_step(const void *inputs, const void *gates, 
         set_error("%s: null pointer", fn);
         return TG_E_ARG;
     }
-    if (m.sequences * m.channels >= ((int64_t)1 << 32) - kStepThreads) {
+    if (m.sequences * m.channels >= kGridThreads - kStepThreads) {
         set_error("%s: 2^32 channels of sequences or more", fn);
         return TG_E_ARG;
     }

@@ -247,7 +247,7 @@ __global__ __launch_bounds__(kMapThreads) void recurrence_maps_kernel(Split m, c
 // The states that the chunks start from: the chunks' maps composed as a thread's rows are, 8 channels and 128 runs of chunks a workgroup.  A run
 // of up to Ahead chunks is read at once and kept; longer ones are read again.  1094 and 2188 chunks of 384 channels, runs of 9 and 18: 24 us
 // together with 24 ahead, 31 with 8; 512 chunks of 2048: 8.5 with 8, 11 with 24.
-constexpr int kStartThreads = 1024, kStartLanesLog2 = 3, kStartRuns = kStartThreads >> kStartLanesLog2, kStartAhead = 8, kStartFurther = 24;
+constexpr int kStartRuns = kStartThreads >> kStartLanesLog2, kStartAhead = 8, kStartFurther = 24;
 template <int Ahead>
 __global__ __launch_bounds__(kStartThreads) void recurrence_starts_kernel(int64_t chunks, int64_t channels, bool backward,
                                                                           const MapWords *__restrict__ maps, float *__restrict__ starts) {

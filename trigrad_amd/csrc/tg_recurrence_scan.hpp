@@ -36,6 +36,7 @@ constexpr int kForwardThreads = 256, kForwardRows = 16, kForwardChunk = kForward
 constexpr int kShortRows = 8, kShortThreads = 256;  // sequences of no more rows have kernels of their own
 constexpr int kBackwardThreads = 256, kBackwardRows = 8, kBackwardChunk = kBackwardThreads * kBackwardRows;
 constexpr int kMapThreads = 256;
+constexpr int kStartThreads = 1024, kStartLanesLog2 = 3;  // of the starting states' launch: 8 channels a workgroup
 // Sequences of one chunk to about four have a large workgroup each instead: no first look, no starting states, one launch.
 constexpr int kWideThreads = 1024, kWideRows = 8, kWideChunk = kWideThreads * kWideRows;
 static_assert(kForwardChunk % kBackwardChunk == 0 && kForwardChunk % (8 * kMapThreads) == 0 && kBackwardChunk % (8 * kMapThreads) == 0, "");
