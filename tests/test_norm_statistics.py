@@ -76,3 +76,20 @@ def test_groups_of_several_tiles(channels, groups, dtype, cuda):
     """Rows of several workgroups, each with some of the groups, the ends of which lie anywhere."""
     x, w, b, dy = test_norm.make(cuda, groups, (1, 1100, channels), dtype, torch.float32)
     test_norm.run_and_check(x, groups, w, b, dy, "silu")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("shape,groups,ahead,lines", [((1024, 4096, 257), 1, None, 1), ((2 ** 21, 65), 1, 2048, 1), ((2 ** 25, 64), 8, 65536, 32)])
+def test_long_chains_of_additions(shape, groups, ahead, lines, cuda):
+    """A thread adds at most 256 values to each other, whatever there are: streamed rows, tokens, held samples.  The gradient of the bias where the first value of every
+    chain is 2^24, to which a 1 is lost: 255 and, over the workgroup's threads of a channel, `lines` more additions, each off by u of the sum."""
+    import trigrad_amd
+    channels = shape[-1]
+    x = torch.zeros(shape, dtype=torch.bfloat16, device=cuda)
+    dy = torch.ones(shape, dtype=torch.bfloat16, device=cuda)
+    (dy[:, 0] if ahead is None else dy[:ahead]).fill_(2.0 ** 24)
+    bias = torch.zeros((channels,), device=cuda, requires_grad=True)
+    (got,) = torch.autograd.grad(trigrad_amd.group_norm(x, groups, None, bias), bias, dy)
+    first = shape[0] if ahead is None else ahead
+    want = first * 2.0 ** 24 + (x.numel() // channels - first)
+    assert ((got.double() - want).abs() <= (255 + lines + 8) * U * want).all(), ((got.double() - want).abs().max() / want / U).item()

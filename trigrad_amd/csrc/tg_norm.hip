@@ -9,7 +9,8 @@
 //             time and goes over many, so that the weights' gradients are summed in registers and come to few partial sums.
 //   streamed  a sample's rows are split over workgroups: one launch sums them, a small one joins the sums, one reads the rows again
 //             (from the last to the first, so that what the first launch read last is still near) and writes.
-// Sums are float32 (of at most a few hundred successive additions), joined in float64; all in a fixed order.
+// A thread's sums are float32, of at most kChain values one after another; its workgroup's threads of a channel (at most 1024, of a row of one access)
+// are added in float32 too, or float64 (streamed forward), and workgroups in float64; all in a fixed order.
 #include <algorithm>
 #include <type_traits>
 
@@ -998,6 +999,7 @@ constexpr int kHeldRows = 8;        // accesses of a thread that are held
 // backward, which reads twice as much.
 constexpr int64_t kLittle = 1 << 20, kLittleBackward = 1 << 18;
 constexpr int kHeldThreads = 1 << 19;  // of all workgroups together, which go over the samples: the chip's places
+constexpr int kChain = 256;            // values that a thread adds one after another, into one channel's sum
 
 constexpr int kTokenThreadsBackward = 1 << 18;  // half as many: each has sums of the weights' gradients to write
 
@@ -1039,7 +1041,8 @@ static Token token_of(const NormShape &m, int vector, bool backward) {
     p.single = backward && units <= 1024;
     const int64_t most = p.single ? 1 : all;
     p.threads = (int)(ceil_div64(ceil_div64(units, most), kWave) * kWave);
-    p.workgroups = (int)std::min<int64_t>(m.samples, std::max<int64_t>(1, (backward ? kTokenThreadsBackward : kHeldThreads) / p.threads / m.groups));
+    const int64_t places = (backward ? kTokenThreadsBackward : kHeldThreads) / p.threads / m.groups;
+    p.workgroups = (int)std::min<int64_t>(m.samples, std::max(places, backward ? ceil_div64(m.samples, kChain) : 1));
     return p;
 }
 
@@ -1054,7 +1057,7 @@ static Streamed streamed_of(const NormShape &m, int vector) {
     const auto splits = [&](int64_t rows, int64_t workgroups) {
         return std::max<int64_t>(1, std::min(ceil_div64(m.positions, p.rows * rows), ceil_div64(workgroups, m.samples * p.tiles)));
     };
-    p.splits = (int)std::max(splits(kNormAhead, 2048), splits(2, 512));
+    p.splits = (int)std::max(std::max(splits(kNormAhead, 2048), splits(2, 512)), ceil_div64(m.positions, (int64_t)p.rows * kChain));
     p.split_rows = ceil_div64(ceil_div64(m.positions, p.splits), p.rows) * p.rows;
     p.splits = (int)ceil_div64(m.positions, p.split_rows);
     p.slots = (int)std::min<int64_t>(m.groups, ((int64_t)p.units * vector - 2 + m.width) / m.width + 1);
@@ -1069,6 +1072,7 @@ struct NormPlan {
     Streamed s;
     int64_t parts, partial, by_group, averages;  // partial sums by channel and by group, averages: reals
     int64_t blocks;
+    int threads;
 };
 static NormPlan plan_of(const NormShape &m, int64_t type, bool backward, bool aligned_only, std::initializer_list<const void *> pointers) {
     NormPlan p = {};
@@ -1080,6 +1084,7 @@ static NormPlan plan_of(const NormShape &m, int64_t type, bool backward, bool al
         p.parts = backward ? p.t.workgroups : 0;
         p.partial = 2 * p.parts * m.channels;
         p.blocks = p.t.workgroups * m.groups;
+        p.threads = p.t.threads;
         return p;
     }
     p.h = held_of(m, p.vector, bytes, backward);
@@ -1087,10 +1092,12 @@ static NormPlan plan_of(const NormShape &m, int64_t type, bool backward, bool al
     // few workgroups leave most of the chip idle: a sample is then better split
     p.held = p.h.threads > 0 && (p.h.turns * slabs >= 128 || m.samples * m.positions * m.channels * bytes <= (backward ? kLittleBackward : kLittle));
     if (p.held) {
-        p.h.workgroups = (int)std::min<int64_t>(p.h.turns, std::max<int64_t>(1, kHeldThreads / p.h.threads / slabs));
+        const int64_t places = std::max<int64_t>(1, kHeldThreads / p.h.threads / slabs), turns = kChain / ceil_div64(m.positions, p.h.rows);
+        p.h.workgroups = (int)std::min(p.h.turns, std::max(places, backward ? ceil_div64(p.h.turns, turns) : 1));
         p.parts = backward ? p.h.workgroups : 0;
         p.partial = 2 * p.parts * m.channels;
         p.blocks = p.h.workgroups * slabs;
+        p.threads = p.h.threads;
         return p;
     }
     const int64_t widest = backward ? gradient_bytes(bytes) : 16;
@@ -1100,15 +1107,16 @@ static NormPlan plan_of(const NormShape &m, int64_t type, bool backward, bool al
     p.partial = backward ? p.parts * 2 * m.channels : 0;
     p.by_group = p.parts * p.s.tiles * p.s.slots * 2 * (backward ? 1 : (int64_t)(sizeof(double) / sizeof(real)));  // forward: float64
     p.blocks = p.parts * p.s.tiles;
+    p.threads = kNormThreads;
     p.averages = backward ? m.samples * m.groups * 2 : 0;
     return p;
 }
 static int64_t norm_bytes(const NormPlan &p) { return (p.partial + p.by_group + p.averages) * (int64_t)sizeof(real); }
 
-// A grid has fewer than 2^32 threads (of the held kernels it has kHeldThreads, or a workgroup a slab).
+// A grid has fewer than 2^32 threads.
 static bool beyond_a_grid(const NormShape &m, const NormPlan &p) {
-    const int64_t joins = m.samples * m.groups + ceil_div64(m.channels, kJoinColumns);
-    return !p.held && !p.token && (p.blocks >= ((int64_t)1 << 32) / kNormThreads || joins >= ((int64_t)1 << 32) / kJoinThreads);
+    const int64_t joins = (p.held || p.token ? 0 : m.samples * m.groups) + ceil_div64(m.channels, kJoinColumns), most = (int64_t)1 << 32;
+    return p.blocks >= most / p.threads || joins >= most / kJoinThreads;
 }
 
 static int too_many(const char *fn) {
