@@ -31,13 +31,14 @@ __device__ __forceinline__ real inverse_root(real v) { return 1.0 / sqrt(v); }
 #else
 // 1 / sqrt(v) to one unit; the hardware's takes numbers below the normal ones for 0
 __device__ __forceinline__ real inverse_root(real v) { return v < 2.0f * FLT_MIN ? 1.0f / sqrtf(v) : __builtin_amdgcn_rsqf(v); }
+// As a power of two of a rounded product, which is half a step of z: what z's own rounding, a step before, costs the exponential too.
 __device__ __forceinline__ real exp_norm(real z) { return __builtin_amdgcn_exp2f(z * 1.44269504f); }
 __device__ __forceinline__ real inverse(real v) { return __builtin_amdgcn_rcpf(v); }
 #endif
 
 // Phi(-|z|) / exp(-z^2 / 2), Phi the normal distribution: a quotient that varies so little that a polynomial of 1 / (1 + 0.3 |z|) has it to
-// five units of 2^-24 of itself wherever the exponential is not 0 (the coefficients by weighted least squares for the smallest relative error),
-// so that the activation keeps its digits far out on the negative side too.
+// ten units of 2^-24 of itself wherever the exponential is not 0, three of them the reciprocal's (the coefficients by weighted least squares for
+// the smallest relative error).  So the activation falls off with its exponential on the negative side instead of ending in a difference's rounding.
 __device__ __forceinline__ real mills(real z) {
 #ifdef TG_DOUBLE_PRECISION
     return z * z < 1400.0 ? 0.5 * erfc(fabs(z) * 0.70710678118654752440) / exp(-0.5 * z * z) : 0.0;
@@ -659,7 +660,7 @@ template <class T, int V> __device__ __forceinline__ void merge(Seen<T, V> &s, c
 
 // Sums of x - p and its square by sample, split and group, around the group's first value p: in float32 by thread about means of its own,
 // moved to p and joined in float64, where it does not matter which value of the group p is.
-// 1920 x 1080 x 32 in bfloat16: 45 us (2.9 TB/s) with 126 registers; the pivot read in front of the rows takes six more and 53 us, sums about p
+// 1920 x 1080 x 32 in bfloat16: 42 us (3.2 TB/s) with 126 registers; the pivot read in front of the rows takes six more and 53 us, sums about p
 // in float32 took 43 and lost the variance's digits where p is far from the mean.
 template <class T, int V>
 __global__ __launch_bounds__(kNormThreads) void norm_sums_kernel(NormShape m, Streamed p, const T *__restrict__ x, double *__restrict__ partial) {
@@ -975,8 +976,8 @@ static int vector_of(int64_t run, int64_t bytes, std::initializer_list<const voi
     return 1;
 }
 // What a thread of the streamed backward kernels reads at once: 16 bytes, or four elements of 16 bits.  Eight of them took 149 registers for the
-// sums and 87 us where four take 92 and 73 (1920 x 1080 x 32 in bfloat16); forward, where there is one array to read, eight are faster (45 us
-// to 56).
+// sums and 87 us where four take 92 and 68 (1920 x 1080 x 32 in bfloat16); forward, where there is one array to read, eight are faster (sums 42 us
+// to 50, the second reading 51 to 54).
 static int64_t gradient_bytes(int64_t element) { return std::min<int64_t>(16, 4 * element); }
 
 // call(T(), integral_constant of the elements of an access), the most of 16-bit ones being Widest.

@@ -5,8 +5,8 @@
 // forward call kept for every chunk: x is read in the place of h, which comes without having been rounded.
 //
 // Eight rows a thread, since x, dh, the gates and eight states of each channel are held: 116 registers with shared gates, 136 without (three waves a
-// SIMD; held to 128 it spills and takes 94 us where it takes 63, 2 x 8192 x 1536 in half precision).  4 x 4096 x 2048 with 16 gates: 57 us,
-// 3.5 TB/s, of which the vector instructions are 35.
+// SIMD; held to 128 it spills and takes 94 us where it takes 63, 2 x 8192 x 1536 in half precision).  4 x 4096 x 2048 with 16 gates: 56 us,
+// 3.6 TB/s, of which the vector instructions are 35.
 #include "tg_recurrence_scan.hpp"
 
 #ifndef TG_DOUBLE_PRECISION

@@ -12,11 +12,11 @@
 // The order of operations is fixed: results do not depend on timing, and no workgroup waits for another.
 //
 // Bound by memory traffic, and by vector instructions beside it (about 20 an element with a logistic function, 10 without).  The first look
-// costs reading inputs twice (backward: gates and dh, not x), the second time mostly from the last-level cache: what is read for
-// the first time comes at 3.9 TB/s on this chip, a copy goes at 4.9 TB/s in and out together.  For 32768 x 2048 in bfloat16 with a gate for every channel
-// the first look takes 69 us (268 MB), the starting states 6, the chunks 91 (402 MB, 4.4 TB/s).  A single launch in which chunks waited for the
-// maps of those before them read everything once and was no faster forward (165 us and the clearing of its words) and slower backward
-// (4 x 4096 x 2048, 16 gates: 148 us against 57 + 6 + 21): a chunk held its registers for three round trips through memory more.
+// costs reading inputs twice (backward: gates and dh, not x).  For 32768 x 2048 in bfloat16 with a gate for every channel it takes 67 us (268 MB,
+// 4.0 TB/s where a kernel that only reads reaches 5), the starting states 8, the chunks 89 (402 MB, 4.5 TB/s).  A single launch in which chunks waited
+// for the maps of those before them read everything once and was no faster forward (155 us at 2.6 TB/s, and the clearing of its words) and slower
+// backward (4 x 4096 x 2048, 16 gates: 148 us against 56 + 7 + 22): its chunks waited for each other, with their registers held for three
+// round trips through memory more.
 //
 // Chunks are small, four or eight waves a SIMD's worth of workgroups beside each other, because a workgroup reads, computes and writes one after
 // another: with 1024 threads, one workgroup a CU, the same backward pass took 80 us.  Chunks of half the rows again would double what the maps and

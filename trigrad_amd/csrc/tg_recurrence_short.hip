@@ -1,8 +1,8 @@
 // tg_recurrence_short.hip -- the gated linear recurrence over sequences of at most eight rows: compositing a few slabs of an image.
 //
 // A thread has a sequence's rows of V channels in registers and walks them, so nothing is composed and nothing waits: memory traffic alone
-// bounds it: eight slabs of 1920 x 1080 take 73 us forward (290 MB read or written, 4.0 TB/s) and 95 backward (555 MB, 5.8 TB/s, part of it still in the
-// last-level cache).  The kernels for longer sequences, with their tables of where sequences begin, took 90 and 175.
+// bounds it: eight slabs of 1920 x 1080 take 72 us forward (290 MB read or written, 4.0 TB/s) and 95 backward (555 MB, 5.8 TB/s; the inputs were
+// read by the forward pass just before).  The kernels for longer sequences, with their tables of where sequences begin, took 90 and 175.
 #include "tg_recurrence_scan.hpp"
 
 #ifndef TG_DOUBLE_PRECISION
