@@ -93,3 +93,26 @@ def test_long_chains_of_additions(shape, groups, ahead, lines, cuda):
     first = shape[0] if ahead is None else ahead
     want = first * 2.0 ** 24 + (x.numel() // channels - first)
     assert ((got.double() - want).abs() <= (255 + lines + 8) * U * want).all(), ((got.double() - want).abs().max() / want / U).item()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("shape,groups", [((64, 512), 8), ((64, 8, 64), 4), ((64, 1024), 1), ((64, 1001), 1), ((1, 30000, 32), 8)])
+def test_the_slope_of_relu_is_its_outputs(shape, groups, cuda):
+    """At the border, where the rounding decides: an output above 0 passes its gradient on, to the bias, the weight and x alike, and one of 0 to none."""
+    import trigrad_amd
+    rng = torch.Generator(cuda).manual_seed(1)
+    channels = shape[-1]
+    x = torch.randn(shape, generator=rng, device=cuda)
+    weight = torch.rand((channels,), generator=rng, device=cuda) + 0.5
+    hat, _ = bounds(x, groups)
+    at = (0,) * (len(shape) - 1)  # the position that z is put to the border for, in every channel
+    bias = -(hat[at] * weight).float()
+    leaves = [t.requires_grad_() for t in (x, weight, bias)]
+    y = trigrad_amd.group_norm(leaves[0], groups, leaves[1], leaves[2], activation="relu")
+    dy = torch.zeros_like(y)
+    dy[at] = 1.0
+    dx, dw, db = torch.autograd.grad(y, leaves, dy)
+    passes = y.detach()[at] > 0
+    assert 0.2 < passes.float().mean() < 0.8
+    assert torch.equal(db, passes.float())
+    assert torch.equal(dw != 0, passes)

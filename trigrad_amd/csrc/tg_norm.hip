@@ -292,7 +292,7 @@ __global__ __launch_bounds__(1024) void norm_held_forward_kernel(NormShape m, He
                 if (k >= rows) break;
                 real out[V];
 #pragma unroll
-                for (int v = 0; v < V; v++) out[v] = activate<decltype(kind)::value, false>(fma(in[k][v] - mean, rstd * w[v], b[v]));
+                for (int v = 0; v < V; v++) out[v] = activate<decltype(kind)::value, false>(fma((in[k][v] - mean) * rstd, w[v], b[v]));
                 store_pack<V>(y + base + pitch * k, out);
             }
         });
@@ -322,7 +322,8 @@ __global__ __launch_bounds__(1024) void norm_held_backward_kernel(NormShape m, H
         const Pack<real, 2> of = load_pack<2>(statistics + (r.active ? 2 * (r.n * m.groups + t.group) : 0));
         const real mean = of[0], rstd = of[1];
         real sum = 0, product = 0;
-        // dz is computed again where it is used: its 32 bits are not held
+        // dz is computed again where it is used: its 32 bits are not held.  z has the same roundings everywhere, so that at the border of ReLU the
+        // output and all gradients agree on the slope.
         by_activation(m.activation, [&](auto kind) {
 #pragma unroll
             for (int k = 0; k < K; k++)
@@ -340,7 +341,7 @@ __global__ __launch_bounds__(1024) void norm_held_backward_kernel(NormShape m, H
         });
         if (grad_x) {
             sum_groups(p, t.segment, t.member, t.members, r.active, sum, product, shared);
-            const real c0 = sum * per_value * rstd, c1 = product * per_value * rstd * rstd;
+            const real c0 = sum * per_value, c1 = product * per_value;
             by_activation(m.activation, [&](auto kind) {
 #pragma unroll
                 for (int k = 0; k < K; k++) {
@@ -348,9 +349,9 @@ __global__ __launch_bounds__(1024) void norm_held_backward_kernel(NormShape m, H
                     real out[V];
 #pragma unroll
                     for (int v = 0; v < V; v++) {
-                        const real d = in[k][v] - mean, wr = rstd * w[v];
-                        const real dz = dy[k][v] * activate<decltype(kind)::value, true>(fma(d, wr, b[v]));
-                        out[v] = fma(dz, wr, fma(d, -c1, -c0));
+                        const real hat = (in[k][v] - mean) * rstd;
+                        const real dz = dy[k][v] * activate<decltype(kind)::value, true>(fma(hat, w[v], b[v]));
+                        out[v] = rstd * fma(dz, w[v], fma(hat, -c1, -c0));
                     }
                     store_pack<V>(grad_x + base + pitch * k, out);
                 }
@@ -463,7 +464,7 @@ __global__ __launch_bounds__(1024) void norm_token_forward_kernel(NormShape m, T
                 load_weights<T, V>(m, weight, low, at, (real)1, w);
                 load_weights<T, V>(m, bias, low, at, (real)0, b);
 #pragma unroll
-                for (int v = 0; v < V; v++) out[v] = activate<decltype(kind)::value, false>(fma(in[k][v] - mean, rstd * w[v], b[v]));
+                for (int v = 0; v < V; v++) out[v] = activate<decltype(kind)::value, false>(fma((in[k][v] - mean) * rstd, w[v], b[v]));
                 store_pack<V>(y + base + at, out);
             }
         });
@@ -518,7 +519,7 @@ __global__ __launch_bounds__(1024) void norm_token_backward_kernel(NormShape m, 
         });
         if (!grad_x) continue;
         sum_token(shared, buffer, sum, product);
-        const real c0 = sum * per_value * rstd, c1 = product * per_value * rstd * rstd;
+        const real c0 = sum * per_value, c1 = product * per_value;
         by_activation(m.activation, [&](auto kind) {
 #pragma unroll
             for (int k = 0; k < K; k++) {
@@ -529,9 +530,9 @@ __global__ __launch_bounds__(1024) void norm_token_backward_kernel(NormShape m, 
                 load_weights<T, V>(m, bias, low, at, (real)0, b);
 #pragma unroll
                 for (int v = 0; v < V; v++) {
-                    const real d = in[k][v] - mean, wr = rstd * w[v];
-                    const real dz = dy[k][v] * activate<decltype(kind)::value, true>(fma(d, wr, b[v]));
-                    out[v] = fma(dz, wr, fma(d, -c1, -c0));
+                    const real hat = (in[k][v] - mean) * rstd;
+                    const real dz = dy[k][v] * activate<decltype(kind)::value, true>(fma(hat, w[v], b[v]));
+                    out[v] = rstd * fma(dz, w[v], fma(hat, -c1, -c0));
                 }
                 store_pack<V>(grad_x + base + at, out);
             }
