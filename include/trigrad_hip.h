@@ -595,6 +595,104 @@ int tg_group_norm_sizes(const tg_norm *n, int64_t out[2]);
 int tg_group_norm_forward(const tg_norm *n);
 int tg_group_norm_backward(const tg_norm *n);
 
+/* Linear attention: S_t = a_t S_{t-1} + k_t v_t^T, o_t = scale S_t^T q_t for every sequence and head, the recurrence above with
+ * a state of key_size x value_size (each at most TG_ATTENTION_SIZE) for a head.
+ *   a = exp(gate) (TG_GATE_LOG) or 1 / (1 + exp(-gate)) (TG_GATE_LOGIT), at most 1; minus infinity is a = 0.
+ * queries and keys are (sequences, length, key_heads, key_size), values (sequences, length, heads, value_size), (length, ...) with
+ * offsets, as above; heads is a multiple of key_heads, and value head h goes with key head h key_heads / heads.  Their last
+ * dimension is dense; the strides of the others (sequence, row, head) are in elements, may be any and are also those of
+ * grad_outputs.  gates: (rows, heads), or (heads) where fixed_gates.  outputs (rows, heads, value_size) and all gradients are
+ * dense; the gradients' rows of no sequence are zeros, as are the outputs'.
+ * initial, final and their gradients are (sequences, heads, key_size, value_size) tg_real; initial, grad_final and every
+ * gradient but grad_outputs may be null (grad_outputs too, then it is zeros).
+ * tg_linear_attention_sizes writes the bytes of `kept` (what the forward call leaves for the backward call; null where none
+ * follows) and of the workspaces of a forward call that is not followed by a backward call, of one that is, and of the backward call. */
+#define TG_ATTENTION_SIZE 128
+
+typedef struct tg_attention {
+    const void *queries;      /* type */
+    const void *keys;
+    const void *values;
+    const void *gates;        /* gate_type: that of values, or tg_real */
+    const tg_real *initial;
+    const int32_t *offsets;   /* (sequences + 1) or null */
+    void *outputs;            /* type */
+    tg_real *final;
+    void *kept;
+    void *workspace;
+    void *stream;
+    const void *grad_outputs; /* type */
+    const tg_real *grad_final;
+    void *grad_queries;       /* type */
+    void *grad_keys;
+    void *grad_values;
+    void *grad_gates;         /* gate_type */
+    tg_real *grad_initial;
+    int64_t sequences;
+    int64_t length;
+    int64_t heads;
+    int64_t key_heads;
+    int64_t key_size;
+    int64_t value_size;
+    int64_t query_strides[3];
+    int64_t key_strides[3];
+    int64_t value_strides[3];
+    int64_t grad_strides[3];
+    int64_t type;
+    int64_t gate_type;
+    int64_t gate_form;
+    int64_t fixed_gates;
+    int64_t kept_bytes;
+    int64_t workspace_bytes;
+    double scale;
+} tg_attention;
+
+int tg_linear_attention_sizes(const tg_attention *a, int64_t out[4]);
+int tg_linear_attention_forward(const tg_attention *a);
+int tg_linear_attention_backward(const tg_attention *a);
+/* One step of every sequence: length is 1, initial the states and final the new ones, which may be the same; kept and workspace
+ * are not used. */
+int tg_linear_attention_step(const tg_attention *a);
+
+/* One step of AdamW over `count` tensors of sizes[i] elements each, in place:
+ *   g = grad grad_scale, m = b1 m + (1 - b1) g, v = b2 v + (1 - b2) g^2,
+ *   p = p (1 - rate decay) - rate / (1 - b1^t) m / (sqrt(v / (1 - b2^t)) + eps);  maximize: -g for g.
+ * params are tg_real, grads of any type, copies (null, or each null) the new params in a type of 16 bits.  t is `step`, or
+ * device_step[0] (float32); the rate is `rate`, or device_rate[0]; grad_scale may be null.  Nothing that is written may overlap
+ * anything else.
+ * bits 32: averages and squares hold m and v as tg_real.  bits 8 (float library): they hold m and sqrt(v) in 8 bits (sign, 4 of
+ * exponent, 3 of fraction, largest 448, smallest 2^-9) in units of scales[i][b][0] and [1] for elements 256 b to 256 b + 255 of
+ * tensor i: the block's largest / 448.  A value becomes one of its two neighbours, the upper one with the probability of what lies
+ * below, by 16 bits of a number mixed of `seed` and the element's place (the tensors laid end to end, each from a multiple of
+ * 256), so that an average of many small changes moves as it should; a square that is not zero does not become zero. */
+typedef struct tg_adamw {
+    tg_real *const *params;
+    const void *const *grads;
+    void *const *averages;
+    void *const *squares;
+    void *const *copies;
+    tg_real *const *scales;
+    const int64_t *sizes;
+    const int64_t *grad_types;
+    const int64_t *copy_types;
+    const float *device_step;
+    const float *device_rate;
+    const tg_real *grad_scale;
+    void *stream;
+    int64_t count;
+    int64_t bits;
+    int64_t seed;
+    int64_t maximize;
+    double step;
+    double rate;
+    double beta1;
+    double beta2;
+    double eps;
+    double decay;
+} tg_adamw;
+
+int tg_adamw_step(const tg_adamw *a);
+
 /* ---- host-side component hooks ---------------------------------------------- */
 
 /* HOST pointers, run on the CPU.  The reference exports the same six functions

@@ -1393,3 +1393,106 @@ def group_norm_backward(grad_y, x, groups, weight, bias, statistics, eps, activa
         n.grad_x, n.grad_weight, n.grad_bias = _address(grad_x), _address(grad_weight), _address(grad_bias)
         _lib.check(lib.tg_group_norm_backward(C.byref(n)), "tg_group_norm_backward", _bits(x))
     return grad_x, grad_weight, grad_bias
+
+
+# ---- linear attention, AdamW ------------------------------------------------------------
+
+def rows_as_they_lie(t):
+    """`t` with its last dimension dense and no negation still to be done; other dimensions keep their strides."""
+    t = t.resolve_neg()
+    return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
+
+
+def _strides(t, packed):
+    """(sequence, row, head) of a (S, T, H, D) or (T, H, D) tensor."""
+    return (C.c_int64 * 3)(0, *t.stride()[:2]) if packed else (C.c_int64 * 3)(*t.stride()[:3])
+
+
+def _attention(queries, keys, values, gates, offsets, sequences, length, gate_form, scale):
+    packed = offsets is not None
+    a = _lib.Attention(queries=_address(queries), keys=_address(keys), values=_address(values), gates=_address(gates), offsets=_address(offsets),
+                       stream=_raw_stream(values.device), sequences=sequences, length=length, heads=values.shape[-2], key_heads=keys.shape[-2],
+                       key_size=keys.shape[-1], value_size=values.shape[-1], query_strides=_strides(queries, packed), key_strides=_strides(keys, packed),
+                       value_strides=_strides(values, packed), type=TYPE_CODES[values.dtype], gate_type=TYPE_CODES[gates.dtype], gate_form=gate_form,
+                       fixed_gates=gates.dim() == 1, scale=scale)
+    lib, sizes = _lib.load(_bits(values)), (C.c_int64 * 4)()
+    _lib.check(lib.tg_linear_attention_sizes(C.byref(a), sizes), "tg_linear_attention_sizes", _bits(values))
+    return lib, a, sizes
+
+
+def _attention_states(keys, values, sequences):
+    return torch.empty((sequences, values.shape[-2], keys.shape[-1], values.shape[-1]), dtype=real_type(values.dtype), device=values.device)
+
+
+def linear_attention_forward(queries, keys, values, gates, initial, offsets, sequences, length, gate_form, scale, for_backward):
+    """-> (outputs, final, kept or None); arguments whose last dimension is dense, checked by trigrad_amd.linear_attention."""
+    dev = values.device
+    with _on_device(dev):
+        lib, a, sizes = _attention(queries, keys, values, gates, offsets, sequences, length, gate_form, scale)
+        outputs = torch.empty(values.shape, dtype=values.dtype, device=dev)
+        final = _attention_states(keys, values, sequences)
+        kept = torch.empty((sizes[0],), dtype=torch.uint8, device=dev) if for_backward else None
+        room = sizes[2] if for_backward else sizes[1]
+        workspace = _bytes(room, dev)
+        a.initial, a.outputs, a.final = _address(initial), _address(outputs), _address(final)
+        a.kept, a.kept_bytes, a.workspace, a.workspace_bytes = _address(kept), sizes[0] if for_backward else 0, _address(workspace), room
+        _lib.check(lib.tg_linear_attention_forward(C.byref(a)), "tg_linear_attention_forward", _bits(values))
+    return outputs, final, kept
+
+
+def linear_attention_backward(queries, keys, values, gates, initial, offsets, kept, grad_outputs, grad_final, sequences, length, gate_form, scale, needed):
+    """-> gradients of queries, keys, values, gates and the initial states, None where not needed."""
+    dev = values.device
+    with _on_device(dev):
+        lib, a, sizes = _attention(queries, keys, values, gates, offsets, sequences, length, gate_form, scale)
+        workspace = _bytes(sizes[3], dev)
+        if grad_outputs is not None:
+            grad_outputs = rows_as_they_lie(grad_outputs)
+            a.grad_outputs, a.grad_strides = _address(grad_outputs), _strides(grad_outputs, offsets is not None)
+        grad_final = None if grad_final is None else dense(grad_final)
+        grads = [torch.empty(t.shape, dtype=t.dtype, device=dev) if need else None for t, need in zip((queries, keys, values, gates), needed)]
+        grads.append(_attention_states(keys, values, sequences) if needed[4] else None)
+        a.initial, a.kept, a.kept_bytes, a.grad_final = _address(initial), _address(kept), sizes[0], _address(grad_final)
+        a.workspace, a.workspace_bytes = _address(workspace), sizes[3]
+        a.grad_queries, a.grad_keys, a.grad_values, a.grad_gates, a.grad_initial = (_address(t) for t in grads)
+        _lib.check(lib.tg_linear_attention_backward(C.byref(a)), "tg_linear_attention_backward", _bits(values))
+    return grads
+
+
+def linear_attention_step(queries, keys, values, gates, state, new_state, gate_form, scale):
+    """-> the outputs; new_state receives the new states."""
+    with _on_device(values.device):
+        outputs = torch.empty(values.shape, dtype=values.dtype, device=values.device)
+        _, a, _ = _attention(queries[:, None], keys[:, None], values[:, None], gates, None, values.shape[0], 1, gate_form, scale)
+        a.initial, a.outputs, a.final = _address(state), _address(outputs), _address(new_state)
+        _lib.check(_lib.load(_bits(values)).tg_linear_attention_step(C.byref(a)), "tg_linear_attention_step", _bits(values))
+    return outputs
+
+
+def adamw_step(params, grads, averages, squares, copies, scales, step, rate, grad_scale, bits, **numbers):
+    """Arguments checked by trigrad_amd.adamw_step; `step` and `rate` are numbers or tensors of one."""
+    count = len(params)
+    device = params[0].device
+
+    def pointers(tensors):
+        return (C.c_void_p * count)(*[_address(t) for t in tensors])
+
+    def codes(values):
+        return (C.c_int64 * count)(*values)
+    with _on_device(device):
+        kept = [pointers(params), pointers(grads), pointers(averages), pointers(squares), codes(t.numel() for t in params),
+                codes(TYPE_CODES[t.dtype] for t in grads)]
+        a = _lib.AdamW(**dict(zip(("params", "grads", "averages", "squares", "sizes", "grad_types"), (C.cast(k, C.c_void_p) for k in kept))),
+                       grad_scale=_address(grad_scale), stream=_raw_stream(device), count=count, bits=bits, **numbers)
+        if copies is not None:
+            kept += [pointers(copies), codes(0 if t is None else TYPE_CODES[t.dtype] for t in copies)]
+            a.copies, a.copy_types = C.cast(kept[-2], C.c_void_p), C.cast(kept[-1], C.c_void_p)
+        if scales is not None:
+            kept.append(pointers(scales))
+            a.scales = C.cast(kept[-1], C.c_void_p)
+        for name, value in (("step", step), ("rate", rate)):
+            if isinstance(value, torch.Tensor):
+                setattr(a, "device_" + name, _address(value))
+            else:
+                setattr(a, name, value)
+        _lib.check(_lib.load(_bits(params[0])).tg_adamw_step(C.byref(a)), "tg_adamw_step", _bits(params[0]))

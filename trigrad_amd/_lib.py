@@ -82,6 +82,11 @@ SIGNATURES = {
     "tg_group_norm_sizes": (_i, [_p, _p]),
     "tg_group_norm_forward": (_i, [_p]),
     "tg_group_norm_backward": (_i, [_p]),
+    "tg_linear_attention_sizes": (_i, [_p, _p]),
+    "tg_linear_attention_forward": (_i, [_p]),
+    "tg_linear_attention_backward": (_i, [_p]),
+    "tg_linear_attention_step": (_i, [_p]),
+    "tg_adamw_step": (_i, [_p]),
     "tg_barycentric": (None, [_p] * 5),
     "tg_barycentric_backward": (None, [_p] * 6),
     "tg_interpolate3_scalar": (_f, [_p, _f, _f, _f, _p]),
@@ -106,6 +111,20 @@ class Norm(C.Structure):
     """tg_norm"""
     _fields_ = _fields("x weight bias y statistics workspace stream grad_y grad_x grad_weight grad_bias",
                        "samples positions channels groups type weight_type activation workspace_bytes", ("eps", C.c_double))
+
+
+class Attention(C.Structure):
+    """tg_attention"""
+    _fields_ = (_fields("queries keys values gates initial offsets outputs final kept workspace stream grad_outputs grad_final grad_queries "
+                        "grad_keys grad_values grad_gates grad_initial", "sequences length heads key_heads key_size value_size")
+                + [(name, _i64 * 3) for name in ("query_strides", "key_strides", "value_strides", "grad_strides")]
+                + _fields("", "type gate_type gate_form fixed_gates kept_bytes workspace_bytes", ("scale", C.c_double)))
+
+
+class AdamW(C.Structure):
+    """tg_adamw"""
+    _fields_ = _fields("params grads averages squares copies scales sizes grad_types copy_types device_step device_rate grad_scale stream",
+                       "count bits seed maximize", *((name, C.c_double) for name in ("step", "rate", "beta1", "beta2", "eps", "decay")))
 
 
 _libs = {}
