@@ -25,7 +25,7 @@ TORCH_MODULE_PATH = os.path.join(LIB_DIR, "trigrad_torch.so")
 SOURCES = ["tg_api.hip", "tg_binning.hip", "tg_scan.hip", "tg_sort.hip", "tg_forward.hip", "tg_forward_few.hip", "tg_forward_packed.hip",
            "tg_backward.hip", "tg_backward_packed.hip", "tg_components.hip", "tg_camera.hip", "tg_frame.hip",
            "tg_recurrence.hip", "tg_recurrence_forward.hip", "tg_recurrence_backward.hip", "tg_recurrence_short.hip", "tg_norm.hip",
-           "tg_attention.hip", "tg_adamw.hip"]
+           "tg_attention.hip", "tg_attention_forward.hip", "tg_attention_backward.hip", "tg_adamw.hip"]
 
 FLAGS = [
     "--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC",

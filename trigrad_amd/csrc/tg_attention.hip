@@ -4,16 +4,21 @@
 //     D_t = a_{t+1} D_{t+1} + scale q_t do_t^T,   dq_t = scale S_t do_t,   dk_t = D_t v_t,   dv_t = D_t^T k_t,   dlog a_t = a_t <D_t, S_{t-1}>,
 // and since <D_t, S_t> is both q_t.dq_t + dlog a_{t+1} and k_t.dk_t + dlog a_t,
 //     dlog a_{t+1} = dlog a_t + k_t.dk_t - q_t.dq_t,   dlog a_1 = <S_0, a_1 D_1>.
+#ifdef TG_DOUBLE_PRECISION
 #include "tg_attention.hpp"
+#else
+#include "tg_attention_chunk.hpp"
+#endif
 
 namespace tg {
-
-// ---- a walk through the rows ----------------------------------------------------------
 
 constexpr int kWalkThreads = 64;
 constexpr int kMost = TG_ATTENTION_SIZE;
 
 template <class T> __device__ __forceinline__ double wide(T v) { return (double)(real)v; }
+
+#ifdef TG_DOUBLE_PRECISION
+// ---- a walk through the rows ----------------------------------------------------------
 
 // A thread has a column of the state, in LDS.
 template <class T, class S>
@@ -133,6 +138,135 @@ __global__ __launch_bounds__(kWalkThreads) void attention_walk_gates_kernel(Atte
     if (m.fixed && lane == 0) sums[s * m.heads + h] = all;
 }
 
+#else
+// ---- units of chunks -------------------------------------------------------------------
+
+constexpr int kPlanThreads = 1024, kScanThreads = 256;
+
+__device__ __forceinline__ int64_t units_of(const AttentionCall &c, int64_t s, int64_t unit_rows, int64_t &first) {
+    if (!c.m.packed) {
+        first = s * c.units;
+        return c.units;
+    }
+    first = c.plan[c.most_units + s];
+    return max((int64_t)0, min((rows_of(c.m, c.offsets, s).count + unit_rows - 1) / unit_rows, c.most_units - first));
+}
+
+// Packed sequences' units: which sequence each is of, and every sequence's first.  One workgroup.
+__global__ __launch_bounds__(kPlanThreads) void attention_plan_kernel(Attention m, const int32_t *__restrict__ offsets, int64_t unit_rows, int64_t most, int32_t *plan) {
+    __shared__ int64_t waves[kPlanThreads / kWave];
+    const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
+    int64_t before = 0;
+    for (int64_t first = 0; first < m.sequences; first += kPlanThreads) {
+        const int64_t s = first + threadIdx.x, n = s < m.sequences ? (rows_of(m, offsets, s).count + unit_rows - 1) / unit_rows : 0;
+        int64_t sum = n;
+#pragma unroll
+        for (int step = 1; step < kWave; step *= 2) {
+            const int64_t other = __shfl_up(sum, step);
+            if (lane >= step) sum += other;
+        }
+        if (lane == kWave - 1) waves[wave] = sum;
+        __syncthreads();
+        int64_t at = before + sum - n;
+        for (int w = 0; w < kPlanThreads / kWave; w++) {
+            if (w < wave) at += waves[w];
+            before += waves[w];
+        }
+        if (s < m.sequences) {
+            plan[most + s] = (int32_t)min(at, most);
+            for (int64_t i = at; i < min(at + n, most); i++) plan[i] = (int32_t)s;
+        }
+        __syncthreads();
+    }
+    for (int64_t i = before + threadIdx.x; i < most; i += kPlanThreads) plan[i] = -1;
+}
+
+// From what units add to a state, the states in front of them (or behind them, from the last to the first): x' = decay x + added.  A thread has an
+// element of the state and reads eight units ahead.
+__global__ __launch_bounds__(kScanThreads) void attention_scan_kernel(AttentionCall c, float *__restrict__ states, const float *__restrict__ from, float *__restrict__ to,
+                                                                      int64_t unit_rows, bool back) {
+    constexpr int kAhead = 8;
+    const int64_t s = blockIdx.x / c.m.heads, size = (int64_t)c.m.key_size * c.m.value_size, i = (int64_t)blockIdx.y * kScanThreads + threadIdx.x;
+    const int head = (int)(blockIdx.x % c.m.heads);
+    if (i >= size) return;
+    int64_t first;
+    const int64_t count = units_of(c, s, unit_rows, first);
+    float x = from ? from[(s * c.m.heads + head) * size + i] : 0.0f;
+    for (int64_t n = 0; n < count; n += kAhead) {
+        float added[kAhead], decay[kAhead];
+#pragma unroll
+        for (int j = 0; j < kAhead; j++) {
+            const int64_t unit = (first + (back ? count - 1 - n - j : n + j)) * c.m.heads + head;
+            added[j] = n + j < count ? states[unit * size + i] : 0.0f;
+            decay[j] = n + j < count ? c.decays[unit] : 0.0f;
+        }
+#pragma unroll
+        for (int j = 0; j < kAhead; j++) {
+            const int64_t unit = (first + (back ? count - 1 - n - j : n + j)) * c.m.heads + head;
+            if (n + j < count) {
+                states[unit * size + i] = x;
+                x = fmaf(decay[j], x, added[j]);
+            }
+        }
+    }
+    if (to) to[(s * c.m.heads + head) * size + i] = x;
+}
+
+// dlog a of a unit's rows: <S, D> in front of it, and what changes it from row to row.
+template <class S> __global__ __launch_bounds__(kScanThreads) void attention_gates_kernel(AttentionCall c, int64_t rows_of_chunk, const float *__restrict__ in_front) {
+    __shared__ double waves[kScanThreads / kWave];
+    const int64_t u = blockIdx.x / c.m.heads, size = (int64_t)c.m.key_size * c.m.value_size;
+    const int head = (int)(blockIdx.x % c.m.heads), lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
+    const Unit unit = rows_of_chunk == 32 ? unit_of<32>(c, u) : unit_of<64>(c, u);
+    if (!unit.there) {
+        if (c.m.fixed && threadIdx.x == 0) c.sums[u * c.m.heads + head] = 0.0;
+        return;
+    }
+    const auto over_waves = [&](double v, double &all) {  // -> the sum over waves before this one
+        __syncthreads();
+        if (lane == kWave - 1) waves[wave] = v;
+        __syncthreads();
+        double before = 0.0;
+        all = 0.0;
+        for (int w = 0; w < kScanThreads / kWave; w++) {
+            if (w < wave) before += waves[w];
+            all += waves[w];
+        }
+        return before;
+    };
+    double product = 0.0, all;
+    const float *gradient = unit.index > 0 ? c.grad_states + ((u - 1) * c.m.heads + head) * size : in_front ? in_front + (unit.sequence * c.m.heads + head) * size : nullptr;
+    if (gradient) {
+        const float *state = c.states + (u * c.m.heads + head) * size;
+        for (int64_t i = threadIdx.x; i < size; i += kScanThreads) product += (double)state[i] * (double)gradient[i];
+    }
+    over_waves(sum_lanes(product, kWave), all);
+    double log_a = all;  // of the first row
+    const int64_t each = (unit.count + kScanThreads - 1) / kScanThreads, first = min(unit.count, threadIdx.x * each), last = min(unit.count, first + each);
+    const int64_t at = head * c.m.rows + unit.first;
+    double sum = 0.0;
+    for (int64_t t = first; t < last; t++) sum += (double)c.changes[1][at + t] - (double)c.changes[0][at + t];
+    double upto = sum;
+#pragma unroll
+    for (int step = 1; step < kWave; step *= 2) {
+        const double other = __shfl_up(upto, step);
+        if (lane >= step) upto += other;
+    }
+    log_a += over_waves(upto, all) + upto - sum;
+    double total = 0.0;
+    for (int64_t t = first; t < last; t++) {
+        total += log_a;
+        const int64_t to = (unit.first + t) * c.m.heads + head;
+        if (!c.m.fixed) ((S *)c.grad_gates)[to] = (S)(float)(log_a * slope_of(c.m.gate_form, (double)(float)((const S *)c.gates)[to]));
+        log_a += (double)c.changes[1][at + t] - (double)c.changes[0][at + t];
+    }
+    if (c.m.fixed) {
+        over_waves(sum_lanes(total, kWave), all);
+        if (threadIdx.x == 0) c.sums[u * c.m.heads + head] = all;
+    }
+}
+#endif  // TG_DOUBLE_PRECISION
+
 template <class S>
 __global__ void attention_fixed_gates_kernel(Attention m, const S *__restrict__ gates, const double *__restrict__ sums, int64_t parts, S *__restrict__ grad_gates) {
     const int h = blockIdx.x;
@@ -143,12 +277,12 @@ __global__ void attention_fixed_gates_kernel(Attention m, const S *__restrict__ 
 }
 
 // Key heads' gradients, the sums of their value heads'.
-template <class T>
-__global__ void attention_shared_kernel(Attention m, const double *__restrict__ parts, T *__restrict__ out) {
+template <class T, class P>
+__global__ void attention_shared_kernel(Attention m, const P *__restrict__ parts, T *__restrict__ out) {
     const int64_t id = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
     if (id >= m.rows * m.key_heads * m.key_size) return;
     const int64_t i = id % m.key_size, head = id / m.key_size;  // row and key head
-    double sum = 0.0;
+    P sum = 0;
     for (int n = 0; n < m.shared; n++) sum += parts[(head * m.shared + n) * m.key_size + i];
     out[id] = (T)(real)sum;
 }
@@ -193,6 +327,21 @@ int attention_shape(const char *fn, const tg_attention &a, Attention &m) {
     return 0;
 }
 
+static unsigned blocks_for(int64_t n) { return (unsigned)std::min<int64_t>(ceil_div64(n, 256), 1 << 20); }
+
+template <class T> static void clear_outside(const tg_attention &a, const Attention &m, T *out, int64_t width) {
+    if (!m.packed || !m.rows || !out) return;
+    TG_LAUNCH_AS("attention_outside", (attention_outside_kernel<T>), dim3(std::min(blocks_for(m.rows * width), 4096u)), dim3(256), 0, (hipStream_t)a.stream, m,
+                 a.offsets, width, out);
+}
+template <class T, class S> static void clear_gradients(const tg_attention &a, const Attention &m) {
+    clear_outside(a, m, (T *)a.grad_queries, (int64_t)m.key_heads * m.key_size);
+    clear_outside(a, m, (T *)a.grad_keys, (int64_t)m.key_heads * m.key_size);
+    clear_outside(a, m, (T *)a.grad_values, (int64_t)m.heads * m.value_size);
+    if (!m.fixed) clear_outside(a, m, (S *)a.grad_gates, (int64_t)m.heads);
+}
+
+#ifdef TG_DOUBLE_PRECISION
 struct WalkRoom {
     int64_t dq, dk, dstate, sums, all;
 };
@@ -206,17 +355,12 @@ static WalkRoom walk_room(const Attention &m) {
     return r;
 }
 
-static unsigned blocks_for(int64_t n) { return (unsigned)std::min<int64_t>(ceil_div64(n, 256), 1 << 20); }
-
 template <class T, class S> static int walk_forward(const tg_attention &a, const Attention &m) {
     const hipStream_t stream = (hipStream_t)a.stream;
     TG_LAUNCH_AS("attention_walk", (attention_walk_kernel<T, S>), dim3((unsigned)(m.sequences * m.heads), (unsigned)ceil_div(m.value_size, kWalkThreads)),
                  dim3(kWalkThreads), 0, stream, m, (const T *)a.queries, (const T *)a.keys, (const T *)a.values, (const S *)a.gates, a.initial, a.offsets,
                  (T *)a.outputs, a.final);
-    if (m.packed && m.rows) {
-        const int64_t width = (int64_t)m.heads * m.value_size;
-        TG_LAUNCH_AS("attention_outside", (attention_outside_kernel<T>), dim3(blocks_for(m.rows * width)), dim3(256), 0, stream, m, a.offsets, width, (T *)a.outputs);
-    }
+    clear_outside(a, m, (T *)a.outputs, (int64_t)m.heads * m.value_size);
     return check_launch("tg_linear_attention_forward");
 }
 
@@ -254,21 +398,208 @@ template <class T, class S> static int walk_backward(const tg_attention &a, cons
     for (int which = 0; which < 2; which++) {
         T *out = (T *)(which ? a.grad_keys : a.grad_queries);
         if (out && n)
-            TG_LAUNCH_AS("attention_shared", (attention_shared_kernel<T>), dim3((unsigned)ceil_div64(n, 256)), dim3(256), 0, stream, m, which ? dk : dq, out);
+            TG_LAUNCH_AS("attention_shared", (attention_shared_kernel<T, double>), dim3((unsigned)ceil_div64(n, 256)), dim3(256), 0, stream, m, which ? dk : dq, out);
     }
-    if (m.packed && m.rows) {
-        const auto outside = [&](auto *out, int64_t width) {
-            using U = std::remove_pointer_t<decltype(out)>;
-            if (out)
-                TG_LAUNCH_AS("attention_outside", (attention_outside_kernel<U>), dim3(blocks_for(m.rows * width)), dim3(256), 0, stream, m, a.offsets, width, out);
-        };
-        outside((T *)a.grad_queries, (int64_t)m.key_heads * m.key_size);
-        outside((T *)a.grad_keys, (int64_t)m.key_heads * m.key_size);
-        outside((T *)a.grad_values, (int64_t)m.heads * m.value_size);
-        if (!m.fixed) outside((S *)a.grad_gates, (int64_t)m.heads);
-    }
+    clear_gradients<T, S>(a, m);
     return check_launch("tg_linear_attention_backward");
 }
+
+static int64_t room_for_walk(const Attention &m) { return walk_room(m).all; }
+
+static int sizes_of(const char *, const tg_attention &, const Attention &m, int64_t out[4]) {
+    out[0] = out[1] = out[2] = 0;
+    out[3] = room_for_walk(m);
+    return 0;
+}
+static int forward(const tg_attention &a, const Attention &m) { return walk_forward<real, real>(a, m); }
+static int backward(const tg_attention &a, const Attention &m) { return walk_backward<real, real>(a, m); }
+
+#else
+
+constexpr int64_t kWanted = 512;      // workgroups: two for each of 256 compute units
+constexpr int64_t kMostChunks = 16;   // of a unit: 1024 rows, beside whose 16 chunks a state that is written and read is little
+constexpr int64_t kMostUnits = 1024;  // of a sequence, which are gone through one after another
+constexpr int64_t kGridThreads = (int64_t)1 << 32;  // a grid has fewer
+
+// How the rows of a call are split, the same forward and backward.
+struct Split {
+    int64_t rows_of_chunk, chunks, units, most_units, size;
+    bool through;
+};
+static int split_of(const char *fn, const tg_attention &a, const Attention &m, Split &s) {
+    s.rows_of_chunk = a.type == TG_TYPE_BF16 ? 64 : 32;
+    s.size = std::max(m.key_size, m.value_size) <= 32 ? 32 : std::max(m.key_size, m.value_size) <= 64 ? 64 : 128;
+    const int64_t of_one = ceil_div64(m.length, s.rows_of_chunk), all = m.packed ? of_one + m.sequences : of_one * m.sequences;
+    // as few chunks to a unit as make the device full: a state is written and read for each
+    s.chunks = std::max<int64_t>(1, std::min(kMostChunks, all * m.heads / kWanted));
+    s.chunks = std::max(s.chunks, ceil_div64(of_one, kMostUnits));
+    s.units = ceil_div64(m.length, s.rows_of_chunk * s.chunks);
+    s.most_units = m.packed ? m.length / (s.rows_of_chunk * s.chunks) + m.sequences : s.units * m.sequences;
+    // sequences and heads enough: the forward pass goes through each from its first row to its last, and reads keys and values once
+    s.through = s.units <= 1 || (!m.packed && m.sequences * m.heads >= kWanted);
+    if (s.most_units * m.heads >= kGridThreads / (4 * s.size) || m.sequences * m.heads >= kGridThreads / (4 * s.size) || s.most_units > 0x7fffffff) {
+        set_error("%s: %lld rows, %lld sequences of %d heads are too many", fn, (long long)m.rows, (long long)m.sequences, m.heads);
+        return TG_E_ARG;
+    }
+    return 0;
+}
+
+// Bytes from the beginning of what the forward call leaves, or of a workspace.
+struct Room {
+    int64_t states, decays, plan, grad_states, changes, sums, grad_initial, shared_queries, shared_keys, all;
+};
+static Room room_of(const tg_attention &a, const Attention &m, const Split &s, bool states, bool backward) {
+    Room r = {};
+    int64_t at = 0;
+    const auto take = [&](bool wanted, int64_t bytes) {
+        const int64_t here = at;
+        if (wanted) at += ceil_div64(bytes, 16) * 16;
+        return here;
+    };
+    const int64_t size = (int64_t)m.key_size * m.value_size * 4, units = s.most_units * m.heads;
+    r.states = take(states, units * size);
+    r.plan = take(states && m.packed, (s.most_units + m.sequences) * 4);
+    r.decays = take(backward || !states, units * 4);
+    r.grad_states = take(backward, units * size);
+    r.changes = take(backward, 2 * m.rows * m.heads * 4);
+    r.sums = take(backward && m.fixed, units * 8);
+    r.grad_initial = take(backward && a.initial, m.sequences * m.heads * size);
+    r.shared_queries = take(backward && m.shared > 1, m.rows * m.heads * m.key_size * 4);
+    r.shared_keys = take(backward && m.shared > 1, m.rows * m.heads * m.key_size * 4);
+    r.all = at;
+    return r;
+}
+
+static int sizes_of(const char *fn, const tg_attention &a, const Attention &m, int64_t out[4]) {
+    Split s;
+    const int code = split_of(fn, a, m, s);
+    if (code) return code;
+    const int64_t kept = room_of(a, m, s, true, false).all, decays = room_of(a, m, s, false, false).all;
+    out[0] = kept;
+    out[1] = s.through ? 0 : kept + decays;
+    out[2] = s.through ? 0 : decays;
+    tg_attention with = a;
+    static const real some = 0;
+    with.initial = &some;  // whether there is one need not be known yet
+    out[3] = room_of(with, m, s, false, true).all;
+    return 0;
+}
+
+static bool in_vectors(const tg_attention &a, const Attention &m) {
+    const int64_t bytes = type_bytes(a.type);
+    if (m.key_size % 8 != 0 || m.value_size % 8 != 0) return false;
+    for (const void *p : {a.queries, a.keys, a.values, (const void *)a.outputs, a.grad_outputs, (const void *)a.grad_queries, (const void *)a.grad_keys, (const void *)a.grad_values})
+        if ((uintptr_t)p % 16 != 0) return false;
+    const auto dense = [&](const Strides &t, int heads) {
+        return (m.packed || m.sequences == 1 || t.sequence * bytes % 16 == 0) && (m.length == 1 || t.row * bytes % 16 == 0) && (heads == 1 || t.head * bytes % 16 == 0);
+    };
+    return dense(m.q, m.key_heads) && dense(m.k, m.key_heads) && dense(m.v, m.heads) && (!a.grad_outputs || dense(m.g, m.heads));
+}
+
+static AttentionCall call_of(const tg_attention &a, const Attention &m, const Split &s) {
+    AttentionCall c = {};
+    c.m = m;
+    c.queries = a.queries;
+    c.keys = a.keys;
+    c.values = a.values;
+    c.gates = a.gates;
+    c.initial = a.initial;
+    c.offsets = a.offsets;
+    c.outputs = a.outputs;
+    c.final = a.final;
+    c.most_units = s.most_units;
+    c.units = s.units;
+    c.chunks = (int)s.chunks;
+    c.wide_gates = a.gate_type == TG_TYPE_F32;
+    c.vector = in_vectors(a, m);
+    c.through = s.through;
+    c.grad_outputs = a.grad_outputs;
+    c.grad_final = a.grad_final;
+    c.grad_values = a.grad_values;
+    c.grad_gates = a.grad_gates;
+    return c;
+}
+
+static void scan(const AttentionCall &c, const Split &s, float *states, const float *from, float *to, bool back, hipStream_t stream) {
+    const int64_t size = (int64_t)c.m.key_size * c.m.value_size;
+    TG_LAUNCH_AS("attention_scan", attention_scan_kernel, dim3((unsigned)(c.m.sequences * c.m.heads), (unsigned)ceil_div64(size, kScanThreads)), dim3(kScanThreads), 0, stream,
+                 c, states, from, to, s.rows_of_chunk * s.chunks, back);
+}
+
+static int forward(const tg_attention &a, const Attention &m) {
+    const hipStream_t stream = (hipStream_t)a.stream;
+    Split s;
+    int code = split_of("tg_linear_attention_forward", a, m, s);
+    if (code) return code;
+    AttentionCall c = call_of(a, m, s);
+    const bool kept = a.kept != nullptr;
+    if (kept || !s.through) {
+        const Room room = room_of(a, m, s, true, false);
+        char *p = (char *)(kept ? a.kept : a.workspace);
+        c.states = (float *)(p + room.states);
+        c.plan = (const int32_t *)(p + room.plan);
+        c.decays = (float *)((char *)a.workspace + (kept ? 0 : room.all));
+        if (m.packed)
+            TG_LAUNCH_AS("attention_plan", attention_plan_kernel, dim3(1), dim3(kPlanThreads), 0, stream, m, a.offsets, s.rows_of_chunk * s.chunks, s.most_units,
+                         (int32_t *)(p + room.plan));
+    }
+    if (m.rows == 0 || s.through) {
+        c.through = true;
+    } else {
+        if ((code = launch_attention_forward(a, c, (int)s.size, true, stream))) return code;
+        scan(c, s, c.states, a.initial, a.final, false, stream);
+    }
+    if ((code = launch_attention_forward(a, c, (int)s.size, false, stream))) return code;
+    return by_types(a.type, a.gate_type, [&](auto t, auto) {
+        clear_outside(a, m, (decltype(t) *)a.outputs, (int64_t)m.heads * m.value_size);
+        return check_launch("tg_linear_attention_forward");
+    });
+}
+
+template <class T, class S> static int backward(const tg_attention &a, const Attention &m) {
+    const hipStream_t stream = (hipStream_t)a.stream;
+    Split s;
+    int code = split_of("tg_linear_attention_backward", a, m, s);
+    if (code) return code;
+    AttentionCall c = call_of(a, m, s);
+    const Room kept = room_of(a, m, s, true, false), room = room_of(a, m, s, false, true);
+    char *w = (char *)a.workspace;
+    c.states = (float *)((char *)a.kept + kept.states);
+    c.plan = (const int32_t *)((char *)a.kept + kept.plan);
+    c.decays = (float *)(w + room.decays);
+    c.grad_states = (float *)(w + room.grad_states);
+    c.changes[0] = (float *)(w + room.changes);
+    c.changes[1] = c.changes[0] + m.rows * m.heads;
+    c.sums = (double *)(w + room.sums);
+    c.grad_queries = m.shared > 1 && a.grad_queries ? w + room.shared_queries : a.grad_queries;
+    c.grad_keys = m.shared > 1 && a.grad_keys ? w + room.shared_keys : a.grad_keys;
+    float *in_front = a.initial && a.grad_gates ? (float *)(w + room.grad_initial) : nullptr;
+    if (a.grad_initial) in_front = a.grad_initial;
+    if (m.rows && (code = launch_attention_backward(a, c, (int)s.size, 0, stream))) return code;
+    scan(c, s, c.grad_states, a.grad_final, in_front, true, stream);
+    if (m.rows && (a.grad_keys || a.grad_values || a.grad_gates) && (code = launch_attention_backward(a, c, (int)s.size, 1, stream))) return code;
+    if (a.grad_gates) {
+        if (m.rows)
+            TG_LAUNCH_AS("attention_gates", (attention_gates_kernel<S>), dim3((unsigned)(s.most_units * m.heads)), dim3(kScanThreads), 0, stream, c, s.rows_of_chunk,
+                         a.initial ? in_front : nullptr);
+        if (m.fixed)
+            TG_LAUNCH_AS("attention_fixed_gates", (attention_fixed_gates_kernel<S>), dim3((unsigned)m.heads), dim3(kWalkThreads), 0, stream, m, (const S *)a.gates, c.sums,
+                         m.rows ? s.most_units : 0, (S *)a.grad_gates);
+    }
+    const int64_t n = m.rows * m.key_heads * m.key_size;
+    for (int which = 0; which < 2 && m.shared > 1; which++) {
+        T *out = (T *)(which ? a.grad_keys : a.grad_queries);
+        if (out && n)
+            TG_LAUNCH_AS("attention_shared", (attention_shared_kernel<T, float>), dim3((unsigned)ceil_div64(n, 256)), dim3(256), 0, stream, m,
+                         (const float *)(which ? c.grad_keys : c.grad_queries), out);
+    }
+    clear_gradients<T, S>(a, m);
+    return check_launch("tg_linear_attention_backward");
+}
+static int backward(const tg_attention &a, const Attention &m) {
+    return by_types(a.type, a.gate_type, [&](auto t, auto s) { return backward<decltype(t), decltype(s)>(a, m); });
+}
+#endif  // TG_DOUBLE_PRECISION
 
 // ---- a single step ----------------------------------------------------------------------
 
@@ -351,36 +682,35 @@ static int check_pointers(const char *fn, std::initializer_list<const void *> ne
 }
 
 extern "C" int tg_linear_attention_sizes(const tg_attention *a, int64_t out[4]) {
-    if (!a || !out) return check_pointers("tg_linear_attention_sizes", {a, out});
+    const char *fn = "tg_linear_attention_sizes";
+    if (!a || !out) return check_pointers(fn, {a, out});
     Attention m;
-    const int code = attention_shape("tg_linear_attention_sizes", *a, m);
-    if (code) return code;
-    out[0] = out[1] = out[2] = 0;
-    out[3] = walk_room(m).all;
-    return 0;
+    const int code = attention_shape(fn, *a, m);
+    return code ? code : sizes_of(fn, *a, m, out);
 }
 
-static int attention_call(const char *fn, const tg_attention *a, bool backward) {
+static int attention_call(const char *fn, const tg_attention *a, bool backward_pass) {
     if (!a) return check_pointers(fn, {a});
     Attention m;
     int code = attention_shape(fn, *a, m);
     if (code) return code;
     int64_t sizes[4];
-    code = tg_linear_attention_sizes(a, sizes);
-    if (code) return code;
-    if (m.sequences == 0) return 0;
+    if ((code = sizes_of(fn, *a, m, sizes))) return code;
     if (m.rows && (code = check_pointers(fn, {a->queries, a->keys, a->values, a->gates}))) return code;
-    if (!backward && (code = check_pointers(fn, {a->final}))) return code;
-    if (!backward && m.rows && (code = check_pointers(fn, {a->outputs}))) return code;
-    if (a->workspace_bytes < sizes[backward ? 3 : 1] || (sizes[backward ? 3 : 1] && !a->workspace)) {
-        set_error("%s: workspace of %lld bytes, %lld needed", fn, (long long)a->workspace_bytes, (long long)sizes[backward ? 3 : 1]);
+    if (!backward_pass && m.sequences && (code = check_pointers(fn, {a->final}))) return code;
+    if (!backward_pass && m.rows && (code = check_pointers(fn, {a->outputs}))) return code;
+    if (backward_pass && sizes[0] && (code = check_pointers(fn, {a->kept}))) return code;
+    if (a->kept && a->kept_bytes < sizes[0]) {
+        set_error("%s: kept has %lld bytes, %lld needed", fn, (long long)a->kept_bytes, (long long)sizes[0]);
         return TG_E_WORKSPACE;
     }
-    return by_types(a->type, a->gate_type, [&](auto t, auto s) {
-        using T = decltype(t);
-        using S = decltype(s);
-        return backward ? walk_backward<T, S>(*a, m) : walk_forward<T, S>(*a, m);
-    });
+    const int64_t room = sizes[backward_pass ? 3 : a->kept ? 2 : 1];
+    if (a->workspace_bytes < room || (room && !a->workspace)) {
+        set_error("%s: workspace of %lld bytes, %lld needed", fn, (long long)a->workspace_bytes, (long long)room);
+        return TG_E_WORKSPACE;
+    }
+    if (m.sequences == 0) return 0;
+    return backward_pass ? backward(*a, m) : forward(*a, m);
 }
 
 extern "C" int tg_linear_attention_forward(const tg_attention *a) { return attention_call("tg_linear_attention_forward", a, false); }

@@ -1,0 +1,360 @@
+// tg_attention_chunk.hpp -- linear attention by chunks of rows on the matrix units: what its kernels share.
+//
+// With L_t the sum of log2 a from a chunk's first row to row t, S_0 the state in front of the chunk and D_C the gradient of the state behind it,
+//     o_s  = scale [ sum_{r <= s} 2^(L_s - L_r) (q_s.k_r) v_r + 2^L_s S_0^T q_s ],      S_C = 2^L_C S_0 + sum_r 2^(L_C - L_r) k_r v_r^T,
+//     dq_s = scale [ sum_{r <= s} 2^(L_s - L_r) (do_s.v_r) k_r + 2^L_s S_0 do_s ],
+//     dk_r = scale sum_{s >= r} 2^(L_s - L_r) (do_s.v_r) q_s + 2^(L_C - L_r) D_C v_r,   D_0 = 2^L_C D_C + scale sum_s 2^L_s q_s do_s^T,
+//     dv_r = scale sum_{s >= r} 2^(L_s - L_r) (q_s.k_r) do_s + 2^(L_C - L_r) D_C^T k_r:
+// products of matrices of at most 64 rows and TG_ATTENTION_SIZE columns.  A workgroup has a head and a run of chunks (a unit), one after another; the states stay in
+// the accumulators of its waves, each of which has sixteen columns of them.
+//
+// Numbers.  Products are of bfloat16 numbers and summed in float32.  What is not one is a sum of "parts" in bfloat16, each the rounded rest of
+// those before: inputs in float16 are two parts and in float32 three, exactly; so are states, and inputs that carry a decay, wherever what they
+// go into is float32 in the end (states, their gradients, gates' gradients: two parts leave an error of 2e-6, three one of 1e-8, below that of
+// the sums).  States that go into an output of 16 bits have two parts, and the matrix of pairs inside a chunk is rounded as the inputs are, once.
+#pragma once
+#include "tg_attention.hpp"
+
+namespace tg {
+
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
+typedef short short4_t __attribute__((ext_vector_type(4)));
+typedef float floatx4 __attribute__((ext_vector_type(4)));
+
+// Parts of an input and of a state that goes into an output of its type; rows of a chunk: as many as leave room in LDS for the parts.
+template <class T> struct Parts;
+template <> struct Parts<bf16_t> { static constexpr int kInput = 1, kState = 2, kRows = 64; };
+template <> struct Parts<half_t> { static constexpr int kInput = 2, kState = 2, kRows = 32; };
+template <> struct Parts<float> { static constexpr int kInput = 3, kState = 3, kRows = 32; };
+constexpr int kWhole = 3;  // parts of a number in float32
+
+// Eight numbers of a lane for v_mfma_f32_16x16x32_bf16: row (of A) or column (of B) lane % 16, and eight of the 32 that are summed over; which,
+// both operands have to agree in.  "Straight": 8 (lane / 16) on.  "Chained": 4 (lane / 16) on, and sixteen further: as two accumulators one above the
+// other hold them (rows 4 (lane / 16) on of column lane % 16), so that a state goes from one product into the next without leaving its lane.
+template <int N> struct Operand { bf16x8 part[N]; };
+
+template <int NA, int NB> __device__ __forceinline__ floatx4 product(const Operand<NA> &a, const Operand<NB> &b, floatx4 sum) {
+    constexpr int kTerms = NA == 2 && NB == 2 ? 3 : NA > NB ? NA : NB;  // parts beyond are below the last ones' rounding
+#pragma unroll
+    for (int i = NA - 1; i >= 0; i--)
+#pragma unroll
+        for (int j = NB - 1; j >= 0; j--)
+            if (i + j < kTerms) sum = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a.part[i], b.part[j], sum, 0, 0, 0);
+    return sum;
+}
+
+template <int N> __device__ __forceinline__ Operand<N> parts_of(const float *x) {
+    Operand<N> o;
+    float rest[8];
+#pragma unroll
+    for (int j = 0; j < 8; j++) rest[j] = x[j];
+#pragma unroll
+    for (int n = 0; n < N; n++)
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+            o.part[n][j] = (__bf16)rest[j];
+            if (n + 1 < N) rest[j] -= (float)o.part[n][j];
+        }
+    return o;
+}
+template <int N> __device__ __forceinline__ Operand<N> operand_of(floatx4 above, floatx4 below) {
+    const float x[8] = {above[0], above[1], above[2], above[3], below[0], below[1], below[2], below[3]};
+    return parts_of<N>(x);
+}
+
+// A matrix of Rows x Columns in LDS, N parts.  Rows are 16 bytes longer than their numbers, so that sixteen rows begin in different banks.
+template <int N, int Rows, int Columns> struct Tile {
+    static constexpr int kStride = Columns + 8, kPart = Rows * kStride, kBytes = N * kPart * 2;
+    __bf16 *at;
+
+    __device__ __forceinline__ Operand<N> straight(int row, int column) const {
+        const int lane = threadIdx.x % kWave;
+        const __bf16 *p = at + (row + lane % 16) * kStride + column + 8 * (lane / 16);
+        Operand<N> o;
+#pragma unroll
+        for (int n = 0; n < N; n++) o.part[n] = *(const bf16x8 *)(p + n * kPart);
+        return o;
+    }
+    __device__ __forceinline__ Operand<N> chained(int row, int column) const {
+        const int lane = threadIdx.x % kWave;
+        const __bf16 *p = at + (row + lane % 16) * kStride + column + 4 * (lane / 16);
+        Operand<N> o;
+#pragma unroll
+        for (int n = 0; n < N; n++) {
+            const bf16x4 a = *(const bf16x4 *)(p + n * kPart), b = *(const bf16x4 *)(p + n * kPart + 16);
+            o.part[n] = __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
+        }
+        return o;
+    }
+    // The transposed matrix's: row or column `column` + lane % 16, chained rows from `row`.  LDS hands out four rows of sixteen columns transposed to
+    // sixteen lanes, of which each points at four neighbours of a row.
+    __device__ __forceinline__ Operand<N> transposed(int row, int column) const {
+        const int lane = threadIdx.x % kWave;
+        const __bf16 *p = at + (row + 4 * (lane / 16) + lane % 16 / 4) * kStride + column + 4 * (lane % 4);
+        Operand<N> o;
+#pragma unroll
+        for (int n = 0; n < N; n++) {
+            const bf16x4 a = turned(p + n * kPart), b = turned(p + n * kPart + 16 * kStride);
+            o.part[n] = __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
+        }
+        return o;
+    }
+    static __device__ __forceinline__ bf16x4 turned(const __bf16 *p) {
+        return __builtin_bit_cast(bf16x4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) short4_t *)p));
+    }
+    // Four neighbours of a row, as numbers.
+    __device__ __forceinline__ floatx4 numbers(int row, int column) const {
+        floatx4 x = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int n = N - 1; n >= 0; n--) {
+            const bf16x4 v = *(const bf16x4 *)(at + n * kPart + row * kStride + column);
+#pragma unroll
+            for (int j = 0; j < 4; j++) x[j] += (float)v[j];
+        }
+        return x;
+    }
+    // An accumulator's four rows (columns here) of its column (a row here): the product's transpose.
+    __device__ __forceinline__ void put(int row, int column, floatx4 x) const {
+        const int lane = threadIdx.x % kWave;
+        __bf16 *p = at + (row + lane % 16) * kStride + column + 4 * (lane / 16);
+#pragma unroll
+        for (int n = 0; n < N; n++) {
+            bf16x4 v;
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                v[j] = (__bf16)x[j];
+                x[j] -= (float)v[j];
+            }
+            *(bf16x4 *)(p + n * kPart) = v;
+        }
+    }
+};
+
+// A transposed input's operand with a weight for each row.
+template <int M, int N> __device__ __forceinline__ Operand<M> weighted(const Operand<N> &o, const float *weights, int row) {
+    const int group = threadIdx.x % kWave / 16;
+    const floatx4 a = *(const floatx4 *)(weights + row + 4 * group), b = *(const floatx4 *)(weights + row + 16 + 4 * group);
+    float x[8];
+#pragma unroll
+    for (int j = 0; j < 8; j++) {
+        x[j] = (float)o.part[N - 1][j];
+#pragma unroll
+        for (int n = N - 2; n >= 0; n--) x[j] += (float)o.part[n][j];
+        x[j] *= j < 4 ? a[j] : b[j - 4];
+    }
+    return parts_of<M>(x);
+}
+
+// ---- reading a chunk ----------------------------------------------------------------------
+
+// A thread's part of a chunk of Rows x D numbers, on its way to LDS: groups of eight neighbours.
+template <class T, int Rows, int D> struct Incoming {
+    static constexpr int kThreads = 4 * D, kGroups = Rows * D / 8 / kThreads;
+    T x[kGroups][8];
+
+    // `count` rows from p on, `size` numbers each; what lies beyond is zero.  vector: groups are whole and aligned.
+    __device__ __forceinline__ void load(const T *p, int64_t row_stride, int64_t count, int size, bool vector) {
+#pragma unroll
+        for (int n = 0; n < kGroups; n++) {
+            const int group = (int)threadIdx.x + n * kThreads, row = group / (D / 8), column = group % (D / 8) * 8;
+            const T *from = p + row * row_stride + column;
+#pragma unroll
+            for (int j = 0; j < 8; j++) x[n][j] = (T)0.0f;
+            if (row >= count || column >= size) continue;
+            if (vector) {
+                constexpr int kWidest = 16 / sizeof(T);
+#pragma unroll
+                for (int j = 0; j < 8; j += kWidest) {
+                    const Pack<T, kWidest> v = load_pack<kWidest>(from + j);
+#pragma unroll
+                    for (int i = 0; i < kWidest; i++) x[n][j + i] = v.v[i];
+                }
+            } else {
+#pragma unroll
+                for (int j = 0; j < 8; j++)
+                    if (column + j < size) x[n][j] = from[j];
+            }
+        }
+    }
+    template <int N> __device__ __forceinline__ void store(const Tile<N, Rows, D> &tile) const {
+#pragma unroll
+        for (int n = 0; n < kGroups; n++) {
+            const int group = (int)threadIdx.x + n * kThreads, row = group / (D / 8), column = group % (D / 8) * 8;
+            float v[8];
+#pragma unroll
+            for (int j = 0; j < 8; j++) v[j] = (float)x[n][j];
+            const Operand<N> o = parts_of<N>(v);
+#pragma unroll
+            for (int i = 0; i < N; i++) *(bf16x8 *)(tile.at + i * Tile<N, Rows, D>::kPart + row * Tile<N, Rows, D>::kStride + column) = o.part[i];
+        }
+    }
+};
+
+// Decays of a chunk.
+template <int Rows> struct alignas(16) Reach {
+    double reach[Rows];   // L
+    float row[Rows];      // scale 2^L
+    float column[Rows];   // 2^(L_C - L)
+    float start[Rows];    // scale 2^L from the unit's beginning
+    float whole;          // 2^L_C
+};
+
+struct AttentionCall {
+    Attention m;
+    const void *queries, *keys, *values, *gates;
+    const float *initial;
+    const int32_t *offsets;
+    const int32_t *plan;    // packed: sequence of each unit, or -1; behind `most_units` of them the first unit of each sequence
+    void *outputs;
+    float *final;
+    float *states;          // of each unit and head, in front of it
+    float *decays;          // of each unit and head
+    int64_t most_units;     // units there may be
+    int64_t units;          // of a sequence, where all are alike
+    int chunks;             // of a unit
+    bool wide_gates, vector;
+    bool through;           // a workgroup has a whole sequence
+    // the backward pass's
+    const void *grad_outputs;
+    const float *grad_final;
+    void *grad_queries, *grad_keys, *grad_values, *grad_gates;
+    float *grad_initial;
+    float *grad_states;     // of each unit and head: what the unit adds to the gradient in front of it, then the gradient behind it
+    float *changes[2];      // of each head and row: what dlog a changes by
+    double *sums;           // of each unit and head: dlog a of all rows
+};
+
+struct Unit {
+    int64_t sequence, index;  // index: in its sequence
+    int64_t first, count;     // rows
+    int64_t base;             // in the sequence
+    bool there;
+};
+template <int Rows> __device__ __forceinline__ Unit unit_of(const AttentionCall &c, int64_t u) {
+    Unit n;
+    if (c.m.packed) {
+        n.sequence = c.plan[u];
+        n.there = n.sequence >= 0;
+        if (!n.there) return n;
+        n.index = u - c.plan[c.most_units + n.sequence];
+    } else {
+        n.sequence = u / c.units;
+        n.index = u - n.sequence * c.units;
+        n.there = true;
+    }
+    const AttentionRows rows = rows_of(c.m, c.offsets, n.sequence);
+    n.base = n.index * c.chunks * Rows;
+    n.first = rows.first + n.base;
+    n.count = max((int64_t)0, min(rows.count - n.base, (int64_t)c.chunks * Rows));
+    return n;
+}
+
+template <class T> __device__ __forceinline__ float gate_at(const AttentionCall &c, int64_t row, int head) {
+    const int64_t at = c.m.fixed ? head : row * c.m.heads + head;
+    return c.wide_gates ? ((const float *)c.gates)[at] : (float)((const T *)c.gates)[at];
+}
+
+// One wave: the decays of `count` rows from row `first` on, where `before` is L from the unit's beginning, which moves on.
+template <class T, int Rows> __device__ __forceinline__ void reach_of(const AttentionCall &c, Reach<Rows> &out, int64_t first, int64_t count, int head, double &before) {
+    const int lane = threadIdx.x % kWave;
+    double sum = lane < count && lane < Rows ? log2_gate(c.m.gate_form, gate_at<T>(c, first + lane, head)) : 0.0;
+#pragma unroll
+    for (int step = 1; step < Rows; step *= 2) {
+        const double other = __shfl_up(sum, step);
+        if (lane >= step) sum += other;
+    }
+    const double whole = __shfl(sum, Rows - 1);
+    if (lane < Rows) {
+        out.reach[lane] = sum;
+        out.row[lane] = c.m.scale * exp2f((float)sum);
+        out.column[lane] = exp2f((float)(whole - sum));
+        out.start[lane] = c.m.scale * exp2f((float)(before + sum));
+        if (lane == 0) out.whole = exp2f((float)whole);
+    }
+    before += whole;
+}
+
+// scale 2^(L_s - L_r) of an accumulator whose columns are rows s (or r) of the chunk, zero where s < r, or, Strict, s <= r.
+template <bool ColumnsAreLater, int Rows> __device__ __forceinline__ floatx4 decays_of(const Reach<Rows> &reach, int row, int column, float scale) {
+    const int lane = threadIdx.x % kWave, x = column + lane % 16, y = row + 4 * (lane / 16);
+    const double here = reach.reach[x];
+    floatx4 d;
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+        const double other = reach.reach[y + j];
+        const float l = (float)(ColumnsAreLater ? here - other : other - here);
+        const bool in = ColumnsAreLater ? x >= y + j : x <= y + j;
+        d[j] = in ? scale * exp2f(l) : 0.0f;
+    }
+    return d;
+}
+
+// Four neighbours of an output's row.
+template <class T> __device__ __forceinline__ void put_row(T *p, int column, int size, bool vector, floatx4 x) {
+    if (vector) {
+        if (column < size) {
+            const float v[4] = {x[0], x[1], x[2], x[3]};
+            store_pack<4>(p + column, v);
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < 4; j++)
+            if (column + j < size) p[column + j] = (T)x[j];
+    }
+}
+
+// The state in accumulators: rows of keys and columns of values (Turned: the other way round), of a wave the sixteen columns from `column` on.
+template <int D> struct State {
+    floatx4 x[D / 16];
+
+    template <bool Turned> static __device__ __forceinline__ int64_t place(int row, int column, int key_size, int value_size) {
+        const int key = Turned ? column : row, value = Turned ? row : column;
+        return key < key_size && value < value_size ? (int64_t)key * value_size + value : -1;
+    }
+    template <bool Turned> __device__ __forceinline__ void load(const float *from, int column, int key_size, int value_size) {
+        const int lane = threadIdx.x % kWave;
+#pragma unroll
+        for (int n = 0; n < D / 16; n++)
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                const int64_t at = place<Turned>(16 * n + 4 * (lane / 16) + j, column + lane % 16, key_size, value_size);
+                x[n][j] = from && at >= 0 ? from[at] : 0.0f;
+            }
+    }
+    template <bool Turned> __device__ __forceinline__ void store(float *to, int column, int key_size, int value_size) const {
+        const int lane = threadIdx.x % kWave;
+#pragma unroll
+        for (int n = 0; n < D / 16; n++)
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                const int64_t at = place<Turned>(16 * n + 4 * (lane / 16) + j, column + lane % 16, key_size, value_size);
+                if (at >= 0) to[at] = x[n][j];
+            }
+    }
+    __device__ __forceinline__ void times(float a) {
+#pragma unroll
+        for (int n = 0; n < D / 16; n++) x[n] *= a;
+    }
+    // Adds its transpose times the rows' columns to `sums`, one of sixteen rows of the tile each.
+    template <int M, int N, int Rows> __device__ __forceinline__ void read_by(const Tile<N, Rows, D> &tile, floatx4 *sums) const {
+#pragma unroll
+        for (int i = 0; i < D / 32; i++) {
+            const Operand<M> mine = operand_of<M>(x[2 * i], x[2 * i + 1]);
+#pragma unroll
+            for (int r = 0; r < Rows / 16; r++) sums[r] = product(mine, tile.chained(16 * r, 32 * i), sums[r]);
+        }
+    }
+    // += the transposed tile's rows times the operands of this wave's columns
+    template <int N, int M, int Rows> __device__ __forceinline__ void add(const Tile<N, Rows, D> &tile, const Operand<M> *columns) {
+#pragma unroll
+        for (int n = 0; n < D / 16; n++)
+#pragma unroll
+            for (int k = 0; k < Rows / 32; k++) x[n] = product(tile.transposed(32 * k, 16 * n), columns[k], x[n]);
+    }
+};
+
+int launch_attention_forward(const tg_attention &a, const AttentionCall &c, int size, bool states_only, hipStream_t stream);
+int launch_attention_backward(const tg_attention &a, const AttentionCall &c, int size, int which, hipStream_t stream);
+
+}  // namespace tg

@@ -1,0 +1,167 @@
+// tg_attention_forward.hip -- linear attention by chunks, forward: what units of chunks add to the state, and the outputs.
+#ifndef TG_DOUBLE_PRECISION
+#include "tg_attention_chunk.hpp"
+
+namespace tg {
+
+// What a unit adds to the state, and its decay.  A chunk is on its way from memory while the one before is computed on.
+template <class T, int D> __global__ __launch_bounds__(4 * D) void attention_states_kernel(AttentionCall c) {
+    constexpr int R = Parts<T>::kRows, N = Parts<T>::kInput;
+    __shared__ __attribute__((aligned(16))) __bf16 lds[(Tile<N, R, D>::kBytes * 2) / 2];
+    __shared__ Reach<R> reaches[2];
+    const Tile<N, R, D> keys{lds}, values{lds + Tile<N, R, D>::kBytes / 2};
+    const int64_t u = blockIdx.x / c.m.heads;
+    const int head = (int)(blockIdx.x % c.m.heads), wave = threadIdx.x / kWave, column = 16 * wave;
+    const Unit unit = unit_of<R>(c, u);
+    if (!unit.there) return;
+    const AttentionRows rows = rows_of(c.m, c.offsets, unit.sequence);
+    const T *k = (const T *)c.keys + place_of(c.m, c.m.k, unit.sequence, rows.first, head / c.m.shared) + unit.base * c.m.k.row,
+            *v = (const T *)c.values + place_of(c.m, c.m.v, unit.sequence, rows.first, head) + unit.base * c.m.v.row;
+    State<D> state = {};
+    double before = 0.0;
+    Incoming<T, R, D> next_k, next_v;
+    next_k.load(k, c.m.k.row, unit.count, c.m.key_size, c.vector);
+    next_v.load(v, c.m.v.row, unit.count, c.m.value_size, c.vector);
+    if (wave == 0) reach_of<T>(c, reaches[0], unit.first, unit.count, head, before);
+    int turn = 0;
+    for (int64_t at = 0; at < unit.count; at += R, turn ^= 1) {
+        next_k.store(keys);
+        next_v.store(values);
+        __syncthreads();
+        if (at + R < unit.count) {
+            next_k.load(k + (at + R) * c.m.k.row, c.m.k.row, unit.count - at - R, c.m.key_size, c.vector);
+            next_v.load(v + (at + R) * c.m.v.row, c.m.v.row, unit.count - at - R, c.m.value_size, c.vector);
+            if (wave == 0) reach_of<T>(c, reaches[turn ^ 1], unit.first + at + R, unit.count - at - R, head, before);
+        }
+        Operand<kWhole> mine[R / 32];
+#pragma unroll
+        for (int n = 0; n < R / 32; n++) mine[n] = weighted<kWhole>(values.transposed(32 * n, column), reaches[turn].column, 32 * n);
+        state.times(reaches[turn].whole);
+        state.add(keys, mine);
+        __syncthreads();
+    }
+    state.template store<false>(c.states + (u * c.m.heads + head) * c.m.key_size * c.m.value_size, column, c.m.key_size, c.m.value_size);
+    if (threadIdx.x == 0) c.decays[u * c.m.heads + head] = exp2f((float)before);
+}
+
+template <class T, int D> __global__ __launch_bounds__(4 * D) void attention_outputs_kernel(AttentionCall c) {
+    constexpr int R = Parts<T>::kRows, N = Parts<T>::kInput, M = Parts<T>::kState, kTiles = R / 16, kWaves = D / 16;
+    using In = Tile<N, R, D>;
+    using Pairs = Tile<N, R, R>;
+    extern __shared__ __attribute__((aligned(16))) char lds[];
+    const In queries{(__bf16 *)lds}, keys{(__bf16 *)(lds + In::kBytes)}, values{(__bf16 *)(lds + 2 * In::kBytes)};
+    const Pairs pairs{(__bf16 *)(lds + 3 * In::kBytes)};
+    Reach<R> *reaches = (Reach<R> *)(lds + 3 * In::kBytes + Pairs::kBytes);
+    const int64_t which = blockIdx.x / c.m.heads;  // a unit, or a sequence
+    const int head = (int)(blockIdx.x % c.m.heads), lane = threadIdx.x % kWave, wave = threadIdx.x / kWave, column = 16 * wave;
+    const int64_t state_size = (int64_t)c.m.key_size * c.m.value_size;
+    Unit unit;
+    int64_t u = which;
+    if (c.through) {
+        const AttentionRows rows = rows_of(c.m, c.offsets, which);
+        unit = {which, 0, rows.first, rows.count, 0, true};
+        u = c.m.packed ? (c.states ? c.plan[c.most_units + which] : 0) : which * c.units;
+    } else {
+        unit = unit_of<R>(c, which);
+    }
+    if (!unit.there) return;
+    const AttentionRows rows = rows_of(c.m, c.offsets, unit.sequence);
+    const T *q = (const T *)c.queries + place_of(c.m, c.m.q, unit.sequence, rows.first, head / c.m.shared) + unit.base * c.m.q.row,
+            *k = (const T *)c.keys + place_of(c.m, c.m.k, unit.sequence, rows.first, head / c.m.shared) + unit.base * c.m.k.row,
+            *v = (const T *)c.values + place_of(c.m, c.m.v, unit.sequence, rows.first, head) + unit.base * c.m.v.row;
+    T *out = (T *)c.outputs + (unit.first * c.m.heads + head) * c.m.value_size;
+    const int64_t out_row = (int64_t)c.m.heads * c.m.value_size;
+    State<D> state;
+    const float *start = c.through ? (c.initial ? c.initial + (unit.sequence * c.m.heads + head) * state_size : nullptr)
+                                   : c.states + (u * c.m.heads + head) * state_size;
+    state.template load<false>(start, column, c.m.key_size, c.m.value_size);
+    double before = 0.0;
+    Incoming<T, R, D> next_q, next_k, next_v;
+    const auto load = [&](int64_t at) {
+        const int64_t left = unit.count - at;
+        next_q.load(q + at * c.m.q.row, c.m.q.row, left, c.m.key_size, c.vector);
+        next_k.load(k + at * c.m.k.row, c.m.k.row, left, c.m.key_size, c.vector);
+        next_v.load(v + at * c.m.v.row, c.m.v.row, left, c.m.value_size, c.vector);
+    };
+    load(0);
+    if (wave == 0) reach_of<T>(c, reaches[0], unit.first, unit.count, head, before);
+    int turn = 0, chunk = 0;
+    for (int64_t at = 0; at < unit.count; at += R, turn ^= 1) {
+        if (c.through && c.states && chunk == 0) {
+            if (u < c.most_units) state.template store<false>(c.states + (u * c.m.heads + head) * state_size, column, c.m.key_size, c.m.value_size);
+            u++;
+        }
+        chunk = chunk + 1 == c.chunks ? 0 : chunk + 1;
+        next_q.store(queries);
+        next_k.store(keys);
+        next_v.store(values);
+        __syncthreads();
+        if (at + R < unit.count) {
+            load(at + R);
+            if (wave == 0) reach_of<T>(c, reaches[turn ^ 1], unit.first + at + R, unit.count - at - R, head, before);
+        }
+        const Reach<R> &reach = reaches[turn];
+        // pairs: row s, column r
+#pragma unroll
+        for (int n = 0; n < (kTiles * kTiles + kWaves - 1) / kWaves; n++) {
+            const int tile = wave + n * kWaves, s = tile / kTiles, r = tile % kTiles;
+            if (tile >= kTiles * kTiles || r > (s | 1)) continue;
+            floatx4 p = {0.0f, 0.0f, 0.0f, 0.0f};
+            if (r <= s) {
+#pragma unroll
+                for (int i = 0; i < D; i += 32) p = product(keys.straight(16 * r, i), queries.straight(16 * s, i), p);
+                p *= decays_of<true>(reach, 16 * r, 16 * s, c.m.scale);
+            }
+            pairs.put(16 * s, 16 * r, p);
+        }
+        Operand<N> mine[R / 32];
+#pragma unroll
+        for (int n = 0; n < R / 32; n++) mine[n] = values.transposed(32 * n, column);
+        floatx4 read[kTiles] = {};
+        state.template read_by<M>(queries, read);
+        __syncthreads();
+#pragma unroll
+        for (int s = 0; s < kTiles; s++) {
+            floatx4 o = read[s];
+            o *= reach.row[16 * s + lane % 16];
+#pragma unroll
+            for (int n = 0; n < R / 32; n++)
+                if (2 * n <= s) o = product(mine[n], pairs.chained(16 * s, 32 * n), o);
+            const int64_t row = at + 16 * s + lane % 16;
+            if (row < unit.count) put_row(out + row * out_row, column + 4 * (lane / 16), c.m.value_size, c.vector, o);
+        }
+        Operand<kWhole> late[R / 32];
+#pragma unroll
+        for (int n = 0; n < R / 32; n++) late[n] = weighted<kWhole>(mine[n], reach.column, 32 * n);
+        state.times(reach.whole);
+        state.add(keys, late);
+        __syncthreads();
+    }
+    if (c.through) state.template store<false>(c.final + (unit.sequence * c.m.heads + head) * state_size, column, c.m.key_size, c.m.value_size);
+}
+
+template <class T, int D> static int launch(const tg_attention &a, const AttentionCall &c, bool states_only, hipStream_t stream) {
+    constexpr int R = Parts<T>::kRows, N = Parts<T>::kInput;
+    const dim3 grid((unsigned)((c.through ? c.m.sequences : c.most_units) * c.m.heads));
+    if (states_only) {
+        TG_LAUNCH_AS("attention_states", (attention_states_kernel<T, D>), grid, dim3(4 * D), 0, stream, c);
+        return 0;
+    }
+    constexpr size_t kBytes = 3 * Tile<N, R, D>::kBytes + Tile<N, R, R>::kBytes + 2 * sizeof(Reach<R>);
+    static size_t reserved[kMaxDevices];
+    const int code = reserve_lds("tg_linear_attention_forward", (const void *)attention_outputs_kernel<T, D>, kBytes, reserved);
+    if (code) return code;
+    TG_LAUNCH_AS("attention_outputs", (attention_outputs_kernel<T, D>), grid, dim3(4 * D), kBytes, stream, c);
+    return 0;
+}
+
+int launch_attention_forward(const tg_attention &a, const AttentionCall &c, int size, bool states_only, hipStream_t stream) {
+    const auto with = [&](auto t) {
+        using T = decltype(t);
+        return size <= 32 ? launch<T, 32>(a, c, states_only, stream) : size <= 64 ? launch<T, 64>(a, c, states_only, stream) : launch<T, 128>(a, c, states_only, stream);
+    };
+    return a.type == TG_TYPE_F32 ? with(float()) : a.type == TG_TYPE_F16 ? with(half_t()) : with(bf16_t());
+}
+
+}  // namespace tg
+#endif
