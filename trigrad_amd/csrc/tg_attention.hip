@@ -513,7 +513,9 @@ static AttentionCall call_of(const tg_attention &a, const Attention &m, const Sp
     c.wide_gates = a.gate_type == TG_TYPE_F32;
     c.vector = in_vectors(a, m);
     c.through = s.through;
-    c.grad_outputs = a.grad_outputs;
+    c.grad_outputs_there = a.grad_outputs != nullptr;
+    c.grad_outputs = a.grad_outputs ? a.grad_outputs : a.values;
+    if (!a.grad_outputs) c.m.g = m.v;
     c.grad_final = a.grad_final;
     c.grad_values = a.grad_values;
     c.grad_gates = a.grad_gates;
@@ -546,10 +548,10 @@ static int forward(const tg_attention &a, const Attention &m) {
     if (m.rows == 0 || s.through) {
         c.through = true;
     } else {
-        if ((code = launch_attention_forward(a, c, (int)s.size, true, stream))) return code;
+        if ((code = launch_attention_forward(a.type, c, (int)s.size, true, stream))) return code;
         scan(c, s, c.states, a.initial, a.final, false, stream);
     }
-    if ((code = launch_attention_forward(a, c, (int)s.size, false, stream))) return code;
+    if ((code = launch_attention_forward(a.type, c, (int)s.size, false, stream))) return code;
     return by_types(a.type, a.gate_type, [&](auto t, auto) {
         clear_outside(a, m, (decltype(t) *)a.outputs, (int64_t)m.heads * m.value_size);
         return check_launch("tg_linear_attention_forward");
@@ -575,9 +577,9 @@ template <class T, class S> static int backward(const tg_attention &a, const Att
     c.grad_keys = m.shared > 1 && a.grad_keys ? w + room.shared_keys : a.grad_keys;
     float *in_front = a.initial && a.grad_gates ? (float *)(w + room.grad_initial) : nullptr;
     if (a.grad_initial) in_front = a.grad_initial;
-    if (m.rows && (code = launch_attention_backward(a, c, (int)s.size, 0, stream))) return code;
+    if (m.rows && (code = launch_attention_backward(a.type, c, (int)s.size, false, stream))) return code;
     scan(c, s, c.grad_states, a.grad_final, in_front, true, stream);
-    if (m.rows && (a.grad_keys || a.grad_values || a.grad_gates) && (code = launch_attention_backward(a, c, (int)s.size, 1, stream))) return code;
+    if (m.rows && (a.grad_keys || a.grad_values || a.grad_gates) && (code = launch_attention_backward(a.type, c, (int)s.size, true, stream))) return code;
     if (a.grad_gates) {
         if (m.rows)
             TG_LAUNCH_AS("attention_gates", (attention_gates_kernel<S>), dim3((unsigned)(s.most_units * m.heads)), dim3(kScanThreads), 0, stream, c, s.rows_of_chunk,

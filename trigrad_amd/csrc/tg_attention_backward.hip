@@ -15,7 +15,7 @@ __device__ __forceinline__ float sum_groups(float v) {
     return v + __shfl_xor(v, 32);
 }
 
-template <class T, int D> __global__ __launch_bounds__(4 * D) void attention_grad_queries_kernel(AttentionCall c) {
+template <class T, int D, bool Vector> __global__ __launch_bounds__(4 * D) void attention_grad_queries_kernel(AttentionCall c) {
     constexpr int R = Parts<T>::kRows, N = Parts<T>::kInput, kTiles = R / 16, kWaves = D / 16;
     using In = Tile<N, R, D>;
     using Pairs = Tile<N, R, R>;
@@ -39,29 +39,30 @@ template <class T, int D> __global__ __launch_bounds__(4 * D) void attention_gra
     State<D> state, change = {};  // rows are values, columns keys
     state.template load<true>(c.states + (u * c.m.heads + head) * state_size, column, c.m.key_size, c.m.value_size);
     double before = 0.0;
-    Incoming<T, R, D> next_q, next_k, next_v, next_g;
+    Incoming<T, R, D, Vector> next_q, next_k, next_v, next_g;
     const auto load = [&](int64_t at) {
         const int64_t left = unit.count - at;
-        next_q.load(q + at * c.m.q.row, c.m.q.row, left, c.m.key_size, c.vector);
-        next_k.load(k + at * c.m.k.row, c.m.k.row, left, c.m.key_size, c.vector);
-        next_v.load(v + at * c.m.v.row, c.m.v.row, left, c.m.value_size, c.vector);
-        next_g.load(g + at * c.m.g.row, c.m.g.row, c.grad_outputs ? left : 0, c.m.value_size, c.vector);
+        next_q.load(q + at * c.m.q.row, c.m.q.row, left, c.m.key_size);
+        next_k.load(k + at * c.m.k.row, c.m.k.row, left, c.m.key_size);
+        next_v.load(v + at * c.m.v.row, c.m.v.row, left, c.m.value_size);
+        next_g.load(g + at * c.m.g.row, c.m.g.row, left, c.m.value_size);
     };
     load(0);
-    if (wave == 0) reach_of<T>(c, reaches[0], unit.first, unit.count, head, before);
+    float gate = 0.0f;  // of the next chunk's row, in the first wave
+    if (wave == 0) reach_of(c, reaches[0], gate_of_lane<T, R>(c, unit.first, unit.count, head), unit.count, before);
     int turn = 0;
     for (int64_t at = 0; at < unit.count; at += R, turn ^= 1) {
-        next_q.store(queries);
-        next_k.store(keys);
-        next_v.store(values);
-        next_g.store(grads);
+        next_q.store(queries, unit.count - at, c.m.key_size);
+        next_k.store(keys, unit.count - at, c.m.key_size);
+        next_v.store(values, unit.count - at, c.m.value_size);
+        next_g.store(grads, c.grad_outputs_there ? unit.count - at : 0, c.m.value_size);
         __syncthreads();
         if (at + R < unit.count) {
             load(at + R);
-            if (wave == 0) reach_of<T>(c, reaches[turn ^ 1], unit.first + at + R, unit.count - at - R, head, before);
+            if (wave == 0) gate = gate_of_lane<T, R>(c, unit.first + at + R, unit.count - at - R, head);
         }
         const Reach<R> &reach = reaches[turn];
-#pragma unroll
+#pragma unroll 1
         for (int n = 0; n < (kTiles * kTiles + kWaves - 1) / kWaves; n++) {
             const int tile = wave + n * kWaves, s = tile / kTiles, r = tile % kTiles;
             if (tile >= kTiles * kTiles) continue;
@@ -105,9 +106,9 @@ template <class T, int D> __global__ __launch_bounds__(4 * D) void attention_gra
             if (row < unit.count && c.grad_queries) {
                 const int64_t to = ((unit.first + row) * c.m.heads + head) * c.m.key_size;
                 if (c.m.shared == 1)
-                    put_row((T *)c.grad_queries + to, column + 4 * (lane / 16), c.m.key_size, c.vector, o);
+                    put_row((T *)c.grad_queries + to, column + 4 * (lane / 16), c.m.key_size, Vector, o);
                 else
-                    put_row((float *)c.grad_queries + to, column + 4 * (lane / 16), c.m.key_size, c.vector, o);
+                    put_row((float *)c.grad_queries + to, column + 4 * (lane / 16), c.m.key_size, Vector, o);
             }
         }
         Operand<kWhole> late[R / 32];
@@ -118,6 +119,7 @@ template <class T, int D> __global__ __launch_bounds__(4 * D) void attention_gra
 #pragma unroll
         for (int n = 0; n < R / 32; n++) late[n] = weighted<kWhole>(queries.transposed(32 * n, column), reach.start, 32 * n);
         change.add(grads, late);
+        if (wave == 0 && at + R < unit.count) reach_of(c, reaches[turn ^ 1], gate, unit.count - at - R, before);
         __syncthreads();
         if (threadIdx.x < R && at + threadIdx.x < unit.count) {
             float x = 0.0f;
@@ -129,10 +131,10 @@ template <class T, int D> __global__ __launch_bounds__(4 * D) void attention_gra
         }
     }
     change.template store<true>(c.grad_states + (u * c.m.heads + head) * state_size, column, c.m.key_size, c.m.value_size);
-    if (threadIdx.x == 0) c.decays[u * c.m.heads + head] = exp2f((float)before);
+    if (threadIdx.x == 0) c.decays[u * c.m.heads + head] = power_of_two((float)before);
 }
 
-template <class T, int D> __global__ __launch_bounds__(4 * D) void attention_grad_keys_kernel(AttentionCall c) {
+template <class T, int D, bool Vector> __global__ __launch_bounds__(4 * D) void attention_grad_keys_kernel(AttentionCall c) {
     constexpr int R = Parts<T>::kRows, N = Parts<T>::kInput, M = Parts<T>::kState, kTiles = R / 16, kWaves = D / 16;
     using In = Tile<N, R, D>;
     using Pairs = Tile<N, R, R>;
@@ -156,30 +158,31 @@ template <class T, int D> __global__ __launch_bounds__(4 * D) void attention_gra
     state.template load<false>(behind, column, c.m.key_size, c.m.value_size);
     turned.template load<true>(behind, column, c.m.key_size, c.m.value_size);
     double before = 0.0;
-    Incoming<T, R, D> next_q, next_k, next_v, next_g;
+    Incoming<T, R, D, Vector> next_q, next_k, next_v, next_g;
     const auto load = [&](int64_t at) {
         const int64_t left = unit.count - at;
-        next_q.load(q + at * c.m.q.row, c.m.q.row, left, c.m.key_size, c.vector);
-        next_k.load(k + at * c.m.k.row, c.m.k.row, left, c.m.key_size, c.vector);
-        next_v.load(v + at * c.m.v.row, c.m.v.row, left, c.m.value_size, c.vector);
-        next_g.load(g + at * c.m.g.row, c.m.g.row, c.grad_outputs ? left : 0, c.m.value_size, c.vector);
+        next_q.load(q + at * c.m.q.row, c.m.q.row, left, c.m.key_size);
+        next_k.load(k + at * c.m.k.row, c.m.k.row, left, c.m.key_size);
+        next_v.load(v + at * c.m.v.row, c.m.v.row, left, c.m.value_size);
+        next_g.load(g + at * c.m.g.row, c.m.g.row, left, c.m.value_size);
     };
     const int64_t last = (unit.count - 1) / R * R;
     load(last);
-    if (wave == 0) reach_of<T>(c, reaches[0], unit.first + last, unit.count - last, head, before);
+    float gate = 0.0f;  // of the next chunk's row, in the first wave
+    if (wave == 0) reach_of(c, reaches[0], gate_of_lane<T, R>(c, unit.first + last, unit.count - last, head), unit.count - last, before);
     int turn = 0;
     for (int64_t at = last; at >= 0; at -= R, turn ^= 1) {
-        next_q.store(queries);
-        next_k.store(keys);
-        next_v.store(values);
-        next_g.store(grads);
+        next_q.store(queries, unit.count - at, c.m.key_size);
+        next_k.store(keys, unit.count - at, c.m.key_size);
+        next_v.store(values, unit.count - at, c.m.value_size);
+        next_g.store(grads, c.grad_outputs_there ? unit.count - at : 0, c.m.value_size);
         __syncthreads();
         if (at > 0) {
             load(at - R);
-            if (wave == 0) reach_of<T>(c, reaches[turn ^ 1], unit.first + at - R, R, head, before);
+            if (wave == 0) gate = gate_of_lane<T, R>(c, unit.first + at - R, R, head);
         }
         const Reach<R> &reach = reaches[turn];
-#pragma unroll
+#pragma unroll 1
         for (int n = 0; n < (kTiles * kTiles + kWaves - 1) / kWaves; n++) {
             const int tile = wave + n * kWaves, r = tile / kTiles, s = tile % kTiles;
             if (tile >= kTiles * kTiles || (s | 1) < r) continue;
@@ -225,11 +228,11 @@ template <class T, int D> __global__ __launch_bounds__(4 * D) void attention_gra
             const int64_t row = at + 16 * r + lane % 16;
             if (row < unit.count) {
                 const int64_t here = (unit.first + row) * c.m.heads + head;
-                if (c.grad_values) put_row((T *)c.grad_values + here * c.m.value_size, column + 4 * (lane / 16), c.m.value_size, c.vector, x);
+                if (c.grad_values) put_row((T *)c.grad_values + here * c.m.value_size, column + 4 * (lane / 16), c.m.value_size, Vector, x);
                 if (c.grad_keys && c.m.shared == 1)
-                    put_row((T *)c.grad_keys + here * c.m.key_size, column + 4 * (lane / 16), c.m.key_size, c.vector, y);
+                    put_row((T *)c.grad_keys + here * c.m.key_size, column + 4 * (lane / 16), c.m.key_size, Vector, y);
                 else if (c.grad_keys)
-                    put_row((float *)c.grad_keys + here * c.m.key_size, column + 4 * (lane / 16), c.m.key_size, c.vector, y);
+                    put_row((float *)c.grad_keys + here * c.m.key_size, column + 4 * (lane / 16), c.m.key_size, Vector, y);
             }
         }
         Operand<kWhole> late[R / 32];
@@ -241,6 +244,7 @@ template <class T, int D> __global__ __launch_bounds__(4 * D) void attention_gra
         for (int n = 0; n < R / 32; n++) late[n] = weighted<kWhole>(mine_q[n], reach.row, 32 * n);
         turned.times(reach.whole);
         turned.add(grads, late);
+        if (wave == 0 && at > 0) reach_of(c, reaches[turn ^ 1], gate, R, before);
         __syncthreads();
         if (threadIdx.x < R && at + threadIdx.x < unit.count) {
             float x = 0.0f;
@@ -251,29 +255,25 @@ template <class T, int D> __global__ __launch_bounds__(4 * D) void attention_gra
     }
 }
 
-template <class T, int D> static int launch(const tg_attention &a, const AttentionCall &c, int which, hipStream_t stream) {
-    constexpr int R = Parts<T>::kRows, N = Parts<T>::kInput, kTiles = R / 16, kWaves = D / 16;
-    constexpr size_t kShared = 4 * Tile<N, R, D>::kBytes + 2 * sizeof(Reach<R>) + kWaves * R * 4;
-    constexpr size_t kQueries = kShared + Tile<N, R, R>::kBytes + 2 * kTiles * R * 4, kKeys = kShared + 2 * Tile<N, R, R>::kBytes;
-    static_assert(kQueries <= 160 * 1024 && kKeys <= 160 * 1024, "LDS");
-    static size_t reserved[2][kMaxDevices];
-    const dim3 grid((unsigned)(c.most_units * c.m.heads));
-    const void *kernel = which ? (const void *)attention_grad_keys_kernel<T, D> : (const void *)attention_grad_queries_kernel<T, D>;
-    const int code = reserve_lds("tg_linear_attention_backward", kernel, which ? kKeys : kQueries, reserved[which]);
-    if (code) return code;
-    if (which)
-        TG_LAUNCH_AS("attention_grad_keys", (attention_grad_keys_kernel<T, D>), grid, dim3(4 * D), kKeys, stream, c);
-    else
-        TG_LAUNCH_AS("attention_grad_queries", (attention_grad_queries_kernel<T, D>), grid, dim3(4 * D), kQueries, stream, c);
-    return 0;
-}
-
-int launch_attention_backward(const tg_attention &a, const AttentionCall &c, int size, int which, hipStream_t stream) {
-    const auto with = [&](auto t) {
+int launch_attention_backward(int64_t type, const AttentionCall &c, int size, bool for_keys, hipStream_t stream) {
+    return by_attention_kernel(type, size, c.vector, [&](auto t, auto d, auto vector) {
         using T = decltype(t);
-        return size <= 32 ? launch<T, 32>(a, c, which, stream) : size <= 64 ? launch<T, 64>(a, c, which, stream) : launch<T, 128>(a, c, which, stream);
-    };
-    return a.type == TG_TYPE_F32 ? with(float()) : a.type == TG_TYPE_F16 ? with(half_t()) : with(bf16_t());
+        constexpr int D = decltype(d)::value, R = Parts<T>::kRows, N = Parts<T>::kInput, kTiles = R / 16, kWaves = D / 16;
+        constexpr bool Vector = decltype(vector)::value;
+        constexpr size_t kShared = 4 * Tile<N, R, D>::kBytes + 2 * sizeof(Reach<R>) + kWaves * R * 4;
+        constexpr size_t kQueries = kShared + Tile<N, R, R>::kBytes + 2 * kTiles * R * 4, kKeys = kShared + 2 * Tile<N, R, R>::kBytes;
+        static_assert(kQueries <= 160 * 1024 && kKeys <= 160 * 1024, "LDS");
+        static size_t reserved[2][kMaxDevices];
+        const dim3 grid((unsigned)(c.most_units * c.m.heads));
+        const void *kernel = for_keys ? (const void *)attention_grad_keys_kernel<T, D, Vector> : (const void *)attention_grad_queries_kernel<T, D, Vector>;
+        const int code = reserve_lds("tg_linear_attention_backward", kernel, for_keys ? kKeys : kQueries, reserved[for_keys]);
+        if (code) return code;
+        if (for_keys)
+            TG_LAUNCH_AS("attention_grad_keys", (attention_grad_keys_kernel<T, D, Vector>), grid, dim3(4 * D), kKeys, stream, c);
+        else
+            TG_LAUNCH_AS("attention_grad_queries", (attention_grad_queries_kernel<T, D, Vector>), grid, dim3(4 * D), kQueries, stream, c);
+        return 0;
+    });
 }
 
 }  // namespace tg

@@ -15,6 +15,8 @@
 #pragma once
 #include "tg_attention.hpp"
 
+#include <type_traits>
+
 namespace tg {
 
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
@@ -148,42 +150,31 @@ template <int M, int N> __device__ __forceinline__ Operand<M> weighted(const Ope
 
 // ---- reading a chunk ----------------------------------------------------------------------
 
-// A thread's part of a chunk of Rows x D numbers, on its way to LDS: groups of eight neighbours.
-template <class T, int Rows, int D> struct Incoming {
-    static constexpr int kThreads = 4 * D, kGroups = Rows * D / 8 / kThreads;
-    T x[kGroups][8];
+// A thread's part of a chunk of Rows x D numbers, on its way to LDS: groups of eight neighbours.  Vector: groups are whole and aligned.
+template <class T, int Rows, int D, bool Vector> struct Incoming {
+    static constexpr int kThreads = 4 * D, kGroups = Rows * D / 8 / kThreads, kWidest = Vector ? 16 / (int)sizeof(T) : 1;
+    Pack<T, kWidest> x[kGroups][8 / kWidest];
 
-    // `count` rows from p on, `size` numbers each; what lies beyond is zero.  vector: groups are whole and aligned.
-    __device__ __forceinline__ void load(const T *p, int64_t row_stride, int64_t count, int size, bool vector) {
+    static __device__ __forceinline__ int row_of(int n) { return ((int)threadIdx.x + n * kThreads) / (D / 8); }
+    static __device__ __forceinline__ int column_of(int n) { return ((int)threadIdx.x + n * kThreads) % (D / 8) * 8; }
+
+    // `count` > 0 rows from p on, `size` numbers each.  What lies beyond is read from places inside, and dropped by store: a load that no branch goes
+    // around is waited for where its numbers are used, after a chunk's computation.
+    __device__ __forceinline__ void load(const T *p, int64_t row_stride, int64_t count, int size) {
 #pragma unroll
         for (int n = 0; n < kGroups; n++) {
-            const int group = (int)threadIdx.x + n * kThreads, row = group / (D / 8), column = group % (D / 8) * 8;
-            const T *from = p + row * row_stride + column;
+            const T *from = p + min((int64_t)row_of(n), count - 1) * row_stride;
 #pragma unroll
-            for (int j = 0; j < 8; j++) x[n][j] = (T)0.0f;
-            if (row >= count || column >= size) continue;
-            if (vector) {
-                constexpr int kWidest = 16 / sizeof(T);
-#pragma unroll
-                for (int j = 0; j < 8; j += kWidest) {
-                    const Pack<T, kWidest> v = load_pack<kWidest>(from + j);
-#pragma unroll
-                    for (int i = 0; i < kWidest; i++) x[n][j + i] = v.v[i];
-                }
-            } else {
-#pragma unroll
-                for (int j = 0; j < 8; j++)
-                    if (column + j < size) x[n][j] = from[j];
-            }
+            for (int j = 0; j < 8; j += kWidest) x[n][j / kWidest] = load_pack<kWidest>(from + min(column_of(n) + j, size - kWidest));
         }
     }
-    template <int N> __device__ __forceinline__ void store(const Tile<N, Rows, D> &tile) const {
+    template <int N> __device__ __forceinline__ void store(const Tile<N, Rows, D> &tile, int64_t count, int size) const {
 #pragma unroll
         for (int n = 0; n < kGroups; n++) {
-            const int group = (int)threadIdx.x + n * kThreads, row = group / (D / 8), column = group % (D / 8) * 8;
+            const int row = row_of(n), column = column_of(n);
             float v[8];
 #pragma unroll
-            for (int j = 0; j < 8; j++) v[j] = (float)x[n][j];
+            for (int j = 0; j < 8; j++) v[j] = row < count && (Vector ? column : column + j) < size ? (float)x[n][j / kWidest].v[j % kWidest] : 0.0f;
             const Operand<N> o = parts_of<N>(v);
 #pragma unroll
             for (int i = 0; i < N; i++) *(bf16x8 *)(tile.at + i * Tile<N, Rows, D>::kPart + row * Tile<N, Rows, D>::kStride + column) = o.part[i];
@@ -213,10 +204,12 @@ struct AttentionCall {
     int64_t most_units;     // units there may be
     int64_t units;          // of a sequence, where all are alike
     int chunks;             // of a unit
-    bool wide_gates, vector;
+    bool wide_gates;
+    bool vector;            // see Incoming
     bool through;           // a workgroup has a whole sequence
     // the backward pass's
     const void *grad_outputs;
+    bool grad_outputs_there;  // false: zeros, and the pointer is to something else of the values' shape
     const float *grad_final;
     void *grad_queries, *grad_keys, *grad_values, *grad_gates;
     float *grad_initial;
@@ -255,24 +248,41 @@ template <class T> __device__ __forceinline__ float gate_at(const AttentionCall 
     return c.wide_gates ? ((const float *)c.gates)[at] : (float)((const T *)c.gates)[at];
 }
 
-// One wave: the decays of `count` rows from row `first` on, where `before` is L from the unit's beginning, which moves on.
-template <class T, int Rows> __device__ __forceinline__ void reach_of(const AttentionCall &c, Reach<Rows> &out, int64_t first, int64_t count, int head, double &before) {
+// v plus that of another lane, where the data-parallel move's control has one, else v.
+template <int Control, int RowMask> __device__ __forceinline__ double plus_lane(double v) {
+    const uint64_t bits = (uint64_t)__double_as_longlong(v);
+    const uint32_t low = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)bits, Control, RowMask, 0xf, false);
+    const uint32_t high = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)(bits >> 32), Control, RowMask, 0xf, false);
+    return v + __longlong_as_double((long long)((uint64_t)high << 32 | low));
+}
+
+__device__ __forceinline__ float power_of_two(float l) { return __builtin_amdgcn_exp2f(l); }  // what is below 2^-126 is zero
+
+// One wave: the decays of `count` rows whose gates its lanes hold, where `before` is L from the unit's beginning, which moves on.
+template <int Rows> __device__ __forceinline__ void reach_of(const AttentionCall &c, Reach<Rows> &out, float gate, int64_t count, double &before) {
     const int lane = threadIdx.x % kWave;
-    double sum = lane < count && lane < Rows ? log2_gate(c.m.gate_form, gate_at<T>(c, first + lane, head)) : 0.0;
-#pragma unroll
-    for (int step = 1; step < Rows; step *= 2) {
-        const double other = __shfl_up(sum, step);
-        if (lane >= step) sum += other;
-    }
-    const double whole = __shfl(sum, Rows - 1);
+    double sum = lane < count && lane < Rows ? log2_gate(c.m.gate_form, gate) : 0.0;
+    sum = plus_lane<0x111, 0xf>(sum);  // sums over sixteen lanes by moves of 1, 2, 4 and 8
+    sum = plus_lane<0x112, 0xf>(sum);
+    sum = plus_lane<0x114, 0xf>(sum);
+    sum = plus_lane<0x118, 0xf>(sum);
+    sum = plus_lane<0x142, 0xa>(sum);  // the last lane of sixteen to the next sixteen, of 32 to the next 32
+    if (Rows > 32) sum = plus_lane<0x143, 0xc>(sum);
+    const uint64_t bits = (uint64_t)__double_as_longlong(sum);
+    const uint32_t low = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)bits, Rows - 1), high = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(bits >> 32), Rows - 1);
+    const double whole = __longlong_as_double((long long)((uint64_t)high << 32 | low));
     if (lane < Rows) {
         out.reach[lane] = sum;
-        out.row[lane] = c.m.scale * exp2f((float)sum);
-        out.column[lane] = exp2f((float)(whole - sum));
-        out.start[lane] = c.m.scale * exp2f((float)(before + sum));
-        if (lane == 0) out.whole = exp2f((float)whole);
+        out.row[lane] = c.m.scale * power_of_two((float)sum);
+        out.column[lane] = power_of_two((float)(whole - sum));
+        out.start[lane] = c.m.scale * power_of_two((float)(before + sum));
+        if (lane == 0) out.whole = power_of_two((float)whole);
     }
     before += whole;
+}
+template <class T, int Rows> __device__ __forceinline__ float gate_of_lane(const AttentionCall &c, int64_t first, int64_t count, int head) {
+    const int lane = threadIdx.x % kWave;
+    return lane < count && lane < Rows ? gate_at<T>(c, first + lane, head) : 0.0f;
 }
 
 // scale 2^(L_s - L_r) of an accumulator whose columns are rows s (or r) of the chunk, zero where s < r, or, Strict, s <= r.
@@ -285,7 +295,7 @@ template <bool ColumnsAreLater, int Rows> __device__ __forceinline__ floatx4 dec
         const double other = reach.reach[y + j];
         const float l = (float)(ColumnsAreLater ? here - other : other - here);
         const bool in = ColumnsAreLater ? x >= y + j : x <= y + j;
-        d[j] = in ? scale * exp2f(l) : 0.0f;
+        d[j] = in ? scale * power_of_two(l) : 0.0f;
     }
     return d;
 }
@@ -354,7 +364,18 @@ template <int D> struct State {
     }
 };
 
-int launch_attention_forward(const tg_attention &a, const AttentionCall &c, int size, bool states_only, hipStream_t stream);
-int launch_attention_backward(const tg_attention &a, const AttentionCall &c, int size, int which, hipStream_t stream);
+// `size`: 32, 64 or 128, of keys and values in the kernel
+int launch_attention_forward(int64_t type, const AttentionCall &c, int size, bool states_only, hipStream_t stream);
+int launch_attention_backward(int64_t type, const AttentionCall &c, int size, bool keys, hipStream_t stream);
+
+// call(T(), constant D, constant Vector)
+template <class Call> int by_attention_kernel(int64_t type, int size, bool vector, Call &&call) {
+    const auto with_type = [&](auto t) {
+        const auto with_size = [&](auto d) { return vector ? call(t, d, std::true_type()) : call(t, d, std::false_type()); };
+        return size <= 32 ? with_size(std::integral_constant<int, 32>()) : size <= 64 ? with_size(std::integral_constant<int, 64>())
+                                                                                       : with_size(std::integral_constant<int, 128>());
+    };
+    return type == TG_TYPE_F32 ? with_type(float()) : type == TG_TYPE_F16 ? with_type(half_t()) : with_type(bf16_t());
+}
 
 }  // namespace tg

@@ -5,7 +5,7 @@
 namespace tg {
 
 // What a unit adds to the state, and its decay.  A chunk is on its way from memory while the one before is computed on.
-template <class T, int D> __global__ __launch_bounds__(4 * D) void attention_states_kernel(AttentionCall c) {
+template <class T, int D, bool Vector> __global__ __launch_bounds__(4 * D) void attention_states_kernel(AttentionCall c) {
     constexpr int R = Parts<T>::kRows, N = Parts<T>::kInput;
     __shared__ __attribute__((aligned(16))) __bf16 lds[(Tile<N, R, D>::kBytes * 2) / 2];
     __shared__ Reach<R> reaches[2];
@@ -19,32 +19,34 @@ template <class T, int D> __global__ __launch_bounds__(4 * D) void attention_sta
             *v = (const T *)c.values + place_of(c.m, c.m.v, unit.sequence, rows.first, head) + unit.base * c.m.v.row;
     State<D> state = {};
     double before = 0.0;
-    Incoming<T, R, D> next_k, next_v;
-    next_k.load(k, c.m.k.row, unit.count, c.m.key_size, c.vector);
-    next_v.load(v, c.m.v.row, unit.count, c.m.value_size, c.vector);
-    if (wave == 0) reach_of<T>(c, reaches[0], unit.first, unit.count, head, before);
+    Incoming<T, R, D, Vector> next_k, next_v;
+    next_k.load(k, c.m.k.row, unit.count, c.m.key_size);
+    next_v.load(v, c.m.v.row, unit.count, c.m.value_size);
+    float gate = 0.0f;  // of the next chunk's row, in the first wave
+    if (wave == 0) reach_of(c, reaches[0], gate_of_lane<T, R>(c, unit.first, unit.count, head), unit.count, before);
     int turn = 0;
     for (int64_t at = 0; at < unit.count; at += R, turn ^= 1) {
-        next_k.store(keys);
-        next_v.store(values);
+        next_k.store(keys, unit.count - at, c.m.key_size);
+        next_v.store(values, unit.count - at, c.m.value_size);
         __syncthreads();
         if (at + R < unit.count) {
-            next_k.load(k + (at + R) * c.m.k.row, c.m.k.row, unit.count - at - R, c.m.key_size, c.vector);
-            next_v.load(v + (at + R) * c.m.v.row, c.m.v.row, unit.count - at - R, c.m.value_size, c.vector);
-            if (wave == 0) reach_of<T>(c, reaches[turn ^ 1], unit.first + at + R, unit.count - at - R, head, before);
+            next_k.load(k + (at + R) * c.m.k.row, c.m.k.row, unit.count - at - R, c.m.key_size);
+            next_v.load(v + (at + R) * c.m.v.row, c.m.v.row, unit.count - at - R, c.m.value_size);
+            if (wave == 0) gate = gate_of_lane<T, R>(c, unit.first + at + R, unit.count - at - R, head);
         }
         Operand<kWhole> mine[R / 32];
 #pragma unroll
         for (int n = 0; n < R / 32; n++) mine[n] = weighted<kWhole>(values.transposed(32 * n, column), reaches[turn].column, 32 * n);
         state.times(reaches[turn].whole);
         state.add(keys, mine);
+        if (wave == 0 && at + R < unit.count) reach_of(c, reaches[turn ^ 1], gate, unit.count - at - R, before);
         __syncthreads();
     }
     state.template store<false>(c.states + (u * c.m.heads + head) * c.m.key_size * c.m.value_size, column, c.m.key_size, c.m.value_size);
-    if (threadIdx.x == 0) c.decays[u * c.m.heads + head] = exp2f((float)before);
+    if (threadIdx.x == 0) c.decays[u * c.m.heads + head] = power_of_two((float)before);
 }
 
-template <class T, int D> __global__ __launch_bounds__(4 * D) void attention_outputs_kernel(AttentionCall c) {
+template <class T, int D, bool Vector> __global__ __launch_bounds__(4 * D) void attention_outputs_kernel(AttentionCall c) {
     constexpr int R = Parts<T>::kRows, N = Parts<T>::kInput, M = Parts<T>::kState, kTiles = R / 16, kWaves = D / 16;
     using In = Tile<N, R, D>;
     using Pairs = Tile<N, R, R>;
@@ -76,15 +78,16 @@ template <class T, int D> __global__ __launch_bounds__(4 * D) void attention_out
                                    : c.states + (u * c.m.heads + head) * state_size;
     state.template load<false>(start, column, c.m.key_size, c.m.value_size);
     double before = 0.0;
-    Incoming<T, R, D> next_q, next_k, next_v;
+    Incoming<T, R, D, Vector> next_q, next_k, next_v;
     const auto load = [&](int64_t at) {
         const int64_t left = unit.count - at;
-        next_q.load(q + at * c.m.q.row, c.m.q.row, left, c.m.key_size, c.vector);
-        next_k.load(k + at * c.m.k.row, c.m.k.row, left, c.m.key_size, c.vector);
-        next_v.load(v + at * c.m.v.row, c.m.v.row, left, c.m.value_size, c.vector);
+        next_q.load(q + at * c.m.q.row, c.m.q.row, left, c.m.key_size);
+        next_k.load(k + at * c.m.k.row, c.m.k.row, left, c.m.key_size);
+        next_v.load(v + at * c.m.v.row, c.m.v.row, left, c.m.value_size);
     };
-    load(0);
-    if (wave == 0) reach_of<T>(c, reaches[0], unit.first, unit.count, head, before);
+    if (unit.count > 0) load(0);
+    float gate = 0.0f;  // of the next chunk's row, in the first wave
+    if (wave == 0) reach_of(c, reaches[0], gate_of_lane<T, R>(c, unit.first, unit.count, head), unit.count, before);
     int turn = 0, chunk = 0;
     for (int64_t at = 0; at < unit.count; at += R, turn ^= 1) {
         if (c.through && c.states && chunk == 0) {
@@ -92,17 +95,17 @@ template <class T, int D> __global__ __launch_bounds__(4 * D) void attention_out
             u++;
         }
         chunk = chunk + 1 == c.chunks ? 0 : chunk + 1;
-        next_q.store(queries);
-        next_k.store(keys);
-        next_v.store(values);
+        next_q.store(queries, unit.count - at, c.m.key_size);
+        next_k.store(keys, unit.count - at, c.m.key_size);
+        next_v.store(values, unit.count - at, c.m.value_size);
         __syncthreads();
         if (at + R < unit.count) {
             load(at + R);
-            if (wave == 0) reach_of<T>(c, reaches[turn ^ 1], unit.first + at + R, unit.count - at - R, head, before);
+            if (wave == 0) gate = gate_of_lane<T, R>(c, unit.first + at + R, unit.count - at - R, head);
         }
         const Reach<R> &reach = reaches[turn];
         // pairs: row s, column r
-#pragma unroll
+#pragma unroll 1
         for (int n = 0; n < (kTiles * kTiles + kWaves - 1) / kWaves; n++) {
             const int tile = wave + n * kWaves, s = tile / kTiles, r = tile % kTiles;
             if (tile >= kTiles * kTiles || r > (s | 1)) continue;
@@ -128,39 +131,36 @@ template <class T, int D> __global__ __launch_bounds__(4 * D) void attention_out
             for (int n = 0; n < R / 32; n++)
                 if (2 * n <= s) o = product(mine[n], pairs.chained(16 * s, 32 * n), o);
             const int64_t row = at + 16 * s + lane % 16;
-            if (row < unit.count) put_row(out + row * out_row, column + 4 * (lane / 16), c.m.value_size, c.vector, o);
+            if (row < unit.count) put_row(out + row * out_row, column + 4 * (lane / 16), c.m.value_size, Vector, o);
         }
         Operand<kWhole> late[R / 32];
 #pragma unroll
         for (int n = 0; n < R / 32; n++) late[n] = weighted<kWhole>(mine[n], reach.column, 32 * n);
         state.times(reach.whole);
         state.add(keys, late);
+        if (wave == 0 && at + R < unit.count) reach_of(c, reaches[turn ^ 1], gate, unit.count - at - R, before);
         __syncthreads();
     }
     if (c.through) state.template store<false>(c.final + (unit.sequence * c.m.heads + head) * state_size, column, c.m.key_size, c.m.value_size);
 }
 
-template <class T, int D> static int launch(const tg_attention &a, const AttentionCall &c, bool states_only, hipStream_t stream) {
-    constexpr int R = Parts<T>::kRows, N = Parts<T>::kInput;
-    const dim3 grid((unsigned)((c.through ? c.m.sequences : c.most_units) * c.m.heads));
-    if (states_only) {
-        TG_LAUNCH_AS("attention_states", (attention_states_kernel<T, D>), grid, dim3(4 * D), 0, stream, c);
-        return 0;
-    }
-    constexpr size_t kBytes = 3 * Tile<N, R, D>::kBytes + Tile<N, R, R>::kBytes + 2 * sizeof(Reach<R>);
-    static size_t reserved[kMaxDevices];
-    const int code = reserve_lds("tg_linear_attention_forward", (const void *)attention_outputs_kernel<T, D>, kBytes, reserved);
-    if (code) return code;
-    TG_LAUNCH_AS("attention_outputs", (attention_outputs_kernel<T, D>), grid, dim3(4 * D), kBytes, stream, c);
-    return 0;
-}
-
-int launch_attention_forward(const tg_attention &a, const AttentionCall &c, int size, bool states_only, hipStream_t stream) {
-    const auto with = [&](auto t) {
+int launch_attention_forward(int64_t type, const AttentionCall &c, int size, bool states_only, hipStream_t stream) {
+    return by_attention_kernel(type, size, c.vector, [&](auto t, auto d, auto vector) {
         using T = decltype(t);
-        return size <= 32 ? launch<T, 32>(a, c, states_only, stream) : size <= 64 ? launch<T, 64>(a, c, states_only, stream) : launch<T, 128>(a, c, states_only, stream);
-    };
-    return a.type == TG_TYPE_F32 ? with(float()) : a.type == TG_TYPE_F16 ? with(half_t()) : with(bf16_t());
+        constexpr int D = decltype(d)::value, R = Parts<T>::kRows, N = Parts<T>::kInput;
+        constexpr bool Vector = decltype(vector)::value;
+        const dim3 grid((unsigned)((c.through ? c.m.sequences : c.most_units) * c.m.heads));
+        if (states_only) {
+            TG_LAUNCH_AS("attention_states", (attention_states_kernel<T, D, Vector>), grid, dim3(4 * D), 0, stream, c);
+            return 0;
+        }
+        constexpr size_t kBytes = 3 * Tile<N, R, D>::kBytes + Tile<N, R, R>::kBytes + 2 * sizeof(Reach<R>);
+        static size_t reserved[kMaxDevices];
+        const int code = reserve_lds("tg_linear_attention_forward", (const void *)attention_outputs_kernel<T, D, Vector>, kBytes, reserved);
+        if (code) return code;
+        TG_LAUNCH_AS("attention_outputs", (attention_outputs_kernel<T, D, Vector>), grid, dim3(4 * D), kBytes, stream, c);
+        return 0;
+    });
 }
 
 }  // namespace tg
