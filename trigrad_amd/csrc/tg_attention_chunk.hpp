@@ -314,33 +314,34 @@ template <class T> __device__ __forceinline__ void put_row(T *p, int column, int
     }
 }
 
+// Keeps the compiler from reading ahead over this point: operands of a whole chunk, read at its beginning, would not fit the registers.
+__device__ __forceinline__ void in_order() { __builtin_amdgcn_sched_barrier(0); }
+
 // The state in accumulators: rows of keys and columns of values (Turned: the other way round), of a wave the sixteen columns from `column` on.
 template <int D> struct State {
     floatx4 x[D / 16];
 
-    template <bool Turned> static __device__ __forceinline__ int64_t place(int row, int column, int key_size, int value_size) {
-        const int key = Turned ? column : row, value = Turned ? row : column;
-        return key < key_size && value < value_size ? (int64_t)key * value_size + value : -1;
+    // call(n, j, the place of x[n][j]) for all that are there.  One offset of a lane and a uniform one beside it, which is not kept over a loop: 32
+    // addresses would be.
+    template <bool Turned, class Call> __device__ __forceinline__ void each(int column, int key_size, int value_size, Call &&call) {
+        const int lane = threadIdx.x % kWave;
+        int across = column + lane % 16, down = 4 * (lane / 16);
+        asm volatile("" : "+v"(across), "+v"(down));
+        const int most = Turned ? value_size : key_size, offset = Turned ? across * value_size + down : down * value_size + across;
+        if (across >= (Turned ? key_size : value_size)) return;
+#pragma unroll
+        for (int n = 0; n < D / 16; n++)
+#pragma unroll
+            for (int j = 0; j < 4; j++)
+                if (down + 16 * n + j < most) call(n, j, offset + (Turned ? 16 * n + j : (16 * n + j) * value_size));
     }
     template <bool Turned> __device__ __forceinline__ void load(const float *from, int column, int key_size, int value_size) {
-        const int lane = threadIdx.x % kWave;
 #pragma unroll
-        for (int n = 0; n < D / 16; n++)
-#pragma unroll
-            for (int j = 0; j < 4; j++) {
-                const int64_t at = place<Turned>(16 * n + 4 * (lane / 16) + j, column + lane % 16, key_size, value_size);
-                x[n][j] = from && at >= 0 ? from[at] : 0.0f;
-            }
+        for (int n = 0; n < D / 16; n++) x[n] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
+        if (from) each<Turned>(column, key_size, value_size, [&](int n, int j, int at) { x[n][j] = from[at]; });
     }
-    template <bool Turned> __device__ __forceinline__ void store(float *to, int column, int key_size, int value_size) const {
-        const int lane = threadIdx.x % kWave;
-#pragma unroll
-        for (int n = 0; n < D / 16; n++)
-#pragma unroll
-            for (int j = 0; j < 4; j++) {
-                const int64_t at = place<Turned>(16 * n + 4 * (lane / 16) + j, column + lane % 16, key_size, value_size);
-                if (at >= 0) to[at] = x[n][j];
-            }
+    template <bool Turned> __device__ __forceinline__ void store(float *to, int column, int key_size, int value_size) {
+        each<Turned>(column, key_size, value_size, [&](int n, int j, int at) { to[at] = x[n][j]; });
     }
     __device__ __forceinline__ void times(float a) {
 #pragma unroll
@@ -353,14 +354,17 @@ template <int D> struct State {
             const Operand<M> mine = operand_of<M>(x[2 * i], x[2 * i + 1]);
 #pragma unroll
             for (int r = 0; r < Rows / 16; r++) sums[r] = product(mine, tile.chained(16 * r, 32 * i), sums[r]);
+            in_order();
         }
     }
     // += the transposed tile's rows times the operands of this wave's columns
     template <int N, int M, int Rows> __device__ __forceinline__ void add(const Tile<N, Rows, D> &tile, const Operand<M> *columns) {
 #pragma unroll
-        for (int n = 0; n < D / 16; n++)
+        for (int n = 0; n < D / 16; n++) {
 #pragma unroll
             for (int k = 0; k < Rows / 32; k++) x[n] = product(tile.transposed(32 * k, 16 * n), columns[k], x[n]);
+            if (n % 2 == 1) in_order();
+        }
     }
 };
 

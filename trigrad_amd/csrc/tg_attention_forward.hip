@@ -5,7 +5,7 @@
 namespace tg {
 
 // What a unit adds to the state, and its decay.  A chunk is on its way from memory while the one before is computed on.
-template <class T, int D, bool Vector> __global__ __launch_bounds__(4 * D) void attention_states_kernel(AttentionCall c) {
+template <class T, int D, bool Vector> __global__ __launch_bounds__(4 * D, 4) void attention_states_kernel(AttentionCall c) {
     constexpr int R = Parts<T>::kRows, N = Parts<T>::kInput;
     __shared__ __attribute__((aligned(16))) __bf16 lds[(Tile<N, R, D>::kBytes * 2) / 2];
     __shared__ Reach<R> reaches[2];
@@ -46,7 +46,7 @@ template <class T, int D, bool Vector> __global__ __launch_bounds__(4 * D) void 
     if (threadIdx.x == 0) c.decays[u * c.m.heads + head] = power_of_two((float)before);
 }
 
-template <class T, int D, bool Vector> __global__ __launch_bounds__(4 * D) void attention_outputs_kernel(AttentionCall c) {
+template <class T, int D, bool Vector> __global__ __launch_bounds__(4 * D, 4) void attention_outputs_kernel(AttentionCall c) {
     constexpr int R = Parts<T>::kRows, N = Parts<T>::kInput, M = Parts<T>::kState, kTiles = R / 16, kWaves = D / 16;
     using In = Tile<N, R, D>;
     using Pairs = Tile<N, R, R>;
@@ -131,6 +131,7 @@ template <class T, int D, bool Vector> __global__ __launch_bounds__(4 * D) void 
             for (int n = 0; n < R / 32; n++)
                 if (2 * n <= s) o = product(mine[n], pairs.chained(16 * s, 32 * n), o);
             const int64_t row = at + 16 * s + lane % 16;
+            in_order();
             if (row < unit.count) put_row(out + row * out_row, column + 4 * (lane / 16), c.m.value_size, Vector, o);
         }
         Operand<kWhole> late[R / 32];
