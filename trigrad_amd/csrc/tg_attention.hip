@@ -315,7 +315,7 @@ int attention_shape(const char *fn, const tg_attention &a, Attention &m) {
     }
     const int64_t limit = (int64_t)1 << 40, heads = a.heads;
     const int64_t rows = a.offsets ? a.length : a.length == 0 ? 0 : a.sequences > limit / a.length ? limit : a.sequences * a.length;
-    if (heads >= (1 << 20) || a.length > 0x7fffffff || a.sequences >= ((int64_t)1 << 29) || rows >= limit / (heads * kMost) ||
+    if (heads >= (1 << 16) || a.length > 0x7fffffff || a.sequences >= ((int64_t)1 << 29) || rows >= limit / (heads * kMost) ||
         a.sequences >= ((int64_t)1 << 31) / heads) {
         set_error("%s: %lld rows, %lld sequences of %lld heads are too many", fn, (long long)rows, (long long)a.sequences, (long long)heads);
         return TG_E_ARG;
@@ -437,7 +437,7 @@ static int split_of(const char *fn, const tg_attention &a, const Attention &m, S
     s.most_units = m.packed ? m.length / (s.rows_of_chunk * s.chunks) + m.sequences : s.units * m.sequences;
     // sequences and heads enough: the forward pass goes through each from its first row to its last, and reads keys and values once
     s.through = s.units <= 1 || (!m.packed && m.sequences * m.heads >= kWanted);
-    if (s.most_units * m.heads >= kGridThreads / (4 * s.size) || m.sequences * m.heads >= kGridThreads / (4 * s.size) || s.most_units > 0x7fffffff) {
+    if (s.most_units * m.heads >= kGridThreads / (8 * s.size) || m.sequences * m.heads >= kGridThreads / (8 * s.size) || s.most_units > 0x7fffffff) {
         set_error("%s: %lld rows, %lld sequences of %d heads are too many", fn, (long long)m.rows, (long long)m.sequences, m.heads);
         return TG_E_ARG;
     }
@@ -487,7 +487,7 @@ static int sizes_of(const char *fn, const tg_attention &a, const Attention &m, i
 
 static bool in_vectors(const tg_attention &a, const Attention &m) {
     const int64_t bytes = type_bytes(a.type);
-    if (m.key_size % 8 != 0 || m.value_size % 8 != 0) return false;
+    if (m.key_size * bytes % 16 != 0 || m.value_size * bytes % 16 != 0) return false;
     for (const void *p : {a.queries, a.keys, a.values, (const void *)a.outputs, a.grad_outputs, (const void *)a.grad_queries, (const void *)a.grad_keys, (const void *)a.grad_values})
         if ((uintptr_t)p % 16 != 0) return false;
     const auto dense = [&](const Strides &t, int heads) {

@@ -69,9 +69,9 @@ template <int N> __device__ __forceinline__ Operand<N> operand_of(floatx4 above,
 template <int N, int Rows, int Columns> struct Tile {
     static constexpr int kStride = Columns + 8, kPart = Rows * kStride, kBytes = N * kPart * 2;
     __bf16 *at;
+    int lane;
 
     __device__ __forceinline__ Operand<N> straight(int row, int column) const {
-        const int lane = threadIdx.x % kWave;
         const __bf16 *p = at + (row + lane % 16) * kStride + column + 8 * (lane / 16);
         Operand<N> o;
 #pragma unroll
@@ -79,7 +79,6 @@ template <int N, int Rows, int Columns> struct Tile {
         return o;
     }
     __device__ __forceinline__ Operand<N> chained(int row, int column) const {
-        const int lane = threadIdx.x % kWave;
         const __bf16 *p = at + (row + lane % 16) * kStride + column + 4 * (lane / 16);
         Operand<N> o;
 #pragma unroll
@@ -92,7 +91,6 @@ template <int N, int Rows, int Columns> struct Tile {
     // The transposed matrix's: row or column `column` + lane % 16, chained rows from `row`.  LDS hands out four rows of sixteen columns transposed to
     // sixteen lanes, of which each points at four neighbours of a row.
     __device__ __forceinline__ Operand<N> transposed(int row, int column) const {
-        const int lane = threadIdx.x % kWave;
         const __bf16 *p = at + (row + 4 * (lane / 16) + lane % 16 / 4) * kStride + column + 4 * (lane % 4);
         Operand<N> o;
 #pragma unroll
@@ -118,7 +116,6 @@ template <int N, int Rows, int Columns> struct Tile {
     }
     // An accumulator's four rows (columns here) of its column (a row here): the product's transpose.
     __device__ __forceinline__ void put(int row, int column, floatx4 x) const {
-        const int lane = threadIdx.x % kWave;
         __bf16 *p = at + (row + lane % 16) * kStride + column + 4 * (lane / 16);
 #pragma unroll
         for (int n = 0; n < N; n++) {
@@ -134,8 +131,8 @@ template <int N, int Rows, int Columns> struct Tile {
 };
 
 // A transposed input's operand with a weight for each row.
-template <int M, int N> __device__ __forceinline__ Operand<M> weighted(const Operand<N> &o, const float *weights, int row) {
-    const int group = threadIdx.x % kWave / 16;
+template <int M, int N> __device__ __forceinline__ Operand<M> weighted(const Operand<N> &o, const float *weights, int row, int lane) {
+    const int group = lane / 16;
     const floatx4 a = *(const floatx4 *)(weights + row + 4 * group), b = *(const floatx4 *)(weights + row + 16 + 4 * group);
     float x[8];
 #pragma unroll
@@ -150,19 +147,22 @@ template <int M, int N> __device__ __forceinline__ Operand<M> weighted(const Ope
 
 // ---- reading a chunk ----------------------------------------------------------------------
 
-// A thread's part of a chunk of Rows x D numbers, on its way to LDS: groups of eight neighbours.  Vector: groups are whole and aligned.
-template <class T, int Rows, int D, bool Vector> struct Incoming {
-    static constexpr int kThreads = 4 * D, kGroups = Rows * D / 8 / kThreads, kWidest = Vector ? 16 / (int)sizeof(T) : 1;
+// A thread's part of a chunk of Rows x D numbers, on its way to LDS: groups of eight neighbours.  Vector: in accesses of 16 bytes, which divide the
+// rows and are aligned.
+template <class T, int Rows, int D, int Threads, bool Vector> struct Incoming {
+    static constexpr int kAll = Rows * D / 8, kGroups = (kAll + Threads - 1) / Threads, kWidest = Vector ? 16 / (int)sizeof(T) : 1;
     Pack<T, kWidest> x[kGroups][8 / kWidest];
 
-    static __device__ __forceinline__ int row_of(int n) { return ((int)threadIdx.x + n * kThreads) / (D / 8); }
-    static __device__ __forceinline__ int column_of(int n) { return ((int)threadIdx.x + n * kThreads) % (D / 8) * 8; }
+    static __device__ __forceinline__ int row_of(int n) { return ((int)threadIdx.x + n * Threads) / (D / 8); }
+    static __device__ __forceinline__ int column_of(int n) { return ((int)threadIdx.x + n * Threads) % (D / 8) * 8; }
+    static __device__ __forceinline__ bool mine(int n) { return kAll % Threads == 0 || (int)threadIdx.x + n * Threads < kAll; }  // for whole waves alike
 
     // `count` > 0 rows from p on, `size` numbers each.  What lies beyond is read from places inside, and dropped by store: a load that no branch goes
     // around is waited for where its numbers are used, after a chunk's computation.
     __device__ __forceinline__ void load(const T *p, int64_t row_stride, int64_t count, int size) {
 #pragma unroll
         for (int n = 0; n < kGroups; n++) {
+            if (!mine(n)) continue;
             const T *from = p + min((int64_t)row_of(n), count - 1) * row_stride;
 #pragma unroll
             for (int j = 0; j < 8; j += kWidest) x[n][j / kWidest] = load_pack<kWidest>(from + min(column_of(n) + j, size - kWidest));
@@ -171,16 +171,23 @@ template <class T, int Rows, int D, bool Vector> struct Incoming {
     template <int N> __device__ __forceinline__ void store(const Tile<N, Rows, D> &tile, int64_t count, int size) const {
 #pragma unroll
         for (int n = 0; n < kGroups; n++) {
+            if (!mine(n)) continue;
             const int row = row_of(n), column = column_of(n);
             float v[8];
 #pragma unroll
-            for (int j = 0; j < 8; j++) v[j] = row < count && (Vector ? column : column + j) < size ? (float)x[n][j / kWidest].v[j % kWidest] : 0.0f;
+            for (int j = 0; j < 8; j++) v[j] = row < count && column + j / kWidest * kWidest < size ? (float)x[n][j / kWidest].v[j % kWidest] : 0.0f;
             const Operand<N> o = parts_of<N>(v);
 #pragma unroll
             for (int i = 0; i < N; i++) *(bf16x8 *)(tile.at + i * Tile<N, Rows, D>::kPart + row * Tile<N, Rows, D>::kStride + column) = o.part[i];
         }
     }
 };
+
+// Waves of a SIMD that kernels are compiled for: four (128 registers a lane) where a CU's 160 KB of LDS have room for as many workgroups.
+constexpr int waves_of_simd(int threads, int lds_bytes) {
+    const int groups = 160 * 1024 / lds_bytes, waves = groups * threads / kWave / 4;
+    return waves > 4 ? 4 : waves < 1 ? 1 : waves;
+}
 
 // Decays of a chunk.
 template <int Rows> struct alignas(16) Reach {
@@ -286,8 +293,8 @@ template <class T, int Rows> __device__ __forceinline__ float gate_of_lane(const
 }
 
 // scale 2^(L_s - L_r) of an accumulator whose columns are rows s (or r) of the chunk, zero where s < r, or, Strict, s <= r.
-template <bool ColumnsAreLater, int Rows> __device__ __forceinline__ floatx4 decays_of(const Reach<Rows> &reach, int row, int column, float scale) {
-    const int lane = threadIdx.x % kWave, x = column + lane % 16, y = row + 4 * (lane / 16);
+template <bool ColumnsAreLater, int Rows> __device__ __forceinline__ floatx4 decays_of(const Reach<Rows> &reach, int row, int column, float scale, int lane) {
+    const int x = column + lane % 16, y = row + 4 * (lane / 16);
     const double here = reach.reach[x];
     floatx4 d;
 #pragma unroll
@@ -300,18 +307,27 @@ template <bool ColumnsAreLater, int Rows> __device__ __forceinline__ floatx4 dec
     return d;
 }
 
-// Four neighbours of an output's row.
-template <class T> __device__ __forceinline__ void put_row(T *p, int column, int size, bool vector, floatx4 x) {
+// Four neighbours of an output's row, `offset` numbers from p on.
+template <class T> __device__ __forceinline__ void put_row(T *p, uint32_t offset, int column, int size, bool vector, floatx4 x) {
     if (vector) {
         if (column < size) {
             const float v[4] = {x[0], x[1], x[2], x[3]};
-            store_pack<4>(p + column, v);
+            store_pack<4>(p + offset, v);
         }
     } else {
 #pragma unroll
         for (int j = 0; j < 4; j++)
-            if (column + j < size) p[column + j] = (T)x[j];
+            if (column + j < size) p[offset + j] = (T)x[j];
     }
+}
+
+// The number of the wave, and a lane's in it.  What is made of lane_of_turn is made again in each turn of a loop: places in LDS and in memory that
+// were kept over all of them would take more registers than the states.
+__device__ __forceinline__ int wave_of() { return __builtin_amdgcn_readfirstlane(threadIdx.x / kWave); }
+__device__ __forceinline__ int lane_of_turn() {
+    int lane = threadIdx.x % kWave;
+    asm volatile("" : "+v"(lane));
+    return lane;
 }
 
 // Keeps the compiler from reading ahead over this point: operands of a whole chunk, read at its beginning, would not fit the registers.
@@ -324,9 +340,7 @@ template <int D> struct State {
     // call(n, j, the place of x[n][j]) for all that are there.  One offset of a lane and a uniform one beside it, which is not kept over a loop: 32
     // addresses would be.
     template <bool Turned, class Call> __device__ __forceinline__ void each(int column, int key_size, int value_size, Call &&call) {
-        const int lane = threadIdx.x % kWave;
-        int across = column + lane % 16, down = 4 * (lane / 16);
-        asm volatile("" : "+v"(across), "+v"(down));
+        const int lane = lane_of_turn(), across = column + lane % 16, down = 4 * (lane / 16);
         const int most = Turned ? value_size : key_size, offset = Turned ? across * value_size + down : down * value_size + across;
         if (across >= (Turned ? key_size : value_size)) return;
 #pragma unroll
@@ -353,17 +367,18 @@ template <int D> struct State {
         for (int i = 0; i < D / 32; i++) {
             const Operand<M> mine = operand_of<M>(x[2 * i], x[2 * i + 1]);
 #pragma unroll
-            for (int r = 0; r < Rows / 16; r++) sums[r] = product(mine, tile.chained(16 * r, 32 * i), sums[r]);
-            in_order();
+            for (int r = 0; r < Rows / 16; r++) {
+                sums[r] = product(mine, tile.chained(16 * r, 32 * i), sums[r]);
+                if (r % 2 == 1) in_order();
+            }
         }
     }
-    // += the transposed tile's rows times the operands of this wave's columns
-    template <int N, int M, int Rows> __device__ __forceinline__ void add(const Tile<N, Rows, D> &tile, const Operand<M> *columns) {
+    // += 32 rows of the tile, transposed, times this wave's columns of as many rows
+    template <int N, int M, int Rows> __device__ __forceinline__ void add(const Tile<N, Rows, D> &tile, int row, const Operand<M> &columns) {
 #pragma unroll
         for (int n = 0; n < D / 16; n++) {
-#pragma unroll
-            for (int k = 0; k < Rows / 32; k++) x[n] = product(tile.transposed(32 * k, 16 * n), columns[k], x[n]);
-            if (n % 2 == 1) in_order();
+            x[n] = product(tile.transposed(row, 16 * n), columns, x[n]);
+            if (n % 4 == 3) in_order();
         }
     }
 };

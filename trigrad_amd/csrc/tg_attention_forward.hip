@@ -4,14 +4,18 @@
 
 namespace tg {
 
+template <class T, int D> constexpr int kStatesLds = 2 * Tile<Parts<T>::kInput, Parts<T>::kRows, D>::kBytes + 2 * (int)sizeof(Reach<Parts<T>::kRows>);
+template <class T, int D> constexpr int kOutputsLds = 3 * Tile<Parts<T>::kInput, Parts<T>::kRows, D>::kBytes +
+                                                      Tile<Parts<T>::kInput, Parts<T>::kRows, Parts<T>::kRows>::kBytes + 2 * (int)sizeof(Reach<Parts<T>::kRows>);
+
 // What a unit adds to the state, and its decay.  A chunk is on its way from memory while the one before is computed on.
-template <class T, int D, bool Vector> __global__ __launch_bounds__(4 * D, 4) void attention_states_kernel(AttentionCall c) {
+template <class T, int D, bool Vector>
+__global__ __launch_bounds__(4 * D, waves_of_simd(4 * D, kStatesLds<T, D>)) void attention_states_kernel(AttentionCall c) {
     constexpr int R = Parts<T>::kRows, N = Parts<T>::kInput;
     __shared__ __attribute__((aligned(16))) __bf16 lds[(Tile<N, R, D>::kBytes * 2) / 2];
     __shared__ Reach<R> reaches[2];
-    const Tile<N, R, D> keys{lds}, values{lds + Tile<N, R, D>::kBytes / 2};
     const int64_t u = blockIdx.x / c.m.heads;
-    const int head = (int)(blockIdx.x % c.m.heads), wave = threadIdx.x / kWave, column = 16 * wave;
+    const int head = (int)(blockIdx.x % c.m.heads), wave = wave_of(), column = 16 * wave;
     const Unit unit = unit_of<R>(c, u);
     if (!unit.there) return;
     const AttentionRows rows = rows_of(c.m, c.offsets, unit.sequence);
@@ -19,13 +23,15 @@ template <class T, int D, bool Vector> __global__ __launch_bounds__(4 * D, 4) vo
             *v = (const T *)c.values + place_of(c.m, c.m.v, unit.sequence, rows.first, head) + unit.base * c.m.v.row;
     State<D> state = {};
     double before = 0.0;
-    Incoming<T, R, D, Vector> next_k, next_v;
+    Incoming<T, R, D, 4 * D, Vector> next_k, next_v;
     next_k.load(k, c.m.k.row, unit.count, c.m.key_size);
     next_v.load(v, c.m.v.row, unit.count, c.m.value_size);
     float gate = 0.0f;  // of the next chunk's row, in the first wave
     if (wave == 0) reach_of(c, reaches[0], gate_of_lane<T, R>(c, unit.first, unit.count, head), unit.count, before);
     int turn = 0;
     for (int64_t at = 0; at < unit.count; at += R, turn ^= 1) {
+        const int lane = lane_of_turn();
+        const Tile<N, R, D> keys{lds, lane}, values{lds + Tile<N, R, D>::kBytes / 2, lane};
         next_k.store(keys, unit.count - at, c.m.key_size);
         next_v.store(values, unit.count - at, c.m.value_size);
         __syncthreads();
@@ -34,11 +40,9 @@ template <class T, int D, bool Vector> __global__ __launch_bounds__(4 * D, 4) vo
             next_v.load(v + (at + R) * c.m.v.row, c.m.v.row, unit.count - at - R, c.m.value_size);
             if (wave == 0) gate = gate_of_lane<T, R>(c, unit.first + at + R, unit.count - at - R, head);
         }
-        Operand<kWhole> mine[R / 32];
-#pragma unroll
-        for (int n = 0; n < R / 32; n++) mine[n] = weighted<kWhole>(values.transposed(32 * n, column), reaches[turn].column, 32 * n);
         state.times(reaches[turn].whole);
-        state.add(keys, mine);
+#pragma unroll
+        for (int n = 0; n < R / 32; n++) state.add(keys, 32 * n, weighted<kWhole>(values.transposed(32 * n, column), reaches[turn].column, 32 * n, lane));
         if (wave == 0 && at + R < unit.count) reach_of(c, reaches[turn ^ 1], gate, unit.count - at - R, before);
         __syncthreads();
     }
@@ -46,16 +50,15 @@ template <class T, int D, bool Vector> __global__ __launch_bounds__(4 * D, 4) vo
     if (threadIdx.x == 0) c.decays[u * c.m.heads + head] = power_of_two((float)before);
 }
 
-template <class T, int D, bool Vector> __global__ __launch_bounds__(4 * D, 4) void attention_outputs_kernel(AttentionCall c) {
+template <class T, int D, bool Vector>
+__global__ __launch_bounds__(4 * D, waves_of_simd(4 * D, kOutputsLds<T, D>)) void attention_outputs_kernel(AttentionCall c) {
     constexpr int R = Parts<T>::kRows, N = Parts<T>::kInput, M = Parts<T>::kState, kTiles = R / 16, kWaves = D / 16;
     using In = Tile<N, R, D>;
     using Pairs = Tile<N, R, R>;
     extern __shared__ __attribute__((aligned(16))) char lds[];
-    const In queries{(__bf16 *)lds}, keys{(__bf16 *)(lds + In::kBytes)}, values{(__bf16 *)(lds + 2 * In::kBytes)};
-    const Pairs pairs{(__bf16 *)(lds + 3 * In::kBytes)};
     Reach<R> *reaches = (Reach<R> *)(lds + 3 * In::kBytes + Pairs::kBytes);
     const int64_t which = blockIdx.x / c.m.heads;  // a unit, or a sequence
-    const int head = (int)(blockIdx.x % c.m.heads), lane = threadIdx.x % kWave, wave = threadIdx.x / kWave, column = 16 * wave;
+    const int head = (int)(blockIdx.x % c.m.heads), wave = wave_of(), column = 16 * wave;
     const int64_t state_size = (int64_t)c.m.key_size * c.m.value_size;
     Unit unit;
     int64_t u = which;
@@ -78,7 +81,7 @@ template <class T, int D, bool Vector> __global__ __launch_bounds__(4 * D, 4) vo
                                    : c.states + (u * c.m.heads + head) * state_size;
     state.template load<false>(start, column, c.m.key_size, c.m.value_size);
     double before = 0.0;
-    Incoming<T, R, D, Vector> next_q, next_k, next_v;
+    Incoming<T, R, D, 4 * D, Vector> next_q, next_k, next_v;
     const auto load = [&](int64_t at) {
         const int64_t left = unit.count - at;
         next_q.load(q + at * c.m.q.row, c.m.q.row, left, c.m.key_size);
@@ -90,6 +93,9 @@ template <class T, int D, bool Vector> __global__ __launch_bounds__(4 * D, 4) vo
     if (wave == 0) reach_of(c, reaches[0], gate_of_lane<T, R>(c, unit.first, unit.count, head), unit.count, before);
     int turn = 0, chunk = 0;
     for (int64_t at = 0; at < unit.count; at += R, turn ^= 1) {
+        const int lane = lane_of_turn();
+        const In queries{(__bf16 *)lds, lane}, keys{(__bf16 *)(lds + In::kBytes), lane}, values{(__bf16 *)(lds + 2 * In::kBytes), lane};
+        const Pairs pairs{(__bf16 *)(lds + 3 * In::kBytes), lane};
         if (c.through && c.states && chunk == 0) {
             if (u < c.most_units) state.template store<false>(c.states + (u * c.m.heads + head) * state_size, column, c.m.key_size, c.m.value_size);
             u++;
@@ -113,16 +119,16 @@ template <class T, int D, bool Vector> __global__ __launch_bounds__(4 * D, 4) vo
             if (r <= s) {
 #pragma unroll
                 for (int i = 0; i < D; i += 32) p = product(keys.straight(16 * r, i), queries.straight(16 * s, i), p);
-                p *= decays_of<true>(reach, 16 * r, 16 * s, c.m.scale);
+                p *= decays_of<true>(reach, 16 * r, 16 * s, c.m.scale, lane);
             }
             pairs.put(16 * s, 16 * r, p);
         }
-        Operand<N> mine[R / 32];
-#pragma unroll
-        for (int n = 0; n < R / 32; n++) mine[n] = values.transposed(32 * n, column);
         floatx4 read[kTiles] = {};
         state.template read_by<M>(queries, read);
         __syncthreads();
+        Operand<N> mine[R / 32];
+#pragma unroll
+        for (int n = 0; n < R / 32; n++) mine[n] = values.transposed(32 * n, column);
 #pragma unroll
         for (int s = 0; s < kTiles; s++) {
             floatx4 o = read[s];
@@ -130,15 +136,14 @@ template <class T, int D, bool Vector> __global__ __launch_bounds__(4 * D, 4) vo
 #pragma unroll
             for (int n = 0; n < R / 32; n++)
                 if (2 * n <= s) o = product(mine[n], pairs.chained(16 * s, 32 * n), o);
-            const int64_t row = at + 16 * s + lane % 16;
             in_order();
-            if (row < unit.count) put_row(out + row * out_row, column + 4 * (lane / 16), c.m.value_size, Vector, o);
+            const int to = column + 4 * (lane / 16);
+            if (16 * s + lane % 16 < unit.count - at)
+                put_row(out + (at + 16 * s) * out_row, (uint32_t)(lane % 16 * (int)out_row + to), to, c.m.value_size, Vector, o);
         }
-        Operand<kWhole> late[R / 32];
-#pragma unroll
-        for (int n = 0; n < R / 32; n++) late[n] = weighted<kWhole>(mine[n], reach.column, 32 * n);
         state.times(reach.whole);
-        state.add(keys, late);
+#pragma unroll
+        for (int n = 0; n < R / 32; n++) state.add(keys, 32 * n, weighted<kWhole>(mine[n], reach.column, 32 * n, lane));
         if (wave == 0 && at + R < unit.count) reach_of(c, reaches[turn ^ 1], gate, unit.count - at - R, before);
         __syncthreads();
     }
@@ -148,14 +153,14 @@ template <class T, int D, bool Vector> __global__ __launch_bounds__(4 * D, 4) vo
 int launch_attention_forward(int64_t type, const AttentionCall &c, int size, bool states_only, hipStream_t stream) {
     return by_attention_kernel(type, size, c.vector, [&](auto t, auto d, auto vector) {
         using T = decltype(t);
-        constexpr int D = decltype(d)::value, R = Parts<T>::kRows, N = Parts<T>::kInput;
+        constexpr int D = decltype(d)::value;
         constexpr bool Vector = decltype(vector)::value;
         const dim3 grid((unsigned)((c.through ? c.m.sequences : c.most_units) * c.m.heads));
         if (states_only) {
             TG_LAUNCH_AS("attention_states", (attention_states_kernel<T, D, Vector>), grid, dim3(4 * D), 0, stream, c);
             return 0;
         }
-        constexpr size_t kBytes = 3 * Tile<N, R, D>::kBytes + Tile<N, R, R>::kBytes + 2 * sizeof(Reach<R>);
+        constexpr int kBytes = kOutputsLds<T, D>;
         static size_t reserved[kMaxDevices];
         const int code = reserve_lds("tg_linear_attention_forward", (const void *)attention_outputs_kernel<T, D, Vector>, kBytes, reserved);
         if (code) return code;
