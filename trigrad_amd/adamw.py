@@ -87,6 +87,9 @@ def adamw_step(
 
     A tensor that is written may not overlap any other.  The call can be captured into a graph, with step and lr as tensors.
     """
+    module = _C.operators_by_torch_module(params[0] if len(params) else None)
+    if module is not None and module.adamw_step(params, grads, exp_avgs, exp_avg_sqs, step, lr, *betas, eps, weight_decay, copies, scales, grad_scale, maximize, seed):
+        return
     for name, tensors in (("grads", grads), ("exp_avgs", exp_avgs), ("exp_avg_sqs", exp_avg_sqs), ("copies", copies), ("scales", scales)):
         if tensors is not None and len(tensors) != len(params):
             raise ValueError(f"{name} must have {len(params)} tensors, but got {len(tensors)}")

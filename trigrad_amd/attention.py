@@ -124,6 +124,11 @@ def linear_attention(
         outputs : as values
         final : (S, H, K, V) float32, the state behind the last step of each sequence
     """
+    module = _C.operators_by_torch_module(values)
+    if module is not None:
+        out = module.linear_attention(queries, keys, values, gates, initial, offsets, GATE_FORMS.get(gate_form), scale)
+        if out is not None:
+            return out
     return LinearAttention.apply(queries, keys, values, gates, initial, offsets, gate_form, scale)
 
 
@@ -147,6 +152,11 @@ def linear_attention_step(
         outputs : as values
         state : the new state (`state` itself, or `out`)
     """
+    module = _C.operators_by_torch_module(values)
+    if module is not None:
+        result = module.linear_attention_step(queries, keys, values, gates, state, GATE_FORMS.get(gate_form), scale, out)
+        if result is not None:
+            return result
     if values.dim() != 3 or keys.dim() != 3 or queries.dim() != 3:
         raise ValueError(f"queries, keys and values must have 3 dimensions, but got {queries.dim()}, {keys.dim()} and {values.dim()}")
     _check(queries[:, None], keys[:, None], values[:, None], gates if gates.dim() == 1 else gates[:, None], state, None, gate_form, "state")

@@ -173,6 +173,12 @@ template <class T, int Rows, int D, int Threads, bool Vector> struct Incoming {
         for (int n = 0; n < kGroups; n++) {
             if (!mine(n)) continue;
             const int row = row_of(n), column = column_of(n);
+            if constexpr (Vector && N == 1) {  // bfloat16 as it is
+                typedef uint32_t words __attribute__((ext_vector_type(4)));
+                const words w = __builtin_bit_cast(words, x[n][0]), none = {0, 0, 0, 0};
+                *(words *)(tile.at + row * Tile<N, Rows, D>::kStride + column) = row < count && column < size ? w : none;
+                continue;
+            }
             float v[8];
 #pragma unroll
             for (int j = 0; j < 8; j++) v[j] = row < count && column + j / kWidest * kWidest < size ? (float)x[n][j / kWidest].v[j % kWidest] : 0.0f;

@@ -441,7 +441,7 @@ PyObject *py_verify(PyObject *, PyObject *wait) {
 
 }  // namespace
 
-#include "tg_torch_operators.hpp"
+#include "tg_torch_attention.hpp"
 
 namespace {
 
@@ -450,6 +450,9 @@ PyMethodDef methods[] = {{"render", reinterpret_cast<PyCFunction>(reinterpret_ca
                          {"linear_recurrence_step", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_linear_recurrence_step)), METH_FASTCALL,
                           nullptr},
                          {"group_norm", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_group_norm)), METH_FASTCALL, nullptr},
+                         {"linear_attention", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_linear_attention)), METH_FASTCALL, nullptr},
+                         {"linear_attention_step", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_linear_attention_step)), METH_FASTCALL, nullptr},
+                         {"adamw_step", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_adamw_step)), METH_FASTCALL, nullptr},
                          {"refuse_stale_leaves", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_refuse_stale_leaves)), METH_FASTCALL, nullptr},
                          {"bind_operators", py_bind_operators, METH_VARARGS, nullptr},
                          {"bind", py_bind, METH_VARARGS, nullptr},

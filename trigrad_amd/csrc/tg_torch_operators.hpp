@@ -19,6 +19,11 @@ struct OperatorLibrary {
     int (*norm_sizes)(const tg_norm *, int64_t *) = nullptr;
     int (*norm_forward)(const tg_norm *) = nullptr;
     int (*norm_backward)(const tg_norm *) = nullptr;
+    int (*attention_sizes)(const tg_attention *, int64_t *) = nullptr;
+    int (*attention_forward)(const tg_attention *) = nullptr;
+    int (*attention_backward)(const tg_attention *) = nullptr;
+    int (*attention_step)(const tg_attention *) = nullptr;
+    int (*adamw_step)(const tg_adamw *) = nullptr;
 } operators;
 
 struct Unlocked {  // the interpreter is others' while this lives
@@ -404,21 +409,6 @@ PyObject *py_refuse_stale_leaves(PyObject *, PyObject *const *args, Py_ssize_t n
     }
     Py_RETURN_NONE;
     END_HANDLE_TH_ERRORS
-}
-
-// bind_operators(addresses of the library's entry points in OperatorLibrary's order)
-PyObject *py_bind_operators(PyObject *, PyObject *args) {
-    unsigned long long a[7];
-    if (!PyArg_ParseTuple(args, "KKKKKKK", &a[0], &a[1], &a[2], &a[3], &a[4], &a[5], &a[6])) return nullptr;
-    const auto set = [](auto &to, unsigned long long from) { to = reinterpret_cast<std::decay_t<decltype(to)>>(from); };
-    set(operators.recurrence_sizes, a[0]);
-    set(operators.recurrence_forward, a[1]);
-    set(operators.recurrence_backward, a[2]);
-    set(operators.recurrence_step, a[3]);
-    set(operators.norm_sizes, a[4]);
-    set(operators.norm_forward, a[5]);
-    set(operators.norm_backward, a[6]);
-    Py_RETURN_NONE;
 }
 
 }  // namespace
