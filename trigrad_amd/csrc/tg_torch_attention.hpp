@@ -259,14 +259,20 @@ PyObject *py_linear_attention_step(PyObject *, PyObject *const *args, Py_ssize_t
 
 // ---- AdamW -------------------------------------------------------------------------------
 
-// The tensors of a list or tuple; false: not a case for this route.
-bool take_tensors(PyObject *arg, size_t count, bool optional, std::vector<at::Tensor> &to) {
+// The tensors of a list or tuple, which holds them for the call, and null for None; false: not a case for this route.
+using Tensors = std::vector<const at::Tensor *>;
+bool take_tensors(PyObject *arg, size_t count, bool optional, Tensors &to) {
     if (optional && arg == Py_None) return true;
     const bool list = PyList_CheckExact(arg);
     if ((!list && !PyTuple_CheckExact(arg)) || (size_t)Py_SIZE(arg) != count) return false;
     to.resize(count);
-    for (size_t i = 0; i < count; i++)
-        if (!take(list ? PyList_GET_ITEM(arg, i) : PyTuple_GET_ITEM(arg, i), optional, to[i])) return false;
+    for (size_t i = 0; i < count; i++) {
+        PyObject *item = list ? PyList_GET_ITEM(arg, i) : PyTuple_GET_ITEM(arg, i);
+        if (optional && item == Py_None) continue;
+        if (!THPVariable_CheckTypeExact(Py_TYPE(item))) return false;  // a tensor or a parameter
+        to[i] = &THPVariable_Unpack(item);
+        if (!to[i]->is_cuda() || at::isTensorSubclassLike(*to[i])) return false;
+    }
     return true;
 }
 
@@ -311,14 +317,14 @@ bool apart(std::vector<std::vector<Extent>> &lists) {
 // adamw_step(params, grads, averages, squares, step, rate, beta1, beta2, eps, decay, copies, scales, grad_scale, maximize, seed) -> True, or None
 PyObject *py_adamw_step(PyObject *, PyObject *const *args, Py_ssize_t n) {
     HANDLE_TH_ERRORS
-    std::vector<at::Tensor> params, grads, averages, squares, copies, scales;
+    Tensors params, grads, averages, squares, copies, scales;
     at::Tensor step, rate, grad_scale;
     tg_adamw c = {};
     if (n != 15 || !plain_call() || (!PyList_CheckExact(args[0]) && !PyTuple_CheckExact(args[0])) || Py_SIZE(args[0]) == 0) Py_RETURN_NONE;
     const size_t count = (size_t)Py_SIZE(args[0]);
     if (!take_tensors(args[0], count, false, params) || !take_tensors(args[1], count, false, grads) || !take_tensors(args[2], count, false, averages) ||
         !take_tensors(args[3], count, false, squares) || !take_tensors(args[10], count, true, copies) || !take_tensors(args[11], count, true, scales) ||
-        !take(args[12], true, grad_scale) || !take_single(args[4], params[0], c.step, step) || !take_single(args[5], params[0], c.rate, rate))
+        !take(args[12], true, grad_scale) || !take_single(args[4], *params[0], c.step, step) || !take_single(args[5], *params[0], c.rate, rate))
         Py_RETURN_NONE;
     double *const numbers[] = {&c.beta1, &c.beta2, &c.eps, &c.decay};
     for (int i = 0; i < 4; i++) {
@@ -330,55 +336,57 @@ PyObject *py_adamw_step(PyObject *, PyObject *const *args, Py_ssize_t n) {
         Py_RETURN_NONE;
     c.maximize = args[13] == Py_True;
     c.seed = (int64_t)(PyLong_AsUnsignedLongLongMask(args[14]) & 0xFFFFFFFFu);
-    const at::Tensor &like = params[0];
-    const auto single = [&](const at::Tensor &t) { return t.device() == like.device() && t.scalar_type() == at::kFloat && t.numel() == 1 && !t.is_neg(); };
+    const at::Tensor &like = *params[0];
+    const c10::Device device = like.device();
+    const auto single = [&](const at::Tensor &t) { return t.device() == device && t.scalar_type() == at::kFloat && t.numel() == 1 && !t.is_neg(); };
     if (grad_scale.defined() && !single(grad_scale)) Py_RETURN_NONE;
     const at::ScalarType state = scales.empty() ? at::kFloat : at::kFloat8_e4m3fn;
     const auto written = [&](const at::Tensor &t, at::ScalarType type) {
-        return t.scalar_type() == type && t.device() == like.device() && t.is_contiguous() && !t.is_neg();
+        return t.scalar_type() == type && t.device() == device && t.is_contiguous() && !t.is_neg();
     };
     std::vector<std::vector<Extent>> extents(6);
-    const auto extent = [](const at::Tensor &t, bool written) {
-        const char *first = static_cast<const char *>(t.data_ptr());
-        return Extent{first, first + t.numel() * t.element_size(), written};
+    for (auto &e : extents) e.reserve(count);
+    const auto extent = [](const void *first, int64_t bytes, bool written) {
+        return Extent{static_cast<const char *>(first), static_cast<const char *>(first) + bytes, written};
     };
     std::vector<const void *> grad_at(count);
     std::vector<void *> param_at(count), average_at(count), square_at(count), copy_at(copies.empty() ? 0 : count), scale_at(scales.empty() ? 0 : count);
     std::vector<int64_t> sizes(count), grad_types(count), copy_types(copies.empty() ? 0 : count, -1);
     const bool recording = at::GradMode::is_enabled();
     for (size_t i = 0; i < count; i++) {
-        const at::Tensor &p = params[i], &g = grads[i];
-        if (!written(p, at::kFloat) || type_code(g.scalar_type()) < 0 || g.device() != like.device() || g.sizes() != p.sizes() || g.is_neg() ||
-            !g.is_contiguous() || !written(averages[i], state) || !written(squares[i], state) || averages[i].sizes() != p.sizes() ||
-            squares[i].sizes() != p.sizes() || (recording && p.requires_grad() && !p.is_leaf()))
+        const at::Tensor &p = *params[i], &g = *grads[i], &average = *averages[i], &square = *squares[i];
+        if (!written(p, at::kFloat) || type_code(g.scalar_type()) < 0 || g.device() != device || g.sizes() != p.sizes() || g.is_neg() ||
+            !g.is_contiguous() || !written(average, state) || !written(square, state) || average.sizes() != p.sizes() || square.sizes() != p.sizes() || (recording && p.requires_grad() && !p.is_leaf()))
             Py_RETURN_NONE;
         param_at[i] = target(p);
         grad_at[i] = address(g);
-        average_at[i] = target(averages[i]);
-        square_at[i] = target(squares[i]);
+        average_at[i] = target(average);
+        square_at[i] = target(square);
         sizes[i] = p.numel();
         grad_types[i] = type_code(g.scalar_type());
-        if (!copies.empty() && copies[i].defined()) {
-            const at::Tensor &t = copies[i];
+        if (!copies.empty() && copies[i]) {
+            const at::Tensor &t = *copies[i];
             if ((!written(t, at::kHalf) && !written(t, at::kBFloat16)) || t.sizes() != p.sizes()) Py_RETURN_NONE;
             copy_at[i] = target(t);
             copy_types[i] = type_code(t.scalar_type());
         }
         if (!scales.empty()) {
-            const at::Tensor &t = scales[i];
+            if (!scales[i]) Py_RETURN_NONE;
+            const at::Tensor &t = *scales[i];
             if (!written(t, at::kFloat) || t.dim() != 2 || t.size(0) != (p.numel() + 255) / 256 || t.size(1) != 2) Py_RETURN_NONE;
             scale_at[i] = target(t);
         }
         if (sizes[i] == 0) continue;
-        extents[0].push_back(extent(p, true));
-        extents[1].push_back(extent(averages[i], true));
-        extents[2].push_back(extent(squares[i], true));
-        extents[3].push_back(extent(g, false));
-        if (!scales.empty()) extents[4].push_back(extent(scales[i], true));
-        if (!copies.empty() && copies[i].defined()) extents[5].push_back(extent(copies[i], true));
+        const int64_t state_bytes = sizes[i] * (scales.empty() ? 4 : 1);
+        extents[0].push_back(extent(param_at[i], sizes[i] * 4, true));
+        extents[1].push_back(extent(average_at[i], state_bytes, true));
+        extents[2].push_back(extent(square_at[i], state_bytes, true));
+        extents[3].push_back(extent(grad_at[i], sizes[i] * (grad_types[i] == TG_TYPE_F32 ? 4 : 2), false));
+        if (!scales.empty()) extents[4].push_back(extent(scale_at[i], scales[i]->numel() * 4, true));
+        if (!copies.empty() && copies[i]) extents[5].push_back(extent(copy_at[i], sizes[i] * 2, true));
     }
     for (const at::Tensor *t : {&step, &rate, &grad_scale})
-        if (t->defined()) extents.push_back({extent(*t, false)});
+        if (t->defined()) extents.push_back({extent(address(*t), 4, false)});
     if (!apart(extents)) Py_RETURN_NONE;
     c.params = reinterpret_cast<float *const *>(param_at.data());
     c.grads = grad_at.data();
@@ -400,8 +408,8 @@ PyObject *py_adamw_step(PyObject *, PyObject *const *args, Py_ssize_t n) {
         c.stream = stream_of(like);
         check(operators.adamw_step(&c), "tg_adamw_step");
         for (const auto *list : {&params, &averages, &squares, &copies, &scales})
-            for (const at::Tensor &t : *list)
-                if (t.defined() && !t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+            for (const at::Tensor *t : *list)
+                if (t && !t->is_inference()) t->unsafeGetTensorImpl()->bump_version();
     }
     Py_RETURN_TRUE;
     END_HANDLE_TH_ERRORS
