@@ -15,18 +15,26 @@ __device__ __forceinline__ float sum_groups(float v) {
     return v + __shfl_xor(v, 32);
 }
 
-// LDS of the two kernels.  Each has 2 D / 16 waves: in the first half (`role` 0) those of one state, in the second those of the other, each wave sixteen columns.
-// With both states in every wave there were two waves a SIMD with 256 registers, a third of whose time was spent waiting for LDS.
-template <class T, int D> constexpr int kBackwardLds = 4 * Tile<Parts<T>::kInput, Parts<T>::kRows, D>::kBytes + 2 * (int)sizeof(Reach<Parts<T>::kRows>) + D / 16 * Parts<T>::kRows * 4;
+// The two kernels have twice the waves of a state: the first half (`role` 0) has one state, the second half the other.  LDS, and waves of a SIMD that
+// they are compiled for: two, with 256 registers, where LDS has room for one workgroup.
+//
+// W of State, 4 x 4096 rows of 16 heads of 128 in bfloat16, and 2 x 3000 of 8 in float32: the queries' kernel 178 and 84 us with one, 185 and 64 with
+// two; the keys' 245 and 139 with one, 185 and 76 with two.  8 x 2048 rows of 32 heads of 64: 128 and 134 with one, 180 and 150 with two.
+template <class T, int D> constexpr int kQueriesColumns = D > 64 && sizeof(T) == 4 ? 2 : 1;
+template <int D> constexpr int kKeysColumns = D > 64 ? 2 : 1;
+template <class T, int D> constexpr int kQueriesThreads = 2 * State<D, kQueriesColumns<T, D>>::kWaves * kWave;
+template <int D> constexpr int kKeysThreads = 2 * State<D, kKeysColumns<D>>::kWaves * kWave;
+template <class T, int D> constexpr int kBackwardLds = 4 * Tile<Parts<T>::kInput, Parts<T>::kRows, D>::kBytes + 2 * (int)sizeof(Reach<Parts<T>::kRows>) +
+                                                       D / 16 * Parts<T>::kRows * 4;
 template <class T> constexpr int kPairsLds = Tile<Parts<T>::kInput, Parts<T>::kRows, Parts<T>::kRows>::kBytes;
 template <class T, int D> constexpr int kQueriesLds = kBackwardLds<T, D> + kPairsLds<T> + 2 * Parts<T>::kRows / 16 * Parts<T>::kRows * 4;
 template <class T, int D> constexpr int kKeysLds = kBackwardLds<T, D> + 2 * kPairsLds<T>;
 
 // The chunks of a unit's tensors on their way to LDS.
-template <class T, int D, bool Vector> struct Four {
+template <class T, int D, int Threads, bool Vector> struct Four {
     static constexpr int R = Parts<T>::kRows, N = Parts<T>::kInput;
     const T *q, *k, *v, *g;
-    Incoming<T, R, D, 8 * D, Vector> next_q, next_k, next_v, next_g;
+    Incoming<T, R, D, Threads, Vector> next_q, next_k, next_v, next_g;
 
     __device__ __forceinline__ Four(const AttentionCall &c, const Unit &unit, int head) {
         const AttentionRows rows = rows_of(c.m, c.offsets, unit.sequence);
@@ -51,8 +59,8 @@ template <class T, int D, bool Vector> struct Four {
 };
 
 template <class T, int D, bool Vector>
-__global__ __launch_bounds__(8 * D, waves_of_simd(8 * D, kQueriesLds<T, D>)) void attention_grad_queries_kernel(AttentionCall c) {
-    constexpr int R = Parts<T>::kRows, N = Parts<T>::kInput, kTiles = R / 16, kWaves = D / 16;
+__global__ __launch_bounds__((kQueriesThreads<T, D>), (waves_of_simd(kQueriesThreads<T, D>, kQueriesLds<T, D>, kQueriesColumns<T, D> * D / 4))) void attention_grad_queries_kernel(AttentionCall c) {
+    constexpr int R = Parts<T>::kRows, N = Parts<T>::kInput, kTiles = R / 16, W = kQueriesColumns<T, D>, kWaves = State<D, W>::kWaves;
     using In = Tile<N, R, D>;
     using Pairs = Tile<N, R, R>;
     extern __shared__ __attribute__((aligned(16))) char lds[];
@@ -62,15 +70,15 @@ __global__ __launch_bounds__(8 * D, waves_of_simd(8 * D, kQueriesLds<T, D>)) voi
     float(*by_earlier)[R] = by_later + kTiles;        // by row r
     const int64_t u = blockIdx.x / c.m.heads;
     const int head = (int)(blockIdx.x % c.m.heads), wave = wave_of();
-    const int role = wave / kWaves, column = 16 * (wave % kWaves);
+    const int role = wave / kWaves, column = 16 * W * (wave % kWaves);
     const int64_t state_size = (int64_t)c.m.key_size * c.m.value_size;
     const Unit unit = unit_of<R>(c, u);
     if (!unit.there) return;
     // rows are values, columns keys: S, which the queries' gradients read, or what the unit adds to D
-    State<D> state;
+    State<D, W> state;
     state.template load<true>(role == 0 ? c.states + (u * c.m.heads + head) * state_size : nullptr, column, c.m.key_size, c.m.value_size);
     double before = 0.0;
-    Four<T, D, Vector> next(c, unit, head);
+    Four<T, D, kQueriesThreads<T, D>, Vector> next(c, unit, head);
     next.load(c, 0, unit.count);
     float gate = 0.0f;  // of the next chunk's row, in the first wave
     if (wave == 0) reach_of(c, reaches[0], gate_of_lane<T, R>(c, unit.first, unit.count, head), unit.count, before);
@@ -87,8 +95,12 @@ __global__ __launch_bounds__(8 * D, waves_of_simd(8 * D, kQueriesLds<T, D>)) voi
             if (wave == 0) gate = gate_of_lane<T, R>(c, unit.first + at + R, unit.count - at - R, head);
         }
         const Reach<R> &reach = reaches[turn];
+        // Pairs by all waves, or, with as many waves that the others have enough to do meanwhile, by those that add to D while those of S read it.
+        constexpr bool kApart = D > 64;
+        floatx4 read[kTiles][W] = {};
+        if (kApart && role == 0) state.template read_by<kWhole>(grads, read);
 #pragma unroll 1
-        for (int tile = wave; tile < kTiles * kTiles; tile += 2 * kWaves) {
+        for (int tile = !kApart ? wave : role == 0 ? kTiles * kTiles : wave - kWaves; tile < kTiles * kTiles; tile += kApart ? kWaves : 2 * kWaves) {
             const int s = tile / kTiles, r = tile % kTiles;
             floatx4 p = {0.0f, 0.0f, 0.0f, 0.0f}, d = p;
             if (r <= s) {
@@ -111,40 +123,58 @@ __global__ __launch_bounds__(8 * D, waves_of_simd(8 * D, kQueriesLds<T, D>)) voi
                 if (lane % 16 == 0) by_earlier[s][16 * r + 4 * (lane / 16) + j] = earlier;
             }
         }
+        if (!kApart && role == 0) state.template read_by<kWhole>(grads, read);
         __syncthreads();
         if (role == 0) {
-            floatx4 read[kTiles] = {};
-            state.template read_by<kWhole>(grads, read);
-            Operand<N> mine[R / 32];
+            Operand<N> mine[R / 32][W];
 #pragma unroll
-            for (int n = 0; n < R / 32; n++) mine[n] = keys.transposed(32 * n, column);
+            for (int n = 0; n < R / 32; n++)
+#pragma unroll
+                for (int w = 0; w < W; w++) mine[n][w] = keys.transposed(32 * n, column + 16 * w);
 #pragma unroll
             for (int s = 0; s < kTiles; s++) {
-                floatx4 o = read[s];
-                o *= reach.row[16 * s + lane % 16];
-                const floatx4 x = queries.numbers(16 * s + lane % 16, column + 4 * (lane / 16));
-                const float sum = sum_groups(o[0] * x[0] + o[1] * x[1] + o[2] * x[2] + o[3] * x[3]);
+                const float decay = reach.row[16 * s + lane % 16];
+                const int to = column + 4 * (lane / 16);
+                float sum = 0.0f;
+#pragma unroll
+                for (int w = 0; w < W; w++) {
+                    read[s][w] *= decay;
+                    const floatx4 x = queries.numbers(16 * s + lane % 16, to + 16 * w);
+#pragma unroll
+                    for (int j = 0; j < 4; j++) sum = fmaf(read[s][w][j], x[j], sum);
+                }
+                sum = sum_groups(sum);
                 if (lane < 16) by_wave[wave][16 * s + lane] = sum;
 #pragma unroll
                 for (int n = 0; n < R / 32; n++)
-                    if (2 * n <= s) o = product(mine[n], pairs.chained(16 * s, 32 * n), o);
+                    if (2 * n <= s) {
+                        const Operand<N> p = pairs.chained(16 * s, 32 * n);
+#pragma unroll
+                        for (int w = 0; w < W; w++) read[s][w] = product(mine[n][w], p, read[s][w]);
+                    }
                 in_order();
                 if (c.grad_queries && 16 * s + lane % 16 < unit.count - at) {
                     const int64_t base = ((unit.first + at + 16 * s) * c.m.heads + head) * c.m.key_size;
-                    const int to = column + 4 * (lane / 16);
                     const uint32_t offset = (uint32_t)(lane % 16 * c.m.heads * c.m.key_size + to);
-                    if (c.m.shared == 1)
-                        put_row((T *)c.grad_queries + base, offset, to, c.m.key_size, Vector, o);
-                    else
-                        put_row((float *)c.grad_queries + base, offset, to, c.m.key_size, Vector, o);
+#pragma unroll
+                    for (int w = 0; w < W; w++) {
+                        if (c.m.shared == 1)
+                            put_row((T *)c.grad_queries + base + 16 * w, offset, to + 16 * w, c.m.key_size, Vector, read[s][w]);
+                        else
+                            put_row((float *)c.grad_queries + base + 16 * w, offset, to + 16 * w, c.m.key_size, Vector, read[s][w]);
+                    }
                 }
             }
             state.times(reach.whole);
 #pragma unroll
-            for (int n = 0; n < R / 32; n++) state.add(values, 32 * n, weighted<kWhole>(mine[n], reach.column, 32 * n, lane));
-        } else {
+            for (int n = 0; n < R / 32; n++) {
+                Operand<kWhole> late[W];
 #pragma unroll
-            for (int n = 0; n < R / 32; n++) state.add(grads, 32 * n, weighted<kWhole>(queries.transposed(32 * n, column), reach.start, 32 * n, lane));
+                for (int w = 0; w < W; w++) late[w] = weighted<kWhole>(mine[n][w], reach.column, 32 * n, lane);
+                state.add(values, 32 * n, late);
+            }
+        } else {
+            state.template add_weighted<kWhole>(grads, queries, column, reach.start);
         }
         if (wave == 0 && at + R < unit.count) reach_of(c, reaches[turn ^ 1], gate, unit.count - at - R, before);
         __syncthreads();
@@ -162,8 +192,8 @@ __global__ __launch_bounds__(8 * D, waves_of_simd(8 * D, kQueriesLds<T, D>)) voi
 }
 
 template <class T, int D, bool Vector>
-__global__ __launch_bounds__(8 * D, waves_of_simd(8 * D, kKeysLds<T, D>)) void attention_grad_keys_kernel(AttentionCall c) {
-    constexpr int R = Parts<T>::kRows, N = Parts<T>::kInput, kTiles = R / 16, kWaves = D / 16;
+__global__ __launch_bounds__(kKeysThreads<D>, (waves_of_simd(kKeysThreads<D>, kKeysLds<T, D>, kKeysColumns<D> * D / 4))) void attention_grad_keys_kernel(AttentionCall c) {
+    constexpr int R = Parts<T>::kRows, N = Parts<T>::kInput, M = Parts<T>::kState, kTiles = R / 16, W = kKeysColumns<D>, kWaves = State<D, W>::kWaves;
     using In = Tile<N, R, D>;
     using Pairs = Tile<N, R, R>;
     extern __shared__ __attribute__((aligned(16))) char lds[];
@@ -171,11 +201,11 @@ __global__ __launch_bounds__(8 * D, waves_of_simd(8 * D, kKeysLds<T, D>)) void a
     float(*by_wave)[R] = (float(*)[R])(reaches + 2);  // k.dk without the chunk's own pairs, of each wave's columns
     const int64_t u = blockIdx.x / c.m.heads;
     const int head = (int)(blockIdx.x % c.m.heads), wave = wave_of();
-    const int role = wave / kWaves, column = 16 * (wave % kWaves);
+    const int role = wave / kWaves, column = 16 * W * (wave % kWaves);
     const int64_t state_size = (int64_t)c.m.key_size * c.m.value_size;
     const Unit unit = unit_of<R>(c, u);
     if (!unit.there || unit.count == 0) return;
-    State<D> state;  // D: rows are keys and columns values (role 0, the values' gradients), or the other way round
+    State<D, W> state;  // D: rows are keys and columns values (role 0, the values' gradients), or the other way round
     const float *behind = c.grad_states + (u * c.m.heads + head) * state_size;
     if (role == 0)
         state.template load<false>(behind, column, c.m.key_size, c.m.value_size);
@@ -184,7 +214,7 @@ __global__ __launch_bounds__(8 * D, waves_of_simd(8 * D, kKeysLds<T, D>)) void a
     void *const out = role ? c.grad_keys : c.grad_values;
     const int size = role ? c.m.key_size : c.m.value_size;
     double before = 0.0;
-    Four<T, D, Vector> next(c, unit, head);
+    Four<T, D, kKeysThreads<D>, Vector> next(c, unit, head);
     const int64_t last = (unit.count - 1) / R * R;
     next.load(c, last, unit.count - last);
     float gate = 0.0f;  // of the next chunk's row, in the first wave
@@ -221,42 +251,66 @@ __global__ __launch_bounds__(8 * D, waves_of_simd(8 * D, kKeysLds<T, D>)) void a
             scores.put(16 * r, 16 * s, p);
             pairs.put(16 * r, 16 * s, d);
         }
-        __syncthreads();
         // the same for both roles: what the state reads, what its transposed rows are added up with, and what of
         const In reading{(__bf16 *)(lds + (role ? 2 : 1) * In::kBytes), lane}, with{(__bf16 *)(lds + (role ? 0 : 3) * In::kBytes), lane},
             adding{(__bf16 *)(lds + (role ? 3 : 0) * In::kBytes), lane};
         const Pairs mine_of{(__bf16 *)(lds + 4 * In::kBytes + role * Pairs::kBytes), lane};
-        floatx4 read[kTiles] = {};
-        state.template read_by<kWhole>(reading, read);
-        Operand<N> mine[R / 32];
+        floatx4 read[kTiles][W] = {};
+        if (role)
+            state.template read_by<kWhole>(reading, read);
+        else
+            state.template read_by<M>(reading, read);
+        __syncthreads();
+        Operand<N> mine[R / 32][W];
 #pragma unroll
-        for (int n = 0; n < R / 32; n++) mine[n] = with.transposed(32 * n, column);
+        for (int n = 0; n < R / 32; n++)
+#pragma unroll
+            for (int w = 0; w < W; w++) mine[n][w] = with.transposed(32 * n, column + 16 * w);
 #pragma unroll
         for (int r = 0; r < kTiles; r++) {
-            floatx4 x = read[r];
-            x *= reach.column[16 * r + lane % 16];
+            const float decay = reach.column[16 * r + lane % 16];
             const int to = column + 4 * (lane / 16);
+#pragma unroll
+            for (int w = 0; w < W; w++) read[r][w] *= decay;
             if (role) {
-                const floatx4 k = keys.numbers(16 * r + lane % 16, to);
-                const float sum = sum_groups(x[0] * k[0] + x[1] * k[1] + x[2] * k[2] + x[3] * k[3]);
+                float sum = 0.0f;
+#pragma unroll
+                for (int w = 0; w < W; w++) {
+                    const floatx4 k = keys.numbers(16 * r + lane % 16, to + 16 * w);
+#pragma unroll
+                    for (int j = 0; j < 4; j++) sum = fmaf(read[r][w][j], k[j], sum);
+                }
+                sum = sum_groups(sum);
                 if (lane < 16) by_wave[wave - kWaves][16 * r + lane] = sum;
             }
 #pragma unroll
             for (int n = 0; n < R / 32; n++)
-                if (2 * n + 1 >= r) x = product(mine[n], mine_of.chained(16 * r, 32 * n), x);
+                if (2 * n + 1 >= r) {
+                    const Operand<N> p = mine_of.chained(16 * r, 32 * n);
+#pragma unroll
+                    for (int w = 0; w < W; w++) read[r][w] = product(mine[n][w], p, read[r][w]);
+                }
             in_order();
             if (out && 16 * r + lane % 16 < unit.count - at) {
                 const int64_t base = ((unit.first + at + 16 * r) * c.m.heads + head) * size;
                 const uint32_t offset = (uint32_t)(lane % 16 * c.m.heads * size + to);
-                if (!role || c.m.shared == 1)
-                    put_row((T *)out + base, offset, to, size, Vector, x);
-                else
-                    put_row((float *)out + base, offset, to, size, Vector, x);
+#pragma unroll
+                for (int w = 0; w < W; w++) {
+                    if (!role || c.m.shared == 1)
+                        put_row((T *)out + base + 16 * w, offset, to + 16 * w, size, Vector, read[r][w]);
+                    else
+                        put_row((float *)out + base + 16 * w, offset, to + 16 * w, size, Vector, read[r][w]);
+                }
             }
         }
         state.times(reach.whole);
 #pragma unroll
-        for (int n = 0; n < R / 32; n++) state.add(adding, 32 * n, weighted<kWhole>(mine[n], reach.row, 32 * n, lane));
+        for (int n = 0; n < R / 32; n++) {
+            Operand<kWhole> late[W];
+#pragma unroll
+            for (int w = 0; w < W; w++) late[w] = weighted<kWhole>(mine[n][w], reach.row, 32 * n, lane);
+            state.add(adding, 32 * n, late);
+        }
         if (wave == 0 && at > 0) reach_of(c, reaches[turn ^ 1], gate, R, before);
         __syncthreads();
         if (threadIdx.x < R && at + threadIdx.x < unit.count) {
@@ -280,9 +334,9 @@ int launch_attention_backward(int64_t type, const AttentionCall &c, int size, bo
         const int code = reserve_lds("tg_linear_attention_backward", kernel, for_keys ? kKeys : kQueries, reserved[for_keys]);
         if (code) return code;
         if (for_keys)
-            TG_LAUNCH_AS("attention_grad_keys", (attention_grad_keys_kernel<T, D, Vector>), grid, dim3(8 * D), kKeys, stream, c);
+            TG_LAUNCH_AS("attention_grad_keys", (attention_grad_keys_kernel<T, D, Vector>), grid, dim3(kKeysThreads<D>), kKeys, stream, c);
         else
-            TG_LAUNCH_AS("attention_grad_queries", (attention_grad_queries_kernel<T, D, Vector>), grid, dim3(8 * D), kQueries, stream, c);
+            TG_LAUNCH_AS("attention_grad_queries", (attention_grad_queries_kernel<T, D, Vector>), grid, dim3((kQueriesThreads<T, D>)), kQueries, stream, c);
         return 0;
     });
 }

@@ -189,10 +189,11 @@ template <class T, int Rows, int D, int Threads, bool Vector> struct Incoming {
     }
 };
 
-// Waves of a SIMD that kernels are compiled for: four (128 registers a lane) where a CU's 160 KB of LDS have room for as many workgroups.
-constexpr int waves_of_simd(int threads, int lds_bytes) {
-    const int groups = 160 * 1024 / lds_bytes, waves = groups * threads / kWave / 4;
-    return waves > 4 ? 4 : waves < 1 ? 1 : waves;
+// Waves of a SIMD that a kernel is compiled for: those of as many workgroups as a CU's 160 KB of LDS have room for, at most four (128 registers a
+// lane), or two for a state of 64 registers.
+constexpr int waves_of_simd(int threads, int lds_bytes, int state_registers) {
+    const int groups = 160 * 1024 / lds_bytes, waves = groups * threads / kWave / 4, most = state_registers > 32 ? 2 : 4;
+    return waves > most ? most : waves < 1 ? 1 : waves;
 }
 
 // Decays of a chunk.
@@ -339,52 +340,79 @@ __device__ __forceinline__ int lane_of_turn() {
 // Keeps the compiler from reading ahead over this point: operands of a whole chunk, read at its beginning, would not fit the registers.
 __device__ __forceinline__ void in_order() { __builtin_amdgcn_sched_barrier(0); }
 
-// The state in accumulators: rows of keys and columns of values (Turned: the other way round), of a wave the sixteen columns from `column` on.
-template <int D> struct State {
-    floatx4 x[D / 16];
+// The state in accumulators: rows of keys and columns of values (Turned: the other way round), of a wave the 16 W columns from `column` on.  With W = 2 an
+// operand from LDS goes into twice as many products, with W = 1 twice as many waves hide each other's latencies.
+template <int D, int W> struct State {
+    static constexpr int kWaves = D / (16 * W);
+    floatx4 x[W][D / 16];
 
-    // call(n, j, the place of x[n][j]) for all that are there.  One offset of a lane and a uniform one beside it, which is not kept over a loop: 32
-    // addresses would be.
+    // call(w, n, j, the place of x[w][n][j]) for all that are there, with one offset of a lane and a uniform one beside it.
     template <bool Turned, class Call> __device__ __forceinline__ void each(int column, int key_size, int value_size, Call &&call) {
-        const int lane = lane_of_turn(), across = column + lane % 16, down = 4 * (lane / 16);
-        const int most = Turned ? value_size : key_size, offset = Turned ? across * value_size + down : down * value_size + across;
-        if (across >= (Turned ? key_size : value_size)) return;
+        const int lane = lane_of_turn();
 #pragma unroll
-        for (int n = 0; n < D / 16; n++)
+        for (int w = 0; w < W; w++) {
+            const int across = column + 16 * w + lane % 16, down = 4 * (lane / 16);
+            const int most = Turned ? value_size : key_size, offset = Turned ? across * value_size + down : down * value_size + across;
+            if (across < (Turned ? key_size : value_size)) {
 #pragma unroll
-            for (int j = 0; j < 4; j++)
-                if (down + 16 * n + j < most) call(n, j, offset + (Turned ? 16 * n + j : (16 * n + j) * value_size));
-    }
-    template <bool Turned> __device__ __forceinline__ void load(const float *from, int column, int key_size, int value_size) {
+                for (int n = 0; n < D / 16; n++)
 #pragma unroll
-        for (int n = 0; n < D / 16; n++) x[n] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
-        if (from) each<Turned>(column, key_size, value_size, [&](int n, int j, int at) { x[n][j] = from[at]; });
-    }
-    template <bool Turned> __device__ __forceinline__ void store(float *to, int column, int key_size, int value_size) {
-        each<Turned>(column, key_size, value_size, [&](int n, int j, int at) { to[at] = x[n][j]; });
-    }
-    __device__ __forceinline__ void times(float a) {
-#pragma unroll
-        for (int n = 0; n < D / 16; n++) x[n] *= a;
-    }
-    // Adds its transpose times the rows' columns to `sums`, one of sixteen rows of the tile each.
-    template <int M, int N, int Rows> __device__ __forceinline__ void read_by(const Tile<N, Rows, D> &tile, floatx4 *sums) const {
-#pragma unroll
-        for (int i = 0; i < D / 32; i++) {
-            const Operand<M> mine = operand_of<M>(x[2 * i], x[2 * i + 1]);
-#pragma unroll
-            for (int r = 0; r < Rows / 16; r++) {
-                sums[r] = product(mine, tile.chained(16 * r, 32 * i), sums[r]);
-                if (r % 2 == 1) in_order();
+                    for (int j = 0; j < 4; j++)
+                        if (down + 16 * n + j < most) call(w, n, j, offset + (Turned ? 16 * n + j : (16 * n + j) * value_size));
             }
         }
     }
+    template <bool Turned> __device__ __forceinline__ void load(const float *from, int column, int key_size, int value_size) {
+#pragma unroll
+        for (int w = 0; w < W; w++)
+#pragma unroll
+            for (int n = 0; n < D / 16; n++) x[w][n] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
+        if (from) each<Turned>(column, key_size, value_size, [&](int w, int n, int j, int at) { x[w][n][j] = from[at]; });
+    }
+    template <bool Turned> __device__ __forceinline__ void store(float *to, int column, int key_size, int value_size) {
+        each<Turned>(column, key_size, value_size, [&](int w, int n, int j, int at) { to[at] = x[w][n][j]; });
+    }
+    __device__ __forceinline__ void times(float a) {
+#pragma unroll
+        for (int w = 0; w < W; w++)
+#pragma unroll
+            for (int n = 0; n < D / 16; n++) x[w][n] *= a;
+    }
+    // Adds its transpose times the rows' columns to `sums`, by sixteen rows of the tile.
+    template <int M, int N, int Rows> __device__ __forceinline__ void read_by(const Tile<N, Rows, D> &tile, floatx4 (&sums)[Rows / 16][W]) const {
+#pragma unroll
+        for (int i = 0; i < D / 32; i++) {
+            Operand<M> mine[W];
+#pragma unroll
+            for (int w = 0; w < W; w++) mine[w] = operand_of<M>(x[w][2 * i], x[w][2 * i + 1]);
+#pragma unroll
+            for (int r = 0; r < Rows / 16; r++) {
+                const Operand<N> theirs = tile.chained(16 * r, 32 * i);
+#pragma unroll
+                for (int w = 0; w < W; w++) sums[r][w] = product(mine[w], theirs, sums[r][w]);
+            }
+            in_order();
+        }
+    }
     // += 32 rows of the tile, transposed, times this wave's columns of as many rows
-    template <int N, int M, int Rows> __device__ __forceinline__ void add(const Tile<N, Rows, D> &tile, int row, const Operand<M> &columns) {
+    template <int N, int M, int Rows> __device__ __forceinline__ void add(const Tile<N, Rows, D> &tile, int row, const Operand<M> (&columns)[W]) {
 #pragma unroll
         for (int n = 0; n < D / 16; n++) {
-            x[n] = product(tile.transposed(row, 16 * n), columns, x[n]);
+            const Operand<N> theirs = tile.transposed(row, 16 * n);
+#pragma unroll
+            for (int w = 0; w < W; w++) x[w][n] = product(theirs, columns[w], x[w][n]);
             if (n % 4 == 3) in_order();
+        }
+    }
+    // ... of this wave's columns of the tile `with`, its rows weighted
+    template <int M, int N, int Rows>
+    __device__ __forceinline__ void add_weighted(const Tile<N, Rows, D> &tile, const Tile<N, Rows, D> &with, int column, const float *weights) {
+#pragma unroll
+        for (int k = 0; k < Rows; k += 32) {
+            Operand<M> mine[W];
+#pragma unroll
+            for (int w = 0; w < W; w++) mine[w] = weighted<M>(with.transposed(k, column + 16 * w), weights, k, tile.lane);
+            add(tile, k, mine);
         }
     }
 };

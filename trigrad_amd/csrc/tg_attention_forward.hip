@@ -7,23 +7,26 @@ namespace tg {
 template <class T, int D> constexpr int kStatesLds = 2 * Tile<Parts<T>::kInput, Parts<T>::kRows, D>::kBytes + 2 * (int)sizeof(Reach<Parts<T>::kRows>);
 template <class T, int D> constexpr int kOutputsLds = 3 * Tile<Parts<T>::kInput, Parts<T>::kRows, D>::kBytes +
                                                       Tile<Parts<T>::kInput, Parts<T>::kRows, Parts<T>::kRows>::kBytes + 2 * (int)sizeof(Reach<Parts<T>::kRows>);
+constexpr int W = 1;  // see State
+template <int D> constexpr int kThreads = State<D, W>::kWaves * kWave;
 
 // What a unit adds to the state, and its decay.  A chunk is on its way from memory while the one before is computed on.
 template <class T, int D, bool Vector>
-__global__ __launch_bounds__(4 * D, waves_of_simd(4 * D, kStatesLds<T, D>)) void attention_states_kernel(AttentionCall c) {
+__global__ __launch_bounds__(kThreads<D>, waves_of_simd(kThreads<D>, kStatesLds<T, D>, W * D / 4)) void attention_states_kernel(AttentionCall c) {
     constexpr int R = Parts<T>::kRows, N = Parts<T>::kInput;
-    __shared__ __attribute__((aligned(16))) __bf16 lds[(Tile<N, R, D>::kBytes * 2) / 2];
+    using In = Tile<N, R, D>;
+    __shared__ __attribute__((aligned(16))) __bf16 lds[In::kBytes];
     __shared__ Reach<R> reaches[2];
     const int64_t u = blockIdx.x / c.m.heads;
-    const int head = (int)(blockIdx.x % c.m.heads), wave = wave_of(), column = 16 * wave;
+    const int head = (int)(blockIdx.x % c.m.heads), wave = wave_of(), column = 16 * W * wave;
     const Unit unit = unit_of<R>(c, u);
     if (!unit.there) return;
     const AttentionRows rows = rows_of(c.m, c.offsets, unit.sequence);
     const T *k = (const T *)c.keys + place_of(c.m, c.m.k, unit.sequence, rows.first, head / c.m.shared) + unit.base * c.m.k.row,
             *v = (const T *)c.values + place_of(c.m, c.m.v, unit.sequence, rows.first, head) + unit.base * c.m.v.row;
-    State<D> state = {};
+    State<D, W> state = {};
     double before = 0.0;
-    Incoming<T, R, D, 4 * D, Vector> next_k, next_v;
+    Incoming<T, R, D, kThreads<D>, Vector> next_k, next_v;
     next_k.load(k, c.m.k.row, unit.count, c.m.key_size);
     next_v.load(v, c.m.v.row, unit.count, c.m.value_size);
     float gate = 0.0f;  // of the next chunk's row, in the first wave
@@ -31,7 +34,7 @@ __global__ __launch_bounds__(4 * D, waves_of_simd(4 * D, kStatesLds<T, D>)) void
     int turn = 0;
     for (int64_t at = 0; at < unit.count; at += R, turn ^= 1) {
         const int lane = lane_of_turn();
-        const Tile<N, R, D> keys{lds, lane}, values{lds + Tile<N, R, D>::kBytes / 2, lane};
+        const In keys{lds, lane}, values{lds + In::kBytes / 2, lane};
         next_k.store(keys, unit.count - at, c.m.key_size);
         next_v.store(values, unit.count - at, c.m.value_size);
         __syncthreads();
@@ -41,8 +44,7 @@ __global__ __launch_bounds__(4 * D, waves_of_simd(4 * D, kStatesLds<T, D>)) void
             if (wave == 0) gate = gate_of_lane<T, R>(c, unit.first + at + R, unit.count - at - R, head);
         }
         state.times(reaches[turn].whole);
-#pragma unroll
-        for (int n = 0; n < R / 32; n++) state.add(keys, 32 * n, weighted<kWhole>(values.transposed(32 * n, column), reaches[turn].column, 32 * n, lane));
+        state.template add_weighted<kWhole>(keys, values, column, reaches[turn].column);
         if (wave == 0 && at + R < unit.count) reach_of(c, reaches[turn ^ 1], gate, unit.count - at - R, before);
         __syncthreads();
     }
@@ -51,14 +53,14 @@ __global__ __launch_bounds__(4 * D, waves_of_simd(4 * D, kStatesLds<T, D>)) void
 }
 
 template <class T, int D, bool Vector>
-__global__ __launch_bounds__(4 * D, waves_of_simd(4 * D, kOutputsLds<T, D>)) void attention_outputs_kernel(AttentionCall c) {
-    constexpr int R = Parts<T>::kRows, N = Parts<T>::kInput, M = Parts<T>::kState, kTiles = R / 16, kWaves = D / 16;
+__global__ __launch_bounds__(kThreads<D>, waves_of_simd(kThreads<D>, kOutputsLds<T, D>, W * D / 4)) void attention_outputs_kernel(AttentionCall c) {
+    constexpr int R = Parts<T>::kRows, N = Parts<T>::kInput, M = Parts<T>::kState, kTiles = R / 16, kWaves = State<D, W>::kWaves;
     using In = Tile<N, R, D>;
     using Pairs = Tile<N, R, R>;
     extern __shared__ __attribute__((aligned(16))) char lds[];
     Reach<R> *reaches = (Reach<R> *)(lds + 3 * In::kBytes + Pairs::kBytes);
     const int64_t which = blockIdx.x / c.m.heads;  // a unit, or a sequence
-    const int head = (int)(blockIdx.x % c.m.heads), wave = wave_of(), column = 16 * wave;
+    const int head = (int)(blockIdx.x % c.m.heads), wave = wave_of(), column = 16 * W * wave;
     const int64_t state_size = (int64_t)c.m.key_size * c.m.value_size;
     Unit unit;
     int64_t u = which;
@@ -76,12 +78,12 @@ __global__ __launch_bounds__(4 * D, waves_of_simd(4 * D, kOutputsLds<T, D>)) voi
             *v = (const T *)c.values + place_of(c.m, c.m.v, unit.sequence, rows.first, head) + unit.base * c.m.v.row;
     T *out = (T *)c.outputs + (unit.first * c.m.heads + head) * c.m.value_size;
     const int64_t out_row = (int64_t)c.m.heads * c.m.value_size;
-    State<D> state;
+    State<D, W> state;
     const float *start = c.through ? (c.initial ? c.initial + (unit.sequence * c.m.heads + head) * state_size : nullptr)
                                    : c.states + (u * c.m.heads + head) * state_size;
     state.template load<false>(start, column, c.m.key_size, c.m.value_size);
     double before = 0.0;
-    Incoming<T, R, D, 4 * D, Vector> next_q, next_k, next_v;
+    Incoming<T, R, D, kThreads<D>, Vector> next_q, next_k, next_v;
     const auto load = [&](int64_t at) {
         const int64_t left = unit.count - at;
         next_q.load(q + at * c.m.q.row, c.m.q.row, left, c.m.key_size);
@@ -112,9 +114,9 @@ __global__ __launch_bounds__(4 * D, waves_of_simd(4 * D, kOutputsLds<T, D>)) voi
         const Reach<R> &reach = reaches[turn];
         // pairs: row s, column r
 #pragma unroll 1
-        for (int n = 0; n < (kTiles * kTiles + kWaves - 1) / kWaves; n++) {
-            const int tile = wave + n * kWaves, s = tile / kTiles, r = tile % kTiles;
-            if (tile >= kTiles * kTiles || r > (s | 1)) continue;
+        for (int tile = wave; tile < kTiles * kTiles; tile += kWaves) {
+            const int s = tile / kTiles, r = tile % kTiles;
+            if (r > (s | 1)) continue;
             floatx4 p = {0.0f, 0.0f, 0.0f, 0.0f};
             if (r <= s) {
 #pragma unroll
@@ -123,27 +125,42 @@ __global__ __launch_bounds__(4 * D, waves_of_simd(4 * D, kOutputsLds<T, D>)) voi
             }
             pairs.put(16 * s, 16 * r, p);
         }
-        floatx4 read[kTiles] = {};
+        floatx4 read[kTiles][W] = {};
         state.template read_by<M>(queries, read);
         __syncthreads();
-        Operand<N> mine[R / 32];
+        Operand<N> mine[R / 32][W];
 #pragma unroll
-        for (int n = 0; n < R / 32; n++) mine[n] = values.transposed(32 * n, column);
+        for (int n = 0; n < R / 32; n++)
+#pragma unroll
+            for (int w = 0; w < W; w++) mine[n][w] = values.transposed(32 * n, column + 16 * w);
 #pragma unroll
         for (int s = 0; s < kTiles; s++) {
-            floatx4 o = read[s];
-            o *= reach.row[16 * s + lane % 16];
+            const float decay = reach.row[16 * s + lane % 16];
+#pragma unroll
+            for (int w = 0; w < W; w++) read[s][w] *= decay;
 #pragma unroll
             for (int n = 0; n < R / 32; n++)
-                if (2 * n <= s) o = product(mine[n], pairs.chained(16 * s, 32 * n), o);
+                if (2 * n <= s) {
+                    const Operand<N> p = pairs.chained(16 * s, 32 * n);
+#pragma unroll
+                    for (int w = 0; w < W; w++) read[s][w] = product(mine[n][w], p, read[s][w]);
+                }
             in_order();
             const int to = column + 4 * (lane / 16);
-            if (16 * s + lane % 16 < unit.count - at)
-                put_row(out + (at + 16 * s) * out_row, (uint32_t)(lane % 16 * (int)out_row + to), to, c.m.value_size, Vector, o);
+            if (16 * s + lane % 16 < unit.count - at) {
+#pragma unroll
+                for (int w = 0; w < W; w++)
+                    put_row(out + (at + 16 * s) * out_row + 16 * w, (uint32_t)(lane % 16 * (int)out_row + to), to + 16 * w, c.m.value_size, Vector, read[s][w]);
+            }
         }
         state.times(reach.whole);
 #pragma unroll
-        for (int n = 0; n < R / 32; n++) state.add(keys, 32 * n, weighted<kWhole>(mine[n], reach.column, 32 * n, lane));
+        for (int n = 0; n < R / 32; n++) {
+            Operand<kWhole> late[W];
+#pragma unroll
+            for (int w = 0; w < W; w++) late[w] = weighted<kWhole>(mine[n][w], reach.column, 32 * n, lane);
+            state.add(keys, 32 * n, late);
+        }
         if (wave == 0 && at + R < unit.count) reach_of(c, reaches[turn ^ 1], gate, unit.count - at - R, before);
         __syncthreads();
     }
@@ -157,14 +174,14 @@ int launch_attention_forward(int64_t type, const AttentionCall &c, int size, boo
         constexpr bool Vector = decltype(vector)::value;
         const dim3 grid((unsigned)((c.through ? c.m.sequences : c.most_units) * c.m.heads));
         if (states_only) {
-            TG_LAUNCH_AS("attention_states", (attention_states_kernel<T, D, Vector>), grid, dim3(4 * D), 0, stream, c);
+            TG_LAUNCH_AS("attention_states", (attention_states_kernel<T, D, Vector>), grid, dim3(kThreads<D>), 0, stream, c);
             return 0;
         }
         constexpr int kBytes = kOutputsLds<T, D>;
         static size_t reserved[kMaxDevices];
         const int code = reserve_lds("tg_linear_attention_forward", (const void *)attention_outputs_kernel<T, D, Vector>, kBytes, reserved);
         if (code) return code;
-        TG_LAUNCH_AS("attention_outputs", (attention_outputs_kernel<T, D, Vector>), grid, dim3(4 * D), kBytes, stream, c);
+        TG_LAUNCH_AS("attention_outputs", (attention_outputs_kernel<T, D, Vector>), grid, dim3(kThreads<D>), kBytes, stream, c);
         return 0;
     });
 }
