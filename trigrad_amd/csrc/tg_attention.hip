@@ -238,7 +238,20 @@ template <class S> __global__ __launch_bounds__(kScanThreads) void attention_gat
     const float *gradient = unit.index > 0 ? c.grad_states + ((u - 1) * c.m.heads + head) * size : in_front ? in_front + (unit.sequence * c.m.heads + head) * size : nullptr;
     if (gradient) {
         const float *state = c.states + (u * c.m.heads + head) * size;
-        for (int64_t i = threadIdx.x; i < size; i += kScanThreads) product += (double)state[i] * (double)gradient[i];
+        // eight products are added in float32, all others in 64 bits
+#pragma unroll 2
+        for (int64_t first = threadIdx.x; first < size; first += 8 * kScanThreads) {
+            float x[8], y[8], sum = 0.0f;
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
+                const int64_t at = min(first + j * kScanThreads, size - 1);
+                x[j] = state[at];
+                y[j] = gradient[at];
+            }
+#pragma unroll
+            for (int j = 0; j < 8; j++) sum = first + j * kScanThreads < size ? fmaf(x[j], y[j], sum) : sum;
+            product += (double)sum;
+        }
     }
     over_waves(sum_lanes(product, kWave), all);
     double log_a = all;  // of the first row
@@ -431,12 +444,12 @@ static int split_of(const char *fn, const tg_attention &a, const Attention &m, S
     s.size = std::max(m.key_size, m.value_size) <= 32 ? 32 : std::max(m.key_size, m.value_size) <= 64 ? 64 : 128;
     const int64_t of_one = ceil_div64(m.length, s.rows_of_chunk);
     s.chunks = 0;
-    // Chunks of a unit: a compute unit takes its units one after another, and a unit, whose state is written and read, as long as its chunks and one
-    // more (two of half the rows).  2 x 3000 rows of 8 heads in float32: six chunks, 256 units, 290 us forward and backward; five, 304 units, 404.
+    // Chunks of a unit: a compute unit takes its units one after another, and a unit, whose state is written and read, as long as its chunks and two
+    // more (four of half the rows).  2 x 3000 rows of 8 heads in float32: six chunks, 256 units, 290 us forward and backward; five, 304 units, 404.
     int64_t least = 0;
     for (int64_t n = std::max<int64_t>(1, ceil_div64(of_one, kMostUnits)), most = std::max(n, kMostChunks); n <= most; n++) {
         const int64_t units = (m.packed ? of_one / n + m.sequences : ceil_div64(of_one, n) * m.sequences) * m.heads;
-        const int64_t time = ceil_div64(units, kComputeUnits) * (n + 64 / s.rows_of_chunk);
+        const int64_t time = ceil_div64(units, kComputeUnits) * (n + 128 / s.rows_of_chunk);
         if (s.chunks == 0 || time < least) {
             s.chunks = n;
             least = time;
