@@ -336,7 +336,7 @@ int attention_shape(const char *fn, const tg_attention &a, Attention &m) {
     const auto strides = [](const int64_t s[3]) { return Strides{s[0], s[1], s[2]}; };
     m = {a.sequences, a.length, rows, (int)a.heads, (int)a.key_heads, (int)(a.heads / a.key_heads), (int)a.key_size, (int)a.value_size,
          strides(a.query_strides), strides(a.key_strides), strides(a.value_strides), strides(a.grad_strides),
-         (int)a.gate_form, a.fixed_gates != 0, a.offsets != nullptr, (float)a.scale};
+         (int)a.gate_form, a.fixed_gates != 0, a.offsets != nullptr, (real)a.scale};
     return 0;
 }
 
@@ -713,6 +713,17 @@ extern "C" int tg_linear_attention_sizes(const tg_attention *a, int64_t out[4]) 
     return code ? code : sizes_of(fn, *a, m, out);
 }
 
+// A fixed decay has a gradient of zero then.
+static int no_sequences(const tg_attention &a, const Attention &m) {
+    if (!m.fixed || !a.grad_gates) return 0;
+    return by_types(a.type, a.gate_type, [&](auto, auto s) {
+        using S = decltype(s);
+        TG_LAUNCH_AS("attention_fixed_gates", (attention_fixed_gates_kernel<S>), dim3((unsigned)m.heads), dim3(kWalkThreads), 0, (hipStream_t)a.stream, m,
+                     (const S *)a.gates, (const double *)nullptr, (int64_t)0, (S *)a.grad_gates);
+        return check_launch("tg_linear_attention_backward");
+    });
+}
+
 static int attention_call(const char *fn, const tg_attention *a, bool backward_pass) {
     if (!a) return check_pointers(fn, {a});
     Attention m;
@@ -733,7 +744,7 @@ static int attention_call(const char *fn, const tg_attention *a, bool backward_p
         set_error("%s: workspace of %lld bytes, %lld needed", fn, (long long)a->workspace_bytes, (long long)room);
         return TG_E_WORKSPACE;
     }
-    if (m.sequences == 0) return 0;
+    if (m.sequences == 0) return backward_pass ? no_sequences(*a, m) : 0;
     return backward_pass ? backward(*a, m) : forward(*a, m);
 }
 

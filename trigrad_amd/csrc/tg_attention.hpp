@@ -15,7 +15,7 @@ struct Attention {
     Strides q, k, v, g;
     int gate_form;
     bool fixed, packed;
-    float scale;
+    real scale;
 };
 
 // The rows of a sequence: `first` counts as the outputs' rows do.
