@@ -429,6 +429,7 @@ static int backward(const tg_attention &a, const Attention &m) { return walk_bac
 
 #else
 
+static_assert(Parts<bf16_t>::kRows == Parts<half_t>::kRows, "rows of a chunk");
 constexpr int64_t kComputeUnits = 256;
 constexpr int64_t kMostChunks = 16;   // of a unit: 1024 rows, beside whose 16 chunks a state that is written and read is little
 constexpr int64_t kMostUnits = 1024;  // of a sequence, which are gone through one after another
@@ -440,7 +441,7 @@ struct Split {
     bool through;
 };
 static int split_of(const char *fn, const tg_attention &a, const Attention &m, Split &s) {
-    s.rows_of_chunk = a.type == TG_TYPE_BF16 ? 64 : 32;
+    s.rows_of_chunk = a.type == TG_TYPE_F32 ? Parts<float>::kRows : Parts<bf16_t>::kRows;
     s.size = std::max(m.key_size, m.value_size) <= 32 ? 32 : std::max(m.key_size, m.value_size) <= 64 ? 64 : 128;
     const int64_t of_one = ceil_div64(m.length, s.rows_of_chunk);
     s.chunks = 0;

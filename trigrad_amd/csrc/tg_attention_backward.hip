@@ -24,9 +24,9 @@ template <class T, int D> constexpr int kQueriesColumns = D > 64 && sizeof(T) ==
 template <int D> constexpr int kKeysColumns = D > 64 ? 2 : 1;
 template <class T, int D> constexpr int kQueriesThreads = 2 * State<D, kQueriesColumns<T, D>>::kWaves * kWave;
 template <int D> constexpr int kKeysThreads = 2 * State<D, kKeysColumns<D>>::kWaves * kWave;
-template <class T, int D> constexpr int kBackwardLds = 4 * Tile<Parts<T>::kInput, Parts<T>::kRows, D>::kBytes + 2 * (int)sizeof(Reach<Parts<T>::kRows>) +
+template <class T, int D> constexpr int kBackwardLds = 4 * Tile<typename Parts<T>::Element, Parts<T>::kInput, Parts<T>::kRows, D>::kBytes + 2 * (int)sizeof(Reach<Parts<T>::kRows>) +
                                                        D / 16 * Parts<T>::kRows * 4;
-template <class T> constexpr int kPairsLds = Tile<Parts<T>::kInput, Parts<T>::kRows, Parts<T>::kRows>::kBytes;
+template <class T> constexpr int kPairsLds = Tile<typename Parts<T>::Element, Parts<T>::kInput, Parts<T>::kRows, Parts<T>::kRows>::kBytes;
 template <class T, int D> constexpr int kQueriesLds = kBackwardLds<T, D> + kPairsLds<T> + 2 * Parts<T>::kRows / 16 * Parts<T>::kRows * 4;
 template <class T, int D> constexpr int kKeysLds = kBackwardLds<T, D> + 2 * kPairsLds<T>;
 
@@ -49,20 +49,23 @@ template <class T, int D, int Threads, bool Vector> struct Four {
         next_v.load(v + at * c.m.v.row, c.m.v.row, left, c.m.value_size);
         next_g.load(g + at * c.m.g.row, c.m.g.row, left, c.m.value_size);
     }
-    __device__ __forceinline__ void store(const AttentionCall &c, const Tile<N, R, D> &queries, const Tile<N, R, D> &keys, const Tile<N, R, D> &values,
-                                          const Tile<N, R, D> &grads, int64_t left) const {
-        next_q.store(queries, left, c.m.key_size);
-        next_k.store(keys, left, c.m.key_size);
-        next_v.store(values, left, c.m.value_size);
-        next_g.store(grads, c.grad_outputs_there ? left : 0, c.m.value_size);
+    template <class Tile> __device__ __forceinline__ void store(const AttentionCall &c, const Tile &queries, const Tile &keys, const Tile &values, const Tile &grads,
+                                                                int64_t left, Reach<R> &reach) const {
+        using E = typename Parts<T>::Element;
+        constexpr bool kScaled = Parts<T>::kScaled;
+        next_q.template store<E, N, kScaled>(queries, left, c.m.key_size, &reach.largest[0]);
+        next_k.template store<E, N, kScaled>(keys, left, c.m.key_size, &reach.largest[1]);
+        next_v.template store<E, N, kScaled>(values, left, c.m.value_size, &reach.largest[2]);
+        next_g.template store<E, N, kScaled>(grads, c.grad_outputs_there ? left : 0, c.m.value_size, &reach.largest[3]);
     }
 };
 
 template <class T, int D, bool Vector>
 __global__ __launch_bounds__((kQueriesThreads<T, D>), (waves_of_simd(kQueriesThreads<T, D>, kQueriesLds<T, D>, kQueriesColumns<T, D> * D / 4))) void attention_grad_queries_kernel(AttentionCall c) {
     constexpr int R = Parts<T>::kRows, N = Parts<T>::kInput, kTiles = R / 16, W = kQueriesColumns<T, D>, kWaves = State<D, W>::kWaves;
-    using In = Tile<N, R, D>;
-    using Pairs = Tile<N, R, R>;
+    using E = typename Parts<T>::Element;
+    using In = Tile<E, N, R, D>;
+    using Pairs = Tile<E, N, R, R>;
     extern __shared__ __attribute__((aligned(16))) char lds[];
     Reach<R> *reaches = (Reach<R> *)(lds + 4 * In::kBytes + Pairs::kBytes);
     float(*by_wave)[R] = (float(*)[R])(reaches + 2);  // q.dq without the chunk's own pairs, of each wave's columns
@@ -82,14 +85,19 @@ __global__ __launch_bounds__((kQueriesThreads<T, D>), (waves_of_simd(kQueriesThr
     next.load(c, 0, unit.count);
     float gate = 0.0f;  // of the next chunk's row, in the first wave
     if (wave == 0) reach_of(c, reaches[0], gate_of_lane<T, R>(c, unit.first, unit.count, head), unit.count, before);
+    if (Parts<T>::kScaled) {
+        if (threadIdx.x < 4) reaches[0].largest[threadIdx.x] = 0;
+        __syncthreads();
+    }
     int turn = 0;
     for (int64_t at = 0; at < unit.count; at += R, turn ^= 1) {
         const int lane = lane_of_turn();
-        const In queries{(__bf16 *)lds, lane}, keys{(__bf16 *)(lds + In::kBytes), lane}, values{(__bf16 *)(lds + 2 * In::kBytes), lane},
-            grads{(__bf16 *)(lds + 3 * In::kBytes), lane};
-        const Pairs pairs{(__bf16 *)(lds + 4 * In::kBytes), lane};
-        next.store(c, queries, keys, values, grads, unit.count - at);
+        const In queries{(E *)lds, lane}, keys{(E *)(lds + In::kBytes), lane}, values{(E *)(lds + 2 * In::kBytes), lane},
+            grads{(E *)(lds + 3 * In::kBytes), lane};
+        const Pairs pairs{(E *)(lds + 4 * In::kBytes), lane};
+        next.store(c, queries, keys, values, grads, unit.count - at, reaches[turn]);
         __syncthreads();
+        if (Parts<T>::kScaled && threadIdx.x < 4) reaches[turn ^ 1].largest[threadIdx.x] = 0;
         if (at + R < unit.count) {
             next.load(c, at + R, unit.count - at - R);
             if (wave == 0) gate = gate_of_lane<T, R>(c, unit.first + at + R, unit.count - at - R, head);
@@ -98,7 +106,9 @@ __global__ __launch_bounds__((kQueriesThreads<T, D>), (waves_of_simd(kQueriesThr
         // Pairs by all waves, or, with as many waves that the others have enough to do meanwhile, by those that add to D while those of S read it.
         constexpr bool kApart = D > 64;
         floatx4 read[kTiles][W] = {};
-        if (kApart && role == 0) state.template read_by<kWhole>(grads, read);
+        float down = 1.0f;
+        if (kApart && role == 0) down = state.template read_by<T, Parts<T>::kWhole>(grads, read);
+        const Scaling scaling = scaling_of_pairs<T>(reach, 2, 3, c.m.value_size, c.m.scale);
 #pragma unroll 1
         for (int tile = !kApart ? wave : role == 0 ? kTiles * kTiles : wave - kWaves; tile < kTiles * kTiles; tile += kApart ? kWaves : 2 * kWaves) {
             const int s = tile / kTiles, r = tile % kTiles;
@@ -114,6 +124,7 @@ __global__ __launch_bounds__((kQueriesThreads<T, D>), (waves_of_simd(kQueriesThr
 #pragma unroll
                 for (int j = 0; j < 4; j++) p[j] = 16 * s + lane % 16 > 16 * r + 4 * (lane / 16) + j ? p[j] * d[j] : 0.0f;
             }
+            if (Parts<T>::kScaled) d *= scaling.up;
             if (r <= (s | 1)) pairs.put(16 * s, 16 * r, d);
             const float later = sum_groups(p[0] + p[1] + p[2] + p[3]);
             if (lane < 16) by_later[r][16 * s + lane] = later;
@@ -123,17 +134,14 @@ __global__ __launch_bounds__((kQueriesThreads<T, D>), (waves_of_simd(kQueriesThr
                 if (lane % 16 == 0) by_earlier[s][16 * r + 4 * (lane / 16) + j] = earlier;
             }
         }
-        if (!kApart && role == 0) state.template read_by<kWhole>(grads, read);
+        if (!kApart && role == 0) down = state.template read_by<T, Parts<T>::kWhole>(grads, read);
         __syncthreads();
+        Operand<E, N> mine[R / 32][W];
         if (role == 0) {
-            Operand<N> mine[R / 32][W];
-#pragma unroll
-            for (int n = 0; n < R / 32; n++)
-#pragma unroll
-                for (int w = 0; w < W; w++) mine[n][w] = keys.transposed(32 * n, column + 16 * w);
-#pragma unroll
-            for (int s = 0; s < kTiles; s++) {
-                const float decay = reach.row[16 * s + lane % 16];
+            columns_of(keys, column, mine);
+            each_of<kTiles>([&](auto number) {
+                constexpr int s = decltype(number)::value;
+                const float decay = reach.row[16 * s + lane % 16] * down;
                 const int to = column + 4 * (lane / 16);
                 float sum = 0.0f;
 #pragma unroll
@@ -145,13 +153,7 @@ __global__ __launch_bounds__((kQueriesThreads<T, D>), (waves_of_simd(kQueriesThr
                 }
                 sum = sum_groups(sum);
                 if (lane < 16) by_wave[wave][16 * s + lane] = sum;
-#pragma unroll
-                for (int n = 0; n < R / 32; n++)
-                    if (2 * n <= s) {
-                        const Operand<N> p = pairs.chained(16 * s, 32 * n);
-#pragma unroll
-                        for (int w = 0; w < W; w++) read[s][w] = product(mine[n][w], p, read[s][w]);
-                    }
+                add_pairs<T, 0, s / 2 + 1>(pairs, 16 * s, mine, scaling.down, read[s]);
                 in_order();
                 if (c.grad_queries && 16 * s + lane % 16 < unit.count - at) {
                     const int64_t base = ((unit.first + at + 16 * s) * c.m.heads + head) * c.m.key_size;
@@ -164,17 +166,11 @@ __global__ __launch_bounds__((kQueriesThreads<T, D>), (waves_of_simd(kQueriesThr
                             put_row((float *)c.grad_queries + base + 16 * w, offset, to + 16 * w, c.m.key_size, Vector, read[s][w]);
                     }
                 }
-            }
-            state.times(reach.whole);
-#pragma unroll
-            for (int n = 0; n < R / 32; n++) {
-                Operand<kWhole> late[W];
-#pragma unroll
-                for (int w = 0; w < W; w++) late[w] = weighted<kWhole>(mine[n][w], reach.column, 32 * n, lane);
-                state.add(values, 32 * n, late);
-            }
+            });
+            state.template fold<T>(reach.whole, values, mine, reach.column);
         } else {
-            state.template add_weighted<kWhole>(grads, queries, column, reach.start);
+            columns_of(queries, column, mine);
+            state.template fold<T>(1.0f, grads, mine, reach.start);
         }
         if (wave == 0 && at + R < unit.count) reach_of(c, reaches[turn ^ 1], gate, unit.count - at - R, before);
         __syncthreads();
@@ -193,9 +189,10 @@ __global__ __launch_bounds__((kQueriesThreads<T, D>), (waves_of_simd(kQueriesThr
 
 template <class T, int D, bool Vector>
 __global__ __launch_bounds__(kKeysThreads<D>, (waves_of_simd(kKeysThreads<D>, kKeysLds<T, D>, kKeysColumns<D> * D / 4))) void attention_grad_keys_kernel(AttentionCall c) {
-    constexpr int R = Parts<T>::kRows, N = Parts<T>::kInput, M = Parts<T>::kState, kTiles = R / 16, W = kKeysColumns<D>, kWaves = State<D, W>::kWaves;
-    using In = Tile<N, R, D>;
-    using Pairs = Tile<N, R, R>;
+    constexpr int R = Parts<T>::kRows, N = Parts<T>::kInput, kTiles = R / 16, W = kKeysColumns<D>, kWaves = State<D, W>::kWaves;
+    using E = typename Parts<T>::Element;
+    using In = Tile<E, N, R, D>;
+    using Pairs = Tile<E, N, R, R>;
     extern __shared__ __attribute__((aligned(16))) char lds[];
     Reach<R> *reaches = (Reach<R> *)(lds + 4 * In::kBytes + 2 * Pairs::kBytes);
     float(*by_wave)[R] = (float(*)[R])(reaches + 2);  // k.dk without the chunk's own pairs, of each wave's columns
@@ -219,19 +216,25 @@ __global__ __launch_bounds__(kKeysThreads<D>, (waves_of_simd(kKeysThreads<D>, kK
     next.load(c, last, unit.count - last);
     float gate = 0.0f;  // of the next chunk's row, in the first wave
     if (wave == 0) reach_of(c, reaches[0], gate_of_lane<T, R>(c, unit.first + last, unit.count - last, head), unit.count - last, before);
+    if (Parts<T>::kScaled) {
+        if (threadIdx.x < 4) reaches[0].largest[threadIdx.x] = 0;
+        __syncthreads();
+    }
     int turn = 0;
     for (int64_t at = last; at >= 0; at -= R, turn ^= 1) {
         const int lane = lane_of_turn();
-        const In queries{(__bf16 *)lds, lane}, keys{(__bf16 *)(lds + In::kBytes), lane}, values{(__bf16 *)(lds + 2 * In::kBytes), lane},
-            grads{(__bf16 *)(lds + 3 * In::kBytes), lane};
-        const Pairs scores{(__bf16 *)(lds + 4 * In::kBytes), lane}, pairs{(__bf16 *)(lds + 4 * In::kBytes + Pairs::kBytes), lane};
-        next.store(c, queries, keys, values, grads, unit.count - at);
+        const In queries{(E *)lds, lane}, keys{(E *)(lds + In::kBytes), lane}, values{(E *)(lds + 2 * In::kBytes), lane},
+            grads{(E *)(lds + 3 * In::kBytes), lane};
+        const Pairs scores{(E *)(lds + 4 * In::kBytes), lane}, pairs{(E *)(lds + 4 * In::kBytes + Pairs::kBytes), lane};
+        next.store(c, queries, keys, values, grads, unit.count - at, reaches[turn]);
         __syncthreads();
+        if (Parts<T>::kScaled && threadIdx.x < 4) reaches[turn ^ 1].largest[threadIdx.x] = 0;
         if (at > 0) {
             next.load(c, at - R, R);
             if (wave == 0) gate = gate_of_lane<T, R>(c, unit.first + at - R, R, head);
         }
         const Reach<R> &reach = reaches[turn];
+        const Scaling for_scores = scaling_of_pairs<T>(reach, 0, 1, c.m.key_size, c.m.scale), for_pairs = scaling_of_pairs<T>(reach, 2, 3, c.m.value_size, c.m.scale);
 #pragma unroll 1
         for (int tile = wave; tile < kTiles * kTiles; tile += 2 * kWaves) {
             const int r = tile / kTiles, s = tile % kTiles;
@@ -247,28 +250,30 @@ __global__ __launch_bounds__(kKeysThreads<D>, (waves_of_simd(kKeysThreads<D>, kK
                 const floatx4 decay = decays_of<false>(reach, 16 * s, 16 * r, c.m.scale, lane);
                 p *= decay;
                 d *= decay;
+                if (Parts<T>::kScaled) {
+                    p *= for_scores.up;
+                    d *= for_pairs.up;
+                }
             }
             scores.put(16 * r, 16 * s, p);
             pairs.put(16 * r, 16 * s, d);
         }
         // the same for both roles: what the state reads, what its transposed rows are added up with, and what of
-        const In reading{(__bf16 *)(lds + (role ? 2 : 1) * In::kBytes), lane}, with{(__bf16 *)(lds + (role ? 0 : 3) * In::kBytes), lane},
-            adding{(__bf16 *)(lds + (role ? 3 : 0) * In::kBytes), lane};
-        const Pairs mine_of{(__bf16 *)(lds + 4 * In::kBytes + role * Pairs::kBytes), lane};
+        const In reading{(E *)(lds + (role ? 2 : 1) * In::kBytes), lane}, with{(E *)(lds + (role ? 0 : 3) * In::kBytes), lane},
+            adding{(E *)(lds + (role ? 3 : 0) * In::kBytes), lane};
+        const Pairs mine_of{(E *)(lds + 4 * In::kBytes + role * Pairs::kBytes), lane};
         floatx4 read[kTiles][W] = {};
+        float down;
         if (role)
-            state.template read_by<kWhole>(reading, read);
+            down = state.template read_by<T, Parts<T>::kWhole>(reading, read);
         else
-            state.template read_by<M>(reading, read);
+            down = state.template read_by<T, Parts<T>::kState>(reading, read);
         __syncthreads();
-        Operand<N> mine[R / 32][W];
-#pragma unroll
-        for (int n = 0; n < R / 32; n++)
-#pragma unroll
-            for (int w = 0; w < W; w++) mine[n][w] = with.transposed(32 * n, column + 16 * w);
-#pragma unroll
-        for (int r = 0; r < kTiles; r++) {
-            const float decay = reach.column[16 * r + lane % 16];
+        Operand<E, N> mine[R / 32][W];
+        columns_of(with, column, mine);
+        each_of<kTiles>([&](auto number) {
+            constexpr int r = decltype(number)::value;
+            const float decay = reach.column[16 * r + lane % 16] * down;
             const int to = column + 4 * (lane / 16);
 #pragma unroll
             for (int w = 0; w < W; w++) read[r][w] *= decay;
@@ -283,13 +288,7 @@ __global__ __launch_bounds__(kKeysThreads<D>, (waves_of_simd(kKeysThreads<D>, kK
                 sum = sum_groups(sum);
                 if (lane < 16) by_wave[wave - kWaves][16 * r + lane] = sum;
             }
-#pragma unroll
-            for (int n = 0; n < R / 32; n++)
-                if (2 * n + 1 >= r) {
-                    const Operand<N> p = mine_of.chained(16 * r, 32 * n);
-#pragma unroll
-                    for (int w = 0; w < W; w++) read[r][w] = product(mine[n][w], p, read[r][w]);
-                }
+            add_pairs<T, r / 2, R / 32>(mine_of, 16 * r, mine, role ? for_pairs.down : for_scores.down, read[r]);
             in_order();
             if (out && 16 * r + lane % 16 < unit.count - at) {
                 const int64_t base = ((unit.first + at + 16 * r) * c.m.heads + head) * size;
@@ -302,15 +301,8 @@ __global__ __launch_bounds__(kKeysThreads<D>, (waves_of_simd(kKeysThreads<D>, kK
                         put_row((float *)out + base + 16 * w, offset, to + 16 * w, size, Vector, read[r][w]);
                 }
             }
-        }
-        state.times(reach.whole);
-#pragma unroll
-        for (int n = 0; n < R / 32; n++) {
-            Operand<kWhole> late[W];
-#pragma unroll
-            for (int w = 0; w < W; w++) late[w] = weighted<kWhole>(mine[n][w], reach.row, 32 * n, lane);
-            state.add(adding, 32 * n, late);
-        }
+        });
+        state.template fold<T>(reach.whole, adding, mine, reach.row);
         if (wave == 0 && at > 0) reach_of(c, reaches[turn ^ 1], gate, R, before);
         __syncthreads();
         if (threadIdx.x < R && at + threadIdx.x < unit.count) {

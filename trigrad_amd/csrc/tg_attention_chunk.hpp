@@ -8,10 +8,12 @@
 // products of matrices of at most 64 rows and TG_ATTENTION_SIZE columns.  A workgroup has a head and a run of chunks (a unit), one after another; the states stay in
 // the accumulators of its waves, each of which has sixteen columns of them.
 //
-// Numbers.  Products are of bfloat16 numbers and summed in float32.  What is not one is a sum of "parts" in bfloat16, each the rounded rest of
-// those before: inputs in float16 are two parts and in float32 three, exactly; so are states, and inputs that carry a decay, wherever what they
-// go into is float32 in the end (states, their gradients, gates' gradients: two parts leave an error of 2e-6, three one of 1e-8, below that of
-// the sums).  States that go into an output of 16 bits have two parts, and the matrix of pairs inside a chunk is rounded as the inputs are, once.
+// Numbers.  Products are of numbers in 16 bits and summed in float32.  What is not one is a sum of "parts", each the rounded rest of those before.
+// In bfloat16, whose range is float32's, inputs in float32 are three parts, exactly; so are states, and inputs that carry a decay, wherever what they
+// go into is float32 in the end (states, their gradients, gates' gradients: two parts leave an error of 2e-6, three one of 1e-8, below that of the
+// sums).  States that go into an output of 16 bits have two parts, and the matrix of pairs inside a chunk is rounded as the inputs are, once.  Inputs in
+// float16 stay as they are, and what meets them is two parts in float16 (an error of 2^-23): states and weighted inputs by a power of two that brings
+// the largest of a wave's numbers near 2^15, pairs by one that brings the largest they could be there.
 #pragma once
 #include "tg_attention.hpp"
 
@@ -19,35 +21,57 @@
 
 namespace tg {
 
-typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
-typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
 typedef short short4_t __attribute__((ext_vector_type(4)));
 typedef float floatx4 __attribute__((ext_vector_type(4)));
+typedef uint32_t uint32x4 __attribute__((ext_vector_type(4)));
 
-// Parts of an input and of a state that goes into an output of its type; rows of a chunk: as many as leave room in LDS for the parts.
+// Parts of an input, of a state that goes into an output of its type and of one that goes into float32, their type, and rows of a chunk: as many as
+// leave room in LDS for the parts.
 template <class T> struct Parts;
-template <> struct Parts<bf16_t> { static constexpr int kInput = 1, kState = 2, kRows = 64; };
-template <> struct Parts<half_t> { static constexpr int kInput = 2, kState = 2, kRows = 32; };
-template <> struct Parts<float> { static constexpr int kInput = 3, kState = 3, kRows = 32; };
-constexpr int kWhole = 3;  // parts of a number in float32
+template <> struct Parts<bf16_t> {
+    using Element = __bf16;
+    static constexpr int kInput = 1, kState = 2, kWhole = 3, kRows = 64;
+    static constexpr bool kScaled = false;
+};
+template <> struct Parts<half_t> {
+    using Element = _Float16;
+    static constexpr int kInput = 1, kState = 2, kWhole = 2, kRows = 64;
+    static constexpr bool kScaled = true;
+};
+template <> struct Parts<float> {
+    using Element = __bf16;
+    static constexpr int kInput = 3, kState = 3, kWhole = 3, kRows = 32;
+    static constexpr bool kScaled = false;
+};
 
-// Eight numbers of a lane for v_mfma_f32_16x16x32_bf16: row (of A) or column (of B) lane % 16, and eight of the 32 that are summed over; which,
-// both operands have to agree in.  "Straight": 8 (lane / 16) on.  "Chained": 4 (lane / 16) on, and sixteen further: as two accumulators one above the
-// other hold them (rows 4 (lane / 16) on of column lane % 16), so that a state goes from one product into the next without leaving its lane.
-template <int N> struct Operand { bf16x8 part[N]; };
+template <class E> struct Vectors {
+    typedef E x8 __attribute__((ext_vector_type(8)));
+    typedef E x4 __attribute__((ext_vector_type(4)));
+};
 
-template <int NA, int NB> __device__ __forceinline__ floatx4 product(const Operand<NA> &a, const Operand<NB> &b, floatx4 sum) {
-    constexpr int kTerms = NA == 2 && NB == 2 ? 3 : NA > NB ? NA : NB;  // parts beyond are below the last ones' rounding
+// Eight numbers of a lane for a product of 16 x 32 by 32 x 16 numbers: row (of A) or column (of B) lane % 16, and eight of the 32 that are summed over;
+// which, both operands have to agree in.  "Straight": 8 (lane / 16) on.  "Chained": 4 (lane / 16) on, and sixteen further: as two accumulators one above
+// the other hold them (rows 4 (lane / 16) on of column lane % 16), so that a state goes from one product into the next without leaving its lane.
+template <class E, int N> struct Operand { typename Vectors<E>::x8 part[N]; };
+
+__device__ __forceinline__ floatx4 multiply(Vectors<__bf16>::x8 a, Vectors<__bf16>::x8 b, floatx4 sum) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, sum, 0, 0, 0);
+}
+__device__ __forceinline__ floatx4 multiply(Vectors<_Float16>::x8 a, Vectors<_Float16>::x8 b, floatx4 sum) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, sum, 0, 0, 0);
+}
+template <class E, int NA, int NB> __device__ __forceinline__ floatx4 product(const Operand<E, NA> &a, const Operand<E, NB> &b, floatx4 sum) {
+    constexpr int kTerms = NA > NB ? NA : NB;  // parts beyond are below the last ones' rounding
 #pragma unroll
     for (int i = NA - 1; i >= 0; i--)
 #pragma unroll
         for (int j = NB - 1; j >= 0; j--)
-            if (i + j < kTerms) sum = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a.part[i], b.part[j], sum, 0, 0, 0);
+            if (i + j < kTerms) sum = multiply(a.part[i], b.part[j], sum);
     return sum;
 }
 
-template <int N> __device__ __forceinline__ Operand<N> parts_of(const float *x) {
-    Operand<N> o;
+template <class E, int N> __device__ __forceinline__ Operand<E, N> parts_of(const float *x) {
+    Operand<E, N> o;
     float rest[8];
 #pragma unroll
     for (int j = 0; j < 8; j++) rest[j] = x[j];
@@ -55,60 +79,81 @@ template <int N> __device__ __forceinline__ Operand<N> parts_of(const float *x) 
     for (int n = 0; n < N; n++)
 #pragma unroll
         for (int j = 0; j < 8; j++) {
-            o.part[n][j] = (__bf16)rest[j];
+            o.part[n][j] = (E)rest[j];
             if (n + 1 < N) rest[j] -= (float)o.part[n][j];
         }
     return o;
 }
-template <int N> __device__ __forceinline__ Operand<N> operand_of(floatx4 above, floatx4 below) {
-    const float x[8] = {above[0], above[1], above[2], above[3], below[0], below[1], below[2], below[3]};
-    return parts_of<N>(x);
+
+// The largest of a wave's numbers, none of which is negative, as bits.
+template <int Control, int RowMask> __device__ __forceinline__ uint32_t or_lane(uint32_t v) {
+    return max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, Control, RowMask, 0xf, false));
+}
+__device__ __forceinline__ uint32_t largest_of_wave(uint32_t v) {
+    v = or_lane<0x111, 0xf>(v);
+    v = or_lane<0x112, 0xf>(v);
+    v = or_lane<0x114, 0xf>(v);
+    v = or_lane<0x118, 0xf>(v);
+    v = or_lane<0x142, 0xa>(v);
+    v = or_lane<0x143, 0xc>(v);
+    return (uint32_t)__builtin_amdgcn_readlane((int)v, kWave - 1);
+}
+
+// A power of two that brings numbers of at most `largest` to at most 2^15, and its reciprocal.
+struct Scaling {
+    float up, down;
+};
+__device__ __forceinline__ Scaling scaling_of(uint32_t largest_bits) {
+    const int exponent = max(1, min(253, 268 - (int)(largest_bits >> 23)));
+    return {__uint_as_float((uint32_t)exponent << 23), __uint_as_float((uint32_t)(254 - exponent) << 23)};
 }
 
 // A matrix of Rows x Columns in LDS, N parts.  Rows are 16 bytes longer than their numbers, so that sixteen rows begin in different banks.
-template <int N, int Rows, int Columns> struct Tile {
+template <class E, int N, int Rows, int Columns> struct Tile {
+    using x8 = typename Vectors<E>::x8;
+    using x4 = typename Vectors<E>::x4;
     static constexpr int kStride = Columns + 8, kPart = Rows * kStride, kBytes = N * kPart * 2;
-    __bf16 *at;
+    E *at;
     int lane;
 
-    __device__ __forceinline__ Operand<N> straight(int row, int column) const {
-        const __bf16 *p = at + (row + lane % 16) * kStride + column + 8 * (lane / 16);
-        Operand<N> o;
+    __device__ __forceinline__ Operand<E, N> straight(int row, int column) const {
+        const E *p = at + (row + lane % 16) * kStride + column + 8 * (lane / 16);
+        Operand<E, N> o;
 #pragma unroll
-        for (int n = 0; n < N; n++) o.part[n] = *(const bf16x8 *)(p + n * kPart);
+        for (int n = 0; n < N; n++) o.part[n] = *(const x8 *)(p + n * kPart);
         return o;
     }
-    __device__ __forceinline__ Operand<N> chained(int row, int column) const {
-        const __bf16 *p = at + (row + lane % 16) * kStride + column + 4 * (lane / 16);
-        Operand<N> o;
+    __device__ __forceinline__ Operand<E, N> chained(int row, int column) const {
+        const E *p = at + (row + lane % 16) * kStride + column + 4 * (lane / 16);
+        Operand<E, N> o;
 #pragma unroll
         for (int n = 0; n < N; n++) {
-            const bf16x4 a = *(const bf16x4 *)(p + n * kPart), b = *(const bf16x4 *)(p + n * kPart + 16);
+            const x4 a = *(const x4 *)(p + n * kPart), b = *(const x4 *)(p + n * kPart + 16);
             o.part[n] = __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
         }
         return o;
     }
     // The transposed matrix's: row or column `column` + lane % 16, chained rows from `row`.  LDS hands out four rows of sixteen columns transposed to
     // sixteen lanes, of which each points at four neighbours of a row.
-    __device__ __forceinline__ Operand<N> transposed(int row, int column) const {
-        const __bf16 *p = at + (row + 4 * (lane / 16) + lane % 16 / 4) * kStride + column + 4 * (lane % 4);
-        Operand<N> o;
+    __device__ __forceinline__ Operand<E, N> transposed(int row, int column) const {
+        const E *p = at + (row + 4 * (lane / 16) + lane % 16 / 4) * kStride + column + 4 * (lane % 4);
+        Operand<E, N> o;
 #pragma unroll
         for (int n = 0; n < N; n++) {
-            const bf16x4 a = turned(p + n * kPart), b = turned(p + n * kPart + 16 * kStride);
+            const x4 a = turned(p + n * kPart), b = turned(p + n * kPart + 16 * kStride);
             o.part[n] = __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
         }
         return o;
     }
-    static __device__ __forceinline__ bf16x4 turned(const __bf16 *p) {
-        return __builtin_bit_cast(bf16x4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) short4_t *)p));
+    static __device__ __forceinline__ x4 turned(const E *p) {
+        return __builtin_bit_cast(x4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) short4_t *)p));
     }
     // Four neighbours of a row, as numbers.
     __device__ __forceinline__ floatx4 numbers(int row, int column) const {
         floatx4 x = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
         for (int n = N - 1; n >= 0; n--) {
-            const bf16x4 v = *(const bf16x4 *)(at + n * kPart + row * kStride + column);
+            const x4 v = *(const x4 *)(at + n * kPart + row * kStride + column);
 #pragma unroll
             for (int j = 0; j < 4; j++) x[j] += (float)v[j];
         }
@@ -116,25 +161,24 @@ template <int N, int Rows, int Columns> struct Tile {
     }
     // An accumulator's four rows (columns here) of its column (a row here): the product's transpose.
     __device__ __forceinline__ void put(int row, int column, floatx4 x) const {
-        __bf16 *p = at + (row + lane % 16) * kStride + column + 4 * (lane / 16);
+        E *p = at + (row + lane % 16) * kStride + column + 4 * (lane / 16);
 #pragma unroll
         for (int n = 0; n < N; n++) {
-            bf16x4 v;
+            x4 v;
 #pragma unroll
             for (int j = 0; j < 4; j++) {
-                v[j] = (__bf16)x[j];
+                v[j] = (E)x[j];
                 x[j] -= (float)v[j];
             }
-            *(bf16x4 *)(p + n * kPart) = v;
+            *(x4 *)(p + n * kPart) = v;
         }
     }
 };
 
-// A transposed input's operand with a weight for each row.
-template <int M, int N> __device__ __forceinline__ Operand<M> weighted(const Operand<N> &o, const float *weights, int row, int lane) {
+// A transposed input's numbers with a weight for each row.
+template <class E, int N> __device__ __forceinline__ void weighted(const Operand<E, N> &o, const float *weights, int row, int lane, float *x) {
     const int group = lane / 16;
     const floatx4 a = *(const floatx4 *)(weights + row + 4 * group), b = *(const floatx4 *)(weights + row + 16 + 4 * group);
-    float x[8];
 #pragma unroll
     for (int j = 0; j < 8; j++) {
         x[j] = (float)o.part[N - 1][j];
@@ -142,7 +186,6 @@ template <int M, int N> __device__ __forceinline__ Operand<M> weighted(const Ope
         for (int n = N - 2; n >= 0; n--) x[j] += (float)o.part[n][j];
         x[j] *= j < 4 ? a[j] : b[j - 4];
     }
-    return parts_of<M>(x);
 }
 
 // ---- reading a chunk ----------------------------------------------------------------------
@@ -168,23 +211,38 @@ template <class T, int Rows, int D, int Threads, bool Vector> struct Incoming {
             for (int j = 0; j < 8; j += kWidest) x[n][j / kWidest] = load_pack<kWidest>(from + min(column_of(n) + j, size - kWidest));
         }
     }
-    template <int N> __device__ __forceinline__ void store(const Tile<N, Rows, D> &tile, int64_t count, int size) const {
+    // `largest`: where the largest of the numbers is kept as bits, if that is wanted (Scaled).
+    template <class E, int N, bool Scaled> __device__ __forceinline__ void store(const Tile<E, N, Rows, D> &tile, int64_t count, int size, uint32_t *largest) const {
+        uint32_t most = 0;
 #pragma unroll
         for (int n = 0; n < kGroups; n++) {
             if (!mine(n)) continue;
             const int row = row_of(n), column = column_of(n);
-            if constexpr (Vector && N == 1) {  // bfloat16 as it is
-                typedef uint32_t words __attribute__((ext_vector_type(4)));
-                const words w = __builtin_bit_cast(words, x[n][0]), none = {0, 0, 0, 0};
-                *(words *)(tile.at + row * Tile<N, Rows, D>::kStride + column) = row < count && column < size ? w : none;
+            if constexpr (Vector && N == 1) {  // as it is
+                const uint32x4 w = __builtin_bit_cast(uint32x4, x[n][0]), none = {0, 0, 0, 0}, v = row < count && column < size ? w : none;
+                *(uint32x4 *)(tile.at + row * Tile<E, N, Rows, D>::kStride + column) = v;
+                if constexpr (Scaled) {
+#pragma unroll
+                    for (int j = 0; j < 4; j++) most = max(most, max(v[j] & 0x7fffu, v[j] >> 16 & 0x7fffu));
+                }
                 continue;
             }
             float v[8];
 #pragma unroll
             for (int j = 0; j < 8; j++) v[j] = row < count && column + j / kWidest * kWidest < size ? (float)x[n][j / kWidest].v[j % kWidest] : 0.0f;
-            const Operand<N> o = parts_of<N>(v);
+            const Operand<E, N> o = parts_of<E, N>(v);
 #pragma unroll
-            for (int i = 0; i < N; i++) *(bf16x8 *)(tile.at + i * Tile<N, Rows, D>::kPart + row * Tile<N, Rows, D>::kStride + column) = o.part[i];
+            for (int i = 0; i < N; i++)
+                *(typename Vectors<E>::x8 *)(tile.at + i * Tile<E, N, Rows, D>::kPart + row * Tile<E, N, Rows, D>::kStride + column) = o.part[i];
+            if constexpr (Scaled) {
+                const uint32x4 w = __builtin_bit_cast(uint32x4, o.part[0]);
+#pragma unroll
+                for (int j = 0; j < 4; j++) most = max(most, max(w[j] & 0x7fffu, w[j] >> 16 & 0x7fffu));
+            }
+        }
+        if constexpr (Scaled) {
+            most = largest_of_wave(most);
+            if (threadIdx.x % kWave == 0) atomicMax(largest, __float_as_uint((float)__builtin_bit_cast(_Float16, (uint16_t)most)));
         }
     }
 };
@@ -203,7 +261,14 @@ template <int Rows> struct alignas(16) Reach {
     float column[Rows];   // 2^(L_C - L)
     float start[Rows];    // scale 2^L from the unit's beginning
     float whole;          // 2^L_C
+    uint32_t largest[4];  // of the chunk's queries, keys, values and gradients of outputs, as bits
 };
+
+// The scaling of products of a row of each of two of a chunk's inputs, of `size` numbers.
+template <class T, int Rows> __device__ __forceinline__ Scaling scaling_of_pairs(const Reach<Rows> &reach, int first, int second, int size, float scale) {
+    if constexpr (!Parts<T>::kScaled) return {1.0f, 1.0f};
+    return scaling_of(__float_as_uint(fabsf(scale) * (float)size * __uint_as_float(reach.largest[first]) * __uint_as_float(reach.largest[second])));
+}
 
 struct AttentionCall {
     Attention m;
@@ -372,50 +437,141 @@ template <int D, int W> struct State {
     template <bool Turned> __device__ __forceinline__ void store(float *to, int column, int key_size, int value_size) {
         each<Turned>(column, key_size, value_size, [&](int w, int n, int j, int at) { to[at] = x[w][n][j]; });
     }
-    __device__ __forceinline__ void times(float a) {
+    // Adds its transpose times the rows' columns to `sums`, by sixteen rows of the tile; -> what the sums are to be multiplied with.
+    template <class T, int M, class E, int N, int Rows> __device__ __forceinline__ float read_by(const Tile<E, N, Rows, D> &tile, floatx4 (&sums)[Rows / 16][W]) const {
+        Scaling scaling = {1.0f, 1.0f};
+        if constexpr (Parts<T>::kScaled) {
+            float most = 0.0f;
 #pragma unroll
-        for (int w = 0; w < W; w++)
+            for (int w = 0; w < W; w++)
 #pragma unroll
-            for (int n = 0; n < D / 16; n++) x[w][n] *= a;
-    }
-    // Adds its transpose times the rows' columns to `sums`, by sixteen rows of the tile.
-    template <int M, int N, int Rows> __device__ __forceinline__ void read_by(const Tile<N, Rows, D> &tile, floatx4 (&sums)[Rows / 16][W]) const {
+                for (int n = 0; n < D / 16; n++)
+#pragma unroll
+                    for (int j = 0; j < 4; j++) most = fmaxf(most, fabsf(x[w][n][j]));
+            scaling = scaling_of(largest_of_wave(__float_as_uint(most)));
+        }
 #pragma unroll
         for (int i = 0; i < D / 32; i++) {
-            Operand<M> mine[W];
+            Operand<E, M> mine[W];
 #pragma unroll
-            for (int w = 0; w < W; w++) mine[w] = operand_of<M>(x[w][2 * i], x[w][2 * i + 1]);
+            for (int w = 0; w < W; w++) {
+                float v[8];
+#pragma unroll
+                for (int j = 0; j < 8; j++) v[j] = Parts<T>::kScaled ? x[w][2 * i + j / 4][j % 4] * scaling.up : x[w][2 * i + j / 4][j % 4];
+                mine[w] = parts_of<E, M>(v);
+            }
 #pragma unroll
             for (int r = 0; r < Rows / 16; r++) {
-                const Operand<N> theirs = tile.chained(16 * r, 32 * i);
+                const Operand<E, N> theirs = tile.chained(16 * r, 32 * i);
 #pragma unroll
                 for (int w = 0; w < W; w++) sums[r][w] = product(mine[w], theirs, sums[r][w]);
             }
             in_order();
         }
+        return scaling.down;
     }
-    // += 32 rows of the tile, transposed, times this wave's columns of as many rows
-    template <int N, int M, int Rows> __device__ __forceinline__ void add(const Tile<N, Rows, D> &tile, int row, const Operand<M> (&columns)[W]) {
+    // decay times itself, plus the tile, transposed, times this wave's columns `mine` of another with a weight for each row
+    template <class T, class E, int N, int Rows>
+    __device__ __forceinline__ void fold(float decay, const Tile<E, N, Rows, D> &tile, const Operand<E, N> (&mine)[Rows / 32][W], const float *weights) {
+        constexpr int M = Parts<T>::kWhole, K = Rows / 32;
+        if constexpr (Parts<T>::kScaled) {
+            float v[K][W][8], most = 0.0f;
 #pragma unroll
-        for (int n = 0; n < D / 16; n++) {
-            const Operand<N> theirs = tile.transposed(row, 16 * n);
+            for (int k = 0; k < K; k++)
 #pragma unroll
-            for (int w = 0; w < W; w++) x[w][n] = product(theirs, columns[w], x[w][n]);
-            if (n % 4 == 3) in_order();
-        }
-    }
-    // ... of this wave's columns of the tile `with`, its rows weighted
-    template <int M, int N, int Rows>
-    __device__ __forceinline__ void add_weighted(const Tile<N, Rows, D> &tile, const Tile<N, Rows, D> &with, int column, const float *weights) {
+                for (int w = 0; w < W; w++) {
+                    weighted(mine[k][w], weights, 32 * k, tile.lane, v[k][w]);
 #pragma unroll
-        for (int k = 0; k < Rows; k += 32) {
-            Operand<M> mine[W];
+                    for (int j = 0; j < 8; j++) most = fmaxf(most, fabsf(v[k][w][j]));
+                }
+            const Scaling scaling = scaling_of(largest_of_wave(__float_as_uint(most)));
+            Operand<E, M> late[K][W];
 #pragma unroll
-            for (int w = 0; w < W; w++) mine[w] = weighted<M>(with.transposed(k, column + 16 * w), weights, k, tile.lane);
-            add(tile, k, mine);
+            for (int k = 0; k < K; k++)
+#pragma unroll
+                for (int w = 0; w < W; w++) {
+#pragma unroll
+                    for (int j = 0; j < 8; j++) v[k][w][j] *= scaling.up;
+                    late[k][w] = parts_of<E, M>(v[k][w]);
+                }
+#pragma unroll
+            for (int n = 0; n < D / 16; n++) {
+                floatx4 sum[W] = {};
+#pragma unroll
+                for (int k = 0; k < K; k++) {
+                    const Operand<E, N> theirs = tile.transposed(32 * k, 16 * n);
+#pragma unroll
+                    for (int w = 0; w < W; w++) sum[w] = product(theirs, late[k][w], sum[w]);
+                }
+#pragma unroll
+                for (int w = 0; w < W; w++)
+#pragma unroll
+                    for (int j = 0; j < 4; j++) x[w][n][j] = fmaf(sum[w][j], scaling.down, x[w][n][j] * decay);
+                if (n % 4 == 3) in_order();
+            }
+        } else {
+#pragma unroll
+            for (int w = 0; w < W; w++)
+#pragma unroll
+                for (int n = 0; n < D / 16; n++) x[w][n] *= decay;
+#pragma unroll
+            for (int k = 0; k < K; k++) {
+                Operand<E, M> late[W];
+#pragma unroll
+                for (int w = 0; w < W; w++) {
+                    float v[8];
+                    weighted(mine[k][w], weights, 32 * k, tile.lane, v);
+                    late[w] = parts_of<E, M>(v);
+                }
+#pragma unroll
+                for (int n = 0; n < D / 16; n++) {
+                    const Operand<E, N> theirs = tile.transposed(32 * k, 16 * n);
+#pragma unroll
+                    for (int w = 0; w < W; w++) x[w][n] = product(theirs, late[w], x[w][n]);
+                    if (n % 4 == 3) in_order();
+                }
+            }
         }
     }
 };
+
+// call(constant 0), ... up to before N
+template <int N, class Call> __device__ __forceinline__ void each_of(Call &&call) {
+    if constexpr (N > 0) {
+        each_of<N - 1>(call);
+        call(std::integral_constant<int, N - 1>());
+    }
+}
+
+// This wave's columns of a tile, for fold.
+template <class E, int N, int Rows, int D, int W>
+__device__ __forceinline__ void columns_of(const Tile<E, N, Rows, D> &tile, int column, Operand<E, N> (&mine)[Rows / 32][W]) {
+#pragma unroll
+    for (int k = 0; k < Rows / 32; k++)
+#pragma unroll
+        for (int w = 0; w < W; w++) mine[k][w] = tile.transposed(32 * k, column + 16 * w);
+}
+
+// += this wave's columns times sixteen rows of pairs from `row` on, those of the columns from First on to before Last.
+template <class T, int First, int Last, class E, int N, int Rows, int W>
+__device__ __forceinline__ void add_pairs(const Tile<E, N, Rows, Rows> &pairs, int row, const Operand<E, N> (&mine)[Rows / 32][W], float down, floatx4 (&sums)[W]) {
+    floatx4 inside[W] = {};
+#pragma unroll
+    for (int k = First; k < Last; k++) {
+        const Operand<E, N> p = pairs.chained(row, 32 * k);
+#pragma unroll
+        for (int w = 0; w < W; w++)
+            if (Parts<T>::kScaled)
+                inside[w] = product(mine[k][w], p, inside[w]);
+            else
+                sums[w] = product(mine[k][w], p, sums[w]);
+    }
+    if (Parts<T>::kScaled)
+#pragma unroll
+        for (int w = 0; w < W; w++)
+#pragma unroll
+            for (int j = 0; j < 4; j++) sums[w][j] = fmaf(inside[w][j], down, sums[w][j]);
+}
 
 // `size`: 32, 64 or 128, of keys and values in the kernel
 int launch_attention_forward(int64_t type, const AttentionCall &c, int size, bool states_only, hipStream_t stream);

@@ -4,9 +4,9 @@
 
 namespace tg {
 
-template <class T, int D> constexpr int kStatesLds = 2 * Tile<Parts<T>::kInput, Parts<T>::kRows, D>::kBytes + 2 * (int)sizeof(Reach<Parts<T>::kRows>);
-template <class T, int D> constexpr int kOutputsLds = 3 * Tile<Parts<T>::kInput, Parts<T>::kRows, D>::kBytes +
-                                                      Tile<Parts<T>::kInput, Parts<T>::kRows, Parts<T>::kRows>::kBytes + 2 * (int)sizeof(Reach<Parts<T>::kRows>);
+template <class T, int D> constexpr int kStatesLds = 2 * Tile<typename Parts<T>::Element, Parts<T>::kInput, Parts<T>::kRows, D>::kBytes + 2 * (int)sizeof(Reach<Parts<T>::kRows>);
+template <class T, int D> constexpr int kOutputsLds = 3 * Tile<typename Parts<T>::Element, Parts<T>::kInput, Parts<T>::kRows, D>::kBytes +
+                                                      Tile<typename Parts<T>::Element, Parts<T>::kInput, Parts<T>::kRows, Parts<T>::kRows>::kBytes + 2 * (int)sizeof(Reach<Parts<T>::kRows>);
 constexpr int W = 1;  // see State
 template <int D> constexpr int kThreads = State<D, W>::kWaves * kWave;
 
@@ -14,8 +14,9 @@ template <int D> constexpr int kThreads = State<D, W>::kWaves * kWave;
 template <class T, int D, bool Vector>
 __global__ __launch_bounds__(kThreads<D>, waves_of_simd(kThreads<D>, kStatesLds<T, D>, W * D / 4)) void attention_states_kernel(AttentionCall c) {
     constexpr int R = Parts<T>::kRows, N = Parts<T>::kInput;
-    using In = Tile<N, R, D>;
-    __shared__ __attribute__((aligned(16))) __bf16 lds[In::kBytes];
+    using E = typename Parts<T>::Element;
+    using In = Tile<E, N, R, D>;
+    __shared__ __attribute__((aligned(16))) E lds[In::kBytes];
     __shared__ Reach<R> reaches[2];
     const int64_t u = blockIdx.x / c.m.heads;
     const int head = (int)(blockIdx.x % c.m.heads), wave = wave_of(), column = 16 * W * wave;
@@ -35,16 +36,17 @@ __global__ __launch_bounds__(kThreads<D>, waves_of_simd(kThreads<D>, kStatesLds<
     for (int64_t at = 0; at < unit.count; at += R, turn ^= 1) {
         const int lane = lane_of_turn();
         const In keys{lds, lane}, values{lds + In::kBytes / 2, lane};
-        next_k.store(keys, unit.count - at, c.m.key_size);
-        next_v.store(values, unit.count - at, c.m.value_size);
+        next_k.template store<E, N, false>(keys, unit.count - at, c.m.key_size, nullptr);
+        next_v.template store<E, N, false>(values, unit.count - at, c.m.value_size, nullptr);
         __syncthreads();
         if (at + R < unit.count) {
             next_k.load(k + (at + R) * c.m.k.row, c.m.k.row, unit.count - at - R, c.m.key_size);
             next_v.load(v + (at + R) * c.m.v.row, c.m.v.row, unit.count - at - R, c.m.value_size);
             if (wave == 0) gate = gate_of_lane<T, R>(c, unit.first + at + R, unit.count - at - R, head);
         }
-        state.times(reaches[turn].whole);
-        state.template add_weighted<kWhole>(keys, values, column, reaches[turn].column);
+        Operand<E, N> mine[R / 32][W];
+        columns_of(values, column, mine);
+        state.template fold<T>(reaches[turn].whole, keys, mine, reaches[turn].column);
         if (wave == 0 && at + R < unit.count) reach_of(c, reaches[turn ^ 1], gate, unit.count - at - R, before);
         __syncthreads();
     }
@@ -55,8 +57,10 @@ __global__ __launch_bounds__(kThreads<D>, waves_of_simd(kThreads<D>, kStatesLds<
 template <class T, int D, bool Vector>
 __global__ __launch_bounds__(kThreads<D>, waves_of_simd(kThreads<D>, kOutputsLds<T, D>, W * D / 4)) void attention_outputs_kernel(AttentionCall c) {
     constexpr int R = Parts<T>::kRows, N = Parts<T>::kInput, M = Parts<T>::kState, kTiles = R / 16, kWaves = State<D, W>::kWaves;
-    using In = Tile<N, R, D>;
-    using Pairs = Tile<N, R, R>;
+    constexpr bool kScaled = Parts<T>::kScaled;
+    using E = typename Parts<T>::Element;
+    using In = Tile<E, N, R, D>;
+    using Pairs = Tile<E, N, R, R>;
     extern __shared__ __attribute__((aligned(16))) char lds[];
     Reach<R> *reaches = (Reach<R> *)(lds + 3 * In::kBytes + Pairs::kBytes);
     const int64_t which = blockIdx.x / c.m.heads;  // a unit, or a sequence
@@ -93,25 +97,31 @@ __global__ __launch_bounds__(kThreads<D>, waves_of_simd(kThreads<D>, kOutputsLds
     if (unit.count > 0) load(0);
     float gate = 0.0f;  // of the next chunk's row, in the first wave
     if (wave == 0) reach_of(c, reaches[0], gate_of_lane<T, R>(c, unit.first, unit.count, head), unit.count, before);
+    if (kScaled) {
+        if (threadIdx.x < 4) reaches[0].largest[threadIdx.x] = 0;
+        __syncthreads();
+    }
     int turn = 0, chunk = 0;
     for (int64_t at = 0; at < unit.count; at += R, turn ^= 1) {
         const int lane = lane_of_turn();
-        const In queries{(__bf16 *)lds, lane}, keys{(__bf16 *)(lds + In::kBytes), lane}, values{(__bf16 *)(lds + 2 * In::kBytes), lane};
-        const Pairs pairs{(__bf16 *)(lds + 3 * In::kBytes), lane};
+        const In queries{(E *)lds, lane}, keys{(E *)(lds + In::kBytes), lane}, values{(E *)(lds + 2 * In::kBytes), lane};
+        const Pairs pairs{(E *)(lds + 3 * In::kBytes), lane};
         if (c.through && c.states && chunk == 0) {
             if (u < c.most_units) state.template store<false>(c.states + (u * c.m.heads + head) * state_size, column, c.m.key_size, c.m.value_size);
             u++;
         }
         chunk = chunk + 1 == c.chunks ? 0 : chunk + 1;
-        next_q.store(queries, unit.count - at, c.m.key_size);
-        next_k.store(keys, unit.count - at, c.m.key_size);
-        next_v.store(values, unit.count - at, c.m.value_size);
+        next_q.template store<E, N, kScaled>(queries, unit.count - at, c.m.key_size, &reaches[turn].largest[0]);
+        next_k.template store<E, N, kScaled>(keys, unit.count - at, c.m.key_size, &reaches[turn].largest[1]);
+        next_v.template store<E, N, false>(values, unit.count - at, c.m.value_size, nullptr);
         __syncthreads();
+        if (kScaled && threadIdx.x < 4) reaches[turn ^ 1].largest[threadIdx.x] = 0;
         if (at + R < unit.count) {
             load(at + R);
             if (wave == 0) gate = gate_of_lane<T, R>(c, unit.first + at + R, unit.count - at - R, head);
         }
         const Reach<R> &reach = reaches[turn];
+        const Scaling scaling = scaling_of_pairs<T>(reach, 0, 1, c.m.key_size, c.m.scale);
         // pairs: row s, column r
 #pragma unroll 1
         for (int tile = wave; tile < kTiles * kTiles; tile += kWaves) {
@@ -121,30 +131,21 @@ __global__ __launch_bounds__(kThreads<D>, waves_of_simd(kThreads<D>, kOutputsLds
             if (r <= s) {
 #pragma unroll
                 for (int i = 0; i < D; i += 32) p = product(keys.straight(16 * r, i), queries.straight(16 * s, i), p);
-                p *= decays_of<true>(reach, 16 * r, 16 * s, c.m.scale, lane);
+                p *= decays_of<true>(reach, 16 * r, 16 * s, c.m.scale * scaling.up, lane);
             }
             pairs.put(16 * s, 16 * r, p);
         }
         floatx4 read[kTiles][W] = {};
-        state.template read_by<M>(queries, read);
+        const float down = state.template read_by<T, M>(queries, read);
         __syncthreads();
-        Operand<N> mine[R / 32][W];
-#pragma unroll
-        for (int n = 0; n < R / 32; n++)
-#pragma unroll
-            for (int w = 0; w < W; w++) mine[n][w] = values.transposed(32 * n, column + 16 * w);
-#pragma unroll
-        for (int s = 0; s < kTiles; s++) {
-            const float decay = reach.row[16 * s + lane % 16];
+        Operand<E, N> mine[R / 32][W];
+        columns_of(values, column, mine);
+        each_of<kTiles>([&](auto number) {
+            constexpr int s = decltype(number)::value;
+            const float decay = reach.row[16 * s + lane % 16] * down;
 #pragma unroll
             for (int w = 0; w < W; w++) read[s][w] *= decay;
-#pragma unroll
-            for (int n = 0; n < R / 32; n++)
-                if (2 * n <= s) {
-                    const Operand<N> p = pairs.chained(16 * s, 32 * n);
-#pragma unroll
-                    for (int w = 0; w < W; w++) read[s][w] = product(mine[n][w], p, read[s][w]);
-                }
+            add_pairs<T, 0, s / 2 + 1>(pairs, 16 * s, mine, scaling.down, read[s]);
             in_order();
             const int to = column + 4 * (lane / 16);
             if (16 * s + lane % 16 < unit.count - at) {
@@ -152,15 +153,8 @@ __global__ __launch_bounds__(kThreads<D>, waves_of_simd(kThreads<D>, kOutputsLds
                 for (int w = 0; w < W; w++)
                     put_row(out + (at + 16 * s) * out_row + 16 * w, (uint32_t)(lane % 16 * (int)out_row + to), to + 16 * w, c.m.value_size, Vector, read[s][w]);
             }
-        }
-        state.times(reach.whole);
-#pragma unroll
-        for (int n = 0; n < R / 32; n++) {
-            Operand<kWhole> late[W];
-#pragma unroll
-            for (int w = 0; w < W; w++) late[w] = weighted<kWhole>(mine[n][w], reach.column, 32 * n, lane);
-            state.add(keys, 32 * n, late);
-        }
+        });
+        state.template fold<T>(reach.whole, keys, mine, reach.column);
         if (wave == 0 && at + R < unit.count) reach_of(c, reaches[turn ^ 1], gate, unit.count - at - R, before);
         __syncthreads();
     }
