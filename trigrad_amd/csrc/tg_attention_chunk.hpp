@@ -108,23 +108,25 @@ __device__ __forceinline__ Scaling scaling_of(uint32_t largest_bits) {
     return {__uint_as_float((uint32_t)exponent << 23), __uint_as_float((uint32_t)(254 - exponent) << 23)};
 }
 
-// A matrix of Rows x Columns in LDS, N parts.  Rows are 16 bytes longer than their numbers, so that sixteen rows begin in different banks.
-template <class E, int N, int Rows, int Columns> struct Tile {
+// A matrix of Rows x Columns in LDS, N parts.  One that is only read by rows has rows 16 bytes longer than their numbers, so that sixteen rows begin in
+// different banks; one that is read transposed too, 32 bytes of four rows at once, has them 32 bytes longer, which sets eight rows apart, and the
+// other eight of sixteen with neighbouring 16 bytes exchanged: no reading meets another in a bank.
+template <class E, int N, int Rows, int Columns, bool Turned = true> struct Tile {
     using x8 = typename Vectors<E>::x8;
     using x4 = typename Vectors<E>::x4;
-    static constexpr int kStride = Columns + 8, kPart = Rows * kStride, kBytes = N * kPart * 2;
+    static constexpr int kExchanged = Turned ? 8 : 0, kStride = Columns + (Turned ? 16 : 8), kPart = Rows * kStride, kBytes = N * kPart * 2;
     E *at;
     int lane;
 
     __device__ __forceinline__ Operand<E, N> straight(int row, int column) const {
-        const E *p = at + (row + lane % 16) * kStride + column + 8 * (lane / 16);
+        const E *p = at + (row + lane % 16) * kStride + column + (8 * (lane / 16) ^ (lane & kExchanged));
         Operand<E, N> o;
 #pragma unroll
         for (int n = 0; n < N; n++) o.part[n] = *(const x8 *)(p + n * kPart);
         return o;
     }
     __device__ __forceinline__ Operand<E, N> chained(int row, int column) const {
-        const E *p = at + (row + lane % 16) * kStride + column + 4 * (lane / 16);
+        const E *p = at + (row + lane % 16) * kStride + column + (4 * (lane / 16) ^ (lane & kExchanged));
         Operand<E, N> o;
 #pragma unroll
         for (int n = 0; n < N; n++) {
@@ -136,7 +138,8 @@ template <class E, int N, int Rows, int Columns> struct Tile {
     // The transposed matrix's: row or column `column` + lane % 16, chained rows from `row`.  LDS hands out four rows of sixteen columns transposed to
     // sixteen lanes, of which each points at four neighbours of a row.
     __device__ __forceinline__ Operand<E, N> transposed(int row, int column) const {
-        const E *p = at + (row + 4 * (lane / 16) + lane % 16 / 4) * kStride + column + 4 * (lane % 4);
+        static_assert(Turned);
+        const E *p = at + (row + 4 * (lane / 16) + lane % 16 / 4) * kStride + column + (4 * (lane % 4) ^ (lane >> 2 & kExchanged));
         Operand<E, N> o;
 #pragma unroll
         for (int n = 0; n < N; n++) {
@@ -148,12 +151,13 @@ template <class E, int N, int Rows, int Columns> struct Tile {
     static __device__ __forceinline__ x4 turned(const E *p) {
         return __builtin_bit_cast(x4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) short4_t *)p));
     }
-    // Four neighbours of a row, as numbers.
+    // Four neighbours, as an accumulator has them: of row `row` + lane % 16, from `column` + 4 (lane / 16) on.
     __device__ __forceinline__ floatx4 numbers(int row, int column) const {
+        const E *p = at + (row + lane % 16) * kStride + column + (4 * (lane / 16) ^ (lane & kExchanged));
         floatx4 x = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
         for (int n = N - 1; n >= 0; n--) {
-            const x4 v = *(const x4 *)(at + n * kPart + row * kStride + column);
+            const x4 v = *(const x4 *)(p + n * kPart);
 #pragma unroll
             for (int j = 0; j < 4; j++) x[j] += (float)v[j];
         }
@@ -161,6 +165,7 @@ template <class E, int N, int Rows, int Columns> struct Tile {
     }
     // An accumulator's four rows (columns here) of its column (a row here): the product's transpose.
     __device__ __forceinline__ void put(int row, int column, floatx4 x) const {
+        static_assert(!Turned);
         E *p = at + (row + lane % 16) * kStride + column + 4 * (lane / 16);
 #pragma unroll
         for (int n = 0; n < N; n++) {
@@ -217,10 +222,11 @@ template <class T, int Rows, int D, int Threads, bool Vector> struct Incoming {
 #pragma unroll
         for (int n = 0; n < kGroups; n++) {
             if (!mine(n)) continue;
-            const int row = row_of(n), column = column_of(n);
+            using In = Tile<E, N, Rows, D>;
+            const int row = row_of(n), column = column_of(n), place = row * In::kStride + (column ^ (row & In::kExchanged));
             if constexpr (Vector && N == 1) {  // as it is
                 const uint32x4 w = __builtin_bit_cast(uint32x4, x[n][0]), none = {0, 0, 0, 0}, v = row < count && column < size ? w : none;
-                *(uint32x4 *)(tile.at + row * Tile<E, N, Rows, D>::kStride + column) = v;
+                *(uint32x4 *)(tile.at + place) = v;
                 if constexpr (Scaled) {
 #pragma unroll
                     for (int j = 0; j < 4; j++) most = max(most, max(v[j] & 0x7fffu, v[j] >> 16 & 0x7fffu));
@@ -233,7 +239,7 @@ template <class T, int Rows, int D, int Threads, bool Vector> struct Incoming {
             const Operand<E, N> o = parts_of<E, N>(v);
 #pragma unroll
             for (int i = 0; i < N; i++)
-                *(typename Vectors<E>::x8 *)(tile.at + i * Tile<E, N, Rows, D>::kPart + row * Tile<E, N, Rows, D>::kStride + column) = o.part[i];
+                *(typename Vectors<E>::x8 *)(tile.at + i * In::kPart + place) = o.part[i];
             if constexpr (Scaled) {
                 const uint32x4 w = __builtin_bit_cast(uint32x4, o.part[0]);
 #pragma unroll
@@ -554,7 +560,7 @@ __device__ __forceinline__ void columns_of(const Tile<E, N, Rows, D> &tile, int 
 
 // += this wave's columns times sixteen rows of pairs from `row` on, those of the columns from First on to before Last.
 template <class T, int First, int Last, class E, int N, int Rows, int W>
-__device__ __forceinline__ void add_pairs(const Tile<E, N, Rows, Rows> &pairs, int row, const Operand<E, N> (&mine)[Rows / 32][W], float down, floatx4 (&sums)[W]) {
+__device__ __forceinline__ void add_pairs(const Tile<E, N, Rows, Rows, false> &pairs, int row, const Operand<E, N> (&mine)[Rows / 32][W], float down, floatx4 (&sums)[W]) {
     floatx4 inside[W] = {};
 #pragma unroll
     for (int k = First; k < Last; k++) {
