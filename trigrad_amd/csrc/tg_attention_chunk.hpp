@@ -70,7 +70,25 @@ template <class E, int NA, int NB> __device__ __forceinline__ floatx4 product(co
     return sum;
 }
 
+// What two numbers' roundings leave of them: sums of two products and a number, exact here, one instruction each where taking a rounded number out of its
+// half and subtracting it are two.  -1 and 0 come from a register: the compiler writes them as constants of another type into the instruction.
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef _Float16 halfx2 __attribute__((ext_vector_type(2)));
+__device__ __forceinline__ void without(bf16x2 rounded, float &x, float &y) {
+    uint32_t first = 0x0000bf80u, second = 0xbf800000u;
+    asm("" : "+s"(first), "+s"(second));
+    x = __builtin_amdgcn_fdot2_f32_bf16(rounded, __builtin_bit_cast(bf16x2, first), x, false);
+    y = __builtin_amdgcn_fdot2_f32_bf16(rounded, __builtin_bit_cast(bf16x2, second), y, false);
+}
+__device__ __forceinline__ void without(halfx2 rounded, float &x, float &y) {
+    uint32_t first = 0x0000bc00u, second = 0xbc000000u;
+    asm("" : "+s"(first), "+s"(second));
+    x = __builtin_amdgcn_fdot2(rounded, __builtin_bit_cast(halfx2, first), x, false);
+    y = __builtin_amdgcn_fdot2(rounded, __builtin_bit_cast(halfx2, second), y, false);
+}
+
 template <class E, int N> __device__ __forceinline__ Operand<E, N> parts_of(const float *x) {
+    typedef E x2 __attribute__((ext_vector_type(2)));
     Operand<E, N> o;
     float rest[8];
 #pragma unroll
@@ -78,9 +96,11 @@ template <class E, int N> __device__ __forceinline__ Operand<E, N> parts_of(cons
 #pragma unroll
     for (int n = 0; n < N; n++)
 #pragma unroll
-        for (int j = 0; j < 8; j++) {
-            o.part[n][j] = (E)rest[j];
-            if (n + 1 < N) rest[j] -= (float)o.part[n][j];
+        for (int j = 0; j < 8; j += 2) {
+            const x2 rounded = {(E)rest[j], (E)rest[j + 1]};
+            o.part[n][j] = rounded[0];
+            o.part[n][j + 1] = rounded[1];
+            if (n + 1 < N) without(rounded, rest[j], rest[j + 1]);
         }
     return o;
 }
