@@ -181,35 +181,39 @@ __global__ __launch_bounds__(kPlanThreads) void attention_plan_kernel(Attention 
     for (int64_t i = before + threadIdx.x; i < most; i += kPlanThreads) plan[i] = -1;
 }
 
-// From what units add to a state, the states in front of them (or behind them, from the last to the first): x' = decay x + added.  A thread has an
-// element of the state and reads eight units ahead.
+// From what units add to a state, the states in front of them (or behind them, from the last to the first): x' = decay x + added.  A thread has V
+// neighbours of the state and reads eight units ahead.
+template <int V>
 __global__ __launch_bounds__(kScanThreads) void attention_scan_kernel(AttentionCall c, float *__restrict__ states, const float *__restrict__ from, float *__restrict__ to,
                                                                       int64_t unit_rows, bool back) {
     constexpr int kAhead = 8;
-    const int64_t s = blockIdx.x / c.m.heads, size = (int64_t)c.m.key_size * c.m.value_size, i = (int64_t)blockIdx.y * kScanThreads + threadIdx.x;
+    const int64_t s = blockIdx.x / c.m.heads, size = (int64_t)c.m.key_size * c.m.value_size, i = ((int64_t)blockIdx.y * kScanThreads + threadIdx.x) * V;
     const int head = (int)(blockIdx.x % c.m.heads);
     if (i >= size) return;
     int64_t first;
     const int64_t count = units_of(c, s, unit_rows, first);
-    float x = from ? from[(s * c.m.heads + head) * size + i] : 0.0f;
+    Pack<float, V> x = {};
+    if (from) x = load_pack<V>(from + (s * c.m.heads + head) * size + i);
     for (int64_t n = 0; n < count; n += kAhead) {
-        float added[kAhead], decay[kAhead];
+        Pack<float, V> added[kAhead];
+        float decay[kAhead];
 #pragma unroll
         for (int j = 0; j < kAhead; j++) {
-            const int64_t unit = (first + (back ? count - 1 - n - j : n + j)) * c.m.heads + head;
-            added[j] = n + j < count ? states[unit * size + i] : 0.0f;
-            decay[j] = n + j < count ? c.decays[unit] : 0.0f;
+            const int64_t here = min(n + j, count - 1), unit = (first + (back ? count - 1 - here : here)) * c.m.heads + head;
+            added[j] = load_pack<V>(states + unit * size + i);
+            decay[j] = c.decays[unit];
         }
 #pragma unroll
         for (int j = 0; j < kAhead; j++) {
             const int64_t unit = (first + (back ? count - 1 - n - j : n + j)) * c.m.heads + head;
             if (n + j < count) {
-                states[unit * size + i] = x;
-                x = fmaf(decay[j], x, added[j]);
+                store_pack<V>(states + unit * size + i, x.v);
+#pragma unroll
+                for (int v = 0; v < V; v++) x.v[v] = fmaf(decay[j], x.v[v], added[j].v[v]);
             }
         }
     }
-    if (to) to[(s * c.m.heads + head) * size + i] = x;
+    if (to) store_pack<V>(to + (s * c.m.heads + head) * size + i, x.v);
 }
 
 // dlog a of a unit's rows: <S, D> in front of it, and what changes it from row to row.
@@ -289,24 +293,46 @@ __global__ void attention_fixed_gates_kernel(Attention m, const S *__restrict__ 
     if (threadIdx.x == 0) grad_gates[h] = (S)(real)(all * slope_of(m.gate_form, wide(gates[h])));
 }
 
-// Key heads' gradients, the sums of their value heads'.
-template <class T, class P>
-__global__ void attention_shared_kernel(Attention m, const P *__restrict__ parts, T *__restrict__ out) {
-    const int64_t id = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
-    if (id >= m.rows * m.key_heads * m.key_size) return;
-    const int64_t i = id % m.key_size, head = id / m.key_size;  // row and key head
-    P sum = 0;
-    for (int n = 0; n < m.shared; n++) sum += parts[(head * m.shared + n) * m.key_size + i];
-    out[id] = (T)(real)sum;
+constexpr int kSharedThreads = 256;
+
+// Key heads' gradients, the sums of their value heads': of queries (y = 0) and of keys.  A row of `lanes` threads (a power of two) has one key head of
+// one row, a thread V of its numbers.
+template <class T, class P, int V> struct SharedParts {
+    const P *parts[2];
+    T *out[2];
+};
+template <class T, class P, int V> __global__ __launch_bounds__(kSharedThreads) void attention_shared_kernel(Attention m, int lanes, SharedParts<T, P, V> both) {
+    const P *parts = both.parts[blockIdx.y];
+    T *out = both.out[blockIdx.y];
+    const int i = threadIdx.x % lanes * V;
+    if (!out || i >= m.key_size) return;
+    const int64_t step = (int64_t)gridDim.x * (kSharedThreads / lanes);
+    for (int64_t head = (int64_t)blockIdx.x * (kSharedThreads / lanes) + threadIdx.x / lanes; head < m.rows * m.key_heads; head += step) {  // row and key head
+        P sum[V] = {};
+#pragma unroll 4
+        for (int n = 0; n < m.shared; n++) {
+            const Pack<P, V> part = load_pack<V>(parts + (head * m.shared + n) * m.key_size + i);
+#pragma unroll
+            for (int v = 0; v < V; v++) sum[v] += part.v[v];
+        }
+        real to[V];
+#pragma unroll
+        for (int v = 0; v < V; v++) to[v] = (real)sum[v];
+        store_pack<V>(out + head * m.key_size + i, to);
+    }
 }
 
-// Rows in front of the first sequence and behind the last one: zeros.
-template <class T> __global__ void attention_outside_kernel(Attention m, const int32_t *__restrict__ offsets, int64_t width, T *__restrict__ out) {
+// Rows in front of the first sequence and behind the last one: zeros, in each of up to four tensors (y) whose rows have `width` pieces of 16 bits.
+struct Outside {
+    uint16_t *out[4];
+    int64_t width[4];
+};
+__global__ void attention_outside_kernel(Attention m, const int32_t *__restrict__ offsets, Outside all) {
     const AttentionRows first = rows_of(m, offsets, 0), last = rows_of(m, offsets, m.sequences - 1);
-    const int64_t end = last.first + last.count, begin = min(first.first, end), outside = m.rows - end + begin;
-    for (int64_t id = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; id < outside * width; id += (int64_t)gridDim.x * blockDim.x) {
-        const int64_t row = id / width;
-        out[(row < begin ? row : row - begin + end) * width + id % width] = (T)(real)0;
+    const int64_t end = last.first + last.count, begin = min(first.first, end), outside = m.rows - end + begin, width = all.width[blockIdx.y];
+    for (int64_t row = blockIdx.x; row < outside; row += gridDim.x) {
+        uint16_t *out = all.out[blockIdx.y] + (row < begin ? row : row - begin + end) * width;
+        for (int64_t i = threadIdx.x; i < width; i += blockDim.x) out[i] = 0;
     }
 }
 
@@ -342,16 +368,39 @@ int attention_shape(const char *fn, const tg_attention &a, Attention &m) {
 
 static unsigned blocks_for(int64_t n) { return (unsigned)std::min<int64_t>(ceil_div64(n, 256), 1 << 20); }
 
-template <class T> static void clear_outside(const tg_attention &a, const Attention &m, T *out, int64_t width) {
-    if (!m.packed || !m.rows || !out) return;
-    TG_LAUNCH_AS("attention_outside", (attention_outside_kernel<T>), dim3(std::min(blocks_for(m.rows * width), 4096u)), dim3(256), 0, (hipStream_t)a.stream, m,
-                 a.offsets, width, out);
+static void clear_outside(const tg_attention &a, const Attention &m, std::initializer_list<std::pair<void *, int64_t>> tensors) {  // and bytes of a row
+    Outside all = {};
+    unsigned n = 0;
+    for (const auto &t : tensors)
+        if (t.first) all.out[n] = (uint16_t *)t.first, all.width[n++] = t.second / 2;
+    if (!m.packed || !m.rows || !n) return;
+    TG_LAUNCH_AS("attention_outside", attention_outside_kernel, dim3((unsigned)std::min<int64_t>(m.rows, 1024), n), dim3(256), 0, (hipStream_t)a.stream, m, a.offsets, all);
+}
+template <class T> static void clear_outputs(const tg_attention &a, const Attention &m) {
+    clear_outside(a, m, {{a.outputs, (int64_t)sizeof(T) * m.heads * m.value_size}});
 }
 template <class T, class S> static void clear_gradients(const tg_attention &a, const Attention &m) {
-    clear_outside(a, m, (T *)a.grad_queries, (int64_t)m.key_heads * m.key_size);
-    clear_outside(a, m, (T *)a.grad_keys, (int64_t)m.key_heads * m.key_size);
-    clear_outside(a, m, (T *)a.grad_values, (int64_t)m.heads * m.value_size);
-    if (!m.fixed) clear_outside(a, m, (S *)a.grad_gates, (int64_t)m.heads);
+    const int64_t keys = (int64_t)sizeof(T) * m.key_heads * m.key_size;
+    clear_outside(a, m, {{a.grad_queries, keys}, {a.grad_keys, keys}, {a.grad_values, (int64_t)sizeof(T) * m.heads * m.value_size},
+                         {m.fixed ? nullptr : a.grad_gates, (int64_t)sizeof(S) * m.heads}});
+}
+
+template <class T, class P> static void add_shared(const tg_attention &a, const Attention &m, const P *queries, const P *keys) {
+    const auto launch = [&](auto vector) {
+        constexpr int V = decltype(vector)::value;
+        int lanes = 1;
+        while (lanes * V < m.key_size) lanes *= 2;
+        const SharedParts<T, P, V> both = {{queries, keys}, {(T *)a.grad_queries, (T *)a.grad_keys}};
+        const int64_t groups = ceil_div64(m.rows * m.key_heads, kSharedThreads / lanes);
+        TG_LAUNCH_AS("attention_shared", (attention_shared_kernel<T, P, V>), dim3((unsigned)std::min<int64_t>(groups, 1 << 16), 2), dim3(kSharedThreads), 0,
+                     (hipStream_t)a.stream, m, lanes, both);
+    };
+    if (!m.rows || (!a.grad_queries && !a.grad_keys)) return;
+    constexpr int kWidest = 16 / (int)sizeof(P);
+    if (m.key_size % kWidest == 0 && (uintptr_t)a.grad_queries % 16 == 0 && (uintptr_t)a.grad_keys % 16 == 0 && (uintptr_t)a.workspace % 16 == 0)
+        launch(std::integral_constant<int, kWidest>());
+    else
+        launch(std::integral_constant<int, 1>());
 }
 
 #ifdef TG_DOUBLE_PRECISION
@@ -373,7 +422,7 @@ template <class T, class S> static int walk_forward(const tg_attention &a, const
     TG_LAUNCH_AS("attention_walk", (attention_walk_kernel<T, S>), dim3((unsigned)(m.sequences * m.heads), (unsigned)ceil_div(m.value_size, kWalkThreads)),
                  dim3(kWalkThreads), 0, stream, m, (const T *)a.queries, (const T *)a.keys, (const T *)a.values, (const S *)a.gates, a.initial, a.offsets,
                  (T *)a.outputs, a.final);
-    clear_outside(a, m, (T *)a.outputs, (int64_t)m.heads * m.value_size);
+    clear_outputs<T>(a, m);
     return check_launch("tg_linear_attention_forward");
 }
 
@@ -407,12 +456,7 @@ template <class T, class S> static int walk_backward(const tg_attention &a, cons
     const int64_t states = m.sequences * m.heads * m.key_size * m.value_size;
     if (a.grad_initial)
         TG_LAUNCH_AS("attention_round", (attention_round_kernel<real>), dim3(blocks_for(states)), dim3(256), 0, stream, dstate, states, a.grad_initial);
-    const int64_t n = m.rows * m.key_heads * m.key_size;
-    for (int which = 0; which < 2; which++) {
-        T *out = (T *)(which ? a.grad_keys : a.grad_queries);
-        if (out && n)
-            TG_LAUNCH_AS("attention_shared", (attention_shared_kernel<T, double>), dim3((unsigned)ceil_div64(n, 256)), dim3(256), 0, stream, m, which ? dk : dq, out);
-    }
+    add_shared<T>(a, m, dq, dk);
     clear_gradients<T, S>(a, m);
     return check_launch("tg_linear_attention_backward");
 }
@@ -547,8 +591,15 @@ static AttentionCall call_of(const tg_attention &a, const Attention &m, const Sp
 
 static void scan(const AttentionCall &c, const Split &s, float *states, const float *from, float *to, bool back, hipStream_t stream) {
     const int64_t size = (int64_t)c.m.key_size * c.m.value_size;
-    TG_LAUNCH_AS("attention_scan", attention_scan_kernel, dim3((unsigned)(c.m.sequences * c.m.heads), (unsigned)ceil_div64(size, kScanThreads)), dim3(kScanThreads), 0, stream,
-                 c, states, from, to, s.rows_of_chunk * s.chunks, back);
+    const auto launch = [&](auto vector) {
+        constexpr int V = decltype(vector)::value;
+        TG_LAUNCH_AS("attention_scan", (attention_scan_kernel<V>), dim3((unsigned)(c.m.sequences * c.m.heads), (unsigned)ceil_div64(size, kScanThreads * V)),
+                     dim3(kScanThreads), 0, stream, c, states, from, to, s.rows_of_chunk * s.chunks, back);
+    };
+    if (size % 4 == 0 && ((uintptr_t)states | (uintptr_t)from | (uintptr_t)to) % 16 == 0)
+        launch(std::integral_constant<int, 4>());
+    else
+        launch(std::integral_constant<int, 1>());
 }
 
 static int forward(const tg_attention &a, const Attention &m) {
@@ -576,7 +627,7 @@ static int forward(const tg_attention &a, const Attention &m) {
     }
     if ((code = launch_attention_forward(a.type, c, (int)s.size, false, stream))) return code;
     return by_types(a.type, a.gate_type, [&](auto t, auto) {
-        clear_outside(a, m, (decltype(t) *)a.outputs, (int64_t)m.heads * m.value_size);
+        clear_outputs<decltype(t)>(a, m);
         return check_launch("tg_linear_attention_forward");
     });
 }
@@ -611,13 +662,7 @@ template <class T, class S> static int backward(const tg_attention &a, const Att
             TG_LAUNCH_AS("attention_fixed_gates", (attention_fixed_gates_kernel<S>), dim3((unsigned)m.heads), dim3(kWalkThreads), 0, stream, m, (const S *)a.gates, c.sums,
                          m.rows ? s.most_units : 0, (S *)a.grad_gates);
     }
-    const int64_t n = m.rows * m.key_heads * m.key_size;
-    for (int which = 0; which < 2 && m.shared > 1; which++) {
-        T *out = (T *)(which ? a.grad_keys : a.grad_queries);
-        if (out && n)
-            TG_LAUNCH_AS("attention_shared", (attention_shared_kernel<T, float>), dim3((unsigned)ceil_div64(n, 256)), dim3(256), 0, stream, m,
-                         (const float *)(which ? c.grad_keys : c.grad_queries), out);
-    }
+    if (m.shared > 1) add_shared<T>(a, m, (const float *)c.grad_queries, (const float *)c.grad_keys);
     clear_gradients<T, S>(a, m);
     return check_launch("tg_linear_attention_backward");
 }
