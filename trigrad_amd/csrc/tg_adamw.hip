@@ -110,15 +110,18 @@ __device__ __forceinline__ uint32_t to8(const float *x) {
 
 // ---- the kernel ---------------------------------------------------------------------------
 
-// Four elements of a block: neighbours in one access (Wide), or 64 apart for tensors that begin off alignment and ends of tensors.
-template <bool Wide, class T> __device__ __forceinline__ void take4(const T *p, uint32_t lane, uint32_t left, T *x) {
+// Four elements of a block that begins at `at`: neighbours in one access (Wide), or 64 apart for tensors that begin off alignment and ends of tensors,
+// zeros behind the end.  All loads are made, in place of those behind the end the last element's, so that none waits for another's result.
+template <bool Wide, class T> __device__ __forceinline__ void take4(const T *p, uint32_t at, uint32_t lane, uint32_t size, T *x) {
     if (Wide) {
-        const Pack<T, 4> v = load_pack<4>(p + 4 * lane);
+        const Pack<T, 4> v = load_pack<4>(p + at + 4 * lane);
 #pragma unroll
         for (int j = 0; j < 4; j++) x[j] = v.v[j];
     } else {
 #pragma unroll
-        for (int j = 0; j < 4; j++) x[j] = lane + 64 * j < left ? p[lane + 64 * j] : (T)0.0f;
+        for (int j = 0; j < 4; j++) x[j] = p[min(at + lane + 64 * j, size - 1)];
+#pragma unroll
+        for (int j = 0; j < 4; j++) x[j] = at + lane + 64 * j < size ? x[j] : (T)0.0f;
     }
 }
 template <bool Wide, class T> __device__ __forceinline__ void put4(T *p, uint32_t lane, uint32_t left, const real *x) {
@@ -139,28 +142,31 @@ template <class G, class C, int Bits> struct AdamwBlock {  // what a lane has of
 };
 
 template <bool Wide, class G, class C, int Bits>
-__device__ __forceinline__ void load_block(AdamwBlock<G, C, Bits> &b, const AdamwLaunch<C, Bits> &a, int n, uint32_t at, uint32_t lane, uint32_t left) {
-    take4<Wide>((const G *)a.g[n] + at, lane, left, b.g);
-    take4<Wide>(a.p[n] + at, lane, left, b.p);
+__device__ __forceinline__ void load_block(AdamwBlock<G, C, Bits> &b, const AdamwLaunch<C, Bits> &a, int n, uint32_t at, uint32_t lane, uint32_t size) {
+    take4<Wide>((const G *)a.g[n], at, lane, size, b.g);
+    take4<Wide>(a.p[n], at, lane, size, b.p);
     if constexpr (Bits == 8) {
-        const uint8_t *m = (const uint8_t *)a.m[n] + at, *v = (const uint8_t *)a.v[n] + at;
+        const uint8_t *m = (const uint8_t *)a.m[n], *v = (const uint8_t *)a.v[n];
         if (Wide) {
-            b.m8 = *(const uint32_t *)(m + 4 * lane);
-            b.v8 = *(const uint32_t *)(v + 4 * lane);
+            b.m8 = *(const uint32_t *)(m + at + 4 * lane);
+            b.v8 = *(const uint32_t *)(v + at + 4 * lane);
         } else {
+            uint8_t m4[4], v4[4];
+            take4<false>(m, at, lane, size, m4);
+            take4<false>(v, at, lane, size, v4);
             b.m8 = b.v8 = 0;
 #pragma unroll
-            for (int j = 0; j < 4; j++)
-                if (lane + 64 * j < left) {
-                    b.m8 |= (uint32_t)m[lane + 64 * j] << 8 * j;
-                    b.v8 |= (uint32_t)v[lane + 64 * j] << 8 * j;
-                }
+            for (int j = 0; j < 4; j++) {
+                b.m8 |= (uint32_t)m4[j] << 8 * j;
+                b.v8 |= (uint32_t)v4[j] << 8 * j;
+            }
         }
-        b.scale_m = a.scales[n][at / kBlock * 2];
-        b.scale_r = a.scales[n][at / kBlock * 2 + 1];
+        const uint32_t block = Wide ? at / kBlock : min(at, size - 1) / kBlock;
+        b.scale_m = a.scales[n][block * 2];
+        b.scale_r = a.scales[n][block * 2 + 1];
     } else {
-        take4<Wide>((const real *)a.m[n] + at, lane, left, b.m);
-        take4<Wide>((const real *)a.v[n] + at, lane, left, b.v);
+        take4<Wide>((const real *)a.m[n], at, lane, size, b.m);
+        take4<Wide>((const real *)a.v[n], at, lane, size, b.v);
     }
 }
 
@@ -241,21 +247,21 @@ template <class G, class C, int Bits> __global__ __launch_bounds__(kThreads) voi
     const uint32_t size = a.size[n], begin = (blockIdx.x - a.piece[n]) * (uint32_t)kPiece + wave * kBlock;
     const AdamwFactors f = factors_of(a);
     const bool wide = (a.wide[n >> 6] >> (n & 63) & 1) != 0;
+    AdamwBlock<G, C, Bits> b[kTurns];
     if (wide && begin + (kTurns - 1) * 4 * kBlock + kBlock <= size) {
-        AdamwBlock<G, C, Bits> b[kTurns];
 #pragma unroll
-        for (int u = 0; u < kTurns; u++) load_block<true>(b[u], a, n, begin + u * 4 * kBlock, lane, kBlock);
+        for (int u = 0; u < kTurns; u++) load_block<true>(b[u], a, n, begin + u * 4 * kBlock, lane, size);
 #pragma unroll
         for (int u = 0; u < kTurns; u++) step_block<true>(b[u], a, f, n, begin + u * 4 * kBlock, lane, kBlock);
         return;
     }
+    if (begin >= size) return;
+#pragma unroll
+    for (int u = 0; u < kTurns; u++) load_block<false>(b[u], a, n, begin + u * 4 * kBlock, lane, size);
+#pragma unroll
     for (int u = 0; u < kTurns; u++) {
         const uint32_t at = begin + u * 4 * kBlock;
-        if (at >= size) return;
-        AdamwBlock<G, C, Bits> b;
-        const uint32_t left = size - at;
-        load_block<false>(b, a, n, at, lane, left);
-        step_block<false>(b, a, f, n, at, lane, left);
+        if (at < size) step_block<false>(b[u], a, f, n, at, lane, size - at);
     }
 }
 
