@@ -515,6 +515,13 @@ def test_library_refuses_on_the_host():
     assert lib.tg_linear_attention_sizes(None, sizes) == -1 and lib.tg_linear_attention_forward(None) == -1 and lib.tg_linear_attention_step(None) == -1
     assert lib.tg_linear_attention_forward(C.byref(_lib.Attention(**good))) == -1  # null pointers
     assert lib.tg_linear_attention_step(C.byref(_lib.Attention(**good))) == -1  # more than a row
+    # sequences and heads of which a grid has no room for
+    many = dict(good, sequences=1 << 23, length=1, heads=2, key_heads=2, key_size=1, value_size=1)
+    some = {name: 16 for name in ("queries", "keys", "values", "gates", "initial", "outputs", "final")}
+    assert lib.tg_linear_attention_step(C.byref(_lib.Attention(**many, **some))) == -1 and b"too many" in lib.tg_last_error()
+    double = _lib.load(64)
+    for types, sequences, code in ((dict(type=3, gate_type=3), 1 << 25, -1), (dict(type=3, gate_type=3), (1 << 25) - 1, 0)):
+        assert double.tg_linear_attention_sizes(C.byref(_lib.Attention(**{**many, **types, "sequences": sequences})), sizes) == code
     some = {name: 16 for name in ("queries", "keys", "values", "gates", "outputs", "final")}  # not touched
     asked()
     if sizes[1]:

@@ -13,6 +13,7 @@
 namespace tg {
 
 constexpr int kWalkThreads = 64;
+constexpr int64_t kGridThreads = (int64_t)1 << 32;  // a grid has fewer
 constexpr int kMost = TG_ATTENTION_SIZE;
 
 template <class T> __device__ __forceinline__ double wide(T v) { return (double)(real)v; }
@@ -366,7 +367,12 @@ int attention_shape(const char *fn, const tg_attention &a, Attention &m) {
     return 0;
 }
 
-static unsigned blocks_for(int64_t n) { return (unsigned)std::min<int64_t>(ceil_div64(n, 256), 1 << 20); }
+// A workgroup of `threads` for each sequence and head.
+static int refuse_many(const char *fn, const Attention &m, int threads) {
+    if (m.sequences * m.heads < kGridThreads / threads) return 0;
+    set_error("%s: %lld sequences of %d heads are too many", fn, (long long)m.sequences, m.heads);
+    return TG_E_ARG;
+}
 
 static void clear_outside(const tg_attention &a, const Attention &m, std::initializer_list<std::pair<void *, int64_t>> tensors) {  // and bytes of a row
     Outside all = {};
@@ -455,7 +461,7 @@ template <class T, class S> static int walk_backward(const tg_attention &a, cons
     }
     const int64_t states = m.sequences * m.heads * m.key_size * m.value_size;
     if (a.grad_initial)
-        TG_LAUNCH_AS("attention_round", (attention_round_kernel<real>), dim3(blocks_for(states)), dim3(256), 0, stream, dstate, states, a.grad_initial);
+        TG_LAUNCH_AS("attention_round", (attention_round_kernel<real>), dim3((unsigned)std::min<int64_t>(ceil_div64(states, 256), 1 << 20)), dim3(256), 0, stream, dstate, states, a.grad_initial);
     add_shared<T>(a, m, dq, dk);
     clear_gradients<T, S>(a, m);
     return check_launch("tg_linear_attention_backward");
@@ -463,7 +469,9 @@ template <class T, class S> static int walk_backward(const tg_attention &a, cons
 
 static int64_t room_for_walk(const Attention &m) { return walk_room(m).all; }
 
-static int sizes_of(const char *, const tg_attention &, const Attention &m, int64_t out[4]) {
+static int sizes_of(const char *fn, const tg_attention &, const Attention &m, int64_t out[4]) {
+    const int code = refuse_many(fn, m, kWalkThreads);
+    if (code) return code;
     out[0] = out[1] = out[2] = 0;
     out[3] = room_for_walk(m);
     return 0;
@@ -477,8 +485,6 @@ static_assert(Parts<bf16_t>::kRows == Parts<half_t>::kRows, "rows of a chunk");
 constexpr int64_t kComputeUnits = 256;
 constexpr int64_t kMostChunks = 16;   // of a unit: 1024 rows, beside whose 16 chunks a state that is written and read is little
 constexpr int64_t kMostUnits = 1024;  // of a sequence, which are gone through one after another
-constexpr int64_t kGridThreads = (int64_t)1 << 32;  // a grid has fewer
-
 // How the rows of a call are split, the same forward and backward.
 struct Split {
     int64_t rows_of_chunk, chunks, units, most_units, size;
@@ -808,6 +814,7 @@ extern "C" int tg_linear_attention_step(const tg_attention *a) {
         return TG_E_ARG;
     }
     if (m.sequences == 0) return 0;
+    if ((code = refuse_many(fn, m, kStepThreads))) return code;
     if ((code = check_pointers(fn, {a->queries, a->keys, a->values, a->gates, a->initial, a->outputs, a->final}))) return code;
     return by_types(a->type, a->gate_type, [&](auto t, auto s) { return step<decltype(t), decltype(s)>(*a, m); });
 }
