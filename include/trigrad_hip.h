@@ -663,8 +663,8 @@ int tg_linear_attention_step(const tg_attention *a);
  * bits 32: averages and squares hold m and v as tg_real.  bits 8 (float library): they hold m and sqrt(v) in 8 bits (sign, 4 of
  * exponent, 3 of fraction, largest 448, smallest 2^-9) in units of scales[i][b][0] and [1] for elements 256 b to 256 b + 255 of
  * tensor i: the block's largest / 448.  A value becomes one of its two neighbours, the upper one with the probability of what lies
- * below, by 16 bits of a number mixed of `seed` and the element's place (the tensors laid end to end, each from a multiple of
- * 256), so that an average of many small changes moves as it should; a square that is not zero does not become zero. */
+ * below, by 16 bits of a number mixed of `seed` (with device_step: seed + t) and the element's place (the tensors laid end to end,
+ * each from a multiple of 256), so that an average of many small changes moves as it should; a square that is not zero does not become zero. */
 typedef struct tg_adamw {
     tg_real *const *params;
     const void *const *grads;

@@ -325,6 +325,34 @@ def test_captured_steps(cuda, bits):
 
 
 @pytest.mark.gpu
+def test_replays_round_as_steps_do(cuda):
+    """Averages in 8 bits are rounded with the step's number, also where the device counts: those of replays are those of eager steps without a
+    count on the device, and small changes are not lost."""
+    import trigrad_amd
+    g = torch.linspace(0.5, 1.5, 1024, device=cuda)
+    states = []
+    for captured in (True, False):
+        p = torch.zeros(1024, device=cuda, requires_grad=True)
+        p.grad = g.clone()
+        optimizer = trigrad_amd.AdamW([p], lr=0.0, state_bits=8, capturable=captured, seed=77)
+        optimizer.step()
+        if captured:
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph):
+                optimizer.step()
+        for _ in range(999):
+            graph.replay() if captured else optimizer.step()
+        torch.cuda.synchronize()
+        s = optimizer.state[p]
+        states.append((s["exp_avg"].float(), s["exp_avg_sq"].float(), s["scales"]))
+    assert all(torch.equal(a, b) for a, b in zip(*states))
+    root = states[0][1] * states[0][2][:, 1].repeat_interleave(256)
+    # 1 - 0.999^1000 = 0.632 of the square, 0.795 of its root.  A root that goes up by steps of at most an eighth of itself, each by chance, has a
+    # variance of at most its square / 16, and its square grows by half a step more: 0.05, beside 6 x 0.2 / 1024^(1/2) = 0.04
+    assert abs((root / g).mean().item() - 0.795) <= 0.09
+
+
+@pytest.mark.gpu
 def test_optimizer_is_torchs(cuda):
     """Ten steps beside torch.optim.AdamW, with groups of their own numbers and a parameter whose gradients begin late."""
     import trigrad_amd

@@ -83,7 +83,10 @@ def adamw_step(
         grad_scale : a tensor of one float32 (float64) that the gradients are multiplied with, as clipping and loss scaling leave one
         maximize : the gradients' opposite
         seed : an integer that is another one in every step, for averages in 8 bits: of its two neighbours in 8 bits a value becomes one by a random
-            number that is mixed of the seed and its place, the nearer one more often, so that small changes are not lost
+            number that is mixed of the seed and its place, the nearer one more often, so that small changes are not lost.  To the seed the number of
+            the step is added where step is a tensor, so that a captured step has other ones in every replay
+
+    A gradient that is not finite makes its element so, and an infinite one with averages in 8 bits its block, whose scale it is.
 
     A tensor that is written may not overlap any other.  The call can be captured into a graph, with step and lr as tensors.
     """
@@ -144,7 +147,7 @@ class AdamW(torch.optim.Optimizer):
         state_bits : 32, or 8: averages in 8 bits with two float32 for every 256 elements, 2.03 bytes a parameter instead of 8
         capturable : steps are counted on the device, so that a step can be captured into a graph (with lr as a tensor where it is to change);
             tensors that had their first gradient in the same step are counted as one
-        seed : of the random numbers that averages in 8 bits are rounded with (a captured step has the same ones in every replay)
+        seed : of the random numbers that averages in 8 bits are rounded with, together with a step's number
 
     Parameters in float16 or bfloat16 are rounded copies of ones in float32 that the state keeps ("master").
     """

@@ -50,9 +50,11 @@ template <class C, int Bits> struct AdamwLaunch {
 // What the step multiplies with.
 struct AdamwFactors {
     real keep, size_of_step, unbias, scale;
+    uint32_t noise;
 };
+constexpr uint32_t kNoiseOfSeed = 0x85EBCA6Bu;
 template <class L> __device__ __forceinline__ AdamwFactors factors_of(const L &a) {
-    AdamwFactors f = {a.keep, a.size_of_step, a.unbias, a.grad_scale ? a.grad_scale[0] : (real)1};
+    AdamwFactors f = {a.keep, a.size_of_step, a.unbias, a.grad_scale ? a.grad_scale[0] : (real)1, a.noise};
     if (a.step || a.rate_at) {  // in 64 bits, as the host has it
         const double rate = a.rate_at ? (double)a.rate_at[0] : a.rate;
         f.keep = (real)(1.0 - rate * a.decay);
@@ -60,6 +62,7 @@ template <class L> __device__ __forceinline__ AdamwFactors factors_of(const L &a
         const double left1 = a.step ? -expm1(t * a.left1) : a.left1, left2 = a.step ? -expm1(t * a.left2) : a.left2;
         f.size_of_step = (real)(rate / left1);
         f.unbias = (real)(1.0 / sqrt(left2));
+        f.noise += (uint32_t)(int64_t)t * kNoiseOfSeed;  // the step's number belongs to the seed, so that replays do not all round alike
     }
     if (a.maximize) f.scale = -f.scale;
     return f;
@@ -210,7 +213,7 @@ __device__ __forceinline__ void step_block(AdamwBlock<G, C, Bits> &b, const Adam
 #pragma unroll
         for (int j = 0; j < 4; j++) {
             const uint32_t place = a.place[n] * kBlock + at + (Wide ? 4 * lane + j : lane + 64 * j);
-            const uint32_t noise = mixed(place * 0x9E3779B1u + a.noise);
+            const uint32_t noise = mixed(place * 0x9E3779B1u + f.noise);
             b.m[j] = neighbour8<false>(b.m[j], unit_m, noise & 0xFFFFu);
             root[j] = neighbour8<true>(root[j], unit_r, noise >> 16);
         }
@@ -289,7 +292,7 @@ template <class G, class C, int Bits> static int launch(const tg_adamw &c, const
     a.b2 = (real)c.beta2;
     a.b2_rest = (real)(1.0 - c.beta2);
     a.eps = (real)c.eps;
-    a.noise = (uint32_t)c.seed * 0x85EBCA6Bu + 0xC2B2AE35u;
+    a.noise = (uint32_t)c.seed * kNoiseOfSeed + 0xC2B2AE35u;
     a.maximize = c.maximize != 0;
     constexpr int kMost = AdamwLaunch<C, Bits>::kMost;
     static_assert(sizeof(a) <= 4096 && kMost <= 128, "kernel arguments, and a bit of `wide` each");

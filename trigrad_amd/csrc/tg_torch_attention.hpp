@@ -5,6 +5,8 @@
 #pragma once
 #include "tg_torch_operators.hpp"
 
+#include <torch/csrc/utils/object_ptr.h>
+
 #include <algorithm>
 #include <vector>
 
@@ -259,15 +261,30 @@ PyObject *py_linear_attention_step(PyObject *, PyObject *const *args, Py_ssize_t
 
 // ---- AdamW -------------------------------------------------------------------------------
 
-// The tensors of a list or tuple, which holds them for the call, and null for None; false: not a case for this route.
-using Tensors = std::vector<const at::Tensor *>;
-bool take_tensors(PyObject *arg, size_t count, bool optional, Tensors &to) {
+// The tensors of a list or tuple, and null for None.  A list is copied to a tuple that holds them for the call: other threads may change it meanwhile.
+struct Tensors {
+    std::vector<const at::Tensor *> at;
+    THPObjectPtr held;
+
+    bool empty() const { return at.empty(); }
+    const at::Tensor *operator[](size_t i) const { return at[i]; }
+    auto begin() const { return at.begin(); }
+    auto end() const { return at.end(); }
+};
+// false: not a case for this route
+bool take_tensors(PyObject *arg, size_t count, bool optional, Tensors &tensors) {
     if (optional && arg == Py_None) return true;
     const bool list = PyList_CheckExact(arg);
     if ((!list && !PyTuple_CheckExact(arg)) || (size_t)Py_SIZE(arg) != count) return false;
+    if (list) {
+        tensors.held = THPObjectPtr(PyList_AsTuple(arg));
+        if (!tensors.held) throw python_error();
+        arg = tensors.held.get();
+    }
+    auto &to = tensors.at;
     to.resize(count);
     for (size_t i = 0; i < count; i++) {
-        PyObject *item = list ? PyList_GET_ITEM(arg, i) : PyTuple_GET_ITEM(arg, i);
+        PyObject *item = PyTuple_GET_ITEM(arg, i);
         if (optional && item == Py_None) continue;
         if (!THPVariable_CheckTypeExact(Py_TYPE(item))) return false;  // a tensor or a parameter
         to[i] = &THPVariable_Unpack(item);
