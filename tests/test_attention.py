@@ -234,6 +234,21 @@ def test_offsets_that_are_none(cuda):
 
 
 @pytest.mark.gpu
+def test_offsets_that_change_between_the_passes(cuda):
+    """What the forward call made of them no longer fits; nothing outside is read or written, and calls that follow are right."""
+    import trigrad_amd
+    parts, _ = make(cuda, 4, 200, 2, 1, 16, 16, F32)
+    for changed in ([200, 200, 200], [0, 0, 0], [0, 10, 5], [-7, 1 << 30, 3]):
+        leaves = [t.detach().requires_grad_() for t in parts]
+        offsets = torch.tensor([0, 90, 200], dtype=torch.int32, device=cuda)
+        o, f = trigrad_amd.linear_attention(*leaves, offsets=offsets)
+        offsets.data.copy_(torch.tensor(changed, dtype=torch.int32))
+        torch.autograd.grad(o.sum() + f.sum(), leaves)
+        torch.cuda.synchronize()
+    check(cuda, parts, None, [0, 90, 200], "log")
+
+
+@pytest.mark.gpu
 def test_elements_beyond_32_bits(cuda):
     """Rows whose places pass 2^31 elements: the last ones as from the state in front of them."""
     import trigrad_amd

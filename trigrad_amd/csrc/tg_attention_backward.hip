@@ -82,7 +82,7 @@ __global__ __launch_bounds__((kQueriesThreads<T, D>), (waves_of_simd(kQueriesThr
     state.template load<true>(role == 0 ? c.states + (u * c.m.heads + head) * state_size : nullptr, column, c.m.key_size, c.m.value_size);
     double before = 0.0;
     Four<T, D, kQueriesThreads<T, D>, Vector> next(c, unit, head);
-    next.load(c, 0, unit.count);
+    if (unit.count > 0) next.load(c, 0, unit.count);  // offsets may have changed since the units were made of them
     float gate = 0.0f;  // of the next chunk's row, in the first wave
     if (wave == 0) reach_of(c, reaches[0], gate_of_lane<T, R>(c, unit.first, unit.count, head), unit.count, before);
     if (Parts<T>::kScaled) {

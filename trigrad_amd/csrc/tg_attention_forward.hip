@@ -28,8 +28,10 @@ __global__ __launch_bounds__(kThreads<D>, waves_of_simd(kThreads<D>, kStatesLds<
     State<D, W> state = {};
     double before = 0.0;
     Incoming<T, R, D, kThreads<D>, Vector> next_k, next_v;
-    next_k.load(k, c.m.k.row, unit.count, c.m.key_size);
-    next_v.load(v, c.m.v.row, unit.count, c.m.value_size);
+    if (unit.count > 0) {
+        next_k.load(k, c.m.k.row, unit.count, c.m.key_size);
+        next_v.load(v, c.m.v.row, unit.count, c.m.value_size);
+    }
     float gate = 0.0f;  // of the next chunk's row, in the first wave
     if (wave == 0) reach_of(c, reaches[0], gate_of_lane<T, R>(c, unit.first, unit.count, head), unit.count, before);
     int turn = 0;
