@@ -217,7 +217,8 @@ __global__ __launch_bounds__(kScanThreads) void attention_scan_kernel(AttentionC
     if (to) store_pack<V>(to + (s * c.m.heads + head) * size + i, x.v);
 }
 
-// dlog a of a unit's rows: <S, D> in front of it, and what changes it from row to row.
+// dlog a of a unit's rows: <S, D> in front of it, and what changes it from row to row.  What is missing at the unit's end to <S, D> behind it, the sum of
+// roundings, goes to the rows in the share of their changes' squares: of a walk whose both ends are known a third of the variance is left.
 template <class S> __global__ __launch_bounds__(kScanThreads) void attention_gates_kernel(AttentionCall c, int64_t rows_of_chunk, const float *__restrict__ in_front) {
     __shared__ double waves[kScanThreads / kWave];
     const int64_t u = blockIdx.x / c.m.heads, size = (int64_t)c.m.key_size * c.m.value_size;
@@ -239,10 +240,9 @@ template <class S> __global__ __launch_bounds__(kScanThreads) void attention_gat
         }
         return before;
     };
-    double product = 0.0, all;
-    const float *gradient = unit.index > 0 ? c.grad_states + ((u - 1) * c.m.heads + head) * size : in_front ? in_front + (unit.sequence * c.m.heads + head) * size : nullptr;
-    if (gradient) {
-        const float *state = c.states + (u * c.m.heads + head) * size;
+    const auto product_of = [&](int64_t at, const float *gradient) {  // this thread's part of <S, D> in front of unit `at`
+        double product = 0.0;
+        const float *state = c.states + (at * c.m.heads + head) * size;
         // eight products are added in float32, all others in 64 bits
 #pragma unroll 2
         for (int64_t first = threadIdx.x; first < size; first += 8 * kScanThreads) {
@@ -257,26 +257,50 @@ template <class S> __global__ __launch_bounds__(kScanThreads) void attention_gat
             for (int j = 0; j < 8; j++) sum = first + j * kScanThreads < size ? fmaf(x[j], y[j], sum) : sum;
             product += (double)sum;
         }
-    }
+        return product;
+    };
+    const auto behind = [&](int64_t at) { return c.grad_states + (at * c.m.heads + head) * size; };
+    const bool last_unit = unit.base + unit.count >= rows_of(c.m, c.offsets, unit.sequence).count;
+    double product = 0.0, product_behind = 0.0, all, at_end;
+    if (unit.index > 0)
+        product = product_of(u, behind(u - 1));
+    else if (in_front)
+        product = product_of(u, in_front + (unit.sequence * c.m.heads + head) * size);
+    if (!last_unit && u + 1 < c.most_units) product_behind = product_of(u + 1, behind(u));
     over_waves(sum_lanes(product, kWave), all);
+    over_waves(sum_lanes(product_behind, kWave), at_end);
+    if (last_unit && c.grad_final) at_end = c.ends[unit.sequence * c.m.heads + head];
     double log_a = all;  // of the first row
     const int64_t each = (unit.count + kScanThreads - 1) / kScanThreads, first = min(unit.count, threadIdx.x * each), last = min(unit.count, first + each);
     const int64_t at = head * c.m.rows + unit.first;
-    double sum = 0.0;
-    for (int64_t t = first; t < last; t++) sum += (double)c.changes[1][at + t] - (double)c.changes[0][at + t];
-    double upto = sum;
+    double sum = 0.0, squares = 0.0, all_squares;
+    const auto change_at = [&](int64_t t, double &square) {
+        const double up = (double)c.changes[1][at + t], down = (double)c.changes[0][at + t];
+        square = up * up + down * down;
+        return up - down;
+    };
+    for (int64_t t = first; t < last; t++) {
+        double square;
+        sum += change_at(t, square);
+        squares += square;
+    }
+    double upto = sum, squares_upto = squares;
 #pragma unroll
     for (int step = 1; step < kWave; step *= 2) {
-        const double other = __shfl_up(upto, step);
-        if (lane >= step) upto += other;
+        const double other = __shfl_up(upto, step), other_squares = __shfl_up(squares_upto, step);
+        if (lane >= step) upto += other, squares_upto += other_squares;
     }
-    log_a += over_waves(upto, all) + upto - sum;
+    const double before = over_waves(upto, all) + upto - sum, squares_before = over_waves(squares_upto, all_squares) + squares_upto - squares;
+    const double share = all_squares > 0.0 ? (at_end - (log_a + all)) / all_squares : 0.0;  // of what is missing, for a square
+    log_a += before + share * squares_before;
     double total = 0.0;
     for (int64_t t = first; t < last; t++) {
         total += log_a;
         const int64_t to = (unit.first + t) * c.m.heads + head;
         if (!c.m.fixed) ((S *)c.grad_gates)[to] = (S)(float)(log_a * slope_of(c.m.gate_form, (double)(float)((const S *)c.gates)[to]));
-        log_a += (double)c.changes[1][at + t] - (double)c.changes[0][at + t];
+        double square;
+        const double change = change_at(t, square);
+        log_a += change + share * square;
     }
     if (c.m.fixed) {
         over_waves(sum_lanes(total, kWave), all);
@@ -519,7 +543,7 @@ static int split_of(const char *fn, const tg_attention &a, const Attention &m, S
 
 // Bytes from the beginning of what the forward call leaves, or of a workspace.
 struct Room {
-    int64_t states, decays, plan, grad_states, changes, sums, grad_initial, shared_queries, shared_keys, all;
+    int64_t states, decays, plan, grad_states, changes, sums, ends, grad_initial, shared_queries, shared_keys, all;
 };
 static Room room_of(const tg_attention &a, const Attention &m, const Split &s, bool states, bool backward) {
     Room r = {};
@@ -536,6 +560,7 @@ static Room room_of(const tg_attention &a, const Attention &m, const Split &s, b
     r.grad_states = take(backward, units * size);
     r.changes = take(backward, 2 * m.rows * m.heads * 4);
     r.sums = take(backward && m.fixed, units * 8);
+    r.ends = take(backward, m.sequences * m.heads * 8);
     r.grad_initial = take(backward && a.initial, m.sequences * m.heads * size);
     r.shared_queries = take(backward && m.shared > 1, m.rows * m.heads * m.key_size * 4);
     r.shared_keys = take(backward && m.shared > 1, m.rows * m.heads * m.key_size * 4);
@@ -653,6 +678,7 @@ template <class T, class S> static int backward(const tg_attention &a, const Att
     c.changes[0] = (float *)(w + room.changes);
     c.changes[1] = c.changes[0] + m.rows * m.heads;
     c.sums = (double *)(w + room.sums);
+    c.ends = (double *)(w + room.ends);
     c.grad_queries = m.shared > 1 && a.grad_queries ? w + room.shared_queries : a.grad_queries;
     c.grad_keys = m.shared > 1 && a.grad_keys ? w + room.shared_keys : a.grad_keys;
     float *in_front = a.initial && a.grad_gates ? (float *)(w + room.grad_initial) : nullptr;

@@ -321,6 +321,7 @@ struct AttentionCall {
     float *grad_states;     // of each unit and head: what the unit adds to the gradient in front of it, then the gradient behind it
     float *changes[2];      // of each head and row: what dlog a changes by
     double *sums;           // of each unit and head: dlog a of all rows
+    double *ends;           // of each sequence and head, where grad_final is there: <S, D> behind its last row
 };
 
 struct Unit {
