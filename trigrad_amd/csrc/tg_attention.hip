@@ -186,7 +186,7 @@ __global__ __launch_bounds__(kPlanThreads) void attention_plan_kernel(Attention 
 // neighbours of the state and reads eight units ahead.
 template <int V>
 __global__ __launch_bounds__(kScanThreads) void attention_scan_kernel(AttentionCall c, float *__restrict__ states, const float *__restrict__ from, float *__restrict__ to,
-                                                                      int64_t unit_rows, bool back) {
+                                                                      float *__restrict__ kept, int64_t unit_rows, bool back) {
     constexpr int kAhead = 8;
     const int64_t s = blockIdx.x / c.m.heads, size = (int64_t)c.m.key_size * c.m.value_size, i = ((int64_t)blockIdx.y * kScanThreads + threadIdx.x) * V;
     const int head = (int)(blockIdx.x % c.m.heads);
@@ -215,6 +215,7 @@ __global__ __launch_bounds__(kScanThreads) void attention_scan_kernel(AttentionC
         }
     }
     if (to) store_pack<V>(to + (s * c.m.heads + head) * size + i, x.v);
+    if (kept) store_pack<V>(kept + (s * c.m.heads + head) * size + i, x.v);
 }
 
 // dlog a of a unit's rows: <S, D> in front of it, and what changes it from row to row.  What is missing at the unit's end to <S, D> behind it, the sum of
@@ -240,9 +241,8 @@ template <class S> __global__ __launch_bounds__(kScanThreads) void attention_gat
         }
         return before;
     };
-    const auto product_of = [&](int64_t at, const float *gradient) {  // this thread's part of <S, D> in front of unit `at`
+    const auto product_of = [&](const float *state, const float *gradient) {  // this thread's part
         double product = 0.0;
-        const float *state = c.states + (at * c.m.heads + head) * size;
         // eight products are added in float32, all others in 64 bits
 #pragma unroll 2
         for (int64_t first = threadIdx.x; first < size; first += 8 * kScanThreads) {
@@ -259,23 +259,25 @@ template <class S> __global__ __launch_bounds__(kScanThreads) void attention_gat
         }
         return product;
     };
-    const auto behind = [&](int64_t at) { return c.grad_states + (at * c.m.heads + head) * size; };
+    const int64_t of_unit = (u * c.m.heads + head) * size, next = c.m.heads * size, of_sequence = (unit.sequence * c.m.heads + head) * size;
     const bool last_unit = unit.base + unit.count >= rows_of(c.m, c.offsets, unit.sequence).count;
     double product = 0.0, product_behind = 0.0, all, at_end;
     if (unit.index > 0)
-        product = product_of(u, behind(u - 1));
+        product = product_of(c.states + of_unit, c.grad_states + of_unit - next);
     else if (in_front)
-        product = product_of(u, in_front + (unit.sequence * c.m.heads + head) * size);
-    if (!last_unit && u + 1 < c.most_units) product_behind = product_of(u + 1, behind(u));
+        product = product_of(c.states + of_unit, in_front + of_sequence);
+    if (!last_unit && u + 1 < c.most_units)
+        product_behind = product_of(c.states + of_unit + next, c.grad_states + of_unit);
+    else if (last_unit && c.grad_final)
+        product_behind = product_of(c.finals + of_sequence, c.grad_final + of_sequence);
     over_waves(sum_lanes(product, kWave), all);
     over_waves(sum_lanes(product_behind, kWave), at_end);
-    if (last_unit && c.grad_final) at_end = c.ends[unit.sequence * c.m.heads + head];
     double log_a = all;  // of the first row
     const int64_t each = (unit.count + kScanThreads - 1) / kScanThreads, first = min(unit.count, threadIdx.x * each), last = min(unit.count, first + each);
     const int64_t at = head * c.m.rows + unit.first;
     double sum = 0.0, squares = 0.0, all_squares;
     const auto change_at = [&](int64_t t, double &square) {
-        const double up = (double)c.changes[1][at + t], down = (double)c.changes[0][at + t];
+        const double up = c.changes[1][at + t], down = c.changes[0][at + t];
         square = up * up + down * down;
         return up - down;
     };
@@ -543,7 +545,7 @@ static int split_of(const char *fn, const tg_attention &a, const Attention &m, S
 
 // Bytes from the beginning of what the forward call leaves, or of a workspace.
 struct Room {
-    int64_t states, decays, plan, grad_states, changes, sums, ends, grad_initial, shared_queries, shared_keys, all;
+    int64_t states, finals, decays, plan, grad_states, changes, sums, grad_initial, shared_queries, shared_keys, all;
 };
 static Room room_of(const tg_attention &a, const Attention &m, const Split &s, bool states, bool backward) {
     Room r = {};
@@ -555,12 +557,12 @@ static Room room_of(const tg_attention &a, const Attention &m, const Split &s, b
     };
     const int64_t size = (int64_t)m.key_size * m.value_size * 4, units = s.most_units * m.heads;
     r.states = take(states, units * size);
+    r.finals = take(states, m.sequences * m.heads * size);
     r.plan = take(states && m.packed, (s.most_units + m.sequences) * 4);
     r.decays = take(backward || !states, units * 4);
     r.grad_states = take(backward, units * size);
-    r.changes = take(backward, 2 * m.rows * m.heads * 4);
+    r.changes = take(backward, 2 * m.rows * m.heads * 8);
     r.sums = take(backward && m.fixed, units * 8);
-    r.ends = take(backward, m.sequences * m.heads * 8);
     r.grad_initial = take(backward && a.initial, m.sequences * m.heads * size);
     r.shared_queries = take(backward && m.shared > 1, m.rows * m.heads * m.key_size * 4);
     r.shared_keys = take(backward && m.shared > 1, m.rows * m.heads * m.key_size * 4);
@@ -620,14 +622,14 @@ static AttentionCall call_of(const tg_attention &a, const Attention &m, const Sp
     return c;
 }
 
-static void scan(const AttentionCall &c, const Split &s, float *states, const float *from, float *to, bool back, hipStream_t stream) {
+static void scan(const AttentionCall &c, const Split &s, float *states, const float *from, float *to, float *kept, bool back, hipStream_t stream) {
     const int64_t size = (int64_t)c.m.key_size * c.m.value_size;
     const auto launch = [&](auto vector) {
         constexpr int V = decltype(vector)::value;
         TG_LAUNCH_AS("attention_scan", (attention_scan_kernel<V>), dim3((unsigned)(c.m.sequences * c.m.heads), (unsigned)ceil_div64(size, kScanThreads * V)),
-                     dim3(kScanThreads), 0, stream, c, states, from, to, s.rows_of_chunk * s.chunks, back);
+                     dim3(kScanThreads), 0, stream, c, states, from, to, kept, s.rows_of_chunk * s.chunks, back);
     };
-    if (size % 4 == 0 && ((uintptr_t)states | (uintptr_t)from | (uintptr_t)to) % 16 == 0)
+    if (size % 4 == 0 && ((uintptr_t)states | (uintptr_t)from | (uintptr_t)to | (uintptr_t)kept) % 16 == 0)
         launch(std::integral_constant<int, 4>());
     else
         launch(std::integral_constant<int, 1>());
@@ -644,6 +646,7 @@ static int forward(const tg_attention &a, const Attention &m) {
         const Room room = room_of(a, m, s, true, false);
         char *p = (char *)(kept ? a.kept : a.workspace);
         c.states = (float *)(p + room.states);
+        c.finals = kept ? (float *)(p + room.finals) : nullptr;
         c.plan = (const int32_t *)(p + room.plan);
         c.decays = (float *)((char *)a.workspace + (kept ? 0 : room.all));
         if (m.packed)
@@ -654,7 +657,7 @@ static int forward(const tg_attention &a, const Attention &m) {
         c.through = true;
     } else {
         if ((code = launch_attention_forward(a.type, c, (int)s.size, true, stream))) return code;
-        scan(c, s, c.states, a.initial, a.final, false, stream);
+        scan(c, s, c.states, a.initial, a.final, c.finals, false, stream);
     }
     if ((code = launch_attention_forward(a.type, c, (int)s.size, false, stream))) return code;
     return by_types(a.type, a.gate_type, [&](auto t, auto) {
@@ -672,19 +675,19 @@ template <class T, class S> static int backward(const tg_attention &a, const Att
     const Room kept = room_of(a, m, s, true, false), room = room_of(a, m, s, false, true);
     char *w = (char *)a.workspace;
     c.states = (float *)((char *)a.kept + kept.states);
+    c.finals = (float *)((char *)a.kept + kept.finals);
     c.plan = (const int32_t *)((char *)a.kept + kept.plan);
     c.decays = (float *)(w + room.decays);
     c.grad_states = (float *)(w + room.grad_states);
-    c.changes[0] = (float *)(w + room.changes);
+    c.changes[0] = (double *)(w + room.changes);
     c.changes[1] = c.changes[0] + m.rows * m.heads;
     c.sums = (double *)(w + room.sums);
-    c.ends = (double *)(w + room.ends);
     c.grad_queries = m.shared > 1 && a.grad_queries ? w + room.shared_queries : a.grad_queries;
     c.grad_keys = m.shared > 1 && a.grad_keys ? w + room.shared_keys : a.grad_keys;
     float *in_front = a.initial && a.grad_gates ? (float *)(w + room.grad_initial) : nullptr;
     if (a.grad_initial) in_front = a.grad_initial;
     if (m.rows && (code = launch_attention_backward(a.type, c, (int)s.size, false, stream))) return code;
-    scan(c, s, c.grad_states, a.grad_final, in_front, true, stream);
+    scan(c, s, c.grad_states, a.grad_final, in_front, nullptr, true, stream);
     if (m.rows && (a.grad_keys || a.grad_values || a.grad_gates) && (code = launch_attention_backward(a.type, c, (int)s.size, true, stream))) return code;
     if (a.grad_gates) {
         if (m.rows)

@@ -175,31 +175,16 @@ __global__ __launch_bounds__((kQueriesThreads<T, D>), (waves_of_simd(kQueriesThr
         if (wave == 0 && at + R < unit.count) reach_of(c, reaches[turn ^ 1], gate, unit.count - at - R, before);
         __syncthreads();
         if (threadIdx.x < R && at + threadIdx.x < unit.count) {
-            float x = 0.0f;
+            double x = 0.0;
 #pragma unroll
-            for (int n = 0; n < kTiles; n++) x += by_later[n][threadIdx.x] - by_earlier[n][threadIdx.x];
+            for (int n = 0; n < kTiles; n++) x += (double)by_later[n][threadIdx.x] - (double)by_earlier[n][threadIdx.x];
 #pragma unroll
-            for (int n = 0; n < kWaves; n++) x += by_wave[n][threadIdx.x];
+            for (int n = 0; n < kWaves; n++) x += (double)by_wave[n][threadIdx.x];
             c.changes[0][head * c.m.rows + unit.first + at + threadIdx.x] = x;
         }
     }
     if (role == 1) state.template store<true>(c.grad_states + (u * c.m.heads + head) * state_size, column, c.m.key_size, c.m.value_size);
     if (threadIdx.x == 0) c.decays[u * c.m.heads + head] = power_of_two((float)before);
-    if (!c.grad_final || !c.grad_gates || unit.base + unit.count < rows_of(c.m, c.offsets, unit.sequence).count) return;
-    // <S, D> behind the sequence's last row
-    double *ends = (double *)lds;
-    if (role == 0) {
-        const float *behind = c.grad_final + (unit.sequence * c.m.heads + head) * state_size;
-        float sum = 0.0f;
-        state.template each<true>(column, c.m.key_size, c.m.value_size, [&](int w, int n, int j, int at) { sum = fmaf(state.x[w][n][j], behind[at], sum); });
-        const double all = sum_lanes((double)sum, kWave);
-        if (threadIdx.x % kWave == 0) ends[wave] = all;
-    }
-    __syncthreads();
-    if (threadIdx.x > 0) return;
-    double all = 0.0;
-    for (int n = 0; n < kWaves; n++) all += ends[n];
-    c.ends[unit.sequence * c.m.heads + head] = all;
 }
 
 template <class T, int D, bool Vector>
@@ -321,9 +306,9 @@ __global__ __launch_bounds__(kKeysThreads<D>, (waves_of_simd(kKeysThreads<D>, kK
         if (wave == 0 && at > 0) reach_of(c, reaches[turn ^ 1], gate, R, before);
         __syncthreads();
         if (threadIdx.x < R && at + threadIdx.x < unit.count) {
-            float x = 0.0f;
+            double x = 0.0;
 #pragma unroll
-            for (int n = 0; n < kWaves; n++) x += by_wave[n][threadIdx.x];
+            for (int n = 0; n < kWaves; n++) x += (double)by_wave[n][threadIdx.x];
             c.changes[1][head * c.m.rows + unit.first + at + threadIdx.x] = x;
         }
     }

@@ -305,6 +305,7 @@ struct AttentionCall {
     void *outputs;
     float *final;
     float *states;          // of each unit and head, in front of it
+    float *finals;          // of each sequence and head, the state behind it, kept for the backward pass; or null
     float *decays;          // of each unit and head
     int64_t most_units;     // units there may be
     int64_t units;          // of a sequence, where all are alike
@@ -319,9 +320,8 @@ struct AttentionCall {
     void *grad_queries, *grad_keys, *grad_values, *grad_gates;
     float *grad_initial;
     float *grad_states;     // of each unit and head: what the unit adds to the gradient in front of it, then the gradient behind it
-    float *changes[2];      // of each head and row: what dlog a changes by
+    double *changes[2];     // of each head and row: what dlog a changes by
     double *sums;           // of each unit and head: dlog a of all rows
-    double *ends;           // of each sequence and head, where grad_final is there: <S, D> behind its last row
 };
 
 struct Unit {

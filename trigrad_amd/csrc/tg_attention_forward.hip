@@ -160,7 +160,9 @@ __global__ __launch_bounds__(kThreads<D>, waves_of_simd(kThreads<D>, kOutputsLds
         if (wave == 0 && at + R < unit.count) reach_of(c, reaches[turn ^ 1], gate, unit.count - at - R, before);
         __syncthreads();
     }
-    if (c.through) state.template store<false>(c.final + (unit.sequence * c.m.heads + head) * state_size, column, c.m.key_size, c.m.value_size);
+#pragma unroll 1
+    for (float *to = c.through ? c.final : nullptr; to; to = to == c.final ? c.finals : nullptr)
+        state.template store<false>(to + (unit.sequence * c.m.heads + head) * state_size, column, c.m.key_size, c.m.value_size);
 }
 
 int launch_attention_forward(int64_t type, const AttentionCall &c, int size, bool states_only, hipStream_t stream) {
