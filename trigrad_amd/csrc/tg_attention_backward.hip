@@ -167,10 +167,10 @@ __global__ __launch_bounds__((kQueriesThreads<T, D>), (waves_of_simd(kQueriesThr
                     }
                 }
             });
-            state.template fold<T>(reach.whole, values, mine, reach.column);
+            state.template fold<T, kFoldApart<T, D, W, false>>(reach.whole, values, mine, reach.column);
         } else {
             columns_of(queries, column, mine);
-            state.template fold<T>(1.0f, grads, mine, reach.start);
+            state.template fold<T, kFoldApart<T, D, W, false>>(1.0f, grads, mine, reach.start);
         }
         if (wave == 0 && at + R < unit.count) reach_of(c, reaches[turn ^ 1], gate, unit.count - at - R, before);
         __syncthreads();
@@ -302,7 +302,7 @@ __global__ __launch_bounds__(kKeysThreads<D>, (waves_of_simd(kKeysThreads<D>, kK
                 }
             }
         });
-        state.template fold<T>(reach.whole, adding, mine, reach.row);
+        state.template fold<T, kFoldApart<T, D, W, false>>(reach.whole, adding, mine, reach.row);
         if (wave == 0 && at > 0) reach_of(c, reaches[turn ^ 1], gate, R, before);
         __syncthreads();
         if (threadIdx.x < R && at + threadIdx.x < unit.count) {

@@ -432,6 +432,11 @@ __device__ __forceinline__ int lane_of_turn() {
 // Keeps the compiler from reading ahead over this point: operands of a whole chunk, read at its beginning, would not fit the registers.
 __device__ __forceinline__ void in_order() { __builtin_amdgcn_sched_barrier(0); }
 
+// Whether State::fold adds up apart, where the registers are enough: 8 x 2048 rows of 32 heads of 64 with fixed decays near 1, states off by 1.1e-7 in
+// place of 2.7e-7 and the decays' gradients by 5e-7 in place of 9e-7, in the same time; but 4 x 4096 rows of 16 heads of 128 the outputs' kernel 160 us
+// in place of 101, and, with two times sixteen columns a wave, the keys' 252 in place of 184.
+template <class T, int D, int W, bool Forward> constexpr bool kFoldApart = Forward ? D <= 64 || Parts<T>::kRows == 32 : W == 1;
+
 // The state in accumulators: rows of keys and columns of values (Turned: the other way round), of a wave the 16 W columns from `column` on.  With W = 2 an
 // operand from LDS goes into twice as many products, with W = 1 twice as many waves hide each other's latencies.
 template <int D, int W> struct State {
@@ -497,8 +502,9 @@ template <int D, int W> struct State {
         }
         return scaling.down;
     }
-    // decay times itself, plus the tile, transposed, times this wave's columns `mine` of another with a weight for each row
-    template <class T, class E, int N, int Rows>
+    // decay times itself, plus the tile, transposed, times this wave's columns `mine` of another with a weight for each row.  Apart: 32 rows are added
+    // up apart, so that a long state is rounded twice a chunk and not by each of six products.
+    template <class T, bool Apart, class E, int N, int Rows>
     __device__ __forceinline__ void fold(float decay, const Tile<E, N, Rows, D> &tile, const Operand<E, N> (&mine)[Rows / 32][W], const float *weights) {
         constexpr int M = Parts<T>::kWhole, K = Rows / 32;
         if constexpr (Parts<T>::kScaled) {
@@ -537,10 +543,12 @@ template <int D, int W> struct State {
                 if (n % 4 == 3) in_order();
             }
         } else {
+            if (!Apart) {
 #pragma unroll
-            for (int w = 0; w < W; w++)
+                for (int w = 0; w < W; w++)
 #pragma unroll
-                for (int n = 0; n < D / 16; n++) x[w][n] *= decay;
+                    for (int n = 0; n < D / 16; n++) x[w][n] *= decay;
+            }
 #pragma unroll
             for (int k = 0; k < K; k++) {
                 Operand<E, M> late[W];
@@ -554,7 +562,11 @@ template <int D, int W> struct State {
                 for (int n = 0; n < D / 16; n++) {
                     const Operand<E, N> theirs = tile.transposed(32 * k, 16 * n);
 #pragma unroll
-                    for (int w = 0; w < W; w++) x[w][n] = product(theirs, late[w], x[w][n]);
+                    for (int w = 0; w < W; w++) {
+                        const floatx4 sum = product(theirs, late[w], Apart ? floatx4{0.0f, 0.0f, 0.0f, 0.0f} : x[w][n]);
+#pragma unroll
+                        for (int j = 0; j < 4; j++) x[w][n][j] = !Apart ? sum[j] : k == 0 ? fmaf(x[w][n][j], decay, sum[j]) : x[w][n][j] + sum[j];
+                    }
                     if (n % 4 == 3) in_order();
                 }
             }

@@ -48,7 +48,7 @@ __global__ __launch_bounds__(kThreads<D>, waves_of_simd(kThreads<D>, kStatesLds<
         }
         Operand<E, N> mine[R / 32][W];
         columns_of(values, column, mine);
-        state.template fold<T>(reaches[turn].whole, keys, mine, reaches[turn].column);
+        state.template fold<T, kFoldApart<T, D, W, true>>(reaches[turn].whole, keys, mine, reaches[turn].column);
         if (wave == 0 && at + R < unit.count) reach_of(c, reaches[turn ^ 1], gate, unit.count - at - R, before);
         __syncthreads();
     }
@@ -156,7 +156,7 @@ __global__ __launch_bounds__(kThreads<D>, waves_of_simd(kThreads<D>, kOutputsLds
                     put_row(out + (at + 16 * s) * out_row + 16 * w, (uint32_t)(lane % 16 * (int)out_row + to), to + 16 * w, c.m.value_size, Vector, read[s][w]);
             }
         });
-        state.template fold<T>(reach.whole, keys, mine, reach.column);
+        state.template fold<T, kFoldApart<T, D, W, true>>(reach.whole, keys, mine, reach.column);
         if (wave == 0 && at + R < unit.count) reach_of(c, reaches[turn ^ 1], gate, unit.count - at - R, before);
         __syncthreads();
     }
