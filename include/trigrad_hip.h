@@ -606,7 +606,7 @@ int tg_group_norm_backward(const tg_norm *n);
  * initial, final and their gradients are (sequences, heads, key_size, value_size) tg_real; initial, grad_final and every
  * gradient but grad_outputs may be null (grad_outputs too, then it is zeros).
  * tg_linear_attention_sizes writes the bytes of `kept` (what the forward call leaves for the backward call; null where none
- * follows) and of the workspaces of a forward call that is not followed by a backward call, of one that is, and of the backward call. */
+ * follows) and of the workspaces of a forward call that is not followed by a backward call, of one that is, and of the backward call; all aligned to 16 bytes. */
 #define TG_ATTENTION_SIZE 128
 
 typedef struct tg_attention {

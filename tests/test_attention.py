@@ -544,6 +544,8 @@ def test_library_refuses_on_the_host():
     assert lib.tg_linear_attention_forward(C.byref(_lib.Attention(**good, **some, kept=16, kept_bytes=sizes[0] - 1))) == -2
     assert lib.tg_linear_attention_backward(C.byref(_lib.Attention(**good, **some, kept=16, kept_bytes=sizes[0], workspace=16, workspace_bytes=sizes[3] - 1))) == -2
     assert lib.tg_linear_attention_backward(C.byref(_lib.Attention(**good, **some, workspace=16, workspace_bytes=sizes[3]))) == -1  # nothing kept
+    assert lib.tg_linear_attention_forward(C.byref(_lib.Attention(**good, **some, kept=24, kept_bytes=sizes[0], workspace=16, workspace_bytes=sizes[2]))) == -2
+    assert lib.tg_linear_attention_backward(C.byref(_lib.Attention(**good, **some, kept=16, kept_bytes=sizes[0], workspace=24, workspace_bytes=sizes[3]))) == -2
 
 
 @pytest.mark.gpu

