@@ -271,7 +271,8 @@ struct Tensors {
     auto begin() const { return at.begin(); }
     auto end() const { return at.end(); }
 };
-// false: not a case for this route
+// false: not a case for this route, as are tensors that are views with a negation still to be done, of another kind than torch's own, or on another
+// device than a GPU.  That is all in a tensor's keys, which are those of the tensor before it as a rule.
 bool take_tensors(PyObject *arg, size_t count, bool optional, Tensors &tensors) {
     if (optional && arg == Py_None) return true;
     const bool list = PyList_CheckExact(arg);
@@ -283,12 +284,16 @@ bool take_tensors(PyObject *arg, size_t count, bool optional, Tensors &tensors) 
     }
     auto &to = tensors.at;
     to.resize(count);
+    c10::DispatchKeySet known;
     for (size_t i = 0; i < count; i++) {
         PyObject *item = PyTuple_GET_ITEM(arg, i);
         if (optional && item == Py_None) continue;
         if (!THPVariable_CheckTypeExact(Py_TYPE(item))) return false;  // a tensor or a parameter
         to[i] = &THPVariable_Unpack(item);
-        if (!to[i]->is_cuda() || at::isTensorSubclassLike(*to[i])) return false;
+        const c10::DispatchKeySet keys = to[i]->key_set();
+        if (keys == known) continue;
+        if (!to[i]->is_cuda() || at::isTensorSubclassLike(*to[i]) || to[i]->is_neg()) return false;
+        known = keys;
     }
     return true;
 }
@@ -359,7 +364,7 @@ PyObject *py_adamw_step(PyObject *, PyObject *const *args, Py_ssize_t n) {
     if (grad_scale.defined() && !single(grad_scale)) Py_RETURN_NONE;
     const at::ScalarType state = scales.empty() ? at::kFloat : at::kFloat8_e4m3fn;
     const auto written = [&](const at::Tensor &t, at::ScalarType type) {
-        return t.scalar_type() == type && t.device() == device && t.is_contiguous() && !t.is_neg();
+        return t.scalar_type() == type && t.device() == device && t.is_contiguous();
     };
     std::vector<std::vector<Extent>> extents(6);
     for (auto &e : extents) e.reserve(count);
@@ -372,7 +377,7 @@ PyObject *py_adamw_step(PyObject *, PyObject *const *args, Py_ssize_t n) {
     const bool recording = at::GradMode::is_enabled();
     for (size_t i = 0; i < count; i++) {
         const at::Tensor &p = *params[i], &g = *grads[i], &average = *averages[i], &square = *squares[i];
-        if (!written(p, at::kFloat) || type_code(g.scalar_type()) < 0 || g.device() != device || g.sizes() != p.sizes() || g.is_neg() ||
+        if (!written(p, at::kFloat) || type_code(g.scalar_type()) < 0 || g.device() != device || g.sizes() != p.sizes() ||
             !g.is_contiguous() || !written(average, state) || !written(square, state) || average.sizes() != p.sizes() || square.sizes() != p.sizes() || (recording && p.requires_grad() && !p.is_leaf()))
             Py_RETURN_NONE;
         param_at[i] = target(p);
