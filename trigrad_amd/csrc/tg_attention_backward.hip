@@ -18,8 +18,10 @@ __device__ __forceinline__ float sum_groups(float v) {
 // The two kernels have twice the waves of a state: the first half (`role` 0) has one state, the second half the other.  LDS, and waves of a SIMD that
 // they are compiled for: two, with 256 registers, where LDS has room for one workgroup.
 //
-// W of State, 4 x 4096 rows of 16 heads of 128 in bfloat16, and 2 x 3000 of 8 in float32: the queries' kernel 178 and 84 us with one, 185 and 64 with
-// two; the keys' 245 and 139 with one, 185 and 76 with two.  8 x 2048 rows of 32 heads of 64: 128 and 134 with one, 180 and 150 with two.
+// W of State, 4 x 4096 rows of 16 heads of 128 in bfloat16, and 2 x 3000 of 8 in float32: the queries' kernel 180 and 81 us with one, 192 and 63 with
+// two; the keys' 335 and 93 with one, 189 and 65 with two.  8 x 2048 rows of 32 heads of 64: 129 and 127 with one, 161 and 141 with two.
+// Instructions bound both: making parts, matrix instructions and readings of LDS take a third to a half of the time each and hardly overlap, as all
+// waves of a workgroup are in the same phase (1.9 TB/s of memory for heads of 128, 2.6 for those of 64).
 template <class T, int D> constexpr int kQueriesColumns = D > 64 && sizeof(T) == 4 ? 2 : 1;
 template <int D> constexpr int kKeysColumns = D > 64 ? 2 : 1;
 template <class T, int D> constexpr int kQueriesThreads = 2 * State<D, kQueriesColumns<T, D>>::kWaves * kWave;
@@ -60,6 +62,7 @@ template <class T, int D, int Threads, bool Vector> struct Four {
     }
 };
 
+// dq, what changes dlog a from q.dq and the pairs, and what the unit adds to D.
 template <class T, int D, bool Vector>
 __global__ __launch_bounds__((kQueriesThreads<T, D>), (waves_of_simd(kQueriesThreads<T, D>, kQueriesLds<T, D>, kQueriesColumns<T, D> * D / 4))) void attention_grad_queries_kernel(AttentionCall c) {
     constexpr int R = Parts<T>::kRows, N = Parts<T>::kInput, kTiles = R / 16, W = kQueriesColumns<T, D>, kWaves = State<D, W>::kWaves;
@@ -187,6 +190,7 @@ __global__ __launch_bounds__((kQueriesThreads<T, D>), (waves_of_simd(kQueriesThr
     if (threadIdx.x == 0) c.decays[u * c.m.heads + head] = power_of_two((float)before);
 }
 
+// dk, dv, and what changes dlog a from k.dk.
 template <class T, int D, bool Vector>
 __global__ __launch_bounds__(kKeysThreads<D>, (waves_of_simd(kKeysThreads<D>, kKeysLds<T, D>, kKeysColumns<D> * D / 4))) void attention_grad_keys_kernel(AttentionCall c) {
     constexpr int R = Parts<T>::kRows, N = Parts<T>::kInput, kTiles = R / 16, W = kKeysColumns<D>, kWaves = State<D, W>::kWaves;

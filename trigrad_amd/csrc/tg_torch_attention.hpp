@@ -1,5 +1,5 @@
 // tg_torch_attention.hpp -- linear attention, its single step and the AdamW step for torch, without the interpreter between a call's steps: a step
-// over 320 small tensors was 1.7 ms of Python around 10 us of a kernel.
+// over 320 small tensors was 1.7 ms of Python around 27 us of kernels, and is 42 us here.
 //
 // What is not the ordinary case is left to the Python functions by returning None: they have the checks and the error texts.
 #pragma once
