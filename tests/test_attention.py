@@ -465,6 +465,37 @@ def test_captured_forward_and_backward(cuda):
 
 
 @pytest.mark.gpu
+def test_two_captured_graphs_at_once(cuda):
+    """Their replays overlap on two streams; each has workspaces of its own."""
+    import trigrad_amd
+    calls, streams, graphs, results = [], [torch.cuda.Stream() for _ in range(2)], [], []
+    for seed, (batch, length) in enumerate(((1, 3000), (3, 1500))):
+        parts, initial = make(cuda, 40 + seed, batch * length, 2, 2, 40, 72, BF16, sequences=batch)
+        leaves = [t.view(batch, length, *t.shape[1:]).detach().requires_grad_() for t in parts] + [initial.requires_grad_()]
+        g = torch.Generator().manual_seed(seed)
+        calls.append((leaves, [torch.randn(batch, length, 4, 72, generator=g).to(cuda, BF16), torch.randn(batch, 4, 40, 72, generator=g).to(cuda)]))
+
+    def run(leaves, grads):
+        out = trigrad_amd.linear_attention(*leaves)
+        return [*(t.detach() for t in out), *torch.autograd.grad(out, leaves, grads)]
+    for call, stream in zip(calls, streams):
+        with torch.cuda.stream(stream):
+            run(*call)
+        torch.cuda.synchronize()
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1], stream=stream):
+            results.append(run(*call))
+    wanted = [run(*call) for call in calls]
+    for _ in range(5):
+        for graph, stream in zip(graphs, streams):
+            with torch.cuda.stream(stream):
+                graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for got, want in zip(results, wanted) for a, b in zip(got, want))
+        torch.randn(1000, device=cuda).sum().item()
+
+
+@pytest.mark.gpu
 def test_capture_beside_an_eager_graph_is_refused(cuda):
     import trigrad_amd
     parts, _ = make(cuda, 9, 100, 1, 1, 16, 16, F32)
