@@ -28,9 +28,8 @@ template <class T, int D> constexpr int kQueriesThreads = 2 * State<D, kQueriesC
 template <int D> constexpr int kKeysThreads = 2 * State<D, kKeysColumns<D>>::kWaves * kWave;
 template <class T, int D> constexpr int kBackwardLds = 4 * Tile<typename Parts<T>::Element, Parts<T>::kInput, Parts<T>::kRows, D>::kBytes + 2 * (int)sizeof(Reach<Parts<T>::kRows>) +
                                                        D / 16 * Parts<T>::kRows * 4;
-template <class T> constexpr int kPairsLds = Tile<typename Parts<T>::Element, Parts<T>::kInput, Parts<T>::kRows, Parts<T>::kRows, false>::kBytes;
-template <class T, int D> constexpr int kQueriesLds = kBackwardLds<T, D> + kPairsLds<T> + 2 * Parts<T>::kRows / 16 * Parts<T>::kRows * 4;
-template <class T, int D> constexpr int kKeysLds = kBackwardLds<T, D> + 2 * kPairsLds<T>;
+template <class T, int D> constexpr int kQueriesLds = kBackwardLds<T, D> + PairsOf<T>::kBytes + 2 * Parts<T>::kRows / 16 * Parts<T>::kRows * 4;
+template <class T, int D> constexpr int kKeysLds = kBackwardLds<T, D> + 2 * PairsOf<T>::kBytes;
 
 // The chunks of a unit's tensors on their way to LDS.
 template <class T, int D, int Threads, bool Vector> struct Four {
@@ -68,7 +67,7 @@ __global__ __launch_bounds__((kQueriesThreads<T, D>), (waves_of_simd(kQueriesThr
     constexpr int R = Parts<T>::kRows, N = Parts<T>::kInput, kTiles = R / 16, W = kQueriesColumns<T, D>, kWaves = State<D, W>::kWaves;
     using E = typename Parts<T>::Element;
     using In = Tile<E, N, R, D>;
-    using Pairs = Tile<E, N, R, R, false>;
+    using Pairs = PairsOf<T>;
     extern __shared__ __attribute__((aligned(16))) char lds[];
     Reach<R> *reaches = (Reach<R> *)(lds + 4 * In::kBytes + Pairs::kBytes);
     float(*by_wave)[R] = (float(*)[R])(reaches + 2);  // q.dq without the chunk's own pairs, of each wave's columns
@@ -196,7 +195,7 @@ __global__ __launch_bounds__(kKeysThreads<D>, (waves_of_simd(kKeysThreads<D>, kK
     constexpr int R = Parts<T>::kRows, N = Parts<T>::kInput, kTiles = R / 16, W = kKeysColumns<D>, kWaves = State<D, W>::kWaves;
     using E = typename Parts<T>::Element;
     using In = Tile<E, N, R, D>;
-    using Pairs = Tile<E, N, R, R, false>;
+    using Pairs = PairsOf<T>;
     extern __shared__ __attribute__((aligned(16))) char lds[];
     Reach<R> *reaches = (Reach<R> *)(lds + 4 * In::kBytes + 2 * Pairs::kBytes);
     float(*by_wave)[R] = (float(*)[R])(reaches + 2);  // k.dk without the chunk's own pairs, of each wave's columns

@@ -11,8 +11,9 @@
 // Numbers.  Products are of numbers in 16 bits and summed in float32.  What is not one is a sum of "parts", each the rounded rest of those before.
 // In bfloat16, whose range is float32's, inputs in float32 are three parts, exactly; so are states, and inputs that carry a decay, wherever what they
 // go into is float32 in the end (states, their gradients, gates' gradients: two parts leave an error of 2e-6, three one of 1e-8, below that of the
-// sums).  States that go into an output of 16 bits have two parts, and the matrix of pairs inside a chunk is rounded as the inputs are, once.  Inputs in
-// float16 stay as they are, and what meets them is two parts in float16 (an error of 2^-23): states and weighted inputs by a power of two that brings
+// sums).  What goes into an output of 16 bits has two parts, states as well as the matrix of pairs inside a chunk: 2^-16 of a term, where the output's own
+// rounding is 2^-8 (pairs in one part left outputs off by 2.3e-3 of their norm in place of 1.7e-3).  Inputs in
+// float16 stay as they are, and what meets them is two parts in float16 (an error of 2^-22): states and weighted inputs by a power of two that brings
 // the largest of a wave's numbers near 2^15, pairs by one that brings the largest they could be there.
 #pragma once
 #include "tg_attention.hpp"
@@ -25,8 +26,8 @@ typedef short short4_t __attribute__((ext_vector_type(4)));
 typedef float floatx4 __attribute__((ext_vector_type(4)));
 typedef uint32_t uint32x4 __attribute__((ext_vector_type(4)));
 
-// Parts of an input, of a state that goes into an output of its type and of one that goes into float32, their type, and rows of a chunk: as many as
-// leave room in LDS for the parts.
+// Parts of an input, of a state or a pair that goes into an output of its type and of what goes into float32, their type, and rows of a chunk: as many
+// as leave room in LDS for the parts.
 template <class T> struct Parts;
 template <> struct Parts<bf16_t> {
     using Element = __bf16;
@@ -212,6 +213,9 @@ template <class E, int N> __device__ __forceinline__ void weighted(const Operand
         x[j] *= j < 4 ? a[j] : b[j - 4];
     }
 }
+
+// The matrix of pairs inside a chunk.
+template <class T> using PairsOf = Tile<typename Parts<T>::Element, Parts<T>::kState, Parts<T>::kRows, Parts<T>::kRows, false>;
 
 // ---- reading a chunk ----------------------------------------------------------------------
 
@@ -593,11 +597,11 @@ __device__ __forceinline__ void columns_of(const Tile<E, N, Rows, D> &tile, int 
 
 // += this wave's columns times sixteen rows of pairs from `row` on, those of the columns from First on to before Last.
 template <class T, int First, int Last, class E, int N, int Rows, int W>
-__device__ __forceinline__ void add_pairs(const Tile<E, N, Rows, Rows, false> &pairs, int row, const Operand<E, N> (&mine)[Rows / 32][W], float down, floatx4 (&sums)[W]) {
+__device__ __forceinline__ void add_pairs(const Tile<E, Parts<T>::kState, Rows, Rows, false> &pairs, int row, const Operand<E, N> (&mine)[Rows / 32][W], float down, floatx4 (&sums)[W]) {
     floatx4 inside[W] = {};
 #pragma unroll
     for (int k = First; k < Last; k++) {
-        const Operand<E, N> p = pairs.chained(row, 32 * k);
+        const Operand<E, Parts<T>::kState> p = pairs.chained(row, 32 * k);
 #pragma unroll
         for (int w = 0; w < W; w++)
             if (Parts<T>::kScaled)

@@ -6,7 +6,7 @@ namespace tg {
 
 template <class T, int D> constexpr int kStatesLds = 2 * Tile<typename Parts<T>::Element, Parts<T>::kInput, Parts<T>::kRows, D>::kBytes + 2 * (int)sizeof(Reach<Parts<T>::kRows>);
 template <class T, int D> constexpr int kOutputsLds = 3 * Tile<typename Parts<T>::Element, Parts<T>::kInput, Parts<T>::kRows, D>::kBytes +
-                                                      Tile<typename Parts<T>::Element, Parts<T>::kInput, Parts<T>::kRows, Parts<T>::kRows, false>::kBytes + 2 * (int)sizeof(Reach<Parts<T>::kRows>);
+                                                      PairsOf<T>::kBytes + 2 * (int)sizeof(Reach<Parts<T>::kRows>);
 constexpr int W = 1;  // see State
 template <int D> constexpr int kThreads = State<D, W>::kWaves * kWave;
 
@@ -65,7 +65,7 @@ __global__ __launch_bounds__(kThreads<D>, waves_of_simd(kThreads<D>, kOutputsLds
     constexpr bool kScaled = Parts<T>::kScaled;
     using E = typename Parts<T>::Element;
     using In = Tile<E, N, R, D>;
-    using Pairs = Tile<E, N, R, R, false>;
+    using Pairs = PairsOf<T>;
     extern __shared__ __attribute__((aligned(16))) char lds[];
     Reach<R> *reaches = (Reach<R> *)(lds + 3 * In::kBytes + Pairs::kBytes);
     const int64_t which = blockIdx.x / c.m.heads;  // a unit, or a sequence
