@@ -51,13 +51,12 @@ template <class T, int D, int Threads, bool Vector> struct Four {
         next_g.load(g + at * c.m.g.row, c.m.g.row, left, c.m.value_size);
     }
     template <class Tile> __device__ __forceinline__ void store(const AttentionCall &c, const Tile &queries, const Tile &keys, const Tile &values, const Tile &grads,
-                                                                int64_t left, Reach<R> &reach) const {
+                                                                int64_t left) const {
         using E = typename Parts<T>::Element;
-        constexpr bool kScaled = Parts<T>::kScaled;
-        next_q.template store<E, N, kScaled>(queries, left, c.m.key_size, &reach.largest[0]);
-        next_k.template store<E, N, kScaled>(keys, left, c.m.key_size, &reach.largest[1]);
-        next_v.template store<E, N, kScaled>(values, left, c.m.value_size, &reach.largest[2]);
-        next_g.template store<E, N, kScaled>(grads, c.grad_outputs_there ? left : 0, c.m.value_size, &reach.largest[3]);
+        next_q.template store<E, N>(queries, left, c.m.key_size);
+        next_k.template store<E, N>(keys, left, c.m.key_size);
+        next_v.template store<E, N>(values, left, c.m.value_size);
+        next_g.template store<E, N>(grads, c.grad_outputs_there ? left : 0, c.m.value_size);
     }
 };
 
@@ -87,19 +86,14 @@ __global__ __launch_bounds__((kQueriesThreads<T, D>), (waves_of_simd(kQueriesThr
     if (unit.count > 0) next.load(c, 0, unit.count);  // offsets may have changed since the units were made of them
     float gate = 0.0f;  // of the next chunk's row, in the first wave
     if (wave == 0) reach_of(c, reaches[0], gate_of_lane<T, R>(c, unit.first, unit.count, head), unit.count, before);
-    if (Parts<T>::kScaled) {
-        if (threadIdx.x < 4) reaches[0].largest[threadIdx.x] = 0;
-        __syncthreads();
-    }
     int turn = 0;
     for (int64_t at = 0; at < unit.count; at += R, turn ^= 1) {
         const int lane = lane_of_turn();
         const In queries{(E *)lds, lane}, keys{(E *)(lds + In::kBytes), lane}, values{(E *)(lds + 2 * In::kBytes), lane},
             grads{(E *)(lds + 3 * In::kBytes), lane};
         const Pairs pairs{(E *)(lds + 4 * In::kBytes), lane};
-        next.store(c, queries, keys, values, grads, unit.count - at, reaches[turn]);
+        next.store(c, queries, keys, values, grads, unit.count - at);
         __syncthreads();
-        if (Parts<T>::kScaled && threadIdx.x < 4) reaches[turn ^ 1].largest[threadIdx.x] = 0;
         if (at + R < unit.count) {
             next.load(c, at + R, unit.count - at - R);
             if (wave == 0) gate = gate_of_lane<T, R>(c, unit.first + at + R, unit.count - at - R, head);
@@ -110,30 +104,39 @@ __global__ __launch_bounds__((kQueriesThreads<T, D>), (waves_of_simd(kQueriesThr
         floatx4 read[kTiles][W] = {};
         float down = 1.0f;
         if (kApart && role == 0) down = state.template read_by<T, Parts<T>::kWhole>(grads, read);
-        const Scaling scaling = scaling_of_pairs<T>(reach, 2, 3, c.m.value_size, c.m.scale);
+        constexpr int kStep = kApart ? kWaves : 2 * kWaves;
+        const int all_tiles = tiles_of_chunk<T>(kStep);
 #pragma unroll 1
-        for (int tile = !kApart ? wave : role == 0 ? kTiles * kTiles : wave - kWaves; tile < kTiles * kTiles; tile += kApart ? kWaves : 2 * kWaves) {
-            const int s = tile / kTiles, r = tile % kTiles;
-            floatx4 p = {0.0f, 0.0f, 0.0f, 0.0f}, d = p;
-            if (r <= s) {
+        for (int tiles = !kApart ? wave : role == 0 ? all_tiles : wave - kWaves; tiles < all_tiles; tiles += kStep) {
+            const int s = tiles * kAcross<T> / kTiles, first = tiles * kAcross<T> % kTiles;
+            const int lane = lane_of_turn();
+            const In q{queries.at, lane}, k{keys.at, lane}, v{values.at, lane}, g{grads.at, lane};
+            floatx4 p[kAcross<T>] = {}, d[kAcross<T>] = {};
+#pragma unroll
+            for (int a = 0; a < kAcross<T>; a++) {
+                const int r = first + a;
+                if (r > s) continue;
 #pragma unroll
                 for (int i = 0; i < D; i += 32) {
-                    p = product(keys.straight(16 * r, i), queries.straight(16 * s, i), p);
-                    d = product(values.straight(16 * r, i), grads.straight(16 * s, i), d);
+                    p[a] = product(k.straight(16 * r, i), q.straight(16 * s, i), p[a]);
+                    d[a] = product(v.straight(16 * r, i), g.straight(16 * s, i), d[a]);
                     if (i % 64 == 32) in_order();
                 }
-                d *= decays_of<true>(reach, 16 * r, 16 * s, c.m.scale, lane);
+                d[a] *= decays_of<true>(reach, 16 * r, 16 * s, c.m.scale, lane);
 #pragma unroll
-                for (int j = 0; j < 4; j++) p[j] = 16 * s + lane % 16 > 16 * r + 4 * (lane / 16) + j ? p[j] * d[j] : 0.0f;
+                for (int j = 0; j < 4; j++) p[a][j] = 16 * s + lane % 16 > 16 * r + 4 * (lane / 16) + j ? p[a][j] * d[a][j] : 0.0f;
             }
-            if (Parts<T>::kScaled) d *= scaling.up;
-            if (r <= (s | 1)) pairs.put(16 * s, 16 * r, d);
-            const float later = sum_groups(p[0] + p[1] + p[2] + p[3]);
-            if (lane < 16) by_later[r][16 * s + lane] = later;
+            if (first <= (s | 1)) put_pairs<T>(Pairs{pairs.at, lane}, 16 * s, 16 * first, d);
 #pragma unroll
-            for (int j = 0; j < 4; j++) {
-                const float earlier = sum_lanes(p[j], 16);
-                if (lane % 16 == 0) by_earlier[s][16 * r + 4 * (lane / 16) + j] = earlier;
+            for (int a = 0; a < kAcross<T>; a++) {
+                const int r = first + a;
+                const float later = sum_groups(p[a][0] + p[a][1] + p[a][2] + p[a][3]);
+                if (lane < 16) by_later[r][16 * s + lane] = later;
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    const float earlier = sum_lanes(p[a][j], 16);
+                    if (lane % 16 == 0) by_earlier[s][16 * r + 4 * (lane / 16) + j] = earlier;
+                }
             }
         }
         if (!kApart && role == 0) down = state.template read_by<T, Parts<T>::kWhole>(grads, read);
@@ -155,7 +158,7 @@ __global__ __launch_bounds__((kQueriesThreads<T, D>), (waves_of_simd(kQueriesThr
                 }
                 sum = sum_groups(sum);
                 if (lane < 16) by_wave[wave][16 * s + lane] = sum;
-                add_pairs<T, 0, s / 2 + 1>(pairs, 16 * s, mine, scaling.down, read[s]);
+                add_pairs<T, 0, s / 2 + 1>(pairs, 16 * s, mine, read[s]);
                 in_order();
                 if (c.grad_queries && 16 * s + lane % 16 < unit.count - at) {
                     const int64_t base = ((unit.first + at + 16 * s) * c.m.heads + head) * c.m.key_size;
@@ -219,47 +222,41 @@ __global__ __launch_bounds__(kKeysThreads<D>, (waves_of_simd(kKeysThreads<D>, kK
     next.load(c, last, unit.count - last);
     float gate = 0.0f;  // of the next chunk's row, in the first wave
     if (wave == 0) reach_of(c, reaches[0], gate_of_lane<T, R>(c, unit.first + last, unit.count - last, head), unit.count - last, before);
-    if (Parts<T>::kScaled) {
-        if (threadIdx.x < 4) reaches[0].largest[threadIdx.x] = 0;
-        __syncthreads();
-    }
     int turn = 0;
     for (int64_t at = last; at >= 0; at -= R, turn ^= 1) {
         const int lane = lane_of_turn();
         const In queries{(E *)lds, lane}, keys{(E *)(lds + In::kBytes), lane}, values{(E *)(lds + 2 * In::kBytes), lane},
             grads{(E *)(lds + 3 * In::kBytes), lane};
         const Pairs scores{(E *)(lds + 4 * In::kBytes), lane}, pairs{(E *)(lds + 4 * In::kBytes + Pairs::kBytes), lane};
-        next.store(c, queries, keys, values, grads, unit.count - at, reaches[turn]);
+        next.store(c, queries, keys, values, grads, unit.count - at);
         __syncthreads();
-        if (Parts<T>::kScaled && threadIdx.x < 4) reaches[turn ^ 1].largest[threadIdx.x] = 0;
         if (at > 0) {
             next.load(c, at - R, R);
             if (wave == 0) gate = gate_of_lane<T, R>(c, unit.first + at - R, R, head);
         }
         const Reach<R> &reach = reaches[turn];
-        const Scaling for_scores = scaling_of_pairs<T>(reach, 0, 1, c.m.key_size, c.m.scale), for_pairs = scaling_of_pairs<T>(reach, 2, 3, c.m.value_size, c.m.scale);
+        const int all_tiles = tiles_of_chunk<T>(2 * kWaves);
 #pragma unroll 1
-        for (int tile = wave; tile < kTiles * kTiles; tile += 2 * kWaves) {
-            const int r = tile / kTiles, s = tile % kTiles;
-            if ((s | 1) < r) continue;
-            floatx4 p = {0.0f, 0.0f, 0.0f, 0.0f}, d = p;
-            if (s >= r) {
+        for (int tiles = wave; tiles < all_tiles; tiles += 2 * kWaves) {
+            const int r = tiles * kAcross<T> / kTiles, first = tiles * kAcross<T> % kTiles;
+            if ((first | 1) < r) continue;
+            floatx4 p[kAcross<T>] = {}, d[kAcross<T>] = {};
+#pragma unroll
+            for (int a = 0; a < kAcross<T>; a++) {
+                const int s = first + a;
+                if (s < r) continue;
 #pragma unroll
                 for (int i = 0; i < D; i += 32) {
-                    p = product(queries.straight(16 * s, i), keys.straight(16 * r, i), p);
-                    d = product(grads.straight(16 * s, i), values.straight(16 * r, i), d);
+                    p[a] = product(queries.straight(16 * s, i), keys.straight(16 * r, i), p[a]);
+                    d[a] = product(grads.straight(16 * s, i), values.straight(16 * r, i), d[a]);
                     if (i % 64 == 32) in_order();
                 }
                 const floatx4 decay = decays_of<false>(reach, 16 * s, 16 * r, c.m.scale, lane);
-                p *= decay;
-                d *= decay;
-                if (Parts<T>::kScaled) {
-                    p *= for_scores.up;
-                    d *= for_pairs.up;
-                }
+                p[a] *= decay;
+                d[a] *= decay;
             }
-            scores.put(16 * r, 16 * s, p);
-            pairs.put(16 * r, 16 * s, d);
+            put_pairs<T>(scores, 16 * r, 16 * first, p);
+            put_pairs<T>(pairs, 16 * r, 16 * first, d);
         }
         // the same for both roles: what the state reads, what its transposed rows are added up with, and what of
         const In reading{(E *)(lds + (role ? 2 : 1) * In::kBytes), lane}, with{(E *)(lds + (role ? 0 : 3) * In::kBytes), lane},
@@ -291,7 +288,7 @@ __global__ __launch_bounds__(kKeysThreads<D>, (waves_of_simd(kKeysThreads<D>, kK
                 sum = sum_groups(sum);
                 if (lane < 16) by_wave[wave - kWaves][16 * r + lane] = sum;
             }
-            add_pairs<T, r / 2, R / 32>(mine_of, 16 * r, mine, role ? for_pairs.down : for_scores.down, read[r]);
+            add_pairs<T, r / 2, R / 32>(mine_of, 16 * r, mine, read[r]);
             in_order();
             if (out && 16 * r + lane % 16 < unit.count - at) {
                 const int64_t base = ((unit.first + at + 16 * r) * c.m.heads + head) * size;

@@ -14,7 +14,8 @@
 // sums).  What goes into an output of 16 bits has two parts, states as well as the matrix of pairs inside a chunk: 2^-16 of a term, where the output's own
 // rounding is 2^-8 (pairs in one part left outputs off by 2.3e-3 of their norm in place of 1.7e-3).  Inputs in
 // float16 stay as they are, and what meets them is two parts in float16 (an error of 2^-22): states and weighted inputs by a power of two that brings
-// the largest of a wave's numbers near 2^15, pairs by one that brings the largest they could be there.
+// the largest of a wave's numbers near 2^15, 32 pairs of a row by one that brings the largest of them there, so that no other row has a part in how
+// they are rounded.
 #pragma once
 #include "tg_attention.hpp"
 
@@ -184,6 +185,11 @@ template <class E, int N, int Rows, int Columns, bool Turned = true> struct Tile
         }
         return x;
     }
+    // What 32 pairs of a row from column 32 `strip` on are to be multiplied with, in the bytes behind the row's numbers.
+    __device__ __forceinline__ float &factor(int row, int strip) const {
+        static_assert(!Turned && Columns <= 128);
+        return ((float *)(at + row * kStride + Columns))[strip];
+    }
     // An accumulator's four rows (columns here) of its column (a row here): the product's transpose.
     __device__ __forceinline__ void put(int row, int column, floatx4 x) const {
         static_assert(!Turned);
@@ -216,7 +222,38 @@ template <class E, int N> __device__ __forceinline__ void weighted(const Operand
 
 // The matrix of pairs inside a chunk.
 template <class T> using PairsOf = Tile<typename Parts<T>::Element, Parts<T>::kState, Parts<T>::kRows, Parts<T>::kRows, false>;
+// Neighbouring tiles of sixteen columns that a wave makes at a time: those of a product over 32 columns where they have one scaling.
+template <class T> constexpr int kAcross = Parts<T>::kScaled ? 2 : 1;
 
+// How many of a chunk's tiles there are for waves that take every `waves`th.  Where that is one turn the compiler does not know it: it would take the loop
+// away, and fill the registers with what is read behind it.
+template <class T> __device__ __forceinline__ int tiles_of_chunk(int waves) {
+    int n = Parts<T>::kRows / 16 * Parts<T>::kRows / 16 / kAcross<T>;
+    if (n <= waves) asm volatile("" : "+s"(n));
+    return n;
+}
+
+// Puts sixteen rows of pairs from `row` on, scaled by row where they have to be.
+template <class T> __device__ __forceinline__ void put_pairs(const PairsOf<T> &pairs, int row, int column, floatx4 (&p)[kAcross<T>]) {
+    if constexpr (Parts<T>::kScaled) {
+        float most = 0.0f;  // of the row's numbers in this lane, then in all four that have some
+#pragma unroll
+        for (int a = 0; a < kAcross<T>; a++)
+#pragma unroll
+            for (int j = 0; j < 4; j++) most = fmaxf(most, fabsf(p[a][j]));
+        most = fmaxf(most, __shfl_xor(most, 16));
+        most = fmaxf(most, __shfl_xor(most, 32));
+        const Scaling scaling = scaling_of(__float_as_uint(most));
+#pragma unroll
+        for (int a = 0; a < kAcross<T>; a++) p[a] *= scaling.up;
+        if (pairs.lane < 16) pairs.factor(row + pairs.lane, column / 32) = scaling.down;
+    }
+#pragma unroll
+    for (int a = 0; a < kAcross<T>; a++) pairs.put(row, column + 16 * a, p[a]);
+}
+
+// Keeps the compiler from reading ahead over this point: operands of a whole chunk, read at its beginning, would not fit the registers.
+__device__ __forceinline__ void in_order() { __builtin_amdgcn_sched_barrier(0); }
 // ---- reading a chunk ----------------------------------------------------------------------
 
 // A thread's part of a chunk of Rows x D numbers, on its way to LDS: groups of eight neighbours.  Vector: in accesses of 16 bytes, which divide the
@@ -240,9 +277,7 @@ template <class T, int Rows, int D, int Threads, bool Vector> struct Incoming {
             for (int j = 0; j < 8; j += kWidest) x[n][j / kWidest] = load_pack<kWidest>(from + min(column_of(n) + j, size - kWidest));
         }
     }
-    // `largest`: where the largest of the numbers is kept as bits, if that is wanted (Scaled).
-    template <class E, int N, bool Scaled> __device__ __forceinline__ void store(const Tile<E, N, Rows, D> &tile, int64_t count, int size, uint32_t *largest) const {
-        uint32_t most = 0;
+    template <class E, int N> __device__ __forceinline__ void store(const Tile<E, N, Rows, D> &tile, int64_t count, int size) const {
 #pragma unroll
         for (int n = 0; n < kGroups; n++) {
             if (!mine(n)) continue;
@@ -251,10 +286,6 @@ template <class T, int Rows, int D, int Threads, bool Vector> struct Incoming {
             if constexpr (Vector && N == 1) {  // as it is
                 const uint32x4 w = __builtin_bit_cast(uint32x4, x[n][0]), none = {0, 0, 0, 0}, v = row < count && column < size ? w : none;
                 *(uint32x4 *)(tile.at + place) = v;
-                if constexpr (Scaled) {
-#pragma unroll
-                    for (int j = 0; j < 4; j++) most = max(most, max(v[j] & 0x7fffu, v[j] >> 16 & 0x7fffu));
-                }
                 continue;
             }
             float v[8];
@@ -264,15 +295,6 @@ template <class T, int Rows, int D, int Threads, bool Vector> struct Incoming {
 #pragma unroll
             for (int i = 0; i < N; i++)
                 *(typename Vectors<E>::x8 *)(tile.at + i * In::kPart + place) = o.part[i];
-            if constexpr (Scaled) {
-                const uint32x4 w = __builtin_bit_cast(uint32x4, o.part[0]);
-#pragma unroll
-                for (int j = 0; j < 4; j++) most = max(most, max(w[j] & 0x7fffu, w[j] >> 16 & 0x7fffu));
-            }
-        }
-        if constexpr (Scaled) {
-            most = largest_of_wave(most);
-            if (threadIdx.x % kWave == 0) atomicMax(largest, __float_as_uint((float)__builtin_bit_cast(_Float16, (uint16_t)most)));
         }
     }
 };
@@ -291,14 +313,7 @@ template <int Rows> struct alignas(16) Reach {
     float column[Rows];   // 2^(L_C - L)
     float start[Rows];    // scale 2^L from the unit's beginning
     float whole;          // 2^L_C
-    uint32_t largest[4];  // of the chunk's queries, keys, values and gradients of outputs, as bits
 };
-
-// The scaling of products of a row of each of two of a chunk's inputs, of `size` numbers.
-template <class T, int Rows> __device__ __forceinline__ Scaling scaling_of_pairs(const Reach<Rows> &reach, int first, int second, int size, float scale) {
-    if constexpr (!Parts<T>::kScaled) return {1.0f, 1.0f};
-    return scaling_of(__float_as_uint(fabsf(scale) * (float)size * __uint_as_float(reach.largest[first]) * __uint_as_float(reach.largest[second])));
-}
 
 struct AttentionCall {
     Attention m;
@@ -432,9 +447,6 @@ __device__ __forceinline__ int lane_of_turn() {
     asm volatile("" : "+v"(lane));
     return lane;
 }
-
-// Keeps the compiler from reading ahead over this point: operands of a whole chunk, read at its beginning, would not fit the registers.
-__device__ __forceinline__ void in_order() { __builtin_amdgcn_sched_barrier(0); }
 
 // Whether State::fold adds up apart, where the registers are enough: 8 x 2048 rows of 32 heads of 64 with fixed decays near 1, states off by 1.1e-7 in
 // place of 2.7e-7 and the decays' gradients by 5e-7 in place of 9e-7, in the same time; but 4 x 4096 rows of 16 heads of 128 the outputs' kernel 160 us
@@ -597,23 +609,23 @@ __device__ __forceinline__ void columns_of(const Tile<E, N, Rows, D> &tile, int 
 
 // += this wave's columns times sixteen rows of pairs from `row` on, those of the columns from First on to before Last.
 template <class T, int First, int Last, class E, int N, int Rows, int W>
-__device__ __forceinline__ void add_pairs(const Tile<E, Parts<T>::kState, Rows, Rows, false> &pairs, int row, const Operand<E, N> (&mine)[Rows / 32][W], float down, floatx4 (&sums)[W]) {
-    floatx4 inside[W] = {};
+__device__ __forceinline__ void add_pairs(const Tile<E, Parts<T>::kState, Rows, Rows, false> &pairs, int row, const Operand<E, N> (&mine)[Rows / 32][W], floatx4 (&sums)[W]) {
 #pragma unroll
     for (int k = First; k < Last; k++) {
         const Operand<E, Parts<T>::kState> p = pairs.chained(row, 32 * k);
+        if constexpr (Parts<T>::kScaled) {
+            const float down = pairs.factor(row + pairs.lane % 16, k);
 #pragma unroll
-        for (int w = 0; w < W; w++)
-            if (Parts<T>::kScaled)
-                inside[w] = product(mine[k][w], p, inside[w]);
-            else
-                sums[w] = product(mine[k][w], p, sums[w]);
+            for (int w = 0; w < W; w++) {
+                const floatx4 inside = product(mine[k][w], p, floatx4{0.0f, 0.0f, 0.0f, 0.0f});
+#pragma unroll
+                for (int j = 0; j < 4; j++) sums[w][j] = fmaf(inside[j], down, sums[w][j]);
+            }
+        } else {
+#pragma unroll
+            for (int w = 0; w < W; w++) sums[w] = product(mine[k][w], p, sums[w]);
+        }
     }
-    if (Parts<T>::kScaled)
-#pragma unroll
-        for (int w = 0; w < W; w++)
-#pragma unroll
-            for (int j = 0; j < 4; j++) sums[w][j] = fmaf(inside[w][j], down, sums[w][j]);
 }
 
 // `size`: 32, 64 or 128, of keys and values in the kernel

@@ -39,8 +39,8 @@ __global__ __launch_bounds__(kThreads<D>, waves_of_simd(kThreads<D>, kStatesLds<
     for (int64_t at = 0; at < unit.count; at += R, turn ^= 1) {
         const int lane = lane_of_turn();
         const In keys{lds, lane}, values{lds + In::kBytes / 2, lane};
-        next_k.template store<E, N, false>(keys, unit.count - at, c.m.key_size, nullptr);
-        next_v.template store<E, N, false>(values, unit.count - at, c.m.value_size, nullptr);
+        next_k.template store<E, N>(keys, unit.count - at, c.m.key_size);
+        next_v.template store<E, N>(values, unit.count - at, c.m.value_size);
         __syncthreads();
         if (at + R < unit.count) {
             next_k.load(k + (at + R) * c.m.k.row, c.m.k.row, unit.count - at - R, c.m.key_size);
@@ -62,7 +62,6 @@ __global__ __launch_bounds__(kThreads<D>, waves_of_simd(kThreads<D>, kStatesLds<
 template <class T, int D, bool Vector>
 __global__ __launch_bounds__(kThreads<D>, waves_of_simd(kThreads<D>, kOutputsLds<T, D>, W * D / 4)) void attention_outputs_kernel(AttentionCall c) {
     constexpr int R = Parts<T>::kRows, N = Parts<T>::kInput, M = Parts<T>::kState, kTiles = R / 16, kWaves = State<D, W>::kWaves;
-    constexpr bool kScaled = Parts<T>::kScaled;
     using E = typename Parts<T>::Element;
     using In = Tile<E, N, R, D>;
     using Pairs = PairsOf<T>;
@@ -102,10 +101,6 @@ __global__ __launch_bounds__(kThreads<D>, waves_of_simd(kThreads<D>, kOutputsLds
     if (unit.count > 0) load(0);
     float gate = 0.0f;  // of the next chunk's row, in the first wave
     if (wave == 0) reach_of(c, reaches[0], gate_of_lane<T, R>(c, unit.first, unit.count, head), unit.count, before);
-    if (kScaled) {
-        if (threadIdx.x < 4) reaches[0].largest[threadIdx.x] = 0;
-        __syncthreads();
-    }
     int turn = 0, chunk = 0;
     for (int64_t at = 0; at < unit.count; at += R, turn ^= 1) {
         const int lane = lane_of_turn();
@@ -116,29 +111,31 @@ __global__ __launch_bounds__(kThreads<D>, waves_of_simd(kThreads<D>, kOutputsLds
             u++;
         }
         chunk = chunk + 1 == c.chunks ? 0 : chunk + 1;
-        next_q.template store<E, N, kScaled>(queries, unit.count - at, c.m.key_size, &reaches[turn].largest[0]);
-        next_k.template store<E, N, kScaled>(keys, unit.count - at, c.m.key_size, &reaches[turn].largest[1]);
-        next_v.template store<E, N, false>(values, unit.count - at, c.m.value_size, nullptr);
+        next_q.template store<E, N>(queries, unit.count - at, c.m.key_size);
+        next_k.template store<E, N>(keys, unit.count - at, c.m.key_size);
+        next_v.template store<E, N>(values, unit.count - at, c.m.value_size);
         __syncthreads();
-        if (kScaled && threadIdx.x < 4) reaches[turn ^ 1].largest[threadIdx.x] = 0;
         if (at + R < unit.count) {
             load(at + R);
             if (wave == 0) gate = gate_of_lane<T, R>(c, unit.first + at + R, unit.count - at - R, head);
         }
         const Reach<R> &reach = reaches[turn];
-        const Scaling scaling = scaling_of_pairs<T>(reach, 0, 1, c.m.key_size, c.m.scale);
         // pairs: row s, column r
+        const int all_tiles = tiles_of_chunk<T>(kWaves);
 #pragma unroll 1
-        for (int tile = wave; tile < kTiles * kTiles; tile += kWaves) {
-            const int s = tile / kTiles, r = tile % kTiles;
-            if (r > (s | 1)) continue;
-            floatx4 p = {0.0f, 0.0f, 0.0f, 0.0f};
-            if (r <= s) {
+        for (int tiles = wave; tiles < all_tiles; tiles += kWaves) {
+            const int s = tiles * kAcross<T> / kTiles, first = tiles * kAcross<T> % kTiles;
+            if (first > (s | 1)) continue;
+            floatx4 p[kAcross<T>] = {};
 #pragma unroll
-                for (int i = 0; i < D; i += 32) p = product(keys.straight(16 * r, i), queries.straight(16 * s, i), p);
-                p *= decays_of<true>(reach, 16 * r, 16 * s, c.m.scale * scaling.up, lane);
+            for (int a = 0; a < kAcross<T>; a++) {
+                const int r = first + a;
+                if (r > s) continue;
+#pragma unroll
+                for (int i = 0; i < D; i += 32) p[a] = product(keys.straight(16 * r, i), queries.straight(16 * s, i), p[a]);
+                p[a] *= decays_of<true>(reach, 16 * r, 16 * s, c.m.scale, lane);
             }
-            pairs.put(16 * s, 16 * r, p);
+            put_pairs<T>(pairs, 16 * s, 16 * first, p);
         }
         floatx4 read[kTiles][W] = {};
         const float down = state.template read_by<T, M>(queries, read);
@@ -150,7 +147,7 @@ __global__ __launch_bounds__(kThreads<D>, waves_of_simd(kThreads<D>, kOutputsLds
             const float decay = reach.row[16 * s + lane % 16] * down;
 #pragma unroll
             for (int w = 0; w < W; w++) read[s][w] *= decay;
-            add_pairs<T, 0, s / 2 + 1>(pairs, 16 * s, mine, scaling.down, read[s]);
+            add_pairs<T, 0, s / 2 + 1>(pairs, 16 * s, mine, read[s]);
             in_order();
             const int to = column + 4 * (lane / 16);
             if (16 * s + lane % 16 < unit.count - at) {
