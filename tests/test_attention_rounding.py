@@ -101,3 +101,57 @@ def test_pairs_of_a_query_that_is_not_finite(cuda, dtype, K, V, value):
     keep = torch.ones_like(got[0], dtype=torch.bool)
     keep[1, 70, 0] = False
     assert torch.equal(got[0][keep], want[0][keep])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("K,V", [(32, 32), (64, 128)])
+@pytest.mark.parametrize("dtype", [F16, BF16, F32])
+def test_values_of_different_size(cuda, dtype, K, V):
+    """Columns of a state far smaller than their neighbours have float32's accuracy too."""
+    parts, _ = make(cuda, 9, 300, 2, 1, K, V, dtype)
+    sizes = 2.0 ** torch.linspace(-9, 12, V, device=cuda).round()[torch.randperm(V, generator=torch.Generator().manual_seed(1)).to(cuda)]
+    parts[2] *= sizes
+    got, wanted = passes(cuda, parts, None, 1)
+    for name, t, (value, magnitude) in list(zip(NAMES, got, wanted))[:2]:
+        assert_rounded_once(name, t, value, magnitude, 300)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("K,V", [(32, 32), (128, 72), (24, 64)])
+@pytest.mark.parametrize("dtype", [F16, BF16, F32])
+@pytest.mark.parametrize("value", [float("inf"), float("nan")])
+def test_columns_that_are_not_finite(cuda, dtype, K, V, value):
+    """A value, or an output's gradient, spoils its own column of states and outputs (in float32 its neighbour's too): the others keep all their terms, bit
+    by bit."""
+    import trigrad_amd
+    parts, h0 = make(cuda, 5, 2 * 200, 2, 1, K, V, dtype, sequences=2)
+    args = [t.view(2, 200, *t.shape[1:]) for t in parts] + [h0]
+    g = torch.Generator().manual_seed(0)
+    grads = [torch.randn(args[2].shape, generator=g).to(cuda, dtype), torch.randn(h0.shape, generator=g).to(cuda)]
+
+    def results(args, grads):
+        leaves = [t.detach().requires_grad_() for t in args]
+        out = trigrad_amd.linear_attention(*leaves)
+        return [*(t.detach() for t in out), *torch.autograd.grad(out, leaves, grads)]
+    want = results(args, grads)
+    column = slice(4 if dtype == F32 else 5, 6)
+    # a value's
+    spoiled = [t.clone() for t in args]
+    spoiled[2][1, 70, 0, 5] = value
+    o, final = results(spoiled, grads)[:2]
+    assert not o[1, 70:, 0, 5].isfinite().any() and not final[1, 0, :, 5].isfinite().any()
+    for t, w, at in ((o, want[0], (1, slice(None), 0, column)), (final, want[1], (1, 0, slice(None), column))):
+        keep = torch.ones_like(t, dtype=torch.bool)
+        keep[at] = False
+        assert torch.equal(t[keep], w[keep])
+    # a gradient's: column 5 of D up to its row, the row's query, the keys up to it (and those of its chunk)
+    spoiled = [t.clone() for t in grads]
+    spoiled[0][1, 70, 0, 5] = value
+    _, _, dq, dk, dv, dg, dh = results(args, spoiled)
+    assert not dq[1, 70, 0].isfinite().any() and not dk[1, :71, 0].isfinite().any()
+    assert not dv[1, :71, 0, 5].isfinite().any() and not dh[1, 0, :, 5].isfinite().any()
+    for t, w, at in ((dq, want[2], (1, 70, 0)), (dk, want[3], (1, slice(0, 128), 0)), (dv, want[4], (1, slice(None), 0, column)), (dg, want[5], (1, slice(None), 0)),
+                     (dh, want[6], (1, 0, slice(None), column))):
+        keep = torch.ones_like(t, dtype=torch.bool)
+        keep[at] = False
+        assert torch.equal(t[keep], w[keep])

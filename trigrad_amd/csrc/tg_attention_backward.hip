@@ -19,10 +19,11 @@ __device__ __forceinline__ float sum_groups(float v) {
 // they are compiled for: two, with 256 registers, where LDS has room for one workgroup.
 //
 // W of State, 4 x 4096 rows of 16 heads of 128 in bfloat16, and 2 x 3000 of 8 in float32: the queries' kernel 180 and 81 us with one, 192 and 63 with
-// two; the keys' 335 and 93 with one, 189 and 65 with two.  8 x 2048 rows of 32 heads of 64: 129 and 127 with one, 161 and 141 with two.
+// two; the keys' 335 and 93 with one, 189 and 65 with two.  8 x 2048 rows of 32 heads of 64: 129 and 127 with one, 161 and 141 with two.  In float16,
+// whose scalings take registers, the first of these forward and backward: 539 with one in the queries' kernel, 512 with two.
 // Instructions bound both: making parts, matrix instructions and readings of LDS take a third to a half of the time each and hardly overlap, as all
 // waves of a workgroup are in the same phase (1.9 TB/s of memory for heads of 128, 2.6 for those of 64).
-template <class T, int D> constexpr int kQueriesColumns = D > 64 && sizeof(T) == 4 ? 2 : 1;
+template <class T, int D> constexpr int kQueriesColumns = D > 64 && (sizeof(T) == 4 || Parts<T>::kScaled) ? 2 : 1;
 template <int D> constexpr int kKeysColumns = D > 64 ? 2 : 1;
 template <class T, int D> constexpr int kQueriesThreads = 2 * State<D, kQueriesColumns<T, D>>::kWaves * kWave;
 template <int D> constexpr int kKeysThreads = 2 * State<D, kKeysColumns<D>>::kWaves * kWave;
@@ -102,8 +103,8 @@ __global__ __launch_bounds__((kQueriesThreads<T, D>), (waves_of_simd(kQueriesThr
         // Pairs by all waves, or, with as many waves that the others have enough to do meanwhile, by those that add to D while those of S read it.
         constexpr bool kApart = D > 64;
         floatx4 read[kTiles][W] = {};
-        float down = 1.0f;
-        if (kApart && role == 0) down = state.template read_by<T, Parts<T>::kWhole>(grads, read);
+        float down[W];
+        if (kApart && role == 0) state.template read_by<T, Parts<T>::kWhole>(grads, read, down);
         constexpr int kStep = kApart ? kWaves : 2 * kWaves;
         const int all_tiles = tiles_of_chunk<T>(kStep);
 #pragma unroll 1
@@ -139,19 +140,18 @@ __global__ __launch_bounds__((kQueriesThreads<T, D>), (waves_of_simd(kQueriesThr
                 }
             }
         }
-        if (!kApart && role == 0) down = state.template read_by<T, Parts<T>::kWhole>(grads, read);
+        if (!kApart && role == 0) state.template read_by<T, Parts<T>::kWhole>(grads, read, down);
         __syncthreads();
         Operand<E, N> mine[R / 32][W];
         if (role == 0) {
             columns_of(keys, column, mine);
             each_of<kTiles>([&](auto number) {
                 constexpr int s = decltype(number)::value;
-                const float decay = reach.row[16 * s + lane % 16] * down;
+                scale_read<T>(read[s], reach.row[16 * s + lane % 16], down, lane);
                 const int to = column + 4 * (lane / 16);
                 float sum = 0.0f;
 #pragma unroll
                 for (int w = 0; w < W; w++) {
-                    read[s][w] *= decay;
                     const floatx4 x = queries.numbers(16 * s, column + 16 * w);
 #pragma unroll
                     for (int j = 0; j < 4; j++) sum = fmaf(read[s][w][j], x[j], sum);
@@ -263,20 +263,18 @@ __global__ __launch_bounds__(kKeysThreads<D>, (waves_of_simd(kKeysThreads<D>, kK
             adding{(E *)(lds + (role ? 3 : 0) * In::kBytes), lane};
         const Pairs mine_of{(E *)(lds + 4 * In::kBytes + role * Pairs::kBytes), lane};
         floatx4 read[kTiles][W] = {};
-        float down;
+        float down[W];
         if (role)
-            down = state.template read_by<T, Parts<T>::kWhole>(reading, read);
+            state.template read_by<T, Parts<T>::kWhole>(reading, read, down);
         else
-            down = state.template read_by<T, Parts<T>::kState>(reading, read);
+            state.template read_by<T, Parts<T>::kState>(reading, read, down);
         __syncthreads();
         Operand<E, N> mine[R / 32][W];
         columns_of(with, column, mine);
         each_of<kTiles>([&](auto number) {
             constexpr int r = decltype(number)::value;
-            const float decay = reach.column[16 * r + lane % 16] * down;
+            scale_read<T>(read[r], reach.column[16 * r + lane % 16], down, lane);
             const int to = column + 4 * (lane / 16);
-#pragma unroll
-            for (int w = 0; w < W; w++) read[r][w] *= decay;
             if (role) {
                 float sum = 0.0f;
 #pragma unroll

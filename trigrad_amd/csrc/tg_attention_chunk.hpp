@@ -13,9 +13,9 @@
 // go into is float32 in the end (states, their gradients, gates' gradients: two parts leave an error of 2e-6, three one of 1e-8, below that of the
 // sums).  What goes into an output of 16 bits has two parts, states as well as the matrix of pairs inside a chunk: 2^-16 of a term, where the output's own
 // rounding is 2^-8 (pairs in one part left outputs off by 2.3e-3 of their norm in place of 1.7e-3).  Inputs in
-// float16 stay as they are, and what meets them is two parts in float16 (an error of 2^-22): states and weighted inputs by a power of two that brings
-// the largest of a wave's numbers near 2^15, 32 pairs of a row by one that brings the largest of them there, so that no other row has a part in how
-// they are rounded.
+// float16 stay as they are, and what meets them is two parts in float16 (an error of 2^-22 of each, or 2^-39 of the largest): a column of a state or of
+// weighted inputs, and 32 pairs of a row, by a power of two that brings the largest of them near 2^15.  What they are summed with has the same column, or row:
+// no other has a part in how they are rounded, also where it is not finite.
 #pragma once
 #include "tg_attention.hpp"
 
@@ -107,26 +107,14 @@ template <class E, int N> __device__ __forceinline__ Operand<E, N> parts_of(cons
     return o;
 }
 
-// The largest of a wave's numbers, none of which is negative, as bits.
-template <int Control, int RowMask> __device__ __forceinline__ uint32_t or_lane(uint32_t v) {
-    return max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, Control, RowMask, 0xf, false));
-}
-__device__ __forceinline__ uint32_t largest_of_wave(uint32_t v) {
-    v = or_lane<0x111, 0xf>(v);
-    v = or_lane<0x112, 0xf>(v);
-    v = or_lane<0x114, 0xf>(v);
-    v = or_lane<0x118, 0xf>(v);
-    v = or_lane<0x142, 0xa>(v);
-    v = or_lane<0x143, 0xc>(v);
-    return (uint32_t)__builtin_amdgcn_readlane((int)v, kWave - 1);
-}
-
-// A power of two that brings numbers of at most `largest` to at most 2^15, and its reciprocal.
+// A power of two that brings the largest of four lanes' numbers (16 lanes apart; `most` is this lane's, none is negative) to at most 2^15, and its reciprocal.
 struct Scaling {
     float up, down;
 };
-__device__ __forceinline__ Scaling scaling_of(uint32_t largest_bits) {
-    const int exponent = max(1, min(253, 268 - (int)(largest_bits >> 23)));
+__device__ __forceinline__ Scaling scaling_of(float most) {
+    most = fmaxf(most, __shfl_xor(most, 16));
+    most = fmaxf(most, __shfl_xor(most, 32));
+    const int exponent = max(1, min(253, 268 - (int)(__float_as_uint(most) >> 23)));
     return {__uint_as_float((uint32_t)exponent << 23), __uint_as_float((uint32_t)(254 - exponent) << 23)};
 }
 
@@ -236,14 +224,12 @@ template <class T> __device__ __forceinline__ int tiles_of_chunk(int waves) {
 // Puts sixteen rows of pairs from `row` on, scaled by row where they have to be.
 template <class T> __device__ __forceinline__ void put_pairs(const PairsOf<T> &pairs, int row, int column, floatx4 (&p)[kAcross<T>]) {
     if constexpr (Parts<T>::kScaled) {
-        float most = 0.0f;  // of the row's numbers in this lane, then in all four that have some
+        float most = 0.0f;  // of the row's numbers in this lane
 #pragma unroll
         for (int a = 0; a < kAcross<T>; a++)
 #pragma unroll
             for (int j = 0; j < 4; j++) most = fmaxf(most, fabsf(p[a][j]));
-        most = fmaxf(most, __shfl_xor(most, 16));
-        most = fmaxf(most, __shfl_xor(most, 32));
-        const Scaling scaling = scaling_of(__float_as_uint(most));
+        const Scaling scaling = scaling_of(most);
 #pragma unroll
         for (int a = 0; a < kAcross<T>; a++) p[a] *= scaling.up;
         if (pairs.lane < 16) pairs.factor(row + pairs.lane, column / 32) = scaling.down;
@@ -485,18 +471,22 @@ template <int D, int W> struct State {
     template <bool Turned> __device__ __forceinline__ void store(float *to, int column, int key_size, int value_size) {
         each<Turned>(column, key_size, value_size, [&](int w, int n, int j, int at) { to[at] = x[w][n][j]; });
     }
-    // Adds its transpose times the rows' columns to `sums`, by sixteen rows of the tile; -> what the sums are to be multiplied with.
-    template <class T, int M, class E, int N, int Rows> __device__ __forceinline__ float read_by(const Tile<E, N, Rows, D> &tile, floatx4 (&sums)[Rows / 16][W]) const {
-        Scaling scaling = {1.0f, 1.0f};
+    // Adds its transpose times the rows' columns to `sums`, by sixteen rows of the tile; `down`: what the sums are to be multiplied with, by column (Scaled).
+    template <class T, int M, class E, int N, int Rows>
+    __device__ __forceinline__ void read_by(const Tile<E, N, Rows, D> &tile, floatx4 (&sums)[Rows / 16][W], float (&down)[W]) const {
+        float up[W];
         if constexpr (Parts<T>::kScaled) {
-            float most = 0.0f;
 #pragma unroll
-            for (int w = 0; w < W; w++)
+            for (int w = 0; w < W; w++) {
+                float most = 0.0f;
 #pragma unroll
                 for (int n = 0; n < D / 16; n++)
 #pragma unroll
                     for (int j = 0; j < 4; j++) most = fmaxf(most, fabsf(x[w][n][j]));
-            scaling = scaling_of(largest_of_wave(__float_as_uint(most)));
+                const Scaling scaling = scaling_of(most);
+                up[w] = scaling.up;
+                down[w] = scaling.down;
+            }
         }
 #pragma unroll
         for (int i = 0; i < D / 32; i++) {
@@ -505,7 +495,7 @@ template <int D, int W> struct State {
             for (int w = 0; w < W; w++) {
                 float v[8];
 #pragma unroll
-                for (int j = 0; j < 8; j++) v[j] = Parts<T>::kScaled ? x[w][2 * i + j / 4][j % 4] * scaling.up : x[w][2 * i + j / 4][j % 4];
+                for (int j = 0; j < 8; j++) v[j] = Parts<T>::kScaled ? x[w][2 * i + j / 4][j % 4] * up[w] : x[w][2 * i + j / 4][j % 4];
                 mine[w] = parts_of<E, M>(v);
             }
 #pragma unroll
@@ -516,7 +506,6 @@ template <int D, int W> struct State {
             }
             in_order();
         }
-        return scaling.down;
     }
     // decay times itself, plus the tile, transposed, times this wave's columns `mine` of another with a weight for each row.  Apart: 32 rows are added
     // up apart, so that a long state is rounded twice a chunk and not by each of six products.
@@ -524,25 +513,26 @@ template <int D, int W> struct State {
     __device__ __forceinline__ void fold(float decay, const Tile<E, N, Rows, D> &tile, const Operand<E, N> (&mine)[Rows / 32][W], const float *weights) {
         constexpr int M = Parts<T>::kWhole, K = Rows / 32;
         if constexpr (Parts<T>::kScaled) {
-            float v[K][W][8], most = 0.0f;
-#pragma unroll
-            for (int k = 0; k < K; k++)
-#pragma unroll
-                for (int w = 0; w < W; w++) {
-                    weighted(mine[k][w], weights, 32 * k, tile.lane, v[k][w]);
-#pragma unroll
-                    for (int j = 0; j < 8; j++) most = fmaxf(most, fabsf(v[k][w][j]));
-                }
-            const Scaling scaling = scaling_of(largest_of_wave(__float_as_uint(most)));
             Operand<E, M> late[K][W];
+            float down[W];
 #pragma unroll
-            for (int k = 0; k < K; k++)
+            for (int w = 0; w < W; w++) {
+                float v[K][8], most = 0.0f;
 #pragma unroll
-                for (int w = 0; w < W; w++) {
+                for (int k = 0; k < K; k++) {
+                    weighted(mine[k][w], weights, 32 * k, tile.lane, v[k]);
 #pragma unroll
-                    for (int j = 0; j < 8; j++) v[k][w][j] *= scaling.up;
-                    late[k][w] = parts_of<E, M>(v[k][w]);
+                    for (int j = 0; j < 8; j++) most = fmaxf(most, fabsf(v[k][j]));
                 }
+                const Scaling scaling = scaling_of(most);
+                down[w] = scaling.down;
+#pragma unroll
+                for (int k = 0; k < K; k++) {
+#pragma unroll
+                    for (int j = 0; j < 8; j++) v[k][j] *= scaling.up;
+                    late[k][w] = parts_of<E, M>(v[k]);
+                }
+            }
 #pragma unroll
             for (int n = 0; n < D / 16; n++) {
                 floatx4 sum[W] = {};
@@ -555,7 +545,7 @@ template <int D, int W> struct State {
 #pragma unroll
                 for (int w = 0; w < W; w++)
 #pragma unroll
-                    for (int j = 0; j < 4; j++) x[w][n][j] = fmaf(sum[w][j], scaling.down, x[w][n][j] * decay);
+                    for (int j = 0; j < 4; j++) x[w][n][j] = fmaf(sum[w][j], down[w], x[w][n][j] * decay);
                 if (n % 4 == 3) in_order();
             }
         } else {
@@ -595,6 +585,18 @@ template <int N, class Call> __device__ __forceinline__ void each_of(Call &&call
     if constexpr (N > 0) {
         each_of<N - 1>(call);
         call(std::integral_constant<int, N - 1>());
+    }
+}
+
+// What a state gave sixteen rows, times their decay, and times what lanes 0 to 15 have for its columns.
+template <class T, int W> __device__ __forceinline__ void scale_read(floatx4 (&read)[W], float decay, const float (&down)[W], int lane) {
+#pragma unroll
+    for (int w = 0; w < W; w++) {
+        read[w] *= decay;
+        if constexpr (Parts<T>::kScaled) {
+#pragma unroll
+            for (int j = 0; j < 4; j++) read[w][j] *= __shfl(down[w], 4 * (lane / 16) + j);
+        }
     }
 }
 

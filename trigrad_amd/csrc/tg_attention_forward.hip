@@ -138,15 +138,14 @@ __global__ __launch_bounds__(kThreads<D>, waves_of_simd(kThreads<D>, kOutputsLds
             put_pairs<T>(pairs, 16 * s, 16 * first, p);
         }
         floatx4 read[kTiles][W] = {};
-        const float down = state.template read_by<T, M>(queries, read);
+        float down[W];
+        state.template read_by<T, M>(queries, read, down);
         __syncthreads();
         Operand<E, N> mine[R / 32][W];
         columns_of(values, column, mine);
         each_of<kTiles>([&](auto number) {
             constexpr int s = decltype(number)::value;
-            const float decay = reach.row[16 * s + lane % 16] * down;
-#pragma unroll
-            for (int w = 0; w < W; w++) read[s][w] *= decay;
+            scale_read<T>(read[s], reach.row[16 * s + lane % 16], down, lane);
             add_pairs<T, 0, s / 2 + 1>(pairs, 16 * s, mine, read[s]);
             in_order();
             const int to = column + 4 * (lane / 16);
