@@ -163,7 +163,7 @@ class AdamW(torch.optim.Optimizer):
                                       capturable=capturable, seed=seed))
 
     def _new_state(self, p, group, first):
-        """The state of a parameter before its first step; `first`: the count of those that begin with it."""
+        """The state of a parameter before its first step; `first`: the count of those on its device that begin with it."""
         state = {"step": first}
         if p.dtype in COPY_TYPES:
             state["master"] = p.detach().to(torch.float32, copy=True, memory_format=torch.contiguous_format)
@@ -184,19 +184,26 @@ class AdamW(torch.optim.Optimizer):
                 loss = closure()
         for group in self.param_groups:
             params = [p for p in group["params"] if p.grad is not None]
-            first = None
+            firsts = {}  # by device
             for p in params:
                 if not self.state[p]:
                     if p.grad.is_sparse:
                         raise RuntimeError("gradients must be dense")
-                    if first is None:
-                        first = torch.zeros(1, dtype=torch.float32, device=p.device) if group["capturable"] else 0
-                    self.state[p].update(self._new_state(p, group, first))
+                    if p.device not in firsts:
+                        firsts[p.device] = torch.zeros(1, dtype=torch.float32, device=p.device) if group["capturable"] else 0
+                    self.state[p].update(self._new_state(p, group, firsts[p.device]))
             calls = {}  # parameters of the same device, type and count together
+            counts = {}  # those on the device, each of which counts once whatever calls read it
             for p in params:
-                count = self.state[p]["step"]
-                same = id(count) if isinstance(count, torch.Tensor) else count
-                calls.setdefault((p.device, self.state[p].get("master", p).dtype, same), []).append(p)
+                state = self.state[p]
+                if isinstance(state["step"], torch.Tensor):
+                    same = id(state["step"])
+                    counts[same] = state["step"]
+                else:
+                    same = state["step"] = state["step"] + 1
+                calls.setdefault((p.device, state.get("master", p).dtype, same), []).append(p)
+            for count in counts.values():
+                count.add_(1.0)
             for together in calls.values():
                 self._step_together(group, together, grad_scale)
         return loss
@@ -204,12 +211,6 @@ class AdamW(torch.optim.Optimizer):
     def _step_together(self, group, params: List[torch.Tensor], grad_scale):
         states = [self.state[p] for p in params]
         count = states[0]["step"]
-        if isinstance(count, torch.Tensor):
-            count.add_(1.0)
-        else:
-            count += 1
-            for s in states:
-                s["step"] = count
         eight = group["state_bits"] == 8
         low = any("master" in s for s in states)
         adamw_step([s.get("master", p) for s, p in zip(states, params)], [p.grad for p in params], [s["exp_avg"] for s in states],
