@@ -56,3 +56,42 @@ def test_devices_of_a_group(calls):
         optimizer.step()
     assert counts_of(calls, params[0]) == [1, 2]
     assert all(len(c["devices"]) == 1 for c in calls) and len(calls) == 4
+
+
+@pytest.mark.parametrize("kwargs", KINDS)
+def test_a_step_without_a_gradient(calls, kwargs):
+    """Such a parameter is where it was: its next step has the next number."""
+    import trigrad_amd
+    a, b, c = leaf(), leaf(), leaf()
+    optimizer = trigrad_amd.AdamW([a, b, c], **kwargs)
+    for skipped in ((), (b,), (b, c), (), (a,), ()):
+        for p in (a, b, c):
+            p.grad = None if any(p is s for s in skipped) else torch.ones_like(p)
+        optimizer.step()
+    assert counts_of(calls, a) == [1, 2, 3, 4, 5] and counts_of(calls, b) == [1, 2, 3, 4] and counts_of(calls, c) == [1, 2, 3, 4, 5]
+    assert [optimizer.state[p]["step"] for p in (a, b, c)] == [5, 4, 5]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kwargs", KINDS)
+def test_optimizer_is_torchs(cuda, kwargs):
+    """A group of two types in which parameters skip steps, saved and loaded half way, beside torch's."""
+    import trigrad_amd
+    g = torch.Generator().manual_seed(0)
+    values = [torch.randn(300, generator=g), torch.randn(200, generator=g, dtype=torch.float64), torch.randn(100, generator=g)]
+    mine, theirs = ([t.to(cuda).requires_grad_() for t in values] for _ in range(2))
+    a, b = trigrad_amd.AdamW(mine, lr=1e-2, **kwargs), torch.optim.AdamW(theirs, lr=1e-2, foreach=False)
+    for turn in range(10):
+        for i, (p, q) in enumerate(zip(mine, theirs)):
+            there = (turn + i) % 3 > 0 or turn < 2
+            p.grad = torch.randn(p.shape, generator=g, dtype=p.dtype).to(cuda) if there else None
+            q.grad = None if p.grad is None else p.grad.clone()
+        a.step()
+        b.step()
+        if turn == 5:
+            state = copy.deepcopy(a.state_dict())
+            a = trigrad_amd.AdamW(mine, lr=5.0, **kwargs)
+            a.load_state_dict(state)
+    for p, q in zip(mine, theirs):  # a change is at most ten rates, rounded like the param in each of ten steps, on either side
+        half = U if p.dtype == torch.float32 else 2.0 ** -53
+        assert ((p - q).abs() <= 2 * 10 * half * (4 * q.abs() + 16 * 0.1)).all()

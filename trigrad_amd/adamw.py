@@ -145,8 +145,8 @@ class AdamW(torch.optim.Optimizer):
     AdamW over groups of parameters, each group a few launches.
         params, lr, betas, eps, weight_decay, maximize : as torch.optim.AdamW takes them; lr may be a tensor of one float32
         state_bits : 32, or 8: averages in 8 bits with two float32 for every 256 elements, 2.03 bytes a parameter instead of 8
-        capturable : steps are counted on the device, so that a step can be captured into a graph (with lr as a tensor where it is to change);
-            tensors that had their first gradient in the same step are counted as one
+        capturable : steps are counted on the device, so that a step can be captured into a graph (with lr as a tensor where it is to change).
+            Tensors that have had gradients in the same steps share a count, and a graph counts for those together that did when it was captured
         seed : of the random numbers that averages in 8 bits are rounded with, together with a step's number
 
     Parameters in float16 or bfloat16 are rounded copies of ones in float32 that the state keeps ("master").
@@ -193,20 +193,37 @@ class AdamW(torch.optim.Optimizer):
                         firsts[p.device] = torch.zeros(1, dtype=torch.float32, device=p.device) if group["capturable"] else 0
                     self.state[p].update(self._new_state(p, group, firsts[p.device]))
             calls = {}  # parameters of the same device, type and count together
-            counts = {}  # those on the device, each of which counts once whatever calls read it
+            counts = self._counts_of(group, params)
             for p in params:
                 state = self.state[p]
                 if isinstance(state["step"], torch.Tensor):
                     same = id(state["step"])
-                    counts[same] = state["step"]
                 else:
                     same = state["step"] = state["step"] + 1
                 calls.setdefault((p.device, state.get("master", p).dtype, same), []).append(p)
-            for count in counts.values():
+            for count in counts:
                 count.add_(1.0)
             for together in calls.values():
                 self._step_together(group, together, grad_scale)
         return loss
+
+    def _counts_of(self, group, params):
+        """The counts on the device of `params`, each of which counts once whatever calls read it; one that others of the group share, who do not step now, stays
+        theirs, and those who do go on with a copy."""
+        stepping = {}
+        for p in params:
+            state = self.state[p]
+            if isinstance(state["step"], torch.Tensor):
+                stepping.setdefault(id(state["step"]), []).append(state)
+        if not stepping:
+            return []
+        if len(params) < len(group["params"]):
+            waiting = {id(self.state[p]["step"]) for p in group["params"] if p.grad is None and self.state.get(p)}
+            for same in waiting & stepping.keys():
+                count = stepping[same][0]["step"].clone()
+                for state in stepping[same]:
+                    state["step"] = count
+        return [states[0]["step"] for states in stepping.values()]
 
     def _step_together(self, group, params: List[torch.Tensor], grad_scale):
         states = [self.state[p] for p in params]
