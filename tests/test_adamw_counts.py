@@ -95,3 +95,26 @@ def test_optimizer_is_torchs(cuda, kwargs):
     for p, q in zip(mine, theirs):  # a change is at most ten rates, rounded like the param in each of ten steps, on either side
         half = U if p.dtype == torch.float32 else 2.0 ** -53
         assert ((p - q).abs() <= 2 * 10 * half * (4 * q.abs() + 16 * 0.1)).all()
+
+
+@pytest.mark.gpu
+def test_captures_that_would_not_count_are_refused(cuda):
+    """A count that the host has is the same in every replay, and a state that a graph makes is made anew."""
+    import trigrad_amd
+    for kwargs, warm, match in (({}, True, "capturable"), ({"capturable": True}, False, "first step"), ({"capturable": True}, True, "others")):
+        params = [torch.ones(50, device=cuda, requires_grad=True) for _ in range(2)]
+        for p in params:
+            p.grad = torch.ones_like(p)
+        optimizer = trigrad_amd.AdamW(params, **kwargs)
+        if warm:
+            optimizer.step()
+        if match == "others":
+            params[1].grad = None
+        before = [p.detach().clone() for p in params]
+        graph = torch.cuda.CUDAGraph()
+        with pytest.raises(RuntimeError, match=match):
+            with torch.cuda.graph(graph):
+                optimizer.step()
+        assert all(torch.equal(p, q) for p, q in zip(params, before))
+        optimizer.step()  # and nothing is left of it
+        assert [int(optimizer.state[p].get("step", 0)) for p in params] == [2 if warm else 1, 1 if match == "others" else 2 if warm else 1]

@@ -146,7 +146,8 @@ class AdamW(torch.optim.Optimizer):
         params, lr, betas, eps, weight_decay, maximize : as torch.optim.AdamW takes them; lr may be a tensor of one float32
         state_bits : 32, or 8: averages in 8 bits with two float32 for every 256 elements, 2.03 bytes a parameter instead of 8
         capturable : steps are counted on the device, so that a step can be captured into a graph (with lr as a tensor where it is to change).
-            Tensors that have had gradients in the same steps share a count, and a graph counts for those together that did when it was captured
+            Tensors that have had gradients in the same steps share a count, and a graph counts for those together that did when it was captured.
+            A first step is not captured, nor any without capturable
         seed : of the random numbers that averages in 8 bits are rounded with, together with a step's number
 
     Parameters in float16 or bfloat16 are rounded copies of ones in float32 that the state keeps ("master").
@@ -184,6 +185,9 @@ class AdamW(torch.optim.Optimizer):
                 loss = closure()
         for group in self.param_groups:
             params = [p for p in group["params"] if p.grad is not None]
+            capturing = any(p.is_cuda for p in params[:1]) and torch.cuda.is_current_stream_capturing()
+            if capturing:
+                self._refuse_what_no_replay_counts(params)
             firsts = {}  # by device
             for p in params:
                 if not self.state[p]:
@@ -193,7 +197,7 @@ class AdamW(torch.optim.Optimizer):
                         firsts[p.device] = torch.zeros(1, dtype=torch.float32, device=p.device) if group["capturable"] else 0
                     self.state[p].update(self._new_state(p, group, firsts[p.device]))
             calls = {}  # parameters of the same device, type and count together
-            counts = self._counts_of(group, params)
+            counts = self._counts_of(group, params, capturing)
             for p in params:
                 state = self.state[p]
                 if isinstance(state["step"], torch.Tensor):
@@ -207,7 +211,15 @@ class AdamW(torch.optim.Optimizer):
                 self._step_together(group, together, grad_scale)
         return loss
 
-    def _counts_of(self, group, params):
+    def _refuse_what_no_replay_counts(self, params):
+        for p in params:
+            state = self.state.get(p)
+            if not state:
+                raise RuntimeError("a parameter's first step cannot be captured: its averages would begin anew in every replay")
+            if not isinstance(state["step"], torch.Tensor):
+                raise RuntimeError("a step that is captured has to be counted on the device: the optimizer must be capturable")
+
+    def _counts_of(self, group, params, capturing):
         """The counts on the device of `params`, each of which counts once whatever calls read it; one that others of the group share, who do not step now, stays
         theirs, and those who do go on with a copy."""
         stepping = {}
@@ -220,6 +232,8 @@ class AdamW(torch.optim.Optimizer):
         if len(params) < len(group["params"]):
             waiting = {id(self.state[p]["step"]) for p in group["params"] if p.grad is None and self.state.get(p)}
             for same in waiting & stepping.keys():
+                if capturing:
+                    raise RuntimeError("a parameter that has no gradient now is counted with others that have one: make a step without capture first")
                 count = stepping[same][0]["step"].clone()
                 for state in stepping[same]:
                     state["step"] = count
