@@ -118,3 +118,16 @@ def test_captures_that_would_not_count_are_refused(cuda):
         assert all(torch.equal(p, q) for p, q in zip(params, before))
         optimizer.step()  # and nothing is left of it
         assert [int(optimizer.state[p].get("step", 0)) for p in params] == [2 if warm else 1, 1 if match == "others" else 2 if warm else 1]
+
+
+@pytest.mark.parametrize("kwargs", KINDS)
+def test_calls_of_a_step_have_seeds_of_their_own(calls, kwargs):
+    """Equal places of two groups are not rounded with the same random numbers; one group's are those of its seed and count."""
+    import trigrad_amd
+    groups = [{"params": [leaf(), leaf()]}, {"params": [leaf()]}, {"params": [leaf()], "seed": 7}]
+    optimizer = trigrad_amd.AdamW(groups, state_bits=8, seed=5, **kwargs)
+    for _ in range(3):
+        optimizer.step()
+    seeds = [c["seed"] & 0xFFFFFFFF for c in calls]
+    assert len(set(seeds)) == (3 if kwargs else 9) and len(set(seeds[:3])) == 3
+    assert seeds[::3] == ([5, 5, 5] if kwargs else [6, 7, 8])

@@ -148,7 +148,8 @@ class AdamW(torch.optim.Optimizer):
         capturable : steps are counted on the device, so that a step can be captured into a graph (with lr as a tensor where it is to change).
             Tensors that have had gradients in the same steps share a count, and a graph counts for those together that did when it was captured.
             A first step is not captured, nor any without capturable
-        seed : of the random numbers that averages in 8 bits are rounded with, together with a step's number
+        seed : of the random numbers that averages in 8 bits are rounded with, together with a step's number and the number of the call in it (one for
+            each group, device, type and count)
 
     Parameters in float16 or bfloat16 are rounded copies of ones in float32 that the state keeps ("master").
     """
@@ -183,6 +184,7 @@ class AdamW(torch.optim.Optimizer):
         if closure is not None:
             with torch.enable_grad():
                 loss = closure()
+        number = 0  # of the step's calls
         for group in self.param_groups:
             params = [p for p in group["params"] if p.grad is not None]
             capturing = any(p.is_cuda for p in params[:1]) and torch.cuda.is_current_stream_capturing()
@@ -208,7 +210,8 @@ class AdamW(torch.optim.Optimizer):
             for count in counts:
                 count.add_(1.0)
             for together in calls.values():
-                self._step_together(group, together, grad_scale)
+                self._step_together(group, together, grad_scale, number)
+                number += 1
         return loss
 
     def _refuse_what_no_replay_counts(self, params):
@@ -239,7 +242,7 @@ class AdamW(torch.optim.Optimizer):
                     state["step"] = count
         return [states[0]["step"] for states in stepping.values()]
 
-    def _step_together(self, group, params: List[torch.Tensor], grad_scale):
+    def _step_together(self, group, params: List[torch.Tensor], grad_scale, number):
         states = [self.state[p] for p in params]
         count = states[0]["step"]
         eight = group["state_bits"] == 8
@@ -248,7 +251,7 @@ class AdamW(torch.optim.Optimizer):
                    [s["exp_avg_sq"] for s in states], count, lr=group["lr"], betas=group["betas"], eps=group["eps"], weight_decay=group["weight_decay"],
                    copies=[p if "master" in s else None for s, p in zip(states, params)] if low else None,
                    scales=[s["scales"] for s in states] if eight else None, grad_scale=grad_scale, maximize=group["maximize"],
-                   seed=group["seed"] + (count if isinstance(count, int) else 0))
+                   seed=group["seed"] + (count if isinstance(count, int) else 0) + (number << 24))
 
     def load_state_dict(self, state_dict):
         """As torch's, with every tensor of the state in the type that it was saved in."""
