@@ -131,3 +131,30 @@ def test_calls_of_a_step_have_seeds_of_their_own(calls, kwargs):
     seeds = [c["seed"] & 0xFFFFFFFF for c in calls]
     assert len(set(seeds)) == (3 if kwargs else 9) and len(set(seeds[:3])) == 3
     assert seeds[::3] == ([5, 5, 5] if kwargs else [6, 7, 8])
+
+
+def test_grad_scale_of_two_types(calls):
+    """One in float32, as clipping leaves it, is for the float64 parameters too."""
+    import trigrad_amd
+    optimizer = trigrad_amd.AdamW([leaf(), leaf(torch.float64)])
+    scale = torch.tensor([0.3])
+    optimizer.step(grad_scale=scale)
+    assert [c["grad_scale"].dtype for c in calls] == [torch.float32, torch.float64]
+    assert calls[0]["grad_scale"] is scale and calls[1]["grad_scale"].item() == scale.item()
+
+
+@pytest.mark.gpu
+def test_steps_of_two_types_with_a_grad_scale(cuda):
+    import trigrad_amd
+    mine, theirs = ([torch.ones(100, dtype=t, device=cuda, requires_grad=True) for t in (torch.float32, torch.float64)] for _ in range(2))
+    a, b = trigrad_amd.AdamW(mine, lr=1e-2), torch.optim.AdamW(theirs, lr=1e-2, foreach=False)
+    scale = torch.tensor([0.25], device=cuda)
+    for turn in range(3):
+        for p, q in zip(mine, theirs):
+            p.grad = torch.full_like(p, turn + 1.0)
+            q.grad = p.grad * 0.25
+        a.step(grad_scale=scale)
+        b.step()
+    for p, q in zip(mine, theirs):  # as in the test beside torch's
+        half = U if p.dtype == torch.float32 else 2.0 ** -53
+        assert ((p - q).abs() <= 2 * 3 * half * (4 * q.abs() + 16 * 0.03)).all()

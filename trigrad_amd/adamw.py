@@ -179,7 +179,7 @@ class AdamW(torch.optim.Optimizer):
 
     @torch.no_grad()
     def step(self, closure=None, grad_scale: Optional[torch.Tensor] = None):
-        """One step of every parameter that has a gradient.  grad_scale: as `adamw_step` takes it."""
+        """One step of every parameter that has a gradient.  grad_scale: as `adamw_step` takes it, for parameters of all types."""
         loss = None
         if closure is not None:
             with torch.enable_grad():
@@ -246,6 +246,8 @@ class AdamW(torch.optim.Optimizer):
         states = [self.state[p] for p in params]
         count = states[0]["step"]
         eight = group["state_bits"] == 8
+        if params[0].dtype == torch.float64 and grad_scale is not None and grad_scale.dtype == torch.float32:
+            grad_scale = grad_scale.double()
         low = any("master" in s for s in states)
         adamw_step([s.get("master", p) for s, p in zip(states, params)], [p.grad for p in params], [s["exp_avg"] for s in states],
                    [s["exp_avg_sq"] for s in states], count, lr=group["lr"], betas=group["betas"], eps=group["eps"], weight_decay=group["weight_decay"],
