@@ -191,26 +191,30 @@ class AdamW(torch.optim.Optimizer):
             if capturing:
                 self._refuse_what_no_replay_counts(params)
             firsts = {}  # by device
-            for p in params:
-                if not self.state[p]:
+            states = [self.state[p] for p in params]
+            for p, state in zip(params, states):
+                if not state:
                     if p.grad.is_sparse:
                         raise RuntimeError("gradients must be dense")
                     if p.device not in firsts:
                         firsts[p.device] = torch.zeros(1, dtype=torch.float32, device=p.device) if group["capturable"] else 0
-                    self.state[p].update(self._new_state(p, group, firsts[p.device]))
+                    state.update(self._new_state(p, group, firsts[p.device]))
             calls = {}  # parameters of the same device, type and count together
-            counts = self._counts_of(group, params, capturing)
-            for p in params:
-                state = self.state[p]
-                if isinstance(state["step"], torch.Tensor):
-                    same = id(state["step"])
+            counted = {}  # states by their count on the device
+            for p, state in zip(params, states):
+                count = state["step"]
+                if isinstance(count, torch.Tensor):
+                    same = id(count)
+                    counted.setdefault(same, []).append(state)
                 else:
-                    same = state["step"] = state["step"] + 1
-                calls.setdefault((p.device, state.get("master", p).dtype, same), []).append(p)
-            for count in counts:
-                count.add_(1.0)
+                    same = state["step"] = count + 1
+                together = calls.setdefault((p.device, state.get("master", p).dtype, same), ([], []))
+                together[0].append(p)
+                together[1].append(state)
+            if counted:
+                self._count(group, counted, capturing)
             for together in calls.values():
-                self._step_together(group, together, grad_scale, number)
+                self._step_together(group, *together, grad_scale, number)
                 number += 1
         return loss
 
@@ -222,28 +226,21 @@ class AdamW(torch.optim.Optimizer):
             if not isinstance(state["step"], torch.Tensor):
                 raise RuntimeError("a step that is captured has to be counted on the device: the optimizer must be capturable")
 
-    def _counts_of(self, group, params, capturing):
-        """The counts on the device of `params`, each of which counts once whatever calls read it; one that others of the group share, who do not step now, stays
-        theirs, and those who do go on with a copy."""
-        stepping = {}
-        for p in params:
-            state = self.state[p]
-            if isinstance(state["step"], torch.Tensor):
-                stepping.setdefault(id(state["step"]), []).append(state)
-        if not stepping:
-            return []
-        if len(params) < len(group["params"]):
-            waiting = {id(self.state[p]["step"]) for p in group["params"] if p.grad is None and self.state.get(p)}
-            for same in waiting & stepping.keys():
+    def _count(self, group, counted, capturing):
+        """Counts a step on the device, once whatever calls read the count.  One that others of the group share, who do not step now, stays theirs, and those who
+        do go on with a copy."""
+        waiting = {id(self.state[p]["step"]) for p in group["params"] if p.grad is None and self.state.get(p)}
+        for same, states in counted.items():
+            count = states[0]["step"]
+            if same in waiting:
                 if capturing:
                     raise RuntimeError("a parameter that has no gradient now is counted with others that have one: make a step without capture first")
-                count = stepping[same][0]["step"].clone()
-                for state in stepping[same]:
+                count = count.clone()
+                for state in states:
                     state["step"] = count
-        return [states[0]["step"] for states in stepping.values()]
+            count.add_(1.0)
 
-    def _step_together(self, group, params: List[torch.Tensor], grad_scale, number):
-        states = [self.state[p] for p in params]
+    def _step_together(self, group, params: List[torch.Tensor], states, grad_scale, number):
         count = states[0]["step"]
         eight = group["state_bits"] == 8
         if params[0].dtype == torch.float64 and grad_scale is not None and grad_scale.dtype == torch.float32:
