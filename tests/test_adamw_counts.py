@@ -158,3 +158,34 @@ def test_steps_of_two_types_with_a_grad_scale(cuda):
     for p, q in zip(mine, theirs):  # as in the test beside torch's
         half = U if p.dtype == torch.float32 else 2.0 ** -53
         assert ((p - q).abs() <= 2 * 3 * half * (4 * q.abs() + 16 * 0.03)).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_parameters_that_lie_otherwise(cuda, dtype, bits):
+    """Channels last, or turned, as torch's takes them: the steps of a contiguous parameter with the same values in the same places in memory."""
+    import trigrad_amd
+    g = torch.Generator().manual_seed(3)
+    x = torch.randn((6, 5, 4, 3), generator=g).to(cuda, dtype)
+    for turn in (lambda t: t.contiguous(memory_format=torch.channels_last), lambda t: t.permute(3, 0, 2, 1).contiguous().permute(1, 3, 2, 0)):
+        p = turn(x).requires_grad_()
+        order = sorted(range(4), key=lambda d: -p.stride(d))
+        q = p.detach().permute(order).clone(memory_format=torch.contiguous_format).requires_grad_()
+        assert not p.is_contiguous()
+        a, b = (trigrad_amd.AdamW([t], lr=1e-2, state_bits=bits) for t in (p, q))
+        for n in range(3):
+            grad = torch.randn(x.shape, generator=g).to(cuda, dtype)
+            p.grad = turn(grad) if n else grad  # a gradient may lie otherwise than its parameter
+            q.grad = grad.permute(order).contiguous()
+            a.step()
+            b.step()
+            if n == 1:
+                state = copy.deepcopy(a.state_dict())
+                a = trigrad_amd.AdamW([p], lr=1e-2, state_bits=bits)
+                a.load_state_dict(state)
+        assert torch.equal(p.permute(order), q) and p.stride() == turn(x).stride()
+    hole = torch.zeros((8, 8), device=cuda)[:, :4].requires_grad_()
+    hole.grad = torch.ones_like(hole)
+    with pytest.raises(ValueError, match="contiguous"):
+        trigrad_amd.AdamW([hole]).step()

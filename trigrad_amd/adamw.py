@@ -151,7 +151,8 @@ class AdamW(torch.optim.Optimizer):
         seed : of the random numbers that averages in 8 bits are rounded with, together with a step's number and the number of the call in it (one for
             each group, device, type and count)
 
-    Parameters in float16 or bfloat16 are rounded copies of ones in float32 that the state keeps ("master").
+    Parameters are dense in memory, in whatever order of their dimensions.  Those in float16 or bfloat16 are rounded copies of ones in float32 that the state
+    keeps ("master").
     """
 
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, *, maximize=False, state_bits=32, capturable=False, seed=0):
@@ -168,13 +169,13 @@ class AdamW(torch.optim.Optimizer):
         """The state of a parameter before its first step; `first`: the count of those on its device that begin with it."""
         state = {"step": first}
         if p.dtype in COPY_TYPES:
-            state["master"] = p.detach().to(torch.float32, copy=True, memory_format=torch.contiguous_format)
+            state["master"] = p.detach().to(torch.float32, copy=True)
         if group["state_bits"] == 8:
-            state["exp_avg"], state["exp_avg_sq"] = (torch.zeros(p.shape, dtype=torch.uint8, device=p.device).view(STATE_TYPE) for _ in range(2))
+            state["exp_avg"], state["exp_avg_sq"] = (torch.zeros_like(p, dtype=torch.uint8, requires_grad=False).view(STATE_TYPE) for _ in range(2))
             state["scales"] = scales_of(p)
         else:
             real = state.get("master", p).dtype
-            state["exp_avg"], state["exp_avg_sq"] = (torch.zeros(p.shape, dtype=real, device=p.device) for _ in range(2))
+            state["exp_avg"], state["exp_avg_sq"] = (torch.zeros_like(p, dtype=real, requires_grad=False) for _ in range(2))
         return state
 
     @torch.no_grad()
@@ -246,10 +247,13 @@ class AdamW(torch.optim.Optimizer):
         if params[0].dtype == torch.float64 and grad_scale is not None and grad_scale.dtype == torch.float32:
             grad_scale = grad_scale.double()
         low = any("master" in s for s in states)
-        adamw_step([s.get("master", p) for s, p in zip(states, params)], [p.grad for p in params], [s["exp_avg"] for s in states],
-                   [s["exp_avg_sq"] for s in states], count, lr=group["lr"], betas=group["betas"], eps=group["eps"], weight_decay=group["weight_decay"],
-                   copies=[p if "master" in s else None for s, p in zip(states, params)] if low else None,
-                   scales=[s["scales"] for s in states] if eight else None, grad_scale=grad_scale, maximize=group["maximize"],
+        lists = [[s.get("master", p) for s, p in zip(states, params)], [p.grad for p in params], [s["exp_avg"] for s in states],
+                 [s["exp_avg_sq"] for s in states], [p if "master" in s else None for s, p in zip(states, params)] if low else None]
+        if not all(map(torch.Tensor.is_contiguous, params)):  # in memory all of a parameter's tensors lie as it does
+            orders = [sorted(range(p.dim()), key=lambda d: -p.stride(d)) for p in params]
+            lists = [None if ts is None else [None if t is None else t.permute(o) for t, o in zip(ts, orders)] for ts in lists]
+        adamw_step(*lists[:4], count, lr=group["lr"], betas=group["betas"], eps=group["eps"], weight_decay=group["weight_decay"],
+                   copies=lists[4], scales=[s["scales"] for s in states] if eight else None, grad_scale=grad_scale, maximize=group["maximize"],
                    seed=group["seed"] + (count if isinstance(count, int) else 0) + (number << 24))
 
     def load_state_dict(self, state_dict):
