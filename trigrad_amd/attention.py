@@ -117,7 +117,9 @@ def linear_attention(
         scale : default 1 / sqrt(K)
 
     Gates are decays, a <= 1; minus infinity is a = 0, where the sequence begins anew.  A value that is not finite makes outputs of its
-    sequence and head that are not, those of up to 63 rows in front of it too.  States are summed in float32 whatever the types.  The call can be
+    sequence and head that are not, those of up to 63 rows in front of it too; what is finite beside it has all its terms.  States are float32 and all sums
+    are, whatever the types; outputs and gradients are rounded to theirs once.  Beside that a term of an output in bfloat16 is off by up to 2^-16 of itself, one of
+    anything in float16 by 2^-22, or by 2^-39 of the largest in its row or column.  The call can be
     captured into a graph, with its backward pass; under capture a leaf of a graph that was made on another stream and still lives is refused.
 
     Returns:

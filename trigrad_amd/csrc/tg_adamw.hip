@@ -73,7 +73,10 @@ template <class L> __device__ __forceinline__ AdamwFactors factors_of(const L &a
 #ifndef TG_DOUBLE_PRECISION
 constexpr float kLargest8 = 448.0f, kLeastLargest = 0x1p-110f;  // a block whose largest is below becomes zeros
 
-__device__ __forceinline__ uint32_t mixed(uint32_t x) {  // products by odd constants and shifts
+// Products by odd constants and shifts: those of C. Wellons' published search for 32-bit mixers of little bias (2018).  The seed's factor and summand are the
+// odd constants of A. Appleby's published finalizer (2011), a place's is the prime next to 2^32 over the golden ratio
+// of D. Knuth's multiplicative hashing.
+__device__ __forceinline__ uint32_t mixed(uint32_t x) {
     x = (x ^ x >> 16) * 0x7FEB352Du;
     x = (x ^ x >> 15) * 0x846CA68Bu;
     return x ^ x >> 16;

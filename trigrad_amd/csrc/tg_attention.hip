@@ -183,8 +183,7 @@ __global__ __launch_bounds__(kPlanThreads) void attention_plan_kernel(Attention 
 }
 
 // From what units add to a state, the states in front of them (or behind them, from the last to the first): x' = decay x + added.  A thread has V
-// neighbours of the state and reads eight units ahead.  95 units of 16 states of 64 x 128: 34 us, 2.9 TB/s (52 with V = 1); sequences of two or three units
-// have few reads on their way.
+// neighbours of the state and reads eight units ahead.  136 units, of 37 sequences, of 16 states of 64 x 128: 34 us, 4.2 TB/s (52 with V = 1).
 template <int V>
 __global__ __launch_bounds__(kScanThreads) void attention_scan_kernel(AttentionCall c, float *__restrict__ states, const float *__restrict__ from, float *__restrict__ to,
                                                                       float *__restrict__ kept, int64_t unit_rows, bool back) {
@@ -523,8 +522,9 @@ static int split_of(const char *fn, const tg_attention &a, const Attention &m, S
     s.size = std::max(m.key_size, m.value_size) <= 32 ? 32 : std::max(m.key_size, m.value_size) <= 64 ? 64 : 128;
     const int64_t of_one = ceil_div64(m.length, s.rows_of_chunk);
     s.chunks = 0;
-    // Chunks of a unit: a compute unit takes its units one after another, and a unit, whose state is written and read, as long as its chunks and two
-    // more (four of half the rows).  2 x 3000 rows of 8 heads in float32: six chunks, 256 units, 290 us forward and backward; five, 304 units, 404.
+    // Chunks of a unit, as if a compute unit took its units one after another, and a unit, whose state is written and read, as long as its chunks and two
+    // more (four of half the rows).  2 x 3000 rows of 8 heads in float32: six chunks, 256 units, 184 us forward and backward; five, 304 units, 282.  Of
+    // heads of at most 64 a compute unit has two or three at once, and packed sequences' last units are half empty: neither is in the model.
     int64_t least = 0;
     for (int64_t n = std::max<int64_t>(1, ceil_div64(of_one, kMostUnits)), most = std::max(n, kMostChunks); n <= most; n++) {
         const int64_t units = (m.packed ? of_one / n + m.sequences : ceil_div64(of_one, n) * m.sequences) * m.heads;

@@ -18,11 +18,11 @@ __device__ __forceinline__ float sum_groups(float v) {
 // The two kernels have twice the waves of a state: the first half (`role` 0) has one state, the second half the other.  LDS, and waves of a SIMD that
 // they are compiled for: two, with 256 registers, where LDS has room for one workgroup.
 //
-// W of State, 4 x 4096 rows of 16 heads of 128 in bfloat16, and 2 x 3000 of 8 in float32: the queries' kernel 180 and 81 us with one, 192 and 63 with
-// two; the keys' 335 and 93 with one, 189 and 65 with two.  8 x 2048 rows of 32 heads of 64: 129 and 127 with one, 161 and 141 with two.  In float16,
+// W of State, 4 x 4096 rows of 16 heads of 128 in bfloat16, and 2 x 3000 of 8 in float32: the queries' kernel 183 and 82 us with one, 197 and 60 with
+// two; the keys' 300 and 87 with one, 198 and 64 with two.  8 x 2048 rows of 32 heads of 64: 136 and 137 with one, 170 and 156 with two.  In float16,
 // whose scalings take registers, the first of these forward and backward: 539 with one in the queries' kernel, 512 with two.
 // Instructions bound both: making parts, matrix instructions and readings of LDS take a third to a half of the time each and hardly overlap, as all
-// waves of a workgroup are in the same phase (1.9 TB/s of memory for heads of 128, 2.6 for those of 64).
+// waves of a workgroup are in the same phase (1.8 TB/s of memory for heads of 128, 2.5 for those of 64).
 template <class T, int D> constexpr int kQueriesColumns = D > 64 && (sizeof(T) == 4 || Parts<T>::kScaled) ? 2 : 1;
 template <int D> constexpr int kKeysColumns = D > 64 ? 2 : 1;
 template <class T, int D> constexpr int kQueriesThreads = 2 * State<D, kQueriesColumns<T, D>>::kWaves * kWave;

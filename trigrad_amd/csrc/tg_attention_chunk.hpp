@@ -323,7 +323,6 @@ struct AttentionCall {
     bool grad_outputs_there;  // false: zeros, and the pointer is to something else of the values' shape
     const float *grad_final;
     void *grad_queries, *grad_keys, *grad_values, *grad_gates;
-    float *grad_initial;
     float *grad_states;     // of each unit and head: what the unit adds to the gradient in front of it, then the gradient behind it
     double *changes[2];     // of each head and row: what dlog a changes by
     double *sums;           // of each unit and head: dlog a of all rows
@@ -396,7 +395,7 @@ template <class T, int Rows> __device__ __forceinline__ float gate_of_lane(const
     return lane < count && lane < Rows ? gate_at<T>(c, first + lane, head) : 0.0f;
 }
 
-// scale 2^(L_s - L_r) of an accumulator whose columns are rows s (or r) of the chunk, zero where s < r, or, Strict, s <= r.
+// scale 2^(L_s - L_r) of an accumulator whose columns are rows s (or r) of the chunk, zero where s < r.
 template <bool ColumnsAreLater, int Rows> __device__ __forceinline__ floatx4 decays_of(const Reach<Rows> &reach, int row, int column, float scale, int lane) {
     const int x = column + lane % 16, y = row + 4 * (lane / 16);
     const double here = reach.reach[x];
@@ -435,8 +434,8 @@ __device__ __forceinline__ int lane_of_turn() {
 }
 
 // Whether State::fold adds up apart, where the registers are enough: 8 x 2048 rows of 32 heads of 64 with fixed decays near 1, states off by 1.1e-7 in
-// place of 2.7e-7 and the decays' gradients by 5e-7 in place of 9e-7, in the same time; but 4 x 4096 rows of 16 heads of 128 the outputs' kernel 160 us
-// in place of 101, and, with two times sixteen columns a wave, the keys' 252 in place of 184.
+// place of 2.7e-7 and the decays' gradients by 5e-7 in place of 9e-7, in the same time; but 4 x 4096 rows of 16 heads of 128 the outputs' kernel 168 us
+// in place of 115, and, with two times sixteen columns a wave, the keys' 261 in place of 198.
 template <class T, int D, int W, bool Forward> constexpr bool kFoldApart = Forward ? D <= 64 || Parts<T>::kRows == 32 : W == 1;
 
 // The state in accumulators: rows of keys and columns of values (Turned: the other way round), of a wave the 16 W columns from `column` on.  With W = 2 an

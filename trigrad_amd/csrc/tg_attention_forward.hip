@@ -11,7 +11,7 @@ constexpr int W = 1;  // see State
 template <int D> constexpr int kThreads = State<D, W>::kWaves * kWave;
 
 // What a unit adds to the state, and its decay.  A chunk is on its way from memory while the one before is computed on.  32768 rows of 16 heads of 128
-// in bfloat16: 72 us, 3.7 TB/s; weighted values in three parts are what it computes.
+// in bfloat16: 73 us, 3.7 TB/s; weighted values in three parts are what it computes.
 template <class T, int D, bool Vector>
 __global__ __launch_bounds__(kThreads<D>, waves_of_simd(kThreads<D>, kStatesLds<T, D>, W * D / 4)) void attention_states_kernel(AttentionCall c) {
     constexpr int R = Parts<T>::kRows, N = Parts<T>::kInput;
@@ -58,7 +58,7 @@ __global__ __launch_bounds__(kThreads<D>, waves_of_simd(kThreads<D>, kStatesLds<
 }
 
 // The outputs, from the states in front of the units, or through whole sequences.  A state is read through its accumulators, the pairs of a chunk
-// through LDS.  32768 rows of 16 heads of 128 in bfloat16: 154 us, 3.5 TB/s; instructions that make a state's parts and the decays of pairs bound it.
+// through LDS.  32768 rows of 16 heads of 128 in bfloat16: 164 us, 3.3 TB/s; instructions that make a state's parts and the decays of pairs bound it.
 template <class T, int D, bool Vector>
 __global__ __launch_bounds__(kThreads<D>, waves_of_simd(kThreads<D>, kOutputsLds<T, D>, W * D / 4)) void attention_outputs_kernel(AttentionCall c) {
     constexpr int R = Parts<T>::kRows, N = Parts<T>::kInput, M = Parts<T>::kState, kTiles = R / 16, kWaves = State<D, W>::kWaves;
